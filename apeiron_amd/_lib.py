@@ -16,7 +16,7 @@ STATUS = {
     5: "UnsupportedQuant", 6: "NonFiniteScale", 7: "FixedOverflow", 8: "AccumulatorOverflow",
     9: "OutputOverflow", 10: "NonFiniteInput", 11: "InputRange", 20: "NoDevice",
     12: "FfnOverflow", 13: "ExpOutOfRange", 14: "ZeroDenominator",
-    21: "InvalidArg", 22: "Hip", 23: "OutOfMemory", 24: "ScratchLimit", 25: "SeqTimeout",
+    21: "InvalidArg", 22: "Hip", 23: "OutOfMemory", 24: "ScratchLimit", 25: "SeqTimeout", 27: "CacheRange",
 }
 
 # Every symbol include/apeiron_hip.h declares.
@@ -32,6 +32,8 @@ EXPORTS = [
     "ah_ffn_prefill_dev", "ah_set_ffn_prefill_form", "ah_swiglu_quant_dev", "ah_ffn_q8_dev",
     "ah_ffn_prefill_q8_dev", "ah_dev_alloc", "ah_dev_free", "ah_copy_to_dev", "ah_copy_to_host", "ah_seq_set_spin_limit", "ah_ctx_scratch_bytes",
     "ah_seq_create", "ah_seq_run", "ah_seq_sync_status", "ah_seq_free", "ah_seq_info",
+    "ah_norm_quant_dev", "ah_rope_create", "ah_rope_free", "ah_rope_info", "ah_rope_dev", "ah_kv4_create",
+    "ah_kv4_free", "ah_kv4_info", "ah_kv4_append_dev", "ah_kv4_read_dev", "ah_kv4_attn_dev", "ah_sample_dev",
 ]
 
 _lib = None
@@ -46,9 +48,37 @@ class SeqStage(ctypes.Structure):
                 ("y", ctypes.c_void_p), ("gate", ctypes.c_void_p), ("up", ctypes.c_void_p),
                 ("n", ctypes.c_size_t), ("h_codes", ctypes.c_void_p), ("h_scales", ctypes.c_void_p)]
 
+
+class RopeSpec(ctypes.Structure):
+    """struct ah_rope_spec of include/apeiron_hip.h."""
+    _fields_ = [("head_dim", ctypes.c_size_t), ("rot_dim", ctypes.c_size_t), ("layout", ctypes.c_uint32),
+                ("scaling", ctypes.c_uint32)] + [(n, ctypes.c_double) for n in
+                                                 ("base", "factor", "low", "high", "original_ctx", "amplitude")]
+
+
+class Kv4Tokens(ctypes.Structure):
+    """struct ah_kv4_tokens of include/apeiron_hip.h."""
+    _fields_ = [("d_seq", ctypes.c_void_p), ("d_pos", ctypes.c_void_p), ("n_tok", ctypes.c_size_t),
+                ("d_table", ctypes.c_void_p), ("n_seq", ctypes.c_size_t), ("table_stride", ctypes.c_size_t)]
+
+
+class Kv4Attn(ctypes.Structure):
+    """struct ah_kv4_attn of include/apeiron_hip.h."""
+    _fields_ = [(n, ctypes.c_size_t) for n in ("n_seq", "n_tok", "n_heads", "max_q", "max_ctx")] + [
+        ("d_q_start", ctypes.c_void_p), ("d_ctx", ctypes.c_void_p), ("d_table", ctypes.c_void_p),
+        ("table_stride", ctypes.c_size_t), ("scale", ctypes.c_float), ("window", ctypes.c_size_t),
+        ("sinks", ctypes.c_size_t)]
+
+
+class SampleParams(ctypes.Structure):
+    """struct ah_sample_params of include/apeiron_hip.h."""
+    _fields_ = [(n, ctypes.c_void_p) for n in ("d_temperature", "d_top_k", "d_top_p", "d_min_p")]
+
+
 S = ctypes.c_size_t
 I32 = ctypes.c_int32
 U32 = ctypes.c_uint32
+F32 = ctypes.c_float
 
 
 def load() -> ctypes.CDLL:
@@ -110,6 +140,18 @@ def load() -> ctypes.CDLL:
         "ah_seq_sync_status": (I32, [P, P, P, ctypes.POINTER(U32)]),
         "ah_seq_free": (I32, [P, P]),
         "ah_seq_info": (I32, [P, ctypes.POINTER(U32), ctypes.POINTER(U32)]),
+        "ah_norm_quant_dev": (I32, [P, P, P, P, F32, S, S, P, P, P, P, P, P]),
+        "ah_rope_create": (I32, [P, ctypes.POINTER(RopeSpec), ctypes.POINTER(P)]),
+        "ah_rope_free": (I32, [P, P]),
+        "ah_rope_info": (I32, [P, P, ctypes.POINTER(ctypes.c_double)]),
+        "ah_rope_dev": (I32, [P, P, P, S, S, P, S, P, S, P]),
+        "ah_kv4_create": (I32, [P, S, S, S, S, ctypes.POINTER(P)]),
+        "ah_kv4_free": (I32, [P, P]),
+        "ah_kv4_info": (I32, [P] + [ctypes.POINTER(S)] * 5),
+        "ah_kv4_append_dev": (I32, [P, P, P, ctypes.POINTER(Kv4Tokens), P, S, S, P, S, P, S, P, S, P]),
+        "ah_kv4_read_dev": (I32, [P, P, ctypes.POINTER(Kv4Tokens), P, P, P]),
+        "ah_kv4_attn_dev": (I32, [P, P, ctypes.POINTER(Kv4Attn), P, S, P, S, P]),
+        "ah_sample_dev": (I32, [P, P, S, S, S, ctypes.POINTER(SampleParams), P, P, P, P]),
     }
     for name, (res, args) in sig.items():
         fn = getattr(L, name)

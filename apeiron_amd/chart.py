@@ -339,6 +339,127 @@ class Seq:
             self.h = None
 
 
+# ---- between the projections: norm, rotary positions, the 4-bit cache, attention, sampling ----------
+
+
+def norm_quant_dev(dev: "Device", x_ptr: int, gain_ptr: int, eps: float, n_tok: int, n: int, *, residual_ptr: int | None = None,
+                   sum_ptr: int | None = None, y_ptr: int | None = None, codes_ptr: int | None = None,
+                   scales_ptr: int | None = None, values_ptr: int | None = None, stream: int | None = None) -> None:
+    """s = x + residual, its RMS norm times gain, and the norm's QuantAct (ah_norm_quant_dev); values: what
+    the codes stand for, as bf16."""
+    _check(dev.lib.ah_norm_quant_dev(dev.h, x_ptr, residual_ptr, gain_ptr, eps, n_tok, n, sum_ptr, y_ptr, codes_ptr, scales_ptr,
+                                     values_ptr, stream), "norm_quant")
+
+
+class Rope:
+    """Rotary positions of a head (ah_rope_*).  ``scaling``: None, ("linear", factor), ("ntk", factor) or
+    ("bands", factor, low, high, original_ctx)."""
+
+    LAYOUTS = {"half": 0, "interleaved": 1}
+    SCALINGS = {"linear": 1, "ntk": 2, "bands": 3}
+
+    def __init__(self, dev: Device, head_dim: int, rot_dim: int | None = None, *, layout: str = "half", base: float = 10000.0,
+                 scaling: tuple | None = None, amplitude: float = 0.0):
+        rot_dim = head_dim if rot_dim is None else rot_dim
+        kind, *rest = scaling or ("none",)
+        rest = [float(v) for v in rest] + [0.0] * (4 - len(rest))
+        spec = _lib.RopeSpec(head_dim, rot_dim, self.LAYOUTS[layout], self.SCALINGS[kind] if scaling else 0, base, *rest, amplitude)
+        h = ctypes.c_void_p()
+        _check(dev.lib.ah_rope_create(dev.h, ctypes.byref(spec), ctypes.byref(h)), "rope_create")
+        self.dev, self.h, self.head_dim, self.rot_dim = dev, h, head_dim, rot_dim
+
+    def info(self) -> tuple[np.ndarray, float]:
+        """(theta f64 [rot_dim / 2], amplitude)."""
+        theta, m = np.zeros(self.rot_dim // 2), ctypes.c_double()
+        _check(self.dev.lib.ah_rope_info(self.h, theta.ctypes.data_as(ctypes.c_void_p), ctypes.byref(m)), "rope_info")
+        return theta, m.value
+
+    def rotate_dev(self, x_ptr: int, y_ptr: int, n_heads: int, pos_ptr: int, n_tok: int, *, x_stride: int | None = None,
+                   y_stride: int | None = None, stream: int | None = None) -> None:
+        row = n_heads * self.head_dim
+        _check(self.dev.lib.ah_rope_dev(self.dev.h, self.h, x_ptr, row if x_stride is None else x_stride, n_heads, pos_ptr, n_tok,
+                                        y_ptr, row if y_stride is None else y_stride, stream), "rope")
+
+    def free(self) -> None:
+        if self.h:
+            self.dev.lib.ah_rope_free(self.dev.h, self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            if self.dev.h:
+                self.free()
+        except Exception:
+            pass
+
+
+class KvCache4:
+    """One layer's paged key/value cache in 4 bits (ah_kv4_*).  Strides are in floats from token to token
+    (None: dense); tokens are named by sequence and position through the caller's page table."""
+
+    def __init__(self, dev: Device, n_pages: int, page_len: int, n_kv_heads: int, head_dim: int):
+        h = ctypes.c_void_p()
+        _check(dev.lib.ah_kv4_create(dev.h, n_pages, page_len, n_kv_heads, head_dim, ctypes.byref(h)), "kv4_create")
+        self.dev, self.h = dev, h
+        self.n_pages, self.page_len, self.n_kv_heads, self.head_dim = n_pages, page_len, n_kv_heads, head_dim
+
+    def info(self) -> tuple[int, int, int, int, int]:
+        """(bytes, n_pages, page_len, n_kv_heads, head_dim)."""
+        v = [ctypes.c_size_t() for _ in range(5)]
+        _check(self.dev.lib.ah_kv4_info(self.h, *map(ctypes.byref, v)), "kv4_info")
+        return tuple(x.value for x in v)
+
+    def append_dev(self, rope: Rope | None, *, k_ptr: int, v_ptr: int, seq_ptr: int, pos_ptr: int, n_tok: int, table_ptr: int,
+                   n_seq: int, table_stride: int, q_ptr: int | None = None, n_heads: int = 0, q_out_ptr: int | None = None,
+                   q_stride: int | None = None, q_out_stride: int | None = None, k_stride: int | None = None,
+                   v_stride: int | None = None, stream: int | None = None) -> None:
+        """Rotates q (into q_out) and k, and puts k and v into the cache, in one launch."""
+        t = _lib.Kv4Tokens(seq_ptr, pos_ptr, n_tok, table_ptr, n_seq, table_stride)
+        row, kv = n_heads * self.head_dim, self.n_kv_heads * self.head_dim
+        _check(self.dev.lib.ah_kv4_append_dev(self.dev.h, self.h, rope.h if rope else None, ctypes.byref(t), q_ptr,
+                                              row if q_stride is None else q_stride, n_heads, q_out_ptr,
+                                              row if q_out_stride is None else q_out_stride, k_ptr,
+                                              kv if k_stride is None else k_stride, v_ptr, kv if v_stride is None else v_stride,
+                                              stream), "kv4_append")
+
+    def read_dev(self, *, seq_ptr: int, pos_ptr: int, n_tok: int, table_ptr: int, n_seq: int, table_stride: int,
+                 k_ptr: int | None = None, v_ptr: int | None = None, stream: int | None = None) -> None:
+        """The values held for tokens, as f16 [n_tok][n_kv_heads][head_dim]."""
+        t = _lib.Kv4Tokens(seq_ptr, pos_ptr, n_tok, table_ptr, n_seq, table_stride)
+        _check(self.dev.lib.ah_kv4_read_dev(self.dev.h, self.h, ctypes.byref(t), k_ptr, v_ptr, stream), "kv4_read")
+
+    def attn_dev(self, q_ptr: int, out_ptr: int, *, n_heads: int, n_tok: int, n_seq: int, q_start_ptr: int, ctx_ptr: int,
+                 table_ptr: int, table_stride: int, max_q: int, max_ctx: int, scale: float, window: int = 0, sinks: int = 0,
+                 q_stride: int | None = None, out_stride: int | None = None, stream: int | None = None) -> None:
+        """Attention of every sequence's last tokens over its positions in the cache."""
+        a = _lib.Kv4Attn(n_seq, n_tok, n_heads, max_q, max_ctx, q_start_ptr, ctx_ptr, table_ptr, table_stride, scale, window, sinks)
+        row = n_heads * self.head_dim
+        _check(self.dev.lib.ah_kv4_attn_dev(self.dev.h, self.h, ctypes.byref(a), q_ptr, row if q_stride is None else q_stride, out_ptr,
+                                            row if out_stride is None else out_stride, stream), "kv4_attn")
+
+    def free(self) -> None:
+        if self.h:
+            self.dev.lib.ah_kv4_free(self.dev.h, self.h)
+            self.h = None
+
+    def __del__(self):
+        try:
+            if self.dev.h:
+                self.free()
+        except Exception:
+            pass
+
+
+def sample_dev(dev: "Device", logits_ptr: int, n_rows: int, n_vocab: int, u_ptr: int, tokens_ptr: int, *, row_stride: int | None = None,
+               probs_ptr: int | None = None, temperature_ptr: int | None = None, top_k_ptr: int | None = None,
+               top_p_ptr: int | None = None, min_p_ptr: int | None = None, stream: int | None = None) -> None:
+    """One token per row of logits by temperature, top-k, top-p and min-p from the rows' random numbers
+    (ah_sample_dev); the parameters are per-row device arrays (None: off)."""
+    p = _lib.SampleParams(temperature_ptr, top_k_ptr, top_p_ptr, min_p_ptr)
+    _check(dev.lib.ah_sample_dev(dev.h, logits_ptr, n_vocab if row_stride is None else row_stride, n_rows, n_vocab, ctypes.byref(p),
+                                 u_ptr, tokens_ptr, probs_ptr, stream), "sample")
+
+
 _default: Device | None = None
 
 

@@ -5,6 +5,7 @@
 // NonFiniteScale refusal (num/dequant.rs:25-41), and plans the kernel launches.
 #include "apeiron_hip.h"
 #include "ah_few.h"
+#include "ah_host.h"
 #include "ah_internal.h"
 
 #include <hip/hip_runtime.h>
@@ -61,6 +62,7 @@ uint32_t ah_few_splits(uint32_t type, uint32_t n_in);
 double ah_few_cost(uint32_t type, uint32_t n_in, uint32_t kpad, uint32_t tok, uint32_t splits, uint32_t waves, size_t wgs,
                    uint32_t cus);
 hipError_t ah_few_init_attrs();
+hipError_t ah_attn_init_attrs();
 hipError_t ah_launch_few(uint32_t type, FewArgs &a, bool ffn, hipStream_t stream);
 hipError_t ah_probe_mfma(uint32_t kind, uint32_t cus, const uint32_t *d_seed, uint32_t *d_sink,
                          hipStream_t stream, double *tops);
@@ -71,32 +73,6 @@ hipError_t ah_probe_mfma(uint32_t kind, uint32_t cus, const uint32_t *d_seed, ui
 // (hipGetSymbolAddress with the context's device current) and kept in ah_ctx::noalloc.
 constexpr size_t kNoAllocScratchBytes = 64ull << 20;
 static __device__ __align__(256) uint8_t scratch[kNoAllocScratchBytes];
-
-struct ah_ctx {
-    int device = -1;
-    uint8_t *noalloc = nullptr;  // this device's copy of `scratch`
-    hipStream_t stream = nullptr;
-    // Two status words: [0] every call's refusals; [1] the refusals of a fused FFN's down
-    // projection, reported only when [0] holds none (the reference refuses the FFN at its first
-    // failing step, so a refused hidden activation is never projected).
-    unsigned long long *d_status = nullptr;
-    int last_hip = 0;
-    uint32_t last_bad_bits = 0;  // f16 bits behind the last AH_ERR_NONFINITE_SCALE
-    int cu_count = 256;
-    uint32_t design[32] = {};  // GEMM design per GGUF type (ah_set_gemm_design; 0 = AUTO)
-    void *scratch = nullptr;  // device scratch for GEMM operands / host-form staging
-    // the unfused prefill FFN's gate / up outputs when the caller keeps none (grown on demand)
-    void *ffn_buf = nullptr;
-    size_t ffn_buf_bytes = 0;
-    uint32_t ffn_form = AH_FFN_PREFILL_AUTO;  // ah_set_ffn_prefill_form
-    size_t scratch_bytes = 0;
-    // streaming-GEMV occupancy by (type, LDS bytes): a runtime query per launch costs more host
-    // time than a small GEMV takes on the device
-    static constexpr int kOccSlots = 16;
-    uint32_t occ_key[kOccSlots] = {};
-    int occ_val[kOccSlots] = {};
-    int occ_n = 0;
-};
 
 struct ah_tensor {
     uint32_t type = 0;
@@ -127,15 +103,6 @@ struct ah_seq {
     unsigned long long *d_status = nullptr;
     uint32_t spin_limit = kSeqSpinLimit;  // polls before a grid-barrier wait gives up
 };
-
-#define AH_HIP(ctx, call)                                                                       \
-    do {                                                                                        \
-        hipError_t e_ = (call);                                                                 \
-        if (e_ != hipSuccess) {                                                                 \
-            if (ctx) (ctx)->last_hip = (int)e_;                                                 \
-            return AH_ERR_HIP;                                                                  \
-        }                                                                                       \
-    } while (0)
 
 namespace {
 
@@ -175,30 +142,6 @@ void scale_offsets(uint32_t t, uint32_t &o0, uint32_t &o1, uint32_t &bb) {
 }
 
 bool f16_nonfinite(uint16_t h) { return ((h >> 10) & 0x1f) == 0x1f; }
-
-hipStream_t pick(ah_ctx *ctx, void *stream) {
-    return stream ? static_cast<hipStream_t>(stream) : ctx->stream;
-}
-
-int32_t ensure_scratch(ah_ctx *ctx, size_t bytes) {
-    if (bytes <= ctx->scratch_bytes) return AH_OK;
-    if (ctx->scratch) {
-        // the old scratch may still be read by queued kernels
-        AH_HIP(ctx, hipDeviceSynchronize());
-        AH_HIP(ctx, hipFree(ctx->scratch));
-        ctx->scratch = nullptr;
-        ctx->scratch_bytes = 0;
-    }
-    size_t want = bytes + (bytes >> 2) + 4096;
-    if (hipMalloc(&ctx->scratch, want) != hipSuccess) {
-        ctx->scratch = nullptr;
-        return AH_ERR_OUT_OF_MEMORY;
-    }
-    ctx->scratch_bytes = want;
-    return AH_OK;
-}
-
-size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
 
 // Work units of a row: Q8_0 / Q5_0 blocks, Q4_K super-blocks (or, with `pairs`, sub-block pairs
 // of 64 elements), Q2_K / Q3_K / Q6_K half super-blocks (128 elements).
@@ -1033,6 +976,7 @@ const char *ah_status_str(int32_t s) {
     case AH_ERR_OUT_OF_MEMORY: return "out of device memory";
     case AH_ERR_SCRATCH_LIMIT: return "call needs more than the fixed scratch of the no-alloc entry point";
     case AH_ERR_SEQ_TIMEOUT: return "sequence barrier timed out";
+    case AH_ERR_CACHE_RANGE: return "sequence, position or page outside the 4-bit cache";
     case AH_ERR_FFN_OVERFLOW: return "FFN overflow";
     case AH_ERR_EXP_RANGE: return "exp out of range";
     case AH_ERR_ZERO_DENOMINATOR: return "zero denominator";
@@ -1054,7 +998,7 @@ int32_t ah_init(int32_t device, ah_ctx **out) {
     ctx->cu_count = prop.multiProcessorCount > 0 ? prop.multiProcessorCount : 256;
     if (hipSetDevice(device) != hipSuccess || hipStreamCreate(&ctx->stream) != hipSuccess ||
         hipMalloc(&ctx->d_status, 2 * sizeof(unsigned long long)) != hipSuccess ||
-        ah_gemv_init_attrs() != hipSuccess || ah_few_init_attrs() != hipSuccess) {
+        ah_gemv_init_attrs() != hipSuccess || ah_few_init_attrs() != hipSuccess || ah_attn_init_attrs() != hipSuccess) {
         delete ctx;
         return AH_ERR_HIP;
     }

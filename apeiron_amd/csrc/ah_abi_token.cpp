@@ -1,0 +1,296 @@
+// ah_abi_token.cpp -- host side of the operators between a token's projections: argument checks, the
+// rope and cache handles, and the plan of the attention's splits.
+#include "ah_host.h"
+#include "ah_kv4.h"
+
+#include <cmath>
+#include <new>
+
+namespace {
+
+constexpr size_t kMaxU32 = 0x7fffffff;
+
+bool tokens_ok(const ah_kv4_tokens *t) {
+    return t->d_seq && t->d_pos && t->d_table && t->n_seq && t->table_stride && t->n_tok <= kMaxU32 && t->n_seq <= kMaxU32 &&
+           t->table_stride <= kMaxU32;
+}
+KvTokens tokens_of(const ah_kv4_tokens *t) {
+    return {t->d_seq, t->d_pos, t->d_table, (uint32_t)t->n_tok, (uint32_t)t->n_seq, (uint32_t)t->table_stride};
+}
+
+} // namespace
+
+extern "C" {
+
+int32_t ah_norm_quant_dev(ah_ctx *ctx, const float *d_x, const float *d_residual, const float *d_gain, float eps, size_t n_tok,
+                          size_t n, float *d_sum, float *d_y, int8_t *d_codes, int64_t *d_scales, uint16_t *d_values,
+                          void *stream) {
+    if (!ctx || (d_codes == nullptr) != (d_scales == nullptr)) return AH_ERR_INVALID_ARG;
+    if (!(eps >= 0.0f) || n > AH_MAX_N_IN || n_tok > kMaxU32) return AH_ERR_INVALID_ARG;
+    if (n_tok == 0 || n == 0) return AH_OK;
+    if (!d_x || !d_gain || (reinterpret_cast<uintptr_t>(d_scales) & 7)) return AH_ERR_INVALID_ARG;
+    NormArgs a = {d_x, d_residual, d_gain, d_sum, d_y, d_codes, d_scales, d_values, (double)eps, (uint32_t)n_tok, (uint32_t)n,
+                  ctx->d_status};
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_norm(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_rope_create(ah_ctx *ctx, const ah_rope_spec *spec, ah_rope **out) {
+    if (!ctx || !spec || !out) return AH_ERR_INVALID_ARG;
+    *out = nullptr;
+    const size_t dim = spec->head_dim, rot = spec->rot_dim;
+    if (dim > kRopeMaxDim || rot < 2 || rot > dim || (rot & 1) || (dim & 1) || spec->layout > AH_ROPE_INTERLEAVED ||
+        spec->scaling > AH_ROPE_BANDS || !(spec->base > 0.0) || !std::isfinite(spec->base) || !std::isfinite(spec->amplitude))
+        return AH_ERR_INVALID_ARG;
+    const bool scaled = spec->scaling != AH_ROPE_NONE, bands = spec->scaling == AH_ROPE_BANDS;
+    if (scaled && (!(spec->factor > 0.0) || !std::isfinite(spec->factor))) return AH_ERR_INVALID_ARG;
+    if (spec->scaling == AH_ROPE_NTK && rot == 2) return AH_ERR_INVALID_ARG;
+    if (bands && (!(spec->high > spec->low) || !std::isfinite(spec->high) || !std::isfinite(spec->low) ||
+                  !(spec->original_ctx > 0.0) || !std::isfinite(spec->original_ctx)))
+        return AH_ERR_INVALID_ARG;
+    ah_rope *r = new (std::nothrow) ah_rope();
+    double *host = r ? new (std::nothrow) double[rot / 2] : nullptr;
+    if (!host) {
+        delete r;
+        return AH_ERR_OUT_OF_MEMORY;
+    }
+    const double base =
+        spec->scaling == AH_ROPE_NTK ? spec->base * std::pow(spec->factor, (double)rot / (double)(rot - 2)) : spec->base;
+    for (size_t j = 0; j < rot / 2; ++j) {
+        double t = std::pow(base, -2.0 * (double)j / (double)rot);
+        if (spec->scaling == AH_ROPE_LINEAR) t /= spec->factor;
+        if (bands) {
+            double g = (spec->original_ctx * t / 6.283185307179586476925 - spec->low) / (spec->high - spec->low);
+            g = g < 0.0 ? 0.0 : g > 1.0 ? 1.0 : g;
+            t = t * ((1.0 - g) / spec->factor + g);
+        }
+        host[j] = t;
+    }
+    r->host = host;
+    r->ref.dim = (uint32_t)dim;
+    r->ref.rot = (uint32_t)rot;
+    r->ref.interleaved = spec->layout == AH_ROPE_INTERLEAVED;
+    r->ref.amplitude = spec->amplitude != 0.0 ? spec->amplitude : bands ? 0.1 * std::log(spec->factor) + 1.0 : 1.0;
+    void *d = nullptr;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e == hipSuccess) e = hipMalloc(&d, rot / 2 * sizeof(double));
+    if (e == hipSuccess) e = hipMemcpy(d, host, rot / 2 * sizeof(double), hipMemcpyHostToDevice);
+    if (e != hipSuccess) {
+        ctx->last_hip = (int)e;
+        if (d) (void)hipFree(d);
+        delete[] host;
+        delete r;
+        return e == hipErrorOutOfMemory ? AH_ERR_OUT_OF_MEMORY : AH_ERR_HIP;
+    }
+    r->ref.theta = static_cast<const double *>(d);
+    *out = r;
+    return AH_OK;
+}
+
+int32_t ah_rope_free(ah_ctx *ctx, ah_rope *rope) {
+    if (!ctx || !rope) return AH_ERR_INVALID_ARG;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    AH_HIP(ctx, hipFree(const_cast<double *>(rope->ref.theta)));
+    delete[] rope->host;
+    delete rope;
+    return AH_OK;
+}
+
+int32_t ah_rope_info(const ah_rope *rope, double *theta, double *amplitude) {
+    if (!rope) return AH_ERR_INVALID_ARG;
+    if (theta)
+        for (uint32_t j = 0; j < rope->ref.rot / 2; ++j) theta[j] = rope->host[j];
+    if (amplitude) *amplitude = rope->ref.amplitude;
+    return AH_OK;
+}
+
+int32_t ah_rope_dev(ah_ctx *ctx, const ah_rope *rope, const float *d_x, size_t x_stride, size_t n_heads, const int32_t *d_pos,
+                    size_t n_tok, float *d_y, size_t y_stride, void *stream) {
+    if (!ctx || !rope || n_tok > kMaxU32 || n_heads > 65536) return AH_ERR_INVALID_ARG;
+    if (n_tok == 0 || n_heads == 0) return AH_OK;
+    const size_t row = n_heads * rope->ref.dim;
+    if (!d_x || !d_y || !d_pos || x_stride < row || y_stride < row || (d_x == d_y && x_stride != y_stride)) return AH_ERR_INVALID_ARG;
+    RopeArgs a = {rope->ref, d_x, d_y, x_stride, y_stride, d_pos, (uint32_t)n_tok, (uint32_t)n_heads};
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_rope(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_kv4_create(ah_ctx *ctx, size_t n_pages, size_t page_len, size_t n_kv_heads, size_t head_dim, ah_kv4 **out) {
+    if (!ctx || !out) return AH_ERR_INVALID_ARG;
+    *out = nullptr;
+    if (n_pages == 0 || n_pages > kMaxU32 || page_len < 32 || page_len > 1024 || (page_len & (page_len - 1)) || n_kv_heads == 0 ||
+        n_kv_heads > 4096 || (head_dim != 64 && head_dim != 128 && head_dim != 256))
+        return AH_ERR_INVALID_ARG;
+    size_t bytes;
+    if (__builtin_mul_overflow(n_pages, n_kv_heads * (page_len / 32) * 36 * head_dim, &bytes)) return AH_ERR_INVALID_ARG;
+    ah_kv4 *c = new (std::nothrow) ah_kv4();
+    if (!c) return AH_ERR_OUT_OF_MEMORY;
+    void *d = nullptr;
+    hipError_t e = hipSetDevice(ctx->device);
+    if (e == hipSuccess) e = hipMalloc(&d, bytes);
+    if (e == hipSuccess) e = hipMemset(d, 0, bytes);
+    if (e == hipSuccess) e = hipStreamSynchronize(nullptr);
+    if (e != hipSuccess) {
+        ctx->last_hip = (int)e;
+        if (d) (void)hipFree(d);
+        delete c;
+        return e == hipErrorOutOfMemory ? AH_ERR_OUT_OF_MEMORY : AH_ERR_HIP;
+    }
+    c->bytes = bytes;
+    c->ref.base = static_cast<uint8_t *>(d);
+    c->ref.n_pages = (uint32_t)n_pages;
+    c->ref.page_shift = (uint32_t)__builtin_ctzll(page_len);
+    c->ref.n_kv = (uint32_t)n_kv_heads;
+    c->ref.dim = (uint32_t)head_dim;
+    *out = c;
+    return AH_OK;
+}
+
+int32_t ah_kv4_free(ah_ctx *ctx, ah_kv4 *cache) {
+    if (!ctx || !cache) return AH_ERR_INVALID_ARG;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, hipStreamSynchronize(ctx->stream));
+    AH_HIP(ctx, hipFree(cache->ref.base));
+    delete cache;
+    return AH_OK;
+}
+
+int32_t ah_kv4_info(const ah_kv4 *cache, size_t *bytes, size_t *n_pages, size_t *page_len, size_t *n_kv_heads, size_t *head_dim) {
+    if (!cache) return AH_ERR_INVALID_ARG;
+    if (bytes) *bytes = cache->bytes;
+    if (n_pages) *n_pages = cache->ref.n_pages;
+    if (page_len) *page_len = (size_t)1 << cache->ref.page_shift;
+    if (n_kv_heads) *n_kv_heads = cache->ref.n_kv;
+    if (head_dim) *head_dim = cache->ref.dim;
+    return AH_OK;
+}
+
+int32_t ah_kv4_append_dev(ah_ctx *ctx, ah_kv4 *cache, const ah_rope *rope, const ah_kv4_tokens *tokens, const float *d_q,
+                          size_t q_stride, size_t n_heads, float *d_q_out, size_t q_out_stride, const float *d_k, size_t k_stride,
+                          const float *d_v, size_t v_stride, void *stream) {
+    if (!ctx || !cache || !tokens) return AH_ERR_INVALID_ARG;
+    if (tokens->n_tok == 0) return AH_OK;
+    if (!tokens_ok(tokens) || !d_k || !d_v || n_heads > 65536) return AH_ERR_INVALID_ARG;
+    const size_t dim = cache->ref.dim, kv = cache->ref.n_kv * dim;
+    if (k_stride < kv || v_stride < kv || (rope && rope->ref.dim != dim)) return AH_ERR_INVALID_ARG;
+    if (n_heads && (!d_q || !d_q_out || q_stride < n_heads * dim || q_out_stride < n_heads * dim ||
+                    (d_q == d_q_out && q_stride != q_out_stride)))
+        return AH_ERR_INVALID_ARG;
+    AppendArgs a = {};
+    a.c = cache->ref;
+    if (rope) a.rope = rope->ref;
+    a.t = tokens_of(tokens);
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.q_out = d_q_out;
+    a.q_stride = q_stride;
+    a.qo_stride = q_out_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.n_heads = (uint32_t)n_heads;
+    a.status = ctx->d_status;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_kv4_append(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *tokens, uint16_t *d_k, uint16_t *d_v, void *stream) {
+    if (!ctx || !cache || !tokens) return AH_ERR_INVALID_ARG;
+    if (tokens->n_tok == 0 || (!d_k && !d_v)) return AH_OK;
+    if (!tokens_ok(tokens)) return AH_ERR_INVALID_ARG;
+    KvReadArgs a = {cache->ref, tokens_of(tokens), d_k, d_v, ctx->d_status};
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_kv4_read(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, const float *d_q, size_t q_stride, float *d_out,
+                        size_t out_stride, void *stream) {
+    if (!ctx || !cache || !p) return AH_ERR_INVALID_ARG;
+    if (p->n_seq == 0 || p->n_tok == 0 || p->n_heads == 0 || p->max_q == 0) return AH_OK;
+    const size_t dim = cache->ref.dim, kv = cache->ref.n_kv;
+    if (!p->d_q_start || !p->d_ctx || !p->d_table || !d_q || !d_out || p->n_seq > 65535 || p->n_tok > kMaxU32 ||
+        p->n_heads > 65536 || p->n_heads % kv || p->table_stride == 0 || p->table_stride > kMaxU32 || q_stride < p->n_heads * dim ||
+        out_stride < p->n_heads * dim || p->window > kMaxU32 || p->sinks > kMaxU32)
+        return AH_ERR_INVALID_ARG;
+    AttnArgs a = {};
+    a.c = cache->ref;
+    a.q_start = p->d_q_start;
+    a.ctx = p->d_ctx;
+    a.table = p->d_table;
+    a.q = d_q;
+    a.out = d_out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.n_seq = (uint32_t)p->n_seq;
+    a.n_tok = (uint32_t)p->n_tok;
+    a.n_heads = (uint32_t)p->n_heads;
+    a.group = (uint32_t)(p->n_heads / kv);
+    a.max_q = (uint32_t)(p->max_q < p->n_tok ? p->max_q : p->n_tok);
+    a.table_stride = (uint32_t)p->table_stride;
+    a.window = (uint32_t)p->window;
+    a.sinks = (uint32_t)p->sinks;
+    a.scale = p->scale;
+    a.status = ctx->d_status;
+    if ((uint64_t)a.max_q * a.group > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
+    // Pieces of the context: enough workgroups for about three a CU, each with at least a tile a wave.
+    const size_t most = p->table_stride << cache->ref.page_shift;
+    const size_t ctx_len = p->max_ctx < most ? p->max_ctx : most;
+    size_t tiles = (ctx_len + 31) / 32;
+    if (p->window) {
+        const size_t seen = (p->window + a.max_q + 31) / 32 + 1 + (p->sinks + 31) / 32;
+        tiles = tiles < seen ? tiles : seen;
+    }
+    const size_t base = ((size_t)a.max_q * a.group + 15) / 16 * kv * p->n_seq, rows = p->n_tok * p->n_heads;
+    size_t splits = (size_t)ctx->cu_count * 3 / base, fit = (tiles + 3) / 4;
+    const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float));
+    splits = splits < fit ? splits : fit;
+    splits = splits < room ? splits : room;
+    splits = splits < 1 ? 1 : splits;
+    size_t chunk = (tiles + splits - 1) / splits;
+    chunk = chunk < 1 ? 1 : chunk;
+    a.chunk = (uint32_t)chunk;
+    a.splits = (uint32_t)((tiles + chunk - 1) / chunk);
+    a.splits = a.splits < 1 ? 1 : a.splits;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    if (a.splits > 1) {
+        const size_t o = align256(a.splits * rows * dim * sizeof(float));
+        const int32_t st = ensure_scratch(ctx, o + a.splits * rows * 2 * sizeof(float));
+        if (st) return st;
+        a.part_o = static_cast<float *>(ctx->scratch);
+        a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch) + o);
+    }
+    AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, size_t n_rows, size_t n_vocab,
+                      const ah_sample_params *params, const float *d_u, int32_t *d_tokens, float *d_probs, void *stream) {
+    if (!ctx || n_rows > kMaxU32 || n_vocab > (1u << 20)) return AH_ERR_INVALID_ARG;
+    if (n_rows == 0) return AH_OK;
+    if (n_vocab == 0 || row_stride < n_vocab || !d_logits || !d_u || !d_tokens) return AH_ERR_INVALID_ARG;
+    SampleArgs a = {};
+    a.logits = d_logits;
+    a.stride = row_stride;
+    a.n_rows = (uint32_t)n_rows;
+    a.n_vocab = (uint32_t)n_vocab;
+    if (params) {
+        a.temperature = params->d_temperature;
+        a.top_k = params->d_top_k;
+        a.top_p = params->d_top_p;
+        a.min_p = params->d_min_p;
+    }
+    a.u = d_u;
+    a.tokens = d_tokens;
+    a.probs = d_probs;
+    a.status = ctx->d_status;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_sample(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+} // extern "C"

@@ -60,6 +60,7 @@ extern "C" {
 #define AH_ERR_OUT_OF_MEMORY 23
 #define AH_ERR_SCRATCH_LIMIT 24       /* a no-alloc call needs more than its fixed scratch  */
 #define AH_ERR_SEQ_TIMEOUT 25         /* a sequence's grid barrier waited past its limit    */
+#define AH_ERR_CACHE_RANGE 27         /* a sequence, position or page outside the 4-bit cache */
 
 /* ggml type ids (format/quant.rs:20-49) */
 #define AH_GGML_Q5_0 6   /* format/quant.rs:28-29, :261-297 */
@@ -357,6 +358,126 @@ int32_t ah_gemm_group_f32_dev(ah_ctx *ctx, size_t n_parts, const ah_tensor *cons
 int32_t ah_gemm_group_q8_dev(ah_ctx *ctx, size_t n_parts, const ah_tensor *const *w,
                              const int8_t *d_codes, const int64_t *d_scales, size_t n_tok,
                              float *const *d_y, void *stream);
+
+/* ---- between the projections: norm, rotary positions, the 4-bit cache, attention, sampling ----
+ *
+ * The operators of a decode token or a prefill chunk that stand between its projections, on the
+ * device, so that f32 activations and QuantActs pass from call to call without the host:
+ *   ah_norm_quant_dev -> q/k/v (ah_gemv_q8_dev, ah_gemm_group_q8_dev) -> ah_kv4_append_dev ->
+ *   ah_kv4_attn_dev -> o (ah_gemv_f32_dev) -> ah_norm_quant_dev -> the FFN (ah_ffn_q8_dev,
+ *   ah_ffn_prefill_q8_dev) -> ... -> ah_norm_quant_dev -> the head -> ah_sample_dev.
+ * No counterpart in the reference's int8 chart (its norm, RoPE, softmax attention and sampler are
+ * exact Q32.32 integer code of the engine: ops/{norm,rope,sampler}.rs, attn.rs).  Activations are f32
+ * rows; sums and statistics are held in f32 or f64. */
+
+/* s = x + residual (residual NULL: s = x); y = s / sqrt(mean(s^2) + eps) * gain per token of n values
+ * (1 <= n <= AH_MAX_N_IN), and y's QuantAct, bit-exact to ah_quant_act_f32_dev on the same y.
+ * Outputs, each NULL to skip: d_sum = s (may be d_x or d_residual itself), d_y = y (may be d_x),
+ * d_codes[n_tok][n] with d_scales[n_tok][ceil(n/32)] (both or neither; 8-byte aligned scales), and
+ * d_values[n_tok][n], the values that the codes stand for as bf16 (exact).  A y that is not finite or
+ * has no Q32.32 value is refused as ah_quant_act_f32_dev refuses it (only where codes or values are
+ * asked for). */
+int32_t ah_norm_quant_dev(ah_ctx *ctx, const float *d_x, const float *d_residual, const float *d_gain, float eps,
+                          size_t n_tok, size_t n, float *d_sum, float *d_y, int8_t *d_codes, int64_t *d_scales,
+                          uint16_t *d_values, void *stream);
+
+/* Rotary positions.  Pair j of the first rot_dim channels of a head turns by position * theta_j, with
+ * theta_j = base^(-2 j / rot_dim); channels past rot_dim pass through.  Layout: HALF pairs channel j
+ * with j + rot_dim / 2, INTERLEAVED 2 j with 2 j + 1.  Scalings for contexts longer than the model's:
+ *   LINEAR: theta / factor;  NTK: base * factor^(rot_dim / (rot_dim - 2)) as the base;
+ *   BANDS: with r = original_ctx * theta / 2 pi turns over the original context and
+ *          g = clamp((r - low) / (high - low), 0, 1), theta * ((1 - g) / factor + g).
+ * amplitude multiplies cosine and sine (0: 1, and 0.1 ln(factor) + 1 for BANDS). */
+#define AH_ROPE_HALF 0u
+#define AH_ROPE_INTERLEAVED 1u
+#define AH_ROPE_NONE 0u
+#define AH_ROPE_LINEAR 1u
+#define AH_ROPE_NTK 2u
+#define AH_ROPE_BANDS 3u
+typedef struct ah_rope ah_rope;
+typedef struct ah_rope_spec {
+    size_t head_dim, rot_dim; /* even; 2 <= rot_dim <= head_dim <= 512 */
+    uint32_t layout, scaling;
+    double base, factor, low, high, original_ctx, amplitude;
+} ah_rope_spec;
+int32_t ah_rope_create(ah_ctx *ctx, const ah_rope_spec *spec, ah_rope **out);
+int32_t ah_rope_free(ah_ctx *ctx, ah_rope *rope);
+/* theta[rot_dim / 2] (host, optional) and the amplitude (optional) of a rope. */
+int32_t ah_rope_info(const ah_rope *rope, double *theta, double *amplitude);
+/* Rotates n_heads heads of every token: rows of x_stride / y_stride floats, head h at h * head_dim.
+ * d_y may be d_x (with the same stride).  d_pos[n_tok]: positions, any int32. */
+int32_t ah_rope_dev(ah_ctx *ctx, const ah_rope *rope, const float *d_x, size_t x_stride, size_t n_heads,
+                    const int32_t *d_pos, size_t n_tok, float *d_y, size_t y_stride, void *stream);
+
+/* A paged key/value cache of one layer, held in 4 bits: n_pages pages of page_len positions (a power
+ * of two, 32 to 1024), n_kv_heads heads of head_dim (64, 128 or 256) channels.  A block is 32 channels of
+ * one position and head: d is the f16 number of 8 significant bits nearest to -m / 8 (m the element of
+ * largest magnitude, the positive one of two), an element's code is clamp(rint(x / d), -8, 7) + 8 and
+ * stands for (code - 8) d: 4.5 bits a channel, every value exact in f16.  A new cache holds zeros. */
+typedef struct ah_kv4 ah_kv4;
+int32_t ah_kv4_create(ah_ctx *ctx, size_t n_pages, size_t page_len, size_t n_kv_heads, size_t head_dim, ah_kv4 **out);
+int32_t ah_kv4_free(ah_ctx *ctx, ah_kv4 *cache);
+/* Bytes on the device (optional), and its geometry (each optional). */
+int32_t ah_kv4_info(const ah_kv4 *cache, size_t *bytes, size_t *n_pages, size_t *page_len, size_t *n_kv_heads,
+                    size_t *head_dim);
+/* Tokens by sequence and position: token t is position d_pos[t] of sequence d_seq[t], in page
+ * d_table[seq][pos / page_len].  d_seq[t] < 0: a padding token, passed over.  A sequence, position or page
+ * out of range is refused with AH_ERR_CACHE_RANGE (ah_sync_status) and the token passed over. */
+typedef struct ah_kv4_tokens {
+    const int32_t *d_seq, *d_pos; /* [n_tok] */
+    size_t n_tok;
+    const int32_t *d_table;       /* [n_seq][table_stride] page indices */
+    size_t n_seq, table_stride;
+} ah_kv4_tokens;
+/* One launch: rotates q into d_q_out (may be d_q with the same stride; n_heads 0: no q), rotates k and
+ * puts it and v into the cache (rope NULL: no rotation).  Rows of *_stride floats, heads contiguous.
+ * The same (seq, pos) twice in a call leaves either's values.  A block with a value that is not finite is
+ * stored as zeros and refused with AH_ERR_NONFINITE_INPUT. */
+int32_t ah_kv4_append_dev(ah_ctx *ctx, ah_kv4 *cache, const ah_rope *rope, const ah_kv4_tokens *tokens, const float *d_q,
+                          size_t q_stride, size_t n_heads, float *d_q_out, size_t q_out_stride, const float *d_k,
+                          size_t k_stride, const float *d_v, size_t v_stride, void *stream);
+/* The values held for tokens, as f16 [n_tok][n_kv_heads][head_dim] (d_k or d_v may be NULL); zeros for
+ * tokens passed over. */
+int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *tokens, uint16_t *d_k, uint16_t *d_v,
+                        void *stream);
+
+/* Attention over the cache.  Sequence s has d_ctx[s] positions in it and asks with the tokens
+ * d_q_start[s] .. d_q_start[s + 1] - 1, which stand at its last positions; a query at position p sees the
+ * positions t <= p and, with window > 0, of those t > p - window or t < sinks.  Head h reads KV head
+ * h / (n_heads / n_kv_heads).  out = sum_t softmax(scale q . k_t) v_t, zeros for a query that sees
+ * nothing (more tokens than positions).  Tokens of no sequence are not written.
+ * max_q: at least the largest number of a sequence's tokens; max_ctx: the largest context expected (it
+ * plans how the contexts are cut; longer ones are still served whole).  A sequence whose tokens, context
+ * or pages are out of range is refused with AH_ERR_CACHE_RANGE: its tokens are not written, or (a page)
+ * the page's positions not seen.  Uses the context's scratch (as ah_gemm_f32_dev). */
+typedef struct ah_kv4_attn {
+    size_t n_seq, n_tok, n_heads, max_q, max_ctx;
+    const int32_t *d_q_start; /* [n_seq + 1] */
+    const int32_t *d_ctx;     /* [n_seq] */
+    const int32_t *d_table;   /* [n_seq][table_stride] */
+    size_t table_stride;
+    float scale;
+    size_t window, sinks;
+} ah_kv4_attn;
+int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, const float *d_q, size_t q_stride,
+                        float *d_out, size_t out_stride, void *stream);
+
+/* One token per row of logits [n_rows][n_vocab] (rows row_stride floats apart; n_vocab <= 2^20).  In the
+ * order (logit descending, index ascending), with weights w = rint(2^32 exp((logit - largest) / T)): the
+ * first top_k tokens are kept (top_k <= 0 or >= n_vocab: all), of those the ones whose preceding weight is
+ * below top_p times the weight of all (top_p >= 1: all), of those the ones with w >= min_p 2^32; the first
+ * always.  The token is the smallest index at which the kept weight up to and with it, in index order,
+ * passes floor(u W), u in [0, 1) the row's random number.  T = 0 takes the first token.  d_probs
+ * (optional): w / W of the token.  Per-row parameters, each NULL for 1, 0, 1 and 0.  A NaN logit is never
+ * drawn and refused with AH_ERR_NONFINITE_INPUT, as is a row without a logit above -inf (its token is
+ * -1); T below 0, infinite or NaN is refused with AH_ERR_INPUT_RANGE and taken as 0. */
+typedef struct ah_sample_params {
+    const float *d_temperature;
+    const int32_t *d_top_k;
+    const float *d_top_p, *d_min_p;
+} ah_sample_params;
+int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, size_t n_rows, size_t n_vocab,
+                      const ah_sample_params *params, const float *d_u, int32_t *d_tokens, float *d_probs, void *stream);
 
 /* ---- debug: exact integer group dots (the bit-exact quantity of the contract) ---- */
 
