@@ -9,6 +9,7 @@
 namespace {
 
 constexpr size_t kMaxU32 = 0x7fffffff;
+constexpr size_t kAttnGroups = 2048;
 
 bool tokens_ok(const ah_kv4_tokens *t) {
     return t->d_seq && t->d_pos && t->d_table && t->n_seq && t->table_stride && t->n_tok <= kMaxU32 && t->n_seq <= kMaxU32 &&
@@ -237,7 +238,8 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     a.scale = p->scale;
     a.status = ctx->d_status;
     if ((uint64_t)a.max_q * a.group > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
-    // Pieces of the context: enough workgroups for about three a CU, each with at least a tile a wave.
+    // Pieces of the context: up to kAttnGroups workgroups in all, each with at least a tile a wave.  The bound
+    // counts every sequence as the longest; of uneven ones about half the workgroups have work.
     const size_t most = p->table_stride << cache->ref.page_shift;
     const size_t ctx_len = p->max_ctx < most ? p->max_ctx : most;
     size_t tiles = (ctx_len + 31) / 32;
@@ -245,13 +247,14 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
         const size_t seen = (p->window + a.max_q + 31) / 32 + 1 + (p->sinks + 31) / 32;
         tiles = tiles < seen ? tiles : seen;
     }
-    const size_t base = ((size_t)a.max_q * a.group + 15) / 16 * kv * p->n_seq, rows = p->n_tok * p->n_heads;
-    size_t splits = (size_t)ctx->cu_count * 3 / base, fit = (tiles + 3) / 4;
+    a.rows = a.max_q * a.group <= 8 ? 8 : 16;
+    const size_t base = ((size_t)a.max_q * a.group + a.rows - 1) / a.rows * kv * p->n_seq, rows = p->n_tok * p->n_heads;
+    size_t splits = kAttnGroups / base, fit = (tiles + 3) / 4;
     const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float));
     splits = splits < fit ? splits : fit;
     splits = splits < room ? splits : room;
     splits = splits < 1 ? 1 : splits;
-    size_t chunk = (tiles + splits - 1) / splits;
+    size_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;  // whole rounds of the four waves
     chunk = chunk < 1 ? 1 : chunk;
     a.chunk = (uint32_t)chunk;
     a.splits = (uint32_t)((tiles + chunk - 1) / chunk);

@@ -24,32 +24,34 @@ constexpr float kUp = 9.0f;
 
 AH_DEV f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
-// 8 codes of a dword as f16 values: low nibbles of its half-words, then the next ones.  1024 + c has c in
-// its lowest mantissa bits; (1024 + c) - 1032 and the product by d are exact.
-AH_DEV f16x2 nibbles(uint32_t w, uint32_t at) {
-    return __builtin_bit_cast(f16x2, ((w >> at) & 0x000F000Fu) | 0x64006400u) - (f16x2)((_Float16)1032.0f);
+// Codes as f16 values.  1024 + c has c in its lowest mantissa bits, 1024 + 16 c in the next four:
+// (1024 + c) - 1032, (1024 + 16 c) / 16 - 72 and the products by d are exact.  The masks stay in registers
+// (an instruction takes one constant from outside them), so a pair is one v_and_or and two packed steps.
+struct Masks {
+    uint32_t low, high;
+    AH_DEV Masks() : low(0x000F000Fu), high(0x00F000F0u) { __asm__("" : "+v"(low), "+v"(high)); }
+};
+AH_DEV f16x2 low_nibbles(uint32_t w, const Masks &k) {
+    return __builtin_bit_cast(f16x2, (w & k.low) | 0x64006400u) - (f16x2)((_Float16)1032.0f);
 }
-AH_DEV f16x2 pair_of(uint16_t h) { return (f16x2)(__builtin_bit_cast(_Float16, h)); }
-AH_DEV f16x8 k_frag(uint32_t w, f16x2 d) {
-    f16x8 f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const f16x2 v = nibbles(w, 4 * k) * d;
-        f[2 * k] = v[0];
-        f[2 * k + 1] = v[1];
-    }
-    return f;
+AH_DEV f16x2 high_nibbles(uint32_t w, const Masks &k) {
+    return __builtin_elementwise_fma(__builtin_bit_cast(f16x2, (w & k.high) | 0x64006400u), (f16x2)((_Float16)0.0625f), (f16x2)((_Float16)-72.0f));
 }
-// The tokens' values of the even (at = 0) or odd (at = 4) channel of a pair: two dwords, four tokens each.
-AH_DEV f16x8 v_frag(uint32_t w0, uint32_t w1, uint32_t at, f16x8 d) {
-    f16x8 f;
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        const f16x2 v = nibbles(k < 2 ? w0 : w1, 8 * (k & 1) + at) * (f16x2){d[2 * k], d[2 * k + 1]};
-        f[2 * k] = v[0];
-        f[2 * k + 1] = v[1];
-    }
-    return f;
+AH_DEV f16x8 join8(f16x2 a, f16x2 b, f16x2 c, f16x2 d) {
+    return (f16x8){a[0], a[1], b[0], b[1], c[0], c[1], d[0], d[1]};
+}
+AH_DEV f16x2 pair_of(uint32_t h) { return __builtin_bit_cast(f16x2, (h & 0xffffu) | h << 16); }
+// Eight channels of a K row: a dword's nibbles 0 and 4, 1 and 5, 2 and 6, 3 and 7.
+AH_DEV f16x8 k_frag(uint32_t w, f16x2 d, const Masks &k) {
+    const uint32_t v = w >> 8;
+    return join8(low_nibbles(w, k) * d, high_nibbles(w, k) * d, low_nibbles(v, k) * d, high_nibbles(v, k) * d);
+}
+// The eight tokens' values of both channels of a pair: two dwords, four tokens each.
+AH_DEV void v_frags(uint32_t w0, uint32_t w1, f16x8 d, const Masks &k, f16x8 &even, f16x8 &odd) {
+    const f16x2 d0 = {d[0], d[1]}, d1 = {d[2], d[3]}, d2 = {d[4], d[5]}, d3 = {d[6], d[7]};
+    const uint32_t u0 = w0 >> 8, u1 = w1 >> 8;
+    even = join8(low_nibbles(w0, k) * d0, low_nibbles(u0, k) * d1, low_nibbles(w1, k) * d2, low_nibbles(u1, k) * d3);
+    odd = join8(high_nibbles(w0, k) * d0, high_nibbles(u0, k) * d1, high_nibbles(w1, k) * d2, high_nibbles(u1, k) * d3);
 }
 
 AH_DEV float xor_lanes(float v, int mask) { return __shfl_xor(v, mask, 64); }
@@ -96,36 +98,100 @@ AH_DEV uint32_t piece_of(const AttnArgs &a, const Tiles &t) {
     return need > a.chunk ? need : a.chunk;
 }
 
-// Sixteen rows (token, head of the group) a workgroup, as the columns of the products: every wave takes
-// tiles of 32 tokens of the workgroup's piece of the context, each with its own running maximum, and the
-// four meet in LDS.  A lane (r, h) holds the scores of column r, tokens 4 h + i of both half-tiles.
-template <int D>
-__global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
+// Byte offset in the cache of tile `tile` of sequence s for head kvh, through the page table; `ok` false where
+// the page is outside.  The index is read through the scalar cache: it is the same for the whole wave.
+AH_DEV const uint8_t *tile_at(const AttnArgs &a, uint32_t s, uint32_t kvh, uint32_t tile, bool &ok) {
+    typedef const int32_t __attribute__((address_space(4))) *cptr;
+    const uint32_t in = a.c.page_shift - 5, pi = tile >> in;
+    const uint32_t page = (uint32_t)((cptr)(uintptr_t)a.table)[(size_t)s * a.table_stride + pi];
+    ok = page < a.c.n_pages;
+    return a.c.base + kv4_tile(a.c, ok ? page : 0, kvh, tile & ((1u << in) - 1));
+}
+
+// One lane's part of a tile.
+template <int D> struct KTile {
+    u32x4 w[D / 64];                       // codes (ah_kv4.h)
+    uint32_t d[D == 256 ? 2 : 1];          // both half-tiles' scales of the lane's channels
+    AH_DEV void load(const uint8_t *t, uint32_t r, uint32_t h) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) __builtin_memcpy(&w[c], t + c * 1024 + (r * 4 + h) * 16, 16);
+        __builtin_memcpy(d, t + 32 * D + (r * (D / 32) + (D == 64 ? h >> 1 : D == 128 ? h : 2 * h)) * 4, D == 256 ? 8 : 4);
+    }
+    AH_DEV uint32_t code(int half, int j) const {
+        return D == 64 ? w[0][2 * half + j] : w[half * (D / 128) + j / 4][j & 3];
+    }
+    AH_DEV f16x2 scale(int half, int j) const {
+        const uint32_t v = d[D == 256 ? j / 4 : 0];
+        return pair_of(half ? v >> 16 : v);
+    }
+};
+template <int D> struct VTile {
+    u32x4 w[D / 64];
+    f16x8 d[D / 32];
+    AH_DEV void load(const uint8_t *t, uint32_t r, uint32_t h) {
+#pragma unroll
+        for (int c = 0; c < D / 64; ++c) __builtin_memcpy(&w[c], t + 16 * D + (c * 16 + r) * 64 + h * 16, 16);
+#pragma unroll
+        for (int g = 0; g < D / 32; ++g) __builtin_memcpy(&d[g], t + 34 * D + (g * 4 + h) * 16, 16);
+    }
+};
+
+AH_DEV float ror8(float v) {  // lane r ^ 8 of each 16 (a rotation by 8)
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true));
+}
+AH_DEV f16x2 pack16(float a, float b) { return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+
+// Rows (token, head of the group) as the 16 columns of the products: every wave takes tiles of 32 tokens of
+// the workgroup's piece of the context, each with its own running maximum, and the four meet in LDS.  A
+// lane (r, h) holds the scores of column r, tokens 4 h + i of both half-tiles.
+//   PACK: 8 rows, column r the hi half of row r & 7 for r < 8 and the lo half for r >= 8: one product gives
+//   both (they meet by a rotation of the columns), half the matrix work where a call has few rows.
+//   Otherwise 16 rows and a product for each half.
+// A tile's K is used first and its V last, so the next tile's K loads go out as soon as the scores are
+// formed and its V loads as soon as the output is: a wave always has half a tile on its way.
+template <int D, bool PACK>
+__global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnArgs a) {
     constexpr int NJ = D / 32;  // contraction steps of K q, and blocks of channels
+    constexpr uint32_t R = PACK ? 8 : 16;
     extern __shared__ float lds[];
     float *red_o = lds;                   // [4][16][D + 4]
     float *red_m = lds + 4 * 16 * (D + 4);  // [4][16], then the sums
     float *red_l = red_m + 64;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t split = blockIdx.x % a.splits, rest = blockIdx.x / a.splits, kvh = rest % a.c.n_kv, rt = rest / a.c.n_kv;
-    const uint32_t s = blockIdx.y;
+    // pieces run slowest: the workgroups without work (pieces past a short context) are the last ones, and
+    // every XCD (workgroups go to them in turn) gets its share of those with work; a context's pieces go
+    // round the XCDs
+    const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units, unit = (blockIdx.x - split * units + split) % units;
+    const uint32_t per = units / a.n_seq, s = unit / per, rest = unit - s * per, rt = rest / a.c.n_kv, kvh = rest - rt * a.c.n_kv;
     const Span p = span_of(a, s);
-    if (p.bad && blockIdx.x == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
-    const uint32_t rows = p.nq * a.group, row0 = rt * 16;
+    if (p.bad && split == 0 && rest == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
+    const uint32_t rows = p.nq * a.group, row0 = rt * R;
     if (row0 >= rows) return;
-    const uint32_t row = row0 + r, tok = row / a.group, hq = kvh * a.group + row % a.group;
-    const bool live = row < rows;
+    const uint32_t row = row0 + r % R, tok = row / a.group, hq = kvh * a.group + row % a.group;
+    const bool live = row < rows, low = PACK && r >= 8;
     const int32_t pos0 = p.ctx - (int32_t)p.nq;
-    const uint32_t last = row0 + 15 < rows ? row0 + 15 : rows - 1;
+    const uint32_t last = row0 + R - 1 < rows ? row0 + R - 1 : rows - 1;
     const int32_t lo = pos0 + (int32_t)(row0 / a.group), hi = pos0 + (int32_t)(last / a.group);
     const int32_t pos = live ? pos0 + (int32_t)tok : -1;
     const Tiles T = tiles_of(a, lo, hi);
     const uint32_t chunk = piece_of(a, T), t0 = split * chunk, t1 = t0 + chunk < T.count ? t0 + chunk : T.count;
     if (split > 0 && t0 >= T.count) return;
 
+    // the first tile's loads go out before q is prepared
+    KTile<D> k;
+    VTile<D> v;
+    bool ok = true;
+    uint32_t ti = t0 + wave;
+    auto tile_of = [&](uint32_t i) { return i < T.head ? i : T.tail + (i - T.head); };
+    if (ti < t1) {
+        const uint8_t *t = tile_at(a, s, kvh, tile_of(ti), ok);
+        k.load(t, r, h);
+        v.load(t, r, h);
+    }
+
     // q, scaled by a power of two so that its largest magnitude is in [2^13, 2^14), as hi + lo
-    f16x8 qh[NJ], ql[NJ];
+    f16x8 qh[NJ], ql[PACK ? 1 : NJ];
     float f;
     {
         const float *q = a.q + (size_t)(p.q0 + tok) * a.q_stride + (size_t)hq * D + h * (D / 4);
@@ -144,15 +210,18 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
         int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;  // top in [2^e, 2^(e+1))
         e = e < -100 ? -100 : e > 127 ? 127 : e;
         const float up = __builtin_ldexpf(1.0f, 13 - e);
-        f = a.scale * kLog2e * __builtin_ldexpf(1.0f, e - 13);
+        // scores times f are in powers of two.  f > 0 (a negative scale turns q's sign), so that the largest
+        // product is also the largest score, and a masked -inf stays that.
+        f = __builtin_fmaxf(__builtin_fabsf(a.scale) * kLog2e * __builtin_ldexpf(1.0f, e - 13), 0x1p-126f);
+        const float sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -up : a.scale > 0.0f ? up : a.scale;
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const float v = x[j][i] * up;
-                const _Float16 hv = (_Float16)v;
-                qh[j][i] = hv;
-                ql[j][i] = (_Float16)(v - (float)hv);
+                const float y = x[j][i] * sign;
+                const _Float16 hv = (_Float16)y, lv = (_Float16)(y - (float)hv);
+                qh[j][i] = low ? lv : hv;
+                if (!PACK) ql[j][i] = lv;
             }
     }
 
@@ -160,71 +229,51 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
 #pragma unroll
     for (int g = 0; g < NJ; ++g) acc[g][0] = acc[g][1] = (f32x4)0.0f;
     float m = kNoMax, l = 0.0f;
-    for (uint32_t ti = t0 + wave; ti < t1; ti += 4) {
-        const uint32_t tile = ti < T.head ? ti : T.tail + (ti - T.head);
-        const uint32_t pi = tile >> (a.c.page_shift - 5);
-        const uint32_t page = (uint32_t)a.table[(size_t)s * a.table_stride + pi];
-        if (page >= a.c.n_pages) {
-            if (lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
-            continue;
-        }
-        const uint8_t *t = a.c.base + kv4_tile(a.c, page, kvh, tile & ((1u << (a.c.page_shift - 5)) - 1));
-        // K: per half-tile NJ dwords of codes, and the scales of this lane's channels
-        uint32_t kc[2][NJ];
-        uint16_t kd[2][D == 256 ? 2 : 1];
-#pragma unroll
-        for (int c = 0; c < D / 64; ++c) {
-            u32x4 w;
-            __builtin_memcpy(&w, t + c * 1024 + (r * 4 + h) * 16, 16);
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                if constexpr (D == 64) kc[i >> 1][i & 1] = w[i];
-                else kc[c / (D / 128)][4 * (c % (D / 128)) + i] = w[i];
-            }
-        }
-        {
-            const uint8_t *sc = t + 32 * D + r * (D / 32) * 4;
-#pragma unroll
-            for (int b = 0; b < (D == 256 ? 2 : 1); ++b) {
-                uint32_t w;
-                __builtin_memcpy(&w, sc + 4 * (D == 64 ? h >> 1 : D == 128 ? h : 2 * h + b), 4);
-                kd[0][b] = (uint16_t)w;
-                kd[1][b] = (uint16_t)(w >> 16);
-            }
-        }
-        float x[8];
+    const Masks mk;
+    const float minus_low = low ? -1.0f : 0.0f;
+    for (; ti < t1; ti += 4) {
+        const uint32_t tile = tile_of(ti), next = ti + 4 < t1 ? ti + 4 : ti;
+        bool ok_next;
+        const uint8_t *tn = tile_at(a, s, kvh, tile_of(next), ok_next);
+        f32x4 c[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            f32x4 c = (f32x4)0.0f;
+            c[half] = (f32x4)0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
-                const f16x8 k = k_frag(kc[half][j], pair_of(kd[half][D == 256 ? j / 4 : 0]));
-                c = mfma16(k, qh[j], c);
-                c = mfma16(k, ql[j], c);
+                const f16x8 kf = k_frag(k.code(half, j), k.scale(half, j), mk);
+                c[half] = mfma16(kf, qh[j], c[half]);
+                if (!PACK) c[half] = mfma16(kf, ql[j], c[half]);
             }
+        }
+        k.load(tn, r, h);
+        float x[8];
 #pragma unroll
-            for (int i = 0; i < 4; ++i) x[4 * half + i] = c[i] * f;
+        for (int i = 0; i < 8; ++i) {
+            const float y = c[i >> 2][i & 3];
+            x[i] = PACK ? y + ror8(y) : y;
         }
         const int32_t first = (int32_t)(tile * 32);
         // a tile that every row sees whole needs no mask
-        const bool whole = first + 31 <= lo && (!a.window || (int64_t)first > (int64_t)hi - (int64_t)a.window || first + 32 <= (int64_t)a.sinks);
+        const bool whole = ok && first + 31 <= lo && (!a.window || (int64_t)first > (int64_t)hi - (int64_t)a.window || first + 32 <= (int64_t)a.sinks);
         if (!whole) {
+            if (!ok && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int32_t k = first + 16 * (i >> 2) + 4 * (int32_t)h + (i & 3);
-                const bool see = k <= pos && (!a.window || (int64_t)k > (int64_t)pos - (int64_t)a.window || (uint32_t)k < a.sinks);
+                const int32_t key = first + 16 * (i >> 2) + 4 * (int32_t)h + (i & 3);
+                const bool see = ok && key <= pos && (!a.window || (int64_t)key > (int64_t)pos - (int64_t)a.window || (uint32_t)key < a.sinks);
                 x[i] = see ? x[i] : -__builtin_inff();
             }
         }
         float top = x[0];
 #pragma unroll
         for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
+        top *= f;
         if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0ull) {
             top = __builtin_fmaxf(top, xor_lanes(top, 16));
             top = __builtin_fmaxf(top, xor_lanes(top, 32));
-            const float next = __builtin_fmaxf(m, top);
-            const float alpha = __builtin_amdgcn_exp2f(m - next);
-            m = next;
+            const float up = __builtin_fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - up);
+            m = up;
             l *= alpha;
 #pragma unroll
             for (int g = 0; g < NJ; ++g) {
@@ -232,40 +281,38 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
                 acc[g][1] *= alpha;
             }
         }
-        const float base = m - kUp;
-        f16x8 ph, pl;
+        const float base = kUp - m;
+        f16x2 ph[4], pl[4];
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float e = __builtin_amdgcn_exp2f(x[i] - base);
-            l += e;
-            const _Float16 hv = (_Float16)e;
-            ph[i] = hv;
-            pl[i] = (_Float16)(e - (float)hv);
+        for (int i = 0; i < 4; ++i) {
+            float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], f, base)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], f, base));
+            l += e0;
+            l += e1;
+            ph[i] = pack16(e0, e1);
+            // what is left of p past its hi half; a packed column takes that or p itself
+            const float k = PACK ? minus_low : -1.0f;
+            pl[i] = pack16(__builtin_fmaf((float)ph[i][0], k, e0), __builtin_fmaf((float)ph[i][1], k, e1));
         }
-        // V: per pair of channel blocks 16 bytes (two blocks' eight tokens), and the tokens' scales
+        const f16x8 pg = join8(pl[0], pl[1], pl[2], pl[3]), pf = PACK ? pg : join8(ph[0], ph[1], ph[2], ph[3]);
 #pragma unroll
-        for (int g2 = 0; g2 < D / 64; ++g2) {
-            u32x4 w;
-            __builtin_memcpy(&w, t + 16 * D + (g2 * 16 + r) * 64 + h * 16, 16);
-#pragma unroll
-            for (int b = 0; b < 2; ++b) {
-                const int g = 2 * g2 + b;
-                f16x8 d;
-                __builtin_memcpy(&d, t + 34 * D + (g * 4 + h) * 16, 16);
-#pragma unroll
-                for (int odd = 0; odd < 2; ++odd) {
-                    const f16x8 v = v_frag(w[2 * b], w[2 * b + 1], 4 * odd, d);
-                    acc[g][odd] = mfma16(v, ph, acc[g][odd]);
-                    acc[g][odd] = mfma16(v, pl, acc[g][odd]);
-                }
+        for (int g = 0; g < NJ; ++g) {
+            f16x8 even, odd;
+            v_frags(v.w[g >> 1][2 * (g & 1)], v.w[g >> 1][2 * (g & 1) + 1], v.d[g], mk, even, odd);
+            acc[g][0] = mfma16(even, pf, acc[g][0]);
+            acc[g][1] = mfma16(odd, pf, acc[g][1]);
+            if (!PACK) {
+                acc[g][0] = mfma16(even, pg, acc[g][0]);
+                acc[g][1] = mfma16(odd, pg, acc[g][1]);
             }
         }
+        v.load(tn, r, h);
+        ok = ok_next;
     }
 
     // the lanes' sums of a column, then the four waves
     l += xor_lanes(l, 16);
     l += xor_lanes(l, 32);
-    if (h == 0) {
+    if (h == 0 && !low) {
         red_m[wave * 16 + r] = m;
         red_l[wave * 16 + r] = l;
     }
@@ -274,14 +321,15 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
         float o[8];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
-            o[2 * i] = acc[g][0][i];
-            o[2 * i + 1] = acc[g][1][i];
+            const float e = acc[g][0][i], d = acc[g][1][i];
+            o[2 * i] = PACK ? e + ror8(e) : e;
+            o[2 * i + 1] = PACK ? d + ror8(d) : d;
         }
-        __builtin_memcpy(red_o + (wave * 16 + r) * (D + 4) + 32 * g + 8 * h, o, 32);
+        if (!low) __builtin_memcpy(red_o + (wave * 16 + r) * (D + 4) + 32 * g + 8 * h, o, 32);
     }
     __syncthreads();
     const uint32_t rr = threadIdx.x >> 4, row_out = row0 + rr;
-    if (row_out >= rows) return;
+    if (rr >= R || row_out >= rows) return;
     float M = kNoMax, L = 0.0f, w4[4];
 #pragma unroll
     for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, red_m[w * 16 + rr]);
@@ -299,9 +347,9 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
         f32x4 o = (f32x4)0.0f;
 #pragma unroll
         for (int w = 0; w < 4; ++w) {
-            f32x4 v;
-            __builtin_memcpy(&v, red_o + (w * 16 + rr) * (D + 4) + c, 16);
-            o += v * w4[w];
+            f32x4 y;
+            __builtin_memcpy(&y, red_o + (w * 16 + rr) * (D + 4) + c, 16);
+            o += y * w4[w];
         }
         o *= inv;
         __builtin_memcpy(dst + c, &o, 16);
@@ -313,13 +361,14 @@ __global__ void __launch_bounds__(256) attn_rows_kernel(AttnArgs a) {
     }
 }
 
-// Joins the pieces of a context: one wave per row (token, head).  A piece past the row's keys was never
-// written; which those are follows from the same tiles_of.
+// Joins the pieces of a context: a workgroup per row (token, head), its waves every fourth piece.  A piece
+// past the row's keys was never written; which those are follows from the same tiles_of.
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, uint32_t tile_rows) {
-    const uint32_t lane = threadIdx.x & 63, s = blockIdx.y;
+    __shared__ float red[4][D + 1];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y;
     const Span p = span_of(a, s);
-    const uint32_t n = p.nq * a.n_heads, it = blockIdx.x * 4 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t n = p.nq * a.n_heads, it = blockIdx.x;
     if (it >= n) return;
     const uint32_t i = it / a.n_heads, head = it % a.n_heads, g = a.group;
     const uint32_t row = i * g + head % g, row0 = row - row % tile_rows;
@@ -335,29 +384,39 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, uint32_t til
     float L = 0.0f, acc[D / 64];
 #pragma unroll
     for (int c = 0; c < D / 64; ++c) acc[c] = 0.0f;
-    for (uint32_t k = 0; k < pieces; ++k) {
+#pragma unroll 4
+    for (uint32_t k = wave; k < pieces; k += 4) {
         const float *ml = a.part_ml + 2 * (k * all + flat), w = __builtin_amdgcn_exp2f(ml[0] - M);
         L += ml[1] * w;
 #pragma unroll
         for (int c = 0; c < D / 64; ++c) acc[c] += a.part_o[(k * all + flat) * D + 64 * c + lane] * w;
     }
-    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    float *dst = a.out + (size_t)(p.q0 + i) * a.out_stride + (size_t)head * D;
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) dst[64 * c + lane] = acc[c] * inv;
+    for (int c = 0; c < D / 64; ++c) red[wave][64 * c + lane] = acc[c];
+    if (lane == 0) red[wave][D] = L;
+    __syncthreads();
+    if (threadIdx.x >= D) return;
+    L = (red[0][D] + red[1][D]) + (red[2][D] + red[3][D]);
+    const float o = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
+    a.out[(size_t)(p.q0 + i) * a.out_stride + (size_t)head * D + threadIdx.x] = L > 0.0f || L != L ? o / L : 0.0f;
 }
 
 template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) * sizeof(float); }
 
 template <int D>
 hipError_t launch(const AttnArgs &a, hipStream_t stream) {
-    const uint32_t tiles = (a.max_q * a.group + 15) / 16;
-    const size_t lds = attn_lds<D>();
-    hipLaunchKernelGGL(attn_rows_kernel<D>, dim3(a.splits * tiles * a.c.n_kv, a.n_seq), dim3(256), lds, stream, a);
+    const bool pack = a.rows == 8;
+    const uint32_t tiles = (a.max_q * a.group + a.rows - 1) / a.rows;
+    hipLaunchKernelGGL((pack ? attn_rows_kernel<D, true> : attn_rows_kernel<D, false>), dim3(a.splits * tiles * a.c.n_kv * a.n_seq), dim3(256),
+                       attn_lds<D>(), stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.max_q * a.n_heads + 3) / 4, a.n_seq), dim3(256), 0, stream, a, 16u);
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.max_q * a.n_heads, a.n_seq), dim3(256), 0, stream, a, a.rows);
     return hipGetLastError();
+}
+
+template <class K> hipError_t allow_lds(K *k, size_t bytes) {
+    return hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
 }
 
 } // namespace
@@ -367,6 +426,6 @@ hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream) {
 }
 
 hipError_t ah_attn_init_attrs() {
-    return hipFuncSetAttribute(reinterpret_cast<const void *>(attn_rows_kernel<256>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                               (int)attn_lds<256>());
+    const hipError_t e = allow_lds(attn_rows_kernel<256, false>, attn_lds<256>());
+    return e != hipSuccess ? e : allow_lds(attn_rows_kernel<256, true>, attn_lds<256>());
 }

@@ -21,34 +21,63 @@ AH_DEV double wave_sum(double v) {
 // row is read once and the quantizer's quads (four lanes a block, ah_units.h) hold whole blocks.  The
 // sum of squares is kept in f64: the f32 row's magnitude cannot overflow it and R is the correctly
 // rounded one whatever the order of the sum.
-template <uint32_t U>
+// Eight consecutive values at any element boundary, `take` of them (constant indices only: the arrays stay
+// in registers).
+template <class T> AH_DEV void load8(T *v, const T *p, uint32_t take) {
+    if (take == 8) {
+        __builtin_memcpy(v, p, 8 * sizeof(T));
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) v[i] = i < take ? p[i] : (T)0;
+}
+template <class T> AH_DEV void store8(T *p, const T *v, uint32_t take) {
+    if (take == 8) {
+        __builtin_memcpy(p, v, 8 * sizeof(T));
+        return;
+    }
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i)
+        if (i < take) p[i] = v[i];
+}
+
+// The same of a row read through a range-checked resource: what lies past its end reads as zero, and no
+// branch stands between the loads of a lane's passes.
+AH_DEV void ld8(float *v, __amdgpu_buffer_rsrc_t r, uint32_t k0) {
+    const u32x4 a = ah_ld128(r, 4 * k0), b = ah_ld128(r, 4 * k0 + 16);
+    __builtin_memcpy(v, &a, 16);
+    __builtin_memcpy(v + 4, &b, 16);
+}
+AH_DEV void st8(__amdgpu_buffer_rsrc_t r, uint32_t k0, const float *v) {
+    u32x4 a, b;
+    __builtin_memcpy(&a, v, 16);
+    __builtin_memcpy(&b, v + 4, 16);
+    __builtin_amdgcn_raw_buffer_store_b128(a, r, (int)(4 * k0), 0, 0);
+    __builtin_amdgcn_raw_buffer_store_b128(b, r, (int)(4 * k0 + 16), 0, 0);
+}
+
+template <uint32_t U, bool RES>
 __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
     __shared__ double red[16];
     const uint32_t tid = threadIdx.x, T = blockDim.x, n = a.n, tok = blockIdx.x;
     const size_t row = (size_t)tok * n;
-    float s[U][8];
-    double ss = 0.0;
+    float s[U][8], r[U][8], g[U][8];
+    const __amdgpu_buffer_rsrc_t xr = ah_rsrc(a.x + row, 4 * n), rr = ah_rsrc(RES ? a.r + row : a.x, 4 * n), gr = ah_rsrc(a.gain, 4 * n);
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         const uint32_t k0 = 8 * (u * T + tid);
-        float r[8];
-        if (k0 + 8 <= n) {
-            __builtin_memcpy(s[u], a.x + row + k0, 32);
-            if (a.r) __builtin_memcpy(r, a.r + row + k0, 32);
-        } else {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                s[u][i] = k0 + i < n ? a.x[row + k0 + i] : 0.0f;
-                if (a.r) r[i] = k0 + i < n ? a.r[row + k0 + i] : 0.0f;
-            }
-        }
-        if (a.r) {
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) s[u][i] += r[i];
-        }
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) ss = __builtin_fma((double)s[u][i], (double)s[u][i], ss);
+        ld8(s[u], xr, k0);
+        if (RES) ld8(r[u], rr, k0);
+        ld8(g[u], gr, k0);
     }
+    double ss = 0.0;
+#pragma unroll
+    for (uint32_t u = 0; u < U; ++u)
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            if (RES) s[u][i] += r[u][i];
+            ss = __builtin_fma((double)s[u][i], (double)s[u][i], ss);
+        }
     ss = wave_sum(ss);
     if (T > 64) {
         if ((tid & 63) == 0) red[tid >> 6] = ss;
@@ -56,24 +85,18 @@ __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
         ss = 0.0;
         for (uint32_t w = 0; w < T / 64; ++w) ss += red[w];
     }
-    const float R = (float)(1.0 / __builtin_sqrt(ss / (double)n + a.eps));
+    // v_rsq_f64 is good to about 2^-28; a Newton step squares that
+    const double mean = ss / (double)n + a.eps, r0 = __builtin_amdgcn_rsq(mean);
+    const float R = (float)(r0 * __builtin_fma(-0.5 * mean, r0 * r0, 1.5));
     const uint32_t nb = (n + 31) / 32;
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         const uint32_t k0 = 8 * (u * T + tid), take = n > k0 ? (n - k0 < 8 ? n - k0 : 8) : 0;
         float y[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) y[i] = (uint32_t)i < take ? (s[u][i] * R) * a.gain[k0 + i] : 0.0f;
-        if (a.sum) {
-            if (take == 8) __builtin_memcpy(a.sum + row + k0, s[u], 32);
-            else
-                for (uint32_t i = 0; i < take; ++i) a.sum[row + k0 + i] = s[u][i];
-        }
-        if (a.y) {
-            if (take == 8) __builtin_memcpy(a.y + row + k0, y, 32);
-            else
-                for (uint32_t i = 0; i < take; ++i) a.y[row + k0 + i] = y[i];
-        }
+        for (uint32_t i = 0; i < 8; ++i) y[i] = (s[u][i] * R) * g[u][i];
+        if (a.sum) st8(ah_rsrc(a.sum + row, 4 * n), k0, s[u]);
+        if (a.y) st8(ah_rsrc(a.y + row, 4 * n), k0, y);
         if (!a.codes && !a.values) continue;
         QuadIn in;
 #pragma unroll
@@ -85,13 +108,10 @@ __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
         const uint32_t b = k0 / 32;
         const QuadOut o = quad_quant(in, AH_SRC_F32, b, a.status, (unsigned long long)row);
         if (a.codes) {
-            int8_t *dst = a.codes + row + k0;
-            if (take == 8) {
-                const u32x2 c = {o.c0, o.c1};
-                __builtin_memcpy(dst, &c, 8);
-            } else {
-                for (uint32_t i = 0; i < take; ++i) dst[i] = (int8_t)(((i < 4 ? o.c0 : o.c1) >> (8 * (i & 3))) & 0xffu);
-            }
+            int8_t c[8];
+            const u32x2 w = {o.c0, o.c1};
+            __builtin_memcpy(c, &w, 8);
+            store8(a.codes + row + k0, c, take);
             if ((tid & 3) == 0 && b < nb) a.scales[(size_t)tok * nb + b] = o.e < 0 ? 0 : (int64_t)(1ull << o.e);
         }
         if (a.values) {  // code * 2^(e - 32): seven bits, exact in bf16
@@ -99,9 +119,7 @@ __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i)
                 v[i] = (uint16_t)(__builtin_bit_cast(uint32_t, (float)(int8_t)(((i < 4 ? o.c0 : o.c1) >> (8 * (i & 3))) & 0xffu) * o.fsc) >> 16);
-            if (take == 8) __builtin_memcpy(a.values + row + k0, v, 16);
-            else
-                for (uint32_t i = 0; i < take; ++i) a.values[row + k0 + i] = v[i];
+            store8(a.values + row + k0, v, take);
         }
     }
 }
@@ -129,14 +147,12 @@ AH_DEV float turn(float a, float ca, float b, float sb) {
 
 // Elements e0 .. e0 + 7 of head row x (take of them) into v, rotated.
 AH_DEV void load_rotated(const RopeRef &r, const float *x, uint32_t e0, uint32_t take, const float *cs, const float *sn, float *v) {
-    if (take == 8) __builtin_memcpy(v, x + e0, 32);
-    else
-        for (uint32_t i = 0; i < 8; ++i) v[i] = i < take ? x[e0 + i] : 0.0f;
+    load8(v, x + e0, take);
     if (!r.theta || e0 >= r.rot) return;
     if (r.interleaved) {
 #pragma unroll
         for (uint32_t i = 0; i < 8; i += 2) {
-            if (e0 + i >= r.rot) break;
+            if (e0 + i >= r.rot) continue;
             const float c = cs[(e0 + i) / 2], s = sn[(e0 + i) / 2], a = v[i], b = v[i + 1];
             v[i] = turn(a, c, b, -s);
             v[i + 1] = turn(b, c, a, s);
@@ -153,9 +169,10 @@ AH_DEV void load_rotated(const RopeRef &r, const float *x, uint32_t e0, uint32_t
         for (uint32_t i = 0; i < 8; ++i) v[i] = turn(v[i], cs[j + i], w[i], first ? -sn[j + i] : sn[j + i]);
         return;
     }
+#pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         const uint32_t e = e0 + i;
-        if (i >= take || e >= r.rot) break;
+        if (i >= take || e >= r.rot) continue;
         const bool first = e < half;
         const uint32_t j = first ? e : e - half;
         v[i] = turn(v[i], cs[j], x[first ? e + half : j], first ? -sn[j] : sn[j]);
@@ -179,9 +196,7 @@ __global__ void __launch_bounds__(256) rope_kernel(RopeArgs a) {
         float v[8];
         if (live) load_rotated(a.rope, x + (size_t)head * a.rope.dim, e0, take, cs, sn, v);
         __syncthreads();
-        if (take == 8) __builtin_memcpy(y + (size_t)head * a.rope.dim + e0, v, 32);
-        else
-            for (uint32_t i = 0; i < take; ++i) y[(size_t)head * a.rope.dim + e0 + i] = v[i];
+        store8(y + (size_t)head * a.rope.dim + e0, v, take);
     }
 }
 
@@ -331,9 +346,10 @@ hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream) {
     // a lane per 8 values up to 1024 lanes, then more passes
     const uint32_t need = (a.n + 7) / 8;
     const uint32_t T = need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : need <= 512 ? 512 : 1024;
-    if (need <= 1024) hipLaunchKernelGGL(norm_quant_kernel<1>, dim3(a.n_tok), dim3(T), 0, stream, a);
-    else if (need <= 2048) hipLaunchKernelGGL(norm_quant_kernel<2>, dim3(a.n_tok), dim3(T), 0, stream, a);
-    else hipLaunchKernelGGL(norm_quant_kernel<4>, dim3(a.n_tok), dim3(T), 0, stream, a);
+    auto *k = need <= 1024   ? (a.r ? norm_quant_kernel<1, true> : norm_quant_kernel<1, false>)
+              : need <= 2048 ? (a.r ? norm_quant_kernel<2, true> : norm_quant_kernel<2, false>)
+                             : (a.r ? norm_quant_kernel<4, true> : norm_quant_kernel<4, false>);
+    hipLaunchKernelGGL(k, dim3(a.n_tok), dim3(T), 0, stream, a);
     return hipGetLastError();
 }
 
