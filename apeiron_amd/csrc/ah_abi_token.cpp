@@ -273,7 +273,7 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
 
 int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, size_t n_rows, size_t n_vocab,
                       const ah_sample_params *params, const float *d_u, int32_t *d_tokens, float *d_probs, void *stream) {
-    if (!ctx || n_rows > kMaxU32 || n_vocab > (1u << 20)) return AH_ERR_INVALID_ARG;
+    if (!ctx || n_rows > 65536 || n_vocab > (1u << 20)) return AH_ERR_INVALID_ARG;
     if (n_rows == 0) return AH_OK;
     if (n_vocab == 0 || row_stride < n_vocab || !d_logits || !d_u || !d_tokens) return AH_ERR_INVALID_ARG;
     SampleArgs a = {};
@@ -292,6 +292,10 @@ int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, siz
     a.probs = d_probs;
     a.status = ctx->d_status;
     AH_HIP(ctx, hipSetDevice(ctx->device));
+    const uint32_t cus = (uint32_t)ctx->cu_count;
+    const int32_t st = ensure_scratch(ctx, ah_sample_plan(a, cus, nullptr));
+    if (st) return st;
+    (void)ah_sample_plan(a, cus, static_cast<uint8_t *>(ctx->scratch));
     AH_HIP(ctx, ah_launch_sample(a, pick(ctx, stream)));
     return AH_OK;
 }

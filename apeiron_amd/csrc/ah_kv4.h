@@ -135,11 +135,19 @@ struct SampleArgs {
     int32_t *tokens;
     float *probs;
     unsigned long long *status;
+    // planned by ah_sample_plan: segments of a row, segments of a workgroup and workgroups of a row, and the scratch
+    uint32_t segs, per, parts;
+    double *bin_mass, *seg_mass;                // [row][bin], [row][segment]
+    uint32_t *bin_count, *group_max, *seg_count; // [row][bin], [row][segment][group], [row][segment]
+    uint16_t *list;                             // [row][segment][kSampleSegList] tokens listed, by place in the segment
 };
+constexpr uint32_t kSampleSegList = 256, kSampleList = 4096, kSampleMaxSegs = 512;
+
 
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream);
 hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream);
 hipError_t ah_launch_kv4_append(const AppendArgs &a, hipStream_t stream);
 hipError_t ah_launch_kv4_read(const KvReadArgs &a, hipStream_t stream);
 hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream);
+size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base);
 hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream);

@@ -7,13 +7,28 @@
 // those the ones with w >= min_p 2^32 (min-p); the first token always.  The draw is the smallest index
 // at which the kept weight up to and with it, in index order, passes floor(u W).
 //
-// No sort: the kept set is a key and, within equal logits, an index; both come from selections by digits
-// of the keys (the f32 bits as an unsigned number of the same order).
+// No sort.  Four launches over segments of 2048 tokens, each reading the row at most once:
+//   scan    the largest key of every group of 64 tokens (a key is the f32 bits as an unsigned number of
+//           the same order), and so M;
+//   count   the tokens and their weight in 1024 bins of (M - l) / T.  With top-k, the k-th largest group
+//           maximum bounds the k-th largest logit from below, and only what reaches it is counted;
+//   gather  from the bins: those kept for certain, those dropped, and the few that a limit falls into,
+//           whose tokens are listed; and each segment's certain weight;
+//   draw    one workgroup a row orders the listed tokens, cuts them, draws a segment and a token in it.
+// A row whose listed tokens pass the lists' room (thousands of equal logits) is cut by selections over
+// the whole row instead.  What bounds it: the row's bytes for many rows (one read from HBM, two more from
+// the cache that holds it), four dependent launches for one.
 #include "ah_kv4.h"
 
 namespace {
 
-constexpr uint32_t kThreads = 1024, kMaxChunks = 256, kChunk = 4096;
+constexpr uint32_t kT = 256;            // threads of every workgroup here
+constexpr uint32_t kSeg = 2048;         // tokens of a segment: eight a thread
+constexpr uint32_t kGroup = 64;         // tokens of a group: eight threads
+constexpr uint32_t kGroups = kSeg / kGroup;
+constexpr uint32_t kBins = 1024;
+constexpr float kBinScale = kBins / 23.0f;  // w is 0 past (M - l) / T = 22.9
+constexpr uint32_t kNone = 0xffffffffu;
 
 AH_DEV uint32_t key_of(float l) {
     l = l != l ? -__builtin_inff() : l + 0.0f;  // NaN is never drawn; -0 and 0 are equal
@@ -22,260 +37,684 @@ AH_DEV uint32_t key_of(float l) {
 }
 AH_DEV float logit_of(uint32_t k) { return __builtin_bit_cast(float, (int32_t)k < 0 ? k & 0x7fffffffu : ~k); }
 
-// The weight of key k: a whole number of 2^-32, as f32 (exact: exp's 24 bits, rounded below 1).
-AH_DEV float weight_of(uint32_t k, uint32_t top, float M, float inv_t) {
+// A row's parameters and what follows from its largest key.
+struct Row {
+    const float *x;
+    float T, p, m, u;
+    int32_t k;
+    uint32_t V, top;
+    float M, inv_t;
+    double floor_w;
+    bool bad_t, greedy, need_k, need_p;
+};
+AH_DEV Row row_of(const SampleArgs &a, uint32_t row) {
+    Row r;
+    r.x = a.logits + (size_t)row * a.stride;
+    r.V = a.n_vocab;
+    r.T = a.temperature ? a.temperature[row] : 1.0f;
+    r.k = a.top_k ? a.top_k[row] : 0;
+    r.p = a.top_p ? a.top_p[row] : 1.0f;
+    r.m = a.min_p ? a.min_p[row] : 0.0f;
+    r.u = a.u[row];
+    r.bad_t = !(r.T >= 0.0f && r.T < __builtin_inff());
+    r.greedy = r.bad_t || r.T == 0.0f || r.k == 1;
+    r.need_k = r.k > 1 && (uint32_t)r.k < r.V;
+    r.need_p = r.p < 1.0f;
+    r.floor_w = (double)(r.m > 0.0f ? (r.m < 1.0f ? r.m : 1.0f) : 0.0f) * 0x1p32;
+    return r;
+}
+AH_DEV void set_top(Row &r, uint32_t top) {
+    r.top = top;
+    r.M = logit_of(top);
+    r.inv_t = 1.0f / r.T;
+}
+AH_DEV float z_of(const Row &r, uint32_t k) {
 #pragma clang fp contract(off)
-    if (k == top) return 0x1p32f;
-    const float z = (logit_of(k) - M) * inv_t;
+    return k == r.top ? 0.0f : (logit_of(k) - r.M) * r.inv_t;
+}
+// The weight: a whole number, as f32 (exact: exp's 24 bits, rounded below 1).
+AH_DEV float weight_at(float z) {
+#pragma clang fp contract(off)
     return __builtin_rintf(expf(z) * 0x1p32f);
 }
+// The bin of a key, kBins where the weight is 0 (monotone in the key, as z is).
+AH_DEV uint32_t bin_at(float z) {
+    const float t = z * -kBinScale;
+    return t < (float)kBins ? (uint32_t)t : kBins;
+}
 
-struct Shared {
-    double mass[256];
-    uint32_t count[256];
-    double chunk[kMaxChunks];
-    double wave_d[16];
-    uint32_t wave_u[16];
-    double d0;
-    uint32_t u0, u1;
+// ---- workgroup scans (kT threads) -------------------------------------------------------------------
+
+struct Scan {
+    double d[kT / 64];
+    uint32_t u[kT / 64];
 };
-
-AH_DEV double block_sum(double v, Shared &S) {
+// Inclusive prefix of v over the workgroup's threads, and the total.
+AH_DEV double scan_d(double v, Scan &S, double &total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double t = __shfl_up(v, o, 64);
+        if ((int)lane >= o) v += t;
+    }
+    __syncthreads();
+    if (lane == 63) S.d[wave] = v;
+    __syncthreads();
+    total = 0.0;
+#pragma unroll
+    for (uint32_t w = 0; w < kT / 64; ++w) {
+        if (w < wave) v += S.d[w];
+        total += S.d[w];
+    }
+    return v;
+}
+AH_DEV uint32_t scan_u(uint32_t v, Scan &S, uint32_t &total) {
+    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = (uint32_t)__shfl_up((int)v, o, 64);
+        if ((int)lane >= o) v += t;
+    }
+    __syncthreads();
+    if (lane == 63) S.u[wave] = v;
+    __syncthreads();
+    total = 0;
+#pragma unroll
+    for (uint32_t w = 0; w < kT / 64; ++w) {
+        if (w < wave) v += S.u[w];
+        total += S.u[w];
+    }
+    return v;
+}
+AH_DEV double sum_d(double v, Scan &S) {
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) S.wave_d[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) S.d[threadIdx.x >> 6] = v;
     __syncthreads();
-    double t = 0.0;
-    for (uint32_t w = 0; w < kThreads / 64; ++w) t += S.wave_d[w];
-    return t;
+    return (S.d[0] + S.d[1]) + (S.d[2] + S.d[3]);
 }
-AH_DEV uint32_t block_min(uint32_t v, Shared &S) {
+AH_DEV uint32_t max_u(uint32_t v, Scan &S) {
 #pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = __builtin_elementwise_min(v, (uint32_t)__shfl_xor((int)v, o, 64));
+    for (int o = 1; o < 64; o <<= 1) v = __builtin_elementwise_max(v, (uint32_t)__shfl_xor((int)v, o, 64));
     __syncthreads();
-    if ((threadIdx.x & 63) == 0) S.wave_u[threadIdx.x >> 6] = v;
+    if ((threadIdx.x & 63) == 0) S.u[threadIdx.x >> 6] = v;
     __syncthreads();
-    uint32_t t = 0xffffffffu;
-    for (uint32_t w = 0; w < kThreads / 64; ++w) t = __builtin_elementwise_min(t, S.wave_u[w]);
-    return t;
+    return __builtin_elementwise_max(__builtin_elementwise_max(S.u[0], S.u[1]), __builtin_elementwise_max(S.u[2], S.u[3]));
+}
+AH_DEV uint32_t min_u(uint32_t v, Scan &S) { return ~max_u(~v, S); }
+
+// The keys of a thread's eight tokens of a segment; 0 (below every key) past the row's end.
+AH_DEV void load_keys(const Row &r, uint32_t seg, uint32_t *k) {
+    const uint32_t i0 = seg * kSeg + 8 * threadIdx.x;
+    float x[8];
+    if (i0 + 8 <= r.V) __builtin_memcpy(x, r.x + i0, 32);
+    else
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) x[i] = i0 + i < r.V ? r.x[i0 + i] : 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) k[i] = i0 + i < r.V ? key_of(x[i]) : 0u;
 }
 
-// One workgroup per row.
-__global__ void __launch_bounds__(kThreads) sample_row_kernel(SampleArgs a) {
-    __shared__ Shared S;
-    const uint32_t row = blockIdx.x, tid = threadIdx.x, V = a.n_vocab;
-    const float *x = a.logits + (size_t)row * a.stride;
-    float T = a.temperature ? a.temperature[row] : 1.0f;
-    const int32_t k_in = a.top_k ? a.top_k[row] : 0;
-    const float p_in = a.top_p ? a.top_p[row] : 1.0f, m_in = a.min_p ? a.min_p[row] : 0.0f, u_in = a.u[row];
-    const unsigned long long key0 = (unsigned long long)row << 8;
-    const bool bad_t = !(T >= 0.0f && T < __builtin_inff());
-    if (tid == 0 && bad_t) ah_record(a.status, key0 + AH_ERR_INPUT_RANGE);
-
+AH_DEV uint32_t top_of(const SampleArgs &a, uint32_t row, Scan &S) {
+    const uint32_t *g = a.group_max + (size_t)row * a.segs * kGroups;
     uint32_t top = 0;
-    bool nan = false;
-    for (uint32_t i = tid; i < V; i += kThreads) {
-        nan |= x[i] != x[i];
-        top = __builtin_elementwise_max(top, key_of(x[i]));
+    for (uint32_t i = threadIdx.x; i < a.segs * kGroups; i += kT) top = __builtin_elementwise_max(top, g[i]);
+    return max_u(top, S);
+}
+
+// The workgroup's row and segments.
+AH_DEV void share(const SampleArgs &a, uint32_t &row, uint32_t &s0, uint32_t &s1) {
+    row = blockIdx.x / a.parts;
+    s0 = (blockIdx.x - row * a.parts) * a.per;
+    s1 = s0 + a.per < a.segs ? s0 + a.per : a.segs;
+}
+
+__global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
+    uint32_t row, s0, s1;
+    share(a, row, s0, s1);
+    Row r;
+    r.x = a.logits + (size_t)row * a.stride;
+    r.V = a.n_vocab;
+    if (s0 == 0) {  // the row's bins, for the next launch
+        for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
+            a.bin_mass[(size_t)row * kBins + i] = 0.0;
+            a.bin_count[(size_t)row * kBins + i] = 0;
+        }
     }
-    if (nan) ah_record(a.status, key0 + AH_ERR_NONFINITE_INPUT);
-    top = ~block_min(~top, S);
-    const float M = logit_of(top);
-    if (M == -__builtin_inff()) {  // nothing to draw
-        if (tid == 0) {
+    bool nan = false;
+    for (uint32_t s = s0; s < s1; ++s) {
+        const uint32_t i0 = s * kSeg + 8 * threadIdx.x;
+        float x[8];
+        if (i0 + 8 <= r.V) __builtin_memcpy(x, r.x + i0, 32);
+        else
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) x[i] = i0 + i < r.V ? r.x[i0 + i] : -__builtin_inff();
+        uint32_t top = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            nan |= x[i] != x[i];
+            top = __builtin_elementwise_max(top, key_of(x[i]));
+        }
+        if (i0 >= r.V) top = 0;
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = __builtin_elementwise_max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        if ((threadIdx.x & 7) == 0) a.group_max[((size_t)row * a.segs + s) * kGroups + threadIdx.x / 8] = top;
+    }
+    if (nan) ah_record(a.status, ((unsigned long long)row << 8) + AH_ERR_NONFINITE_INPUT);
+}
+
+__global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
+    __shared__ double mass[kBins];
+    __shared__ uint32_t count[kBins];
+    __shared__ Scan S;
+    __shared__ uint32_t found;
+    uint32_t row, s0, s1;
+    share(a, row, s0, s1);
+    Row r = row_of(a, row);
+    if (r.greedy || (!r.need_k && !r.need_p)) return;
+    set_top(r, top_of(a, row, S));
+    if (r.M == -__builtin_inff()) return;
+    // the last bin that can hold one of the first k: every group's largest is a token of its own
+    uint32_t last = kBins - 1;
+    if (r.need_k) {
+        for (uint32_t i = threadIdx.x; i < kBins; i += kT) count[i] = 0;
+        if (threadIdx.x == 0) found = kBins - 1;
+        __syncthreads();
+        const uint32_t *g = a.group_max + (size_t)row * a.segs * kGroups;
+        for (uint32_t i = threadIdx.x; i < a.segs * kGroups; i += kT) {
+            const uint32_t k = g[i], b = k ? bin_at(z_of(r, k)) : kBins;
+            if (b < kBins) atomicAdd(&count[b], 1u);
+        }
+        __syncthreads();
+        uint32_t c[4], total;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) c[i] = count[4 * threadIdx.x + i];
+        uint32_t cum = scan_u((c[0] + c[1]) + (c[2] + c[3]), S, total) - ((c[0] + c[1]) + (c[2] + c[3]));
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (cum < (uint32_t)r.k && cum + c[i] >= (uint32_t)r.k) found = 4 * threadIdx.x + i;
+            cum += c[i];
+        }
+        __syncthreads();
+        last = found;
+    }
+    for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
+        count[i] = 0;
+        mass[i] = 0.0;
+    }
+    __syncthreads();
+    for (uint32_t s = s0; s < s1; ++s) {
+        uint32_t k[8];
+        load_keys(r, s, k);
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float z = z_of(r, k[i]);
+            const uint32_t b = k[i] ? bin_at(z) : kBins;
+            if (b > last) continue;
+            if (r.need_k) atomicAdd(&count[b], 1u);
+            if (r.need_p) unsafeAtomicAdd(&mass[b], (double)weight_at(z));
+        }
+    }
+    __syncthreads();
+    for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
+        if (count[i]) atomicAdd(&a.bin_count[(size_t)row * kBins + i], count[i]);
+        if (mass[i] > 0.0) unsafeAtomicAdd(&a.bin_mass[(size_t)row * kBins + i], mass[i]);
+    }
+}
+
+// What the bins say.  Tokens of bins below g0 are kept and those of bins past g1 dropped (min-p apart); the
+// k-th token is in bin bk (kNone: fewer than k tokens have weight), `before_k` tokens weighing `mass_k` ahead of
+// that bin; `mass_0` is the weight ahead of bin g0 and `all` that of every bin.
+struct Limits {
+    uint32_t g0, g1, bk, before_k;
+    double mass_k, mass_0, all;
+};
+struct LimitsLds {
+    uint32_t bk, before_k, g0, g1;
+    double mass_k, mass_0, w_low, w_high;
+};
+AH_DEV Limits limits_of(const SampleArgs &a, const Row &r, uint32_t row, Scan &S, LimitsLds &L) {
+    Limits o = {kBins, kBins, kNone, 0, 0.0, 0.0, 0.0};
+    if (!r.need_k && !r.need_p) return o;
+    const uint32_t t = threadIdx.x;
+    uint32_t c[4];
+    double m[4];
+    __builtin_memcpy(c, a.bin_count + (size_t)row * kBins + 4 * t, 16);
+    __builtin_memcpy(m, a.bin_mass + (size_t)row * kBins + 4 * t, 32);
+    if (t == 0) {
+        L.bk = kNone;
+        L.g0 = L.g1 = kBins - 1;
+    }
+    uint32_t total;
+    const uint32_t csum = (c[0] + c[1]) + (c[2] + c[3]);
+    const double msum = (m[0] + m[1]) + (m[2] + m[3]);
+    uint32_t cum = scan_u(csum, S, total) - csum;
+    double all;
+    const double m0 = scan_d(msum, S, all) - msum;
+    double cm = m0;
+    if (r.need_k) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            if (cum < (uint32_t)r.k && cum + c[i] >= (uint32_t)r.k) {
+                L.bk = 4 * t + i;
+                L.before_k = cum;
+                L.mass_k = cm;
+                L.w_high = cm + m[i];
+            }
+            cum += c[i];
+            cm += m[i];
+        }
+        __syncthreads();
+        o.bk = L.bk;
+    }
+    if (o.bk != kNone) {
+        o.before_k = L.before_k;
+        o.mass_k = L.mass_k;
+    }
+    if (!r.need_p) {
+        o.g0 = o.g1 = o.bk != kNone ? o.bk : kBins;
+        return o;
+    }
+    // the weight of the first k is between these, and so is the limit between p times them
+    const double p = (double)(r.p > 0.0f ? r.p : 0.0f);
+    const double low = p * (o.bk != kNone ? o.mass_k : all), high = p * (o.bk != kNone ? L.w_high : all);
+    cm = m0;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        const double next = cm + m[i];
+        const uint32_t b = 4 * t + i;
+        if (next >= low && (b == 0 || cm < low)) {
+            L.g0 = b;
+            L.mass_0 = cm;
+        }
+        if (next >= high && (b == 0 || cm < high)) L.g1 = b;
+        cm = next;
+    }
+    __syncthreads();
+    o.g0 = L.g0;
+    o.g1 = o.bk < L.g1 ? o.bk : L.g1;
+    o.mass_0 = L.mass_0;
+    o.all = all;
+    return o;
+}
+AH_DEV bool listed(const Limits &o, const Row &r, uint32_t b) {
+    return (b >= o.g0 && b <= o.g1 && b < kBins) || (r.need_p && b == o.bk);
+}
+
+__global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
+    __shared__ Scan S;
+    __shared__ LimitsLds L;
+    uint32_t row, s0, s1;
+    share(a, row, s0, s1);
+    Row r = row_of(a, row);
+    if (r.greedy) return;
+    set_top(r, top_of(a, row, S));
+    if (r.M == -__builtin_inff()) return;
+    const Limits o = limits_of(a, r, row, S, L);
+    for (uint32_t s = s0; s < s1; ++s) {
+        uint32_t k[8], n = 0;
+        load_keys(r, s, k);
+        double sure = 0.0;
+        uint32_t mask = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            const float z = z_of(r, k[i]);
+            const uint32_t b = k[i] ? bin_at(z) : kBins;
+            if (b < o.g0 && b < kBins) {
+                const double w = (double)weight_at(z);
+                sure += w < r.floor_w ? 0.0 : w;
+            } else if (listed(o, r, b)) {
+                mask |= 1u << i;
+                ++n;
+            }
+        }
+        sure = sum_d(sure, S);
+        uint32_t total;
+        uint32_t at = scan_u(n, S, total) - n;
+        const size_t seg = (size_t)row * a.segs + s;
+        if (total <= kSampleSegList) {
+            uint16_t *list = a.list + seg * kSampleSegList;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i)
+                if (mask >> i & 1u) list[at++] = (uint16_t)(8 * threadIdx.x + i);
+        }
+        if (threadIdx.x == 0) {
+            a.seg_mass[seg] = sure;
+            a.seg_count[seg] = total;
+        }
+    }
+}
+
+// ---- the cut ----------------------------------------------------------------------------------------
+
+struct DrawLds {
+    Scan S;
+    LimitsLds L;
+    double mass[256];
+    uint32_t count[256];
+    double seg[kSampleMaxSegs];
+    uint32_t start[kSampleMaxSegs + 1];
+    uint32_t key[kSampleList], idx[kSampleList];
+    uint32_t u0, u1;
+    double d0;
+};
+
+// The kept set's last token in the order: keys above `key` are kept, and of those equal to it the ones up
+// to index `last`.
+struct Cut {
+    uint32_t key, last;
+};
+
+// The index of the nth (1 ..) of n tokens in index order that have key `cut`.
+template <class Key, class Index> AH_DEV uint32_t nth_equal(uint32_t n, Key key, Index index, uint32_t cut, uint32_t nth, DrawLds &D) {
+    uint32_t seen = 0;
+    for (uint32_t base = 0; base < n && seen < nth; base += kT) {
+        const uint32_t i = base + threadIdx.x;
+        const bool eq = i < n && key(i) == cut;
+        uint32_t total;
+        const uint32_t at = seen + scan_u(eq, D.S, total);
+        if (eq && at == nth) D.u0 = index(i);
+        seen += total;
+    }
+    __syncthreads();
+    return D.u0;
+}
+
+// The cut over n tokens in index order (a list, or the whole row), by digits of the keys.  in_k(key) and
+// in_p(key): whether such a token counts for the top-k and for the top-p limit.  need: tokens that top-k still
+// keeps of its own; W0: the weight ahead of those (without top-k: of every token); before: the weight ahead of
+// top-p's.
+template <class Key, class Index, class InK, class InP>
+AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, InP in_p, bool do_k, uint32_t need, double W0, double before,
+                      DrawLds &D) {
+    const uint32_t t = threadIdx.x;
+    Cut c = {0, kNone};
+    uint32_t keep = 0, cut_k = 0;  // of those at the cut
+    bool partial = false;
+    if (do_k) {
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            D.count[t] = 0;
+            __syncthreads();
+            for (uint32_t i = t; i < n; i += kT) {
+                const uint32_t k = key(i);
+                if (in_k(k) && (shift == 24 || (k >> (shift + 8)) == (cut_k >> (shift + 8)))) atomicAdd(&D.count[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            const uint32_t mine = D.count[255 - t];
+            uint32_t total;
+            const uint32_t cum = scan_u(mine, D.S, total);
+            if (cum >= need && cum - mine < need) {
+                D.u0 = 255 - t;
+                D.u1 = cum - mine;
+            }
+            __syncthreads();
+            cut_k |= D.u0 << shift;
+            need -= D.u1;
+        }
+        keep = need;
+        partial = D.count[D.u0] > need;
+        c.key = cut_k;
+    }
+    if (r.need_p) {
+        const double w_cut = do_k ? (double)weight_at(z_of(r, cut_k)) : 0.0;
+        double W = W0;
+        if (do_k) {
+            double s = 0.0;
+            for (uint32_t i = t; i < n; i += kT) {
+                const uint32_t k = key(i);
+                if (in_k(k) && k > cut_k) s += (double)weight_at(z_of(r, k));
+            }
+            W += sum_d(s, D.S) + (double)keep * w_cut;
+        }
+        double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
+        goal = goal < 1.0 ? 1.0 : goal;  // the first token always
+        uint32_t cut_p = 0, all = 0;
+        for (int shift = 24; shift >= 0; shift -= 8) {
+            __syncthreads();
+            D.mass[t] = 0.0;
+            D.count[t] = 0;
+            __syncthreads();
+            for (uint32_t i = t; i < n; i += kT) {
+                const uint32_t k = key(i);
+                if (!in_p(k) || (do_k && k <= cut_k) || !(shift == 24 || (k >> (shift + 8)) == (cut_p >> (shift + 8)))) continue;
+                unsafeAtomicAdd(&D.mass[(k >> shift) & 255u], (double)weight_at(z_of(r, k)));
+                atomicAdd(&D.count[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            double mine = D.mass[255 - t];
+            uint32_t cnt = D.count[255 - t];
+            if (do_k && in_p(cut_k) && (shift == 24 || (cut_k >> (shift + 8)) == (cut_p >> (shift + 8))) && 255 - t == ((cut_k >> shift) & 255u)) {
+                mine += (double)keep * w_cut;
+                cnt += keep;
+            }
+            double total;
+            const double cum = before + scan_d(mine, D.S, total);
+            if (cum >= goal && cum - mine < goal) {
+                D.u0 = 255 - t;
+                D.u1 = cnt;
+                D.d0 = cum - mine;
+            }
+            __syncthreads();
+            cut_p |= D.u0 << shift;
+            all = D.u1;
+            before = D.d0;
+        }
+        const double w = (double)weight_at(z_of(r, cut_p)), q = (goal - before) / w;
+        uint32_t m = q >= (double)all ? all : q <= 1.0 ? 1u : (uint32_t)q;
+        while (m < all && before + (double)m * w < goal) ++m;
+        while (m > 1 && before + (double)(m - 1) * w >= goal) --m;
+        partial = m < all || (do_k && cut_p == cut_k && partial);
+        keep = m;
+        c.key = cut_p;
+    }
+    if (partial) c.last = nth_equal(n, key, index, c.key, keep, D);
+    return c;
+}
+
+__global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
+    __shared__ DrawLds D;
+    const uint32_t row = blockIdx.x, t = threadIdx.x;
+    Row r = row_of(a, row);
+    const unsigned long long key0 = (unsigned long long)row << 8;
+    if (t == 0 && r.bad_t) ah_record(a.status, key0 + AH_ERR_INPUT_RANGE);
+    set_top(r, top_of(a, row, D.S));
+    if (r.M == -__builtin_inff()) {  // nothing to draw
+        if (t == 0) {
             ah_record(a.status, key0 + AH_ERR_NONFINITE_INPUT);
             a.tokens[row] = -1;
             if (a.probs) a.probs[row] = 0.0f;
         }
         return;
     }
-    if (bad_t || T == 0.0f || k_in == 1) {
-        uint32_t at = 0xffffffffu;
-        for (uint32_t i = tid; i < V; i += kThreads)
-            if (key_of(x[i]) == top) at = __builtin_elementwise_min(at, i);
-        at = block_min(at, S);
-        if (tid == 0) {
-            a.tokens[row] = (int32_t)at;
+    if (r.greedy) {  // the first group that holds the largest, and in it the first token
+        const uint32_t *g = a.group_max + (size_t)row * a.segs * kGroups;
+        uint32_t at = kNone;
+        for (uint32_t i = t; i < a.segs * kGroups; i += kT)
+            if (g[i] == r.top) at = __builtin_elementwise_min(at, i);
+        at = min_u(at, D.S);
+        const uint32_t i = at * kGroup + t;
+        const bool here = t < kGroup && i < r.V && key_of(r.x[i]) == r.top;
+        const uint64_t b = __builtin_amdgcn_ballot_w64(here);
+        if (t == 0) {
+            a.tokens[row] = (int32_t)(at * kGroup + (uint32_t)__builtin_ctzll(b));
             if (a.probs) a.probs[row] = 1.0f;
         }
         return;
     }
-    const float inv_t = 1.0f / T;
-
-    // the cut: keys above `cut`, and of those equal to it the first `equal`, `have` being all of them
-    uint32_t cut = 0, equal = 0xffffffffu;
-    bool partial = false;  // not every token of the cut's logit is kept
-    if (k_in > 1 && (uint32_t)k_in < V) {
-        uint32_t need = (uint32_t)k_in, prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) S.count[tid] = 0;
-            __syncthreads();
-            for (uint32_t i = tid; i < V; i += kThreads) {
-                const uint32_t k = key_of(x[i]);
-                if (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8))) atomicAdd(&S.count[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            if (tid == 0) {
-                uint32_t n = 0;
-                int b = 255;
-                for (; b > 0; --b) {
-                    if (n + S.count[b] >= need) break;
-                    n += S.count[b];
-                }
-                S.u0 = (uint32_t)b;
-                S.u1 = n;
-            }
-            __syncthreads();
-            prefix |= S.u0 << shift;
-            need -= S.u1;
+    const Limits o = limits_of(a, r, row, D.S, D.L);
+    const bool do_k = o.bk != kNone, limited = do_k || r.need_p;
+    // the segments' certain weights, and where their listed tokens start
+    bool full = false;
+    uint32_t n = 0;
+    for (uint32_t base = 0; base < a.segs; base += kT) {
+        const uint32_t s = base + t;
+        uint32_t c = 0;
+        if (s < a.segs) {
+            D.seg[s] = a.seg_mass[(size_t)row * a.segs + s];
+            c = a.seg_count[(size_t)row * a.segs + s];
         }
-        cut = prefix;
-        equal = need;
-        partial = S.count[S.u0] > need;
+        full |= c > kSampleSegList;
+        uint32_t total;
+        const uint32_t end = n + scan_u(c, D.S, total);
+        if (s < a.segs) D.start[s + 1] = end;
+        n += total;
     }
-    // the weight of the kept, and the cut by mass
-    if (p_in < 1.0f) {
-        const float w_cut = equal == 0xffffffffu ? 0.0f : weight_of(cut, top, M, inv_t);
-        double W = 0.0;
-        for (uint32_t i = tid; i < V; i += kThreads) {
-            const uint32_t k = key_of(x[i]);
-            if (equal == 0xffffffffu || k > cut) W += (double)weight_of(k, top, M, inv_t);
-        }
-        W = block_sum(W, S) + (equal == 0xffffffffu ? 0.0 : (double)equal * (double)w_cut);
-        const double goal = (double)(p_in > 0.0f ? p_in : 0.0f) * W;
-        double before = 0.0;
-        uint32_t prefix = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
-            __syncthreads();
-            if (tid < 256) {
-                S.mass[tid] = 0.0;
-                S.count[tid] = 0;
-            }
-            __syncthreads();
-            for (uint32_t i = tid; i < V; i += kThreads) {
-                const uint32_t k = key_of(x[i]);
-                if ((equal == 0xffffffffu || k > cut) && (shift == 24 || (k >> (shift + 8)) == (prefix >> (shift + 8)))) {
-                    atomicAdd(&S.mass[(k >> shift) & 255u], (double)weight_of(k, top, M, inv_t));
-                    atomicAdd(&S.count[(k >> shift) & 255u], 1u);
-                }
-            }
-            __syncthreads();
-            if (tid == 0) {
-                if (equal != 0xffffffffu && (shift == 24 || (cut >> (shift + 8)) == (prefix >> (shift + 8)))) {
-                    S.mass[(cut >> shift) & 255u] += (double)equal * (double)w_cut;
-                    S.count[(cut >> shift) & 255u] += equal;
-                }
-                double n = before;
-                int b = 255, at = -1;
-                for (; b >= 0; --b) {
-                    if (!S.count[b]) continue;
-                    at = b;  // the last digit in use, if no mass reaches the goal
-                    if (n + S.mass[b] >= goal) break;
-                    n += S.mass[b];
-                }
-                S.u0 = (uint32_t)at;
-                S.u1 = b >= 0 ? 1u : 0u;
-                S.d0 = b >= 0 ? n : n - S.mass[at];
-            }
-            __syncthreads();
-            prefix |= S.u0 << shift;
-            before = S.d0;
-        }
-        const uint32_t all = S.count[S.u0];
-        const double w = (double)weight_of(prefix, top, M, inv_t);
-        uint32_t n = all;
-        if (w > 0.0) {
-            double q = (goal - before) / w;
-            n = q >= (double)all ? all : q <= 1.0 ? 1u : (uint32_t)q;
-            while (n < all && before + (double)n * w < goal) ++n;
-            while (n > 1 && before + (double)(n - 1) * w >= goal) --n;
-        }
-        partial = n < all || (equal != 0xffffffffu && prefix == cut && partial);
-        cut = prefix;
-        equal = n;
-    }
-    // the index of the last token kept of the cut's logit
-    uint32_t last = 0xffffffffu;
-    if (partial) {
-        uint32_t seen = 0;
-        for (uint32_t base = 0; base < V; base += kThreads) {
-            const uint32_t i = base + tid;
-            const bool eq = i < V && key_of(x[i]) == cut;
-            const uint64_t b = __builtin_amdgcn_ballot_w64(eq);
-            __syncthreads();
-            if ((tid & 63) == 0) S.wave_u[tid >> 6] = (uint32_t)__builtin_popcountll(b);
-            __syncthreads();
-            uint32_t mine = seen, total = 0;
-            for (uint32_t w = 0; w < kThreads / 64; ++w) {
-                if (w < (tid >> 6)) mine += S.wave_u[w];
-                total += S.wave_u[w];
-            }
-            mine += (uint32_t)__builtin_popcountll(b & ((1ull << (tid & 63)) - 1));
-            if (eq && mine + 1 == equal) S.u0 = i;
-            seen += total;
-            if (seen >= equal) break;
-        }
-        __syncthreads();
-        last = S.u0;
-        __syncthreads();
-    }
-    const double floor_w = (double)(m_in > 0.0f ? (m_in < 1.0f ? m_in : 1.0f) : 0.0f) * 0x1p32;
-    auto kept = [&](uint32_t i) -> double {
-        const uint32_t k = key_of(x[i]);
-        if (k < cut || (k == cut && i > last)) return 0.0;
-        const float w = weight_of(k, top, M, inv_t);
-        return (double)w < floor_w ? 0.0 : (double)w;
+    if (t == 0) D.start[0] = 0;
+    full = max_u(full, D.S) != 0 || n > kSampleList;
+    Cut c = {0, kNone};
+    auto kept = [&](uint32_t i, uint32_t k) -> double {
+        if (limited && (k < c.key || (k == c.key && i > c.last))) return 0.0;
+        const float z = z_of(r, k);
+        if (!k || bin_at(z) == kBins) return 0.0;
+        const double w = (double)weight_at(z);
+        return w < r.floor_w ? 0.0 : w;
     };
-    const uint32_t chunks = (V + kChunk - 1) / kChunk;
-    double W = 0.0;
-    for (uint32_t c = 0; c < chunks; ++c) {
-        double s = 0.0;
-        for (uint32_t j = 0; j < kChunk / kThreads; ++j) {
-            const uint32_t i = c * kChunk + j * kThreads + tid;
-            if (i < V) s += kept(i);
+    if (full) {
+        const auto key = [&](uint32_t i) { return key_of(r.x[i]); };
+        const auto index = [](uint32_t i) { return i; };
+        const auto weighs = [&](uint32_t k) { return bin_at(z_of(r, k)) < kBins; };
+        c = select_cut(r, r.V, key, index, weighs, weighs, do_k, (uint32_t)r.k, do_k ? 0.0 : o.all, 0.0, D);
+        for (uint32_t s = 0; s < a.segs; ++s) {
+            uint32_t k[8];
+            load_keys(r, s, k);
+            double w = 0.0;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) w += kept(s * kSeg + 8 * t + i, k[i]);
+            w = sum_d(w, D.S);
+            if (t == 0) D.seg[s] = w;
         }
-        s = block_sum(s, S);
-        if (tid == 0) S.chunk[c] = s;
-        W += s;
+    } else if (n) {
+        // a wave per segment copies its list: the tokens stay in index order
+        for (uint32_t s = t >> 6; s < a.segs; s += kT / 64) {
+            const uint32_t b = D.start[s], m = D.start[s + 1] - b;
+            for (uint32_t j = t & 63; j < m; j += 64) {
+                const uint32_t i = s * kSeg + a.list[((size_t)row * a.segs + s) * kSampleSegList + j];
+                D.idx[b + j] = i;
+                D.key[b + j] = key_of(r.x[i]);
+            }
+        }
+        __syncthreads();
+        const auto bin = [&](uint32_t k) { return bin_at(z_of(r, k)); };
+        if (n <= kT) {
+            // a token a thread, its place among the others by comparing with each
+            const bool live = t < n;
+            const uint32_t k = live ? D.key[t] : 0u, b = live ? bin(k) : kBins;
+            const bool ink = live && do_k && b == o.bk, inp = live && b >= o.g0 && b <= o.g1;
+            const double w = live ? (double)weight_at(z_of(r, k)) : 0.0;
+            bool keep = live;
+            double goal = 0.0;
+            if (do_k) {
+                uint32_t rank = 0;
+                for (uint32_t j = 0; j < n; ++j) {
+                    const uint32_t kj = D.key[j];
+                    if ((kj > k || (kj == k && j < t)) && bin(kj) == o.bk) ++rank;
+                }
+                keep = ink ? o.before_k + rank < (uint32_t)r.k : live;
+            }
+            if (r.need_p) {
+                const double W = do_k ? o.mass_k + sum_d(ink && keep ? w : 0.0, D.S) : o.all;
+                goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
+                goal = goal < 1.0 ? 1.0 : goal;
+                D.mass[t] = inp && keep ? w : 0.0;
+                __syncthreads();
+                double before = o.mass_0;
+                for (uint32_t j = 0; j < n; ++j) {
+                    const uint32_t kj = D.key[j];
+                    if (kj > k || (kj == k && j < t)) before += D.mass[j];
+                }
+                keep = inp && keep && before < goal;
+            } else {
+                keep = ink && keep;
+            }
+            c.key = min_u(keep ? k : kNone, D.S);
+            c.last = max_u(keep && k == c.key ? D.idx[t] : 0u, D.S);
+        } else {
+            const auto key = [&](uint32_t i) { return D.key[i]; };
+            const auto index = [&](uint32_t i) { return D.idx[i]; };
+            const auto in_k = [&](uint32_t k) { return bin(k) == o.bk; };
+            const auto in_p = [&](uint32_t k) { return bin(k) >= o.g0 && bin(k) <= o.g1; };
+            c = select_cut(r, n, key, index, in_k, in_p, do_k, (uint32_t)r.k - o.before_k, do_k ? o.mass_k : o.all, o.mass_0, D);
+        }
+        for (uint32_t j = t; j < n; j += kT) {
+            const double w = kept(D.idx[j], D.key[j]);
+            if (w > 0.0) unsafeAtomicAdd(&D.seg[D.idx[j] / kSeg], w);
+        }
     }
     __syncthreads();
-    double goal = __builtin_floor((double)(u_in > 0.0f ? u_in : 0.0f) * W);
+    // the segment, then the token in it
+    double W = 0.0;
+    for (uint32_t base = 0; base < a.segs; base += kT) {
+        double total;
+        scan_d(base + t < a.segs ? D.seg[base + t] : 0.0, D.S, total);
+        W += total;
+    }
+    double goal = __builtin_floor((double)(r.u > 0.0f ? r.u : 0.0f) * W);
     goal = goal < W ? goal : W - 1.0;
-    uint32_t c = 0;
     double before = 0.0;
-    while (c + 1 < chunks && before + S.chunk[c] <= goal) before += S.chunk[c++];
-    // inside the chunk: 1024 tokens at a time, a prefix sum over them
-    for (uint32_t j = 0; j < kChunk / kThreads; ++j) {
-        const uint32_t i = c * kChunk + j * kThreads + tid;
-        const double w = i < V ? kept(i) : 0.0;
-        double pre = w;
+    for (uint32_t base = 0; base < a.segs; base += kT) {
+        const double mine = base + t < a.segs ? D.seg[base + t] : 0.0;
+        double total;
+        const double cum = before + scan_d(mine, D.S, total);
+        if (cum > goal && cum - mine <= goal) {
+            D.u0 = base + t;
+            D.d0 = cum - mine;
+        }
+        before += total;
+    }
+    __syncthreads();
+    const uint32_t s = D.u0;
+    before = D.d0;
+    uint32_t k[8];
+    double w[8], mine = 0.0, total;
+    load_keys(r, s, k);
 #pragma unroll
-        for (int o = 1; o < 64; o <<= 1) {
-            const double t = __shfl_up(pre, o, 64);
-            if ((int)(tid & 63) >= o) pre += t;
+    for (uint32_t i = 0; i < 8; ++i) {
+        w[i] = kept(s * kSeg + 8 * t + i, k[i]);
+        mine += w[i];
+    }
+    double cum = before + scan_d(mine, D.S, total) - mine;
+#pragma unroll
+    for (uint32_t i = 0; i < 8; ++i) {
+        if (cum <= goal && cum + w[i] > goal) {
+            a.tokens[row] = (int32_t)(s * kSeg + 8 * t + i);
+            if (a.probs) a.probs[row] = (float)(w[i] / W);
         }
-        __syncthreads();
-        if ((tid & 63) == 63) S.wave_d[tid >> 6] = pre;
-        __syncthreads();
-        double off = before, all = 0.0;
-        for (uint32_t v = 0; v < kThreads / 64; ++v) {
-            if (v < (tid >> 6)) off += S.wave_d[v];
-            all += S.wave_d[v];
-        }
-        if (w > 0.0 && off + pre > goal && off + pre - w <= goal) {
-            a.tokens[row] = (int32_t)i;
-            if (a.probs) a.probs[row] = (float)(w / W);
-        }
-        before += all;
-        if (before > goal) break;
+        cum += w[i];
     }
 }
 
 } // namespace
 
 hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(sample_row_kernel, dim3(a.n_rows), dim3(kThreads), 0, stream, a);
+    const dim3 grid(a.n_rows * a.parts), block(kT);
+    hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_count_kernel, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_gather_kernel, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_draw_kernel, dim3(a.n_rows), block, 0, stream, a);
     return hipGetLastError();
+}
+
+// Bytes of scratch, and (with a base) the pointers in it.
+size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
+    a.segs = (a.n_vocab + kSeg - 1) / kSeg;
+    // about eight workgroups a CU, each of whole segments of one row
+    const uint64_t want = 8ull * cus, all = (uint64_t)a.n_rows * a.segs;
+    uint64_t per = (all + want - 1) / want;
+    a.per = (uint32_t)(per < 1 ? 1 : per < a.segs ? per : a.segs);
+    a.parts = (a.segs + a.per - 1) / a.per;
+    size_t at = 0;
+    auto take = [&](size_t bytes) {
+        uint8_t *p = base ? base + at : nullptr;
+        at += (bytes + 255) & ~(size_t)255;
+        return p;
+    };
+    a.bin_mass = reinterpret_cast<double *>(take(8 * (size_t)a.n_rows * kBins));
+    a.seg_mass = reinterpret_cast<double *>(take(8 * (size_t)all));
+    a.bin_count = reinterpret_cast<uint32_t *>(take(4 * (size_t)a.n_rows * kBins));
+    a.group_max = reinterpret_cast<uint32_t *>(take(4 * (size_t)all * kGroups));
+    a.seg_count = reinterpret_cast<uint32_t *>(take(4 * (size_t)all));
+    a.list = reinterpret_cast<uint16_t *>(take(2 * (size_t)all * kSampleSegList));
+    return at;
 }

@@ -462,7 +462,8 @@ typedef struct ah_kv4_attn {
 int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, const float *d_q, size_t q_stride,
                         float *d_out, size_t out_stride, void *stream);
 
-/* One token per row of logits [n_rows][n_vocab] (rows row_stride floats apart; n_vocab <= 2^20).  In the
+/* One token per row of logits [n_rows][n_vocab] (rows row_stride floats apart; n_vocab <= 2^20, n_rows <=
+ * 65536).  Uses the context's scratch (as ah_gemm_f32_dev).  In the
  * order (logit descending, index ascending), with weights w = rint(2^32 exp((logit - largest) / T)): the
  * first top_k tokens are kept (top_k <= 0 or >= n_vocab: all), of those the ones whose preceding weight is
  * below top_p times the weight of all (top_p >= 1: all), of those the ones with w >= min_p 2^32; the first
