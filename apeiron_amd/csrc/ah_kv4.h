@@ -138,10 +138,10 @@ struct SampleArgs {
     // planned by ah_sample_plan: segments of a row, segments of a workgroup and workgroups of a row, and the scratch
     uint32_t segs, per, parts;
     double *bin_mass, *seg_mass;                // [row][bin], [row][segment]
-    uint32_t *bin_count, *group_max, *seg_count; // [row][bin], [row][segment][group], [row][segment]
+    uint32_t *bin_count, *group_max, *seg_max, *seg_count; // [row][bin], [row][segment][group], [row][segment]
     uint16_t *list;                             // [row][segment][kSampleSegList] tokens listed, by place in the segment
 };
-constexpr uint32_t kSampleSegList = 256, kSampleList = 4096, kSampleMaxSegs = 512;
+constexpr uint32_t kSampleSegList = 64, kSampleList = 4096, kSampleMaxSegs = 2048;
 
 
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream);

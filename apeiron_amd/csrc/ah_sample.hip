@@ -7,11 +7,12 @@
 // those the ones with w >= min_p 2^32 (min-p); the first token always.  The draw is the smallest index
 // at which the kept weight up to and with it, in index order, passes floor(u W).
 //
-// No sort.  Four launches over segments of 2048 tokens, each reading the row at most once:
-//   scan    the largest key of every group of 64 tokens (a key is the f32 bits as an unsigned number of
-//           the same order), and so M;
-//   count   the tokens and their weight in 1024 bins of (M - l) / T.  With top-k, the k-th largest group
-//           maximum bounds the k-th largest logit from below, and only what reaches it is counted;
+// No sort.  Four launches over segments of 512 tokens (a wave's eight tokens a lane), each reading the row
+// at most once:
+//   scan    the largest key of every group of 64 tokens and of every segment (a key is the f32 bits as an
+//           unsigned number of the same order), and so M;
+//   count   the tokens and their weight in 1024 bins of (M - l) / T.  With top-k, the k-th largest segment
+//           or group maximum bounds the k-th largest logit from below, and only what reaches it is counted;
 //   gather  from the bins: those kept for certain, those dropped, and the few that a limit falls into,
 //           whose tokens are listed; and each segment's certain weight;
 //   draw    one workgroup a row orders the listed tokens, cuts them, draws a segment and a token in it.
@@ -23,8 +24,8 @@
 namespace {
 
 constexpr uint32_t kT = 256;            // threads of every workgroup here
-constexpr uint32_t kSeg = 2048;         // tokens of a segment: eight a thread
-constexpr uint32_t kGroup = 64;         // tokens of a group: eight threads
+constexpr uint32_t kSeg = 512;          // tokens of a segment: eight a lane of one wave
+constexpr uint32_t kGroup = 64;         // tokens of a group: eight lanes
 constexpr uint32_t kGroups = kSeg / kGroup;
 constexpr uint32_t kBins = 1024;
 constexpr float kBinScale = kBins / 23.0f;  // w is 0 past (M - l) / T = 22.9
@@ -144,30 +145,55 @@ AH_DEV uint32_t max_u(uint32_t v, Scan &S) {
 }
 AH_DEV uint32_t min_u(uint32_t v, Scan &S) { return ~max_u(~v, S); }
 
-// The keys of a thread's eight tokens of a segment; 0 (below every key) past the row's end.
-AH_DEV void load_keys(const Row &r, uint32_t seg, uint32_t *k) {
-    const uint32_t i0 = seg * kSeg + 8 * threadIdx.x;
-    float x[8];
+AH_DEV uint32_t wave_prefix(uint32_t v) {  // inclusive
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const uint32_t t = (uint32_t)__shfl_up((int)v, o, 64);
+        if ((int)(threadIdx.x & 63) >= o) v += t;
+    }
+    return v;
+}
+AH_DEV double wave_prefix(double v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double t = __shfl_up(v, o, 64);
+        if ((int)(threadIdx.x & 63) >= o) v += t;
+    }
+    return v;
+}
+
+// A lane's eight logits of a segment (-inf past the row's end), and their keys (0, below every key, there).
+AH_DEV void load_logits(const Row &r, uint32_t seg, float *x) {
+    const uint32_t i0 = seg * kSeg + 8 * (threadIdx.x & 63);
     if (i0 + 8 <= r.V) __builtin_memcpy(x, r.x + i0, 32);
     else
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) x[i] = i0 + i < r.V ? r.x[i0 + i] : 0.0f;
+        for (uint32_t i = 0; i < 8; ++i) x[i] = i0 + i < r.V ? r.x[i0 + i] : -__builtin_inff();
+}
+AH_DEV void keys_of(const Row &r, uint32_t seg, const float *x, uint32_t *k) {
+    const uint32_t i0 = seg * kSeg + 8 * (threadIdx.x & 63);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) k[i] = i0 + i < r.V ? key_of(x[i]) : 0u;
 }
+AH_DEV void load_keys(const Row &r, uint32_t seg, uint32_t *k) {
+    float x[8];
+    load_logits(r, seg, x);
+    keys_of(r, seg, x, k);
+}
 
 AH_DEV uint32_t top_of(const SampleArgs &a, uint32_t row, Scan &S) {
-    const uint32_t *g = a.group_max + (size_t)row * a.segs * kGroups;
+    const uint32_t *g = a.seg_max + (size_t)row * a.segs;
     uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < a.segs * kGroups; i += kT) top = __builtin_elementwise_max(top, g[i]);
+    for (uint32_t i = threadIdx.x; i < a.segs; i += kT) top = __builtin_elementwise_max(top, g[i]);
     return max_u(top, S);
 }
 
-// The workgroup's row and segments.
+// The workgroup's row, and the segments of this wave: s0, s0 + 4, .. below s1.
 AH_DEV void share(const SampleArgs &a, uint32_t &row, uint32_t &s0, uint32_t &s1) {
     row = blockIdx.x / a.parts;
-    s0 = (blockIdx.x - row * a.parts) * a.per;
-    s1 = s0 + a.per < a.segs ? s0 + a.per : a.segs;
+    const uint32_t b = (blockIdx.x - row * a.parts) * a.per;
+    s0 = b + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    s1 = b + a.per < a.segs ? b + a.per : a.segs;
 }
 
 __global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
@@ -176,30 +202,31 @@ __global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
     Row r;
     r.x = a.logits + (size_t)row * a.stride;
     r.V = a.n_vocab;
-    if (s0 == 0) {  // the row's bins, for the next launch
+    if (blockIdx.x % a.parts == 0) {  // the row's bins, for the next launch
         for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
             a.bin_mass[(size_t)row * kBins + i] = 0.0;
             a.bin_count[(size_t)row * kBins + i] = 0;
         }
     }
     bool nan = false;
-    for (uint32_t s = s0; s < s1; ++s) {
-        const uint32_t i0 = s * kSeg + 8 * threadIdx.x;
+    for (uint32_t s = s0; s < s1; s += kT / 64) {
         float x[8];
-        if (i0 + 8 <= r.V) __builtin_memcpy(x, r.x + i0, 32);
-        else
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) x[i] = i0 + i < r.V ? r.x[i0 + i] : -__builtin_inff();
-        uint32_t top = 0;
+        uint32_t k[8], top = 0;
+        load_logits(r, s, x);
+        keys_of(r, s, x, k);
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
             nan |= x[i] != x[i];
-            top = __builtin_elementwise_max(top, key_of(x[i]));
+            top = __builtin_elementwise_max(top, k[i]);
         }
-        if (i0 >= r.V) top = 0;
 #pragma unroll
         for (int o = 1; o < 8; o <<= 1) top = __builtin_elementwise_max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        if ((threadIdx.x & 7) == 0) a.group_max[((size_t)row * a.segs + s) * kGroups + threadIdx.x / 8] = top;
+        const uint32_t lane = threadIdx.x & 63;
+        const size_t seg = (size_t)row * a.segs + s;
+        if ((lane & 7) == 0) a.group_max[seg * kGroups + lane / 8] = top;
+#pragma unroll
+        for (int o = 8; o < 64; o <<= 1) top = __builtin_elementwise_max(top, (uint32_t)__shfl_xor((int)top, o, 64));
+        if (lane == 0) a.seg_max[seg] = top;
     }
     if (nan) ah_record(a.status, ((unsigned long long)row << 8) + AH_ERR_NONFINITE_INPUT);
 }
@@ -221,8 +248,11 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
         for (uint32_t i = threadIdx.x; i < kBins; i += kT) count[i] = 0;
         if (threadIdx.x == 0) found = kBins - 1;
         __syncthreads();
-        const uint32_t *g = a.group_max + (size_t)row * a.segs * kGroups;
-        for (uint32_t i = threadIdx.x; i < a.segs * kGroups; i += kT) {
+        // (few tokens asked for: the segments' are bound enough, and an eighth as many to look at)
+        const bool few = (uint64_t)r.k * 2 <= a.segs;
+        const uint32_t *g = few ? a.seg_max + (size_t)row * a.segs : a.group_max + (size_t)row * a.segs * kGroups;
+        const uint32_t n_max = few ? a.segs : a.segs * kGroups;
+        for (uint32_t i = threadIdx.x; i < n_max; i += kT) {
             const uint32_t k = g[i], b = k ? bin_at(z_of(r, k)) : kBins;
             if (b < kBins) atomicAdd(&count[b], 1u);
         }
@@ -244,7 +274,7 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
         mass[i] = 0.0;
     }
     __syncthreads();
-    for (uint32_t s = s0; s < s1; ++s) {
+    for (uint32_t s = s0; s < s1; s += kT / 64) {
         uint32_t k[8];
         load_keys(r, s, k);
 #pragma unroll
@@ -352,7 +382,8 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     set_top(r, top_of(a, row, S));
     if (r.M == -__builtin_inff()) return;
     const Limits o = limits_of(a, r, row, S, L);
-    for (uint32_t s = s0; s < s1; ++s) {
+    const uint32_t lane = threadIdx.x & 63;
+    for (uint32_t s = s0; s < s1; s += kT / 64) {
         uint32_t k[8], n = 0;
         load_keys(r, s, k);
         double sure = 0.0;
@@ -369,17 +400,24 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
                 ++n;
             }
         }
-        sure = sum_d(sure, S);
-        uint32_t total;
-        uint32_t at = scan_u(n, S, total) - n;
         const size_t seg = (size_t)row * a.segs + s;
-        if (total <= kSampleSegList) {
-            uint16_t *list = a.list + seg * kSampleSegList;
+        uint32_t total = 0;
+        if (__builtin_amdgcn_ballot_w64(n != 0) != 0ull) {
+            const uint32_t end = wave_prefix(n);
+            total = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+            uint32_t at = end - n;
+            if (total <= kSampleSegList) {
+                uint16_t *list = a.list + seg * kSampleSegList;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i)
-                if (mask >> i & 1u) list[at++] = (uint16_t)(8 * threadIdx.x + i);
+                for (uint32_t i = 0; i < 8; ++i)
+                    if (mask >> i & 1u) list[at++] = (uint16_t)(8 * lane + i);
+            }
         }
-        if (threadIdx.x == 0) {
+        if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) {
+#pragma unroll
+            for (int q = 1; q < 64; q <<= 1) sure += __shfl_xor(sure, q, 64);
+        }
+        if (lane == 0) {
             a.seg_mass[seg] = sure;
             a.seg_count[seg] = total;
         }
@@ -576,24 +614,27 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         const auto index = [](uint32_t i) { return i; };
         const auto weighs = [&](uint32_t k) { return bin_at(z_of(r, k)) < kBins; };
         c = select_cut(r, r.V, key, index, weighs, weighs, do_k, (uint32_t)r.k, do_k ? 0.0 : o.all, 0.0, D);
-        for (uint32_t s = 0; s < a.segs; ++s) {
+        __syncthreads();
+        for (uint32_t s = t >> 6; s < a.segs; s += kT / 64) {
             uint32_t k[8];
             load_keys(r, s, k);
             double w = 0.0;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) w += kept(s * kSeg + 8 * t + i, k[i]);
-            w = sum_d(w, D.S);
-            if (t == 0) D.seg[s] = w;
+            for (uint32_t i = 0; i < 8; ++i) w += kept(s * kSeg + 8 * (t & 63) + i, k[i]);
+#pragma unroll
+            for (int q = 1; q < 64; q <<= 1) w += __shfl_xor(w, q, 64);
+            if ((t & 63) == 0) D.seg[s] = w;
         }
     } else if (n) {
-        // a wave per segment copies its list: the tokens stay in index order
-        for (uint32_t s = t >> 6; s < a.segs; s += kT / 64) {
-            const uint32_t b = D.start[s], m = D.start[s + 1] - b;
-            for (uint32_t j = t & 63; j < m; j += 64) {
-                const uint32_t i = s * kSeg + a.list[((size_t)row * a.segs + s) * kSampleSegList + j];
-                D.idx[b + j] = i;
-                D.key[b + j] = key_of(r.x[i]);
-            }
+        // listed token j is in the last segment that starts at or before it
+        __syncthreads();
+        for (uint32_t j = t; j < n; j += kT) {
+            uint32_t s = 0;
+            for (uint32_t step = kSampleMaxSegs / 2; step; step >>= 1)
+                if (s + step < a.segs && D.start[s + step] <= j) s += step;
+            const uint32_t i = s * kSeg + a.list[((size_t)row * a.segs + s) * kSampleSegList + (j - D.start[s])];
+            D.idx[j] = i;
+            D.key[j] = key_of(r.x[i]);
         }
         __syncthreads();
         const auto bin = [&](uint32_t k) { return bin_at(z_of(r, k)); };
@@ -602,14 +643,18 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
             const bool live = t < n;
             const uint32_t k = live ? D.key[t] : 0u, b = live ? bin(k) : kBins;
             const bool ink = live && do_k && b == o.bk, inp = live && b >= o.g0 && b <= o.g1;
+
             const double w = live ? (double)weight_at(z_of(r, k)) : 0.0;
             bool keep = live;
             double goal = 0.0;
             if (do_k) {
+                D.count[t] = ink ? k : 0u;
+                __syncthreads();
                 uint32_t rank = 0;
+#pragma unroll 8
                 for (uint32_t j = 0; j < n; ++j) {
-                    const uint32_t kj = D.key[j];
-                    if ((kj > k || (kj == k && j < t)) && bin(kj) == o.bk) ++rank;
+                    const uint32_t kj = D.count[j];
+                    rank += kj > k || (kj == k && j < t) ? 1u : 0u;
                 }
                 keep = ink ? o.before_k + rank < (uint32_t)r.k : live;
             }
@@ -620,9 +665,10 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
                 D.mass[t] = inp && keep ? w : 0.0;
                 __syncthreads();
                 double before = o.mass_0;
+#pragma unroll 8
                 for (uint32_t j = 0; j < n; ++j) {
                     const uint32_t kj = D.key[j];
-                    if (kj > k || (kj == k && j < t)) before += D.mass[j];
+                    before += kj > k || (kj == k && j < t) ? D.mass[j] : 0.0;
                 }
                 keep = inp && keep && before < goal;
             } else {
@@ -664,17 +710,17 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         before += total;
     }
     __syncthreads();
+    if (t >= 64) return;
     const uint32_t s = D.u0;
-    before = D.d0;
     uint32_t k[8];
-    double w[8], mine = 0.0, total;
+    double w[8], mine = 0.0;
     load_keys(r, s, k);
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         w[i] = kept(s * kSeg + 8 * t + i, k[i]);
         mine += w[i];
     }
-    double cum = before + scan_d(mine, D.S, total) - mine;
+    double cum = D.d0 + wave_prefix(mine) - mine;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         if (cum <= goal && cum + w[i] > goal) {
@@ -701,8 +747,8 @@ size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
     a.segs = (a.n_vocab + kSeg - 1) / kSeg;
     // about eight workgroups a CU, each of whole segments of one row
     const uint64_t want = 8ull * cus, all = (uint64_t)a.n_rows * a.segs;
-    uint64_t per = (all + want - 1) / want;
-    a.per = (uint32_t)(per < 1 ? 1 : per < a.segs ? per : a.segs);
+    uint64_t per = ((all + want - 1) / want + 3) / 4 * 4;  // whole rounds of a workgroup's four waves
+    a.per = (uint32_t)(per < 4 ? 4 : per);
     a.parts = (a.segs + a.per - 1) / a.per;
     size_t at = 0;
     auto take = [&](size_t bytes) {
@@ -714,6 +760,7 @@ size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
     a.seg_mass = reinterpret_cast<double *>(take(8 * (size_t)all));
     a.bin_count = reinterpret_cast<uint32_t *>(take(4 * (size_t)a.n_rows * kBins));
     a.group_max = reinterpret_cast<uint32_t *>(take(4 * (size_t)all * kGroups));
+    a.seg_max = reinterpret_cast<uint32_t *>(take(4 * (size_t)all));
     a.seg_count = reinterpret_cast<uint32_t *>(take(4 * (size_t)all));
     a.list = reinterpret_cast<uint16_t *>(take(2 * (size_t)all * kSampleSegList));
     return at;

@@ -577,6 +577,32 @@ def test_sampling_ties_take_the_lowest_indices(dev):
     assert st == OK and tok[0] == 250 and abs(prob[0] - 1 / 251) < 1e-8
 
 
+@pytest.mark.parametrize("V,kind", [(1 << 20, "equal"), (70000, "equal"), (151936, "narrow"), (1 << 20, "normal"), (9000, "narrow"), (40000, "rounded")])
+@pytest.mark.parametrize("k,p", [(0, 0.3), (5000, 1.0), (5000, 0.7), (300, 0.9), (0, 1.0)])
+def test_sampling_of_flat_rows(dev, V, kind, k, p):
+    """Limits that fall among hundreds to all of a row's tokens: long lists, and rows past the lists' room."""
+    rng = np.random.default_rng(V + k)
+    x = {"equal": lambda: np.zeros(V), "narrow": lambda: 1e-3 * rng.standard_normal(V), "normal": lambda: rng.standard_normal(V),
+         "rounded": lambda: np.rint(2 * rng.standard_normal(V)) / 2}[kind]().astype(np.float32)[None]
+    # within a tie the token is certain in the middle of its interval; the limits stand between two tokens (their
+    # weights differ by less than exp's error, but not within a tie)
+    pi = p
+    if p < 1:
+        w, order, _ = kept_weights(x[0], 0.9, k, 1.0, 0.0)
+        n = int((w > 0).sum() * p)
+        c = np.cumsum(w[order]) / w.sum()
+        pi = float(np.float32((c[n] + c[n - 1]) / 2))
+    w, order, _ = kept_weights(x[0], 0.9, k, pi, 0.0)
+    run = np.cumsum(w)
+    for q in (0.1, 0.95):
+        t = int(np.searchsorted(run, q * run[-1]))
+        u = (run[t] - w[t] / 2) / run[-1]
+        st, tok, prob = sample(dev, x, [u], 0.9, k, pi)
+        # f32 p and u, and exp's error over a million equal shares, move the token by a few places at most
+        assert st == OK and w[tok[0]] > 0 and abs(run[tok[0]] - run[t]) <= (2.0 ** -18 * run[-1] + 2 * w.max())
+        assert abs(prob[0] / (w[tok[0]] / run[-1]) - 1) <= 2.0 ** -17 + 4.0 / (w > 0).sum()
+
+
 def test_sampling_defaults_infinities_and_refusals(dev):
     rng = np.random.default_rng(0)
     x = rng.standard_normal((4, 3000)).astype(np.float32)
