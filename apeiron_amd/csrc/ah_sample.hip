@@ -86,81 +86,73 @@ AH_DEV uint32_t bin_at(float z) {
 
 // ---- workgroup scans (kT threads) -------------------------------------------------------------------
 
+// v of another lane through DPP (no LDS); lanes without a source, and rows outside ROWS, get 0.
+template <int CTRL, int ROWS> AH_DEV uint32_t dpp0(uint32_t v) {
+    return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
+}
+template <int CTRL, int ROWS> AH_DEV double dpp0(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)dpp0<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp0<CTRL, ROWS>((uint32_t)b));
+}
+struct Add {
+    template <class T> AH_DEV T operator()(T a, T b) const { return a + b; }
+};
+struct Max {
+    AH_DEV uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+};
+// Inclusive prefix over the wave (0 the operation's identity): inside rows of 16 by shifts of 1, 2, 4 and 8,
+// then the rows' ends passed on.
+template <class Op, class T> AH_DEV T wave_prefix(T v) {
+    const Op op;
+    v = op(v, dpp0<0x111, 0xF>(v));
+    v = op(v, dpp0<0x112, 0xF>(v));
+    v = op(v, dpp0<0x114, 0xF>(v));
+    v = op(v, dpp0<0x118, 0xF>(v));
+    v = op(v, dpp0<0x142, 0xA>(v));
+    return op(v, dpp0<0x143, 0xC>(v));
+}
+AH_DEV uint32_t last_lane(uint32_t v) { return (uint32_t)__builtin_amdgcn_readlane((int)v, 63); }
+AH_DEV double last_lane(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    return __builtin_bit_cast(double, (uint64_t)last_lane((uint32_t)(b >> 32)) << 32 | last_lane((uint32_t)b));
+}
+
 struct Scan {
     double d[kT / 64];
     uint32_t u[kT / 64];
+    AH_DEV double *of(double) { return d; }
+    AH_DEV uint32_t *of(uint32_t) { return u; }
 };
 // Inclusive prefix of v over the workgroup's threads, and the total.
-AH_DEV double scan_d(double v, Scan &S, double &total) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double t = __shfl_up(v, o, 64);
-        if ((int)lane >= o) v += t;
-    }
+template <class Op, class T> AH_DEV T scan(T v, Scan &S, T &total) {
+    const Op op;
+    const uint32_t wave = threadIdx.x >> 6;
+    T *at = S.of(v);
+    v = wave_prefix<Op>(v);
     __syncthreads();
-    if (lane == 63) S.d[wave] = v;
+    if ((threadIdx.x & 63) == 63) at[wave] = v;
     __syncthreads();
-    total = 0.0;
+    total = (T)0;
 #pragma unroll
     for (uint32_t w = 0; w < kT / 64; ++w) {
-        if (w < wave) v += S.d[w];
-        total += S.d[w];
+        if (w < wave) v = op(v, at[w]);
+        total = op(total, at[w]);
     }
     return v;
 }
-AH_DEV uint32_t scan_u(uint32_t v, Scan &S, uint32_t &total) {
-    const uint32_t lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t t = (uint32_t)__shfl_up((int)v, o, 64);
-        if ((int)lane >= o) v += t;
-    }
-    __syncthreads();
-    if (lane == 63) S.u[wave] = v;
-    __syncthreads();
-    total = 0;
-#pragma unroll
-    for (uint32_t w = 0; w < kT / 64; ++w) {
-        if (w < wave) v += S.u[w];
-        total += S.u[w];
-    }
-    return v;
-}
+AH_DEV double scan_d(double v, Scan &S, double &total) { return scan<Add>(v, S, total); }
+AH_DEV uint32_t scan_u(uint32_t v, Scan &S, uint32_t &total) { return scan<Add>(v, S, total); }
 AH_DEV double sum_d(double v, Scan &S) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v += __shfl_xor(v, o, 64);
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) S.d[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return (S.d[0] + S.d[1]) + (S.d[2] + S.d[3]);
+    double total;
+    scan<Add>(v, S, total);
+    return total;
 }
 AH_DEV uint32_t max_u(uint32_t v, Scan &S) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = __builtin_elementwise_max(v, (uint32_t)__shfl_xor((int)v, o, 64));
-    __syncthreads();
-    if ((threadIdx.x & 63) == 0) S.u[threadIdx.x >> 6] = v;
-    __syncthreads();
-    return __builtin_elementwise_max(__builtin_elementwise_max(S.u[0], S.u[1]), __builtin_elementwise_max(S.u[2], S.u[3]));
+    uint32_t total;
+    scan<Max>(v, S, total);
+    return total;
 }
 AH_DEV uint32_t min_u(uint32_t v, Scan &S) { return ~max_u(~v, S); }
-
-AH_DEV uint32_t wave_prefix(uint32_t v) {  // inclusive
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const uint32_t t = (uint32_t)__shfl_up((int)v, o, 64);
-        if ((int)(threadIdx.x & 63) >= o) v += t;
-    }
-    return v;
-}
-AH_DEV double wave_prefix(double v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double t = __shfl_up(v, o, 64);
-        if ((int)(threadIdx.x & 63) >= o) v += t;
-    }
-    return v;
-}
 
 // A lane's eight logits of a segment (-inf past the row's end), and their keys (0, below every key, there).
 AH_DEV void load_logits(const Row &r, uint32_t seg, float *x) {
@@ -275,6 +267,7 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
     }
     __syncthreads();
     for (uint32_t s = s0; s < s1; s += kT / 64) {
+        if (bin_at(z_of(r, a.seg_max[(size_t)row * a.segs + s])) > last) continue;  // none of its tokens reaches the bound
         uint32_t k[8];
         load_keys(r, s, k);
 #pragma unroll
@@ -304,14 +297,21 @@ struct LimitsLds {
     uint32_t bk, before_k, g0, g1;
     double mass_k, mass_0, w_low, w_high;
 };
-AH_DEV Limits limits_of(const SampleArgs &a, const Row &r, uint32_t row, Scan &S, LimitsLds &L) {
+// A thread's four bins, loaded ahead of what else a kernel waits for.
+struct Bins {
+    uint32_t c[4];
+    double m[4];
+    AH_DEV Bins(const SampleArgs &a, uint32_t row) {
+        __builtin_memcpy(c, a.bin_count + (size_t)row * kBins + 4 * threadIdx.x, 16);
+        __builtin_memcpy(m, a.bin_mass + (size_t)row * kBins + 4 * threadIdx.x, 32);
+    }
+};
+AH_DEV Limits limits_of(const SampleArgs &a, const Row &r, const Bins &B, Scan &S, LimitsLds &L) {
     Limits o = {kBins, kBins, kNone, 0, 0.0, 0.0, 0.0};
     if (!r.need_k && !r.need_p) return o;
     const uint32_t t = threadIdx.x;
-    uint32_t c[4];
-    double m[4];
-    __builtin_memcpy(c, a.bin_count + (size_t)row * kBins + 4 * t, 16);
-    __builtin_memcpy(m, a.bin_mass + (size_t)row * kBins + 4 * t, 32);
+    const uint32_t *c = B.c;
+    const double *m = B.m;
     if (t == 0) {
         L.bk = kNone;
         L.g0 = L.g1 = kBins - 1;
@@ -377,13 +377,25 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     __shared__ LimitsLds L;
     uint32_t row, s0, s1;
     share(a, row, s0, s1);
+    const Bins B(a, row);
     Row r = row_of(a, row);
     if (r.greedy) return;
     set_top(r, top_of(a, row, S));
     if (r.M == -__builtin_inff()) return;
-    const Limits o = limits_of(a, r, row, S, L);
+    const Limits o = limits_of(a, r, B, S, L);
     const uint32_t lane = threadIdx.x & 63;
+    // the last bin with a token to keep or to list (no bin: tokens without weight, as a whole)
+    const uint32_t end_k = o.bk != kNone ? o.bk : o.g1;
+    const uint32_t last = o.g0 == kBins ? kBins - 1 : end_k > o.g1 ? end_k : o.g1;
     for (uint32_t s = s0; s < s1; s += kT / 64) {
+        const size_t seg = (size_t)row * a.segs + s;
+        if (bin_at(z_of(r, a.seg_max[seg])) > last) {
+            if (lane == 0) {
+                a.seg_mass[seg] = 0.0;
+                a.seg_count[seg] = 0;
+            }
+            continue;
+        }
         uint32_t k[8], n = 0;
         load_keys(r, s, k);
         double sure = 0.0;
@@ -400,11 +412,10 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
                 ++n;
             }
         }
-        const size_t seg = (size_t)row * a.segs + s;
         uint32_t total = 0;
         if (__builtin_amdgcn_ballot_w64(n != 0) != 0ull) {
-            const uint32_t end = wave_prefix(n);
-            total = (uint32_t)__builtin_amdgcn_readlane((int)end, 63);
+            const uint32_t end = wave_prefix<Add>(n);
+            total = last_lane(end);
             uint32_t at = end - n;
             if (total <= kSampleSegList) {
                 uint16_t *list = a.list + seg * kSampleSegList;
@@ -413,10 +424,7 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
                     if (mask >> i & 1u) list[at++] = (uint16_t)(8 * lane + i);
             }
         }
-        if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) {
-#pragma unroll
-            for (int q = 1; q < 64; q <<= 1) sure += __shfl_xor(sure, q, 64);
-        }
+        if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
         if (lane == 0) {
             a.seg_mass[seg] = sure;
             a.seg_count[seg] = total;
@@ -432,7 +440,7 @@ struct DrawLds {
     double mass[256];
     uint32_t count[256];
     double seg[kSampleMaxSegs];
-    uint32_t start[kSampleMaxSegs + 1];
+    uint32_t start[kSampleMaxSegs];
     uint32_t key[kSampleList], idx[kSampleList];
     uint32_t u0, u1;
     double d0;
@@ -554,6 +562,18 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
 __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
     __shared__ DrawLds D;
     const uint32_t row = blockIdx.x, t = threadIdx.x;
+    const Bins B(a, row);
+    // this thread's segments: their certain weights, and how many tokens each lists
+    const uint32_t each = (a.segs + kT - 1) / kT, g0 = t * each < a.segs ? t * each : a.segs, g1 = g0 + each < a.segs ? g0 + each : a.segs;
+    uint32_t n_mine = 0;
+    bool full = false;
+    for (uint32_t s = g0; s < g1; ++s) {
+        const uint32_t c = a.seg_count[(size_t)row * a.segs + s];
+        D.seg[s] = a.seg_mass[(size_t)row * a.segs + s];
+        D.start[s] = c;
+        full |= c > kSampleSegList;
+        n_mine += c;
+    }
     Row r = row_of(a, row);
     const unsigned long long key0 = (unsigned long long)row << 8;
     if (t == 0 && r.bad_t) ah_record(a.status, key0 + AH_ERR_INPUT_RANGE);
@@ -581,25 +601,17 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         }
         return;
     }
-    const Limits o = limits_of(a, r, row, D.S, D.L);
+    const Limits o = limits_of(a, r, B, D.S, D.L);
     const bool do_k = o.bk != kNone, limited = do_k || r.need_p;
-    // the segments' certain weights, and where their listed tokens start
-    bool full = false;
-    uint32_t n = 0;
-    for (uint32_t base = 0; base < a.segs; base += kT) {
-        const uint32_t s = base + t;
-        uint32_t c = 0;
-        if (s < a.segs) {
-            D.seg[s] = a.seg_mass[(size_t)row * a.segs + s];
-            c = a.seg_count[(size_t)row * a.segs + s];
+    uint32_t n;
+    {  // where each segment's listed tokens start
+        uint32_t at = scan_u(n_mine, D.S, n) - n_mine;
+        for (uint32_t s = g0; s < g1; ++s) {
+            const uint32_t c = D.start[s];
+            D.start[s] = at;
+            at += c;
         }
-        full |= c > kSampleSegList;
-        uint32_t total;
-        const uint32_t end = n + scan_u(c, D.S, total);
-        if (s < a.segs) D.start[s + 1] = end;
-        n += total;
     }
-    if (t == 0) D.start[0] = 0;
     full = max_u(full, D.S) != 0 || n > kSampleList;
     Cut c = {0, kNone};
     auto kept = [&](uint32_t i, uint32_t k) -> double {
@@ -621,8 +633,7 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
             double w = 0.0;
 #pragma unroll
             for (uint32_t i = 0; i < 8; ++i) w += kept(s * kSeg + 8 * (t & 63) + i, k[i]);
-#pragma unroll
-            for (int q = 1; q < 64; q <<= 1) w += __shfl_xor(w, q, 64);
+            w = last_lane(wave_prefix<Add>(w));
             if ((t & 63) == 0) D.seg[s] = w;
         }
     } else if (n) {
@@ -690,24 +701,18 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
     }
     __syncthreads();
     // the segment, then the token in it
-    double W = 0.0;
-    for (uint32_t base = 0; base < a.segs; base += kT) {
-        double total;
-        scan_d(base + t < a.segs ? D.seg[base + t] : 0.0, D.S, total);
-        W += total;
-    }
+    double W, own = 0.0;
+    for (uint32_t s = g0; s < g1; ++s) own += D.seg[s];
+    double ahead = scan_d(own, D.S, W) - own;
     double goal = __builtin_floor((double)(r.u > 0.0f ? r.u : 0.0f) * W);
     goal = goal < W ? goal : W - 1.0;
-    double before = 0.0;
-    for (uint32_t base = 0; base < a.segs; base += kT) {
-        const double mine = base + t < a.segs ? D.seg[base + t] : 0.0;
-        double total;
-        const double cum = before + scan_d(mine, D.S, total);
-        if (cum > goal && cum - mine <= goal) {
-            D.u0 = base + t;
-            D.d0 = cum - mine;
+    for (uint32_t s = g0; s < g1; ++s) {
+        const double w = D.seg[s];
+        if (ahead <= goal && ahead + w > goal) {
+            D.u0 = s;
+            D.d0 = ahead;
         }
-        before += total;
+        ahead += w;
     }
     __syncthreads();
     if (t >= 64) return;
@@ -720,7 +725,7 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         w[i] = kept(s * kSeg + 8 * t + i, k[i]);
         mine += w[i];
     }
-    double cum = D.d0 + wave_prefix(mine) - mine;
+    double cum = D.d0 + wave_prefix<Add>(mine) - mine;
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) {
         if (cum <= goal && cum + w[i] > goal) {
