@@ -69,20 +69,25 @@ AH_DEV void set_top(Row &r, uint32_t top) {
     r.M = logit_of(top);
     r.inv_t = 1.0f / r.T;
 }
-AH_DEV float z_of(const Row &r, uint32_t k) {
+// A logit's z = (l - M) / T, from the logit itself (NaN as -inf) or its key (0 past the row's end).
+AH_DEV float z_at(const Row &r, float l) {
 #pragma clang fp contract(off)
-    return k == r.top ? 0.0f : (logit_of(k) - r.M) * r.inv_t;
+    l = __builtin_fmaxf(l, -__builtin_inff());
+    return l == r.M ? 0.0f : (l - r.M) * r.inv_t;
 }
-// The weight: a whole number, as f32 (exact: exp's 24 bits, rounded below 1).
+AH_DEV float z_of(const Row &r, uint32_t k) { return k ? z_at(r, logit_of(k)) : -__builtin_inff(); }
+// The weight: a whole number, as f32 (exact: exp's 24 bits, rounded below 1).  exp(z) = 2^(z log2 e), the
+// product's own rounding carried as a factor next to 1: about 1.5 units of f32's last place.
 AH_DEV float weight_at(float z) {
 #pragma clang fp contract(off)
-    return __builtin_rintf(expf(z) * 0x1p32f);
+    const float l2e = 0x1.715476p+0f, rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;  // log2 e = l2e + rest
+    const float t = z * l2e;
+    if (!(t > -40.0f)) return 0.0f;
+    const float d = __builtin_fmaf(z, rest, __builtin_fmaf(z, l2e, -t)), e = __builtin_amdgcn_exp2f(t);
+    return __builtin_rintf(__builtin_fmaf(e, d * ln2, e) * 0x1p32f);
 }
-// The bin of a key, kBins where the weight is 0 (monotone in the key, as z is).
-AH_DEV uint32_t bin_at(float z) {
-    const float t = z * -kBinScale;
-    return t < (float)kBins ? (uint32_t)t : kBins;
-}
+// The bin of z, kBins where the weight is 0.
+AH_DEV uint32_t bin_at(float z) { return (uint32_t)__builtin_fminf(z * -kBinScale, (float)kBins); }
 
 // ---- workgroup scans (kT threads) -------------------------------------------------------------------
 
@@ -245,7 +250,7 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
         const uint32_t *g = few ? a.seg_max + (size_t)row * a.segs : a.group_max + (size_t)row * a.segs * kGroups;
         const uint32_t n_max = few ? a.segs : a.segs * kGroups;
         for (uint32_t i = threadIdx.x; i < n_max; i += kT) {
-            const uint32_t k = g[i], b = k ? bin_at(z_of(r, k)) : kBins;
+            const uint32_t b = bin_at(z_of(r, g[i]));
             if (b < kBins) atomicAdd(&count[b], 1u);
         }
         __syncthreads();
@@ -268,12 +273,12 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
     __syncthreads();
     for (uint32_t s = s0; s < s1; s += kT / 64) {
         if (bin_at(z_of(r, a.seg_max[(size_t)row * a.segs + s])) > last) continue;  // none of its tokens reaches the bound
-        uint32_t k[8];
-        load_keys(r, s, k);
+        float x[8];
+        load_logits(r, s, x);
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
-            const float z = z_of(r, k[i]);
-            const uint32_t b = k[i] ? bin_at(z) : kBins;
+            const float z = z_at(r, x[i]);
+            const uint32_t b = bin_at(z);
             if (b > last) continue;
             if (r.need_k) atomicAdd(&count[b], 1u);
             if (r.need_p) unsafeAtomicAdd(&mass[b], (double)weight_at(z));
@@ -396,14 +401,15 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
             }
             continue;
         }
-        uint32_t k[8], n = 0;
-        load_keys(r, s, k);
+        float x[8];
+        uint32_t n = 0;
+        load_logits(r, s, x);
         double sure = 0.0;
         uint32_t mask = 0;
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) {
-            const float z = z_of(r, k[i]);
-            const uint32_t b = k[i] ? bin_at(z) : kBins;
+            const float z = z_at(r, x[i]);
+            const uint32_t b = bin_at(z);
             if (b < o.g0 && b < kBins) {
                 const double w = (double)weight_at(z);
                 sure += w < r.floor_w ? 0.0 : w;
@@ -467,6 +473,14 @@ template <class Key, class Index> AH_DEV uint32_t nth_equal(uint32_t n, Key key,
     return D.u0;
 }
 
+// The digit at which keys between lo and hi first differ, as a shift, and what they share above it.
+AH_DEV int first_digit(uint32_t lo, uint32_t hi, uint32_t &shared) {
+    const uint32_t x = lo ^ hi;
+    const int shift = x ? (31 - __builtin_clz(x)) / 8 * 8 : 0;
+    shared = shift == 24 ? 0 : hi >> (shift + 8) << (shift + 8);
+    return shift;
+}
+
 // The cut over n tokens in index order (a list, or the whole row), by digits of the keys.  in_k(key) and
 // in_p(key): whether such a token counts for the top-k and for the top-p limit.  need: tokens that top-k still
 // keeps of its own; W0: the weight ahead of those (without top-k: of every token); before: the weight ahead of
@@ -479,7 +493,17 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
     uint32_t keep = 0, cut_k = 0;  // of those at the cut
     bool partial = false;
     if (do_k) {
-        for (int shift = 24; shift >= 0; shift -= 8) {
+        uint32_t lo = kNone, hi = 0;
+        for (uint32_t i = t; i < n; i += kT) {
+            const uint32_t k = key(i);
+            if (in_k(k)) {
+                lo = __builtin_elementwise_min(lo, k);
+                hi = __builtin_elementwise_max(hi, k);
+            }
+        }
+        lo = min_u(lo, D.S);
+        hi = max_u(hi, D.S);
+        for (int shift = first_digit(lo, hi, cut_k); shift >= 0; shift -= 8) {
             __syncthreads();
             D.count[t] = 0;
             __syncthreads();
@@ -516,8 +540,17 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
         }
         double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
         goal = goal < 1.0 ? 1.0 : goal;  // the first token always
-        uint32_t cut_p = 0, all = 0;
-        for (int shift = 24; shift >= 0; shift -= 8) {
+        uint32_t cut_p = 0, all = 0, lo = do_k && in_p(cut_k) ? cut_k : kNone, hi = lo == kNone ? 0u : cut_k;
+        for (uint32_t i = t; i < n; i += kT) {
+            const uint32_t k = key(i);
+            if (in_p(k) && !(do_k && k <= cut_k)) {
+                lo = __builtin_elementwise_min(lo, k);
+                hi = __builtin_elementwise_max(hi, k);
+            }
+        }
+        lo = min_u(lo, D.S);
+        hi = max_u(hi, D.S);
+        for (int shift = first_digit(lo, hi, cut_p); shift >= 0; shift -= 8) {
             __syncthreads();
             D.mass[t] = 0.0;
             D.count[t] = 0;
@@ -617,7 +650,7 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
     auto kept = [&](uint32_t i, uint32_t k) -> double {
         if (limited && (k < c.key || (k == c.key && i > c.last))) return 0.0;
         const float z = z_of(r, k);
-        if (!k || bin_at(z) == kBins) return 0.0;
+        if (bin_at(z) == kBins) return 0.0;
         const double w = (double)weight_at(z);
         return w < r.floor_w ? 0.0 : w;
     };
@@ -652,7 +685,7 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         if (n <= kT) {
             // a token a thread, its place among the others by comparing with each
             const bool live = t < n;
-            const uint32_t k = live ? D.key[t] : 0u, b = live ? bin(k) : kBins;
+            const uint32_t k = live ? D.key[t] : 0u, b = bin(k);
             const bool ink = live && do_k && b == o.bk, inp = live && b >= o.g0 && b <= o.g1;
 
             const double w = live ? (double)weight_at(z_of(r, k)) : 0.0;
