@@ -12,6 +12,7 @@ namespace {
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef float f32x16 __attribute__((ext_vector_type(16)));
 
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNoMax = -3.402823466e38f;  // below every finite score
@@ -23,6 +24,8 @@ constexpr float kSlack = 4.0f;
 constexpr float kUp = 9.0f;
 
 AH_DEV f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+AH_DEV f32x16 mfma32(f16x8 a, f16x8 b, f32x16 c) { return __builtin_amdgcn_mfma_f32_32x32x16_f16(a, b, c, 0, 0, 0); }
 
 // Codes as f16 values.  1024 + c has c in its lowest mantissa bits, 1024 + 16 c in the next four:
 // (1024 + c) - 1032, (1024 + 16 c) / 16 - 72 and the products by d are exact.  The masks stay in registers
@@ -141,6 +144,17 @@ AH_DEV float ror8(float v) {  // lane r ^ 8 of each 16 (a rotation by 8)
 }
 AH_DEV f16x2 pack16(float a, float b) { return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a, b)); }
 
+// q's power-of-two scale: `up` makes the row's largest magnitude (of `top` over its lanes) lie in [2^13, 2^14) and
+// carries the scale's sign; scores times f are in powers of two.  f > 0, so that the largest product is also
+// the largest score and a masked -inf stays that.
+AH_DEV void q_scale(float scale, float top, float &up, float &f) {
+    int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;  // top in [2^e, 2^(e+1))
+    e = e < -100 ? -100 : e > 127 ? 127 : e;
+    up = __builtin_ldexpf(1.0f, 13 - e);
+    f = __builtin_fmaxf(__builtin_fabsf(scale) * kLog2e * __builtin_ldexpf(1.0f, e - 13), 0x1p-126f);
+    up = scale == 0.0f ? 0.0f : scale < 0.0f ? -up : scale > 0.0f ? up : scale;
+}
+
 // Rows (token, head of the group) as the 16 columns of the products: every wave takes tiles of 32 tokens of
 // the workgroup's piece of the context, each with its own running maximum, and the four meet in LDS.  A
 // lane (r, h) holds the scores of column r, tokens 4 h + i of both half-tiles.
@@ -207,13 +221,8 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnAr
         }
         top = __builtin_fmaxf(top, xor_lanes(top, 16));
         top = __builtin_fmaxf(top, xor_lanes(top, 32));
-        int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;  // top in [2^e, 2^(e+1))
-        e = e < -100 ? -100 : e > 127 ? 127 : e;
-        const float up = __builtin_ldexpf(1.0f, 13 - e);
-        // scores times f are in powers of two.  f > 0 (a negative scale turns q's sign), so that the largest
-        // product is also the largest score, and a masked -inf stays that.
-        f = __builtin_fmaxf(__builtin_fabsf(a.scale) * kLog2e * __builtin_ldexpf(1.0f, e - 13), 0x1p-126f);
-        const float sign = a.scale == 0.0f ? 0.0f : a.scale < 0.0f ? -up : a.scale > 0.0f ? up : a.scale;
+        float sign;
+        q_scale(a.scale, top, sign, f);
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
@@ -361,6 +370,238 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnAr
     }
 }
 
+// Chunks of tokens: 128 rows (token, head of the group) a workgroup, 32 a wave as the columns of 32x32 products,
+// over 64 keys at a time.  The four waves turn a tile's codes into f16 in LDS together (once for 128 rows), in
+// one of two buffers while they compute on the other: one barrier a tile.  A lane (c, h) = (lane & 31,
+// lane >> 5) holds column c's scores of the tokens 8 b + 4 h + i; V's rows lie in LDS with the tokens in the
+// order of those scores, so p stays in its lane here too.
+//   LDS: K [64 tokens][D], V [D channels][64 tokens], rows 16 bytes longer than their values: 16 lanes' rows
+//   start 4 banks apart, so a 16-byte read of the wave meets no conflict.
+template <int D> struct TileLds {
+    static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;
+};
+template <int D>
+__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnArgs a) {
+    constexpr int NK = D / 16, NN = D / 32, NU = D / 64;  // contraction steps of K q; channel blocks; 16-byte units
+    typedef TileLds<D> Lds;
+    extern __shared__ uint8_t tile_lds[];
+    const uint32_t lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    // pieces slowest; then the last rows first: with a causal mask they have the most keys
+    const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units, unit = blockIdx.x - split * units;
+    const uint32_t others = a.n_seq * a.c.n_kv, per = units / others, rt = per - 1 - unit / others, rest = unit % others;
+    const uint32_t s = rest / a.c.n_kv, kvh = rest - s * a.c.n_kv;
+    const Span p = span_of(a, s);
+    if (p.bad && split == 0 && rt == 0 && kvh == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
+    const uint32_t rows = p.nq * a.group, row0 = rt * 128;
+    if (row0 >= rows) return;
+    const int32_t pos0 = p.ctx - (int32_t)p.nq;
+    const uint32_t last = row0 + 127 < rows ? row0 + 127 : rows - 1;
+    const Tiles T = tiles_of(a, pos0 + (int32_t)(row0 / a.group), pos0 + (int32_t)(last / a.group));
+    const uint32_t chunk = piece_of(a, T), t0 = split * chunk, t1 = t0 + chunk < T.count ? t0 + chunk : T.count;
+    if (split > 0 && t0 >= T.count) return;
+    // this wave's rows and the positions they span
+    const uint32_t wrow = row0 + 32 * wave, row = wrow + c, tok = row / a.group, hq = kvh * a.group + row % a.group;
+    const bool live = row < rows, any = wrow < rows;
+    const uint32_t wlast = wrow + 31 < rows ? wrow + 31 : rows - 1;
+    const int32_t lo = pos0 + (int32_t)(wrow / a.group), hi = any ? pos0 + (int32_t)(wlast / a.group) : -1;
+    const int32_t pos = live ? pos0 + (int32_t)tok : -1;
+    auto tile_of = [&](uint32_t i) { return i < T.head ? i : T.tail + (i - T.head); };
+
+    // A wave's share of a tile of 64 tokens: of its K and V units (1 KB of codes of 32 tokens), every fourth.
+    constexpr int NS = D == 64 ? 1 : D / 128;  // of each kind
+    const uint32_t kr = lane & 15, kq = lane >> 4;
+    u32x4 kw[NS], vw[NS];
+    uint32_t kd[NS];
+    f16x8 vd[NS][2];
+    auto unit_at = [&](int i) { return D == 64 ? wave & 1 : wave + 4 * i; };  // of 2 NU: tile * NU + chunk
+    const bool do_k = D != 64 || wave < 2, do_v = D != 64 || wave >= 2;
+    uint32_t bad = 0;  // of the tiles whose codes are on their way: bit 0 and 1
+    auto fetch = [&](uint32_t ti) {
+        bad = 0;
+        const uint8_t *base[2];
+#pragma unroll
+        for (uint32_t j = 0; j < 2; ++j) {
+            bool ok;
+            base[j] = tile_at(a, s, kvh, tile_of(ti + j < t1 ? ti + j : t1 - 1), ok);
+            if (!ok || ti + j >= t1) bad |= 1u << j;
+            if (!ok && ti + j < t1 && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
+        }
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const uint32_t u = unit_at(i), ch = u % NU;
+            const uint8_t *t = u < (uint32_t)NU ? base[0] : base[1];
+            if (do_k) {
+                const uint32_t blk = D == 64 ? kq >> 1 : D == 128 ? kq : 2 * kq + (ch & 1);
+                __builtin_memcpy(&kw[i], t + ch * 1024 + (kr * 4 + kq) * 16, 16);
+                __builtin_memcpy(&kd[i], t + 32 * D + (kr * (D / 32) + blk) * 4, 4);
+            }
+            if (do_v) {
+                __builtin_memcpy(&vw[i], t + 16 * D + (ch * 16 + kr) * 64 + kq * 16, 16);
+#pragma unroll
+                for (int b = 0; b < 2; ++b) __builtin_memcpy(&vd[i][b], t + 34 * D + ((2 * ch + b) * 4 + kq) * 16, 16);
+            }
+        }
+    };
+    const Masks mk;
+    auto spread = [&](uint8_t *buf) {
+#pragma unroll
+        for (int i = 0; i < NS; ++i) {
+            const uint32_t u = unit_at(i), ch = u % NU, t32 = 32 * (u / NU);
+            if (do_k) {
+#pragma unroll
+                for (int w = 0; w < 4; ++w) {
+                    const uint32_t half = D == 64 ? w >> 1 : D == 128 ? ch : ch >> 1;
+                    const uint32_t chan = D == 64 ? kq * 16 + 8 * (w & 1) : D == 128 ? kq * 32 + 8 * w : kq * 64 + (ch & 1) * 32 + 8 * w;
+                    const f16x8 v = k_frag(kw[i][w], pair_of(half ? kd[i] >> 16 : kd[i]), mk);
+                    __builtin_memcpy(buf + (t32 + 16 * half + kr) * Lds::kK + 2 * chan, &v, 16);
+                }
+            }
+            if (do_v) {
+#pragma unroll
+                for (int b = 0; b < 2; ++b) {
+                    f16x8 even, odd;
+                    v_frags(vw[i][2 * b], vw[i][2 * b + 1], vd[i][b], mk, even, odd);
+                    uint8_t *to = buf + 64 * Lds::kK + 2 * (16 * (2 * ch + b) + kr) * Lds::kV + 2 * (t32 + (kq & 1) * 8 + (kq >> 1) * 4);
+                    __builtin_memcpy(to, &even, 8);  // half-tile 0's four tokens, then half-tile 1's
+                    __builtin_memcpy(to + 32, reinterpret_cast<const char *>(&even) + 8, 8);
+                    __builtin_memcpy(to + Lds::kV, &odd, 8);
+                    __builtin_memcpy(to + Lds::kV + 32, reinterpret_cast<const char *>(&odd) + 8, 8);
+                }
+            }
+        }
+    };
+
+    f32x16 acc[NN];
+#pragma unroll
+    for (int n = 0; n < NN; ++n) acc[n] = (f32x16)0.0f;
+    float m = kNoMax, l = 0.0f;
+    if (t0 < t1) {
+        fetch(t0);
+        f16x8 qh[NK], ql[NK];
+        float f;
+        {
+            const float *q = a.q + (size_t)(p.q0 + (live ? tok : 0)) * a.q_stride + (size_t)(live ? hq : 0) * D + 8 * h;
+            float x[NK][8], top = 0.0f, up;
+#pragma unroll
+            for (int k = 0; k < NK; ++k) {
+                __builtin_memcpy(x[k], q + 16 * k, 32);
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    x[k][i] = live ? x[k][i] : 0.0f;
+                    top = __builtin_fmaxf(top, __builtin_fabsf(x[k][i]));
+                }
+            }
+            q_scale(a.scale, __builtin_fmaxf(top, xor_lanes(top, 32)), up, f);
+#pragma unroll
+            for (int k = 0; k < NK; ++k)
+#pragma unroll
+                for (int i = 0; i < 8; ++i) {
+                    const float y = x[k][i] * up;
+                    const _Float16 hv = (_Float16)y;
+                    qh[k][i] = hv;
+                    ql[k][i] = (_Float16)(y - (float)hv);
+                }
+        }
+        uint32_t bad_now = bad;
+        spread(tile_lds);
+        if (t0 + 2 < t1) fetch(t0 + 2);
+        __syncthreads();
+        for (uint32_t ti = t0, at = 0; ti < t1; ti += 2, at ^= 1) {
+            const uint8_t *buf = tile_lds + at * Lds::kBytes;
+            const int32_t first0 = (int32_t)(32 * tile_of(ti)), first1 = (int32_t)(32 * tile_of(ti + 1 < t1 ? ti + 1 : ti));
+            // a wave whose rows all stand before the tile (a causal mask) only helps to load
+            const bool work = any && (first0 <= hi || first1 <= hi);
+            f32x16 sc[2];
+            if (work) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    sc[j] = (f32x16)0.0f;
+#pragma unroll
+                    for (int k = 0; k < NK; ++k) {
+                        f16x8 kf;
+                        __builtin_memcpy(&kf, buf + (32 * j + c) * Lds::kK + 2 * (16 * k + 8 * h), 16);
+                        sc[j] = mfma32(kf, qh[k], sc[j]);
+                        sc[j] = mfma32(kf, ql[k], sc[j]);
+                    }
+                }
+            }
+            if (ti + 2 < t1) spread(tile_lds + (at ^ 1) * Lds::kBytes);
+            const uint32_t bad_next = bad;
+            if (ti + 4 < t1) fetch(ti + 4);
+            if (work) {
+#pragma unroll
+                for (int j = 0; j < 2; ++j) {
+                    const int32_t first = j ? first1 : first0;
+                    const bool ok = !(bad_now >> j & 1u);
+                    const bool whole = ok && first + 31 <= lo &&
+                                       (!a.window || (int64_t)first > (int64_t)hi - (int64_t)a.window || first + 32 <= (int64_t)a.sinks);
+                    if (!whole) {
+#pragma unroll
+                        for (int i = 0; i < 16; ++i) {
+                            const int32_t key = first + 8 * (i >> 2) + 4 * (int32_t)h + (i & 3);
+                            const bool see = ok && key <= pos && (!a.window || (int64_t)key > (int64_t)pos - (int64_t)a.window || (uint32_t)key < a.sinks);
+                            sc[j][i] = see ? sc[j][i] : -__builtin_inff();
+                        }
+                    }
+                }
+                float top = sc[0][0];
+#pragma unroll
+                for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, sc[i >> 4][i & 15]);
+                top *= f;
+                if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0ull) {
+                    const float up = __builtin_fmaxf(m, __builtin_fmaxf(top, xor_lanes(top, 32))), alpha = __builtin_amdgcn_exp2f(m - up);
+                    m = up;
+                    l *= alpha;
+#pragma unroll
+                    for (int n = 0; n < NN; ++n) acc[n] *= alpha;
+                }
+                const float base = kUp - m;
+#pragma unroll
+                for (int g = 0; g < 4; ++g) {  // 16 tokens
+                    f16x2 ph[4], pl[4];
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) {
+                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + 2 * i], f, base));
+                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + 2 * i + 1], f, base));
+                        l += e0;
+                        l += e1;
+                        ph[i] = pack16(e0, e1);
+                        pl[i] = pack16(e0 - (float)ph[i][0], e1 - (float)ph[i][1]);
+                    }
+                    const f16x8 pf = join8(ph[0], ph[1], ph[2], ph[3]), pg = join8(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+                    for (int n = 0; n < NN; ++n) {
+                        f16x8 vf;
+                        __builtin_memcpy(&vf, buf + 64 * Lds::kK + (32 * n + c) * Lds::kV + 2 * (16 * g + 8 * h), 16);
+                        acc[n] = mfma32(vf, pf, acc[n]);
+                        acc[n] = mfma32(vf, pg, acc[n]);
+                    }
+                }
+            }
+            bad_now = bad_next;
+            __syncthreads();
+        }
+    }
+    l += xor_lanes(l, 32);
+    if (!live) return;
+    const size_t flat = (size_t)(p.q0 + tok) * a.n_heads + hq, all = (size_t)a.n_tok * a.n_heads;
+    const float inv = a.splits > 1 ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    float *dst = a.splits > 1 ? a.part_o + (split * all + flat) * D : a.out + (size_t)(p.q0 + tok) * a.out_stride + (size_t)hq * D;
+#pragma unroll
+    for (int n = 0; n < NN; ++n)
+#pragma unroll
+        for (int b = 0; b < 4; ++b) {
+            const f32x4 o = (f32x4){acc[n][4 * b], acc[n][4 * b + 1], acc[n][4 * b + 2], acc[n][4 * b + 3]} * inv;
+            __builtin_memcpy(dst + 32 * n + 8 * b + 4 * h, &o, 16);
+        }
+    if (a.splits > 1 && h == 0) {
+        float *ml = a.part_ml + 2 * (split * all + flat);
+        ml[0] = m;
+        ml[1] = l;
+    }
+}
+
 // Joins the pieces of a context: a workgroup per row (token, head), its waves every fourth piece.  A piece
 // past the row's keys was never written; which those are follows from the same tiles_of.
 template <int D>
@@ -405,10 +646,11 @@ template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) *
 
 template <int D>
 hipError_t launch(const AttnArgs &a, hipStream_t stream) {
-    const bool pack = a.rows == 8;
     const uint32_t tiles = (a.max_q * a.group + a.rows - 1) / a.rows;
-    hipLaunchKernelGGL((pack ? attn_rows_kernel<D, true> : attn_rows_kernel<D, false>), dim3(a.splits * tiles * a.c.n_kv * a.n_seq), dim3(256),
-                       attn_lds<D>(), stream, a);
+    const dim3 grid(a.splits * tiles * a.c.n_kv * a.n_seq);
+    if (a.rows == 128) hipLaunchKernelGGL(attn_tile_kernel<D>, grid, dim3(256), 2 * TileLds<D>::kBytes, stream, a);
+    else if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false>), grid, dim3(256), attn_lds<D>(), stream, a);
+    else hipLaunchKernelGGL((attn_rows_kernel<D, true>), grid, dim3(256), attn_lds<D>(), stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
     hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.max_q * a.n_heads, a.n_seq), dim3(256), 0, stream, a, a.rows);
@@ -426,6 +668,8 @@ hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream) {
 }
 
 hipError_t ah_attn_init_attrs() {
-    const hipError_t e = allow_lds(attn_rows_kernel<256, false>, attn_lds<256>());
-    return e != hipSuccess ? e : allow_lds(attn_rows_kernel<256, true>, attn_lds<256>());
+    hipError_t e = allow_lds(attn_rows_kernel<256, false>, attn_lds<256>());
+    if (e == hipSuccess) e = allow_lds(attn_rows_kernel<256, true>, attn_lds<256>());
+    if (e == hipSuccess) e = allow_lds(attn_tile_kernel<128>, 2 * TileLds<128>::kBytes);
+    return e != hipSuccess ? e : allow_lds(attn_tile_kernel<256>, 2 * TileLds<256>::kBytes);
 }

@@ -121,7 +121,7 @@ struct AttnArgs {
     // the split of the contexts: `splits` pieces of `chunk` tiles each; with several, partial results
     // go to part_o [splits][n_tok * n_heads][dim] and part_ml [splits][n_tok * n_heads][2]
     uint32_t splits, chunk;
-    uint32_t rows;  // rows (token, head of a KV head's group) of a workgroup: 8 or 16
+    uint32_t rows;  // rows (token, head of a KV head's group) of a workgroup: 8, 16 or 128
     float *part_o, *part_ml;
     unsigned long long *status;
 };
