@@ -249,7 +249,7 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     }
     a.rows = a.max_q * a.group <= 8 ? 8 : a.max_q * a.group < 64 ? 16 : 128;
     const size_t base = ((size_t)a.max_q * a.group + a.rows - 1) / a.rows * kv * p->n_seq, rows = p->n_tok * p->n_heads;
-    size_t splits = (a.rows == 128 ? 512 : kAttnGroups) / base, fit = a.rows == 128 ? (tiles + 7) / 8 : (tiles + 3) / 4;
+    size_t splits = (a.rows == 128 ? 768 : kAttnGroups) / base, fit = a.rows == 128 ? (tiles + 7) / 8 : (tiles + 3) / 4;
     const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float));
     splits = splits < fit ? splits : fit;
     splits = splits < room ? splits : room;

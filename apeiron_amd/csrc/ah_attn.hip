@@ -188,6 +188,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnAr
     const uint32_t last = row0 + R - 1 < rows ? row0 + R - 1 : rows - 1;
     const int32_t lo = pos0 + (int32_t)(row0 / a.group), hi = pos0 + (int32_t)(last / a.group);
     const int32_t pos = live ? pos0 + (int32_t)tok : -1;
+    // the keys below which the window hides one (for this row, and for the last of the rows), and the sinks
+    const int32_t low_key = a.window ? pos - (int32_t)a.window + 1 : 0, low_all = a.window ? hi - (int32_t)a.window + 1 : 0;
+    const int32_t sink_key = (int32_t)a.sinks;
     const Tiles T = tiles_of(a, lo, hi);
     const uint32_t chunk = piece_of(a, T), t0 = split * chunk, t1 = t0 + chunk < T.count ? t0 + chunk : T.count;
     if (split > 0 && t0 >= T.count) return;
@@ -264,13 +267,14 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnAr
         }
         const int32_t first = (int32_t)(tile * 32);
         // a tile that every row sees whole needs no mask
-        const bool whole = ok && first + 31 <= lo && (!a.window || (int64_t)first > (int64_t)hi - (int64_t)a.window || first + 32 <= (int64_t)a.sinks);
+        const bool whole = ok && first + 31 <= lo && (first >= low_all || first + 32 <= sink_key);
         if (!whole) {
             if (!ok && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
+            const int32_t top_key = ok ? pos : -1;
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const int32_t key = first + 16 * (i >> 2) + 4 * (int32_t)h + (i & 3);
-                const bool see = ok && key <= pos && (!a.window || (int64_t)key > (int64_t)pos - (int64_t)a.window || (uint32_t)key < a.sinks);
+                const bool see = key <= top_key && (key >= low_key || key < sink_key);
                 x[i] = see ? x[i] : -__builtin_inff();
             }
         }
@@ -406,6 +410,9 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
     const uint32_t wlast = wrow + 31 < rows ? wrow + 31 : rows - 1;
     const int32_t lo = pos0 + (int32_t)(wrow / a.group), hi = any ? pos0 + (int32_t)(wlast / a.group) : -1;
     const int32_t pos = live ? pos0 + (int32_t)tok : -1;
+    // the keys below which the window hides one (for this row, and for the last of the rows), and the sinks
+    const int32_t low_key = a.window ? pos - (int32_t)a.window + 1 : 0, low_all = a.window ? hi - (int32_t)a.window + 1 : 0;
+    const int32_t sink_key = (int32_t)a.sinks;
     auto tile_of = [&](uint32_t i) { return i < T.head ? i : T.tail + (i - T.head); };
 
     // A wave's share of a tile of 64 tokens: of its K and V units (1 KB of codes of 32 tokens), every fourth.
@@ -514,11 +521,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
             const bool work = any && (first0 <= hi || first1 <= hi);
             f32x16 sc[2];
             if (work) {
+                sc[0] = sc[1] = (f32x16)0.0f;
 #pragma unroll
-                for (int j = 0; j < 2; ++j) {
-                    sc[j] = (f32x16)0.0f;
+                for (int k = 0; k < NK; ++k) {
 #pragma unroll
-                    for (int k = 0; k < NK; ++k) {
+                    for (int j = 0; j < 2; ++j) {
                         f16x8 kf;
                         __builtin_memcpy(&kf, buf + (32 * j + c) * Lds::kK + 2 * (16 * k + 8 * h), 16);
                         sc[j] = mfma32(kf, qh[k], sc[j]);
@@ -534,13 +541,13 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
                 for (int j = 0; j < 2; ++j) {
                     const int32_t first = j ? first1 : first0;
                     const bool ok = !(bad_now >> j & 1u);
-                    const bool whole = ok && first + 31 <= lo &&
-                                       (!a.window || (int64_t)first > (int64_t)hi - (int64_t)a.window || first + 32 <= (int64_t)a.sinks);
+                    const bool whole = ok && first + 31 <= lo && (first >= low_all || first + 32 <= sink_key);
                     if (!whole) {
+                        const int32_t top_key = ok ? pos : -1;
 #pragma unroll
                         for (int i = 0; i < 16; ++i) {
                             const int32_t key = first + 8 * (i >> 2) + 4 * (int32_t)h + (i & 3);
-                            const bool see = ok && key <= pos && (!a.window || (int64_t)key > (int64_t)pos - (int64_t)a.window || (uint32_t)key < a.sinks);
+                            const bool see = key <= top_key && (key >= low_key || key < sink_key);
                             sc[j][i] = see ? sc[j][i] : -__builtin_inff();
                         }
                     }
@@ -602,18 +609,20 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
     }
 }
 
-// Joins the pieces of a context: a workgroup per row (token, head), its waves every fourth piece.  A piece
-// past the row's keys was never written; which those are follows from the same tiles_of.
-template <int D>
-__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, uint32_t tile_rows) {
+// Joins the pieces of a context.  WIDE: a workgroup per row (token, head), its waves every fourth piece, for a few
+// rows in many pieces; otherwise a wave per row.  A piece past the row's keys was never written; which those
+// are follows from the same tiles_of.
+template <int D, bool WIDE>
+__global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
+    constexpr int E = D / 64;  // channels of a lane
     __shared__ float red[4][D + 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y;
     const Span p = span_of(a, s);
-    const uint32_t n = p.nq * a.n_heads, it = blockIdx.x;
+    const uint32_t n = p.nq * a.n_heads, it = WIDE ? blockIdx.x : 4 * blockIdx.x + wave;
     if (it >= n) return;
     const uint32_t i = it / a.n_heads, head = it % a.n_heads, g = a.group;
-    const uint32_t row = i * g + head % g, row0 = row - row % tile_rows;
-    const uint32_t last = row0 + tile_rows - 1 < p.nq * g ? row0 + tile_rows - 1 : p.nq * g - 1;
+    const uint32_t row = i * g + head % g, row0 = row - row % a.rows;
+    const uint32_t last = row0 + a.rows - 1 < p.nq * g ? row0 + a.rows - 1 : p.nq * g - 1;
     const int32_t pos0 = p.ctx - (int32_t)p.nq;
     const Tiles T = tiles_of(a, pos0 + (int32_t)(row0 / g), pos0 + (int32_t)(last / g));
     const uint32_t chunk = piece_of(a, T), pieces = T.count ? (T.count + chunk - 1) / chunk : 1;
@@ -622,24 +631,35 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a, uint32_t til
     for (uint32_t k = lane; k < pieces; k += 64) M = __builtin_fmaxf(M, a.part_ml[2 * (k * all + flat)]);
 #pragma unroll
     for (int o = 1; o < 64; o <<= 1) M = __builtin_fmaxf(M, xor_lanes(M, o));
-    float L = 0.0f, acc[D / 64];
+    float L = 0.0f, acc[E];
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) acc[c] = 0.0f;
+    for (int c = 0; c < E; ++c) acc[c] = 0.0f;
 #pragma unroll 4
-    for (uint32_t k = wave; k < pieces; k += 4) {
-        const float *ml = a.part_ml + 2 * (k * all + flat), w = __builtin_amdgcn_exp2f(ml[0] - M);
+    for (uint32_t k = WIDE ? wave : 0; k < pieces; k += WIDE ? 4 : 1) {
+        float ml[2], o[E];
+        __builtin_memcpy(ml, a.part_ml + 2 * (k * all + flat), 8);
+        __builtin_memcpy(o, a.part_o + (k * all + flat) * D + E * lane, 4 * E);
+        const float w = __builtin_amdgcn_exp2f(ml[0] - M);
         L += ml[1] * w;
 #pragma unroll
-        for (int c = 0; c < D / 64; ++c) acc[c] += a.part_o[(k * all + flat) * D + 64 * c + lane] * w;
+        for (int c = 0; c < E; ++c) acc[c] += o[c] * w;
+    }
+    float *dst = a.out + (size_t)(p.q0 + i) * a.out_stride + (size_t)head * D;
+    if (!WIDE) {
+        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+#pragma unroll
+        for (int c = 0; c < E; ++c) acc[c] *= inv;
+        __builtin_memcpy(dst + E * lane, acc, 4 * E);
+        return;
     }
 #pragma unroll
-    for (int c = 0; c < D / 64; ++c) red[wave][64 * c + lane] = acc[c];
+    for (int c = 0; c < E; ++c) red[wave][E * lane + c] = acc[c];
     if (lane == 0) red[wave][D] = L;
     __syncthreads();
     if (threadIdx.x >= D) return;
     L = (red[0][D] + red[1][D]) + (red[2][D] + red[3][D]);
     const float o = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-    a.out[(size_t)(p.q0 + i) * a.out_stride + (size_t)head * D + threadIdx.x] = L > 0.0f || L != L ? o / L : 0.0f;
+    dst[threadIdx.x] = L > 0.0f || L != L ? o / L : 0.0f;
 }
 
 template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) * sizeof(float); }
@@ -653,7 +673,9 @@ hipError_t launch(const AttnArgs &a, hipStream_t stream) {
     else hipLaunchKernelGGL((attn_rows_kernel<D, true>), grid, dim3(256), attn_lds<D>(), stream, a);
     hipError_t e = hipGetLastError();
     if (e != hipSuccess || a.splits == 1) return e;
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3(a.max_q * a.n_heads, a.n_seq), dim3(256), 0, stream, a, a.rows);
+    const uint32_t rows = a.max_q * a.n_heads;
+    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<D, true>), dim3(rows, a.n_seq), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL((attn_join_kernel<D, false>), dim3((rows + 3) / 4, a.n_seq), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
