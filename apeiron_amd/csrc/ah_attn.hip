@@ -451,32 +451,38 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
         }
     };
     const Masks mk;
+    // the share's conversions, in steps small enough to stand between two products
+    constexpr int kSpreads = D == 64 ? 4 : 6 * NS;
+    auto spread_k = [&](uint8_t *buf, int i, int w) {
+        const uint32_t u = unit_at(i), ch = u % NU, t32 = 32 * (u / NU);
+        const uint32_t half = D == 64 ? w >> 1 : D == 128 ? ch : ch >> 1;
+        const uint32_t chan = D == 64 ? kq * 16 + 8 * (w & 1) : D == 128 ? kq * 32 + 8 * w : kq * 64 + (ch & 1) * 32 + 8 * w;
+        const f16x8 v = k_frag(kw[i][w], pair_of(half ? kd[i] >> 16 : kd[i]), mk);
+        __builtin_memcpy(buf + (t32 + 16 * half + kr) * Lds::kK + 2 * chan, &v, 16);
+    };
+    auto spread_v = [&](uint8_t *buf, int i, int b) {
+        const uint32_t u = unit_at(i), ch = u % NU, t32 = 32 * (u / NU);
+        f16x8 even, odd;
+        v_frags(vw[i][2 * b], vw[i][2 * b + 1], vd[i][b], mk, even, odd);
+        uint8_t *to = buf + 64 * Lds::kK + 2 * (16 * (2 * ch + b) + kr) * Lds::kV + 2 * (t32 + (kq & 1) * 8 + (kq >> 1) * 4);
+        __builtin_memcpy(to, &even, 8);  // half-tile 0's four tokens, then half-tile 1's
+        __builtin_memcpy(to + 32, reinterpret_cast<const char *>(&even) + 8, 8);
+        __builtin_memcpy(to + Lds::kV, &odd, 8);
+        __builtin_memcpy(to + Lds::kV + 32, reinterpret_cast<const char *>(&odd) + 8, 8);
+    };
+    auto spread_step = [&](uint8_t *buf, int n) {
+        if (D == 64) {
+            if (do_k) spread_k(buf, 0, n);
+            else if (n < 2) spread_v(buf, 0, n);
+        } else {
+            const int i = n / 6, k = n % 6;
+            if (k < 4) spread_k(buf, i, k);
+            else spread_v(buf, i, k - 4);
+        }
+    };
     auto spread = [&](uint8_t *buf) {
 #pragma unroll
-        for (int i = 0; i < NS; ++i) {
-            const uint32_t u = unit_at(i), ch = u % NU, t32 = 32 * (u / NU);
-            if (do_k) {
-#pragma unroll
-                for (int w = 0; w < 4; ++w) {
-                    const uint32_t half = D == 64 ? w >> 1 : D == 128 ? ch : ch >> 1;
-                    const uint32_t chan = D == 64 ? kq * 16 + 8 * (w & 1) : D == 128 ? kq * 32 + 8 * w : kq * 64 + (ch & 1) * 32 + 8 * w;
-                    const f16x8 v = k_frag(kw[i][w], pair_of(half ? kd[i] >> 16 : kd[i]), mk);
-                    __builtin_memcpy(buf + (t32 + 16 * half + kr) * Lds::kK + 2 * chan, &v, 16);
-                }
-            }
-            if (do_v) {
-#pragma unroll
-                for (int b = 0; b < 2; ++b) {
-                    f16x8 even, odd;
-                    v_frags(vw[i][2 * b], vw[i][2 * b + 1], vd[i][b], mk, even, odd);
-                    uint8_t *to = buf + 64 * Lds::kK + 2 * (16 * (2 * ch + b) + kr) * Lds::kV + 2 * (t32 + (kq & 1) * 8 + (kq >> 1) * 4);
-                    __builtin_memcpy(to, &even, 8);  // half-tile 0's four tokens, then half-tile 1's
-                    __builtin_memcpy(to + 32, reinterpret_cast<const char *>(&even) + 8, 8);
-                    __builtin_memcpy(to + Lds::kV, &odd, 8);
-                    __builtin_memcpy(to + Lds::kV + 32, reinterpret_cast<const char *>(&odd) + 8, 8);
-                }
-            }
-        }
+        for (int n = 0; n < kSpreads; ++n) spread_step(buf, n);
     };
 
     f32x16 acc[NN];
@@ -519,73 +525,144 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
             const int32_t first0 = (int32_t)(32 * tile_of(ti)), first1 = (int32_t)(32 * tile_of(ti + 1 < t1 ? ti + 1 : ti));
             // a wave whose rows all stand before the tile (a causal mask) only helps to load
             const bool work = any && (first0 <= hi || first1 <= hi);
-            f32x16 sc[2];
+            uint8_t *other = tile_lds + (at ^ 1) * Lds::kBytes;
             if (work) {
-                sc[0] = sc[1] = (f32x16)0.0f;
-#pragma unroll
-                for (int k = 0; k < NK; ++k) {
-#pragma unroll
-                    for (int j = 0; j < 2; ++j) {
-                        f16x8 kf;
-                        __builtin_memcpy(&kf, buf + (32 * j + c) * Lds::kK + 2 * (16 * k + 8 * h), 16);
-                        sc[j] = mfma32(kf, qh[k], sc[j]);
-                        sc[j] = mfma32(kf, ql[k], sc[j]);
-                    }
-                }
-            }
-            if (ti + 2 < t1) spread(tile_lds + (at ^ 1) * Lds::kBytes);
-            const uint32_t bad_next = bad;
-            if (ti + 4 < t1) fetch(ti + 4);
-            if (work) {
-#pragma unroll
-                for (int j = 0; j < 2; ++j) {
+                // Two halves of 32 keys, their matrix and vector work side by side: the exponentials of one half
+                // stand between the products K q of the other, those of the other between the products P V of the
+                // first, and the next tile's conversion between the last products.  (Past the last tile that
+                // converts what is left in the registers into a buffer that nobody reads.)
+                f32x16 sc[2];
+                uint32_t ph[8], pl[8], pn[8], pm[8];  // f16 pairs
+                auto k_read = [&](int j, int k) {
+                    f16x8 v;
+                    __builtin_memcpy(&v, buf + (32 * j + c) * Lds::kK + 2 * (16 * k + 8 * h), 16);
+                    return v;
+                };
+                auto v_read = [&](int g, int n) {
+                    f16x8 v;
+                    __builtin_memcpy(&v, buf + 64 * Lds::kK + (32 * n + c) * Lds::kV + 2 * (16 * g + 8 * h), 16);
+                    return v;
+                };
+                auto mask = [&](int j) {
                     const int32_t first = j ? first1 : first0;
                     const bool ok = !(bad_now >> j & 1u);
-                    const bool whole = ok && first + 31 <= lo && (first >= low_all || first + 32 <= sink_key);
-                    if (!whole) {
-                        const int32_t top_key = ok ? pos : -1;
+                    if (ok && first + 31 <= lo && (first >= low_all || first + 32 <= sink_key)) return;
+                    const int32_t top_key = ok ? pos : -1;
 #pragma unroll
-                        for (int i = 0; i < 16; ++i) {
-                            const int32_t key = first + 8 * (i >> 2) + 4 * (int32_t)h + (i & 3);
-                            const bool see = key <= top_key && (key >= low_key || key < sink_key);
-                            sc[j][i] = see ? sc[j][i] : -__builtin_inff();
-                        }
+                    for (int i = 0; i < 16; ++i) {
+                        const int32_t key = first + 8 * (i >> 2) + 4 * (int32_t)h + (i & 3);
+                        const bool see = key <= top_key && (key >= low_key || key < sink_key);
+                        sc[j][i] = see ? sc[j][i] : -__builtin_inff();
                     }
-                }
-                float top = sc[0][0];
+                };
+                auto follow = [&](int j) {  // the running maximum
+                    float top = sc[j][0];
 #pragma unroll
-                for (int i = 1; i < 32; ++i) top = __builtin_fmaxf(top, sc[i >> 4][i & 15]);
-                top *= f;
-                if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0ull) {
+                    for (int i = 1; i < 16; ++i) top = __builtin_fmaxf(top, sc[j][i]);
+                    top *= f;
+                    if (__builtin_amdgcn_ballot_w64(top > m + kSlack) == 0ull) return;
                     const float up = __builtin_fmaxf(m, __builtin_fmaxf(top, xor_lanes(top, 32))), alpha = __builtin_amdgcn_exp2f(m - up);
                     m = up;
                     l *= alpha;
 #pragma unroll
                     for (int n = 0; n < NN; ++n) acc[n] *= alpha;
+                };
+                // (the empty asm keeps a pair between the products it is written between: the compiler would gather
+                // all of them where they are used)
+                auto exp_pair = [&](int j, int i, float base, uint32_t &hi2, uint32_t &lo2) {
+                    const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][2 * i], f, base));
+                    const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][2 * i + 1], f, base));
+                    l += e0;
+                    l += e1;
+                    const f16x2 t = pack16(e0, e1);
+                    hi2 = __builtin_bit_cast(uint32_t, t);
+                    lo2 = __builtin_bit_cast(uint32_t, pack16(__builtin_fmaf((float)t[0], -1.0f, e0), __builtin_fmaf((float)t[1], -1.0f, e1)));
+                    __asm__ volatile("" : "+v"(hi2), "+v"(lo2), "+v"(l));
+                };
+                auto frag = [](const uint32_t *v) { return __builtin_bit_cast(f16x8, (u32x4){v[0], v[1], v[2], v[3]}); };
+                sc[0] = sc[1] = (f32x16)0.0f;
+                f16x8 kf = k_read(0, 0);
+#pragma unroll
+                for (int k = 0; k < NK; ++k) {
+                    const f16x8 next = k + 1 < NK ? k_read(0, k + 1) : k_read(1, 0);
+                    sc[0] = mfma32(kf, qh[k], sc[0]);
+                    sc[0] = mfma32(kf, ql[k], sc[0]);
+                    kf = next;
                 }
-                const float base = kUp - m;
+                mask(0);
+                follow(0);
+                const float base0 = kUp - m;
+                f16x8 vf;
 #pragma unroll
-                for (int g = 0; g < 4; ++g) {  // 16 tokens
-                    f16x2 ph[4], pl[4];
+                for (int k = 0; k < NK; ++k) {
+                    f16x8 next;
+                    if (k + 1 < NK) next = k_read(1, k + 1);
+                    else vf = v_read(0, 0);
+                    sc[1] = mfma32(kf, qh[k], sc[1]);
+                    sc[1] = mfma32(kf, ql[k], sc[1]);
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) {
-                        const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + 2 * i], f, base));
-                        const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[g >> 1][8 * (g & 1) + 2 * i + 1], f, base));
-                        l += e0;
-                        l += e1;
-                        ph[i] = pack16(e0, e1);
-                        pl[i] = pack16(e0 - (float)ph[i][0], e1 - (float)ph[i][1]);
-                    }
-                    const f16x8 pf = join8(ph[0], ph[1], ph[2], ph[3]), pg = join8(pl[0], pl[1], pl[2], pl[3]);
-#pragma unroll
-                    for (int n = 0; n < NN; ++n) {
-                        f16x8 vf;
-                        __builtin_memcpy(&vf, buf + 64 * Lds::kK + (32 * n + c) * Lds::kV + 2 * (16 * g + 8 * h), 16);
-                        acc[n] = mfma32(vf, pf, acc[n]);
-                        acc[n] = mfma32(vf, pg, acc[n]);
-                    }
+                    for (int i = 8 * k / NK; i < 8 * (k + 1) / NK; ++i) exp_pair(0, i, base0, ph[i], pl[i]);
+                    if (k + 1 < NK) kf = next;
+                    __builtin_amdgcn_sched_barrier(0);
                 }
+                mask(1);
+                // p of the first half was taken at the maximum so far: a new one scales its product with the rest
+                f16x8 pf[2], pg[2];
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    pf[g] = frag(ph + 4 * g);
+                    pg[g] = frag(pl + 4 * g);
+                }
+                float top1 = sc[1][0];
+#pragma unroll
+                for (int i = 1; i < 16; ++i) top1 = __builtin_fmaxf(top1, sc[1][i]);
+                top1 *= f;
+                const bool moves = __builtin_amdgcn_ballot_w64(top1 > m + kSlack) != 0ull;
+                float alpha = 1.0f;
+                if (moves) {
+                    const float up = __builtin_fmaxf(m, __builtin_fmaxf(top1, xor_lanes(top1, 32)));
+                    alpha = __builtin_amdgcn_exp2f(m - up);
+                    m = up;
+                    l *= alpha;
+                }
+                const float base1 = kUp - m;
+#pragma unroll
+                for (int q = 0; q < 2 * NN; ++q) {
+                    const int g = q / NN, n = q % NN;
+                    const f16x8 next = q + 1 < 2 * NN ? v_read((q + 1) / NN, (q + 1) % NN) : v_read(2, 0);
+                    acc[n] = mfma32(vf, pf[g], acc[n]);
+                    acc[n] = mfma32(vf, pg[g], acc[n]);
+#pragma unroll
+                    for (int i = 8 * q / (2 * NN); i < 8 * (q + 1) / (2 * NN); ++i) exp_pair(1, i, base1, pn[i], pm[i]);
+                    vf = next;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+                if (moves) {
+#pragma unroll
+                    for (int n = 0; n < NN; ++n) acc[n] *= alpha;
+                }
+#pragma unroll
+                for (int g = 0; g < 2; ++g) {
+                    pf[g] = frag(pn + 4 * g);
+                    pg[g] = frag(pm + 4 * g);
+                }
+#pragma unroll
+                for (int q = 0; q < 2 * NN; ++q) {
+                    const int g = q / NN, n = q % NN;
+                    f16x8 next;
+                    if (q + 1 < 2 * NN) next = v_read(2 + (q + 1) / NN, (q + 1) % NN);
+                    acc[n] = mfma32(vf, pf[g], acc[n]);
+                    acc[n] = mfma32(vf, pg[g], acc[n]);
+#pragma unroll
+                    for (int i = kSpreads * q / (2 * NN); i < kSpreads * (q + 1) / (2 * NN); ++i) spread_step(other, i);
+                    if (q + 1 < 2 * NN) vf = next;
+                    __builtin_amdgcn_sched_barrier(0);
+                }
+            } else {
+                spread(other);
             }
+            const uint32_t bad_next = bad;
+            if (ti + 4 < t1) fetch(ti + 4);
             bad_now = bad_next;
             __syncthreads();
         }
