@@ -247,9 +247,13 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
         const size_t seen = (p->window + a.max_q + 31) / 32 + 1 + (p->sinks + 31) / 32;
         tiles = tiles < seen ? tiles : seen;
     }
-    a.rows = a.max_q * a.group <= 8 ? 8 : a.max_q * a.group < 64 ? 16 : 128;
+    // The kernel: 8 packed rows or 16 rows a workgroup, or 128 over tiles in LDS.  Those pay past 32 rows and past
+    // 64 units of 16 rows in all: below, a workgroup's longer start shows (one sequence of 2000 keys, 2 KV heads of
+    // 128, 126 rows each: 21 us against 12; 512 rows, 64 units: 24 against 23; 8 sequences of 126 rows: 25 against 34).
+    const size_t unit_rows = (size_t)a.max_q * a.group, units = (unit_rows + 15) / 16 * kv * p->n_seq;
+    a.rows = unit_rows <= 8 ? 8 : unit_rows <= 32 || units <= 64 ? 16 : 128;
     const size_t base = ((size_t)a.max_q * a.group + a.rows - 1) / a.rows * kv * p->n_seq, rows = p->n_tok * p->n_heads;
-    size_t splits = (a.rows == 128 ? 768 : kAttnGroups) / base, fit = a.rows == 128 ? (tiles + 7) / 8 : (tiles + 3) / 4;
+    size_t splits = (a.rows == 128 ? 1100 : kAttnGroups) / base, fit = a.rows == 128 ? (tiles + 7) / 8 : (tiles + 3) / 4;
     const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float));
     splits = splits < fit ? splits : fit;
     splits = splits < room ? splits : room;

@@ -385,8 +385,9 @@ template <int D> struct TileLds {
     static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;
 };
 template <int D>
-__global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
     constexpr int NK = D / 16, NN = D / 32, NU = D / 64;  // contraction steps of K q; channel blocks; 16-byte units
+    constexpr int kAhead = D == 256 ? 3 : 1;  // more, where the registers do not cost a wave per SIMD
     typedef TileLds<D> Lds;
     extern __shared__ uint8_t tile_lds[];
     const uint32_t lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
@@ -580,29 +581,34 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
                     __asm__ volatile("" : "+v"(hi2), "+v"(lo2), "+v"(l));
                 };
                 auto frag = [](const uint32_t *v) { return __builtin_bit_cast(f16x8, (u32x4){v[0], v[1], v[2], v[3]}); };
+                // One stream of fragments from LDS, read kAhead steps before its two products: the halves' K rows, then
+                // the channels of V for 16 tokens after 16.
+                constexpr int kK = 2 * NK, kAll = kK + 4 * NN, kRing = kAhead + 1;
+                f16x8 ring[kRing];
+                auto read = [&](int i) {
+                    if (i < kK) ring[i % kRing] = k_read(i / NK, i % NK);
+                    else if (i < kAll) ring[i % kRing] = v_read((i - kK) / NN, (i - kK) % NN);
+                };
+#pragma unroll
+                for (int i = 0; i < kAhead; ++i) read(i);
                 sc[0] = sc[1] = (f32x16)0.0f;
-                f16x8 kf = k_read(0, 0);
 #pragma unroll
                 for (int k = 0; k < NK; ++k) {
-                    const f16x8 next = k + 1 < NK ? k_read(0, k + 1) : k_read(1, 0);
-                    sc[0] = mfma32(kf, qh[k], sc[0]);
-                    sc[0] = mfma32(kf, ql[k], sc[0]);
-                    kf = next;
+                    read(k + kAhead);
+                    sc[0] = mfma32(ring[k % kRing], qh[k], sc[0]);
+                    sc[0] = mfma32(ring[k % kRing], ql[k], sc[0]);
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 mask(0);
                 follow(0);
                 const float base0 = kUp - m;
-                f16x8 vf;
 #pragma unroll
                 for (int k = 0; k < NK; ++k) {
-                    f16x8 next;
-                    if (k + 1 < NK) next = k_read(1, k + 1);
-                    else vf = v_read(0, 0);
-                    sc[1] = mfma32(kf, qh[k], sc[1]);
-                    sc[1] = mfma32(kf, ql[k], sc[1]);
+                    read(NK + k + kAhead);
+                    sc[1] = mfma32(ring[(NK + k) % kRing], qh[k], sc[1]);
+                    sc[1] = mfma32(ring[(NK + k) % kRing], ql[k], sc[1]);
 #pragma unroll
                     for (int i = 8 * k / NK; i < 8 * (k + 1) / NK; ++i) exp_pair(0, i, base0, ph[i], pl[i]);
-                    if (k + 1 < NK) kf = next;
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 mask(1);
@@ -629,12 +635,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
 #pragma unroll
                 for (int q = 0; q < 2 * NN; ++q) {
                     const int g = q / NN, n = q % NN;
-                    const f16x8 next = q + 1 < 2 * NN ? v_read((q + 1) / NN, (q + 1) % NN) : v_read(2, 0);
-                    acc[n] = mfma32(vf, pf[g], acc[n]);
-                    acc[n] = mfma32(vf, pg[g], acc[n]);
+                    read(kK + q + kAhead);
+                    acc[n] = mfma32(ring[(kK + q) % kRing], pf[g], acc[n]);
+                    acc[n] = mfma32(ring[(kK + q) % kRing], pg[g], acc[n]);
 #pragma unroll
                     for (int i = 8 * q / (2 * NN); i < 8 * (q + 1) / (2 * NN); ++i) exp_pair(1, i, base1, pn[i], pm[i]);
-                    vf = next;
                     __builtin_amdgcn_sched_barrier(0);
                 }
                 if (moves) {
@@ -649,13 +654,11 @@ __global__ void __launch_bounds__(256, D == 256 ? 1 : 2) attn_tile_kernel(AttnAr
 #pragma unroll
                 for (int q = 0; q < 2 * NN; ++q) {
                     const int g = q / NN, n = q % NN;
-                    f16x8 next;
-                    if (q + 1 < 2 * NN) next = v_read(2 + (q + 1) / NN, (q + 1) % NN);
-                    acc[n] = mfma32(vf, pf[g], acc[n]);
-                    acc[n] = mfma32(vf, pg[g], acc[n]);
+                    read(kK + 2 * NN + q + kAhead);
+                    acc[n] = mfma32(ring[(kK + 2 * NN + q) % kRing], pf[g], acc[n]);
+                    acc[n] = mfma32(ring[(kK + 2 * NN + q) % kRing], pg[g], acc[n]);
 #pragma unroll
                     for (int i = kSpreads * q / (2 * NN); i < kSpreads * (q + 1) / (2 * NN); ++i) spread_step(other, i);
-                    if (q + 1 < 2 * NN) vf = next;
                     __builtin_amdgcn_sched_barrier(0);
                 }
             } else {
