@@ -998,6 +998,8 @@ int32_t ah_init(int32_t device, ah_ctx **out) {
     ctx->cu_count = prop.multiProcessorCount > 0 ? prop.multiProcessorCount : 256;
     if (hipSetDevice(device) != hipSuccess || hipStreamCreate(&ctx->stream) != hipSuccess ||
         hipMalloc(&ctx->d_status, 2 * sizeof(unsigned long long)) != hipSuccess ||
+        hipMalloc(&ctx->d_count, kCounts * sizeof(uint32_t)) != hipSuccess ||
+        hipMemset(ctx->d_count, 0, kCounts * sizeof(uint32_t)) != hipSuccess ||
         ah_gemv_init_attrs() != hipSuccess || ah_few_init_attrs() != hipSuccess || ah_attn_init_attrs() != hipSuccess) {
         delete ctx;
         return AH_ERR_HIP;
@@ -1007,6 +1009,7 @@ int32_t ah_init(int32_t device, ah_ctx **out) {
     if (se != hipSuccess || !sp || reset_status(ctx) != AH_OK) {
         ctx->last_hip = (int)se;
         (void)hipFree(ctx->d_status);
+        (void)hipFree(ctx->d_count);
         (void)hipStreamDestroy(ctx->stream);
         delete ctx;
         return AH_ERR_HIP;
@@ -1023,6 +1026,7 @@ int32_t ah_destroy(ah_ctx *ctx) {
     if (ctx->scratch) (void)hipFree(ctx->scratch);
     if (ctx->ffn_buf) (void)hipFree(ctx->ffn_buf);
     (void)hipFree(ctx->d_status);
+    (void)hipFree(ctx->d_count);
     (void)hipStreamDestroy(ctx->stream);
     delete ctx;
     return AH_OK;

@@ -9,7 +9,8 @@
 namespace {
 
 constexpr size_t kMaxU32 = 0x7fffffff;
-constexpr size_t kAttnGroups = 2048;
+constexpr size_t kAttnGroups = 2048;  // (ah_ctx::d_count has an entry for every unit that is split)
+////static_assert(kAttnGroups / 2 <= kCounts, "units of at least two pieces");
 
 bool tokens_ok(const ah_kv4_tokens *t) {
     return t->d_seq && t->d_pos && t->d_table && t->n_seq && t->table_stride && t->n_tok <= kMaxU32 && t->n_seq <= kMaxU32 &&
@@ -238,8 +239,6 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     a.scale = p->scale;
     a.status = ctx->d_status;
     if ((uint64_t)a.max_q * a.group > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
-    // Pieces of the context: up to kAttnGroups workgroups in all, each with at least a tile a wave.  The bound
-    // counts every sequence as the longest; of uneven ones about half the workgroups have work.
     const size_t most = p->table_stride << cache->ref.page_shift;
     const size_t ctx_len = p->max_ctx < most ? p->max_ctx : most;
     size_t tiles = (ctx_len + 31) / 32;
@@ -253,16 +252,41 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     const size_t unit_rows = (size_t)a.max_q * a.group, units = (unit_rows + 15) / 16 * kv * p->n_seq;
     a.rows = unit_rows <= 8 ? 8 : unit_rows <= 32 || units <= 64 ? 16 : 128;
     const size_t base = ((size_t)a.max_q * a.group + a.rows - 1) / a.rows * kv * p->n_seq, rows = p->n_tok * p->n_heads;
-    size_t splits = (a.rows == 128 ? 1100 : kAttnGroups) / base, fit = a.rows == 128 ? (tiles + 7) / 8 : (tiles + 3) / 4;
-    const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float));
-    splits = splits < fit ? splits : fit;
-    splits = splits < room ? splits : room;
-    splits = splits < 1 ? 1 : splits;
-    size_t chunk = ((tiles + splits - 1) / splits + 3) / 4 * 4;  // whole rounds of the four waves
+    size_t chunk;
+    if (a.rows == 128) {
+        // about four workgroups a CU, of at least eight tiles; none where the rows alone come near two a CU (8192
+        // tokens of 12 heads, 768 workgroups: 392 us, in two pieces each 577)
+        size_t splits = base >= 400 ? 1 : 1100 / base;
+        splits = splits < (tiles + 7) / 8 ? splits : (tiles + 7) / 8;
+        splits = splits < 1 ? 1 : splits;
+        chunk = (tiles + splits - 1) / splits;
+    } else {
+        // With few units a piece's tiles (0.7 us for each of a wave) stand against the join (0.1 us a piece):
+        // sqrt(1.75 tiles) pieces, past 40 of them two joins and 16 tiles a piece.  Once that passes a
+        // workgroup a CU, pieces of 16 tiles (a workgroup costs its start and end).  One sequence of 4001 keys
+        // in pieces of 4, 8, 16 and 24 tiles 10.6, 10.0, 10.7 and 13.3 us, 16 windows of 4096 15.1, 11.7, 10.6 and
+        // 11.6, 128 sequences of 1000 24, 19, 16 and 16.
+        const double wish = std::sqrt(1.75 * (double)tiles);
+        double pieces = wish <= 40.0 ? wish : (double)tiles / 16.0;
+        if (pieces * (double)base > 256.0) {
+            const double most_pieces = (double)(kAttnGroups / base), by_tiles = (double)tiles / 16.0;
+            pieces = by_tiles < most_pieces ? by_tiles : most_pieces;
+            pieces = pieces * (double)base > 256.0 ? pieces : 256.0 / (double)base;
+        }
+        chunk = pieces < 1.0 ? tiles : 4 * (size_t)((double)tiles / (4.0 * pieces) + 0.5);  // whole rounds of the four waves
+    }
+    const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float)), least = room < 1 ? tiles : (tiles + room - 1) / room;
+    const size_t most_groups = base <= kAttnGroups / 2 ? kAttnGroups / base : 1;
+    chunk = chunk < least ? least : chunk;
+    if (a.rows != 128) {
+        const size_t fit = (tiles + most_groups - 1) / most_groups;
+        chunk = chunk < fit ? fit : chunk;
+    }
     chunk = chunk < 1 ? 1 : chunk;
     a.chunk = (uint32_t)chunk;
     a.splits = (uint32_t)((tiles + chunk - 1) / chunk);
     a.splits = a.splits < 1 ? 1 : a.splits;
+    a.join = a.splits <= 40 ? a.splits : (uint32_t)std::ceil(std::sqrt((double)a.splits));
     AH_HIP(ctx, hipSetDevice(ctx->device));
     if (a.splits > 1) {
         const size_t o = align256(a.splits * rows * dim * sizeof(float));
@@ -270,6 +294,7 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
         if (st) return st;
         a.part_o = static_cast<float *>(ctx->scratch);
         a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch) + o);
+        a.count = ctx->d_count;
     }
     AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
     return AH_OK;

@@ -11,9 +11,14 @@ namespace {
 
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x4 __attribute__((ext_vector_type(4)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
 typedef float f32x16 __attribute__((ext_vector_type(16)));
 
+// Cache policy of the partial results that one workgroup writes and another reads in the same launch: device
+// scope (sc1), past the XCDs' own L2s.
+constexpr int kDevice = 16;
 constexpr float kLog2e = 1.44269504088896340736f;
 constexpr float kNoMax = -3.402823466e38f;  // below every finite score
 // The running maximum follows the scores only when one passes it by more than this (in powers of two):
@@ -341,37 +346,96 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnAr
         if (!low) __builtin_memcpy(red_o + (wave * 16 + r) * (D + 4) + 32 * g + 8 * h, o, 32);
     }
     __syncthreads();
-    const uint32_t rr = threadIdx.x >> 4, row_out = row0 + rr;
-    if (rr >= R || row_out >= rows) return;
-    float M = kNoMax, L = 0.0f, w4[4];
+    const uint32_t pieces = T.count ? (T.count + chunk - 1) / chunk : 1;
+    const size_t all = (size_t)a.n_tok * a.n_heads;
+    auto flat_of = [&](uint32_t rw) { return (size_t)(p.q0 + rw / a.group) * a.n_heads + kvh * a.group + rw % a.group; };
+    auto out_of = [&](uint32_t rw) { return a.out + (size_t)(p.q0 + rw / a.group) * a.out_stride + (size_t)(kvh * a.group + rw % a.group) * D; };
+    const uint32_t n_rows = last - row0 + 1;
+    const __amdgpu_buffer_rsrc_t po = ah_rsrc(a.part_o, (uint32_t)(a.splits * all * D * 4)), pm = ah_rsrc(a.part_ml, (uint32_t)(a.splits * all * 8));
+    {
+        const uint32_t rr = threadIdx.x >> 4;
+        if (rr < n_rows) {
+            float M = kNoMax, L = 0.0f, w4[4];
 #pragma unroll
-    for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, red_m[w * 16 + rr]);
+            for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, red_m[w * 16 + rr]);
 #pragma unroll
-    for (int w = 0; w < 4; ++w) {
-        w4[w] = __builtin_amdgcn_exp2f(red_m[w * 16 + rr] - M);
-        L += red_l[w * 16 + rr] * w4[w];
-    }
-    const uint32_t tok_out = p.q0 + row_out / a.group, head_out = kvh * a.group + row_out % a.group;
-    const size_t flat = (size_t)tok_out * a.n_heads + head_out;
-    const float inv = a.splits > 1 ? 1.0f : L > 0.0f || L != L ? 1.0f / L : 0.0f;
-    float *dst = a.splits > 1 ? a.part_o + ((size_t)split * a.n_tok * a.n_heads + flat) * D
-                              : a.out + (size_t)tok_out * a.out_stride + (size_t)head_out * D;
-    for (uint32_t c = 4 * (threadIdx.x & 15); c < (uint32_t)D; c += 64) {
-        f32x4 o = (f32x4)0.0f;
+            for (int w = 0; w < 4; ++w) {
+                w4[w] = __builtin_amdgcn_exp2f(red_m[w * 16 + rr] - M);
+                L += red_l[w * 16 + rr] * w4[w];
+            }
+            const float inv = pieces > 1 ? 1.0f : L > 0.0f || L != L ? 1.0f / L : 0.0f;
+            const size_t at = split * all + flat_of(row0 + rr);
+            for (uint32_t c = 4 * (threadIdx.x & 15); c < (uint32_t)D; c += 64) {
+                f32x4 o = (f32x4)0.0f;
 #pragma unroll
-        for (int w = 0; w < 4; ++w) {
-            f32x4 y;
-            __builtin_memcpy(&y, red_o + (w * 16 + rr) * (D + 4) + c, 16);
-            o += y * w4[w];
+                for (int w = 0; w < 4; ++w) {
+                    f32x4 y;
+                    __builtin_memcpy(&y, red_o + (w * 16 + rr) * (D + 4) + c, 16);
+                    o += y * w4[w];
+                }
+                o *= inv;
+                if (pieces > 1) __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), po, (int)(4 * (at * D + c)), 0, kDevice);
+                else __builtin_memcpy(out_of(row0 + rr) + c, &o, 16);
+            }
+            if (pieces > 1 && (threadIdx.x & 15) == 0)
+                __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2){M, L}), pm, (int)(8 * at), 0, kDevice);
         }
-        o *= inv;
-        __builtin_memcpy(dst + c, &o, 16);
     }
-    if (a.splits > 1 && (threadIdx.x & 15) == 0) {
-        float *ml = a.part_ml + 2 * ((size_t)split * a.n_tok * a.n_heads + flat);
-        ml[0] = M;
-        ml[1] = L;
+    if (pieces == 1) return;
+    // The pieces are joined in groups of a.join and the groups then into one, each by the workgroup that arrives
+    // last: it finds the others' partial results complete (device-scope stores, waited for before the count) and
+    // reads them with device-scope loads.  One workgroup reads a piece's rows in about 0.1 us, so two levels of
+    // sqrt(pieces) keep a long context's join near the time of a tile.  Counters are left at zero for the next call.
+    constexpr uint32_t kLanes = D / 4;  // of a row, 16 bytes each
+    auto arrive = [&](uint32_t *counter, uint32_t of) {  // whether this workgroup is the last of them
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        if (threadIdx.x == 0) {
+            const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (n == of - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            red_m[0] = __builtin_bit_cast(float, n);
+        }
+        __syncthreads();
+        return __builtin_bit_cast(uint32_t, red_m[0]) == of - 1;
+    };
+    // pieces first, first + step, ..: to the output, or as one piece in the first one's place
+    auto join = [&](uint32_t first, uint32_t step, uint32_t n, bool out) {
+        for (uint32_t rr = threadIdx.x / kLanes; rr < n_rows; rr += 256 / kLanes) {
+            const uint32_t gl = threadIdx.x % kLanes;
+            const size_t flat = flat_of(row0 + rr);
+            float M = kNoMax;
+            for (uint32_t k = gl; k < n; k += kLanes)
+                M = __builtin_fmaxf(M, __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(pm, (int)(8 * ((first + k * step) * all + flat)), 0, kDevice)));
+#pragma unroll
+            for (uint32_t o = 1; o < kLanes; o <<= 1) M = __builtin_fmaxf(M, xor_lanes(M, (int)o));
+            float L = 0.0f;
+            f32x4 sum = (f32x4)0.0f;
+#pragma unroll 8
+            for (uint32_t k = 0; k < n; ++k) {
+                const size_t at = (first + k * step) * all + flat;
+                const f32x2 ml = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(pm, (int)(8 * at), 0, kDevice));
+                const f32x4 o = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(po, (int)(4 * (at * D + 4 * gl)), 0, kDevice));
+                const float w = __builtin_amdgcn_exp2f(ml[0] - M);
+                L += ml[1] * w;
+                sum += o * w;
+            }
+            if (out) {
+                sum *= L > 0.0f || L != L ? 1.0f / L : 0.0f;
+                __builtin_memcpy(out_of(row0 + rr) + 4 * gl, &sum, 16);
+            } else {
+                const size_t at = first * all + flat;
+                __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, sum), po, (int)(4 * (at * D + 4 * gl)), 0, kDevice);
+                if (gl == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2){M, L}), pm, (int)(8 * at), 0, kDevice);
+            }
+        }
+    };
+    const uint32_t group = split / a.join, first = group * a.join, groups = (pieces + a.join - 1) / a.join;
+    const uint32_t members = first + a.join <= pieces ? a.join : pieces - first;
+    if (members > 1) {
+        if (!arrive(a.count + units + unit * ((a.splits + a.join - 1) / a.join) + group, members)) return;
+        join(first, 1, members, groups == 1);
     }
+    if (groups > 1 && arrive(a.count + unit, groups)) join(0, a.join, groups, true);
 }
 
 // Chunks of tokens: 128 rows (token, head of the group) a workgroup, 32 a wave as the columns of 32x32 products,
@@ -689,16 +753,14 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     }
 }
 
-// Joins the pieces of a context.  WIDE: a workgroup per row (token, head), its waves every fourth piece, for a few
-// rows in many pieces; otherwise a wave per row.  A piece past the row's keys was never written; which those
-// are follows from the same tiles_of.
-template <int D, bool WIDE>
+// Joins the pieces of attn_tile_kernel's contexts: a wave per row (token, head).  A piece past the row's keys was
+// never written; which those are follows from the same tiles_of.
+template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     constexpr int E = D / 64;  // channels of a lane
-    __shared__ float red[4][D + 1];
     const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y;
     const Span p = span_of(a, s);
-    const uint32_t n = p.nq * a.n_heads, it = WIDE ? blockIdx.x : 4 * blockIdx.x + wave;
+    const uint32_t n = p.nq * a.n_heads, it = 4 * blockIdx.x + wave;
     if (it >= n) return;
     const uint32_t i = it / a.n_heads, head = it % a.n_heads, g = a.group;
     const uint32_t row = i * g + head % g, row0 = row - row % a.rows;
@@ -715,7 +777,7 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 #pragma unroll
     for (int c = 0; c < E; ++c) acc[c] = 0.0f;
 #pragma unroll 4
-    for (uint32_t k = WIDE ? wave : 0; k < pieces; k += WIDE ? 4 : 1) {
+    for (uint32_t k = 0; k < pieces; ++k) {
         float ml[2], o[E];
         __builtin_memcpy(ml, a.part_ml + 2 * (k * all + flat), 8);
         __builtin_memcpy(o, a.part_o + (k * all + flat) * D + E * lane, 4 * E);
@@ -724,22 +786,10 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 #pragma unroll
         for (int c = 0; c < E; ++c) acc[c] += o[c] * w;
     }
-    float *dst = a.out + (size_t)(p.q0 + i) * a.out_stride + (size_t)head * D;
-    if (!WIDE) {
-        const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
 #pragma unroll
-        for (int c = 0; c < E; ++c) acc[c] *= inv;
-        __builtin_memcpy(dst + E * lane, acc, 4 * E);
-        return;
-    }
-#pragma unroll
-    for (int c = 0; c < E; ++c) red[wave][E * lane + c] = acc[c];
-    if (lane == 0) red[wave][D] = L;
-    __syncthreads();
-    if (threadIdx.x >= D) return;
-    L = (red[0][D] + red[1][D]) + (red[2][D] + red[3][D]);
-    const float o = (red[0][threadIdx.x] + red[1][threadIdx.x]) + (red[2][threadIdx.x] + red[3][threadIdx.x]);
-    dst[threadIdx.x] = L > 0.0f || L != L ? o / L : 0.0f;
+    for (int c = 0; c < E; ++c) acc[c] *= inv;
+    __builtin_memcpy(a.out + (size_t)(p.q0 + i) * a.out_stride + (size_t)head * D + E * lane, acc, 4 * E);
 }
 
 template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) * sizeof(float); }
@@ -752,10 +802,8 @@ hipError_t launch(const AttnArgs &a, hipStream_t stream) {
     else if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false>), grid, dim3(256), attn_lds<D>(), stream, a);
     else hipLaunchKernelGGL((attn_rows_kernel<D, true>), grid, dim3(256), attn_lds<D>(), stream, a);
     hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1) return e;
-    const uint32_t rows = a.max_q * a.n_heads;
-    if (a.splits > 8) hipLaunchKernelGGL((attn_join_kernel<D, true>), dim3(rows, a.n_seq), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL((attn_join_kernel<D, false>), dim3((rows + 3) / 4, a.n_seq), dim3(256), 0, stream, a);
+    if (e != hipSuccess || a.splits == 1 || a.rows != 128) return e;  // (the rows kernel joins by itself)
+    hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.max_q * a.n_heads + 3) / 4, a.n_seq), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 

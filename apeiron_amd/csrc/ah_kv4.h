@@ -123,6 +123,10 @@ struct AttnArgs {
     uint32_t splits, chunk;
     uint32_t rows;  // rows (token, head of a KV head's group) of a workgroup: 8, 16 or 128
     float *part_o, *part_ml;
+    // attn_rows_kernel's join: pieces of a group, and the arrivals (zero between calls) of every unit's groups,
+    // [unit], then of every group's pieces, [unit][group]
+    uint32_t join;
+    uint32_t *count;
     unsigned long long *status;
 };
 
