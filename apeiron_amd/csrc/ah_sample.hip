@@ -47,6 +47,7 @@ struct Row {
     float M, inv_t;
     double floor_w;
     bool bad_t, greedy, need_k, need_p;
+    bool few;  // so few tokens asked for that the segments' maxima bound them: the bins are not needed
 };
 AH_DEV Row row_of(const SampleArgs &a, uint32_t row) {
     Row r;
@@ -61,6 +62,7 @@ AH_DEV Row row_of(const SampleArgs &a, uint32_t row) {
     r.greedy = r.bad_t || r.T == 0.0f || r.k == 1;
     r.need_k = r.k > 1 && (uint32_t)r.k < r.V;
     r.need_p = r.p < 1.0f;
+    r.few = !r.greedy && r.need_k && (uint64_t)r.k * 2 <= a.segs;
     r.floor_w = (double)(r.m > 0.0f ? (r.m < 1.0f ? r.m : 1.0f) : 0.0f) * 0x1p32;
     return r;
 }
@@ -228,6 +230,33 @@ __global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
     if (nan) ah_record(a.status, ((unsigned long long)row << 8) + AH_ERR_NONFINITE_INPUT);
 }
 
+// The last bin that can hold one of the first k: every segment's (or group's) largest is a token of its own, so the
+// k-th largest of them bounds the k-th largest logit from below.  Segments do where there are twice k of them.
+AH_DEV uint32_t bound_of(const SampleArgs &a, const Row &r, uint32_t row, Scan &S, uint32_t *count, uint32_t &found) {
+    for (uint32_t i = threadIdx.x; i < kBins; i += kT) count[i] = 0;
+    if (threadIdx.x == 0) found = kBins - 1;
+    __syncthreads();
+    const uint32_t *g = r.few ? a.seg_max + (size_t)row * a.segs : a.group_max + (size_t)row * a.segs * kGroups;
+    const uint32_t n = r.few ? a.segs : a.segs * kGroups;
+    for (uint32_t i = threadIdx.x; i < n; i += kT) {
+        const uint32_t b = bin_at(z_of(r, g[i]));
+        if (b < kBins) atomicAdd(&count[b], 1u);
+    }
+    __syncthreads();
+    uint32_t c[4], total;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c[i] = count[4 * threadIdx.x + i];
+    const uint32_t mine = (c[0] + c[1]) + (c[2] + c[3]);
+    uint32_t cum = scan_u(mine, S, total) - mine;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (cum < (uint32_t)r.k && cum + c[i] >= (uint32_t)r.k) found = 4 * threadIdx.x + i;
+        cum += c[i];
+    }
+    __syncthreads();
+    return found;
+}
+
 __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
     __shared__ double mass[kBins];
     __shared__ uint32_t count[kBins];
@@ -236,36 +265,11 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
     uint32_t row, s0, s1;
     share(a, row, s0, s1);
     Row r = row_of(a, row);
-    if (r.greedy || (!r.need_k && !r.need_p)) return;
+    if (r.greedy || r.few || (!r.need_k && !r.need_p)) return;
     set_top(r, top_of(a, row, S));
     if (r.M == -__builtin_inff()) return;
-    // the last bin that can hold one of the first k: every group's largest is a token of its own
-    uint32_t last = kBins - 1;
-    if (r.need_k) {
-        for (uint32_t i = threadIdx.x; i < kBins; i += kT) count[i] = 0;
-        if (threadIdx.x == 0) found = kBins - 1;
-        __syncthreads();
-        // (few tokens asked for: the segments' are bound enough, and an eighth as many to look at)
-        const bool few = (uint64_t)r.k * 2 <= a.segs;
-        const uint32_t *g = few ? a.seg_max + (size_t)row * a.segs : a.group_max + (size_t)row * a.segs * kGroups;
-        const uint32_t n_max = few ? a.segs : a.segs * kGroups;
-        for (uint32_t i = threadIdx.x; i < n_max; i += kT) {
-            const uint32_t b = bin_at(z_of(r, g[i]));
-            if (b < kBins) atomicAdd(&count[b], 1u);
-        }
-        __syncthreads();
-        uint32_t c[4], total;
-#pragma unroll
-        for (int i = 0; i < 4; ++i) c[i] = count[4 * threadIdx.x + i];
-        uint32_t cum = scan_u((c[0] + c[1]) + (c[2] + c[3]), S, total) - ((c[0] + c[1]) + (c[2] + c[3]));
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            if (cum < (uint32_t)r.k && cum + c[i] >= (uint32_t)r.k) found = 4 * threadIdx.x + i;
-            cum += c[i];
-        }
-        __syncthreads();
-        last = found;
-    }
+    const uint32_t last = r.need_k ? bound_of(a, r, row, S, count, found) : kBins - 1;
+    __syncthreads();
     for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
         count[i] = 0;
         mass[i] = 0.0;
@@ -380,6 +384,7 @@ AH_DEV bool listed(const Limits &o, const Row &r, uint32_t b) {
 __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     __shared__ Scan S;
     __shared__ LimitsLds L;
+    __shared__ uint32_t count[kBins], found;
     uint32_t row, s0, s1;
     share(a, row, s0, s1);
     const Bins B(a, row);
@@ -387,7 +392,9 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     if (r.greedy) return;
     set_top(r, top_of(a, row, S));
     if (r.M == -__builtin_inff()) return;
-    const Limits o = limits_of(a, r, B, S, L);
+    Limits o = {0, 0, kNone, 0, 0.0, 0.0, 0.0};
+    if (r.few) o.g1 = bound_of(a, r, row, S, count, found);  // all that reaches the bound is listed
+    else o = limits_of(a, r, B, S, L);
     const uint32_t lane = threadIdx.x & 63;
     // the last bin with a token to keep or to list (no bin: tokens without weight, as a whole)
     const uint32_t end_k = o.bk != kNone ? o.bk : o.g1;
@@ -441,10 +448,10 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
 // ---- the cut ----------------------------------------------------------------------------------------
 
 struct DrawLds {
+    alignas(16) double mass[256];
+    alignas(16) uint32_t count[256];
     Scan S;
     LimitsLds L;
-    double mass[256];
-    uint32_t count[256];
     double seg[kSampleMaxSegs];
     uint32_t start[kSampleMaxSegs];
     uint32_t key[kSampleList], idx[kSampleList];
@@ -592,6 +599,64 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
     return c;
 }
 
+// The cut of at most kT / P listed tokens: P neighbouring threads a token, its place among the others by comparing
+// with each (four at a time; tokens that do not count are key 0, below every key).
+template <uint32_t P> AH_DEV Cut place_cut(const Row &r, const Limits &o, uint32_t n, bool do_k, DrawLds &D) {
+    const uint32_t t = threadIdx.x, me = t / P, part = t % P;
+    const bool live = me < n;
+    const uint32_t k = live ? D.key[me] : 0u;
+    const float z = z_of(r, k);
+    const uint32_t b = bin_at(z);
+    const bool ink = live && do_k && (r.few || b == o.bk), inp = live && b >= o.g0 && b <= o.g1;
+    const double w = live ? (double)weight_at(z) : 0.0;
+    bool keep = live;
+    if (do_k) {
+        if (part == 0) D.count[me] = ink ? k : 0u;
+        __syncthreads();
+        uint32_t rank = 0;
+#pragma unroll 2
+        for (uint32_t j = 4 * part; j < n; j += 4 * P) {
+            uint32_t other[4];
+            __builtin_memcpy(other, D.count + j, 16);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) rank += other[i] > (j + i < me ? k - 1 : k) ? 1u : 0u;
+        }
+#pragma unroll
+        for (uint32_t q = 1; q < P; q <<= 1) rank += (uint32_t)__shfl_xor((int)rank, (int)q, 64);
+        keep = ink ? o.before_k + rank < (uint32_t)r.k : live;
+    }
+    if (r.need_p) {
+        const double W = do_k || r.few ? o.mass_k + sum_d((ink || r.few) && keep && part == 0 ? w : 0.0, D.S) : o.all;
+        double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
+        goal = goal < 1.0 ? 1.0 : goal;
+        __syncthreads();
+        if (part == 0) {
+            D.count[me] = inp && keep ? k : 0u;
+            D.mass[me] = inp && keep ? w : 0.0;
+        }
+        __syncthreads();
+        double before = 0.0;
+#pragma unroll 2
+        for (uint32_t j = 4 * part; j < n; j += 4 * P) {
+            uint32_t other[4];
+            double m[4];
+            __builtin_memcpy(other, D.count + j, 16);
+            __builtin_memcpy(m, D.mass + j, 32);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) before += other[i] > (j + i < me ? k - 1 : k) ? m[i] : 0.0;
+        }
+#pragma unroll
+        for (uint32_t q = 1; q < P; q <<= 1) before += __shfl_xor(before, (int)q, 64);
+        keep = inp && keep && o.mass_0 + before < goal;
+    } else {
+        keep = ink && keep;
+    }
+    Cut c;
+    c.key = min_u(keep ? k : kNone, D.S);
+    c.last = max_u(keep && k == c.key ? D.idx[me] : 0u, D.S);
+    return c;
+}
+
 __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
     __shared__ DrawLds D;
     const uint32_t row = blockIdx.x, t = threadIdx.x;
@@ -634,8 +699,8 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         }
         return;
     }
-    const Limits o = limits_of(a, r, B, D.S, D.L);
-    const bool do_k = o.bk != kNone, limited = do_k || r.need_p;
+    Limits o = {0, kBins - 1, kNone, 0, 0.0, 0.0, 0.0};
+    if (!r.few) o = limits_of(a, r, B, D.S, D.L);
     uint32_t n;
     {  // where each segment's listed tokens start
         uint32_t at = scan_u(n_mine, D.S, n) - n_mine;
@@ -646,6 +711,8 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         }
     }
     full = max_u(full, D.S) != 0 || n > kSampleList;
+    // (of few, every listed token counts for both limits; fewer than k of them are all that have weight)
+    const bool do_k = r.few ? n >= (uint32_t)r.k : o.bk != kNone, limited = do_k || r.need_p;
     Cut c = {0, kNone};
     auto kept = [&](uint32_t i, uint32_t k) -> double {
         if (limited && (k < c.key || (k == c.key && i > c.last))) return 0.0;
@@ -658,6 +725,11 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         const auto key = [&](uint32_t i) { return key_of(r.x[i]); };
         const auto index = [](uint32_t i) { return i; };
         const auto weighs = [&](uint32_t k) { return bin_at(z_of(r, k)) < kBins; };
+        if (r.few && !do_k) {
+            double w = 0.0;
+            for (uint32_t i = t; i < r.V; i += kT) w += (double)weight_at(z_of(r, key(i)));
+            o.all = sum_d(w, D.S);
+        }
         c = select_cut(r, r.V, key, index, weighs, weighs, do_k, (uint32_t)r.k, do_k ? 0.0 : o.all, 0.0, D);
         __syncthreads();
         for (uint32_t s = t >> 6; s < a.segs; s += kT / 64) {
@@ -683,47 +755,11 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
         __syncthreads();
         const auto bin = [&](uint32_t k) { return bin_at(z_of(r, k)); };
         if (n <= kT) {
-            // a token a thread, its place among the others by comparing with each
-            const bool live = t < n;
-            const uint32_t k = live ? D.key[t] : 0u, b = bin(k);
-            const bool ink = live && do_k && b == o.bk, inp = live && b >= o.g0 && b <= o.g1;
-
-            const double w = live ? (double)weight_at(z_of(r, k)) : 0.0;
-            bool keep = live;
-            double goal = 0.0;
-            if (do_k) {
-                D.count[t] = ink ? k : 0u;
-                __syncthreads();
-                uint32_t rank = 0;
-#pragma unroll 8
-                for (uint32_t j = 0; j < n; ++j) {
-                    const uint32_t kj = D.count[j];
-                    rank += kj > k || (kj == k && j < t) ? 1u : 0u;
-                }
-                keep = ink ? o.before_k + rank < (uint32_t)r.k : live;
-            }
-            if (r.need_p) {
-                const double W = do_k ? o.mass_k + sum_d(ink && keep ? w : 0.0, D.S) : o.all;
-                goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
-                goal = goal < 1.0 ? 1.0 : goal;
-                D.mass[t] = inp && keep ? w : 0.0;
-                __syncthreads();
-                double before = o.mass_0;
-#pragma unroll 8
-                for (uint32_t j = 0; j < n; ++j) {
-                    const uint32_t kj = D.key[j];
-                    before += kj > k || (kj == k && j < t) ? D.mass[j] : 0.0;
-                }
-                keep = inp && keep && before < goal;
-            } else {
-                keep = ink && keep;
-            }
-            c.key = min_u(keep ? k : kNone, D.S);
-            c.last = max_u(keep && k == c.key ? D.idx[t] : 0u, D.S);
+            c = n <= kT / 4 ? place_cut<4>(r, o, n, do_k, D) : n <= kT / 2 ? place_cut<2>(r, o, n, do_k, D) : place_cut<1>(r, o, n, do_k, D);
         } else {
             const auto key = [&](uint32_t i) { return D.key[i]; };
             const auto index = [&](uint32_t i) { return D.idx[i]; };
-            const auto in_k = [&](uint32_t k) { return bin(k) == o.bk; };
+            const auto in_k = [&](uint32_t k) { return r.few || bin(k) == o.bk; };
             const auto in_p = [&](uint32_t k) { return bin(k) >= o.g0 && bin(k) <= o.g1; };
             c = select_cut(r, n, key, index, in_k, in_p, do_k, (uint32_t)r.k - o.before_k, do_k ? o.mass_k : o.all, o.mass_0, D);
         }

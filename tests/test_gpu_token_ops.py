@@ -578,7 +578,7 @@ def test_sampling_ties_take_the_lowest_indices(dev):
 
 
 @pytest.mark.parametrize("V,kind", [(1 << 20, "equal"), (70000, "equal"), (151936, "narrow"), (1 << 20, "normal"), (9000, "narrow"), (40000, "rounded")])
-@pytest.mark.parametrize("k,p", [(0, 0.3), (5000, 1.0), (5000, 0.7), (300, 0.9), (0, 1.0)])
+@pytest.mark.parametrize("k,p", [(0, 0.3), (5000, 1.0), (5000, 0.7), (300, 0.9), (0, 1.0), (3, 1.0), (100, 0.6), (16, 0.7)])
 def test_sampling_of_flat_rows(dev, V, kind, k, p):
     """Limits that fall among hundreds to all of a row's tokens: long lists, and rows past the lists' room."""
     rng = np.random.default_rng(V + k)
