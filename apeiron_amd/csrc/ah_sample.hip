@@ -195,6 +195,28 @@ AH_DEV void share(const SampleArgs &a, uint32_t &row, uint32_t &s0, uint32_t &s1
     s1 = b + a.per < a.segs ? b + a.per : a.segs;
 }
 
+// Calls f(segment, logits) for those of this wave's segments whose largest token's bin is at most `last`, the next
+// one's logits on their way meanwhile; skipped(segment) with a lane for each of the others.
+template <class F, class G> AH_DEV void each_segment(const SampleArgs &a, const Row &r, uint32_t row, uint32_t s0, uint32_t s1, uint32_t last, F f, G skipped) {
+    constexpr uint32_t W = kT / 64;
+    for (uint32_t base = s0; base < s1; base += 64 * W) {
+        const uint32_t mine = base + W * (threadIdx.x & 63);
+        const bool in = mine < s1, use = in && bin_at(z_of(r, a.seg_max[(size_t)row * a.segs + (in ? mine : base)])) <= last;
+        if (in && !use) skipped(mine);
+        uint64_t todo = __builtin_amdgcn_ballot_w64(use);
+        float x[8], next[8];
+        if (todo) load_logits(r, base + W * (uint32_t)__builtin_ctzll(todo), next);
+        while (todo) {
+            const uint32_t s = base + W * (uint32_t)__builtin_ctzll(todo);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = next[i];
+            todo &= todo - 1;
+            if (todo) load_logits(r, base + W * (uint32_t)__builtin_ctzll(todo), next);
+            f(s, x);
+        }
+    }
+}
+
 __global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
     uint32_t row, s0, s1;
     share(a, row, s0, s1);
@@ -275,19 +297,19 @@ __global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
         mass[i] = 0.0;
     }
     __syncthreads();
-    for (uint32_t s = s0; s < s1; s += kT / 64) {
-        if (bin_at(z_of(r, a.seg_max[(size_t)row * a.segs + s])) > last) continue;  // none of its tokens reaches the bound
-        float x[8];
-        load_logits(r, s, x);
+    each_segment(
+        a, r, row, s0, s1, last,
+        [&](uint32_t, const float *x) {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float z = z_at(r, x[i]);
-            const uint32_t b = bin_at(z);
-            if (b > last) continue;
-            if (r.need_k) atomicAdd(&count[b], 1u);
-            if (r.need_p) unsafeAtomicAdd(&mass[b], (double)weight_at(z));
-        }
-    }
+            for (int i = 0; i < 8; ++i) {
+                const float z = z_at(r, x[i]);
+                const uint32_t b = bin_at(z);
+                if (b > last) continue;
+                if (r.need_k) atomicAdd(&count[b], 1u);
+                if (r.need_p) unsafeAtomicAdd(&mass[b], (double)weight_at(z));
+            }
+        },
+        [](uint32_t) {});
     __syncthreads();
     for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
         if (count[i]) atomicAdd(&a.bin_count[(size_t)row * kBins + i], count[i]);
@@ -399,50 +421,46 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     // the last bin with a token to keep or to list (no bin: tokens without weight, as a whole)
     const uint32_t end_k = o.bk != kNone ? o.bk : o.g1;
     const uint32_t last = o.g0 == kBins ? kBins - 1 : end_k > o.g1 ? end_k : o.g1;
-    for (uint32_t s = s0; s < s1; s += kT / 64) {
-        const size_t seg = (size_t)row * a.segs + s;
-        if (bin_at(z_of(r, a.seg_max[seg])) > last) {
+    each_segment(
+        a, r, row, s0, s1, last,
+        [&](uint32_t s, const float *x) {
+            const size_t seg = (size_t)row * a.segs + s;
+            uint32_t n = 0, mask = 0;
+            double sure = 0.0;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float z = z_at(r, x[i]);
+                const uint32_t b = bin_at(z);
+                if (b < o.g0 && b < kBins) {
+                    const double w = (double)weight_at(z);
+                    sure += w < r.floor_w ? 0.0 : w;
+                } else if (listed(o, r, b)) {
+                    mask |= 1u << i;
+                    ++n;
+                }
+            }
+            uint32_t total = 0;
+            if (__builtin_amdgcn_ballot_w64(n != 0) != 0ull) {
+                const uint32_t end = wave_prefix<Add>(n);
+                total = last_lane(end);
+                uint32_t at = end - n;
+                if (total <= kSampleSegList) {
+                    uint16_t *list = a.list + seg * kSampleSegList;
+#pragma unroll
+                    for (uint32_t i = 0; i < 8; ++i)
+                        if (mask >> i & 1u) list[at++] = (uint16_t)(8 * lane + i);
+                }
+            }
+            if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
             if (lane == 0) {
-                a.seg_mass[seg] = 0.0;
-                a.seg_count[seg] = 0;
+                a.seg_mass[seg] = sure;
+                a.seg_count[seg] = total;
             }
-            continue;
-        }
-        float x[8];
-        uint32_t n = 0;
-        load_logits(r, s, x);
-        double sure = 0.0;
-        uint32_t mask = 0;
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            const float z = z_at(r, x[i]);
-            const uint32_t b = bin_at(z);
-            if (b < o.g0 && b < kBins) {
-                const double w = (double)weight_at(z);
-                sure += w < r.floor_w ? 0.0 : w;
-            } else if (listed(o, r, b)) {
-                mask |= 1u << i;
-                ++n;
-            }
-        }
-        uint32_t total = 0;
-        if (__builtin_amdgcn_ballot_w64(n != 0) != 0ull) {
-            const uint32_t end = wave_prefix<Add>(n);
-            total = last_lane(end);
-            uint32_t at = end - n;
-            if (total <= kSampleSegList) {
-                uint16_t *list = a.list + seg * kSampleSegList;
-#pragma unroll
-                for (uint32_t i = 0; i < 8; ++i)
-                    if (mask >> i & 1u) list[at++] = (uint16_t)(8 * lane + i);
-            }
-        }
-        if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
-        if (lane == 0) {
-            a.seg_mass[seg] = sure;
-            a.seg_count[seg] = total;
-        }
-    }
+        },
+        [&](uint32_t s) {
+            a.seg_mass[(size_t)row * a.segs + s] = 0.0;
+            a.seg_count[(size_t)row * a.segs + s] = 0;
+        });
 }
 
 // ---- the cut ----------------------------------------------------------------------------------------
