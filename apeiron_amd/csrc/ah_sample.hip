@@ -46,6 +46,7 @@ struct Row {
     uint32_t V, top;
     float M, inv_t;
     double floor_w;
+    float floor_f;  // the least f32 not below it
     bool bad_t, greedy, need_k, need_p;
     bool few;  // so few tokens asked for that the segments' maxima bound them: the bins are not needed
 };
@@ -64,6 +65,8 @@ AH_DEV Row row_of(const SampleArgs &a, uint32_t row) {
     r.need_p = r.p < 1.0f;
     r.few = !r.greedy && r.need_k && (uint64_t)r.k * 2 <= a.segs;
     r.floor_w = (double)(r.m > 0.0f ? (r.m < 1.0f ? r.m : 1.0f) : 0.0f) * 0x1p32;
+    r.floor_f = (float)r.floor_w;
+    if ((double)r.floor_f < r.floor_w) r.floor_f = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r.floor_f) + 1);
     return r;
 }
 AH_DEV void set_top(Row &r, uint32_t top) {
@@ -83,9 +86,8 @@ AH_DEV float z_of(const Row &r, uint32_t k) { return k ? z_at(r, logit_of(k)) : 
 AH_DEV float weight_at(float z) {
 #pragma clang fp contract(off)
     const float l2e = 0x1.715476p+0f, rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;  // log2 e = l2e + rest
-    const float t = z * l2e;
-    if (!(t > -40.0f)) return 0.0f;
-    const float d = __builtin_fmaf(z, rest, __builtin_fmaf(z, l2e, -t)), e = __builtin_amdgcn_exp2f(t);
+    z = __builtin_fmaxf(z, -28.0f);  // (the weight is 0 there; z may be -inf)
+    const float t = z * l2e, d = __builtin_fmaf(z, rest, __builtin_fmaf(z, l2e, -t)), e = __builtin_amdgcn_exp2f(t);
     return __builtin_rintf(__builtin_fmaf(e, d * ln2, e) * 0x1p32f);
 }
 // The bin of z, kBins where the weight is 0.
@@ -399,9 +401,17 @@ AH_DEV Limits limits_of(const SampleArgs &a, const Row &r, const Bins &B, Scan &
     o.all = all;
     return o;
 }
-AH_DEV bool listed(const Limits &o, const Row &r, uint32_t b) {
-    return (b >= o.g0 && b <= o.g1 && b < kBins) || (r.need_p && b == o.bk);
-}
+// Whether a bin's tokens are listed: bins g0 to g1, and the top-k one where top-p needs its weight.  (No branches.)
+struct Listed {
+    uint32_t from, span, also;
+    AH_DEV Listed(const Limits &o, const Row &r) {
+        const uint32_t to = o.g1 < kBins ? o.g1 : kBins - 1;
+        from = o.g0 <= to ? o.g0 : 0xfffff000u;  // (no bin is that far below it)
+        span = o.g0 <= to ? to - o.g0 : 0u;
+        also = r.need_p ? o.bk : kNone;
+    }
+    AH_DEV bool operator()(uint32_t b) const { return (b - from <= span) | (b == also); }
+};
 
 __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     __shared__ Scan S;
@@ -417,7 +427,8 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     Limits o = {0, 0, kNone, 0, 0.0, 0.0, 0.0};
     if (r.few) o.g1 = bound_of(a, r, row, S, count, found);  // all that reaches the bound is listed
     else o = limits_of(a, r, B, S, L);
-    const uint32_t lane = threadIdx.x & 63;
+    const uint32_t lane = threadIdx.x & 63, g0 = o.g0 < kBins ? o.g0 : kBins;
+    const Listed listed(o, r);
     // the last bin with a token to keep or to list (no bin: tokens without weight, as a whole)
     const uint32_t end_k = o.bk != kNone ? o.bk : o.g1;
     const uint32_t last = o.g0 == kBins ? kBins - 1 : end_k > o.g1 ? end_k : o.g1;
@@ -431,14 +442,12 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
             for (uint32_t i = 0; i < 8; ++i) {
                 const float z = z_at(r, x[i]);
                 const uint32_t b = bin_at(z);
-                if (b < o.g0 && b < kBins) {
-                    const double w = (double)weight_at(z);
-                    sure += w < r.floor_w ? 0.0 : w;
-                } else if (listed(o, r, b)) {
-                    mask |= 1u << i;
-                    ++n;
-                }
+                // (no branches: the row's lanes take both sides nearly always)
+                const float w = weight_at(z);
+                sure += (double)(((b < g0) & (w >= r.floor_f)) ? w : 0.0f);
+                mask |= (uint32_t)listed(b) << i;
             }
+            n = (uint32_t)__builtin_popcount(mask);
             uint32_t total = 0;
             if (__builtin_amdgcn_ballot_w64(n != 0) != 0ull) {
                 const uint32_t end = wave_prefix<Add>(n);
@@ -446,9 +455,7 @@ __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
                 uint32_t at = end - n;
                 if (total <= kSampleSegList) {
                     uint16_t *list = a.list + seg * kSampleSegList;
-#pragma unroll
-                    for (uint32_t i = 0; i < 8; ++i)
-                        if (mask >> i & 1u) list[at++] = (uint16_t)(8 * lane + i);
+                    for (; mask; mask &= mask - 1) list[at++] = (uint16_t)(8 * lane + (uint32_t)__builtin_ctz(mask));
                 }
             }
             if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
@@ -837,10 +844,10 @@ hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream) {
 // Bytes of scratch, and (with a base) the pointers in it.
 size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
     a.segs = (a.n_vocab + kSeg - 1) / kSeg;
-    // about eight workgroups a CU, each of whole segments of one row
-    const uint64_t want = 8ull * cus, all = (uint64_t)a.n_rows * a.segs;
-    uint64_t per = ((all + want - 1) / want + 3) / 4 * 4;  // whole rounds of a workgroup's four waves
-    a.per = (uint32_t)(per < 4 ? 4 : per);
+    // at most eight workgroups a CU (all that a CU holds: one more would start when the first ends), each of whole
+    // rounds of its four waves over one row's segments
+    const uint64_t all = (uint64_t)a.n_rows * a.segs, want = 8ull * cus / a.n_rows, parts = want < 1 ? 1 : want;
+    a.per = (uint32_t)(((a.segs + parts - 1) / parts + 3) / 4 * 4);
     a.parts = (a.segs + a.per - 1) / a.per;
     size_t at = 0;
     auto take = [&](size_t bytes) {
