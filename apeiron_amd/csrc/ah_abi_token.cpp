@@ -9,8 +9,10 @@
 namespace {
 
 constexpr size_t kMaxU32 = 0x7fffffff;
-constexpr size_t kAttnGroups = 2048;  // (ah_ctx::d_count has an entry for every unit that is split)
-////static_assert(kAttnGroups / 2 <= kCounts, "units of at least two pieces");
+// Workgroups that a split attention over few rows aims at.  ah_ctx::d_count has an entry for every unit and for every
+// group of its pieces: at most kAttnGroups / 2 of each (two pieces, one group), and fewer of both with more pieces.
+constexpr size_t kAttnGroups = 2048;
+static_assert(kAttnGroups <= kCounts, "an entry for each unit and each group of pieces");
 
 bool tokens_ok(const ah_kv4_tokens *t) {
     return t->d_seq && t->d_pos && t->d_table && t->n_seq && t->table_stride && t->n_tok <= kMaxU32 && t->n_seq <= kMaxU32 &&
@@ -320,6 +322,8 @@ int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, siz
     a.tokens = d_tokens;
     a.probs = d_probs;
     a.status = ctx->d_status;
+    a.arrived = ctx->d_count;
+    a.n_counts = (uint32_t)kCounts;
     AH_HIP(ctx, hipSetDevice(ctx->device));
     const uint32_t cus = (uint32_t)ctx->cu_count;
     const int32_t st = ensure_scratch(ctx, ah_sample_plan(a, cus, nullptr));

@@ -130,6 +130,12 @@ struct AttnArgs {
     unsigned long long *status;
 };
 
+// What a row's scan and count leave for the launches after them (ah_sample.hip).
+struct SampleLimits {
+    uint32_t g0, g1, bk, before_k;
+    double mass_k, mass_0, all;
+    uint32_t top, last, done;  // the largest key, the last bin to look at, whether the token is drawn
+};
 struct SampleArgs {
     const float *logits;
     uint64_t stride;
@@ -139,14 +145,18 @@ struct SampleArgs {
     int32_t *tokens;
     float *probs;
     unsigned long long *status;
-    // planned by ah_sample_plan: segments of a row, segments of a workgroup and workgroups of a row, and the scratch
-    uint32_t segs, per, parts;
-    double *bin_mass, *seg_mass;                // [row][bin], [row][segment]
-    uint32_t *bin_count, *group_max, *seg_max, *seg_count; // [row][bin], [row][segment][group], [row][segment]
-    uint16_t *list;                             // [row][segment][kSampleSegList] tokens listed, by place in the segment
+    uint32_t *arrived;  // [n_counts], zero between calls
+    uint32_t n_counts;
+    // planned by ah_sample_plan: groups and chunks of a row, chunks of a workgroup and workgroups of a row, and the scratch
+    uint32_t groups, chunks, per, parts;
+    bool draw;  // in the gather's launch
+    SampleLimits *limits;                          // [row]
+    double *bin_mass, *chunk_mass;                 // [row][bin], [row][chunk]
+    float *group_max;                              // [row][group]
+    uint32_t *bin_count, *chunk_count;             // [row][bin], [row][chunk]
+    uint16_t *list;                                // [row][chunk][kSampleChunkList] tokens listed, by place in the chunk
 };
-constexpr uint32_t kSampleSegList = 64, kSampleList = 4096, kSampleMaxSegs = 2048;
-
+constexpr uint32_t kSampleChunkList = 256, kSampleList = 4096, kSampleMaxChunks = 512;
 
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream);
 hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream);

@@ -7,29 +7,36 @@
 // those the ones with w >= min_p 2^32 (min-p); the first token always.  The draw is the smallest index
 // at which the kept weight up to and with it, in index order, passes floor(u W).
 //
-// No sort.  Four launches over segments of 512 tokens (a wave's eight tokens a lane), each reading the row
-// at most once:
-//   scan    the largest key of every group of 64 tokens and of every segment (a key is the f32 bits as an
-//           unsigned number of the same order), and so M;
-//   count   the tokens and their weight in 1024 bins of (M - l) / T.  With top-k, the k-th largest segment
-//           or group maximum bounds the k-th largest logit from below, and only what reaches it is counted;
-//   gather  from the bins: those kept for certain, those dropped, and the few that a limit falls into,
-//           whose tokens are listed; and each segment's certain weight;
-//   draw    one workgroup a row orders the listed tokens, cuts them, draws a segment and a token in it.
+// No sort.  Four launches over chunks of 2048 tokens, each reading what it needs of the row once:
+//   scan    the largest key of every group of 64 tokens (a key is the f32 bits as an unsigned number of the
+//           same order);
+//   count   M, and with top-k the bound, a bin of (M - l) / T that the k-th largest group maximum is in: every
+//           maximum is a token of its own, so no token past it is among the first k, and only about k groups
+//           reach it.  With a small k (and for a greedy row) one workgroup lists their tokens, cuts and draws, and
+//           the row is done.  Otherwise the tokens and their weight in 1024 bins, of the groups that reach the
+//           bound; the row's workgroup that arrives last finds in them the bins that are kept, those dropped,
+//           and the few that a limit falls into;
+//   gather  each chunk's certain weight, and a list of the tokens in the few bins;
+//   draw    one workgroup a row orders the listed tokens, cuts them, draws a chunk and a token in it (of few rows,
+//           in the gather's launch).
 // A row whose listed tokens pass the lists' room (thousands of equal logits) is cut by selections over
-// the whole row instead.  What bounds it: the row's bytes for many rows (one read from HBM, two more from
-// the cache that holds it), four dependent launches for one.
+// the whole row instead.
 #include "ah_kv4.h"
+
+#include <type_traits>
 
 namespace {
 
-constexpr uint32_t kT = 256;            // threads of every workgroup here
-constexpr uint32_t kSeg = 512;          // tokens of a segment: eight a lane of one wave
-constexpr uint32_t kGroup = 64;         // tokens of a group: eight lanes
-constexpr uint32_t kGroups = kSeg / kGroup;
+constexpr uint32_t kT = 256, kW = kT / 64;  // threads and waves of every workgroup here
+constexpr uint32_t kGroup = 64;             // tokens of a group: eight lanes of eight
+constexpr uint32_t kChunk = 2048;           // tokens of a chunk, one wave's in count and gather
+constexpr uint32_t kGroups = kChunk / kGroup;
 constexpr uint32_t kBins = 1024;
 constexpr float kBinScale = kBins / 23.0f;  // w is 0 past (M - l) / T = 22.9
 constexpr uint32_t kNone = 0xffffffffu;
+// Up to kSmallK tokens asked for, a row's first workgroup counts alone, and draws if the groups that reach the bound
+// (as many, and a few in the bound's own bin) and their tokens fit.
+constexpr uint32_t kSmallK = 56, kSmallGroups = 64, kSmallList = 1024;
 
 AH_DEV uint32_t key_of(float l) {
     l = l != l ? -__builtin_inff() : l + 0.0f;  // NaN is never drawn; -0 and 0 are equal
@@ -48,22 +55,24 @@ struct Row {
     double floor_w;
     float floor_f;  // the least f32 not below it
     bool bad_t, greedy, need_k, need_p;
-    bool few;  // so few tokens asked for that the segments' maxima bound them: the bins are not needed
 };
 AH_DEV Row row_of(const SampleArgs &a, uint32_t row) {
     Row r;
     r.x = a.logits + (size_t)row * a.stride;
     r.V = a.n_vocab;
-    r.T = a.temperature ? a.temperature[row] : 1.0f;
-    r.k = a.top_k ? a.top_k[row] : 0;
-    r.p = a.top_p ? a.top_p[row] : 1.0f;
-    r.m = a.min_p ? a.min_p[row] : 0.0f;
-    r.u = a.u[row];
+    // five loads at once: an absent parameter's reads u instead
+    const float *u = a.u + row;
+    const float T = *(a.temperature ? a.temperature + row : u), p = *(a.top_p ? a.top_p + row : u), m = *(a.min_p ? a.min_p + row : u);
+    const int32_t k = *(a.top_k ? a.top_k + row : reinterpret_cast<const int32_t *>(u));
+    r.u = *u;
+    r.T = a.temperature ? T : 1.0f;
+    r.k = a.top_k ? k : 0;
+    r.p = a.top_p ? p : 1.0f;
+    r.m = a.min_p ? m : 0.0f;
     r.bad_t = !(r.T >= 0.0f && r.T < __builtin_inff());
     r.greedy = r.bad_t || r.T == 0.0f || r.k == 1;
-    r.need_k = r.k > 1 && (uint32_t)r.k < r.V;
-    r.need_p = r.p < 1.0f;
-    r.few = !r.greedy && r.need_k && (uint64_t)r.k * 2 <= a.segs;
+    r.need_k = !r.greedy && r.k > 1 && (uint32_t)r.k < r.V;
+    r.need_p = !r.greedy && r.p < 1.0f;
     r.floor_w = (double)(r.m > 0.0f ? (r.m < 1.0f ? r.m : 1.0f) : 0.0f) * 0x1p32;
     r.floor_f = (float)r.floor_w;
     if ((double)r.floor_f < r.floor_w) r.floor_f = __builtin_bit_cast(float, __builtin_bit_cast(uint32_t, r.floor_f) + 1);
@@ -74,10 +83,10 @@ AH_DEV void set_top(Row &r, uint32_t top) {
     r.M = logit_of(top);
     r.inv_t = 1.0f / r.T;
 }
-// A logit's z = (l - M) / T, from the logit itself (NaN as -inf) or its key (0 past the row's end).
+// A logit's z = (l - M) / T, from the logit itself (NaN stays one: no bin and no weight) or its key (0 past the
+// row's end).
 AH_DEV float z_at(const Row &r, float l) {
 #pragma clang fp contract(off)
-    l = __builtin_fmaxf(l, -__builtin_inff());
     return l == r.M ? 0.0f : (l - r.M) * r.inv_t;
 }
 AH_DEV float z_of(const Row &r, uint32_t k) { return k ? z_at(r, logit_of(k)) : -__builtin_inff(); }
@@ -86,12 +95,13 @@ AH_DEV float z_of(const Row &r, uint32_t k) { return k ? z_at(r, logit_of(k)) : 
 AH_DEV float weight_at(float z) {
 #pragma clang fp contract(off)
     const float l2e = 0x1.715476p+0f, rest = 0x1.4ae0cp-26f, ln2 = 0x1.62e43p-1f;  // log2 e = l2e + rest
-    z = __builtin_fmaxf(z, -28.0f);  // (the weight is 0 there; z may be -inf)
+    z = __builtin_fmaxf(z, -28.0f);  // (the weight is 0 there; z may be -inf or NaN)
     const float t = z * l2e, d = __builtin_fmaf(z, rest, __builtin_fmaf(z, l2e, -t)), e = __builtin_amdgcn_exp2f(t);
     return __builtin_rintf(__builtin_fmaf(e, d * ln2, e) * 0x1p32f);
 }
-// The bin of z, kBins where the weight is 0.
-AH_DEV uint32_t bin_at(float z) { return (uint32_t)__builtin_fminf(z * -kBinScale, (float)kBins); }
+// The place of z among the bins, and its bin: kBins where the weight is 0.
+AH_DEV float place_at(float z) { return z * -kBinScale; }
+AH_DEV uint32_t bin_at(float z) { return (uint32_t)__builtin_fminf(place_at(z), (float)kBins); }
 
 // ---- workgroup scans (kT threads) -------------------------------------------------------------------
 
@@ -99,15 +109,17 @@ AH_DEV uint32_t bin_at(float z) { return (uint32_t)__builtin_fminf(z * -kBinScal
 template <int CTRL, int ROWS> AH_DEV uint32_t dpp0(uint32_t v) {
     return (uint32_t)__builtin_amdgcn_update_dpp(0, (int)v, CTRL, ROWS, 0xF, false);
 }
+template <int CTRL, int ROWS> AH_DEV uint64_t dpp0(uint64_t v) {
+    return (uint64_t)dpp0<CTRL, ROWS>((uint32_t)(v >> 32)) << 32 | dpp0<CTRL, ROWS>((uint32_t)v);
+}
 template <int CTRL, int ROWS> AH_DEV double dpp0(double v) {
-    const uint64_t b = __builtin_bit_cast(uint64_t, v);
-    return __builtin_bit_cast(double, (uint64_t)dpp0<CTRL, ROWS>((uint32_t)(b >> 32)) << 32 | dpp0<CTRL, ROWS>((uint32_t)b));
+    return __builtin_bit_cast(double, dpp0<CTRL, ROWS>(__builtin_bit_cast(uint64_t, v)));
 }
 struct Add {
     template <class T> AH_DEV T operator()(T a, T b) const { return a + b; }
 };
 struct Max {
-    AH_DEV uint32_t operator()(uint32_t a, uint32_t b) const { return a > b ? a : b; }
+    template <class T> AH_DEV T operator()(T a, T b) const { return a > b ? a : b; }
 };
 // Inclusive prefix over the wave (0 the operation's identity): inside rows of 16 by shifts of 1, 2, 4 and 8,
 // then the rows' ends passed on.
@@ -163,188 +175,555 @@ AH_DEV uint32_t max_u(uint32_t v, Scan &S) {
 }
 AH_DEV uint32_t min_u(uint32_t v, Scan &S) { return ~max_u(~v, S); }
 
-// A lane's eight logits of a segment (-inf past the row's end), and their keys (0, below every key, there).
-AH_DEV void load_logits(const Row &r, uint32_t seg, float *x) {
-    const uint32_t i0 = seg * kSeg + 8 * (threadIdx.x & 63);
+// Eight logits of the row (-inf past its end), and their keys (0, below every key, there).
+AH_DEV void load_logits(const Row &r, uint32_t i0, float *x) {
     if (i0 + 8 <= r.V) __builtin_memcpy(x, r.x + i0, 32);
     else
 #pragma unroll
         for (uint32_t i = 0; i < 8; ++i) x[i] = i0 + i < r.V ? r.x[i0 + i] : -__builtin_inff();
 }
-AH_DEV void keys_of(const Row &r, uint32_t seg, const float *x, uint32_t *k) {
-    const uint32_t i0 = seg * kSeg + 8 * (threadIdx.x & 63);
+AH_DEV void keys_of(const Row &r, uint32_t i0, const float *x, uint32_t *k) {
 #pragma unroll
     for (uint32_t i = 0; i < 8; ++i) k[i] = i0 + i < r.V ? key_of(x[i]) : 0u;
 }
-AH_DEV void load_keys(const Row &r, uint32_t seg, uint32_t *k) {
+AH_DEV void load_keys(const Row &r, uint32_t i0, uint32_t *k) {
     float x[8];
-    load_logits(r, seg, x);
-    keys_of(r, seg, x, k);
+    load_logits(r, i0, x);
+    keys_of(r, i0, x, k);
 }
 
-AH_DEV uint32_t top_of(const SampleArgs &a, uint32_t row, Scan &S) {
-    const uint32_t *g = a.seg_max + (size_t)row * a.segs;
-    uint32_t top = 0;
-    for (uint32_t i = threadIdx.x; i < a.segs; i += kT) top = __builtin_elementwise_max(top, g[i]);
-    return max_u(top, S);
-}
+// What one workgroup writes and another reads in the same launch goes past the XCDs' own L2s.
+template <class T> AH_DEV void put(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
+template <class T> AH_DEV T get(const T *p) { return __hip_atomic_load(const_cast<T *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// The workgroup's row, and the segments of this wave: s0, s0 + 4, .. below s1.
-AH_DEV void share(const SampleArgs &a, uint32_t &row, uint32_t &s0, uint32_t &s1) {
+// The workgroup's row and its chunks.
+AH_DEV void share(const SampleArgs &a, uint32_t &row, uint32_t &c0, uint32_t &c1) {
     row = blockIdx.x / a.parts;
-    const uint32_t b = (blockIdx.x - row * a.parts) * a.per;
-    s0 = b + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    s1 = b + a.per < a.segs ? b + a.per : a.segs;
+    c0 = (blockIdx.x - row * a.parts) * a.per;
+    c1 = c0 + a.per < a.chunks ? c0 + a.per : a.chunks;
+}
+// Whether this workgroup is the row's last in the launch: it then finds what the others have put.  The counters
+// are left at zero.
+AH_DEV bool last_of_row(const SampleArgs &a, uint32_t row, uint32_t &word) {
+    __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+    __syncthreads();
+    if (threadIdx.x == 0) {
+        const uint32_t n = __hip_atomic_fetch_add(a.arrived + row, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+        if (n == a.parts - 1) put(a.arrived + row, 0u);
+        word = n;
+    }
+    __syncthreads();
+    return word == a.parts - 1;
 }
 
-// Calls f(segment, logits) for those of this wave's segments whose largest token's bin is at most `last`, the next
-// one's logits on their way meanwhile; skipped(segment) with a lane for each of the others.
-template <class F, class G> AH_DEV void each_segment(const SampleArgs &a, const Row &r, uint32_t row, uint32_t s0, uint32_t s1, uint32_t last, F f, G skipped) {
-    constexpr uint32_t W = kT / 64;
-    for (uint32_t base = s0; base < s1; base += 64 * W) {
-        const uint32_t mine = base + W * (threadIdx.x & 63);
-        const bool in = mine < s1, use = in && bin_at(z_of(r, a.seg_max[(size_t)row * a.segs + (in ? mine : base)])) <= last;
-        if (in && !use) skipped(mine);
-        uint64_t todo = __builtin_amdgcn_ballot_w64(use);
-        float x[8], next[8];
-        if (todo) load_logits(r, base + W * (uint32_t)__builtin_ctzll(todo), next);
-        while (todo) {
-            const uint32_t s = base + W * (uint32_t)__builtin_ctzll(todo);
-#pragma unroll
-            for (int i = 0; i < 8; ++i) x[i] = next[i];
-            todo &= todo - 1;
-            if (todo) load_logits(r, base + W * (uint32_t)__builtin_ctzll(todo), next);
-            f(s, x);
-        }
-    }
-}
+// ---- the cut ----------------------------------------------------------------------------------------
 
-__global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
-    uint32_t row, s0, s1;
-    share(a, row, s0, s1);
-    Row r;
-    r.x = a.logits + (size_t)row * a.stride;
-    r.V = a.n_vocab;
-    if (blockIdx.x % a.parts == 0) {  // the row's bins, for the next launch
-        for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
-            a.bin_mass[(size_t)row * kBins + i] = 0.0;
-            a.bin_count[(size_t)row * kBins + i] = 0;
-        }
-    }
-    bool nan = false;
-    for (uint32_t s = s0; s < s1; s += kT / 64) {
-        float x[8];
-        uint32_t k[8], top = 0;
-        load_logits(r, s, x);
-        keys_of(r, s, x, k);
-#pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) {
-            nan |= x[i] != x[i];
-            top = __builtin_elementwise_max(top, k[i]);
-        }
-#pragma unroll
-        for (int o = 1; o < 8; o <<= 1) top = __builtin_elementwise_max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        const uint32_t lane = threadIdx.x & 63;
-        const size_t seg = (size_t)row * a.segs + s;
-        if ((lane & 7) == 0) a.group_max[seg * kGroups + lane / 8] = top;
-#pragma unroll
-        for (int o = 8; o < 64; o <<= 1) top = __builtin_elementwise_max(top, (uint32_t)__shfl_xor((int)top, o, 64));
-        if (lane == 0) a.seg_max[seg] = top;
-    }
-    if (nan) ah_record(a.status, ((unsigned long long)row << 8) + AH_ERR_NONFINITE_INPUT);
-}
-
-// The last bin that can hold one of the first k: every segment's (or group's) largest is a token of its own, so the
-// k-th largest of them bounds the k-th largest logit from below.  Segments do where there are twice k of them.
-AH_DEV uint32_t bound_of(const SampleArgs &a, const Row &r, uint32_t row, Scan &S, uint32_t *count, uint32_t &found) {
-    for (uint32_t i = threadIdx.x; i < kBins; i += kT) count[i] = 0;
-    if (threadIdx.x == 0) found = kBins - 1;
-    __syncthreads();
-    const uint32_t *g = r.few ? a.seg_max + (size_t)row * a.segs : a.group_max + (size_t)row * a.segs * kGroups;
-    const uint32_t n = r.few ? a.segs : a.segs * kGroups;
-    for (uint32_t i = threadIdx.x; i < n; i += kT) {
-        const uint32_t b = bin_at(z_of(r, g[i]));
-        if (b < kBins) atomicAdd(&count[b], 1u);
-    }
-    __syncthreads();
-    uint32_t c[4], total;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) c[i] = count[4 * threadIdx.x + i];
-    const uint32_t mine = (c[0] + c[1]) + (c[2] + c[3]);
-    uint32_t cum = scan_u(mine, S, total) - mine;
-#pragma unroll
-    for (int i = 0; i < 4; ++i) {
-        if (cum < (uint32_t)r.k && cum + c[i] >= (uint32_t)r.k) found = 4 * threadIdx.x + i;
-        cum += c[i];
-    }
-    __syncthreads();
-    return found;
-}
-
-__global__ void __launch_bounds__(kT) sample_count_kernel(SampleArgs a) {
-    __shared__ double mass[kBins];
-    __shared__ uint32_t count[kBins];
-    __shared__ Scan S;
-    __shared__ uint32_t found;
-    uint32_t row, s0, s1;
-    share(a, row, s0, s1);
-    Row r = row_of(a, row);
-    if (r.greedy || r.few || (!r.need_k && !r.need_p)) return;
-    set_top(r, top_of(a, row, S));
-    if (r.M == -__builtin_inff()) return;
-    const uint32_t last = r.need_k ? bound_of(a, r, row, S, count, found) : kBins - 1;
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
-        count[i] = 0;
-        mass[i] = 0.0;
-    }
-    __syncthreads();
-    each_segment(
-        a, r, row, s0, s1, last,
-        [&](uint32_t, const float *x) {
-#pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float z = z_at(r, x[i]);
-                const uint32_t b = bin_at(z);
-                if (b > last) continue;
-                if (r.need_k) atomicAdd(&count[b], 1u);
-                if (r.need_p) unsafeAtomicAdd(&mass[b], (double)weight_at(z));
-            }
-        },
-        [](uint32_t) {});
-    __syncthreads();
-    for (uint32_t i = threadIdx.x; i < kBins; i += kT) {
-        if (count[i]) atomicAdd(&a.bin_count[(size_t)row * kBins + i], count[i]);
-        if (mass[i] > 0.0) unsafeAtomicAdd(&a.bin_mass[(size_t)row * kBins + i], mass[i]);
-    }
-}
+// The list of tokens (in index order) that a cut is looked for in, and what the search needs.
+template <uint32_t LIST> struct CutLds {
+    alignas(16) double mass[kT];
+    uint32_t count[kT];
+    alignas(16) uint32_t key[LIST], idx[LIST];
+    alignas(16) uint32_t near_key[kT];
+    uint32_t near_idx[kT];
+    Scan S;
+    uint32_t u0, u1;
+    double d0;
+};
 
 // What the bins say.  Tokens of bins below g0 are kept and those of bins past g1 dropped (min-p apart); the
 // k-th token is in bin bk (kNone: fewer than k tokens have weight), `before_k` tokens weighing `mass_k` ahead of
 // that bin; `mass_0` is the weight ahead of bin g0 and `all` that of every bin.
-struct Limits {
-    uint32_t g0, g1, bk, before_k;
-    double mass_k, mass_0, all;
+typedef SampleLimits Limits;
+
+// The kept set's last token in the order: keys above `key` are kept, and of those equal to it the ones up
+// to index `last`.
+struct Cut {
+    uint32_t key, last;
 };
+
+// The index of the nth (1 ..) of n tokens in index order that have key `cut`.
+template <class Key, class Index, class Lds> AH_DEV uint32_t nth_equal(uint32_t n, Key key, Index index, uint32_t cut, uint32_t nth, Lds &D) {
+    uint32_t seen = 0;
+    for (uint32_t base = 0; base < n && seen < nth; base += kT) {
+        const uint32_t i = base + threadIdx.x;
+        const bool eq = i < n && key(i) == cut;
+        uint32_t total;
+        const uint32_t at = seen + scan_u(eq, D.S, total);
+        if (eq && at == nth) D.u0 = index(i);
+        seen += total;
+    }
+    __syncthreads();
+    return D.u0;
+}
+
+// The digit at which keys between lo and hi first differ, as a shift, and what they share above it.
+AH_DEV int first_digit(uint32_t lo, uint32_t hi, uint32_t &shared) {
+    const uint32_t x = lo ^ hi;
+    const int shift = x ? (31 - __builtin_clz(x)) / 8 * 8 : 0;
+    shared = shift == 24 ? 0 : hi >> (shift + 8) << (shift + 8);
+    return shift;
+}
+
+// The cut over n tokens in index order (a list, or the whole row), by digits of the keys.  in_k(key) and
+// in_p(key): whether such a token counts for the top-k and for the top-p limit.  need: tokens that top-k still
+// keeps of its own; W0: the weight ahead of those (without top-k: of every token); before: the weight ahead of
+// top-p's.
+template <class Key, class Index, class InK, class InP, class Lds>
+AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, InP in_p, bool do_k, uint32_t need, double W0, double before,
+                      Lds &D) {
+    const uint32_t t = threadIdx.x;
+    Cut c = {0, kNone};
+    uint32_t keep = 0, cut_k = 0;  // of those at the cut
+    bool partial = false;
+    if (do_k) {
+        uint32_t lo = kNone, hi = 0;
+#pragma unroll 1
+        for (uint32_t i = t; i < n; i += kT) {
+            const uint32_t k = key(i);
+            if (in_k(k)) {
+                lo = __builtin_elementwise_min(lo, k);
+                hi = __builtin_elementwise_max(hi, k);
+            }
+        }
+        lo = min_u(lo, D.S);
+        hi = max_u(hi, D.S);
+        for (int shift = first_digit(lo, hi, cut_k); shift >= 0; shift -= 8) {
+            __syncthreads();
+            D.count[t] = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t i = t; i < n; i += kT) {
+                const uint32_t k = key(i);
+                if (in_k(k) && (shift == 24 || (k >> (shift + 8)) == (cut_k >> (shift + 8)))) atomicAdd(&D.count[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            const uint32_t mine = D.count[255 - t];
+            uint32_t total;
+            const uint32_t cum = scan_u(mine, D.S, total);
+            if (cum >= need && cum - mine < need) {
+                D.u0 = 255 - t;
+                D.u1 = cum - mine;
+            }
+            __syncthreads();
+            cut_k |= D.u0 << shift;
+            need -= D.u1;
+        }
+        keep = need;
+        partial = D.count[D.u0] > need;
+        c.key = cut_k;
+    }
+    if (r.need_p) {
+        const double w_cut = do_k ? (double)weight_at(z_of(r, cut_k)) : 0.0;
+        double W = W0;
+        if (do_k) {
+            double s = 0.0;
+#pragma unroll 1
+            for (uint32_t i = t; i < n; i += kT) {
+                const uint32_t k = key(i);
+                if (in_k(k) && k > cut_k) s += (double)weight_at(z_of(r, k));
+            }
+            W += sum_d(s, D.S) + (double)keep * w_cut;
+        }
+        double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
+        goal = goal < 1.0 ? 1.0 : goal;  // the first token always
+        uint32_t cut_p = 0, all = 0, lo = do_k && in_p(cut_k) ? cut_k : kNone, hi = lo == kNone ? 0u : cut_k;
+#pragma unroll 1
+        for (uint32_t i = t; i < n; i += kT) {
+            const uint32_t k = key(i);
+            if (in_p(k) && !(do_k && k <= cut_k)) {
+                lo = __builtin_elementwise_min(lo, k);
+                hi = __builtin_elementwise_max(hi, k);
+            }
+        }
+        lo = min_u(lo, D.S);
+        hi = max_u(hi, D.S);
+        for (int shift = first_digit(lo, hi, cut_p); shift >= 0; shift -= 8) {
+            __syncthreads();
+            D.mass[t] = 0.0;
+            D.count[t] = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t i = t; i < n; i += kT) {
+                const uint32_t k = key(i);
+                if (!in_p(k) || (do_k && k <= cut_k) || !(shift == 24 || (k >> (shift + 8)) == (cut_p >> (shift + 8)))) continue;
+                unsafeAtomicAdd(&D.mass[(k >> shift) & 255u], (double)weight_at(z_of(r, k)));
+                atomicAdd(&D.count[(k >> shift) & 255u], 1u);
+            }
+            __syncthreads();
+            double mine = D.mass[255 - t];
+            uint32_t cnt = D.count[255 - t];
+            if (do_k && in_p(cut_k) && (shift == 24 || (cut_k >> (shift + 8)) == (cut_p >> (shift + 8))) && 255 - t == ((cut_k >> shift) & 255u)) {
+                mine += (double)keep * w_cut;
+                cnt += keep;
+            }
+            double total;
+            const double cum = before + scan_d(mine, D.S, total);
+            if (cum >= goal && cum - mine < goal) {
+                D.u0 = 255 - t;
+                D.u1 = cnt;
+                D.d0 = cum - mine;
+            }
+            __syncthreads();
+            cut_p |= D.u0 << shift;
+            all = D.u1;
+            before = D.d0;
+        }
+        const double w = (double)weight_at(z_of(r, cut_p)), q = (goal - before) / w;
+        uint32_t m = q >= (double)all ? all : q <= 1.0 ? 1u : (uint32_t)q;
+        while (m < all && before + (double)m * w < goal) ++m;
+        while (m > 1 && before + (double)(m - 1) * w >= goal) --m;
+        partial = m < all || (do_k && cut_p == cut_k && partial);
+        keep = m;
+        c.key = cut_p;
+    }
+    if (partial) c.last = nth_equal(n, key, index, c.key, keep, D);
+    return c;
+}
+
+// The cut of the list's n tokens in two stages, the first k's and top-p's.  The limit of a stage is where the running
+// sum (of ones, of weights) in the order reaches its goal; of more than kFew tokens, those of the one of 256 equal
+// parts of the limit's bins in which it does are taken out first, and among what is left four neighbouring threads find
+// the sum ahead of a token by comparing with all.  whole: the list is every token that can be among the first k.
+// False: more than kT tokens in such a part.
+constexpr uint32_t kFew = kT / 4;
+template <class Lds> AH_DEV bool cut_list(const Row &r, const Limits &o, uint32_t n, bool do_k, bool whole, Cut &c, Lds &D) {
+    const uint32_t t = threadIdx.x, each = (n + kT - 1) / kT, j0 = t * each, j1 = j0 + each < n ? j0 + each : n;
+    c = {0, kNone};
+#pragma unroll 1
+    // (a list of just the first k needs no cut)
+    for (uint32_t stage = do_k && !(whole && n == (uint32_t)r.k) ? 0 : 1; stage < (r.need_p ? 2u : 1u); ++stage) {
+        const bool p = stage == 1;
+        const float k_from = whole ? 0.0f : (float)o.bk, k_to = whole ? (float)(o.g1 + 1) : (float)(o.bk + 1);
+        float from = k_from, to = k_to;
+        // tokens that count: at places between the two, and up to the cut so far
+        const auto in = [&](uint32_t j) {
+            const uint32_t k = D.key[j];
+            const float y = place_at(z_of(r, k));
+            return (y >= from) & (y < to) & ((k > c.key) | ((k == c.key) & (D.idx[j] <= c.last)));
+        };
+        const auto value = [&](uint32_t j) { return p ? (double)weight_at(z_of(r, D.key[j])) : 1.0; };
+        double goal = (double)((uint32_t)r.k - o.before_k), before = 0.0;
+        if (p) {
+            double W = o.all;
+            if (do_k || whole) {
+                double w = 0.0;
+#pragma unroll 1
+                for (uint32_t j = t; j < n; j += kT) w += in(j) ? value(j) : 0.0;
+                W = o.mass_k + sum_d(w, D.S);
+            }
+            goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
+            goal = goal < 1.0 ? 1.0 : goal;  // the first token always
+            before = o.mass_0;
+            from = (float)o.g0;
+            to = (float)(o.g1 + 1);
+        }
+        const float scale = (float)kT / (to - from);
+        const auto part = [&](uint32_t j) { return n <= kFew ? 0u : (uint32_t)__builtin_fminf((place_at(z_of(r, D.key[j])) - from) * scale, (float)(kT - 1)); };
+        uint32_t the = 0;
+        if (n > kFew) {
+            D.mass[t] = 0.0;
+            if (t == 0) D.u0 = 0;
+            __syncthreads();
+#pragma unroll 1
+            for (uint32_t j = t; j < n; j += kT)
+                if (in(j)) unsafeAtomicAdd(&D.mass[part(j)], value(j));
+            __syncthreads();
+            const double mine = D.mass[t];
+            double total;
+            const double sum = before + scan_d(mine, D.S, total);
+            if (sum >= goal && sum - mine < goal) {
+                D.u0 = t;
+                D.d0 = sum - mine;
+            }
+            __syncthreads();
+            the = D.u0;
+            before = D.d0;
+        }
+        D.near_key[t] = 0;
+        D.mass[t] = 0.0;
+        uint32_t count = 0, m;
+#pragma unroll 1
+        for (uint32_t j = j0; j < j1; ++j) count += in(j) && part(j) == the ? 1u : 0u;
+        uint32_t at = scan_u(count, D.S, m) - count;
+        if (m > kT) return false;
+#pragma unroll 1
+        for (uint32_t j = j0; j < j1; ++j)
+            if (in(j) && part(j) == the) {
+                D.near_key[at] = D.key[j];
+                D.near_idx[at] = D.idx[j];
+                D.mass[at++] = value(j);
+            }
+        __syncthreads();
+        const double ahead = before;
+#pragma unroll 1
+        for (uint32_t me = t / 4; me < m; me += kFew) {
+            const uint32_t k = D.near_key[me], idx = D.near_idx[me];
+            const double mine = D.mass[me];
+            before = 0.0;
+#pragma unroll 2
+            for (uint32_t j = 4 * (t & 3); j < m; j += 16) {  // (past the m tokens: key 0, below every key)
+                uint32_t other[4];
+                double w[4];
+                __builtin_memcpy(other, D.near_key + j, 16);
+                __builtin_memcpy(w, D.mass + j, 32);
+#pragma unroll
+                for (uint32_t i = 0; i < 4; ++i) w[i] = other[i] > (j + i < me ? k - 1 : k) ? w[i] : 0.0;
+                before += (w[0] + w[1]) + (w[2] + w[3]);
+            }
+            before += dpp0<0xB1, 0xF>(before);  // the other three of the quad
+            before += dpp0<0x4E, 0xF>(before);
+            before += ahead;
+            if (before < goal && before + mine >= goal) {
+                D.u0 = k;
+                D.u1 = idx;
+            }
+        }
+        __syncthreads();
+        c = {D.u0, D.u1};
+    }
+    return true;
+}
+
+// A token's weight if it is kept: under a limit, up to the cut.
+AH_DEV double kept_weight(const Row &r, const Cut &c, bool limited, uint32_t i, uint32_t k) {
+    if (limited && (k < c.key || (k == c.key && i > c.last))) return 0.0;
+    const float z = z_of(r, k);
+    if (bin_at(z) == kBins) return 0.0;
+    const double w = (double)weight_at(z);
+    return w < r.floor_w ? 0.0 : w;
+}
+AH_DEV double goal_of(const Row &r, double W) {
+    const double goal = __builtin_floor((double)(r.u > 0.0f ? r.u : 0.0f) * W);
+    return goal < W ? goal : W - 1.0;
+}
+
+// ---- scan -------------------------------------------------------------------------------------------
+
+__global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
+    uint32_t row, c0, c1;
+    share(a, row, c0, c1);
+    Row r;
+    r.x = a.logits + (size_t)row * a.stride;
+    r.V = a.n_vocab;
+    const uint32_t t = threadIdx.x, wave = __builtin_amdgcn_readfirstlane(t >> 6), lane = t & 63;
+    if (c0 == 0) {  // the row's bins, for the next launch
+        for (uint32_t i = t; i < kBins; i += kT) {
+            a.bin_mass[(size_t)row * kBins + i] = 0.0;
+            a.bin_count[(size_t)row * kBins + i] = 0;
+        }
+    }
+    // a wave takes 512 tokens at a time
+    const uint32_t end = c1 * kChunk < r.V ? c1 * kChunk : r.V;
+    bool nan = false;
+    for (uint32_t base = c0 * kChunk + wave * 512; base < end; base += kW * 512) {
+        const uint32_t i0 = base + 8 * lane, group = i0 / kGroup;
+        float x[8], top = -__builtin_inff();  // (a NaN is passed over)
+        load_logits(r, i0, x);
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) {
+            nan |= x[i] != x[i];
+            top = __builtin_fmaxf(top, x[i]);
+        }
+#pragma unroll
+        for (int o = 1; o < 8; o <<= 1) top = __builtin_fmaxf(top, __shfl_xor(top, o, 64));
+        if ((lane & 7) == 0 && group < a.groups) a.group_max[(size_t)row * a.groups + group] = top;
+    }
+    if (nan) ah_record(a.status, ((unsigned long long)row << 8) + AH_ERR_NONFINITE_INPUT);
+}
+
+// ---- count ------------------------------------------------------------------------------------------
+
 struct LimitsLds {
     uint32_t bk, before_k, g0, g1;
-    double mass_k, mass_0, w_low, w_high;
+    double mass_k, mass_0, w_high;
 };
-// A thread's four bins, loaded ahead of what else a kernel waits for.
-struct Bins {
-    uint32_t c[4];
-    double m[4];
-    AH_DEV Bins(const SampleArgs &a, uint32_t row) {
-        __builtin_memcpy(c, a.bin_count + (size_t)row * kBins + 4 * threadIdx.x, 16);
-        __builtin_memcpy(m, a.bin_mass + (size_t)row * kBins + 4 * threadIdx.x, 32);
+struct CountLds {
+    union {
+        double mass[kBins];
+        CutLds<kSmallList> cut;  // (of a row that is finished at once)
+    };
+    alignas(16) uint32_t count[kBins], near[kSmallGroups], group[kSmallGroups];
+    Scan S;
+    LimitsLds L;
+    uint32_t found, reach, word;
+};
+
+// A row's group maxima, every kT-th in a thread, the first kHeld of them in registers.
+struct GroupMaxima {
+    static constexpr uint32_t kHeld = 10;
+    const float *g;
+    uint32_t n;
+    float held[kHeld];
+    AH_DEV GroupMaxima(const SampleArgs &a, uint32_t row) {
+        g = a.group_max + (size_t)row * a.groups;
+        n = a.groups;
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) held[i] = i * kT + threadIdx.x < n ? g[i * kT + threadIdx.x] : -__builtin_inff();
+    }
+    // f(maximum) of each (-inf without one); g(group) of those for which f holds
+    template <class F> AH_DEV void each(F f) const {
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) f(held[i]);
+#pragma unroll 1
+        for (uint32_t j = kHeld * kT + threadIdx.x; j < n; j += kT) f(g[j]);
+    }
+    template <class F, class H> AH_DEV void those(F f, H h) const {
+        uint32_t mask = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) mask |= f(held[i]) ? 1u << i : 0u;
+#pragma unroll 1
+        for (; mask; mask &= mask - 1) h((uint32_t)__builtin_ctz(mask) * kT + threadIdx.x);
+#pragma unroll 1
+        for (uint32_t j = kHeld * kT + threadIdx.x; j < n; j += kT)
+            if (f(g[j])) h(j);
     }
 };
-AH_DEV Limits limits_of(const SampleArgs &a, const Row &r, const Bins &B, Scan &S, LimitsLds &L) {
-    Limits o = {kBins, kBins, kNone, 0, 0.0, 0.0, 0.0};
-    if (!r.need_k && !r.need_p) return o;
+
+// The bin that the k-th largest group maximum is in (the last one if fewer have weight), and how many groups reach it.
+AH_DEV uint32_t bound_of(const Row &r, const GroupMaxima &G, CountLds &D) {
     const uint32_t t = threadIdx.x;
-    const uint32_t *c = B.c;
-    const double *m = B.m;
+    for (uint32_t i = t; i < kBins; i += kT) D.count[i] = 0;
+    if (t < kSmallGroups) D.near[t] = kNone;
+    if (t == 0) {
+        D.found = kBins - 1;
+        D.reach = kNone;
+        D.word = 0;
+    }
+    __syncthreads();
+    G.each([&](float x) {
+        const uint32_t b = bin_at(z_at(r, x));
+        if (b < kBins) atomicAdd(&D.count[b], 1u);
+    });
+    __syncthreads();
+    uint32_t c[4], total;
+    __builtin_memcpy(c, D.count + 4 * t, 16);
+    const uint32_t mine = (c[0] + c[1]) + (c[2] + c[3]);
+    uint32_t cum = scan_u(mine, D.S, total) - mine;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        if (cum < (uint32_t)r.k && cum + c[i] >= (uint32_t)r.k) {
+            D.found = 4 * t + i;
+            D.reach = cum + c[i];
+        }
+        cum += c[i];
+    }
+    __syncthreads();
+    return D.reach == kNone ? total : D.reach;
+}
+
+// A row whose first k tokens are all in `reach` groups (at most kSmallGroups): lists the tokens in bins up to `last`,
+// cuts them and draws.  False if they are more than the list holds.
+AH_DEV bool finish_small(const SampleArgs &a, const Row &r, uint32_t row, const GroupMaxima &G, uint32_t reach, uint32_t last, CountLds &D) {
+    const uint32_t t = threadIdx.x, sub = 8 * (t & 7);
+    CutLds<kSmallList> &C = D.cut;
+    uint32_t total;
+    const float end = (float)(last + 1);
+    G.those([&](float m) { return place_at(z_at(r, m)) < end; }, [&](uint32_t g) { D.near[atomicAdd(&D.word, 1u)] = g; });
+    __syncthreads();
+    if (t < reach) {  // in their order
+        const uint32_t mine = D.near[t];
+        uint32_t rank = 0;
+#pragma unroll 4
+        for (uint32_t j = 0; j < kSmallGroups; j += 4) {
+            uint32_t other[4];
+            __builtin_memcpy(other, D.near + j, 16);
+#pragma unroll
+            for (uint32_t i = 0; i < 4; ++i) rank += other[i] < mine ? 1u : 0u;
+        }
+        D.group[rank] = mine;
+    }
+    __syncthreads();
+    // 32 groups a round, eight threads each
+    constexpr uint32_t kRounds = kSmallGroups * 8 / kT;
+    float x[kRounds][8];
+    uint32_t i0[kRounds], mask[kRounds], packed = 0;
+#pragma unroll
+    for (uint32_t q = 0; q < kRounds; ++q) {
+        const uint32_t g = q * (kT / 8) + t / 8;
+        i0[q] = g < reach ? D.group[g] * kGroup + sub : r.V;
+        load_logits(r, i0[q], x[q]);
+    }
+#pragma unroll
+    for (uint32_t q = 0; q < kRounds; ++q) {
+        mask[q] = 0;
+#pragma unroll
+        for (uint32_t i = 0; i < 8; ++i) mask[q] |= place_at(z_at(r, x[q][i])) < end ? 1u << i : 0u;
+        packed += (uint32_t)__builtin_popcount(mask[q]) << (16 * q);
+    }
+    static_assert(kRounds == 2, "two rounds' counts in one word");
+    const uint32_t before = scan_u(packed, D.S, total) - packed, n = (total & 0xffffu) + (total >> 16);
+    if (n > kSmallList) return false;
+    uint32_t to = before & 0xffffu;
+#pragma unroll
+    for (uint32_t q = 0; q < kRounds; ++q) {
+#pragma unroll 1
+        for (; mask[q]; mask[q] &= mask[q] - 1) {
+            const uint32_t i = i0[q] + (uint32_t)__builtin_ctz(mask[q]);
+            C.key[to] = key_of(r.x[i]);
+            C.idx[to++] = i;
+        }
+        to = (total & 0xffffu) + (before >> 16);
+    }
+    __syncthreads();
+    const Limits o = {0, last, kNone, 0, 0.0, 0.0, 0.0, r.top, last, 0};
+    const bool do_k = n >= (uint32_t)r.k;  // (fewer are all that have weight)
+    Cut c;
+    if (!cut_list(r, o, n, do_k, true, c, C)) return false;
+    // the draw, in the list's order
+    const uint32_t each = (n + kT - 1) / kT, j0 = t * each, j1 = j0 + each < n ? j0 + each : n;
+    const auto weight = [&](uint32_t j) { return kept_weight(r, c, do_k || r.need_p, C.idx[j], C.key[j]); };
+    double own = 0.0, W;
+#pragma unroll 1
+    for (uint32_t j = j0; j < j1; ++j) own += weight(j);
+    double ahead = scan_d(own, C.S, W) - own;
+    const double goal = goal_of(r, W);
+    if (ahead <= goal && ahead + own > goal) {
+#pragma unroll 1
+        for (uint32_t j = j0; j < j1; ++j) {
+            const double w = weight(j);
+            if (ahead <= goal && ahead + w > goal) {
+                a.tokens[row] = (int32_t)C.idx[j];
+                if (a.probs) a.probs[row] = (float)(w / W);
+            }
+            ahead += w;
+        }
+    }
+    return true;
+}
+
+// Calls f(place of a lane's first token in the chunk, its logits) over those groups of a chunk whose largest token's
+// bin is at most `last`, in their order: eight groups a round, eight lanes each (-inf in a lane without), the next
+// round's logits on their way meanwhile.
+template <class F> AH_DEV void each_group(const SampleArgs &a, const Row &r, uint32_t row, uint32_t chunk, uint32_t last, F f) {
+    const uint32_t lane = threadIdx.x & 63, g = chunk * kGroups + lane;
+    const bool in = lane < kGroups && g < a.groups, use = in && bin_at(z_at(r, a.group_max[(size_t)row * a.groups + (in ? g : 0)])) <= last;
+    const uint64_t todo = __builtin_amdgcn_ballot_w64(use);
+    const uint32_t n = (uint32_t)__builtin_popcountll(todo);
+    if (n == 0) return;
+    // lane j: the j-th of the groups
+    const uint32_t rank = __builtin_amdgcn_mbcnt_lo((uint32_t)todo, 0u);
+    const int list = __builtin_amdgcn_ds_permute((int)(4 * (use ? rank : 63u)), (int)lane);
+    float x[8], next[8];
+    uint32_t at, at_next;
+    auto load = [&](uint32_t j) {
+        const uint32_t mine = j + (lane >> 3);
+        at_next = (uint32_t)__builtin_amdgcn_ds_bpermute((int)(4 * (mine & 31)), list) * kGroup + 8 * (lane & 7);
+        load_logits(r, mine < n ? chunk * kChunk + at_next : r.V, next);
+    };
+    load(0);
+    for (uint32_t j = 0; j < n; j += 8) {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = next[i];
+        at = at_next;
+        if (j + 8 < n) load(j + 8);
+        f(at, x);
+    }
+}
+
+// The limits from a row's bins, four of them (c, m) in each thread.
+AH_DEV Limits limits_of(const Row &r, const uint32_t *c, const double *m, Scan &S, LimitsLds &L) {
+    Limits o = {kBins, kBins, kNone, 0, 0.0, 0.0, 0.0, 0, 0, 0};
+    const uint32_t t = threadIdx.x;
     if (t == 0) {
         L.bk = kNone;
         L.g0 = L.g1 = kBins - 1;
@@ -401,434 +780,289 @@ AH_DEV Limits limits_of(const SampleArgs &a, const Row &r, const Bins &B, Scan &
     o.all = all;
     return o;
 }
-// Whether a bin's tokens are listed: bins g0 to g1, and the top-k one where top-p needs its weight.  (No branches.)
-struct Listed {
-    uint32_t from, span, also;
-    AH_DEV Listed(const Limits &o, const Row &r) {
-        const uint32_t to = o.g1 < kBins ? o.g1 : kBins - 1;
-        from = o.g0 <= to ? o.g0 : 0xfffff000u;  // (no bin is that far below it)
-        span = o.g0 <= to ? to - o.g0 : 0u;
-        also = r.need_p ? o.bk : kNone;
-    }
-    AH_DEV bool operator()(uint32_t b) const { return (b - from <= span) | (b == also); }
-};
 
-__global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
-    __shared__ Scan S;
-    __shared__ LimitsLds L;
-    __shared__ uint32_t count[kBins], found;
-    uint32_t row, s0, s1;
-    share(a, row, s0, s1);
-    const Bins B(a, row);
+__global__ void __launch_bounds__(kT, 8) sample_count_kernel(SampleArgs a) {
+    __shared__ CountLds D;
+    uint32_t row, c0, c1;
+    share(a, row, c0, c1);
+    const GroupMaxima G(a, row);  // (on their way before anything is waited for)
     Row r = row_of(a, row);
-    if (r.greedy) return;
-    set_top(r, top_of(a, row, S));
-    if (r.M == -__builtin_inff()) return;
-    Limits o = {0, 0, kNone, 0, 0.0, 0.0, 0.0};
-    if (r.few) o.g1 = bound_of(a, r, row, S, count, found);  // all that reaches the bound is listed
-    else o = limits_of(a, r, B, S, L);
-    const uint32_t lane = threadIdx.x & 63, g0 = o.g0 < kBins ? o.g0 : kBins;
-    const Listed listed(o, r);
-    // the last bin with a token to keep or to list (no bin: tokens without weight, as a whole)
-    const uint32_t end_k = o.bk != kNone ? o.bk : o.g1;
-    const uint32_t last = o.g0 == kBins ? kBins - 1 : end_k > o.g1 ? end_k : o.g1;
-    each_segment(
-        a, r, row, s0, s1, last,
-        [&](uint32_t s, const float *x) {
-            const size_t seg = (size_t)row * a.segs + s;
-            uint32_t n = 0, mask = 0;
-            double sure = 0.0;
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const float z = z_at(r, x[i]);
-                const uint32_t b = bin_at(z);
-                // (no branches: the row's lanes take both sides nearly always)
-                const float w = weight_at(z);
-                sure += (double)(((b < g0) & (w >= r.floor_f)) ? w : 0.0f);
-                mask |= (uint32_t)listed(b) << i;
+    const uint32_t t = threadIdx.x;
+    bool counts = r.need_k || r.need_p;
+    const bool alone = !counts || a.parts == 1 || (r.need_k && (uint32_t)r.k <= kSmallK);
+    if (alone && c0 != 0) return;
+    float top = -__builtin_inff();
+    G.each([&](float m) { top = __builtin_fmaxf(top, m); });
+    set_top(r, max_u(key_of(top), D.S));
+    Limits o = {kBins, kBins, kNone, 0, 0.0, 0.0, 0.0, r.top, kBins - 1, 0};
+    if (r.greedy || r.M == -__builtin_inff()) {
+        if (c0 != 0) return;
+        const unsigned long long key0 = (unsigned long long)row << 8;
+        if (t == 0 && r.bad_t) ah_record(a.status, key0 + AH_ERR_INPUT_RANGE);
+        if (r.M == -__builtin_inff()) {  // nothing to draw
+            if (t == 0) {
+                ah_record(a.status, key0 + AH_ERR_NONFINITE_INPUT);
+                a.tokens[row] = -1;
+                if (a.probs) a.probs[row] = 0.0f;
             }
-            n = (uint32_t)__builtin_popcount(mask);
-            uint32_t total = 0;
-            if (__builtin_amdgcn_ballot_w64(n != 0) != 0ull) {
-                const uint32_t end = wave_prefix<Add>(n);
-                total = last_lane(end);
-                uint32_t at = end - n;
-                if (total <= kSampleSegList) {
-                    uint16_t *list = a.list + seg * kSampleSegList;
-                    for (; mask; mask &= mask - 1) list[at++] = (uint16_t)(8 * lane + (uint32_t)__builtin_ctz(mask));
-                }
+        } else {  // the first group that holds the largest, and in it the first token
+            uint32_t at = kNone;
+            G.those([&](float m) { return m == r.M; }, [&](uint32_t g) { at = __builtin_elementwise_min(at, g); });
+            at = min_u(at, D.S);
+            const uint32_t i = at * kGroup + (t & 63);
+            const uint64_t b = __builtin_amdgcn_ballot_w64(i < r.V && key_of(r.x[i < r.V ? i : 0]) == r.top);
+            if (t == 0) {
+                a.tokens[row] = (int32_t)(at * kGroup + (uint32_t)__builtin_ctzll(b));
+                if (a.probs) a.probs[row] = 1.0f;
             }
-            if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
-            if (lane == 0) {
-                a.seg_mass[seg] = sure;
-                a.seg_count[seg] = total;
-            }
-        },
-        [&](uint32_t s) {
-            a.seg_mass[(size_t)row * a.segs + s] = 0.0;
-            a.seg_count[(size_t)row * a.segs + s] = 0;
-        });
-}
-
-// ---- the cut ----------------------------------------------------------------------------------------
-
-struct DrawLds {
-    alignas(16) double mass[256];
-    alignas(16) uint32_t count[256];
-    Scan S;
-    LimitsLds L;
-    double seg[kSampleMaxSegs];
-    uint32_t start[kSampleMaxSegs];
-    uint32_t key[kSampleList], idx[kSampleList];
-    uint32_t u0, u1;
-    double d0;
-};
-
-// The kept set's last token in the order: keys above `key` are kept, and of those equal to it the ones up
-// to index `last`.
-struct Cut {
-    uint32_t key, last;
-};
-
-// The index of the nth (1 ..) of n tokens in index order that have key `cut`.
-template <class Key, class Index> AH_DEV uint32_t nth_equal(uint32_t n, Key key, Index index, uint32_t cut, uint32_t nth, DrawLds &D) {
-    uint32_t seen = 0;
-    for (uint32_t base = 0; base < n && seen < nth; base += kT) {
-        const uint32_t i = base + threadIdx.x;
-        const bool eq = i < n && key(i) == cut;
-        uint32_t total;
-        const uint32_t at = seen + scan_u(eq, D.S, total);
-        if (eq && at == nth) D.u0 = index(i);
-        seen += total;
+        }
+        o.done = 1;
+        counts = false;
+    } else if (r.need_k) {
+        const uint32_t reach = bound_of(r, G, D);
+        o.last = D.found;
+        if (alone && reach <= kSmallGroups) {
+            o.done = finish_small(a, r, row, G, reach, o.last, D);
+            counts = !o.done;
+        }
+    }
+    if (!counts) {
+        if (t == 0) a.limits[row] = o;
+        return;
+    }
+    const uint32_t last = o.last;
+    if (alone) c1 = a.chunks;
+    __syncthreads();
+    for (uint32_t i = t; i < kBins; i += kT) {
+        D.count[i] = 0;
+        D.mass[i] = 0.0;
     }
     __syncthreads();
-    return D.u0;
-}
-
-// The digit at which keys between lo and hi first differ, as a shift, and what they share above it.
-AH_DEV int first_digit(uint32_t lo, uint32_t hi, uint32_t &shared) {
-    const uint32_t x = lo ^ hi;
-    const int shift = x ? (31 - __builtin_clz(x)) / 8 * 8 : 0;
-    shared = shift == 24 ? 0 : hi >> (shift + 8) << (shift + 8);
-    return shift;
-}
-
-// The cut over n tokens in index order (a list, or the whole row), by digits of the keys.  in_k(key) and
-// in_p(key): whether such a token counts for the top-k and for the top-p limit.  need: tokens that top-k still
-// keeps of its own; W0: the weight ahead of those (without top-k: of every token); before: the weight ahead of
-// top-p's.
-template <class Key, class Index, class InK, class InP>
-AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, InP in_p, bool do_k, uint32_t need, double W0, double before,
-                      DrawLds &D) {
-    const uint32_t t = threadIdx.x;
-    Cut c = {0, kNone};
-    uint32_t keep = 0, cut_k = 0;  // of those at the cut
-    bool partial = false;
-    if (do_k) {
-        uint32_t lo = kNone, hi = 0;
-        for (uint32_t i = t; i < n; i += kT) {
-            const uint32_t k = key(i);
-            if (in_k(k)) {
-                lo = __builtin_elementwise_min(lo, k);
-                hi = __builtin_elementwise_max(hi, k);
-            }
-        }
-        lo = min_u(lo, D.S);
-        hi = max_u(hi, D.S);
-        for (int shift = first_digit(lo, hi, cut_k); shift >= 0; shift -= 8) {
-            __syncthreads();
-            D.count[t] = 0;
-            __syncthreads();
-            for (uint32_t i = t; i < n; i += kT) {
-                const uint32_t k = key(i);
-                if (in_k(k) && (shift == 24 || (k >> (shift + 8)) == (cut_k >> (shift + 8)))) atomicAdd(&D.count[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            const uint32_t mine = D.count[255 - t];
-            uint32_t total;
-            const uint32_t cum = scan_u(mine, D.S, total);
-            if (cum >= need && cum - mine < need) {
-                D.u0 = 255 - t;
-                D.u1 = cum - mine;
-            }
-            __syncthreads();
-            cut_k |= D.u0 << shift;
-            need -= D.u1;
-        }
-        keep = need;
-        partial = D.count[D.u0] > need;
-        c.key = cut_k;
-    }
-    if (r.need_p) {
-        const double w_cut = do_k ? (double)weight_at(z_of(r, cut_k)) : 0.0;
-        double W = W0;
-        if (do_k) {
-            double s = 0.0;
-            for (uint32_t i = t; i < n; i += kT) {
-                const uint32_t k = key(i);
-                if (in_k(k) && k > cut_k) s += (double)weight_at(z_of(r, k));
-            }
-            W += sum_d(s, D.S) + (double)keep * w_cut;
-        }
-        double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
-        goal = goal < 1.0 ? 1.0 : goal;  // the first token always
-        uint32_t cut_p = 0, all = 0, lo = do_k && in_p(cut_k) ? cut_k : kNone, hi = lo == kNone ? 0u : cut_k;
-        for (uint32_t i = t; i < n; i += kT) {
-            const uint32_t k = key(i);
-            if (in_p(k) && !(do_k && k <= cut_k)) {
-                lo = __builtin_elementwise_min(lo, k);
-                hi = __builtin_elementwise_max(hi, k);
-            }
-        }
-        lo = min_u(lo, D.S);
-        hi = max_u(hi, D.S);
-        for (int shift = first_digit(lo, hi, cut_p); shift >= 0; shift -= 8) {
-            __syncthreads();
-            D.mass[t] = 0.0;
-            D.count[t] = 0;
-            __syncthreads();
-            for (uint32_t i = t; i < n; i += kT) {
-                const uint32_t k = key(i);
-                if (!in_p(k) || (do_k && k <= cut_k) || !(shift == 24 || (k >> (shift + 8)) == (cut_p >> (shift + 8)))) continue;
-                unsafeAtomicAdd(&D.mass[(k >> shift) & 255u], (double)weight_at(z_of(r, k)));
-                atomicAdd(&D.count[(k >> shift) & 255u], 1u);
-            }
-            __syncthreads();
-            double mine = D.mass[255 - t];
-            uint32_t cnt = D.count[255 - t];
-            if (do_k && in_p(cut_k) && (shift == 24 || (cut_k >> (shift + 8)) == (cut_p >> (shift + 8))) && 255 - t == ((cut_k >> shift) & 255u)) {
-                mine += (double)keep * w_cut;
-                cnt += keep;
-            }
-            double total;
-            const double cum = before + scan_d(mine, D.S, total);
-            if (cum >= goal && cum - mine < goal) {
-                D.u0 = 255 - t;
-                D.u1 = cnt;
-                D.d0 = cum - mine;
-            }
-            __syncthreads();
-            cut_p |= D.u0 << shift;
-            all = D.u1;
-            before = D.d0;
-        }
-        const double w = (double)weight_at(z_of(r, cut_p)), q = (goal - before) / w;
-        uint32_t m = q >= (double)all ? all : q <= 1.0 ? 1u : (uint32_t)q;
-        while (m < all && before + (double)m * w < goal) ++m;
-        while (m > 1 && before + (double)(m - 1) * w >= goal) --m;
-        partial = m < all || (do_k && cut_p == cut_k && partial);
-        keep = m;
-        c.key = cut_p;
-    }
-    if (partial) c.last = nth_equal(n, key, index, c.key, keep, D);
-    return c;
-}
-
-// The cut of at most kT / P listed tokens: P neighbouring threads a token, its place among the others by comparing
-// with each (four at a time; tokens that do not count are key 0, below every key).
-template <uint32_t P> AH_DEV Cut place_cut(const Row &r, const Limits &o, uint32_t n, bool do_k, DrawLds &D) {
-    const uint32_t t = threadIdx.x, me = t / P, part = t % P;
-    const bool live = me < n;
-    const uint32_t k = live ? D.key[me] : 0u;
-    const float z = z_of(r, k);
-    const uint32_t b = bin_at(z);
-    const bool ink = live && do_k && (r.few || b == o.bk), inp = live && b >= o.g0 && b <= o.g1;
-    const double w = live ? (double)weight_at(z) : 0.0;
-    bool keep = live;
-    if (do_k) {
-        if (part == 0) D.count[me] = ink ? k : 0u;
-        __syncthreads();
-        uint32_t rank = 0;
-#pragma unroll 2
-        for (uint32_t j = 4 * part; j < n; j += 4 * P) {
-            uint32_t other[4];
-            __builtin_memcpy(other, D.count + j, 16);
+    for (uint32_t c = c0 + __builtin_amdgcn_readfirstlane(t >> 6); c < c1; c += kW)
+        each_group(a, r, row, c, last, [&](uint32_t, const float *x) {
 #pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) rank += other[i] > (j + i < me ? k - 1 : k) ? 1u : 0u;
-        }
+            for (int i = 0; i < 8; ++i) {
+                const float z = z_at(r, x[i]);
+                const uint32_t b = bin_at(z);
+                if (b > last) continue;
+                if (r.need_k) atomicAdd(&D.count[b], 1u);
+                if (r.need_p) unsafeAtomicAdd(&D.mass[b], (double)weight_at(z));
+            }
+        });
+    __syncthreads();
+    uint32_t n[4];
+    double m[4];
+    if (alone) {
 #pragma unroll
-        for (uint32_t q = 1; q < P; q <<= 1) rank += (uint32_t)__shfl_xor((int)rank, (int)q, 64);
-        keep = ink ? o.before_k + rank < (uint32_t)r.k : live;
-    }
-    if (r.need_p) {
-        const double W = do_k || r.few ? o.mass_k + sum_d((ink || r.few) && keep && part == 0 ? w : 0.0, D.S) : o.all;
-        double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
-        goal = goal < 1.0 ? 1.0 : goal;
-        __syncthreads();
-        if (part == 0) {
-            D.count[me] = inp && keep ? k : 0u;
-            D.mass[me] = inp && keep ? w : 0.0;
+        for (int i = 0; i < 4; ++i) {
+            n[i] = D.count[4 * t + i];
+            m[i] = D.mass[4 * t + i];
         }
-        __syncthreads();
-        double before = 0.0;
-#pragma unroll 2
-        for (uint32_t j = 4 * part; j < n; j += 4 * P) {
-            uint32_t other[4];
-            double m[4];
-            __builtin_memcpy(other, D.count + j, 16);
-            __builtin_memcpy(m, D.mass + j, 32);
-#pragma unroll
-            for (uint32_t i = 0; i < 4; ++i) before += other[i] > (j + i < me ? k - 1 : k) ? m[i] : 0.0;
-        }
-#pragma unroll
-        for (uint32_t q = 1; q < P; q <<= 1) before += __shfl_xor(before, (int)q, 64);
-        keep = inp && keep && o.mass_0 + before < goal;
     } else {
-        keep = ink && keep;
+        uint32_t *bc = a.bin_count + (size_t)row * kBins;
+        double *bm = a.bin_mass + (size_t)row * kBins;
+        for (uint32_t i = t; i <= last; i += kT) {
+            if (D.count[i]) atomicAdd(bc + i, D.count[i]);
+            if (D.mass[i] > 0.0) unsafeAtomicAdd(bm + i, D.mass[i]);
+        }
+        if (!last_of_row(a, row, D.word)) return;
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            n[i] = get(bc + 4 * t + i);
+            m[i] = get(bm + 4 * t + i);
+        }
     }
-    Cut c;
-    c.key = min_u(keep ? k : kNone, D.S);
-    c.last = max_u(keep && k == c.key ? D.idx[me] : 0u, D.S);
-    return c;
+    o = limits_of(r, n, m, D.S, D.L);
+    o.top = r.top;
+    // the last bin with a token to keep or to list (no bin: tokens without weight, as a whole)
+    const uint32_t end_k = o.bk != kNone ? o.bk : o.g1;
+    o.last = o.g0 == kBins ? kBins - 1 : end_k > o.g1 ? end_k : o.g1;
+    if (t == 0) a.limits[row] = o;
 }
 
-__global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
-    __shared__ DrawLds D;
-    const uint32_t row = blockIdx.x, t = threadIdx.x;
-    const Bins B(a, row);
-    // this thread's segments: their certain weights, and how many tokens each lists
-    const uint32_t each = (a.segs + kT - 1) / kT, g0 = t * each < a.segs ? t * each : a.segs, g1 = g0 + each < a.segs ? g0 + each : a.segs;
-    uint32_t n_mine = 0;
+// ---- draw -------------------------------------------------------------------------------------------
+
+struct DrawLds {
+    CutLds<kSampleList> cut;
+    double mass[kSampleMaxChunks];
+    uint32_t start[kSampleMaxChunks];
+};
+
+// SAME: in the launch that gathered.
+template <bool SAME, class T> AH_DEV T gathered(const T *p) { return SAME ? get(p) : *p; }
+
+template <bool SAME> AH_DEV void draw(const SampleArgs &a, uint32_t row, const Limits &o, DrawLds &D) {
+    CutLds<kSampleList> &C = D.cut;
+    const uint32_t t = threadIdx.x;
+    // this thread's chunks: their certain weights, and how many tokens each lists
+    const uint32_t each = (a.chunks + kT - 1) / kT, g0 = t * each < a.chunks ? t * each : a.chunks, g1 = g0 + each < a.chunks ? g0 + each : a.chunks;
+    uint32_t n_mine = 0, n;
     bool full = false;
     for (uint32_t s = g0; s < g1; ++s) {
-        const uint32_t c = a.seg_count[(size_t)row * a.segs + s];
-        D.seg[s] = a.seg_mass[(size_t)row * a.segs + s];
+        const uint32_t c = gathered<SAME>(&a.chunk_count[(size_t)row * a.chunks + s]);
+        D.mass[s] = gathered<SAME>(&a.chunk_mass[(size_t)row * a.chunks + s]);
         D.start[s] = c;
-        full |= c > kSampleSegList;
+        full |= c > kSampleChunkList;
         n_mine += c;
     }
     Row r = row_of(a, row);
-    const unsigned long long key0 = (unsigned long long)row << 8;
-    if (t == 0 && r.bad_t) ah_record(a.status, key0 + AH_ERR_INPUT_RANGE);
-    set_top(r, top_of(a, row, D.S));
-    if (r.M == -__builtin_inff()) {  // nothing to draw
-        if (t == 0) {
-            ah_record(a.status, key0 + AH_ERR_NONFINITE_INPUT);
-            a.tokens[row] = -1;
-            if (a.probs) a.probs[row] = 0.0f;
-        }
-        return;
+    set_top(r, o.top);
+    uint32_t at = scan_u(n_mine, C.S, n) - n_mine;  // where each chunk's listed tokens start
+    for (uint32_t s = g0; s < g1; ++s) {
+        const uint32_t c = D.start[s];
+        D.start[s] = at;
+        for (const uint32_t e = at + c; at < e; ++at)
+            if (at < kSampleList) C.idx[at] = s;  // the chunk of each
     }
-    if (r.greedy) {  // the first group that holds the largest, and in it the first token
-        const uint32_t *g = a.group_max + (size_t)row * a.segs * kGroups;
-        uint32_t at = kNone;
-        for (uint32_t i = t; i < a.segs * kGroups; i += kT)
-            if (g[i] == r.top) at = __builtin_elementwise_min(at, i);
-        at = min_u(at, D.S);
-        const uint32_t i = at * kGroup + t;
-        const bool here = t < kGroup && i < r.V && key_of(r.x[i]) == r.top;
-        const uint64_t b = __builtin_amdgcn_ballot_w64(here);
-        if (t == 0) {
-            a.tokens[row] = (int32_t)(at * kGroup + (uint32_t)__builtin_ctzll(b));
-            if (a.probs) a.probs[row] = 1.0f;
-        }
-        return;
-    }
-    Limits o = {0, kBins - 1, kNone, 0, 0.0, 0.0, 0.0};
-    if (!r.few) o = limits_of(a, r, B, D.S, D.L);
-    uint32_t n;
-    {  // where each segment's listed tokens start
-        uint32_t at = scan_u(n_mine, D.S, n) - n_mine;
-        for (uint32_t s = g0; s < g1; ++s) {
-            const uint32_t c = D.start[s];
-            D.start[s] = at;
-            at += c;
-        }
-    }
-    full = max_u(full, D.S) != 0 || n > kSampleList;
-    // (of few, every listed token counts for both limits; fewer than k of them are all that have weight)
-    const bool do_k = r.few ? n >= (uint32_t)r.k : o.bk != kNone, limited = do_k || r.need_p;
+    full = max_u(full, C.S) != 0 || n > kSampleList;
+    const bool do_k = o.bk != kNone, limited = do_k || r.need_p;
     Cut c = {0, kNone};
-    auto kept = [&](uint32_t i, uint32_t k) -> double {
-        if (limited && (k < c.key || (k == c.key && i > c.last))) return 0.0;
-        const float z = z_of(r, k);
-        if (bin_at(z) == kBins) return 0.0;
-        const double w = (double)weight_at(z);
-        return w < r.floor_w ? 0.0 : w;
-    };
-    if (full) {
+    if (!full && n) {
+        // a load of the list and one of the logit follow each other: four tokens a thread at once
+        for (uint32_t j0 = t; j0 < n; j0 += 4 * kT) {
+            uint32_t i[4], j[4];
+            float x[4];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                j[q] = j0 + q * kT < n ? j0 + q * kT : j0;  // (past the list: the thread's first once more)
+                i[q] = C.idx[j[q]];
+            }
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q)
+                i[q] = i[q] * kChunk + gathered<SAME>(&a.list[((size_t)row * a.chunks + i[q]) * kSampleChunkList + (j[q] - D.start[i[q]])]);
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) x[q] = r.x[i[q]];
+#pragma unroll
+            for (uint32_t q = 0; q < 4; ++q) {
+                C.idx[j[q]] = i[q];
+                C.key[j[q]] = key_of(x[q]);
+            }
+        }
+        __syncthreads();
+        full = !cut_list(r, o, n, do_k, false, c, C);
+#pragma unroll 1
+        for (uint32_t j = t; j < n && !full; j += kT) {
+            const double w = kept_weight(r, c, limited, C.idx[j], C.key[j]);
+            if (w > 0.0) unsafeAtomicAdd(&D.mass[C.idx[j] / kChunk], w);
+        }
+    }
+    if (full) {  // too many equal, or nearly equal: over the whole row
         const auto key = [&](uint32_t i) { return key_of(r.x[i]); };
         const auto index = [](uint32_t i) { return i; };
         const auto weighs = [&](uint32_t k) { return bin_at(z_of(r, k)) < kBins; };
-        if (r.few && !do_k) {
-            double w = 0.0;
-            for (uint32_t i = t; i < r.V; i += kT) w += (double)weight_at(z_of(r, key(i)));
-            o.all = sum_d(w, D.S);
-        }
-        c = select_cut(r, r.V, key, index, weighs, weighs, do_k, (uint32_t)r.k, do_k ? 0.0 : o.all, 0.0, D);
         __syncthreads();
-        for (uint32_t s = t >> 6; s < a.segs; s += kT / 64) {
-            uint32_t k[8];
-            load_keys(r, s, k);
+        c = select_cut(r, r.V, key, index, weighs, weighs, do_k, (uint32_t)r.k, do_k ? 0.0 : o.all, 0.0, C);
+        __syncthreads();
+#pragma unroll 1
+        for (uint32_t s = t >> 6; s < a.chunks; s += kW) {
             double w = 0.0;
-#pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) w += kept(s * kSeg + 8 * (t & 63) + i, k[i]);
+#pragma unroll 1
+            for (uint32_t i = s * kChunk + (t & 63), q = 0; q < kChunk / 64; ++q, i += 64)
+                if (i < r.V) w += kept_weight(r, c, limited, i, key_of(r.x[i]));
             w = last_lane(wave_prefix<Add>(w));
-            if ((t & 63) == 0) D.seg[s] = w;
-        }
-    } else if (n) {
-        // listed token j is in the last segment that starts at or before it
-        __syncthreads();
-        for (uint32_t j = t; j < n; j += kT) {
-            uint32_t s = 0;
-            for (uint32_t step = kSampleMaxSegs / 2; step; step >>= 1)
-                if (s + step < a.segs && D.start[s + step] <= j) s += step;
-            const uint32_t i = s * kSeg + a.list[((size_t)row * a.segs + s) * kSampleSegList + (j - D.start[s])];
-            D.idx[j] = i;
-            D.key[j] = key_of(r.x[i]);
-        }
-        __syncthreads();
-        const auto bin = [&](uint32_t k) { return bin_at(z_of(r, k)); };
-        if (n <= kT) {
-            c = n <= kT / 4 ? place_cut<4>(r, o, n, do_k, D) : n <= kT / 2 ? place_cut<2>(r, o, n, do_k, D) : place_cut<1>(r, o, n, do_k, D);
-        } else {
-            const auto key = [&](uint32_t i) { return D.key[i]; };
-            const auto index = [&](uint32_t i) { return D.idx[i]; };
-            const auto in_k = [&](uint32_t k) { return r.few || bin(k) == o.bk; };
-            const auto in_p = [&](uint32_t k) { return bin(k) >= o.g0 && bin(k) <= o.g1; };
-            c = select_cut(r, n, key, index, in_k, in_p, do_k, (uint32_t)r.k - o.before_k, do_k ? o.mass_k : o.all, o.mass_0, D);
-        }
-        for (uint32_t j = t; j < n; j += kT) {
-            const double w = kept(D.idx[j], D.key[j]);
-            if (w > 0.0) unsafeAtomicAdd(&D.seg[D.idx[j] / kSeg], w);
+            if ((t & 63) == 0) D.mass[s] = w;
         }
     }
     __syncthreads();
-    // the segment, then the token in it
+    // the chunk, then the token in it
+    if (t == 0) C.u0 = 0;
     double W, own = 0.0;
-    for (uint32_t s = g0; s < g1; ++s) own += D.seg[s];
-    double ahead = scan_d(own, D.S, W) - own;
-    double goal = __builtin_floor((double)(r.u > 0.0f ? r.u : 0.0f) * W);
-    goal = goal < W ? goal : W - 1.0;
+    for (uint32_t s = g0; s < g1; ++s) own += D.mass[s];
+    double ahead = scan_d(own, C.S, W) - own;
+    const double goal = goal_of(r, W);
     for (uint32_t s = g0; s < g1; ++s) {
-        const double w = D.seg[s];
+        const double w = D.mass[s];
         if (ahead <= goal && ahead + w > goal) {
-            D.u0 = s;
-            D.d0 = ahead;
+            C.u0 = s;
+            C.d0 = ahead;
         }
         ahead += w;
     }
     __syncthreads();
-    if (t >= 64) return;
-    const uint32_t s = D.u0;
+    const uint32_t i0 = C.u0 * kChunk + 8 * t;
     uint32_t k[8];
-    double w[8], mine = 0.0;
-    load_keys(r, s, k);
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        w[i] = kept(s * kSeg + 8 * t + i, k[i]);
-        mine += w[i];
-    }
-    double cum = D.d0 + wave_prefix<Add>(mine) - mine;
-#pragma unroll
-    for (uint32_t i = 0; i < 8; ++i) {
-        if (cum <= goal && cum + w[i] > goal) {
-            a.tokens[row] = (int32_t)(s * kSeg + 8 * t + i);
-            if (a.probs) a.probs[row] = (float)(w[i] / W);
+    load_keys(r, i0, k);
+    __builtin_memcpy(C.key + 8 * t, k, 32);  // (its own alone)
+    double mine = 0.0, total;
+#pragma unroll 1
+    for (uint32_t i = 0; i < 8; ++i) mine += kept_weight(r, c, limited, i0 + i, C.key[8 * t + i]);
+    double cum = C.d0 + scan_d(mine, C.S, total) - mine;
+    if (cum <= goal && cum + mine > goal) {
+#pragma unroll 1
+        for (uint32_t i = 0; i < 8; ++i) {
+            const double w = kept_weight(r, c, limited, i0 + i, C.key[8 * t + i]);
+            if (cum <= goal && cum + w > goal) {
+                a.tokens[row] = (int32_t)(i0 + i);
+                if (a.probs) a.probs[row] = (float)(w / W);
+            }
+            cum += w;
         }
-        cum += w[i];
     }
 }
+
+__global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
+    __shared__ DrawLds D;
+    const Limits o = a.limits[blockIdx.x];
+    if (!o.done) draw<false>(a, blockIdx.x, o, D);
+}
+
+// ---- gather -----------------------------------------------------------------------------------------
+
+// DRAW: with the draw, by the row's workgroup that arrives last.
+template <bool DRAW> __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
+    __shared__ typename std::conditional<DRAW, DrawLds, char>::type D;
+    uint32_t row, c0, c1;
+    share(a, row, c0, c1);
+    const Limits o = a.limits[row];
+    if (o.done) return;
+    Row r = row_of(a, row);
+    set_top(r, o.top);
+    const uint32_t lane = threadIdx.x & 63;
+    // places among the bins: kept below `sure_to`, listed from `from` up to `to` and, where top-p needs the weight of
+    // the first k, in bin bk.  (No branches over the tokens: a wave takes both sides nearly always.)
+    const float sure_to = (float)o.g0, from = (float)o.g0, to = (float)((o.g1 < kBins ? o.g1 : kBins - 1) + 1);
+    const bool also = r.need_p && o.bk != kNone;
+    const float also_from = (float)o.bk, also_to = (float)(o.bk + 1);
+    for (uint32_t c = c0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < c1; c += kW) {
+        const size_t chunk = (size_t)row * a.chunks + c;
+        uint16_t *list = a.list + chunk * kSampleChunkList;
+        double sure = 0.0;
+        uint32_t listed = 0;
+        each_group(a, r, row, c, o.last, [&](uint32_t at, const float *x) {
+            uint32_t mask = 0;
+#pragma unroll
+            for (uint32_t i = 0; i < 8; ++i) {
+                const float z = z_at(r, x[i]), y = place_at(z), w = weight_at(z);
+                sure += (double)(((y < sure_to) & (w >= r.floor_f)) ? w : 0.0f);
+                mask |= ((y >= from) & (y < to)) ? 1u << i : 0u;
+                if (also) mask |= ((y >= also_from) & (y < also_to)) ? 1u << i : 0u;
+            }
+            if (__builtin_amdgcn_ballot_w64(mask != 0) == 0ull) return;
+            const uint32_t n = (uint32_t)__builtin_popcount(mask), sum = wave_prefix<Add>(n);
+            uint32_t place = listed + sum - n;
+            listed += last_lane(sum);
+            if (listed <= kSampleChunkList)
+                for (; mask; mask &= mask - 1) {
+                    const uint16_t v = (uint16_t)(at + (uint32_t)__builtin_ctz(mask));
+                    if (DRAW) put(list + place++, v);
+                    else list[place++] = v;
+                }
+        });
+        if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
+        if (lane == 0) {
+            put(a.chunk_mass + chunk, sure);
+            put(a.chunk_count + chunk, listed);
+        }
+    }
+    if constexpr (DRAW) {
+        if (a.parts > 1 && !last_of_row(a, row, D.cut.u1)) return;
+        __syncthreads();
+        draw<true>(a, row, o, D);
+    }
+}
+
+static_assert(kChunk == 8 * kT, "the draw takes a chunk at once");
+static_assert(kSampleMaxChunks * kChunk >= 1u << 20, "the longest row");
 
 } // namespace
 
@@ -836,31 +1070,39 @@ hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream) {
     const dim3 grid(a.n_rows * a.parts), block(kT);
     hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, stream, a);
     hipLaunchKernelGGL(sample_count_kernel, grid, block, 0, stream, a);
-    hipLaunchKernelGGL(sample_gather_kernel, grid, block, 0, stream, a);
-    hipLaunchKernelGGL(sample_draw_kernel, dim3(a.n_rows), block, 0, stream, a);
+    if (a.draw) {
+        hipLaunchKernelGGL(sample_gather_kernel<true>, grid, block, 0, stream, a);
+    } else {
+        hipLaunchKernelGGL(sample_gather_kernel<false>, grid, block, 0, stream, a);
+        hipLaunchKernelGGL(sample_draw_kernel, dim3(a.n_rows), block, 0, stream, a);
+    }
     return hipGetLastError();
 }
 
 // Bytes of scratch, and (with a base) the pointers in it.
 size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
-    a.segs = (a.n_vocab + kSeg - 1) / kSeg;
-    // at most eight workgroups a CU (all that a CU holds: one more would start when the first ends), each of whole
-    // rounds of its four waves over one row's segments
-    const uint64_t all = (uint64_t)a.n_rows * a.segs, want = 8ull * cus / a.n_rows, parts = want < 1 ? 1 : want;
-    a.per = (uint32_t)(((a.segs + parts - 1) / parts + 3) / 4 * 4);
-    a.parts = (a.segs + a.per - 1) / a.per;
+    a.groups = (a.n_vocab + kGroup - 1) / kGroup;
+    a.chunks = (a.n_vocab + kChunk - 1) / kChunk;
+    // at most eight workgroups a CU (all that a CU holds: one more would start when the first ends); several of a
+    // row where there is a counter for their arrivals
+    const uint32_t want = a.n_rows <= a.n_counts ? 8 * cus / a.n_rows : 1, parts = want < 1 ? 1 : want;
+    a.per = (a.chunks + parts - 1) / parts;
+    a.parts = (a.chunks + a.per - 1) / a.per;
+    // A launch less where the draw's LDS leaves every workgroup its place (three a CU)
+    a.draw = a.n_rows * a.parts <= 3 * cus;
+    const size_t rows = a.n_rows;
     size_t at = 0;
     auto take = [&](size_t bytes) {
         uint8_t *p = base ? base + at : nullptr;
         at += (bytes + 255) & ~(size_t)255;
         return p;
     };
-    a.bin_mass = reinterpret_cast<double *>(take(8 * (size_t)a.n_rows * kBins));
-    a.seg_mass = reinterpret_cast<double *>(take(8 * (size_t)all));
-    a.bin_count = reinterpret_cast<uint32_t *>(take(4 * (size_t)a.n_rows * kBins));
-    a.group_max = reinterpret_cast<uint32_t *>(take(4 * (size_t)all * kGroups));
-    a.seg_max = reinterpret_cast<uint32_t *>(take(4 * (size_t)all));
-    a.seg_count = reinterpret_cast<uint32_t *>(take(4 * (size_t)all));
-    a.list = reinterpret_cast<uint16_t *>(take(2 * (size_t)all * kSampleSegList));
+    a.limits = reinterpret_cast<SampleLimits *>(take(sizeof(SampleLimits) * rows));
+    a.bin_mass = reinterpret_cast<double *>(take(8 * rows * kBins));
+    a.chunk_mass = reinterpret_cast<double *>(take(8 * rows * a.chunks));
+    a.bin_count = reinterpret_cast<uint32_t *>(take(4 * rows * kBins));
+    a.group_max = reinterpret_cast<float *>(take(4 * rows * a.groups));
+    a.chunk_count = reinterpret_cast<uint32_t *>(take(4 * rows * a.chunks));
+    a.list = reinterpret_cast<uint16_t *>(take(2 * rows * a.chunks * kSampleChunkList));
     return at;
 }

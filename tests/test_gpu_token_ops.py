@@ -603,6 +603,33 @@ def test_sampling_of_flat_rows(dev, V, kind, k, p):
         assert abs(prob[0] / (w[tok[0]] / run[-1]) - 1) <= 2.0 ** -17 + 4.0 / (w > 0).sum()
 
 
+@pytest.mark.parametrize("rows,V", [(13, 151936), (300, 5000), (900, 2049), (3100, 2100)])
+@pytest.mark.parametrize("order", ["random", "falling"])
+def test_sampling_of_many_rows(dev, rows, V, order):
+    """Many rows of mixed parameters in one call: few and several workgroups a row, rows that end early beside rows
+    that do not, likely tokens spread over the row or next to each other (as in a vocabulary by frequency)."""
+    rng = np.random.default_rng(rows)
+    x = (2.5 * rng.standard_normal((rows, V))).astype(np.float32)
+    if order == "falling":
+        x = np.ascontiguousarray(np.sort(x, axis=1)[:, ::-1])
+    T = rng.choice([0.0, 0.3, 0.7, 1.3], rows).astype(np.float32)
+    k = rng.choice([0, 1, 2, 20, 56, 57, 64, 300, 1000], rows).astype(np.int32)
+    p = rng.choice([1.0, 0.9, 0.5], rows).astype(np.float32)
+    u, want, prob = [], [], []
+    for i in range(rows):
+        if T[i] > 0 and p[i] < 1:
+            p[i] = safe_p(x[i], float(T[i]), int(k[i]), float(p[i]))
+        w, _, _ = kept_weights(x[i], float(T[i]), int(k[i]), float(p[i]), 0.0)
+        run = np.cumsum(w)
+        t = int(rng.choice(np.nonzero(w > 2e-5 * run[-1])[0]))
+        u.append((run[t] - w[t] / 2) / run[-1])
+        want.append(t)
+        prob.append(w[t] / run[-1])
+    st, tok, got = sample(dev, x, u, T, k, p)
+    assert st == OK and tok.tolist() == want
+    assert (np.abs(got - np.array(prob)) <= 2.0 ** -17 * np.array(prob)).all()
+
+
 def test_sampling_defaults_infinities_and_refusals(dev):
     rng = np.random.default_rng(0)
     x = rng.standard_normal((4, 3000)).astype(np.float32)
