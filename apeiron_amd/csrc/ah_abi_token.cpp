@@ -264,16 +264,17 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
         chunk = (tiles + splits - 1) / splits;
     } else {
         // With few units a piece's tiles (0.7 us for each of a wave) stand against the join (0.1 us a piece):
-        // sqrt(1.75 tiles) pieces, past 40 of them two joins and 16 tiles a piece.  Once that passes a
-        // workgroup a CU, pieces of 16 tiles (a workgroup costs its start and end).  One sequence of 4001 keys
-        // in pieces of 4, 8, 16 and 24 tiles 10.6, 10.0, 10.7 and 13.3 us, 16 windows of 4096 15.1, 11.7, 10.6 and
-        // 11.6, 128 sequences of 1000 24, 19, 16 and 16.
-        const double wish = std::sqrt(1.75 * (double)tiles);
+        // sqrt(1.75 tiles) pieces, past 40 of them two joins and 16 tiles a piece.  One sequence of 4001 keys in pieces
+        // of 4, 8, 16 and 24 tiles: 10.6, 10.0, 10.7 and 13.3 us.  Once that passes a workgroup a CU (two, where two
+        // joins pay for themselves: 120000 keys in 256 workgroups 24.5 us, in 469 21.8), pieces of 32 tiles, since a
+        // workgroup costs its start and end.  With 2 KV heads of 128, in pieces of 16, 32 and 64 tiles: 128 sequences
+        // of 1000 keys 16.6, 13.4 and 13.4 us, of 4000 41.9, 35.8 and 35.6; 64 of 1 to 16384 52, 46 and 52.
+        const double wish = std::sqrt(1.75 * (double)tiles), groups = wish <= 40.0 ? 256.0 : 512.0;
         double pieces = wish <= 40.0 ? wish : (double)tiles / 16.0;
-        if (pieces * (double)base > 256.0) {
-            const double most_pieces = (double)(kAttnGroups / base), by_tiles = (double)tiles / 16.0;
+        if (pieces * (double)base > groups) {
+            const double most_pieces = (double)(kAttnGroups / base), by_tiles = (double)tiles / 32.0;
             pieces = by_tiles < most_pieces ? by_tiles : most_pieces;
-            pieces = pieces * (double)base > 256.0 ? pieces : 256.0 / (double)base;
+            pieces = pieces * (double)base > groups ? pieces : groups / (double)base;
         }
         chunk = pieces < 1.0 ? tiles : 4 * (size_t)((double)tiles / (4.0 * pieces) + 0.5);  // whole rounds of the four waves
     }
