@@ -169,7 +169,7 @@ AH_DEV void q_scale(float scale, float top, float &up, float &f) {
 // A tile's K is used first and its V last, so the next tile's K loads go out as soon as the scores are
 // formed and its V loads as soon as the output is: a wave always has half a tile on its way.
 template <int D, bool PACK>
-__global__ void __launch_bounds__(256, D == 256 ? 2 : 4) attn_rows_kernel(AttnArgs a) {
+__global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_rows_kernel(AttnArgs a) {
     constexpr int NJ = D / 32;  // contraction steps of K q, and blocks of channels
     constexpr uint32_t R = PACK ? 8 : 16;
     extern __shared__ float lds[];
