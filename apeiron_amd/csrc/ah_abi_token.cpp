@@ -14,12 +14,122 @@ constexpr size_t kMaxU32 = 0x7fffffff;
 constexpr size_t kAttnGroups = 2048;
 static_assert(kAttnGroups <= kCounts, "an entry for each unit and each group of pieces");
 
+constexpr size_t kMaxGrid = ((size_t)1 << 32) / 256 - 1;  // workgroups of 256 threads in a launch
+
 bool tokens_ok(const ah_kv4_tokens *t) {
     return t->d_seq && t->d_pos && t->d_table && t->n_seq && t->table_stride && t->n_tok <= kMaxU32 && t->n_seq <= kMaxU32 &&
            t->table_stride <= kMaxU32;
 }
 KvTokens tokens_of(const ah_kv4_tokens *t) {
     return {t->d_seq, t->d_pos, t->d_table, (uint32_t)t->n_tok, (uint32_t)t->n_seq, (uint32_t)t->table_stride};
+}
+
+// The tiles that a sequence's rows see at most.
+size_t most_tiles(const AttnArgs &a, size_t max_ctx, size_t max_q) {
+    const size_t room = (size_t)a.table_stride << a.c.page_shift, tiles = ((max_ctx < room ? max_ctx : room) + 31) / 32;
+    if (!a.window) return tiles;
+    const size_t seen = (a.window + max_q + 31) / 32 + 1 + ((size_t)a.sinks + 31) / 32;
+    return tiles < seen ? tiles : seen;
+}
+
+// Room for the partial results of `rows` rows in each of a.splits pieces.
+int32_t attn_scratch(ah_ctx *ctx, AttnArgs &a, size_t rows) {
+    if (a.splits == 1) return AH_OK;
+    const size_t o = align256(a.splits * rows * a.c.dim * sizeof(float));
+    const int32_t st = ensure_scratch(ctx, o + a.splits * rows * 2 * sizeof(float));
+    if (st) return st;
+    a.part_o = static_cast<float *>(ctx->scratch);
+    a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch) + o);
+    a.count = ctx->d_count;
+    return AH_OK;
+}
+// At most these pieces: 256 MiB of partial results.
+size_t most_pieces(const AttnArgs &a, size_t rows) {
+    const size_t n = ((size_t)256 << 20) / (rows * (a.c.dim + 2) * sizeof(float));
+    return n < 1 ? 1 : n;
+}
+// Pieces of `chunk` tiles each.
+int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t chunk, void *stream) {
+    chunk = chunk < 1 ? 1 : chunk;
+    a.chunk = (uint32_t)chunk;
+    a.splits = (uint32_t)((tiles + chunk - 1) / chunk);
+    a.splits = a.splits < 1 ? 1 : a.splits;
+    a.join = a.splits <= 40 ? a.splits : (uint32_t)std::ceil(std::sqrt((double)a.splits));
+    if (units > kMaxGrid / a.splits) return AH_ERR_INVALID_ARG;
+    a.grid = (uint32_t)(units * a.splits);
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    const int32_t st = attn_scratch(ctx, a, (size_t)a.n_tok * a.n_heads);
+    if (st) return st;
+    AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+// Sequences of at most `most` rows, by workgroups of 8 or 16.
+int32_t attn_rows(ah_ctx *ctx, AttnArgs a, size_t max_ctx, size_t most, void *stream) {
+    a.rows = most <= 8 ? 8 : 16;
+    a.most_rows = (uint32_t)most;
+    const size_t per = (most + a.rows - 1) / a.rows, base = per * a.c.n_kv * a.n_seq, rows = (size_t)a.n_tok * a.n_heads;
+    const size_t tiles = most_tiles(a, max_ctx, most / a.group);
+    // With few units a piece's tiles (0.7 us for each of a wave) stand against the join (0.1 us a piece):
+    // sqrt(1.75 tiles) pieces, past 40 of them two joins and 16 tiles a piece.  One sequence of 4001 keys in pieces
+    // of 4, 8, 16 and 24 tiles: 10.6, 10.0, 10.7 and 13.3 us.  Once that passes a workgroup a CU (two, where two
+    // joins pay for themselves: 120000 keys in 256 workgroups 24.5 us, in 469 21.8), pieces of 32 tiles, since a
+    // workgroup costs its start and end.  With 2 KV heads of 128, in pieces of 16, 32 and 64 tiles: 128 sequences
+    // of 1000 keys 16.6, 13.4 and 13.4 us, of 4000 41.9, 35.8 and 35.6; 64 of 1 to 16384 52, 46 and 52.
+    const double wish = std::sqrt(1.75 * (double)tiles), groups = wish <= 40.0 ? 256.0 : 512.0;
+    double pieces = wish <= 40.0 ? wish : (double)tiles / 16.0;
+    if (pieces * (double)base > groups) {
+        const double most_pieces = (double)(kAttnGroups / base), by_tiles = (double)tiles / 32.0;
+        pieces = by_tiles < most_pieces ? by_tiles : most_pieces;
+        pieces = pieces * (double)base > groups ? pieces : groups / (double)base;
+    }
+    size_t chunk = pieces < 1.0 ? tiles : 4 * (size_t)((double)tiles / (4.0 * pieces) + 0.5);  // whole rounds of the four waves
+    size_t fit = base <= kAttnGroups / 2 ? kAttnGroups / base : 1;
+    fit = fit < most_pieces(a, rows) ? fit : most_pieces(a, rows);
+    chunk = chunk < (tiles + fit - 1) / fit ? (tiles + fit - 1) / fit : chunk;
+    return attn_launch(ctx, a, base, tiles, chunk, stream);
+}
+
+// Sequences of at least a.least_rows rows, by workgroups of 128.
+int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
+    a.rows = 128;
+    const size_t rows = (size_t)a.n_tok * a.n_heads, per = ((size_t)a.max_q * a.group + 127) / 128;
+    const size_t tiles = most_tiles(a, max_ctx, a.max_q);
+    // the numbers that units of 128 rows have (of uneven sequences at most one more for each)
+    const bool even = (size_t)a.n_tok == (size_t)a.n_seq * a.max_q;
+    a.per = even || a.n_seq == 1 ? (uint32_t)per : 0;
+    const size_t units = a.per ? per * a.n_seq : ((size_t)a.n_tok * a.group >> 7) + a.n_seq;
+    // Pieces by the time that they take, in us: workgroups in rounds of as many as the CUs hold (their registers and
+    // LDS: three of heads of 64, two of 128, one of 256), the matrix work of a CU's shared among them (tile: that of 128
+    // rows and 32 keys), a workgroup's start and end, and a piece's results written and read again in a launch more.
+    // One sequence, 2 KV heads, in 1100 / units pieces and in these: 512 tokens over 4096 keys, heads of 64, 128 and
+    // 256, 44 -> 41, 57 -> 50 and 85 -> 63 us.
+    const size_t tokens = a.least_rows ? a.max_q : a.n_tok;  // (with least_rows, the other sequences are single tokens)
+    size_t base = even ? per * a.n_seq * a.c.n_kv : (tokens * a.group + 127) / 128 * a.c.n_kv;
+    // uneven sequences: the longest ones' workgroups are alone in the end, as if there were fewer
+    if (!even && !a.least_rows) base = (base * 3 + 4) / 5;
+    const double tile = a.c.dim * 0.0077, alone = 1.4 * tile, start = 5.0, join = (double)rows * a.c.dim * 8.0 / 4e6;
+    const size_t held = a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1, cus = (size_t)ctx->cu_count, places = held * cus;
+    auto round = [&](size_t n, size_t per_piece) {  // n workgroups at once
+        const double t = (double)((n + cus - 1) / cus) * tile;
+        return (double)per_piece * (t > alone ? t : alone) + start;
+    };
+    // pieces of a length end together; where a causal mask or the sequences make them uneven the next ones fill in
+    const bool alike = even && max_ctx >= 2 * (size_t)a.max_q;
+    size_t splits = 1, most = (tiles + 7) / 8;
+    most = most < most_pieces(a, rows) ? most : most_pieces(a, rows);
+    double best = 0.0;
+    for (size_t n = 1; n <= most && n <= 64; ++n) {
+        const size_t all = base * n, full = all / places, rest = all % places, per_piece = (tiles + n - 1) / n;
+        double t = (double)full * round(places, per_piece) + (rest ? round(rest, per_piece) : 0.0);
+        if (!alike && full) t = (double)all / (double)places * round(places, per_piece);
+        t += n > 1 ? 3.0 + (double)n * join : 0.0;
+        if (n == 1 || t < best) {
+            best = t;
+            splits = n;
+        }
+    }
+    return attn_launch(ctx, a, units * a.c.n_kv, tiles, (tiles + splits - 1) / splits, stream);
 }
 
 } // namespace
@@ -240,67 +350,20 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     a.sinks = (uint32_t)p->sinks;
     a.scale = p->scale;
     a.status = ctx->d_status;
-    if ((uint64_t)a.max_q * a.group > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
-    const size_t most = p->table_stride << cache->ref.page_shift;
-    const size_t ctx_len = p->max_ctx < most ? p->max_ctx : most;
-    size_t tiles = (ctx_len + 31) / 32;
-    if (p->window) {
-        const size_t seen = (p->window + a.max_q + 31) / 32 + 1 + (p->sinks + 31) / 32;
-        tiles = tiles < seen ? tiles : seen;
-    }
     // The kernel: 8 packed rows or 16 rows a workgroup, or 128 over tiles in LDS.  Those pay past 32 rows and past
     // 64 units of 16 rows in all: below, a workgroup's longer start shows (one sequence of 2000 keys, 2 KV heads of
     // 128, 126 rows each: 21 us against 12; 512 rows, 64 units: 24 against 23; 8 sequences of 126 rows: 25 against 34).
     const size_t unit_rows = (size_t)a.max_q * a.group, units = (unit_rows + 15) / 16 * kv * p->n_seq;
-    a.rows = unit_rows <= 8 ? 8 : unit_rows <= 32 || units <= 64 ? 16 : 128;
-    const size_t base = ((size_t)a.max_q * a.group + a.rows - 1) / a.rows * kv * p->n_seq, rows = p->n_tok * p->n_heads;
-    size_t chunk;
-    if (a.rows == 128) {
-        // about four workgroups a CU, of at least eight tiles; none where the rows alone come near two a CU (8192
-        // tokens of 12 heads, 768 workgroups: 392 us, in two pieces each 577)
-        size_t splits = base >= 400 ? 1 : 1100 / base;
-        splits = splits < (tiles + 7) / 8 ? splits : (tiles + 7) / 8;
-        splits = splits < 1 ? 1 : splits;
-        chunk = (tiles + splits - 1) / splits;
-    } else {
-        // With few units a piece's tiles (0.7 us for each of a wave) stand against the join (0.1 us a piece):
-        // sqrt(1.75 tiles) pieces, past 40 of them two joins and 16 tiles a piece.  One sequence of 4001 keys in pieces
-        // of 4, 8, 16 and 24 tiles: 10.6, 10.0, 10.7 and 13.3 us.  Once that passes a workgroup a CU (two, where two
-        // joins pay for themselves: 120000 keys in 256 workgroups 24.5 us, in 469 21.8), pieces of 32 tiles, since a
-        // workgroup costs its start and end.  With 2 KV heads of 128, in pieces of 16, 32 and 64 tiles: 128 sequences
-        // of 1000 keys 16.6, 13.4 and 13.4 us, of 4000 41.9, 35.8 and 35.6; 64 of 1 to 16384 52, 46 and 52.
-        const double wish = std::sqrt(1.75 * (double)tiles), groups = wish <= 40.0 ? 256.0 : 512.0;
-        double pieces = wish <= 40.0 ? wish : (double)tiles / 16.0;
-        if (pieces * (double)base > groups) {
-            const double most_pieces = (double)(kAttnGroups / base), by_tiles = (double)tiles / 32.0;
-            pieces = by_tiles < most_pieces ? by_tiles : most_pieces;
-            pieces = pieces * (double)base > groups ? pieces : groups / (double)base;
-        }
-        chunk = pieces < 1.0 ? tiles : 4 * (size_t)((double)tiles / (4.0 * pieces) + 0.5);  // whole rounds of the four waves
-    }
-    const size_t room = ((size_t)256 << 20) / (rows * (dim + 2) * sizeof(float)), least = room < 1 ? tiles : (tiles + room - 1) / room;
-    const size_t most_groups = base <= kAttnGroups / 2 ? kAttnGroups / base : 1;
-    chunk = chunk < least ? least : chunk;
-    if (a.rows != 128) {
-        const size_t fit = (tiles + most_groups - 1) / most_groups;
-        chunk = chunk < fit ? fit : chunk;
-    }
-    chunk = chunk < 1 ? 1 : chunk;
-    a.chunk = (uint32_t)chunk;
-    a.splits = (uint32_t)((tiles + chunk - 1) / chunk);
-    a.splits = a.splits < 1 ? 1 : a.splits;
-    a.join = a.splits <= 40 ? a.splits : (uint32_t)std::ceil(std::sqrt((double)a.splits));
-    AH_HIP(ctx, hipSetDevice(ctx->device));
-    if (a.splits > 1) {
-        const size_t o = align256(a.splits * rows * dim * sizeof(float));
-        const int32_t st = ensure_scratch(ctx, o + a.splits * rows * 2 * sizeof(float));
+    if (unit_rows > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
+    if (unit_rows <= 32 || units <= 64) return attn_rows(ctx, a, p->max_ctx, unit_rows, stream);
+    // A few long chunks among single tokens (the others' mean is a part of 128 rows): the two kinds by a launch each.
+    const size_t few = a.group <= 8 ? 8 : 32, others = a.n_tok > a.max_q ? a.n_tok - a.max_q : 0;
+    if (a.n_seq > 1 && a.group <= few && others * a.group < (size_t)128 * (a.n_seq - 1)) {
+        const int32_t st = attn_rows(ctx, a, p->max_ctx, few, stream);
         if (st) return st;
-        a.part_o = static_cast<float *>(ctx->scratch);
-        a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch) + o);
-        a.count = ctx->d_count;
+        a.least_rows = (uint32_t)few + 1;
     }
-    AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
-    return AH_OK;
+    return attn_tiles(ctx, a, p->max_ctx, stream);
 }
 
 int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, size_t n_rows, size_t n_vocab,

@@ -81,6 +81,21 @@ AH_DEV Span span_of(const AttnArgs &a, uint32_t s) {
     return p;
 }
 
+// The last of n things, in the order of their starts, that starts at or before `at` (the first one if none does): the
+// wave's lanes look at 64 of them at a time.
+template <class F> AH_DEV uint32_t last_starting(uint32_t n, uint32_t at, F start) {
+    const uint32_t lane = threadIdx.x & 63;
+    uint32_t lo = 0;
+    while (n > 1) {
+        const uint32_t step = (n + 63) / 64, i = lane * step;
+        const uint32_t count = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < n && start(lo + (i < n ? i : 0)) <= at));
+        const uint32_t skip = (count ? count - 1 : 0) * step;
+        lo += skip;
+        n = n - skip < step ? n - skip : step;
+    }
+    return lo;
+}
+
 // The tiles that rows at positions lo .. hi see: [0, head) and [tail, end).
 struct Tiles {
     uint32_t head, tail, end, count;
@@ -186,7 +201,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
     const Span p = span_of(a, s);
     if (p.bad && split == 0 && rest == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
     const uint32_t rows = p.nq * a.group, row0 = rt * R;
-    if (row0 >= rows) return;
+    if (row0 >= rows || rows > a.most_rows) return;
     const uint32_t row = row0 + r % R, tok = row / a.group, hq = kvh * a.group + row % a.group;
     const bool live = row < rows, low = PACK && r >= 8;
     const int32_t pos0 = p.ctx - (int32_t)p.nq;
@@ -456,14 +471,22 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     extern __shared__ uint8_t tile_lds[];
     const uint32_t lane = threadIdx.x & 63, c = lane & 31, h = lane >> 5;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    // pieces slowest; then the last rows first: with a causal mask they have the most keys
-    const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units, unit = blockIdx.x - split * units;
-    const uint32_t others = a.n_seq * a.c.n_kv, per = units / others, rt = per - 1 - unit / others, rest = unit % others;
-    const uint32_t s = rest / a.c.n_kv, kvh = rest - s * a.c.n_kv;
+    // Pieces slowest; then the last rows first: with a causal mask they have the most keys.  Even sequences have `per`
+    // units of 128 rows each.  Of uneven ones, sequence s has its units from start(s) on: floor of its first row / 128,
+    // and one more for each sequence before it, so that few numbers have no rows.
+    const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units;
+    uint32_t unit = blockIdx.x - split * units;
+    if (a.per && a.n_seq > 1) {  // workgroups go to the eight XCDs in turn: neighbouring units to one, whose L2 they share
+        const uint32_t x = unit & 7, more = units & 7;
+        unit = x * (units / 8) + (x < more ? x : more) + unit / 8;
+    }
+    const uint32_t at = units / a.c.n_kv - 1 - unit / a.c.n_kv, kvh = unit % a.c.n_kv;
+    auto start = [&](uint32_t i) { return (uint32_t)((uint64_t)(uint32_t)a.q_start[i] * a.group >> 7) + i; };
+    const uint32_t s = a.per ? at / a.per : last_starting(a.n_seq, at, start), rt = at - (a.per ? s * a.per : start(s));
+    if (split == 0 && kvh == 0 && at < a.n_seq && threadIdx.x == 0 && span_of(a, at).bad) ah_record(a.status, ((unsigned long long)at << 8) + AH_ERR_CACHE_RANGE);
     const Span p = span_of(a, s);
-    if (p.bad && split == 0 && rt == 0 && kvh == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
     const uint32_t rows = p.nq * a.group, row0 = rt * 128;
-    if (row0 >= rows) return;
+    if (rt >= (rows + 127) / 128 || rows < a.least_rows) return;
     const int32_t pos0 = p.ctx - (int32_t)p.nq;
     const uint32_t last = row0 + 127 < rows ? row0 + 127 : rows - 1;
     const Tiles T = tiles_of(a, pos0 + (int32_t)(row0 / a.group), pos0 + (int32_t)(last / a.group));
@@ -758,11 +781,13 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     constexpr int E = D / 64;  // channels of a lane
-    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), s = blockIdx.y;
+    const uint32_t lane = threadIdx.x & 63, it = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t tok = it / a.n_heads, head = it - tok * a.n_heads, g = a.group;
+    if (tok >= a.n_tok) return;
+    const uint32_t s = last_starting(a.n_seq, tok, [&](uint32_t i) { return (uint32_t)a.q_start[i]; });
     const Span p = span_of(a, s);
-    const uint32_t n = p.nq * a.n_heads, it = 4 * blockIdx.x + wave;
-    if (it >= n) return;
-    const uint32_t i = it / a.n_heads, head = it % a.n_heads, g = a.group;
+    if (tok < p.q0 || tok - p.q0 >= p.nq || p.nq * g < a.least_rows) return;
+    const uint32_t i = tok - p.q0;
     const uint32_t row = i * g + head % g, row0 = row - row % a.rows;
     const uint32_t last = row0 + a.rows - 1 < p.nq * g ? row0 + a.rows - 1 : p.nq * g - 1;
     const int32_t pos0 = p.ctx - (int32_t)p.nq;
@@ -796,14 +821,14 @@ template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) *
 
 template <int D>
 hipError_t launch(const AttnArgs &a, hipStream_t stream) {
-    const uint32_t tiles = (a.max_q * a.group + a.rows - 1) / a.rows;
-    const dim3 grid(a.splits * tiles * a.c.n_kv * a.n_seq);
-    if (a.rows == 128) hipLaunchKernelGGL(attn_tile_kernel<D>, grid, dim3(256), 2 * TileLds<D>::kBytes, stream, a);
-    else if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false>), grid, dim3(256), attn_lds<D>(), stream, a);
-    else hipLaunchKernelGGL((attn_rows_kernel<D, true>), grid, dim3(256), attn_lds<D>(), stream, a);
-    hipError_t e = hipGetLastError();
-    if (e != hipSuccess || a.splits == 1 || a.rows != 128) return e;  // (the rows kernel joins by itself)
-    hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.max_q * a.n_heads + 3) / 4, a.n_seq), dim3(256), 0, stream, a);
+    const dim3 grid(a.grid), block(256);
+    if (a.rows != 128) {
+        if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false>), grid, block, attn_lds<D>(), stream, a);
+        else hipLaunchKernelGGL((attn_rows_kernel<D, true>), grid, block, attn_lds<D>(), stream, a);
+        return hipGetLastError();
+    }
+    hipLaunchKernelGGL(attn_tile_kernel<D>, grid, block, 2 * TileLds<D>::kBytes, stream, a);
+    if (a.splits > 1) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.n_tok * a.n_heads + 3) / 4), block, 0, stream, a);
     return hipGetLastError();
 }
 

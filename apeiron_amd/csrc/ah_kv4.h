@@ -122,6 +122,10 @@ struct AttnArgs {
     // go to part_o [splits][n_tok * n_heads][dim] and part_ml [splits][n_tok * n_heads][2]
     uint32_t splits, chunk;
     uint32_t rows;  // rows (token, head of a KV head's group) of a workgroup: 8, 16 or 128
+    uint32_t grid;
+    // sequences that the launch takes: for 8 and 16 rows those with at most most_rows, for 128 with at least least_rows
+    uint32_t most_rows, least_rows;
+    uint32_t per;  // units of 128 rows of every sequence; 0: they differ
     float *part_o, *part_ml;
     // attn_rows_kernel's join: pieces of a group, and the arrivals (zero between calls) of every unit's groups,
     // [unit], then of every group's pieces, [unit][group]

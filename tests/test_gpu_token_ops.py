@@ -411,6 +411,25 @@ def test_attention_of_chunks_causal_window_sinks(dev, dim, kv, G, page, window, 
     attend(dev, P, qs, ctx, kv * G, dim ** -0.5, k, v, window=window, sinks=sinks, pad=4)
 
 
+@pytest.mark.parametrize("dim,kv,G", [(64, 2, 7), (128, 1, 4), (256, 1, 3), (64, 1, 12)])
+@pytest.mark.parametrize("window,sinks", [(0, 0), (100, 2)])
+def test_attention_of_chunks_among_single_tokens(dev, dim, kv, G, window, sinks):
+    """Long chunks, short ones, single tokens and sequences without any in one call, more than a wave has lanes."""
+    rng = np.random.default_rng(dim + G)
+    qs = [1] * 70 + [0, 2, 0, 9]
+    for at, n in ((0, 260), (13, 40), (69, 300)):
+        qs[at] = n
+    ctx = [int(n + rng.integers(0, 90)) for n in qs]
+    P, k, v = filled(dev, ctx, 64, kv, dim, seed=dim)
+    attend(dev, P, qs, ctx, kv * G, dim ** -0.5, k, v, window=window, sinks=sinks)
+
+
+@pytest.mark.parametrize("dim,kv,G,n,q,c", [(64, 1, 7, 9, 100, 700), (128, 2, 4, 8, 64, 300), (256, 1, 2, 3, 128, 400), (128, 1, 3, 17, 43, 90)])
+def test_attention_of_even_chunks(dev, dim, kv, G, n, q, c):
+    P, k, v = filled(dev, [c] * n, 32, kv, dim, seed=n)
+    attend(dev, P, [q] * n, [c] * n, kv * G, dim ** -0.5, k, v)
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_attention_of_large_scores_and_long_contexts(dev, dim):
     # scores of tens of units (few keys carry the row), q far from one, and a context cut in many pieces
