@@ -340,6 +340,9 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(KvReadArgs a) {
     }
 }
 
+// Lanes of a token's workgroup: whole waves, up to four.
+uint32_t lanes_for(size_t items) { return items >= 256 ? 256 : (uint32_t)(items + 63) / 64 * 64; }
+
 } // namespace
 
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream) {
@@ -354,16 +357,17 @@ hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream) {
 }
 
 hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(rope_kernel, dim3(a.n_tok), dim3(256), 0, stream, a);
+    // (at least a head's lanes: up to 64)
+    hipLaunchKernelGGL(rope_kernel, dim3(a.n_tok), dim3(lanes_for((size_t)(a.rope.dim + 7) / 8 * a.n_heads)), 0, stream, a);
     return hipGetLastError();
 }
 
 hipError_t ah_launch_kv4_append(const AppendArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(kv4_append_kernel, dim3(a.t.n_tok), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv4_append_kernel, dim3(a.t.n_tok), dim3(lanes_for((size_t)a.c.dim / 8 * (a.n_heads + 2 * a.c.n_kv))), 0, stream, a);
     return hipGetLastError();
 }
 
 hipError_t ah_launch_kv4_read(const KvReadArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(kv4_read_kernel, dim3(a.t.n_tok), dim3(256), 0, stream, a);
+    hipLaunchKernelGGL(kv4_read_kernel, dim3(a.t.n_tok), dim3(lanes_for((size_t)a.c.dim / 8 * 2 * a.c.n_kv)), 0, stream, a);
     return hipGetLastError();
 }
