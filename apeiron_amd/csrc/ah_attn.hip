@@ -183,6 +183,11 @@ AH_DEV void q_scale(float scale, float top, float &up, float &f) {
 //   Otherwise 16 rows and a product for each half.
 // A tile's K is used first and its V last, so the next tile's K loads go out as soon as the scores are
 // formed and its V loads as soon as the output is: a wave always has half a tile on its way.
+//   What bounds it: for many keys in all the cache's bytes (64 sequences of 1 to 16384 keys, 12 heads of 128 over
+// 2: 151 MB in 48 us, 3.2 TB/s; 128 of 4000 with 8 KV heads 590 MB in 131, 4.5 TB/s), for few the chain of a launch, a
+// page's index, a tile, the partial results' way to the last workgroup and back (4001 keys: 9.8 us).  A unit
+// over all keys in one workgroup, joined by nobody, costs 0.7 us a tile and wave; a second launch for the join
+// 5 us more; equal shares of all units' tiles for every workgroup (two units in one) up to 10.
 template <int D, bool PACK>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_rows_kernel(AttnArgs a) {
     constexpr int NJ = D / 32;  // contraction steps of K q, and blocks of channels
@@ -460,6 +465,12 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
 // order of those scores, so p stays in its lane here too.
 //   LDS: K [64 tokens][D], V [D channels][64 tokens], rows 16 bytes longer than their values: 16 lanes' rows
 //   start 4 banks apart, so a 16-byte read of the wave meets no conflict.
+//   What bounds it: the matrix cores, which the two halves of q and of p use twice (8192 tokens, 12 heads of 128:
+// 206 GFLOP of keys and values, 412 with the halves, in 393 us: 1050 TFLOP/s; a large f16 library product reaches
+// 1068 on this card); half of their peak, the rest the vector work of the exponentials and the codes' conversion that the
+// products do not cover (about 7 instructions hide behind one).  For chunks of a few hundred tokens the unit's start
+// and the join (1205 tokens of 5 sequences over up to 6007 keys, heads of 64: 67 and 13 us under a tracer).  With the four waves
+// each converting its own fragments (no LDS) 8192 tokens took 670 us.
 template <int D> struct TileLds {
     static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;
 };
@@ -777,7 +788,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
 }
 
 // Joins the pieces of attn_tile_kernel's contexts: a wave per row (token, head).  A piece past the row's keys was
-// never written; which those are follows from the same tiles_of.
+// never written; which those are follows from the same tiles_of.  Bound by the partial results' bytes.
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     constexpr int E = D / 64;  // channels of a lane

@@ -21,6 +21,11 @@
 //           in the gather's launch).
 // A row whose listed tokens pass the lists' room (thousands of equal logits) is cut by selections over
 // the whole row instead.
+//   What bounds it, of 192 rows of 151936 with mixed parameters, 71 us (117 MB; 25 us by a copy's rate): scan
+// 18.5 us from the Infinity Cache and 27 from memory; count and gather 18 and 14 us, the vector work of a weight (an
+// exponential, its place among the bins, f64 sums) for each token of the groups that reach the bound, all of them
+// without top-k; draw 13 us, the chain of loads and barriers of its slowest row.  One row with k = 40: 2.9, 8.5 and
+// 1.6 us, such chains; a launch each costs the host as much.
 #include "ah_kv4.h"
 
 #include <type_traits>
@@ -241,15 +246,15 @@ struct Cut {
     uint32_t key, last;
 };
 
-// The index of the nth (1 ..) of n tokens in index order that have key `cut`.
-template <class Key, class Index, class Lds> AH_DEV uint32_t nth_equal(uint32_t n, Key key, Index index, uint32_t cut, uint32_t nth, Lds &D) {
+// The index of the nth (1 ..) of n tokens that have key `cut`.
+template <class Key, class Lds> AH_DEV uint32_t nth_equal(uint32_t n, Key key, uint32_t cut, uint32_t nth, Lds &D) {
     uint32_t seen = 0;
     for (uint32_t base = 0; base < n && seen < nth; base += kT) {
         const uint32_t i = base + threadIdx.x;
         const bool eq = i < n && key(i) == cut;
         uint32_t total;
         const uint32_t at = seen + scan_u(eq, D.S, total);
-        if (eq && at == nth) D.u0 = index(i);
+        if (eq && at == nth) D.u0 = i;
         seen += total;
     }
     __syncthreads();
@@ -264,13 +269,13 @@ AH_DEV int first_digit(uint32_t lo, uint32_t hi, uint32_t &shared) {
     return shift;
 }
 
-// The cut over n tokens in index order (a list, or the whole row), by digits of the keys.  in_k(key) and
-// in_p(key): whether such a token counts for the top-k and for the top-p limit.  need: tokens that top-k still
-// keeps of its own; W0: the weight ahead of those (without top-k: of every token); before: the weight ahead of
-// top-p's.
-template <class Key, class Index, class InK, class InP, class Lds>
-AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, InP in_p, bool do_k, uint32_t need, double W0, double before,
-                      Lds &D) {
+// The cut over the whole row, by digits of the keys.  do_k: top-k falls into the tokens that have weight; all_weight: theirs.
+template <class Lds> AH_DEV Cut select_cut(const Row &r, bool do_k, double all_weight, Lds &D) {
+    const uint32_t n = r.V;
+    const auto key = [&](uint32_t i) { return key_of(r.x[i]); };
+    const auto weighs = [&](uint32_t k) { return bin_at(z_of(r, k)) < kBins; };
+    uint32_t need = (uint32_t)r.k;
+    double before = 0.0;
     const uint32_t t = threadIdx.x;
     Cut c = {0, kNone};
     uint32_t keep = 0, cut_k = 0;  // of those at the cut
@@ -280,7 +285,7 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
 #pragma unroll 1
         for (uint32_t i = t; i < n; i += kT) {
             const uint32_t k = key(i);
-            if (in_k(k)) {
+            if (weighs(k)) {
                 lo = __builtin_elementwise_min(lo, k);
                 hi = __builtin_elementwise_max(hi, k);
             }
@@ -294,7 +299,7 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
 #pragma unroll 1
             for (uint32_t i = t; i < n; i += kT) {
                 const uint32_t k = key(i);
-                if (in_k(k) && (shift == 24 || (k >> (shift + 8)) == (cut_k >> (shift + 8)))) atomicAdd(&D.count[(k >> shift) & 255u], 1u);
+                if (weighs(k) && (shift == 24 || (k >> (shift + 8)) == (cut_k >> (shift + 8)))) atomicAdd(&D.count[(k >> shift) & 255u], 1u);
             }
             __syncthreads();
             const uint32_t mine = D.count[255 - t];
@@ -314,23 +319,23 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
     }
     if (r.need_p) {
         const double w_cut = do_k ? (double)weight_at(z_of(r, cut_k)) : 0.0;
-        double W = W0;
+        double W = do_k ? 0.0 : all_weight;
         if (do_k) {
             double s = 0.0;
 #pragma unroll 1
             for (uint32_t i = t; i < n; i += kT) {
                 const uint32_t k = key(i);
-                if (in_k(k) && k > cut_k) s += (double)weight_at(z_of(r, k));
+                if (weighs(k) && k > cut_k) s += (double)weight_at(z_of(r, k));
             }
             W += sum_d(s, D.S) + (double)keep * w_cut;
         }
         double goal = (double)(r.p > 0.0f ? r.p : 0.0f) * W;
         goal = goal < 1.0 ? 1.0 : goal;  // the first token always
-        uint32_t cut_p = 0, all = 0, lo = do_k && in_p(cut_k) ? cut_k : kNone, hi = lo == kNone ? 0u : cut_k;
+        uint32_t cut_p = 0, all = 0, lo = do_k && weighs(cut_k) ? cut_k : kNone, hi = lo == kNone ? 0u : cut_k;
 #pragma unroll 1
         for (uint32_t i = t; i < n; i += kT) {
             const uint32_t k = key(i);
-            if (in_p(k) && !(do_k && k <= cut_k)) {
+            if (weighs(k) && !(do_k && k <= cut_k)) {
                 lo = __builtin_elementwise_min(lo, k);
                 hi = __builtin_elementwise_max(hi, k);
             }
@@ -345,14 +350,14 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
 #pragma unroll 1
             for (uint32_t i = t; i < n; i += kT) {
                 const uint32_t k = key(i);
-                if (!in_p(k) || (do_k && k <= cut_k) || !(shift == 24 || (k >> (shift + 8)) == (cut_p >> (shift + 8)))) continue;
+                if (!weighs(k) || (do_k && k <= cut_k) || !(shift == 24 || (k >> (shift + 8)) == (cut_p >> (shift + 8)))) continue;
                 unsafeAtomicAdd(&D.mass[(k >> shift) & 255u], (double)weight_at(z_of(r, k)));
                 atomicAdd(&D.count[(k >> shift) & 255u], 1u);
             }
             __syncthreads();
             double mine = D.mass[255 - t];
             uint32_t cnt = D.count[255 - t];
-            if (do_k && in_p(cut_k) && (shift == 24 || (cut_k >> (shift + 8)) == (cut_p >> (shift + 8))) && 255 - t == ((cut_k >> shift) & 255u)) {
+            if (do_k && weighs(cut_k) && (shift == 24 || (cut_k >> (shift + 8)) == (cut_p >> (shift + 8))) && 255 - t == ((cut_k >> shift) & 255u)) {
                 mine += (double)keep * w_cut;
                 cnt += keep;
             }
@@ -376,7 +381,7 @@ AH_DEV Cut select_cut(const Row &r, uint32_t n, Key key, Index index, InK in_k, 
         keep = m;
         c.key = cut_p;
     }
-    if (partial) c.last = nth_equal(n, key, index, c.key, keep, D);
+    if (partial) c.last = nth_equal(n, key, c.key, keep, D);
     return c;
 }
 
@@ -947,11 +952,8 @@ template <bool SAME> AH_DEV void draw(const SampleArgs &a, uint32_t row, const L
         }
     }
     if (full) {  // too many equal, or nearly equal: over the whole row
-        const auto key = [&](uint32_t i) { return key_of(r.x[i]); };
-        const auto index = [](uint32_t i) { return i; };
-        const auto weighs = [&](uint32_t k) { return bin_at(z_of(r, k)) < kBins; };
         __syncthreads();
-        c = select_cut(r, r.V, key, index, weighs, weighs, do_k, (uint32_t)r.k, do_k ? 0.0 : o.all, 0.0, C);
+        c = select_cut(r, do_k, o.all, C);
         __syncthreads();
 #pragma unroll 1
         for (uint32_t s = t >> 6; s < a.chunks; s += kW) {
