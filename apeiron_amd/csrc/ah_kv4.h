@@ -157,10 +157,9 @@ struct SampleArgs {
     SampleLimits *limits;                          // [row]
     double *bin_mass, *chunk_mass;                 // [row][bin], [row][chunk]
     float *group_max;                              // [row][group]
-    uint32_t *bin_count, *chunk_count;             // [row][bin], [row][chunk]
-    uint16_t *list;                                // [row][chunk][kSampleChunkList] tokens listed, by place in the chunk
+    uint32_t *bin_count, *bits;                    // [row][bin]; a bit for each token listed, [row][chunk]
 };
-constexpr uint32_t kSampleChunkList = 256, kSampleList = 4096, kSampleMaxChunks = 512;
+constexpr uint32_t kSampleList = 4096, kSampleMaxChunks = 512;
 
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream);
 hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream);

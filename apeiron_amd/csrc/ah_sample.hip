@@ -16,16 +16,18 @@
 //           the row is done.  Otherwise the tokens and their weight in 1024 bins, of the groups that reach the
 //           bound; the row's workgroup that arrives last finds in them the bins that are kept, those dropped,
 //           and the few that a limit falls into;
-//   gather  each chunk's certain weight, and a list of the tokens in the few bins;
-//   draw    one workgroup a row orders the listed tokens, cuts them, draws a chunk and a token in it (of few rows,
-//           in the gather's launch).
-// A row whose listed tokens pass the lists' room (thousands of equal logits) is cut by selections over
+//   gather  each chunk's certain weight, and a bit for each token in the few bins;
+//   draw    one workgroup a row lists those tokens, orders them, cuts, draws a chunk and a token in it (of few rows, in
+//           the gather's launch).
+// A row whose listed tokens pass the list's room (thousands of equal logits) is cut by selections over
 // the whole row instead.
-//   What bounds it, of 192 rows of 151936 with mixed parameters, 71 us (117 MB; 25 us by a copy's rate): scan
-// 18.5 us from the Infinity Cache and 27 from memory; count and gather 18 and 14 us, the vector work of a weight (an
+//   What bounds it, of 192 rows of 151936 with mixed parameters, 73 us (117 MB; 25 us by a copy's rate): scan
+// 18.6 us from the Infinity Cache and 27 from memory; count and gather 18 and 15 us, the vector work of a weight (an
 // exponential, its place among the bins, f64 sums) for each token of the groups that reach the bound, all of them
-// without top-k; draw 13 us, the chain of loads and barriers of its slowest row.  One row with k = 40: 2.9, 8.5 and
-// 1.6 us, such chains; a launch each costs the host as much.
+// without top-k; draw 15 us, the chain of loads and barriers of its slowest row.  One row with k = 40: 2.7, 8.9 and
+// 2 us, such chains; a launch each costs the host as much.  Bits for the listed tokens, not lists of each chunk's: a
+// vocabulary in the order of its logits has all of a bin in a chunk or two (top-p 0.9 of one such row 41 us against
+// the 1100 of the selections over the row, of one in any order 34 against 30).
 #include "ah_kv4.h"
 
 #include <type_traits>
@@ -696,14 +698,16 @@ AH_DEV bool finish_small(const SampleArgs &a, const Row &r, uint32_t row, const 
     return true;
 }
 
-// Calls f(place of a lane's first token in the chunk, its logits) over those groups of a chunk whose largest token's
-// bin is at most `last`, in their order: eight groups a round, eight lanes each (-inf in a lane without), the next
-// round's logits on their way meanwhile.
-template <class F> AH_DEV void each_group(const SampleArgs &a, const Row &r, uint32_t row, uint32_t chunk, uint32_t last, F f) {
+// Calls f(place of a lane's first token in the chunk, its logits, whether there is one) over those groups of a chunk
+// whose largest token's bin is at most `last`, in their order: eight groups a round, eight lanes each, the next round's
+// logits on their way meanwhile.  skipped(group) for each of the chunk's others, past the row's end too.
+template <class F, class G>
+AH_DEV void each_group(const SampleArgs &a, const Row &r, uint32_t row, uint32_t chunk, uint32_t last, F f, G skipped) {
     const uint32_t lane = threadIdx.x & 63, g = chunk * kGroups + lane;
     const bool in = lane < kGroups && g < a.groups, use = in && bin_at(z_at(r, a.group_max[(size_t)row * a.groups + (in ? g : 0)])) <= last;
     const uint64_t todo = __builtin_amdgcn_ballot_w64(use);
     const uint32_t n = (uint32_t)__builtin_popcountll(todo);
+    if (lane < kGroups && !use) skipped(lane);
     if (n == 0) return;
     // lane j: the j-th of the groups
     const uint32_t rank = __builtin_amdgcn_mbcnt_lo((uint32_t)todo, 0u);
@@ -721,7 +725,7 @@ template <class F> AH_DEV void each_group(const SampleArgs &a, const Row &r, uin
         for (int i = 0; i < 8; ++i) x[i] = next[i];
         at = at_next;
         if (j + 8 < n) load(j + 8);
-        f(at, x);
+        f(at, x, j + (lane >> 3) < n);
     }
 }
 
@@ -844,16 +848,19 @@ __global__ void __launch_bounds__(kT, 8) sample_count_kernel(SampleArgs a) {
     }
     __syncthreads();
     for (uint32_t c = c0 + __builtin_amdgcn_readfirstlane(t >> 6); c < c1; c += kW)
-        each_group(a, r, row, c, last, [&](uint32_t, const float *x) {
+        each_group(
+            a, r, row, c, last,
+            [&](uint32_t, const float *x, bool) {  // (-inf in a lane without a group: no bin)
 #pragma unroll
-            for (int i = 0; i < 8; ++i) {
-                const float z = z_at(r, x[i]);
-                const uint32_t b = bin_at(z);
-                if (b > last) continue;
-                if (r.need_k) atomicAdd(&D.count[b], 1u);
-                if (r.need_p) unsafeAtomicAdd(&D.mass[b], (double)weight_at(z));
-            }
-        });
+                for (int i = 0; i < 8; ++i) {
+                    const float z = z_at(r, x[i]);
+                    const uint32_t b = bin_at(z);
+                    if (b > last) continue;
+                    if (r.need_k) atomicAdd(&D.count[b], 1u);
+                    if (r.need_p) unsafeAtomicAdd(&D.mass[b], (double)weight_at(z));
+                }
+            },
+            [](uint32_t) {});
     __syncthreads();
     uint32_t n[4];
     double m[4];
@@ -890,7 +897,6 @@ __global__ void __launch_bounds__(kT, 8) sample_count_kernel(SampleArgs a) {
 struct DrawLds {
     CutLds<kSampleList> cut;
     double mass[kSampleMaxChunks];
-    uint32_t start[kSampleMaxChunks];
 };
 
 // SAME: in the launch that gathered.
@@ -899,50 +905,37 @@ template <bool SAME, class T> AH_DEV T gathered(const T *p) { return SAME ? get(
 template <bool SAME> AH_DEV void draw(const SampleArgs &a, uint32_t row, const Limits &o, DrawLds &D) {
     CutLds<kSampleList> &C = D.cut;
     const uint32_t t = threadIdx.x;
-    // this thread's chunks: their certain weights, and how many tokens each lists
+    // this thread's chunks' certain weights, and its words of the listed tokens' bits
     const uint32_t each = (a.chunks + kT - 1) / kT, g0 = t * each < a.chunks ? t * each : a.chunks, g1 = g0 + each < a.chunks ? g0 + each : a.chunks;
-    uint32_t n_mine = 0, n;
-    bool full = false;
-    for (uint32_t s = g0; s < g1; ++s) {
-        const uint32_t c = gathered<SAME>(&a.chunk_count[(size_t)row * a.chunks + s]);
-        D.mass[s] = gathered<SAME>(&a.chunk_mass[(size_t)row * a.chunks + s]);
-        D.start[s] = c;
-        full |= c > kSampleChunkList;
-        n_mine += c;
-    }
+    for (uint32_t s = g0; s < g1; ++s) D.mass[s] = gathered<SAME>(&a.chunk_mass[(size_t)row * a.chunks + s]);
+    const uint32_t words = a.chunks * (kChunk / 32), own_words = (words + kT - 1) / kT, w0 = t * own_words, w1 = w0 + own_words < words ? w0 + own_words : words;
+    const uint32_t *bits = a.bits + (size_t)row * words;
+    constexpr uint32_t kHeld = 20;  // (a row of 163840 tokens), the rest read twice
+    uint32_t n_mine = 0, n, held[kHeld];
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) held[i] = w0 + i < w1 ? gathered<SAME>(&bits[w0 + i]) : 0u;
+#pragma unroll
+    for (uint32_t i = 0; i < kHeld; ++i) n_mine += (uint32_t)__builtin_popcount(held[i]);
+    for (uint32_t w = w0 + kHeld; w < w1; ++w) n_mine += (uint32_t)__builtin_popcount(gathered<SAME>(&bits[w]));
     Row r = row_of(a, row);
     set_top(r, o.top);
-    uint32_t at = scan_u(n_mine, C.S, n) - n_mine;  // where each chunk's listed tokens start
-    for (uint32_t s = g0; s < g1; ++s) {
-        const uint32_t c = D.start[s];
-        D.start[s] = at;
-        for (const uint32_t e = at + c; at < e; ++at)
-            if (at < kSampleList) C.idx[at] = s;  // the chunk of each
+    uint32_t at = scan_u(n_mine, C.S, n) - n_mine;
+    bool full = n > kSampleList;
+    if (!full && n_mine) {
+        const auto list = [&](uint32_t w, uint32_t b) {
+#pragma unroll 1
+            for (; b; b &= b - 1) C.idx[at++] = w * 32 + (uint32_t)__builtin_ctz(b);
+        };
+#pragma unroll
+        for (uint32_t i = 0; i < kHeld; ++i) list(w0 + i, held[i]);
+        for (uint32_t w = w0 + kHeld; w < w1; ++w) list(w, gathered<SAME>(&bits[w]));
     }
-    full = max_u(full, C.S) != 0 || n > kSampleList;
     const bool do_k = o.bk != kNone, limited = do_k || r.need_p;
     Cut c = {0, kNone};
     if (!full && n) {
-        // a load of the list and one of the logit follow each other: four tokens a thread at once
-        for (uint32_t j0 = t; j0 < n; j0 += 4 * kT) {
-            uint32_t i[4], j[4];
-            float x[4];
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) {
-                j[q] = j0 + q * kT < n ? j0 + q * kT : j0;  // (past the list: the thread's first once more)
-                i[q] = C.idx[j[q]];
-            }
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q)
-                i[q] = i[q] * kChunk + gathered<SAME>(&a.list[((size_t)row * a.chunks + i[q]) * kSampleChunkList + (j[q] - D.start[i[q]])]);
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) x[q] = r.x[i[q]];
-#pragma unroll
-            for (uint32_t q = 0; q < 4; ++q) {
-                C.idx[j[q]] = i[q];
-                C.key[j[q]] = key_of(x[q]);
-            }
-        }
+        __syncthreads();
+#pragma unroll 4
+        for (uint32_t j = t; j < n; j += kT) C.key[j] = key_of(r.x[C.idx[j]]);
         __syncthreads();
         full = !cut_list(r, o, n, do_k, false, c, C);
 #pragma unroll 1
@@ -1027,33 +1020,32 @@ template <bool DRAW> __global__ void __launch_bounds__(kT) sample_gather_kernel(
     const float also_from = (float)o.bk, also_to = (float)(o.bk + 1);
     for (uint32_t c = c0 + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6); c < c1; c += kW) {
         const size_t chunk = (size_t)row * a.chunks + c;
-        uint16_t *list = a.list + chunk * kSampleChunkList;
+        uint8_t *bits = reinterpret_cast<uint8_t *>(a.bits) + chunk * (kChunk / 8);
         double sure = 0.0;
-        uint32_t listed = 0;
-        each_group(a, r, row, c, o.last, [&](uint32_t at, const float *x) {
-            uint32_t mask = 0;
+        each_group(
+            a, r, row, c, o.last,
+            [&](uint32_t at, const float *x, bool live) {
+                uint32_t mask = 0;
 #pragma unroll
-            for (uint32_t i = 0; i < 8; ++i) {
-                const float z = z_at(r, x[i]), y = place_at(z), w = weight_at(z);
-                sure += (double)(((y < sure_to) & (w >= r.floor_f)) ? w : 0.0f);
-                mask |= ((y >= from) & (y < to)) ? 1u << i : 0u;
-                if (also) mask |= ((y >= also_from) & (y < also_to)) ? 1u << i : 0u;
-            }
-            if (__builtin_amdgcn_ballot_w64(mask != 0) == 0ull) return;
-            const uint32_t n = (uint32_t)__builtin_popcount(mask), sum = wave_prefix<Add>(n);
-            uint32_t place = listed + sum - n;
-            listed += last_lane(sum);
-            if (listed <= kSampleChunkList)
-                for (; mask; mask &= mask - 1) {
-                    const uint16_t v = (uint16_t)(at + (uint32_t)__builtin_ctz(mask));
-                    if (DRAW) put(list + place++, v);
-                    else list[place++] = v;
+                for (uint32_t i = 0; i < 8; ++i) {
+                    const float z = z_at(r, x[i]), y = place_at(z), w = weight_at(z);
+                    sure += (double)(((y < sure_to) & (w >= r.floor_f)) ? w : 0.0f);
+                    mask |= ((y >= from) & (y < to)) ? 1u << i : 0u;
+                    if (also) mask |= ((y >= also_from) & (y < also_to)) ? 1u << i : 0u;
                 }
-        });
+                if (live) {
+                    if (DRAW) put(bits + at / 8, (uint8_t)mask);
+                    else bits[at / 8] = (uint8_t)mask;
+                }
+            },
+            [&](uint32_t g) {
+                if (DRAW) put(reinterpret_cast<uint64_t *>(bits) + g, (uint64_t)0);
+                else reinterpret_cast<uint64_t *>(bits)[g] = 0;
+            });
         if (__builtin_amdgcn_ballot_w64(sure > 0.0) != 0ull) sure = last_lane(wave_prefix<Add>(sure));
         if (lane == 0) {
-            put(a.chunk_mass + chunk, sure);
-            put(a.chunk_count + chunk, listed);
+            if (DRAW) put(a.chunk_mass + chunk, sure);
+            else a.chunk_mass[chunk] = sure;
         }
     }
     if constexpr (DRAW) {
@@ -1104,7 +1096,6 @@ size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
     a.chunk_mass = reinterpret_cast<double *>(take(8 * rows * a.chunks));
     a.bin_count = reinterpret_cast<uint32_t *>(take(4 * rows * kBins));
     a.group_max = reinterpret_cast<float *>(take(4 * rows * a.groups));
-    a.chunk_count = reinterpret_cast<uint32_t *>(take(4 * rows * a.chunks));
-    a.list = reinterpret_cast<uint16_t *>(take(2 * rows * a.chunks * kSampleChunkList));
+    a.bits = reinterpret_cast<uint32_t *>(take(rows * a.chunks * (kChunk / 8)));
     return at;
 }
