@@ -447,9 +447,12 @@ int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *t
  * h / (n_heads / n_kv_heads).  out = sum_t softmax(scale q . k_t) v_t, zeros for a query that sees
  * nothing (more tokens than positions).  Tokens of no sequence are not written.
  * max_q: at least the largest number of a sequence's tokens; max_ctx: the largest context expected (it
- * plans how the contexts are cut; longer ones are still served whole).  A sequence whose tokens, context
- * or pages are out of range is refused with AH_ERR_CACHE_RANGE: its tokens are not written, or (a page)
- * the page's positions not seen.  Uses the context's scratch (as ah_gemm_f32_dev). */
+ * plans how the contexts are cut; longer ones are still served whole).  Single tokens and chunks may be
+ * mixed in a call.  A sequence whose tokens, context or pages are out of range is refused with
+ * AH_ERR_CACHE_RANGE: its tokens are not written, or (a page) the page's positions not seen.  At most 65535
+ * sequences, 2^23 rows (tokens times heads a KV head) of a sequence, and 2^24 workgroups' worth of both.
+ * Uses the context's scratch (as ah_gemm_f32_dev): a call that is captured into a graph is made once before
+ * at the same sizes, so that the scratch has grown. */
 typedef struct ah_kv4_attn {
     size_t n_seq, n_tok, n_heads, max_q, max_ctx;
     const int32_t *d_q_start; /* [n_seq + 1] */
@@ -463,7 +466,7 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *arg
                         float *d_out, size_t out_stride, void *stream);
 
 /* One token per row of logits [n_rows][n_vocab] (rows row_stride floats apart; n_vocab <= 2^20, n_rows <=
- * 65536).  Uses the context's scratch (as ah_gemm_f32_dev).  In the
+ * 65536).  Uses the context's scratch (as ah_gemm_f32_dev; before a capture, as ah_kv4_attn_dev).  In the
  * order (logit descending, index ascending), with weights w = rint(2^32 exp((logit - largest) / T)): the
  * first top_k tokens are kept (top_k <= 0 or >= n_vocab: all), of those the ones whose preceding weight is
  * below top_p times the weight of all (top_p >= 1: all), of those the ones with w >= min_p 2^32; the first
