@@ -151,8 +151,9 @@ struct SampleArgs {
     unsigned long long *status;
     uint32_t *arrived;  // [n_counts], zero between calls
     uint32_t n_counts;
-    // planned by ah_sample_plan: groups and chunks of a row, chunks of a workgroup and workgroups of a row, and the scratch
-    uint32_t groups, chunks, per, parts;
+    // planned by ah_sample_plan: groups and chunks of a row, chunks of a workgroup and workgroups of a row (in the scan,
+    // and after it), and the scratch
+    uint32_t groups, chunks, scan_per, scan_parts, per, parts;
     bool draw;  // in the gather's launch
     SampleLimits *limits;                          // [row]
     double *bin_mass, *chunk_mass;                 // [row][bin], [row][chunk]

@@ -203,11 +203,11 @@ AH_DEV void load_keys(const Row &r, uint32_t i0, uint32_t *k) {
 template <class T> AH_DEV void put(T *p, T v) { __hip_atomic_store(p, v, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 template <class T> AH_DEV T get(const T *p) { return __hip_atomic_load(const_cast<T *>(p), __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT); }
 
-// The workgroup's row and its chunks.
-AH_DEV void share(const SampleArgs &a, uint32_t &row, uint32_t &c0, uint32_t &c1) {
-    row = blockIdx.x / a.parts;
-    c0 = (blockIdx.x - row * a.parts) * a.per;
-    c1 = c0 + a.per < a.chunks ? c0 + a.per : a.chunks;
+// The workgroup's row and its chunks, with `parts` workgroups a row of `per` chunks each.
+AH_DEV void share(const SampleArgs &a, uint32_t parts, uint32_t per, uint32_t &row, uint32_t &c0, uint32_t &c1) {
+    row = blockIdx.x / parts;
+    c0 = (blockIdx.x - row * parts) * per;
+    c1 = c0 + per < a.chunks ? c0 + per : a.chunks;
 }
 // Whether this workgroup is the row's last in the launch: it then finds what the others have put.  The counters
 // are left at zero.
@@ -508,7 +508,7 @@ AH_DEV double goal_of(const Row &r, double W) {
 
 __global__ void __launch_bounds__(kT) sample_scan_kernel(SampleArgs a) {
     uint32_t row, c0, c1;
-    share(a, row, c0, c1);
+    share(a, a.scan_parts, a.scan_per, row, c0, c1);
     Row r;
     r.x = a.logits + (size_t)row * a.stride;
     r.V = a.n_vocab;
@@ -793,7 +793,7 @@ AH_DEV Limits limits_of(const Row &r, const uint32_t *c, const double *m, Scan &
 __global__ void __launch_bounds__(kT, 8) sample_count_kernel(SampleArgs a) {
     __shared__ CountLds D;
     uint32_t row, c0, c1;
-    share(a, row, c0, c1);
+    share(a, a.parts, a.per, row, c0, c1);
     const GroupMaxima G(a, row);  // (on their way before anything is waited for)
     Row r = row_of(a, row);
     const uint32_t t = threadIdx.x;
@@ -1007,7 +1007,7 @@ __global__ void __launch_bounds__(kT) sample_draw_kernel(SampleArgs a) {
 template <bool DRAW> __global__ void __launch_bounds__(kT) sample_gather_kernel(SampleArgs a) {
     __shared__ typename std::conditional<DRAW, DrawLds, char>::type D;
     uint32_t row, c0, c1;
-    share(a, row, c0, c1);
+    share(a, a.parts, a.per, row, c0, c1);
     const Limits o = a.limits[row];
     if (o.done) return;
     Row r = row_of(a, row);
@@ -1062,7 +1062,7 @@ static_assert(kSampleMaxChunks * kChunk >= 1u << 20, "the longest row");
 
 hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream) {
     const dim3 grid(a.n_rows * a.parts), block(kT);
-    hipLaunchKernelGGL(sample_scan_kernel, grid, block, 0, stream, a);
+    hipLaunchKernelGGL(sample_scan_kernel, dim3(a.n_rows * a.scan_parts), block, 0, stream, a);
     hipLaunchKernelGGL(sample_count_kernel, grid, block, 0, stream, a);
     if (a.draw) {
         hipLaunchKernelGGL(sample_gather_kernel<true>, grid, block, 0, stream, a);
@@ -1077,13 +1077,22 @@ hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream) {
 size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base) {
     a.groups = (a.n_vocab + kGroup - 1) / kGroup;
     a.chunks = (a.n_vocab + kChunk - 1) / kChunk;
-    // at most eight workgroups a CU (all that a CU holds: one more would start when the first ends); several of a
-    // row where there is a counter for their arrivals
-    const uint32_t want = a.n_rows <= a.n_counts ? 8 * cus / a.n_rows : 1, parts = want < 1 ? 1 : want;
-    a.per = (a.chunks + parts - 1) / parts;
-    a.parts = (a.chunks + a.per - 1) / a.per;
-    // A launch less where the draw's LDS leaves every workgroup its place (three a CU)
-    a.draw = a.n_rows * a.parts <= 3 * cus;
+    // At most eight workgroups a CU, all that a CU holds (one more would start when the first ends).  After the scan a
+    // workgroup takes a chunk for each of its waves: with one it brought its bins to the row's four times as often (24
+    // rows, top-p: count 31 us against 15).
+    auto cut = [&](uint32_t least, uint32_t &parts, uint32_t &per) {
+        const uint32_t want = 8 * cus / a.n_rows, most = want < 1 ? 1 : want;
+        per = ((a.chunks + most - 1) / most + least - 1) / least * least;
+        parts = (a.chunks + per - 1) / per;
+    };
+    cut(1, a.scan_parts, a.scan_per);
+    cut(kW, a.parts, a.per);
+    if (a.n_rows > a.n_counts) {  // no counter for the arrivals
+        a.parts = 1;
+        a.per = a.chunks;
+    }
+    // A launch less for few rows, whose launches are the host's time (24 rows: gather and draw 22 us in one, 18 in two)
+    a.draw = a.n_rows * a.parts <= cus;
     const size_t rows = a.n_rows;
     size_t at = 0;
     auto take = [&](size_t bytes) {
