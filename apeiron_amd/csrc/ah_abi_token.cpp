@@ -54,7 +54,8 @@ int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t
     a.chunk = (uint32_t)chunk;
     a.splits = (uint32_t)((tiles + chunk - 1) / chunk);
     a.splits = a.splits < 1 ? 1 : a.splits;
-    a.join = a.splits <= 40 ? a.splits : (uint32_t)std::ceil(std::sqrt((double)a.splits));
+    if (a.rows != 128) a.join = a.splits <= 40 ? a.splits : (uint32_t)std::ceil(std::sqrt((double)a.splits));
+    else a.join = a.splits <= 3 && a.c.dim == 64 && units <= kCounts;
     if (units > kMaxGrid / a.splits) return AH_ERR_INVALID_ARG;
     a.grid = (uint32_t)(units * a.splits);
     AH_HIP(ctx, hipSetDevice(ctx->device));

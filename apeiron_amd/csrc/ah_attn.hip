@@ -769,10 +769,63 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
         }
     }
     l += xor_lanes(l, 32);
+    const uint32_t pieces = D == 64 && a.join && T.count ? (T.count + chunk - 1) / chunk : 1;
+    if (D == 64 && pieces > 1) {
+        // Few pieces are joined by the unit's workgroup that arrives last (as in attn_rows_kernel), each lane its own place
+        // of all of them, in their order whichever is last: a launch less, but a memory round trip for each piece.
+        // 2048 tokens in 2 pieces 57 -> 46 us, 512 over 4096 keys in 6 41 -> 46.  Larger heads have no registers for it:
+        // of 128, 3 to 5 us slower in every call, of 256 in 2 pieces 84 -> 89.
+        const size_t flat = (size_t)(p.q0 + tok) * a.n_heads + hq, all = (size_t)a.n_tok * a.n_heads;
+        const __amdgpu_buffer_rsrc_t po = ah_rsrc(a.part_o, (uint32_t)(a.splits * all * D * 4)), pm = ah_rsrc(a.part_ml, (uint32_t)(a.splits * all * 8));
+        if (live) {
+            const size_t at = split * all + flat;
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4 o = {acc[n][4 * b], acc[n][4 * b + 1], acc[n][4 * b + 2], acc[n][4 * b + 3]};
+                    __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, o), po, (int)(4 * (at * D + 32 * n + 8 * b + 4 * h)), 0, kDevice);
+                }
+            if (h == 0) __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2){m, l}), pm, (int)(8 * at), 0, kDevice);
+        }
+        __asm__ volatile("s_waitcnt vmcnt(0)" ::: "memory");
+        __syncthreads();
+        uint32_t *turn = reinterpret_cast<uint32_t *>(tile_lds);
+        if (threadIdx.x == 0) {
+            uint32_t *counter = a.count + (blockIdx.x - split * units);
+            const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            if (n == pieces - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
+            *turn = n;
+        }
+        __syncthreads();
+        if (*turn != pieces - 1 || !live) return;
+        m = kNoMax;
+        for (uint32_t k = 0; k < pieces; ++k)
+            m = __builtin_fmaxf(m, __builtin_bit_cast(float, __builtin_amdgcn_raw_buffer_load_b32(pm, (int)(8 * (k * all + flat)), 0, kDevice)));
+        l = 0.0f;
+#pragma unroll
+        for (int n = 0; n < NN; ++n) acc[n] = (f32x16)0.0f;
+#pragma unroll 1
+        for (uint32_t k = 0; k < pieces; ++k) {
+            const size_t at = k * all + flat;
+            const f32x2 ml = __builtin_bit_cast(f32x2, __builtin_amdgcn_raw_buffer_load_b64(pm, (int)(8 * at), 0, kDevice));
+            const float w = __builtin_amdgcn_exp2f(ml[0] - m);
+            l += ml[1] * w;
+#pragma unroll
+            for (int n = 0; n < NN; ++n)
+#pragma unroll
+                for (int b = 0; b < 4; ++b) {
+                    const f32x4 o = __builtin_bit_cast(f32x4, __builtin_amdgcn_raw_buffer_load_b128(po, (int)(4 * (at * D + 32 * n + 8 * b + 4 * h)), 0, kDevice));
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) acc[n][4 * b + i] += o[i] * w;
+                }
+        }
+    }
     if (!live) return;
     const size_t flat = (size_t)(p.q0 + tok) * a.n_heads + hq, all = (size_t)a.n_tok * a.n_heads;
-    const float inv = a.splits > 1 ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
-    float *dst = a.splits > 1 ? a.part_o + (split * all + flat) * D : a.out + (size_t)(p.q0 + tok) * a.out_stride + (size_t)hq * D;
+    const bool part = a.splits > 1 && !(D == 64 && a.join);
+    const float inv = part ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
+    float *dst = part ? a.part_o + (split * all + flat) * D : a.out + (size_t)(p.q0 + tok) * a.out_stride + (size_t)hq * D;
 #pragma unroll
     for (int n = 0; n < NN; ++n)
 #pragma unroll
@@ -780,7 +833,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
             const f32x4 o = (f32x4){acc[n][4 * b], acc[n][4 * b + 1], acc[n][4 * b + 2], acc[n][4 * b + 3]} * inv;
             __builtin_memcpy(dst + 32 * n + 8 * b + 4 * h, &o, 16);
         }
-    if (a.splits > 1 && h == 0) {
+    if (part && h == 0) {
         float *ml = a.part_ml + 2 * (split * all + flat);
         ml[0] = m;
         ml[1] = l;
@@ -839,7 +892,7 @@ hipError_t launch(const AttnArgs &a, hipStream_t stream) {
         return hipGetLastError();
     }
     hipLaunchKernelGGL(attn_tile_kernel<D>, grid, block, 2 * TileLds<D>::kBytes, stream, a);
-    if (a.splits > 1) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.n_tok * a.n_heads + 3) / 4), block, 0, stream, a);
+    if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.n_tok * a.n_heads + 3) / 4), block, 0, stream, a);
     return hipGetLastError();
 }
 

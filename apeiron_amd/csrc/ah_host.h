@@ -5,7 +5,8 @@
 
 #include "apeiron_hip.h"
 
-constexpr size_t kCounts = 3072;
+// Counters by which workgroups of a launch find the last of them: a unit's of a split attention, a row's of sampling.
+constexpr size_t kCounts = 65536;
 
 struct ah_ctx {
     int device = -1;
@@ -15,7 +16,7 @@ struct ah_ctx {
     // projection, reported only when [0] holds none (the reference refuses the FFN at its first
     // failing step, so a refused hidden activation is never projected).
     unsigned long long *d_status = nullptr;
-    uint32_t *d_count = nullptr;  // kCounts arrival counters of split attention, zero between calls
+    uint32_t *d_count = nullptr;  // [kCounts], zero between calls
     int last_hip = 0;
     uint32_t last_bad_bits = 0;  // f16 bits behind the last AH_ERR_NONFINITE_SCALE
     int cu_count = 256;

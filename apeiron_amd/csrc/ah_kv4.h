@@ -127,8 +127,9 @@ struct AttnArgs {
     uint32_t most_rows, least_rows;
     uint32_t per;  // units of 128 rows of every sequence; 0: they differ
     float *part_o, *part_ml;
-    // attn_rows_kernel's join: pieces of a group, and the arrivals (zero between calls) of every unit's groups,
-    // [unit], then of every group's pieces, [unit][group]
+    // The join in the launch: of attn_rows_kernel, pieces of a group, and the arrivals (zero between calls) of every
+    // unit's groups, [unit], then of every group's pieces, [unit][group]; of attn_tile_kernel, whether it is there, and
+    // the arrivals of every unit's pieces
     uint32_t join;
     uint32_t *count;
     unsigned long long *status;
