@@ -469,7 +469,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
 // 206 GFLOP of keys and values, 412 with the halves, in 393 us: 1050 TFLOP/s; a large f16 library product reaches
 // 1068 on this card); half of their peak, the rest the vector work of the exponentials and the codes' conversion that the
 // products do not cover (about 7 instructions hide behind one).  For chunks of a few hundred tokens the unit's start
-// and the join (1205 tokens of 5 sequences over up to 6007 keys, heads of 64: 67 and 13 us under a tracer).  With the four waves
+// and the join (1205 tokens of 5 sequences over up to 6007 keys, heads of 64: 67 and 8 us under a tracer).  With the four waves
 // each converting its own fragments (no LDS) 8192 tokens took 670 us.
 template <int D> struct TileLds {
     static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;
@@ -840,45 +840,41 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     }
 }
 
-// Joins the pieces of attn_tile_kernel's contexts: a wave per row (token, head).  A piece past the row's keys was
-// never written; which those are follows from the same tiles_of.  Bound by the partial results' bytes.
+// Joins the pieces of attn_tile_kernel's contexts: a wave takes 256 / D heads of a token, four channels a lane.  A piece
+// past a row's keys was never written; which those are follows from the same tiles_of.  Bound by the partial results'
+// bytes.
 template <int D>
 __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
-    constexpr int E = D / 64;  // channels of a lane
+    constexpr uint32_t kLanes = D / 4, kHeads = 64 / kLanes;
     const uint32_t lane = threadIdx.x & 63, it = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t tok = it / a.n_heads, head = it - tok * a.n_heads, g = a.group;
+    const uint32_t per = (a.n_heads + kHeads - 1) / kHeads, tok = it / per, head = (it - tok * per) * kHeads + lane / kLanes, g = a.group;
     if (tok >= a.n_tok) return;
     const uint32_t s = last_starting(a.n_seq, tok, [&](uint32_t i) { return (uint32_t)a.q_start[i]; });
     const Span p = span_of(a, s);
-    if (tok < p.q0 || tok - p.q0 >= p.nq || p.nq * g < a.least_rows) return;
+    if (tok < p.q0 || tok - p.q0 >= p.nq || p.nq * g < a.least_rows || head >= a.n_heads) return;
     const uint32_t i = tok - p.q0;
     const uint32_t row = i * g + head % g, row0 = row - row % a.rows;
     const uint32_t last = row0 + a.rows - 1 < p.nq * g ? row0 + a.rows - 1 : p.nq * g - 1;
     const int32_t pos0 = p.ctx - (int32_t)p.nq;
     const Tiles T = tiles_of(a, pos0 + (int32_t)(row0 / g), pos0 + (int32_t)(last / g));
-    const uint32_t chunk = piece_of(a, T), pieces = T.count ? (T.count + chunk - 1) / chunk : 1;
-    const size_t all = (size_t)a.n_tok * a.n_heads, flat = (size_t)(p.q0 + i) * a.n_heads + head;
-    float M = kNoMax;
-    for (uint32_t k = lane; k < pieces; k += 64) M = __builtin_fmaxf(M, a.part_ml[2 * (k * all + flat)]);
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) M = __builtin_fmaxf(M, xor_lanes(M, o));
-    float L = 0.0f, acc[E];
-#pragma unroll
-    for (int c = 0; c < E; ++c) acc[c] = 0.0f;
+    const uint32_t chunk = piece_of(a, T), pieces = T.count ? (T.count + chunk - 1) / chunk : 1, c = 4 * (lane % kLanes);
+    const size_t all = (size_t)a.n_tok * a.n_heads, flat = (size_t)tok * a.n_heads + head;
+    float M = kNoMax, L = 0.0f;
+#pragma unroll 4
+    for (uint32_t k = 0; k < pieces; ++k) M = __builtin_fmaxf(M, a.part_ml[2 * (k * all + flat)]);
+    f32x4 sum = (f32x4)0.0f;
 #pragma unroll 4
     for (uint32_t k = 0; k < pieces; ++k) {
-        float ml[2], o[E];
-        __builtin_memcpy(ml, a.part_ml + 2 * (k * all + flat), 8);
-        __builtin_memcpy(o, a.part_o + (k * all + flat) * D + E * lane, 4 * E);
+        f32x2 ml;
+        f32x4 o;
+        __builtin_memcpy(&ml, a.part_ml + 2 * (k * all + flat), 8);
+        __builtin_memcpy(&o, a.part_o + (k * all + flat) * D + c, 16);
         const float w = __builtin_amdgcn_exp2f(ml[0] - M);
         L += ml[1] * w;
-#pragma unroll
-        for (int c = 0; c < E; ++c) acc[c] += o[c] * w;
+        sum += o * w;
     }
-    const float inv = L > 0.0f || L != L ? 1.0f / L : 0.0f;
-#pragma unroll
-    for (int c = 0; c < E; ++c) acc[c] *= inv;
-    __builtin_memcpy(a.out + (size_t)(p.q0 + i) * a.out_stride + (size_t)head * D + E * lane, acc, 4 * E);
+    sum *= L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    __builtin_memcpy(a.out + (size_t)tok * a.out_stride + (size_t)head * D + c, &sum, 16);
 }
 
 template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) * sizeof(float); }
@@ -892,7 +888,8 @@ hipError_t launch(const AttnArgs &a, hipStream_t stream) {
         return hipGetLastError();
     }
     hipLaunchKernelGGL(attn_tile_kernel<D>, grid, block, 2 * TileLds<D>::kBytes, stream, a);
-    if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.n_tok * a.n_heads + 3) / 4), block, 0, stream, a);
+    const uint32_t per = (a.n_heads + 256 / D - 1) / (256 / D);
+    if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.n_tok * per + 3) / 4), block, 0, stream, a);
     return hipGetLastError();
 }
 

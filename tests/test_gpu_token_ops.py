@@ -430,6 +430,59 @@ def test_attention_of_even_chunks(dev, dim, kv, G, n, q, c):
     attend(dev, P, [q] * n, [c] * n, kv * G, dim ** -0.5, k, v)
 
 
+@pytest.mark.parametrize("dim,kv,G,n,q,c,pad", [(64, 2, 7, 1, 300, 700, 1), (64, 2, 2, 3, 1, 900, 3), (128, 1, 6, 2, 90, 500, 2), (256, 1, 3, 2, 5, 300, 1),
+                                                (64, 1, 7, 1, 2048, 2048, 1)])
+def test_attention_of_rows_off_the_16_byte_grid(dev, dim, kv, G, n, q, c, pad):
+    P, k, v = filled(dev, [c] * n, 64, kv, dim, seed=pad)
+    attend(dev, P, [q] * n, [c] * n, kv * G, dim ** -0.5, k, v, pad=pad)
+
+
+@pytest.mark.parametrize("dim,G,qs,ctx", [(64, 7, [1, 1], [900, 70]), (64, 7, [600], [700]), (64, 7, [300, 120], [2000, 900]), (128, 6, [200, 1, 90], [3000, 800, 90]),
+                                          (256, 4, [64], [1500])])
+def test_operators_replayed_as_a_graph(dev, dim, G, qs, ctx):
+    """Norm, append, attention (pieces joined in the launch and by another) and sampling captured in a row: every
+    replay, with eager work of the same context and synchronizations between, leaves what the eager calls leave."""
+    kv, n_tok, n, V = 2, sum(qs), len(qs), 7001
+    heads, rng = kv * G, np.random.default_rng(dim + n_tok)
+    P, _, _ = filled(dev, ctx, 64, kv, dim, seed=3)
+    rope = chart.Rope(dev, dim)
+    f32 = lambda *s: cuda(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+    x, gain, q, k, v, logits = f32(n_tok, 640), f32(640), f32(n_tok, heads * dim), f32(n_tok, kv * dim), f32(n_tok, kv * dim), f32(40, V)
+    seq = cuda(np.repeat(np.arange(n), qs).astype(np.int32))
+    pos = cuda(np.concatenate([c - m + np.arange(m) for m, c in zip(qs, ctx)]).astype(np.int32))
+    start, cx = cuda(np.concatenate([[0], np.cumsum(qs)]).astype(np.int32)), cuda(np.asarray(ctx, np.int32))
+    u, p, top = cuda(rng.random(40).astype(np.float32)), cuda(rng.choice([1.0, 0.9], 40).astype(np.float32)), cuda(rng.choice([0, 1, 30, 300], 40).astype(np.int32))
+    out = [torch.zeros(n_tok, 640, dtype=torch.int8, device="cuda"), torch.zeros(n_tok, 20, dtype=torch.int64, device="cuda"), torch.zeros_like(q),
+           torch.zeros_like(q), torch.zeros(40, dtype=torch.int32, device="cuda"), torch.zeros(40, device="cuda")]
+
+    def run():
+        st = stream()
+        chart.norm_quant_dev(dev, ptr(x), ptr(gain), 1e-6, n_tok, 640, codes_ptr=ptr(out[0]), scales_ptr=ptr(out[1]), stream=st)
+        P.cache.append_dev(rope, q_ptr=ptr(q), n_heads=heads, q_out_ptr=ptr(out[2]), k_ptr=ptr(k), v_ptr=ptr(v), seq_ptr=ptr(seq), pos_ptr=ptr(pos), n_tok=n_tok,
+                           table_ptr=ptr(P.table), n_seq=n, table_stride=P.per, stream=st)
+        P.cache.attn_dev(ptr(out[2]), ptr(out[3]), n_heads=heads, n_tok=n_tok, n_seq=n, q_start_ptr=ptr(start), ctx_ptr=ptr(cx), table_ptr=ptr(P.table),
+                         table_stride=P.per, max_q=max(qs), max_ctx=max(ctx), scale=dim ** -0.5, stream=st)
+        chart.sample_dev(dev, ptr(logits), 40, V, ptr(u), ptr(out[4]), probs_ptr=ptr(out[5]), top_k_ptr=ptr(top), top_p_ptr=ptr(p), stream=st)
+
+    run()
+    torch.cuda.synchronize()
+    want = [t.clone() for t in out]
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph, stream=torch.cuda.Stream()):
+        run()
+    for i in range(5):
+        for t in out:
+            t.zero_()
+        graph.replay()
+        if i % 2:
+            torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want)), i
+        torch.cuda.synchronize()
+        chart.sample_dev(dev, ptr(logits), 40, V, ptr(u), ptr(out[4]), stream=stream())  # (the same scratch and counters)
+        (f32(64, 64) @ f32(64, 64)).sum().item()
+    assert dev.sync_status(stream()) == OK
+
+
 @pytest.mark.parametrize("dim", [64, 128, 256])
 def test_attention_of_large_scores_and_long_contexts(dev, dim):
     # scores of tens of units (few keys carry the row), q far from one, and a context cut in many pieces
