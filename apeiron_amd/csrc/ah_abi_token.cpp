@@ -105,7 +105,8 @@ int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
     // rows and 32 keys), a workgroup's start and end, and a piece's results written and read again in a launch more.
     // One sequence, 2 KV heads, in 1100 / units pieces and in these: 512 tokens over 4096 keys, heads of 64, 128 and
     // 256, 44 -> 41, 57 -> 50 and 85 -> 63 us.
-    const size_t tokens = a.least_rows ? a.max_q : a.n_tok;  // (with least_rows, the other sequences are single tokens)
+    // (with least_rows, most of the other sequences are single tokens)
+    const size_t chunks = a.n_tok - (a.n_seq - 1), tokens = !a.least_rows ? a.n_tok : a.n_tok > a.n_seq && chunks > a.max_q ? chunks : a.max_q;
     size_t base = even ? per * a.n_seq * a.c.n_kv : (tokens * a.group + 127) / 128 * a.c.n_kv;
     // uneven sequences: the longest ones' workgroups are alone in the end, as if there were fewer
     if (!even && !a.least_rows) base = (base * 3 + 4) / 5;
