@@ -8,8 +8,7 @@
 // at which the kept weight up to and with it, in index order, passes floor(u W).
 //
 // No sort.  Four launches over chunks of 2048 tokens, each reading what it needs of the row once:
-//   scan    the largest key of every group of 64 tokens (a key is the f32 bits as an unsigned number of the
-//           same order);
+//   scan    the largest logit of every group of 64 tokens;
 //   count   M, and with top-k the bound, a bin of (M - l) / T that the k-th largest group maximum is in: every
 //           maximum is a token of its own, so no token past it is among the first k, and only about k groups
 //           reach it.  With a small k (and for a greedy row) one workgroup lists their tokens, cuts and draws, and
@@ -45,6 +44,7 @@ constexpr uint32_t kNone = 0xffffffffu;
 // (as many, and a few in the bound's own bin) and their tokens fit.
 constexpr uint32_t kSmallK = 56, kSmallGroups = 64, kSmallList = 1024;
 
+// A logit as an unsigned number of the same order.
 AH_DEV uint32_t key_of(float l) {
     l = l != l ? -__builtin_inff() : l + 0.0f;  // NaN is never drawn; -0 and 0 are equal
     const uint32_t b = __builtin_bit_cast(uint32_t, l);
