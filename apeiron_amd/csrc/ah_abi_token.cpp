@@ -104,7 +104,7 @@ int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
     // LDS: three of heads of 64, two of 128, one of 256), the matrix work of a CU's shared among them (tile: that of 128
     // rows and 32 keys), a workgroup's start and end, and a piece's results written and read again in a launch more.
     // One sequence, 2 KV heads, in 1100 / units pieces and in these: 512 tokens over 4096 keys, heads of 64, 128 and
-    // 256, 44 -> 41, 57 -> 50 and 85 -> 63 us.
+    // 256, 44 -> 41, 57 -> 50 and 85 -> 63 us; 2048 tokens of a prompt 54 -> 44, 69 -> 56 and 112 -> 71.
     // (with least_rows, most of the other sequences are single tokens)
     const size_t chunks = a.n_tok - (a.n_seq - 1), tokens = !a.least_rows ? a.n_tok : a.n_tok > a.n_seq && chunks > a.max_q ? chunks : a.max_q;
     size_t base = even ? per * a.n_seq * a.c.n_kv : (tokens * a.group + 127) / 128 * a.c.n_kv;
@@ -116,16 +116,28 @@ int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
         const double t = (double)((n + cus - 1) / cus) * tile;
         return (double)per_piece * (t > alone ? t : alone) + start;
     };
-    // pieces of a length end together; where a causal mask or the sequences make them uneven the next ones fill in
-    const bool alike = even && max_ctx >= 2 * (size_t)a.max_q;
+    // Pieces of a length end together.  Under a causal mask (whole prompts) half of the workgroups and half of the keys
+    // are there, longest first, and the shorter ones share the CUs or fill in, with a part of a piece at the end; uneven
+    // sequences fill in too.
+    const bool causal = even && max_ctx < 2 * (size_t)a.max_q;
     size_t splits = 1, most = (tiles + 7) / 8;
     most = most < most_pieces(a, rows) ? most : most_pieces(a, rows);
     double best = 0.0;
     for (size_t n = 1; n <= most && n <= 64; ++n) {
-        const size_t all = base * n, full = all / places, rest = all % places, per_piece = (tiles + n - 1) / n;
-        double t = (double)full * round(places, per_piece) + (rest ? round(rest, per_piece) : 0.0);
-        if (!alike && full) t = (double)all / (double)places * round(places, per_piece);
-        t += n > 1 ? 3.0 + (double)n * join : 0.0;
+        const size_t all = causal ? base * (n + 1) / 2 : base * n, full = all / places, rest = all % places, per_piece = (tiles + n - 1) / n;
+        double t;
+        if (causal && all > places) {
+            t = ((double)base * (double)tiles * 0.5 / (double)places + (n > 1 ? 0.3 : 0.0) * (double)per_piece) * (held * tile > alone ? held * tile : alone) +
+                start * (double)all / (double)places;
+        } else if (causal) {
+            const double shared = (double)((all + cus - 1) / cus), t0 = (shared - (shared - 1.0) * 0.5 / (double)n) * tile;
+            t = (double)per_piece * (t0 > alone ? t0 : alone) + start;
+        } else if (!even && full) {
+            t = (double)all / (double)places * round(places, per_piece);
+        } else {
+            t = (double)full * round(places, per_piece) + (rest ? round(rest, per_piece) : 0.0);
+        }
+        if (n > 1) t += 3.0 + (double)n * (a.c.dim == 64 && n <= 3 ? 0.5 : 1.0) * join;
         if (n == 1 || t < best) {
             best = t;
             splits = n;
