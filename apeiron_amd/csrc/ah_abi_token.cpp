@@ -364,12 +364,15 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     a.sinks = (uint32_t)p->sinks;
     a.scale = p->scale;
     a.status = ctx->d_status;
-    // The kernel: 8 packed rows or 16 rows a workgroup, or 128 over tiles in LDS.  Those pay past 32 rows and past
-    // 64 units of 16 rows in all: below, a workgroup's longer start shows (one sequence of 2000 keys, 2 KV heads of
-    // 128, 126 rows each: 21 us against 12; 512 rows, 64 units: 24 against 23; 8 sequences of 126 rows: 25 against 34).
+    // The kernel: 8 packed rows or 16 rows a workgroup, or 128 over tiles in LDS.  Those start later and need many rows
+    // of a sequence (they convert the cache's codes once for all of them, the others once for 16).  2 KV heads, rows a
+    // sequence and sequences: 56 and 64 of 1000 keys, heads of 64, 128 and 256, 15, 22 and 37 us by 16 rows against 24,
+    // 34 and 53; 120 and 16 of 2000 16, 25 and 41 against 22, 31 and 51; 8 KV heads of 128: 80 and 16 of 2000 keys (640
+    // units of 16 rows) 47 against 50, 120 and 16 (1024) 72 against 59; one of 512 rows of 2 KV heads (64 units) 24
+    // against 23.
     const size_t unit_rows = (size_t)a.max_q * a.group, units = (unit_rows + 15) / 16 * kv * p->n_seq;
     if (unit_rows > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
-    if (unit_rows <= 32 || units <= 64) return attn_rows(ctx, a, p->max_ctx, unit_rows, stream);
+    if (unit_rows <= 64 || (unit_rows <= 128 && units <= 640) || units <= 64) return attn_rows(ctx, a, p->max_ctx, unit_rows, stream);
     // A few long chunks among single tokens (the others' mean is a part of 128 rows): the two kinds by a launch each.
     const size_t few = a.group <= 8 ? 8 : 32, others = a.n_tok > a.max_q ? a.n_tok - a.max_q : 0;
     if (a.n_seq > 1 && a.group <= few && others * a.group < (size_t)128 * (a.n_seq - 1)) {
