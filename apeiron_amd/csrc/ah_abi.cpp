@@ -524,9 +524,9 @@ int32_t few_quantize(ah_ctx *ctx, FewArgs &a, void *stream, uint8_t *fixed, size
     if (fixed) {
         if (need > fixed_cap) return AH_ERR_SCRATCH_LIMIT;
     } else {
-        const int32_t st = ensure_scratch(ctx, need);
+        const int32_t st = ensure_scratch(ctx, need, stream);
         if (st) return st;
-        S = static_cast<uint8_t *>(ctx->scratch);
+        S = static_cast<uint8_t *>(ctx->scratch.p);
     }
     QuantArgs q;
     q.x = a.x;
@@ -694,12 +694,12 @@ int32_t gemm_group_launch(ah_ctx *ctx, size_t n_parts, const ah_tensor *const *w
         if (src == AH_SRC_CODES && n_in_sz % 4) {
             if (fixed) return AH_ERR_INVALID_ARG;
             pitch = (n_in_sz + 3) & ~(size_t)3;
-            int32_t st = ensure_scratch(ctx, n_tok * pitch);
+            int32_t st = ensure_scratch(ctx, n_tok * pitch, stream);
             if (st) return st;
             AH_HIP(ctx, hipSetDevice(ctx->device));
-            AH_HIP(ctx, hipMemcpy2DAsync(ctx->scratch, pitch, x, n_in_sz, n_in_sz, n_tok, hipMemcpyDeviceToDevice,
+            AH_HIP(ctx, hipMemcpy2DAsync(ctx->scratch.p, pitch, x, n_in_sz, n_in_sz, n_tok, hipMemcpyDeviceToDevice,
                                          pick(ctx, stream)));
-            codes = static_cast<const int8_t *>(ctx->scratch);
+            codes = static_cast<const int8_t *>(ctx->scratch.p);
         }
         auto x_of = [&](size_t c) -> const void * {
             return src == AH_SRC_F32 ? static_cast<const void *>(static_cast<const float *>(x) + c * n_in_sz)
@@ -836,9 +836,9 @@ int32_t gemm_group_launch(ah_ctx *ctx, size_t n_parts, const ah_tensor *const *w
     if (fixed) {
         if (off > fixed_cap) return AH_ERR_SCRATCH_LIMIT;
     } else {
-        const int32_t st = ensure_scratch(ctx, off);
+        const int32_t st = ensure_scratch(ctx, off, stream);
         if (st) return st;
-        S = static_cast<uint8_t *>(ctx->scratch);
+        S = static_cast<uint8_t *>(ctx->scratch.p);
     }
     _Float16 *xh = any_f16 ? reinterpret_cast<_Float16 *>(S + o_xh) : nullptr;
     _Float16 *xf = any_tile ? reinterpret_cast<_Float16 *>(S + o_xf) : nullptr;
@@ -1023,8 +1023,8 @@ int32_t ah_destroy(ah_ctx *ctx) {
     if (!ctx) return AH_ERR_INVALID_ARG;
     (void)hipSetDevice(ctx->device);
     (void)hipStreamSynchronize(ctx->stream);
-    if (ctx->scratch) (void)hipFree(ctx->scratch);
-    if (ctx->ffn_buf) (void)hipFree(ctx->ffn_buf);
+    release(ctx->scratch);
+    release(ctx->ffn_buf);
     (void)hipFree(ctx->d_status);
     (void)hipFree(ctx->d_count);
     (void)hipStreamDestroy(ctx->stream);
@@ -1354,20 +1354,9 @@ static int32_t ffn_prefill_gate_up(ah_ctx *ctx, const ah_tensor *gate, const ah_
     float *g = d_gate_y, *u = d_up_y;
     if (!g || !u) {
         const size_t want = 2 * align256(n_tok * n_ff * 4);
-        if (want > ctx->ffn_buf_bytes) {
-            if (ctx->ffn_buf) {
-                AH_HIP(ctx, hipDeviceSynchronize());  // queued kernels may still use the old buffer
-                AH_HIP(ctx, hipFree(ctx->ffn_buf));
-                ctx->ffn_buf = nullptr;
-                ctx->ffn_buf_bytes = 0;
-            }
-            if (hipMalloc(&ctx->ffn_buf, want) != hipSuccess) {
-                ctx->ffn_buf = nullptr;
-                return AH_ERR_OUT_OF_MEMORY;
-            }
-            ctx->ffn_buf_bytes = want;
-        }
-        float *b = static_cast<float *>(ctx->ffn_buf);
+        const int32_t gst = grow(ctx, ctx->ffn_buf, want, want, stream);
+        if (gst) return gst;
+        float *b = static_cast<float *>(ctx->ffn_buf.p);
         if (!g) g = b;
         if (!u) u = reinterpret_cast<float *>(reinterpret_cast<uint8_t *>(b) + align256(n_tok * n_ff * 4));
     }
@@ -1876,7 +1865,7 @@ int32_t ah_set_gemm_design(ah_ctx *ctx, uint32_t ggml_type, uint32_t design) {
 
 int32_t ah_ctx_scratch_bytes(const ah_ctx *ctx, size_t *bytes) {
     if (!ctx || !bytes) return AH_ERR_INVALID_ARG;
-    *bytes = ctx->scratch_bytes;
+    *bytes = ctx->scratch.bytes + ctx->scratch.old_bytes;
     return AH_OK;
 }
 
@@ -1920,9 +1909,9 @@ int32_t ah_sync_status(ah_ctx *ctx, void *stream) {
 int32_t ah_probe_mfma_peak(ah_ctx *ctx, uint32_t kind, double *tera_ops) {
     if (!ctx || !tera_ops || kind > 1) return AH_ERR_INVALID_ARG;
     const size_t o_sink = 256, sink_bytes = (size_t)2 * ctx->cu_count * 256 * 4;
-    int32_t st = ensure_scratch(ctx, o_sink + sink_bytes);
+    int32_t st = ensure_scratch(ctx, o_sink + sink_bytes, nullptr);
     if (st) return st;
-    uint8_t *S = static_cast<uint8_t *>(ctx->scratch);
+    uint8_t *S = static_cast<uint8_t *>(ctx->scratch.p);
     const uint32_t seed[8] = {0x9e3779b9u, 0x7f4a7c15u, 0x85ebca6bu, 0xc2b2ae35u,
                               0x27d4eb2fu, 0x165667b1u, 0xd3a2646cu, 0xfd7046c5u};
     AH_HIP(ctx, hipSetDevice(ctx->device));
@@ -1940,9 +1929,9 @@ int32_t ah_matvec_q8act(ah_ctx *ctx, const ah_tensor *w, const int8_t *codes, co
     if (n_codes != w->n_in) return AH_ERR_SHAPE_MISMATCH;
     const size_t nb = (w->n_in + 31) / 32;
     const size_t oc = 0, os = align256(w->n_in), oy = align256(os + nb * 8);
-    int32_t st = ensure_scratch(ctx, oy + w->n_out * 4);
+    int32_t st = ensure_scratch(ctx, oy + w->n_out * 4, nullptr);
     if (st) return st;
-    uint8_t *S = static_cast<uint8_t *>(ctx->scratch);
+    uint8_t *S = static_cast<uint8_t *>(ctx->scratch.p);
     AH_HIP(ctx, hipSetDevice(ctx->device));
     if (w->n_in) {
         AH_HIP(ctx, hipMemcpy(S + oc, codes, w->n_in, hipMemcpyHostToDevice));
@@ -1988,9 +1977,9 @@ int32_t ah_quant_act(ah_ctx *ctx, const int64_t *x, size_t n, int8_t *codes, int
     if (n == 0) return AH_OK;
     const size_t nb = (n + 31) / 32;
     const size_t ox = 0, oc = align256(n * 8), os = align256(oc + n);
-    int32_t st = ensure_scratch(ctx, os + nb * 8);
+    int32_t st = ensure_scratch(ctx, os + nb * 8, nullptr);
     if (st) return st;
-    uint8_t *S = static_cast<uint8_t *>(ctx->scratch);
+    uint8_t *S = static_cast<uint8_t *>(ctx->scratch.p);
     AH_HIP(ctx, hipSetDevice(ctx->device));
     AH_HIP(ctx, hipMemcpy(S + ox, x, n * 8, hipMemcpyHostToDevice));
     st = quant_dev(ctx, AH_SRC_Q32, S + ox, 1, n, reinterpret_cast<int8_t *>(S + oc),

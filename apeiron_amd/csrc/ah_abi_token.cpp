@@ -33,13 +33,13 @@ size_t most_tiles(const AttnArgs &a, size_t max_ctx, size_t max_q) {
 }
 
 // Room for the partial results of `rows` rows in each of a.splits pieces.
-int32_t attn_scratch(ah_ctx *ctx, AttnArgs &a, size_t rows) {
+int32_t attn_scratch(ah_ctx *ctx, AttnArgs &a, size_t rows, void *stream) {
     if (a.splits == 1) return AH_OK;
     const size_t o = align256(a.splits * rows * a.c.dim * sizeof(float));
-    const int32_t st = ensure_scratch(ctx, o + a.splits * rows * 2 * sizeof(float));
+    const int32_t st = ensure_scratch(ctx, o + a.splits * rows * 2 * sizeof(float), stream);
     if (st) return st;
-    a.part_o = static_cast<float *>(ctx->scratch);
-    a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch) + o);
+    a.part_o = static_cast<float *>(ctx->scratch.p);
+    a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch.p) + o);
     a.count = ctx->d_count;
     return AH_OK;
 }
@@ -59,7 +59,7 @@ int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t
     if (units > kMaxGrid / a.splits) return AH_ERR_INVALID_ARG;
     a.grid = (uint32_t)(units * a.splits);
     AH_HIP(ctx, hipSetDevice(ctx->device));
-    const int32_t st = attn_scratch(ctx, a, (size_t)a.n_tok * a.n_heads);
+    const int32_t st = attn_scratch(ctx, a, (size_t)a.n_tok * a.n_heads, stream);
     if (st) return st;
     AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
     return AH_OK;
@@ -407,9 +407,9 @@ int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, siz
     a.n_counts = (uint32_t)kCounts;
     AH_HIP(ctx, hipSetDevice(ctx->device));
     const uint32_t cus = (uint32_t)ctx->cu_count;
-    const int32_t st = ensure_scratch(ctx, ah_sample_plan(a, cus, nullptr));
+    const int32_t st = ensure_scratch(ctx, ah_sample_plan(a, cus, nullptr), stream);
     if (st) return st;
-    (void)ah_sample_plan(a, cus, static_cast<uint8_t *>(ctx->scratch));
+    (void)ah_sample_plan(a, cus, static_cast<uint8_t *>(ctx->scratch.p));
     AH_HIP(ctx, ah_launch_sample(a, pick(ctx, stream)));
     return AH_OK;
 }

@@ -294,7 +294,9 @@ int32_t ah_seq_info(const ah_seq *seq, uint32_t *grid, uint32_t *act_bytes);
  * in-stream pass into context scratch (grown on demand, never shrunk), which also holds split-K
  * partials.  (Calls of a few tokens quantize inside the kernel where that is cheaper.)  GEMM calls
  * on one context share that scratch: calls on different streams of the same context must not
- * overlap (use one context per stream for concurrent prefills). */
+ * overlap (use one context per stream for concurrent prefills).  A call captured into a graph is made
+ * once before at the same sizes, so that the scratch has grown; scratch that a captured call has used is
+ * kept until ah_destroy when a later call outgrows it, so the graph may be replayed after any other calls. */
 int32_t ah_gemm_f32_dev(ah_ctx *ctx, const ah_tensor *w, const float *d_x, size_t n_tok,
                         float *d_y, void *stream);
 /* ah_gemm_f32_dev that allocates nothing.  No counterpart in the reference: it is for callers
@@ -310,8 +312,9 @@ int32_t ah_gemm_f32_dev(ah_ctx *ctx, const ah_tensor *w, const float *d_x, size_
 int32_t ah_gemm_f32_noalloc_dev(ah_ctx *ctx, const ah_tensor *w, const float *d_x, size_t n_tok,
                                 float *d_y, void *stream);
 int32_t ah_gemm_noalloc_scratch_bytes(size_t *bytes);
-/* Bytes of device scratch the context holds (grown on demand by the allocating GEMM forms; 0 until
- * one of them runs): lets a caller check that a sequence of calls allocated nothing. */
+/* Bytes of device scratch the context holds (grown on demand by the allocating GEMM forms, attention and
+ * sampling; 0 until one of them runs), what is kept for captured calls counted in: lets a caller check
+ * that a sequence of calls allocated nothing. */
 int32_t ah_ctx_scratch_bytes(const ah_ctx *ctx, size_t *bytes);
 /* Same from pre-quantized codes[n_tok][n_in] + scales[n_tok][ceil(n_in/32)]. */
 int32_t ah_gemm_q8_dev(ah_ctx *ctx, const ah_tensor *w, const int8_t *d_codes,
@@ -451,8 +454,7 @@ int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *t
  * mixed in a call.  A sequence whose tokens, context or pages are out of range is refused with
  * AH_ERR_CACHE_RANGE: its tokens are not written, or (a page) the page's positions not seen.  At most 65535
  * sequences, 2^23 rows (tokens times heads a KV head) of a sequence, and 2^24 workgroups' worth of both.
- * Uses the context's scratch (as ah_gemm_f32_dev): a call that is captured into a graph is made once before
- * at the same sizes, so that the scratch has grown. */
+ * Uses the context's scratch (as ah_gemm_f32_dev, also for calls captured into a graph). */
 typedef struct ah_kv4_attn {
     size_t n_seq, n_tok, n_heads, max_q, max_ctx;
     const int32_t *d_q_start; /* [n_seq + 1] */
@@ -466,7 +468,7 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *arg
                         float *d_out, size_t out_stride, void *stream);
 
 /* One token per row of logits [n_rows][n_vocab] (rows row_stride floats apart; n_vocab <= 2^20, n_rows <=
- * 65536).  Uses the context's scratch (as ah_gemm_f32_dev; before a capture, as ah_kv4_attn_dev).  In the
+ * 65536).  Uses the context's scratch (as ah_gemm_f32_dev, also for calls captured into a graph).  In the
  * order (logit descending, index ascending), with weights w = rint(2^32 exp((logit - largest) / T)): the
  * first top_k tokens are kept (top_k <= 0 or >= n_vocab: all), of those the ones whose preceding weight is
  * below top_p times the weight of all (top_p >= 1: all), of those the ones with w >= min_p 2^32; the first
