@@ -96,6 +96,21 @@ template <class F> AH_DEV uint32_t last_starting(uint32_t n, uint32_t at, F star
     return lo;
 }
 
+// The sequence for which holds(i) is true (any, if there is none).  Where the entries of q_start in range ascend, sequence i
+// holds what lies between start(i) and start(i + 1).  One out of range leads the search astray: a find that the entries
+// beside it don't confirm is looked up among all sequences.
+template <class S, class H> AH_DEV uint32_t sequence_of(const AttnArgs &a, uint32_t at, S start, H holds) {
+    uint32_t s = last_starting(a.n_seq, at, start);
+    auto in_range = [&](uint32_t i) { return (uint32_t)a.q_start[i] <= a.n_tok; };
+    if (in_range(s) && in_range(s + 1) && (start(s) <= at ? s + 1 == a.n_seq || start(s + 1) > at : s == 0)) return s;
+    for (uint32_t base = 0; base < a.n_seq; base += 64) {
+        const uint32_t i = base + (threadIdx.x & 63);
+        const uint64_t b = __builtin_amdgcn_ballot_w64(i < a.n_seq && holds(i < a.n_seq ? i : 0));
+        if (b) s = base + 63 - (uint32_t)__builtin_clzll(b);
+    }
+    return s;
+}
+
 // The tiles that rows at positions lo .. hi see: [0, head) and [tail, end).
 struct Tiles {
     uint32_t head, tail, end, count;
@@ -493,7 +508,11 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     }
     const uint32_t at = units / a.c.n_kv - 1 - unit / a.c.n_kv, kvh = unit % a.c.n_kv;
     auto start = [&](uint32_t i) { return (uint32_t)((uint64_t)(uint32_t)a.q_start[i] * a.group >> 7) + i; };
-    const uint32_t s = a.per ? at / a.per : last_starting(a.n_seq, at, start), rt = at - (a.per ? s * a.per : start(s));
+    auto holds = [&](uint32_t i) {
+        const Span p = span_of(a, i);
+        return at >= start(i) && at - start(i) < (p.nq * a.group + 127) / 128;
+    };
+    const uint32_t s = a.per ? at / a.per : sequence_of(a, at, start, holds), rt = at - (a.per ? s * a.per : start(s));
     if (split == 0 && kvh == 0 && at < a.n_seq && threadIdx.x == 0 && span_of(a, at).bad) ah_record(a.status, ((unsigned long long)at << 8) + AH_ERR_CACHE_RANGE);
     const Span p = span_of(a, s);
     const uint32_t rows = p.nq * a.group, row0 = rt * 128;
@@ -849,7 +868,12 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     const uint32_t lane = threadIdx.x & 63, it = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     const uint32_t per = (a.n_heads + kHeads - 1) / kHeads, tok = it / per, head = (it - tok * per) * kHeads + lane / kLanes, g = a.group;
     if (tok >= a.n_tok) return;
-    const uint32_t s = last_starting(a.n_seq, tok, [&](uint32_t i) { return (uint32_t)a.q_start[i]; });
+    auto start = [&](uint32_t i) { return (uint32_t)a.q_start[i]; };
+    auto holds = [&](uint32_t i) {
+        const Span p = span_of(a, i);
+        return tok >= p.q0 && tok - p.q0 < p.nq;
+    };
+    const uint32_t s = sequence_of(a, tok, start, holds);
     const Span p = span_of(a, s);
     if (tok < p.q0 || tok - p.q0 >= p.nq || p.nq * g < a.least_rows || head >= a.n_heads) return;
     const uint32_t i = tok - p.q0;

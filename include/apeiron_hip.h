@@ -452,7 +452,8 @@ int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *t
  * max_q: at least the largest number of a sequence's tokens; max_ctx: the largest context expected (it
  * plans how the contexts are cut; longer ones are still served whole).  Single tokens and chunks may be
  * mixed in a call.  A sequence whose tokens, context or pages are out of range is refused with
- * AH_ERR_CACHE_RANGE: its tokens are not written, or (a page) the page's positions not seen.  At most 65535
+ * AH_ERR_CACHE_RANGE: its tokens are not written, or (a page) the page's positions not seen, and the others are
+ * served (two that such an entry of d_q_start leaves out of order: either's tokens may stay unwritten).  At most 65535
  * sequences, 2^23 rows (tokens times heads a KV head) of a sequence, and 2^24 workgroups' worth of both.
  * Uses the context's scratch (as ah_gemm_f32_dev, also for calls captured into a graph). */
 typedef struct ah_kv4_attn {
