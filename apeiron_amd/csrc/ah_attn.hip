@@ -3,8 +3,10 @@
 // o = sum_t softmax_t(scale q . k_t) v_t over the keys t a query at position p sees: t <= p and, with a
 // window, t > p - window or t < sinks.  One pass over the cache with the running maximum and sum of the
 // softmax in f32, K q and P V on the f16 matrix cores.  The cache's values are exact in f16; q and p are
-// carried as f16 pairs hi + lo (22 bits), each pair's two products summed in the f32 accumulator, so the
-// result is that of f32 arithmetic.
+// carried as f16 pairs hi + lo, both rounded to nearest (23 bits: a lost half would cost 12 of them), each pair's
+// two products summed in the f32 accumulator.  What is left are f32's roundings of scores, exponentials and
+// running sums: 4e-7 to 9e-7 of the outputs (root mean square against 64 bits, 4001 to 30000 keys), 7e-7 to
+// 2.1e-6 with plain f32 operations.
 #include "ah_kv4.h"
 
 namespace {
@@ -24,9 +26,9 @@ constexpr float kNoMax = -3.402823466e38f;  // below every finite score
 // The running maximum follows the scores only when one passes it by more than this (in powers of two):
 // then p <= 2^kSlack, and a rescale of the accumulators is rare after the first tiles.
 constexpr float kSlack = 4.0f;
-// p is kept times 2^kUp: a weight of 2^-13 of the largest still has its 22 bits in two f16 halves (f16's
-// subnormals end at 2^-24), and the largest, 2^(kUp + kSlack), is a finite f16.
-constexpr float kUp = 9.0f;
+// p is kept times 2^kUp: two f16 halves hold it within 2^-23 of itself or 2^-36 of the largest weight, whichever is
+// more (f16's subnormals are 2^-24 apart), and the largest, 2^(kUp + kSlack), is a finite f16.
+constexpr float kUp = 11.0f;
 
 AH_DEV f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
 
@@ -177,7 +179,7 @@ template <int D> struct VTile {
 AH_DEV float ror8(float v) {  // lane r ^ 8 of each 16 (a rotation by 8)
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), 0x128, 0xF, 0xF, true));
 }
-AH_DEV f16x2 pack16(float a, float b) { return __builtin_bit_cast(f16x2, __builtin_amdgcn_cvt_pkrtz(a, b)); }
+AH_DEV f16x2 pack16(float a, float b) { return __builtin_convertvector((f32x2){a, b}, f16x2); }  // to nearest: what is cut off has no bias
 
 // q's power-of-two scale: `up` makes the row's largest magnitude (of `top` over its lanes) lie in [2^13, 2^14) and
 // carries the scale's sign; scores times f are in powers of two.  f > 0, so that the largest product is also
@@ -335,17 +337,19 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
             }
         }
         const float base = kUp - m;
+        float ls = 0.0f;  // the tile's weights, as in attn_tile_kernel
         f16x2 ph[4], pl[4];
 #pragma unroll
         for (int i = 0; i < 4; ++i) {
             float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], f, base)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], f, base));
-            l += e0;
-            l += e1;
+            ls = i ? ls + e0 : e0;
+            ls += e1;
             ph[i] = pack16(e0, e1);
             // what is left of p past its hi half; a packed column takes that or p itself
             const float k = PACK ? minus_low : -1.0f;
             pl[i] = pack16(__builtin_fmaf((float)ph[i][0], k, e0), __builtin_fmaf((float)ph[i][1], k, e1));
         }
+        l += ls;
         const f16x8 pg = join8(pl[0], pl[1], pl[2], pl[3]), pf = PACK ? pg : join8(ph[0], ph[1], ph[2], ph[3]);
 #pragma unroll
         for (int g = 0; g < NJ; ++g) {
@@ -650,6 +654,9 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
                 // first, and the next tile's conversion between the last products.  (Past the last tile that
                 // converts what is left in the registers into a buffer that nobody reads.)
                 f32x16 sc[2];
+                // A half's weights are summed alone and added to l once.  Added one by one, those below the last place of a sum that
+                // one key rules are each lost or rounded up: 40037 keys of 2^-20 to 2^-24 of the first, 7e-5 of the outputs.
+                float ls;
                 uint32_t ph[8], pl[8], pn[8], pm[8];  // f16 pairs
                 auto k_read = [&](int j, int k) {
                     f16x8 v;
@@ -690,12 +697,12 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
                 auto exp_pair = [&](int j, int i, float base, uint32_t &hi2, uint32_t &lo2) {
                     const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][2 * i], f, base));
                     const float e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(sc[j][2 * i + 1], f, base));
-                    l += e0;
-                    l += e1;
+                    ls = i ? ls + e0 : e0;
+                    ls += e1;
                     const f16x2 t = pack16(e0, e1);
                     hi2 = __builtin_bit_cast(uint32_t, t);
                     lo2 = __builtin_bit_cast(uint32_t, pack16(__builtin_fmaf((float)t[0], -1.0f, e0), __builtin_fmaf((float)t[1], -1.0f, e1)));
-                    __asm__ volatile("" : "+v"(hi2), "+v"(lo2), "+v"(l));
+                    __asm__ volatile("" : "+v"(hi2), "+v"(lo2), "+v"(ls));
                 };
                 auto frag = [](const uint32_t *v) { return __builtin_bit_cast(f16x8, (u32x4){v[0], v[1], v[2], v[3]}); };
                 // One stream of fragments from LDS, read kAhead steps before its two products: the halves' K rows, then
@@ -728,6 +735,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
                     for (int i = 8 * k / NK; i < 8 * (k + 1) / NK; ++i) exp_pair(0, i, base0, ph[i], pl[i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                l += ls;
                 mask(1);
                 // p of the first half was taken at the maximum so far: a new one scales its product with the rest
                 f16x8 pf[2], pg[2];
@@ -759,6 +767,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
                     for (int i = 8 * q / (2 * NN); i < 8 * (q + 1) / (2 * NN); ++i) exp_pair(1, i, base1, pn[i], pm[i]);
                     __builtin_amdgcn_sched_barrier(0);
                 }
+                l += ls;
                 if (moves) {
 #pragma unroll
                     for (int n = 0; n < NN; ++n) acc[n] *= alpha;
