@@ -14,7 +14,7 @@ constexpr size_t kMaxU32 = 0x7fffffff;
 constexpr size_t kAttnGroups = 2048;
 static_assert(kAttnGroups <= kCounts, "an entry for each unit and each group of pieces");
 
-constexpr size_t kMaxGrid = ((size_t)1 << 32) / 256 - 1;  // workgroups of 256 threads in a launch
+constexpr size_t max_grid(size_t threads) { return 0xffffffffu / threads; }  // workgroups of a launch: under 2^32 threads
 
 bool tokens_ok(const ah_kv4_tokens *t) {
     return t->d_seq && t->d_pos && t->d_table && t->n_seq && t->table_stride && t->n_tok <= kMaxU32 && t->n_seq <= kMaxU32 &&
@@ -56,7 +56,7 @@ int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t
     a.splits = a.splits < 1 ? 1 : a.splits;
     if (a.rows != 128) a.join = a.splits <= 40 ? a.splits : (uint32_t)std::ceil(std::sqrt((double)a.splits));
     else a.join = a.splits <= 3 && a.c.dim == 64 && units <= kCounts;
-    if (units > kMaxGrid / a.splits) return AH_ERR_INVALID_ARG;
+    if (units > max_grid(256) / a.splits) return AH_ERR_INVALID_ARG;
     a.grid = (uint32_t)(units * a.splits);
     AH_HIP(ctx, hipSetDevice(ctx->device));
     const int32_t st = attn_scratch(ctx, a, (size_t)a.n_tok * a.n_heads, stream);
@@ -156,7 +156,7 @@ int32_t ah_norm_quant_dev(ah_ctx *ctx, const float *d_x, const float *d_residual
     if (!ctx || (d_codes == nullptr) != (d_scales == nullptr)) return AH_ERR_INVALID_ARG;
     if (!(eps >= 0.0f) || n > AH_MAX_N_IN || n_tok > kMaxU32) return AH_ERR_INVALID_ARG;
     if (n_tok == 0 || n == 0) return AH_OK;
-    if (!d_x || !d_gain || (reinterpret_cast<uintptr_t>(d_scales) & 7)) return AH_ERR_INVALID_ARG;
+    if (!d_x || !d_gain || (reinterpret_cast<uintptr_t>(d_scales) & 7) || n_tok > max_grid(norm_lanes(n))) return AH_ERR_INVALID_ARG;
     NormArgs a = {d_x, d_residual, d_gain, d_sum, d_y, d_codes, d_scales, d_values, (double)eps, (uint32_t)n_tok, (uint32_t)n,
                   ctx->d_status};
     AH_HIP(ctx, hipSetDevice(ctx->device));
@@ -239,7 +239,9 @@ int32_t ah_rope_dev(ah_ctx *ctx, const ah_rope *rope, const float *d_x, size_t x
     if (!ctx || !rope || n_tok > kMaxU32 || n_heads > 65536) return AH_ERR_INVALID_ARG;
     if (n_tok == 0 || n_heads == 0) return AH_OK;
     const size_t row = n_heads * rope->ref.dim;
-    if (!d_x || !d_y || !d_pos || x_stride < row || y_stride < row || (d_x == d_y && x_stride != y_stride)) return AH_ERR_INVALID_ARG;
+    if (!d_x || !d_y || !d_pos || x_stride < row || y_stride < row || (d_x == d_y && x_stride != y_stride) ||
+        n_tok > max_grid(rope_lanes(rope->ref.dim, n_heads)))
+        return AH_ERR_INVALID_ARG;
     RopeArgs a = {rope->ref, d_x, d_y, x_stride, y_stride, d_pos, (uint32_t)n_tok, (uint32_t)n_heads};
     AH_HIP(ctx, hipSetDevice(ctx->device));
     AH_HIP(ctx, ah_launch_rope(a, pick(ctx, stream)));
@@ -303,7 +305,8 @@ int32_t ah_kv4_append_dev(ah_ctx *ctx, ah_kv4 *cache, const ah_rope *rope, const
     if (tokens->n_tok == 0) return AH_OK;
     if (!tokens_ok(tokens) || !d_k || !d_v || n_heads > 65536) return AH_ERR_INVALID_ARG;
     const size_t dim = cache->ref.dim, kv = cache->ref.n_kv * dim;
-    if (k_stride < kv || v_stride < kv || (rope && rope->ref.dim != dim)) return AH_ERR_INVALID_ARG;
+    if (k_stride < kv || v_stride < kv || (rope && rope->ref.dim != dim) || tokens->n_tok > max_grid(append_lanes(cache->ref, n_heads)))
+        return AH_ERR_INVALID_ARG;
     if (n_heads && (!d_q || !d_q_out || q_stride < n_heads * dim || q_out_stride < n_heads * dim ||
                     (d_q == d_q_out && q_stride != q_out_stride)))
         return AH_ERR_INVALID_ARG;
@@ -329,7 +332,7 @@ int32_t ah_kv4_append_dev(ah_ctx *ctx, ah_kv4 *cache, const ah_rope *rope, const
 int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *tokens, uint16_t *d_k, uint16_t *d_v, void *stream) {
     if (!ctx || !cache || !tokens) return AH_ERR_INVALID_ARG;
     if (tokens->n_tok == 0 || (!d_k && !d_v)) return AH_OK;
-    if (!tokens_ok(tokens)) return AH_ERR_INVALID_ARG;
+    if (!tokens_ok(tokens) || tokens->n_tok > max_grid(append_lanes(cache->ref, 0))) return AH_ERR_INVALID_ARG;
     KvReadArgs a = {cache->ref, tokens_of(tokens), d_k, d_v, ctx->d_status};
     AH_HIP(ctx, hipSetDevice(ctx->device));
     AH_HIP(ctx, ah_launch_kv4_read(a, pick(ctx, stream)));

@@ -163,6 +163,16 @@ struct SampleArgs {
 };
 constexpr uint32_t kSampleList = 4096, kSampleMaxChunks = 512;
 
+// Threads of a token's workgroup: of the norm a lane per 8 values up to 1024 lanes, then more passes; of the others
+// whole waves for `items` lanes' work, up to four.
+inline uint32_t norm_lanes(size_t n) {
+    const size_t need = (n + 7) / 8;
+    return need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : need <= 512 ? 512 : 1024;
+}
+inline uint32_t lanes_for(size_t items) { return items >= 256 ? 256 : (uint32_t)(items + 63) / 64 * 64; }
+inline uint32_t rope_lanes(size_t dim, size_t n_heads) { return lanes_for((dim + 7) / 8 * n_heads); }  // (a head takes up to 64)
+inline uint32_t append_lanes(const Kv4Ref &c, size_t n_heads) { return lanes_for(c.dim / 8 * (n_heads + 2 * (size_t)c.n_kv)); }  // the read's: no heads
+
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream);
 hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream);
 hipError_t ah_launch_kv4_append(const AppendArgs &a, hipStream_t stream);

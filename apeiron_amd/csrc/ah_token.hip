@@ -351,15 +351,10 @@ __global__ void __launch_bounds__(256) kv4_read_kernel(KvReadArgs a) {
     }
 }
 
-// Lanes of a token's workgroup: whole waves, up to four.
-uint32_t lanes_for(size_t items) { return items >= 256 ? 256 : (uint32_t)(items + 63) / 64 * 64; }
-
 } // namespace
 
 hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream) {
-    // a lane per 8 values up to 1024 lanes, then more passes
-    const uint32_t need = (a.n + 7) / 8;
-    const uint32_t T = need <= 64 ? 64 : need <= 128 ? 128 : need <= 256 ? 256 : need <= 512 ? 512 : 1024;
+    const uint32_t need = (a.n + 7) / 8, T = norm_lanes(a.n);
     auto *k = need <= 1024   ? (a.r ? norm_quant_kernel<1, true> : norm_quant_kernel<1, false>)
               : need <= 2048 ? (a.r ? norm_quant_kernel<2, true> : norm_quant_kernel<2, false>)
                              : (a.r ? norm_quant_kernel<4, true> : norm_quant_kernel<4, false>);
@@ -368,17 +363,16 @@ hipError_t ah_launch_norm(const NormArgs &a, hipStream_t stream) {
 }
 
 hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream) {
-    // (at least a head's lanes: up to 64)
-    hipLaunchKernelGGL(rope_kernel, dim3(a.n_tok), dim3(lanes_for((size_t)(a.rope.dim + 7) / 8 * a.n_heads)), 0, stream, a);
+    hipLaunchKernelGGL(rope_kernel, dim3(a.n_tok), dim3(rope_lanes(a.rope.dim, a.n_heads)), 0, stream, a);
     return hipGetLastError();
 }
 
 hipError_t ah_launch_kv4_append(const AppendArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(kv4_append_kernel, dim3(a.t.n_tok), dim3(lanes_for((size_t)a.c.dim / 8 * (a.n_heads + 2 * a.c.n_kv))), 0, stream, a);
+    hipLaunchKernelGGL(kv4_append_kernel, dim3(a.t.n_tok), dim3(append_lanes(a.c, a.n_heads)), 0, stream, a);
     return hipGetLastError();
 }
 
 hipError_t ah_launch_kv4_read(const KvReadArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(kv4_read_kernel, dim3(a.t.n_tok), dim3(lanes_for((size_t)a.c.dim / 8 * 2 * a.c.n_kv)), 0, stream, a);
+    hipLaunchKernelGGL(kv4_read_kernel, dim3(a.t.n_tok), dim3(append_lanes(a.c, 0)), 0, stream, a);
     return hipGetLastError();
 }

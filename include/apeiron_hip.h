@@ -371,7 +371,8 @@ int32_t ah_gemm_group_q8_dev(ah_ctx *ctx, size_t n_parts, const ah_tensor *const
  *   ah_ffn_prefill_q8_dev) -> ... -> ah_norm_quant_dev -> the head -> ah_sample_dev.
  * No counterpart in the reference's int8 chart (its norm, RoPE, softmax attention and sampler are
  * exact Q32.32 integer code of the engine: ops/{norm,rope,sampler}.rs, attn.rs).  Activations are f32
- * rows; sums and statistics are held in f32 or f64. */
+ * rows; sums and statistics are held in f32 or f64.  A call takes as many tokens as a launch holds
+ * workgroups, 2^24 - 1 at least (the norm 2^22 - 1); more are refused with AH_ERR_INVALID_ARG. */
 
 /* s = x + residual (residual NULL: s = x); y = s / sqrt(mean(s^2) + eps) * gain per token of n values
  * (1 <= n <= AH_MAX_N_IN), and y's QuantAct, bit-exact to ah_quant_act_f32_dev on the same y.

@@ -3,7 +3,7 @@ sequences, pieces joined in the launch (heads of 64) and by another (128, 256), 
 import numpy as np
 import pytest
 
-from test_gpu_token_ops import CACHE, OK, cuda, dev, filled, ptr, stream  # noqa: F401
+from test_gpu_token_ops import CACHE, INVALID, OK, cuda, dev, filled, ptr, stream  # noqa: F401
 
 torch = pytest.importorskip("torch")
 pytestmark = pytest.mark.gpu
@@ -63,3 +63,25 @@ def test_a_start_out_of_range_leaves_the_other_sequences(dev, dim, G, qs, ctx): 
     st, o = C(start=start)
     kept = C.rows(*range(1, n - 3))
     assert st == CACHE and np.array_equal(o[kept], good[kept]) and (o[~kept] == 7).all()
+
+
+def test_more_tokens_than_a_launch_holds_are_refused(dev):  # noqa: F811
+    """A workgroup a token, fewer than 2^32 threads a launch: refused on the host, nothing is read."""
+    from apeiron_amd import _lib, chart
+
+    L, h, x = dev.lib, dev.h, torch.zeros(64, device="cuda")
+    p = ptr(x)
+    # (values of a token, its threads)
+    for n, threads in ((32, 64), (1024, 128), (2048, 256), (4096, 512), (4097, 1024), (32768, 1024)):
+        assert L.ah_norm_quant_dev(h, p, None, p, 1e-6, (1 << 32) // threads, n, None, p, None, None, None, None) == INVALID, n
+    rope, cache = chart.Rope(dev, 128), chart.KvCache4(dev, 2, 32, 8, 128)
+    assert L.ah_rope_dev(h, rope.h, p, 16 * 128, 16, p, 1 << 24, p, 16 * 128, None) == INVALID
+    assert L.ah_rope_dev(h, rope.h, p, 128, 1, p, 1 << 26, p, 128, None) == INVALID
+    t = _lib.Kv4Tokens(p, p, 1 << 24, p, 1, 1)
+    assert L.ah_kv4_append_dev(h, cache.h, None, t, None, 0, 0, None, 0, p, 1024, p, 1024, None) == INVALID
+    assert L.ah_kv4_append_dev(h, cache.h, rope.h, t, p, 2048, 16, p, 2048, p, 1024, p, 1024, None) == INVALID
+    assert L.ah_kv4_read_dev(h, cache.h, t, p, p, None) == INVALID
+    small = chart.KvCache4(dev, 2, 32, 1, 64)  # a wave a token
+    t = _lib.Kv4Tokens(p, p, 1 << 26, p, 1, 1)
+    assert L.ah_kv4_append_dev(h, small.h, None, t, None, 0, 0, None, 0, p, 64, p, 64, None) == INVALID
+    assert dev.sync_status(stream()) == OK
