@@ -19,6 +19,7 @@ libapeiron_hip.so.
 from __future__ import annotations
 
 import ctypes
+import weakref
 from dataclasses import dataclass
 
 import numpy as np
@@ -55,7 +56,8 @@ class Device:
     """One ah_ctx on one GPU (the backend's context; not thread-safe, like the reference pool)."""
 
     def __init__(self, device: int = 0):
-        self.lib = _lib.load()
+        self.lib, self.h = _lib.load(), None
+        self._held = weakref.WeakSet()  # ropes and caches, which close() frees
         h = ctypes.c_void_p()
         _check(self.lib.ah_init(device, ctypes.byref(h)), "ah_init")
         self.h = h
@@ -63,6 +65,8 @@ class Device:
 
     def close(self) -> None:
         if self.h:
+            for held in list(self._held):
+                held.free()
             self.lib.ah_destroy(self.h)
             self.h = None
 
@@ -367,6 +371,7 @@ class Rope:
         h = ctypes.c_void_p()
         _check(dev.lib.ah_rope_create(dev.h, ctypes.byref(spec), ctypes.byref(h)), "rope_create")
         self.dev, self.h, self.head_dim, self.rot_dim = dev, h, head_dim, rot_dim
+        dev._held.add(self)
 
     def info(self) -> tuple[np.ndarray, float]:
         """(theta f64 [rot_dim / 2], amplitude)."""
@@ -402,6 +407,7 @@ class KvCache4:
         _check(dev.lib.ah_kv4_create(dev.h, n_pages, page_len, n_kv_heads, head_dim, ctypes.byref(h)), "kv4_create")
         self.dev, self.h = dev, h
         self.n_pages, self.page_len, self.n_kv_heads, self.head_dim = n_pages, page_len, n_kv_heads, head_dim
+        dev._held.add(self)
 
     def info(self) -> tuple[int, int, int, int, int]:
         """(bytes, n_pages, page_len, n_kv_heads, head_dim)."""
