@@ -3,6 +3,7 @@ sequences, pieces joined in the launch (heads of 64) and by another (128, 256), 
 import numpy as np
 import pytest
 
+from test_attention_accuracy import bound
 from test_gpu_token_ops import CACHE, INVALID, OK, cuda, dev, filled, ptr, stream  # noqa: F401
 
 torch = pytest.importorskip("torch")
@@ -28,6 +29,22 @@ class Call:
                               table_ptr=ptr(table), table_stride=self.P.per, max_q=max(self.qs), max_ctx=int(self.ctx.max()), scale=self.dim ** -0.5,
                               stream=stream())
         return self.dev.sync_status(stream()), out.cpu().numpy()
+
+    def exact(self, s, hidden=()):
+        """f64 attention of sequence s, its pages `hidden` not seen, and its largest score in powers of two."""
+        n, c, page, kv = self.qs[s], int(self.ctx[s]), self.P.cache.page_len, self.P.cache.n_kv_heads
+        q = self.q[self.start[s]:self.start[s + 1]].reshape(n, self.heads, self.dim).astype(np.float64)
+        key = np.arange(c)
+        see = (key <= (c - n + np.arange(n))[:, None]) & ~np.isin(key // page, hidden)
+        out, S = np.zeros(q.shape), 0.0
+        for h in range(self.heads):
+            g = h * kv // self.heads
+            x = np.where(see, q[:, h] @ self.k[s][:c, g].astype(np.float64).T * self.dim ** -0.5, -np.inf)
+            top = x.max(-1, keepdims=True)
+            p = np.exp(x - np.where(np.isfinite(top), top, 0))
+            S, den = max(S, np.abs(x[see]).max() * np.log2(np.e)), p.sum(-1, keepdims=True)
+            out[:, h] = p @ self.v[s][:c, g].astype(np.float64) / np.where(den > 0, den, 1)
+        return out.reshape(n, -1), S
 
     def rows(self, *seqs):
         """The tokens of these sequences, as a mask."""
@@ -63,6 +80,82 @@ def test_a_start_out_of_range_leaves_the_other_sequences(dev, dim, G, qs, ctx): 
     st, o = C(start=start)
     kept = C.rows(*range(1, n - 3))
     assert st == CACHE and np.array_equal(o[kept], good[kept]) and (o[~kept] == 7).all()
+
+
+MIXED = ([1] * 20 + [300, 0] + [1] * 20 + [150], [130 + 9 * i for i in range(20)] + [901, 40] + [77 + 9 * i for i in range(20)] + [150])
+SIZES = pytest.mark.parametrize("qs,ctx", [EVEN, UNEVEN, MIXED], ids=["even", "uneven", "mixed"])
+
+
+@pytest.mark.parametrize("dim,G", [(64, 7), (128, 4), (256, 2)])
+@SIZES
+def test_contexts_and_lengths_out_of_range(dev, dim, G, qs, ctx):  # noqa: F811
+    C = Call(dev, dim, G, qs, ctx, page=32)
+    st, good = C()
+    assert st == OK
+    longest = int(np.argmax(qs))
+    for s in sorted({0, longest, len(qs) - 1}):
+        for value in (-1, -2 ** 31, C.P.per * 32 + 1, 2 ** 31 - 1):
+            c = C.ctx.copy()
+            c[s] = value
+            st, o = C(ctx=c)
+            kept = ~C.rows(s)
+            assert st == CACHE and np.array_equal(o[kept], good[kept]) and (o[~kept] == 7).all(), (s, value)
+    # a sequence that is longer than max_q (its neighbour gives it a token)
+    if longest + 1 < len(qs) and qs[longest + 1]:
+        start = C.start.copy()
+        start[longest + 1] += 1
+        st, o = C(start=start)
+        kept = ~C.rows(longest, longest + 1)
+        assert st == CACHE and np.array_equal(o[kept], good[kept]) and (o[start[longest]:start[longest + 1]] == 7).all()
+    # no keys: zeros, and nothing is refused
+    c = C.ctx.copy()
+    c[longest] = 0
+    st, o = C(ctx=c)
+    assert st == OK and (o[C.rows(longest)] == 0).all() and np.array_equal(o[~C.rows(longest)], good[~C.rows(longest)])
+
+
+@pytest.mark.parametrize("dim,G", [(64, 7), (128, 4), (256, 2)])
+@SIZES
+def test_pages_out_of_range_are_not_seen(dev, dim, G, qs, ctx):  # noqa: F811
+    """Pages of one tile: the first and the second of a pair of tiles, neighbours, the last one, and all of a row's."""
+    C = Call(dev, dim, G, qs, ctx, page=32)
+    st, good = C()
+    assert st == OK
+    n_pages = C.P.cache.n_pages
+    for s in sorted({int(np.argmax(qs)), len(qs) - 1}):
+        last = (ctx[s] - 1) // 32
+        for hidden in sorted({(0,), (1,), (0, 1), (last,), (last - 1,), tuple(range(last // 2))}):
+            hidden = [p for p in hidden if 0 <= p <= last]
+            if not hidden or len(hidden) == last + 1:
+                continue
+            table = C.P.table.clone()
+            for i, p in enumerate(hidden):
+                table[s, p] = (-1, n_pages, 2 ** 31 - 1, -2 ** 31)[i % 4]
+            st, o = C(table=table)
+            kept = ~C.rows(s)
+            ref, S = C.exact(s, hidden)
+            err = np.linalg.norm(o[~kept] - ref) / np.linalg.norm(ref)
+            assert st == CACHE and np.array_equal(o[kept], good[kept]), (s, hidden)
+            assert err <= bound(S, ctx[s]) and (o[~kept][(ref == 0).all(-1)] == 0).all(), (s, hidden, err)
+
+
+@pytest.mark.parametrize("dim,G", [(64, 7), (128, 4), (256, 2)])
+@SIZES
+def test_rows_that_are_not_finite_stay_alone(dev, dim, G, qs, ctx):  # noqa: F811
+    C = Call(dev, dim, G, qs, ctx, page=64)
+    st, good = C()
+    at = [(int(C.start[int(np.argmax(qs))]) + 3, 1), (len(C.q) - 1, 0)]
+    for bad in (np.nan, np.inf):
+        q = C.q.copy()
+        for tok, head in at:
+            q[tok, head * dim + 5] = bad
+        st, o = C(q=q)
+        assert st == OK
+        o, whole = o.reshape(len(q), -1, dim), good.reshape(len(q), -1, dim)
+        touched = np.zeros(o.shape[:2], bool)
+        for tok, head in at:
+            touched[tok, head] = True
+        assert np.isnan(o[touched]).all() and np.array_equal(o[~touched], whole[~touched])
 
 
 def test_more_tokens_than_a_launch_holds_are_refused(dev):  # noqa: F811
