@@ -108,7 +108,10 @@ int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
     // (with least_rows, most of the other sequences are single tokens)
     const size_t chunks = a.n_tok - (a.n_seq - 1), tokens = !a.least_rows ? a.n_tok : a.n_tok > a.n_seq && chunks > a.max_q ? chunks : a.max_q;
     size_t base = even ? per * a.n_seq * a.c.n_kv : (tokens * a.group + 127) / 128 * a.c.n_kv;
-    // uneven sequences: the longest ones' workgroups are alone in the end, as if there were fewer
+    // Uneven sequences: the longest ones' workgroups are alone in the end, as if there were fewer.  With this and
+    // without, us: heads of 64, 2 chunks of 600 over up to 8000 keys 73 and 87 (six other calls the same); of 256, 5 of
+    // 301 over 6007 162 and 203.  Elsewhere it asks for too many pieces of the larger heads: of 128, 5 of 301 over 6007 110
+    // and 89, 16 of 100 over 2000 55 and 48; of 256, 85 and 68 there, 8 of 256 over 4096 115 and 109.
     if (!even && !a.least_rows) base = (base * 3 + 4) / 5;
     const double tile = a.c.dim * 0.0077, alone = 1.4 * tile, start = 5.0, join = (double)rows * a.c.dim * 8.0 / 4e6;
     const size_t held = a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1, cus = (size_t)ctx->cu_count, places = held * cus;
@@ -118,7 +121,8 @@ int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
     };
     // Pieces of a length end together.  Under a causal mask (whole prompts) half of the workgroups and half of the keys
     // are there, longest first, and the shorter ones share the CUs or fill in, with a part of a piece at the end; uneven
-    // sequences fill in too.
+    // sequences fill in too.  With the causal form and without, us: heads of 64, prompts of 2048 and 4096 tokens 42 and 45,
+    // 93 and 113; of 128, 2048 55 and 59; of 256 72 and 88, 196 and 246 (and 4 prompts of 700 72 and 57: the other way).
     const bool causal = even && max_ctx < 2 * (size_t)a.max_q;
     size_t splits = 1, most = (tiles + 7) / 8;
     most = most < most_pieces(a, rows) ? most : most_pieces(a, rows);

@@ -487,8 +487,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
 //   What bounds it: the matrix cores, which the two halves of q and of p use twice (8192 tokens, 12 heads of 128:
 // 206 GFLOP of keys and values, 412 with the halves, in 393 us: 1050 TFLOP/s; a large f16 library product reaches
 // 1068 on this card); half of their peak, the rest the vector work of the exponentials and the codes' conversion that the
-// products do not cover (about 7 instructions hide behind one).  For chunks of a few hundred tokens the unit's start
-// and the join (1205 tokens of 5 sequences over up to 6007 keys, heads of 64: 67 and 8 us under a tracer).  With the four waves
+// products do not cover (about 7 instructions hide behind one).  Heads of 64 have 11.7 vector instructions a product:
+// while a CU works these take 56% of a SIMD's cycles and the products 35%.  Heads of 256 have 8.1, but one wave a SIMD to
+// cover either: 43% and 40%.  For chunks of a few hundred tokens the unit's start and the join (1205 tokens of 5
+// sequences over up to 6007 keys, heads of 64: 67 and 8 us under a tracer).  With the four waves
 // each converting its own fragments (no LDS) 8192 tokens took 670 us.
 template <int D> struct TileLds {
     static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;

@@ -23,7 +23,9 @@
 //   What bounds it, of 192 rows of 151936 with mixed parameters, 73 us (117 MB; 25 us by a copy's rate): scan
 // 18.6 us from the Infinity Cache and 27 from memory; count and gather 18 and 15 us, the vector work of a weight (an
 // exponential, its place among the bins, f64 sums) for each token of the groups that reach the bound, all of them
-// without top-k; draw 15 us, the chain of loads and barriers of its slowest row.  One row with k = 40: 2.7, 8.9 and
+// without top-k (vector instructions take 41% and 50% of the SIMDs' cycles while a CU works, the waves wait in 56%
+// and 60% of theirs); draw 15 us, the chain of loads and barriers of its slowest row (13% and 72%).  Rows of 262144:
+// 104 us for 192 (42 by a copy's rate), 17.8 for one.  One row with k = 40: 2.7, 8.9 and
 // 2 us, such chains; a launch each costs the host as much.  Bits for the listed tokens, not lists of each chunk's: a
 // vocabulary in the order of its logits has all of a bin in a chunk or two (top-p 0.9 of one such row 41 us against
 // the 1100 of the selections over the row, of one in any order 34 against 30).

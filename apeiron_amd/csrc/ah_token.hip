@@ -19,8 +19,9 @@ AH_DEV double wave_sum(double v) {
 // s = x + r, R = 1 / sqrt(mean(s^2) + eps), y = (s R) gain, and quant_act of y's 32-blocks.  One
 // workgroup per token: a lane keeps 8 consecutive values of each of its U passes in registers, so the
 // row is read once and the quantizer's quads (four lanes a block, ah_units.h) hold whole blocks.  The
-// sum of squares is kept in f64: the f32 row's magnitude cannot overflow it and R is the correctly
-// rounded one whatever the order of the sum.  y is rounded once to f32 by each of its two products, and
+// sum of squares is kept in f64: the f32 row's magnitude cannot overflow it, and whatever the order of the
+// sum R is the nearest f32 number, unless what it stands for lies within about 2^-45 of itself of the middle of
+// two.  y is rounded once to f32 by each of its two products, and
 // once more to seven bits by the quantizer, as the projections take it.
 //   What bounds it: memory (2039 tokens of 8957 with every output, 279 MB in 62.6 us: 4.45 TB/s, of 4.74
 // that a copy reaches); under a few hundred tokens the launch (512 of 1536 4.9 us, one of 896 2.6).  Rows
@@ -134,7 +135,8 @@ __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
 // The angle pos * theta and its cosine and sine are formed in f64 (a position of 10^5 leaves an f32
 // angle no fraction) and rounded to f32 once; the rotation's products are rounded one by one, so that a
 // rotated value does not depend on which of them the compiler would fuse.  A token's sines are formed once
-// for all of its heads: a workgroup takes a token.
+// for all of its heads: a workgroup takes a token.  What bounds rope_kernel: memory (32768 tokens of 32 heads of 128,
+// 1.07 GB in 242 us, 4.45 TB/s; 4093 of 14 heads 15.2 us against 12.4), the host's call for few (7.8 us).
 
 AH_DEV void rope_table(const RopeRef &r, int32_t pos, float *cs, float *sn) {
     for (uint32_t i = threadIdx.x; i < r.rot / 2; i += blockDim.x) {
@@ -262,8 +264,10 @@ AH_DEV bool block_codes(const float *v, uint32_t *c, float &d) {
 // One workgroup per token: cosines and sines once, then 8 channels a lane over q's heads, k's and v's; one
 // launch for the three.  k and v are rounded to the cache's four bits here, once.  What bounds it: memory
 // (4093 tokens, 12 heads of 128 and 2 KV heads, 60 MB in 15.1 us, 4.0 TB/s, the sines beside it), the launch
-// for few (8 tokens 4.3 us).  A token's codes are bytes of its own in a tile that 32 tokens share, so tokens
-// need no order.
+// for few (8 tokens 4.3 us).  Without q the stores: V's codes go out byte by byte, and of 8192 tokens of 2 KV heads
+// of 128 10.7 MB are written for 2.4 (12 us; 524288 tokens 496 us, 1.9 times a copy's time, and of heads of
+// 64, half a wave's lanes idle, 381 and 3 times).  A token's codes are bytes of its own in a tile that 32 tokens
+// share, so tokens need no order.
 __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
     __shared__ float cs[128], sn[128];
     const uint32_t tok = blockIdx.x, dim = a.c.dim, per = dim / 8, kv = a.c.n_kv;
@@ -312,7 +316,8 @@ __global__ void __launch_bounds__(256) kv4_append_kernel(AppendArgs a) {
     }
 }
 
-// The values of tokens, for whoever wants them outside the attention: 4093 tokens 5.0 us.
+// The values of tokens, for whoever wants them outside the attention: 4093 tokens 5.0 us, 524288 of 2 heads of 128 349 us,
+// 2.4 times a copy's time (V's codes are read byte by byte); generation does not call it.
 __global__ void __launch_bounds__(256) kv4_read_kernel(KvReadArgs a) {
     const uint32_t tok = blockIdx.x, dim = a.c.dim, per = dim / 8, kv = a.c.n_kv;
     uint32_t page = 0, in_page = 0;
