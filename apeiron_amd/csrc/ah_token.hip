@@ -19,10 +19,10 @@ AH_DEV double wave_sum(double v) {
 // s = x + r, R = 1 / sqrt(mean(s^2) + eps), y = (s R) gain, and quant_act of y's 32-blocks.  One
 // workgroup per token: a lane keeps 8 consecutive values of each of its U passes in registers, so the
 // row is read once and the quantizer's quads (four lanes a block, ah_units.h) hold whole blocks.  The
-// sum of squares is kept in f64: the f32 row's magnitude cannot overflow it, and whatever the order of the
-// sum R is the nearest f32 number, unless what it stands for lies within about 2^-45 of itself of the middle of
-// two.  y is rounded once to f32 by each of its two products, and
-// once more to seven bits by the quantizer, as the projections take it.
+// sum of squares is kept in f64, which the f32 row's magnitude cannot overflow, and R as two f32: y is
+// rounded to f32 once, to the nearest (but for values within about 2^-44 of themselves of the middle of two), and
+// once more to seven bits by the quantizer, as the projections take it.  Rounded three times (R and two
+// products), y put more codes on the other side of a half than the exact one's.
 //   What bounds it: memory (2039 tokens of 8957 with every output, 279 MB in 62.6 us: 4.45 TB/s, of 4.74
 // that a copy reaches); under a few hundred tokens the launch (512 of 1536 4.9 us, one of 896 2.6).  Rows
 // come through range-checked resources: with a branch for a row's last values the arrays of a lane left
@@ -62,6 +62,13 @@ AH_DEV void st8(__amdgpu_buffer_rsrc_t r, uint32_t k0, const float *v) {
     __builtin_amdgcn_raw_buffer_store_b128(b, r, (int)(4 * k0 + 16), 0, 0);
 }
 
+// (s (rh + rl)) g: the product by R with its own rounding's rest, then one rounding of both times g.
+AH_DEV float rounded_once(float s, float rh, float rl, float g) {
+#pragma clang fp contract(off)
+    const float t = s * rh, rest = __builtin_fmaf(s, rl, __builtin_fmaf(s, rh, -t));
+    return __builtin_fmaf(t, g, rest * g);
+}
+
 template <uint32_t U, bool RES>
 __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
     __shared__ double red[16];
@@ -93,14 +100,15 @@ __global__ void __launch_bounds__(1024) norm_quant_kernel(NormArgs a) {
     }
     // v_rsq_f64 is good to about 2^-28; a Newton step squares that
     const double mean = ss / (double)n + a.eps, r0 = __builtin_amdgcn_rsq(mean);
-    const float R = (float)(r0 * __builtin_fma(-0.5 * mean, r0 * r0, 1.5));
+    const double R = r0 * __builtin_fma(-0.5 * mean, r0 * r0, 1.5);
+    const float rh = (float)R, rl = (float)(R - (double)rh);
     const uint32_t nb = (n + 31) / 32;
 #pragma unroll
     for (uint32_t u = 0; u < U; ++u) {
         const uint32_t k0 = 8 * (u * T + tid), take = n > k0 ? (n - k0 < 8 ? n - k0 : 8) : 0;
         float y[8];
 #pragma unroll
-        for (uint32_t i = 0; i < 8; ++i) y[i] = (s[u][i] * R) * g[u][i];
+        for (uint32_t i = 0; i < 8; ++i) y[i] = rounded_once(s[u][i], rh, rl, g[u][i]);
         if (a.sum) st8(ah_rsrc(a.sum + row, 4 * n), k0, s[u]);
         if (a.y) st8(ah_rsrc(a.y + row, 4 * n), k0, y);
         if (!a.codes && !a.values) continue;
