@@ -21,8 +21,8 @@ AH_DEV double wave_sum(double v) {
 // row is read once and the quantizer's quads (four lanes a block, ah_units.h) hold whole blocks.  The
 // sum of squares is kept in f64, which the f32 row's magnitude cannot overflow, and R as two f32: y is
 // rounded to f32 once, to the nearest (but for values within about 2^-44 of themselves of the middle of two), and
-// once more to seven bits by the quantizer, as the projections take it.  Rounded three times (R and two
-// products), y put more codes on the other side of a half than the exact one's.
+// once more to seven bits by the quantizer, as the projections take it.  Codes that differ from the exact y's,
+// which f32 rounds to a half: 58 of 42 million, with R and both products rounded 68.
 //   What bounds it: memory (2039 tokens of 8957 with every output, 279 MB in 62.6 us: 4.45 TB/s, of 4.74
 // that a copy reaches); under a few hundred tokens the launch (512 of 1536 4.9 us, one of 896 2.6).  Rows
 // come through range-checked resources: with a branch for a row's last values the arrays of a lane left
