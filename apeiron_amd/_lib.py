@@ -33,7 +33,8 @@ EXPORTS = [
     "ah_ffn_prefill_q8_dev", "ah_dev_alloc", "ah_dev_free", "ah_copy_to_dev", "ah_copy_to_host", "ah_seq_set_spin_limit", "ah_ctx_scratch_bytes",
     "ah_seq_create", "ah_seq_run", "ah_seq_sync_status", "ah_seq_free", "ah_seq_info",
     "ah_norm_quant_dev", "ah_rope_create", "ah_rope_free", "ah_rope_info", "ah_rope_dev", "ah_kv4_create",
-    "ah_kv4_free", "ah_kv4_info", "ah_kv4_append_dev", "ah_kv4_read_dev", "ah_kv4_attn_dev", "ah_sample_dev",
+    "ah_kv4_free", "ah_kv4_info", "ah_kv4_append_dev", "ah_kv4_read_dev", "ah_kv4_attn_dev", "ah_kv4_attn_shared_dev", "ah_kv4_block_means_dev", "ah_kv4_attn_blocks_dev",
+    "ah_conv_dev", "ah_delta_rule_dev", "ah_sample_dev",
 ]
 
 _lib = None
@@ -68,6 +69,30 @@ class Kv4Attn(ctypes.Structure):
         ("d_q_start", ctypes.c_void_p), ("d_ctx", ctypes.c_void_p), ("d_table", ctypes.c_void_p),
         ("table_stride", ctypes.c_size_t), ("scale", ctypes.c_float), ("window", ctypes.c_size_t),
         ("sinks", ctypes.c_size_t)]
+
+
+class Kv4Blocks(ctypes.Structure):
+    """struct ah_kv4_blocks of include/apeiron_hip.h."""
+    _fields_ = [(n, ctypes.c_size_t) for n in ("block_len", "n_top", "n_first", "n_last")] + [("d_means", ctypes.c_void_p)]
+
+
+class StateSeqs(ctypes.Structure):
+    """struct ah_state_seqs of include/apeiron_hip.h."""
+    _fields_ = [(n, ctypes.c_size_t) for n in ("n_seq", "n_tok", "max_q", "n_slots")] + [
+        (n, ctypes.c_void_p) for n in ("d_q_start", "d_from", "d_to")]
+
+
+class Conv(ctypes.Structure):
+    """struct ah_conv of include/apeiron_hip.h."""
+    _fields_ = [("n_channels", ctypes.c_size_t), ("width", ctypes.c_size_t), ("d_weight", ctypes.c_void_p),
+                ("d_bias", ctypes.c_void_p), ("silu", ctypes.c_int32), ("d_state", ctypes.c_void_p)]
+
+
+class DeltaRule(ctypes.Structure):
+    """struct ah_delta_rule of include/apeiron_hip.h."""
+    _fields_ = [(n, ctypes.c_size_t) for n in ("n_heads", "n_k_heads", "k_dim", "v_dim")] + [
+        ("d_a_log", ctypes.c_void_p), ("d_dt_bias", ctypes.c_void_p), ("scale", ctypes.c_float), ("norm_eps", ctypes.c_float),
+        ("d_state", ctypes.c_void_p)]
 
 
 class SampleParams(ctypes.Structure):
@@ -151,6 +176,11 @@ def load() -> ctypes.CDLL:
         "ah_kv4_append_dev": (I32, [P, P, P, ctypes.POINTER(Kv4Tokens), P, S, S, P, S, P, S, P, S, P]),
         "ah_kv4_read_dev": (I32, [P, P, ctypes.POINTER(Kv4Tokens), P, P, P]),
         "ah_kv4_attn_dev": (I32, [P, P, ctypes.POINTER(Kv4Attn), P, S, P, S, P]),
+        "ah_kv4_attn_shared_dev": (I32, [P, P, ctypes.POINTER(Kv4Attn), S, P, P, S, P, S, P]),
+        "ah_kv4_block_means_dev": (I32, [P, P, ctypes.POINTER(Kv4Tokens), S, P, P]),
+        "ah_kv4_attn_blocks_dev": (I32, [P, P, ctypes.POINTER(Kv4Attn), ctypes.POINTER(Kv4Blocks), P, S, P, S, P, P]),
+        "ah_conv_dev": (I32, [P, ctypes.POINTER(StateSeqs), ctypes.POINTER(Conv), P, S, P, S, P]),
+        "ah_delta_rule_dev": (I32, [P, ctypes.POINTER(StateSeqs), ctypes.POINTER(DeltaRule)] + [P, S] * 6 + [P]),
         "ah_sample_dev": (I32, [P, P, S, S, S, ctypes.POINTER(SampleParams), P, P, P, P]),
     }
     for name, (res, args) in sig.items():

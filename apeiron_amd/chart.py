@@ -443,6 +443,36 @@ class KvCache4:
         _check(self.dev.lib.ah_kv4_attn_dev(self.dev.h, self.h, ctypes.byref(a), q_ptr, row if q_stride is None else q_stride, out_ptr,
                                             row if out_stride is None else out_stride, stream), "kv4_attn")
 
+    def attn_shared_dev(self, q_ptr: int, out_ptr: int, *, prefix_len: int, prefix_table_ptr: int | None, n_heads: int, n_tok: int, n_seq: int,
+                        q_start_ptr: int, ctx_ptr: int, table_ptr: int, table_stride: int, max_q: int, max_ctx: int, scale: float,
+                        q_stride: int | None = None, out_stride: int | None = None, stream: int | None = None) -> None:
+        """attn_dev for sequences that begin with the same prefix_len positions, in the pages of prefix_table (ah_kv4_attn_shared_dev)."""
+        a = _lib.Kv4Attn(n_seq, n_tok, n_heads, max_q, max_ctx, q_start_ptr, ctx_ptr, table_ptr, table_stride, scale, 0, 0)
+        row = n_heads * self.head_dim
+        _check(self.dev.lib.ah_kv4_attn_shared_dev(self.dev.h, self.h, ctypes.byref(a), prefix_len, prefix_table_ptr, q_ptr,
+                                                   row if q_stride is None else q_stride, out_ptr, row if out_stride is None else out_stride,
+                                                   stream), "kv4_attn_shared")
+
+    def block_means_dev(self, means_ptr: int, *, block_len: int, seq_ptr: int, pos_ptr: int, n_tok: int, table_ptr: int, n_seq: int,
+                        table_stride: int, stream: int | None = None) -> None:
+        """The means of the keys of the blocks that the tokens end (ah_kv4_block_means_dev), into f16
+        [n_pages][page_len / block_len][n_kv_heads][head_dim]."""
+        t = _lib.Kv4Tokens(seq_ptr, pos_ptr, n_tok, table_ptr, n_seq, table_stride)
+        _check(self.dev.lib.ah_kv4_block_means_dev(self.dev.h, self.h, ctypes.byref(t), block_len, means_ptr, stream), "kv4_block_means")
+
+    def attn_blocks_dev(self, q_ptr: int, out_ptr: int, *, means_ptr: int, block_len: int, n_top: int, n_first: int = 0, n_last: int = 0,
+                        n_heads: int, n_tok: int, n_seq: int, q_start_ptr: int, ctx_ptr: int, table_ptr: int, table_stride: int, max_q: int,
+                        max_ctx: int, scale: float, chosen_ptr: int | None = None, q_stride: int | None = None,
+                        out_stride: int | None = None, stream: int | None = None) -> None:
+        """Attention over the first blocks, the last ones, the query's own and the n_top whose means it scores highest
+        (ah_kv4_attn_blocks_dev)."""
+        a = _lib.Kv4Attn(n_seq, n_tok, n_heads, max_q, max_ctx, q_start_ptr, ctx_ptr, table_ptr, table_stride, scale, 0, 0)
+        b = _lib.Kv4Blocks(block_len, n_top, n_first, n_last, means_ptr)
+        row = n_heads * self.head_dim
+        _check(self.dev.lib.ah_kv4_attn_blocks_dev(self.dev.h, self.h, ctypes.byref(a), ctypes.byref(b), q_ptr,
+                                                   row if q_stride is None else q_stride, out_ptr, row if out_stride is None else out_stride,
+                                                   chosen_ptr, stream), "kv4_attn_blocks")
+
     def free(self) -> None:
         if self.h:
             self.dev.lib.ah_kv4_free(self.dev.h, self.h)
@@ -454,6 +484,32 @@ class KvCache4:
                 self.free()
         except Exception:
             pass
+
+
+def conv_dev(dev: "Device", x_ptr: int, y_ptr: int, *, n_channels: int, width: int, weight_ptr: int, state_ptr: int, n_seq: int, n_tok: int,
+             max_q: int, n_slots: int, q_start_ptr: int, from_ptr: int, to_ptr: int, bias_ptr: int | None = None, silu: bool = False,
+             x_stride: int | None = None, y_stride: int | None = None, stream: int | None = None) -> None:
+    """The short causal convolution of a recurrent layer's channels (ah_conv_dev); the inputs before the call's are read from and
+    left in slots of state [n_slots][width - 1][n_channels]."""
+    s = _lib.StateSeqs(n_seq, n_tok, max_q, n_slots, q_start_ptr, from_ptr, to_ptr)
+    c = _lib.Conv(n_channels, width, weight_ptr, bias_ptr, int(silu), state_ptr)
+    _check(dev.lib.ah_conv_dev(dev.h, ctypes.byref(s), ctypes.byref(c), x_ptr, n_channels if x_stride is None else x_stride, y_ptr,
+                               n_channels if y_stride is None else y_stride, stream), "conv")
+
+
+def delta_rule_dev(dev: "Device", q_ptr: int, k_ptr: int, v_ptr: int, a_ptr: int, b_ptr: int, out_ptr: int, *, n_heads: int, n_k_heads: int,
+                   k_dim: int, v_dim: int, scale: float, state_ptr: int, n_seq: int, n_tok: int, max_q: int, n_slots: int, q_start_ptr: int,
+                   from_ptr: int, to_ptr: int, a_log_ptr: int | None = None, dt_bias_ptr: int | None = None, norm_eps: float = -1.0,
+                   q_stride: int | None = None, k_stride: int | None = None, v_stride: int | None = None, a_stride: int | None = None,
+                   b_stride: int | None = None, out_stride: int | None = None, stream: int | None = None) -> None:
+    """The gated delta rule (ah_delta_rule_dev), from and to slots of state [n_slots][n_heads][k_dim][v_dim]."""
+    s = _lib.StateSeqs(n_seq, n_tok, max_q, n_slots, q_start_ptr, from_ptr, to_ptr)
+    d = _lib.DeltaRule(n_heads, n_k_heads, k_dim, v_dim, a_log_ptr, dt_bias_ptr, scale, norm_eps, state_ptr)
+    key, value = n_k_heads * k_dim, n_heads * v_dim
+    _check(dev.lib.ah_delta_rule_dev(dev.h, ctypes.byref(s), ctypes.byref(d), q_ptr, key if q_stride is None else q_stride, k_ptr,
+                                     key if k_stride is None else k_stride, v_ptr, value if v_stride is None else v_stride, a_ptr,
+                                     n_heads if a_stride is None else a_stride, b_ptr, n_heads if b_stride is None else b_stride, out_ptr,
+                                     value if out_stride is None else out_stride, stream), "delta_rule")
 
 
 def sample_dev(dev: "Device", logits_ptr: int, n_rows: int, n_vocab: int, u_ptr: int, tokens_ptr: int, *, row_stride: int | None = None,

@@ -1,0 +1,95 @@
+// ah_abi_state.cpp -- host side of a recurrent layer's operators: argument checks and the launches' shapes.
+#include "ah_host.h"
+#include "ah_state.h"
+
+namespace {
+
+constexpr size_t kMaxU32 = 0x7fffffff, kMaxGrid = 0xffffffffu / 256;  // (workgroups of 256 threads: under 2^32 threads)
+
+// The sequences of a call; false where they are refused.
+bool seqs_of(const ah_state_seqs *p, StateSeqs &s) {
+    if (!p->d_q_start || !p->d_from || !p->d_to || p->n_seq > 65535 || p->n_tok > kMaxU32 || p->n_slots > kMaxU32) return false;
+    s = {p->d_q_start, p->d_from, p->d_to, (uint32_t)p->n_seq, (uint32_t)p->n_tok, (uint32_t)(p->max_q < p->n_tok ? p->max_q : p->n_tok), (uint32_t)p->n_slots};
+    return true;
+}
+
+} // namespace
+
+extern "C" {
+
+int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *p, const float *d_x, size_t x_stride, float *d_y, size_t y_stride,
+                    void *stream) {
+    if (!ctx || !seqs || !p || p->width < 2 || p->width > kConvMaxWidth || p->n_channels > ((size_t)1 << 20)) return AH_ERR_INVALID_ARG;
+    if (seqs->n_seq == 0 || p->n_channels == 0) return AH_OK;
+    ConvArgs a = {};
+    if (!seqs_of(seqs, a.s) || !p->d_weight || !p->d_state) return AH_ERR_INVALID_ARG;
+    const size_t C = p->n_channels, n_tok = a.s.n_tok;
+    if (n_tok && (!d_x || !d_y || x_stride < C || y_stride < C || overlap(d_x, x_stride, C, d_y, y_stride, C, n_tok))) return AH_ERR_INVALID_ARG;
+    a.x = d_x;
+    a.y = d_y;
+    a.x_stride = x_stride;
+    a.y_stride = y_stride;
+    a.weight = p->d_weight;
+    a.bias = p->d_bias;
+    a.state = p->d_state;
+    a.n_ch = (uint32_t)C;
+    a.width = (uint32_t)p->width;
+    a.silu = p->silu != 0;
+    a.status = ctx->d_status;
+    const size_t blocks = (C + 1023) / 1024, max_q = a.s.max_q ? a.s.max_q : 1;
+    a.tile = 32;
+    const bool even = n_tok == (size_t)a.s.n_seq * a.s.max_q || a.s.n_seq == 1;
+    a.per = even ? (uint32_t)((max_q + a.tile - 1) / a.tile) : 0;
+    const size_t tiles = even ? (size_t)a.per * a.s.n_seq : n_tok / a.tile + a.s.n_seq;
+    if (tiles > kMaxGrid / blocks) return AH_ERR_INVALID_ARG;
+    a.tiles = (uint32_t)tiles;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_conv(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta_rule *p, const float *d_q, size_t q_stride, const float *d_k,
+                          size_t k_stride, const float *d_v, size_t v_stride, const float *d_a, size_t a_stride, const float *d_b, size_t b_stride,
+                          float *d_out, size_t out_stride, void *stream) {
+    if (!ctx || !seqs || !p) return AH_ERR_INVALID_ARG;
+    const size_t H = p->n_heads, K = p->n_k_heads, dk = p->k_dim, dv = p->v_dim;
+    if ((dk != 64 && dk != 128) || (dv != 64 && dv != 128 && dv != 256) || H > 4096 || K == 0 || H % K || (p->d_a_log == nullptr) != (p->d_dt_bias == nullptr))
+        return AH_ERR_INVALID_ARG;
+    if (seqs->n_seq == 0 || H == 0) return AH_OK;
+    DeltaArgs a = {};
+    if (!seqs_of(seqs, a.s) || !p->d_state) return AH_ERR_INVALID_ARG;
+    const size_t n = a.s.n_tok;
+    if (n && (!d_q || !d_k || !d_v || !d_a || !d_b || !d_out || q_stride < K * dk || k_stride < K * dk || v_stride < H * dv || a_stride < H || b_stride < H ||
+              out_stride < H * dv || overlap(d_q, q_stride, K * dk, d_out, out_stride, H * dv, n) || overlap(d_k, k_stride, K * dk, d_out, out_stride, H * dv, n) ||
+              overlap(d_v, v_stride, H * dv, d_out, out_stride, H * dv, n) || overlap(d_a, a_stride, H, d_out, out_stride, H * dv, n) ||
+              overlap(d_b, b_stride, H, d_out, out_stride, H * dv, n)))
+        return AH_ERR_INVALID_ARG;
+    if ((size_t)a.s.n_seq * H * (dv / 32) > kMaxU32) return AH_ERR_INVALID_ARG;
+    a.q = d_q;
+    a.k = d_k;
+    a.v = d_v;
+    a.a = d_a;
+    a.b = d_b;
+    a.a_log = p->d_a_log;
+    a.dt_bias = p->d_dt_bias;
+    a.out = d_out;
+    a.state = p->d_state;
+    a.q_stride = q_stride;
+    a.k_stride = k_stride;
+    a.v_stride = v_stride;
+    a.a_stride = a_stride;
+    a.b_stride = b_stride;
+    a.out_stride = out_stride;
+    a.n_heads = (uint32_t)H;
+    a.group = (uint32_t)(H / K);
+    a.k_dim = (uint32_t)dk;
+    a.v_dim = (uint32_t)dv;
+    a.scale = p->scale;
+    a.norm_eps = p->norm_eps;
+    a.status = ctx->d_status;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_delta(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+} // extern "C"

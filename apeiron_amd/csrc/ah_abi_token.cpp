@@ -32,14 +32,14 @@ size_t most_tiles(const AttnArgs &a, size_t max_ctx, size_t max_q) {
     return tiles < seen ? tiles : seen;
 }
 
-// Room for the partial results of `rows` rows in each of a.splits pieces.
-int32_t attn_scratch(ah_ctx *ctx, AttnArgs &a, size_t rows, void *stream) {
-    if (a.splits == 1) return AH_OK;
+// Room for the partial results of `rows` rows in each of a.splits pieces, behind `kept` bytes of the scratch.
+int32_t attn_scratch(ah_ctx *ctx, AttnArgs &a, size_t rows, size_t kept, void *stream) {
+    if (a.splits == 1 && kept == 0) return AH_OK;
     const size_t o = align256(a.splits * rows * a.c.dim * sizeof(float));
-    const int32_t st = ensure_scratch(ctx, o + a.splits * rows * 2 * sizeof(float), stream);
+    const int32_t st = ensure_scratch(ctx, kept + (a.splits > 1 ? o + a.splits * rows * 2 * sizeof(float) : 0), stream);
     if (st) return st;
-    a.part_o = static_cast<float *>(ctx->scratch.p);
-    a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch.p) + o);
+    a.part_o = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch.p) + kept);
+    a.part_ml = reinterpret_cast<float *>(static_cast<uint8_t *>(ctx->scratch.p) + kept + o);
     a.count = ctx->d_count;
     return AH_OK;
 }
@@ -48,8 +48,8 @@ size_t most_pieces(const AttnArgs &a, size_t rows) {
     const size_t n = ((size_t)256 << 20) / (rows * (a.c.dim + 2) * sizeof(float));
     return n < 1 ? 1 : n;
 }
-// Pieces of `chunk` tiles each.
-int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t chunk, void *stream) {
+// Pieces of `chunk` tiles each, and the scratch that they take behind `kept` bytes.
+int32_t attn_pieces(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t chunk, size_t kept, void *stream) {
     chunk = chunk < 1 ? 1 : chunk;
     a.chunk = (uint32_t)chunk;
     a.splits = (uint32_t)((tiles + chunk - 1) / chunk);
@@ -59,18 +59,20 @@ int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t
     if (units > max_grid(256) / a.splits) return AH_ERR_INVALID_ARG;
     a.grid = (uint32_t)(units * a.splits);
     AH_HIP(ctx, hipSetDevice(ctx->device));
-    const int32_t st = attn_scratch(ctx, a, (size_t)a.n_tok * a.n_heads, stream);
+    return attn_scratch(ctx, a, (size_t)a.n_tok * a.n_heads, kept, stream);
+}
+int32_t attn_launch(ah_ctx *ctx, AttnArgs &a, size_t units, size_t tiles, size_t chunk, void *stream) {
+    const int32_t st = attn_pieces(ctx, a, units, tiles, chunk, 0, stream);
     if (st) return st;
     AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
     return AH_OK;
 }
 
-// Sequences of at most `most` rows, by workgroups of 8 or 16.
-int32_t attn_rows(ah_ctx *ctx, AttnArgs a, size_t max_ctx, size_t most, void *stream) {
+// Sequences of at most `most` rows over at most `tiles` tiles, by workgroups of 8 or 16: their pieces.
+int32_t attn_rows_plan(ah_ctx *ctx, AttnArgs &a, size_t tiles, size_t most, size_t kept, void *stream) {
     a.rows = most <= 8 ? 8 : 16;
     a.most_rows = (uint32_t)most;
     const size_t per = (most + a.rows - 1) / a.rows, base = per * a.c.n_kv * a.n_seq, rows = (size_t)a.n_tok * a.n_heads;
-    const size_t tiles = most_tiles(a, max_ctx, most / a.group);
     // With few units a piece's tiles (0.7 us for each of a wave) stand against the join (0.1 us a piece):
     // sqrt(1.75 tiles) pieces, past 40 of them two joins and 16 tiles a piece.  One sequence of 4001 keys in pieces
     // of 4, 8, 16 and 24 tiles: 10.6, 10.0, 10.7 and 13.3 us.  Once that passes a workgroup a CU (two, where two
@@ -88,7 +90,13 @@ int32_t attn_rows(ah_ctx *ctx, AttnArgs a, size_t max_ctx, size_t most, void *st
     size_t fit = base <= kAttnGroups / 2 ? kAttnGroups / base : 1;
     fit = fit < most_pieces(a, rows) ? fit : most_pieces(a, rows);
     chunk = chunk < (tiles + fit - 1) / fit ? (tiles + fit - 1) / fit : chunk;
-    return attn_launch(ctx, a, base, tiles, chunk, stream);
+    return attn_pieces(ctx, a, base, tiles, chunk, kept, stream);
+}
+int32_t attn_rows(ah_ctx *ctx, AttnArgs a, size_t max_ctx, size_t most, void *stream) {
+    const int32_t st = attn_rows_plan(ctx, a, most_tiles(a, max_ctx, most / a.group), most, 0, stream);
+    if (st) return st;
+    AH_HIP(ctx, ah_launch_attn(a, pick(ctx, stream)));
+    return AH_OK;
 }
 
 // Sequences of at least a.least_rows rows, by workgroups of 128.
@@ -149,6 +157,37 @@ int32_t attn_tiles(ah_ctx *ctx, AttnArgs a, size_t max_ctx, void *stream) {
     }
     return attn_launch(ctx, a, units * a.c.n_kv, tiles, (tiles + splits - 1) / splits, stream);
 }
+
+// The checks that every form of attention makes, and its arguments.
+int32_t attn_args(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, const float *d_q, size_t q_stride, float *d_out,
+                  size_t out_stride, AttnArgs &a) {
+    const size_t dim = cache->ref.dim, kv = cache->ref.n_kv;
+    if (!p->d_q_start || !p->d_ctx || !p->d_table || !d_q || !d_out || p->n_seq > 65535 || p->n_tok > kMaxU32 ||
+        p->n_heads > 65536 || p->n_heads % kv || p->table_stride == 0 || p->table_stride > kMaxU32 || q_stride < p->n_heads * dim ||
+        out_stride < p->n_heads * dim || p->window > kMaxU32 || p->sinks > kMaxU32)
+        return AH_ERR_INVALID_ARG;
+    a = {};
+    a.c = cache->ref;
+    a.q_start = p->d_q_start;
+    a.ctx = p->d_ctx;
+    a.table = p->d_table;
+    a.q = d_q;
+    a.out = d_out;
+    a.q_stride = q_stride;
+    a.out_stride = out_stride;
+    a.n_seq = (uint32_t)p->n_seq;
+    a.n_tok = (uint32_t)p->n_tok;
+    a.n_heads = (uint32_t)p->n_heads;
+    a.group = (uint32_t)(p->n_heads / kv);
+    a.max_q = (uint32_t)(p->max_q < p->n_tok ? p->max_q : p->n_tok);
+    a.table_stride = (uint32_t)p->table_stride;
+    a.window = (uint32_t)p->window;
+    a.sinks = (uint32_t)p->sinks;
+    a.scale = p->scale;
+    a.status = ctx->d_status;
+    return (size_t)a.max_q * a.group > kMaxU32 / 256 ? AH_ERR_INVALID_ARG : AH_OK;
+}
+bool empty(const ah_kv4_attn *p) { return p->n_seq == 0 || p->n_tok == 0 || p->n_heads == 0 || p->max_q == 0; }
 
 } // namespace
 
@@ -346,31 +385,11 @@ int32_t ah_kv4_read_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *t
 int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, const float *d_q, size_t q_stride, float *d_out,
                         size_t out_stride, void *stream) {
     if (!ctx || !cache || !p) return AH_ERR_INVALID_ARG;
-    if (p->n_seq == 0 || p->n_tok == 0 || p->n_heads == 0 || p->max_q == 0) return AH_OK;
-    const size_t dim = cache->ref.dim, kv = cache->ref.n_kv;
-    if (!p->d_q_start || !p->d_ctx || !p->d_table || !d_q || !d_out || p->n_seq > 65535 || p->n_tok > kMaxU32 ||
-        p->n_heads > 65536 || p->n_heads % kv || p->table_stride == 0 || p->table_stride > kMaxU32 || q_stride < p->n_heads * dim ||
-        out_stride < p->n_heads * dim || p->window > kMaxU32 || p->sinks > kMaxU32)
-        return AH_ERR_INVALID_ARG;
-    AttnArgs a = {};
-    a.c = cache->ref;
-    a.q_start = p->d_q_start;
-    a.ctx = p->d_ctx;
-    a.table = p->d_table;
-    a.q = d_q;
-    a.out = d_out;
-    a.q_stride = q_stride;
-    a.out_stride = out_stride;
-    a.n_seq = (uint32_t)p->n_seq;
-    a.n_tok = (uint32_t)p->n_tok;
-    a.n_heads = (uint32_t)p->n_heads;
-    a.group = (uint32_t)(p->n_heads / kv);
-    a.max_q = (uint32_t)(p->max_q < p->n_tok ? p->max_q : p->n_tok);
-    a.table_stride = (uint32_t)p->table_stride;
-    a.window = (uint32_t)p->window;
-    a.sinks = (uint32_t)p->sinks;
-    a.scale = p->scale;
-    a.status = ctx->d_status;
+    if (empty(p)) return AH_OK;
+    AttnArgs a;
+    const int32_t bad = attn_args(ctx, cache, p, d_q, q_stride, d_out, out_stride, a);
+    if (bad) return bad;
+    const size_t kv = a.c.n_kv;
     // The kernel: 8 packed rows or 16 rows a workgroup, or 128 over tiles in LDS.  Those start later and need many rows
     // of a sequence (they convert the cache's codes once for all of them, the others once for 16).  2 KV heads, rows a
     // sequence and sequences: 56 and 64 of 1000 keys, heads of 64, 128 and 256, 15, 22 and 37 us by 16 rows against 24,
@@ -378,7 +397,6 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
     // units of 16 rows) 47 against 50, 120 and 16 (1024) 72 against 59; one of 512 rows of 2 KV heads (64 units) 24
     // against 23.
     const size_t unit_rows = (size_t)a.max_q * a.group, units = (unit_rows + 15) / 16 * kv * p->n_seq;
-    if (unit_rows > kMaxU32 / 256) return AH_ERR_INVALID_ARG;
     if (unit_rows <= 64 || (unit_rows <= 128 && units <= 640) || units <= 64) return attn_rows(ctx, a, p->max_ctx, unit_rows, stream);
     // A few long chunks among single tokens (the others' mean is a part of 128 rows): the two kinds by a launch each.
     const size_t few = a.group <= 8 ? 8 : 32, others = a.n_tok > a.max_q ? a.n_tok - a.max_q : 0;
@@ -388,6 +406,119 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, 
         a.least_rows = (uint32_t)few + 1;
     }
     return attn_tiles(ctx, a, p->max_ctx, stream);
+}
+
+int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, size_t prefix_len, const int32_t *d_prefix_table,
+                               const float *d_q, size_t q_stride, float *d_out, size_t out_stride, void *stream) {
+    if (!ctx || !cache || !p || p->window || p->sinks || prefix_len > kMaxU32) return AH_ERR_INVALID_ARG;
+    if (prefix_len == 0) return ah_kv4_attn_dev(ctx, cache, p, d_q, q_stride, d_out, out_stride, stream);
+    if (empty(p)) return AH_OK;
+    AttnArgs a;
+    const int32_t bad = attn_args(ctx, cache, p, d_q, q_stride, d_out, out_stride, a);
+    if (bad) return bad;
+    const size_t rows = (size_t)a.n_tok * a.n_heads, batch = (size_t)a.n_tok * a.group;
+    if (!d_prefix_table || batch > kMaxU32 / 256 || rows * a.c.dim > ((size_t)1 << 30) - 1 ||
+        overlap(d_q, q_stride, a.n_heads * a.c.dim, d_out, out_stride, a.n_heads * a.c.dim, a.n_tok))
+        return AH_ERR_INVALID_ARG;
+    a.first_key = (uint32_t)prefix_len;
+    AttnArgs pre = a, own = a;
+    const size_t kv = a.c.n_kv, cus = (size_t)ctx->cu_count, most = most_pieces(a, rows);
+    // n pieces of `tiles` tiles for `units` workgroups: as many as fill `places`, at least `least` tiles each.
+    auto cut = [&](AttnArgs &x, size_t units, size_t tiles, size_t places, size_t least) {
+        size_t n = places / units, fit = (tiles + least - 1) / least;
+        n = n < fit ? n : fit;
+        n = n < most / 2 ? n : most / 2;
+        n = n < 1 ? 1 : n;
+        const size_t chunk = tiles ? (tiles + n - 1) / n : 1;
+        x.chunk = (uint32_t)chunk;
+        x.splits = (uint32_t)(tiles ? (tiles + chunk - 1) / chunk : 1);
+        x.grid = (uint32_t)(units * x.splits);
+        return units <= max_grid(256) / x.splits;
+    };
+    // The prefix: the whole batch as one sequence.
+    pre.n_seq = 1;
+    pre.table = d_prefix_table;
+    pre.table_stride = (uint32_t)((prefix_len - 1) >> a.c.page_shift) + 1;
+    pre.rows = batch <= 8 ? 8 : batch <= 128 ? 16 : 128;
+    const size_t held = a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1, units = (batch + pre.rows - 1) / pre.rows;
+    pre.per = (uint32_t)units;
+    if (!cut(pre, units * kv, (prefix_len + 31) / 32, pre.rows == 128 ? held * cus : 2 * cus, 4)) return AH_ERR_INVALID_ARG;
+    // What follows it: each sequence for itself.
+    const size_t per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
+    const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
+    own.rows = per_seq <= 8 ? 8 : 16;
+    size_t own_units = (per_seq + own.rows - 1) / own.rows * kv * a.n_seq;
+    if (per_seq > 128 && tiles > 64) {
+        own.rows = 128;
+        own.per = (size_t)a.n_tok == (size_t)a.n_seq * a.max_q || a.n_seq == 1 ? (uint32_t)((per_seq + 127) / 128) : 0;
+        own_units = (own.per ? (size_t)own.per * a.n_seq : ((size_t)a.n_tok * a.group >> 7) + a.n_seq) * kv;
+    }
+    if (!cut(own, own_units, tiles, 2 * cus, 4)) return AH_ERR_INVALID_ARG;
+    a.splits = pre.splits + own.splits;
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    const int32_t st = attn_scratch(ctx, a, rows, 0, stream);
+    if (st) return st;
+    pre.part_o = a.part_o;
+    pre.part_ml = a.part_ml;
+    own.part_o = a.part_o + (size_t)pre.splits * rows * a.c.dim;
+    own.part_ml = a.part_ml + (size_t)pre.splits * rows * 2;
+    AH_HIP(ctx, ah_launch_attn_shared(pre, own, a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+// Block sizes that the pages are cut into.
+static bool block_ok(const ah_kv4 *cache, size_t len) {
+    return len >= 32 && !(len & (len - 1)) && len <= (size_t)1 << cache->ref.page_shift;
+}
+
+int32_t ah_kv4_block_means_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *tokens, size_t block_len, uint16_t *d_means, void *stream) {
+    if (!ctx || !cache || !tokens || !block_ok(cache, block_len)) return AH_ERR_INVALID_ARG;
+    if (tokens->n_tok == 0) return AH_OK;
+    if (!tokens_ok(tokens) || !d_means || (reinterpret_cast<uintptr_t>(d_means) & 15) || tokens->n_tok > max_grid(256)) return AH_ERR_INVALID_ARG;
+    MeansArgs a = {cache->ref, tokens_of(tokens), (uint32_t)__builtin_ctzll(block_len), d_means, ctx->d_status};
+    AH_HIP(ctx, hipSetDevice(ctx->device));
+    AH_HIP(ctx, ah_launch_block_means(a, pick(ctx, stream)));
+    return AH_OK;
+}
+
+int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *p, const ah_kv4_blocks *blocks, const float *d_q,
+                               size_t q_stride, float *d_out, size_t out_stride, int32_t *d_chosen, void *stream) {
+    if (!ctx || !cache || !p || !blocks || p->window || p->sinks || !block_ok(cache, blocks->block_len) || blocks->n_top == 0 ||
+        blocks->n_top > 4096 || blocks->n_first > 4096 || blocks->n_last > 4096)
+        return AH_ERR_INVALID_ARG;
+    if (empty(p)) return AH_OK;
+    BlockArgs b = {};
+    const int32_t bad = attn_args(ctx, cache, p, d_q, q_stride, d_out, out_stride, b.a);
+    if (bad) return bad;
+    AttnArgs &a = b.a;
+    const size_t units = (size_t)a.n_tok * a.c.n_kv, per_page = ((size_t)1 << a.c.page_shift) / blocks->block_len;
+    if (!blocks->d_means || (reinterpret_cast<uintptr_t>(blocks->d_means) & 15) || units > max_grid(256) || a.group > 4096 ||
+        overlap(d_q, q_stride, a.n_heads * a.c.dim, d_out, out_stride, a.n_heads * a.c.dim, a.n_tok))
+        return AH_ERR_INVALID_ARG;
+    b.means = blocks->d_means;
+    b.shift = (uint32_t)__builtin_ctzll(blocks->block_len);
+    b.top = (uint32_t)blocks->n_top;
+    b.first = (uint32_t)blocks->n_first;
+    b.last = (uint32_t)blocks->n_last;
+    b.chosen = d_chosen;
+    // Lists, then scores that do not fit a workgroup's LDS, then the attention's partial results.
+    const size_t places = a.table_stride * per_page, all = places < kMaxU32 / 32 ? places : kMaxU32 / 32, read = b.top + (size_t)b.first + b.last + 1, entries = read < all ? read : all;
+    a.list_stride = (uint32_t)entries + 1;
+    a.block_shift = b.shift - 5;
+    b.most = (uint32_t)all;
+    b.lds_keys = (uint32_t)(all < kLdsKeys ? all : kLdsKeys);
+    const size_t keys_at = align256(units * a.list_stride * sizeof(uint32_t)), kept = keys_at + (all > kLdsKeys ? align256(units * all * sizeof(uint64_t)) : 0);
+    AttnArgs rows = a;
+    rows.n_seq = a.n_tok;  // every token for itself
+    rows.max_q = 1;
+    const int32_t st = attn_rows_plan(ctx, rows, entries << a.block_shift, a.group, kept, stream);
+    if (st) return st;
+    b.list = static_cast<uint32_t *>(ctx->scratch.p);
+    b.keys = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(ctx->scratch.p) + keys_at);
+    rows.list = b.list;
+    AH_HIP(ctx, ah_launch_block_choice(b, pick(ctx, stream)));
+    AH_HIP(ctx, ah_launch_attn_blocks(rows, pick(ctx, stream)));
+    return AH_OK;
 }
 
 int32_t ah_sample_dev(ah_ctx *ctx, const float *d_logits, size_t row_stride, size_t n_rows, size_t n_vocab,

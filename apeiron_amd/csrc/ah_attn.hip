@@ -7,7 +7,7 @@
 // two products summed in the f32 accumulator.  What is left are f32's roundings of scores, exponentials and
 // running sums: 4e-7 to 9e-7 of the outputs (root mean square against 64 bits, 4001 to 30000 keys), 7e-7 to
 // 2.1e-6 with plain f32 operations.
-#include "ah_kv4.h"
+#include "ah_attn.h"
 
 namespace {
 
@@ -66,53 +66,6 @@ AH_DEV void v_frags(uint32_t w0, uint32_t w1, f16x8 d, const Masks &k, f16x8 &ev
 
 AH_DEV float xor_lanes(float v, int mask) { return __shfl_xor(v, mask, 64); }
 
-// What a workgroup of a sequence works on.
-struct Span {
-    uint32_t q0, nq;      // its tokens
-    int32_t ctx;          // keys
-    bool bad;
-};
-AH_DEV Span span_of(const AttnArgs &a, uint32_t s) {
-    Span p;
-    const int32_t b = a.q_start[s], e = a.q_start[s + 1], c = a.ctx[s];
-    const uint64_t room = (uint64_t)a.table_stride << a.c.page_shift;
-    p.bad = b < 0 || e < b || (uint32_t)e > a.n_tok || (uint32_t)(e - b) > a.max_q || c < 0 || (uint64_t)c > room;
-    p.q0 = p.bad ? 0 : (uint32_t)b;
-    p.nq = p.bad ? 0 : (uint32_t)(e - b);
-    p.ctx = p.bad ? 0 : c;
-    return p;
-}
-
-// The last of n things, in the order of their starts, that starts at or before `at` (the first one if none does): the
-// wave's lanes look at 64 of them at a time.
-template <class F> AH_DEV uint32_t last_starting(uint32_t n, uint32_t at, F start) {
-    const uint32_t lane = threadIdx.x & 63;
-    uint32_t lo = 0;
-    while (n > 1) {
-        const uint32_t step = (n + 63) / 64, i = lane * step;
-        const uint32_t count = (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(i < n && start(lo + (i < n ? i : 0)) <= at));
-        const uint32_t skip = (count ? count - 1 : 0) * step;
-        lo += skip;
-        n = n - skip < step ? n - skip : step;
-    }
-    return lo;
-}
-
-// The sequence for which holds(i) is true (any, if there is none).  Where the entries of q_start in range ascend, sequence i
-// holds what lies between start(i) and start(i + 1).  One out of range leads the search astray: a find that the entries
-// beside it don't confirm is looked up among all sequences.
-template <class S, class H> AH_DEV uint32_t sequence_of(const AttnArgs &a, uint32_t at, S start, H holds) {
-    uint32_t s = last_starting(a.n_seq, at, start);
-    auto in_range = [&](uint32_t i) { return (uint32_t)a.q_start[i] <= a.n_tok; };
-    if (in_range(s) && in_range(s + 1) && (start(s) <= at ? s + 1 == a.n_seq || start(s + 1) > at : s == 0)) return s;
-    for (uint32_t base = 0; base < a.n_seq; base += 64) {
-        const uint32_t i = base + (threadIdx.x & 63);
-        const uint64_t b = __builtin_amdgcn_ballot_w64(i < a.n_seq && holds(i < a.n_seq ? i : 0));
-        if (b) s = base + 63 - (uint32_t)__builtin_clzll(b);
-    }
-    return s;
-}
-
 // The tiles that rows at positions lo .. hi see: [0, head) and [tail, end).
 struct Tiles {
     uint32_t head, tail, end, count;
@@ -132,6 +85,36 @@ AH_DEV Tiles tiles_of(const AttnArgs &a, int32_t lo, int32_t hi) {
     return t;
 }
 
+// What a launch reads of the contexts:
+//   kAll: the positions that a query sees, in its sequence's pages;
+//   kPrefix: every row the first first_key positions, in the pages of one table: the whole batch as one sequence;
+//   kAfter: as kAll, from position first_key on;
+//   kBlocks: every (token, KV head) the blocks that it has a list of, as if they stood one after the other.
+// kPrefix and kAfter leave their pieces for attn_meet_kernel, pieces of kAfter without a key with no weight.
+enum { kAll, kPrefix, kAfter, kBlocks };
+template <int MODE> AH_DEV Span span_in(const AttnArgs &a, uint32_t s, uint32_t kvh) {
+    if (MODE == kPrefix) return {0, a.n_tok, (int32_t)a.first_key, false};
+    if (MODE == kBlocks) {  // [0] of a list: its keys, kNoList where the token is no sequence's
+        const uint32_t keys = a.list[((size_t)s * a.c.n_kv + kvh) * a.list_stride];
+        return {s, keys == kNoList ? 0u : 1u, keys == kNoList ? 0 : (int32_t)keys, keys == kNoList};
+    }
+    Span p = span_of(a, s);
+    if (MODE == kAfter && !p.bad && (uint32_t)(p.ctx - (int32_t)p.nq) < a.first_key) p = {0, 0, 0, true};
+    return p;
+}
+template <int MODE> AH_DEV int32_t position_of(const Span &p, uint32_t tok) {  // of a span's token
+    return MODE == kPrefix ? p.ctx - 1 : p.ctx - (int32_t)p.nq + (int32_t)tok;
+}
+template <int MODE> AH_DEV Tiles tiles_in(const AttnArgs &a, int32_t lo, int32_t hi) {
+    if (MODE != kAfter) return tiles_of(a, lo, hi);
+    Tiles t;
+    t.end = hi < 0 ? 0 : ((uint32_t)hi >> 5) + 1;
+    t.head = 0;
+    t.tail = a.first_key >> 5;
+    t.count = t.end > t.tail ? t.end - t.tail : 0;
+    return t;
+}
+
 // Tiles of a piece: the planned chunk, or more where a context is longer than the caller's bound.
 AH_DEV uint32_t piece_of(const AttnArgs &a, const Tiles &t) {
     const uint32_t need = (t.count + a.splits - 1) / a.splits;
@@ -146,6 +129,14 @@ AH_DEV const uint8_t *tile_at(const AttnArgs &a, uint32_t s, uint32_t kvh, uint3
     const uint32_t page = (uint32_t)((cptr)(uintptr_t)a.table)[(size_t)s * a.table_stride + pi];
     ok = page < a.c.n_pages;
     return a.c.base + kv4_tile(a.c, ok ? page : 0, kvh, tile & ((1u << in) - 1));
+}
+
+template <int MODE> AH_DEV const uint8_t *tile_in(const AttnArgs &a, uint32_t s, uint32_t kvh, uint32_t tile, bool &ok) {
+    if (MODE != kBlocks) return tile_at(a, s, kvh, tile, ok);
+    typedef const uint32_t __attribute__((address_space(4))) *cptr;
+    const uint32_t at = ((cptr)(uintptr_t)a.list)[((size_t)s * a.c.n_kv + kvh) * a.list_stride + 1 + (tile >> a.block_shift)];
+    ok = at != kNoList;
+    return a.c.base + (uint64_t)((ok ? at : 0) + (tile & ((1u << a.block_shift) - 1))) * (36u * a.c.dim);
 }
 
 // One lane's part of a tile.
@@ -205,7 +196,7 @@ AH_DEV void q_scale(float scale, float top, float &up, float &f) {
 // page's index, a tile, the partial results' way to the last workgroup and back (4001 keys: 9.8 us).  A unit
 // over all keys in one workgroup, joined by nobody, costs 0.7 us a tile and wave; a second launch for the join
 // 5 us more; equal shares of all units' tiles for every workgroup (two units in one) up to 10.
-template <int D, bool PACK>
+template <int D, bool PACK, int MODE>
 __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_rows_kernel(AttnArgs a) {
     constexpr int NJ = D / 32;  // contraction steps of K q, and blocks of channels
     constexpr uint32_t R = PACK ? 8 : 16;
@@ -220,22 +211,22 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
     // round the XCDs
     const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units, unit = (blockIdx.x - split * units + split) % units;
     const uint32_t per = units / a.n_seq, s = unit / per, rest = unit - s * per, rt = rest / a.c.n_kv, kvh = rest - rt * a.c.n_kv;
-    const Span p = span_of(a, s);
-    if (p.bad && split == 0 && rest == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
+    const Span p = span_in<MODE>(a, s, kvh);
+    if (MODE != kBlocks && p.bad && split == 0 && rest == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
     const uint32_t rows = p.nq * a.group, row0 = rt * R;
-    if (row0 >= rows || rows > a.most_rows) return;
+    if (row0 >= rows || (MODE == kAll && rows > a.most_rows)) return;
     const uint32_t row = row0 + r % R, tok = row / a.group, hq = kvh * a.group + row % a.group;
     const bool live = row < rows, low = PACK && r >= 8;
-    const int32_t pos0 = p.ctx - (int32_t)p.nq;
     const uint32_t last = row0 + R - 1 < rows ? row0 + R - 1 : rows - 1;
-    const int32_t lo = pos0 + (int32_t)(row0 / a.group), hi = pos0 + (int32_t)(last / a.group);
-    const int32_t pos = live ? pos0 + (int32_t)tok : -1;
+    const int32_t lo = position_of<MODE>(p, row0 / a.group), hi = position_of<MODE>(p, last / a.group);
+    const int32_t pos = live ? position_of<MODE>(p, tok) : -1;
     // the keys below which the window hides one (for this row, and for the last of the rows), and the sinks
-    const int32_t low_key = a.window ? pos - (int32_t)a.window + 1 : 0, low_all = a.window ? hi - (int32_t)a.window + 1 : 0;
+    const int32_t low_key = MODE == kAfter ? (int32_t)a.first_key : a.window ? pos - (int32_t)a.window + 1 : 0;
+    const int32_t low_all = MODE == kAfter ? (int32_t)a.first_key : a.window ? hi - (int32_t)a.window + 1 : 0;
     const int32_t sink_key = (int32_t)a.sinks;
-    const Tiles T = tiles_of(a, lo, hi);
+    const Tiles T = tiles_in<MODE>(a, lo, hi);
     const uint32_t chunk = piece_of(a, T), t0 = split * chunk, t1 = t0 + chunk < T.count ? t0 + chunk : T.count;
-    if (split > 0 && t0 >= T.count) return;
+    if (MODE != kAfter && split > 0 && t0 >= T.count) return;
 
     // the first tile's loads go out before q is prepared
     KTile<D> k;
@@ -244,7 +235,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
     uint32_t ti = t0 + wave;
     auto tile_of = [&](uint32_t i) { return i < T.head ? i : T.tail + (i - T.head); };
     if (ti < t1) {
-        const uint8_t *t = tile_at(a, s, kvh, tile_of(ti), ok);
+        const uint8_t *t = tile_in<MODE>(a, s, kvh, tile_of(ti), ok);
         k.load(t, r, h);
         v.load(t, r, h);
     }
@@ -288,7 +279,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
     for (; ti < t1; ti += 4) {
         const uint32_t tile = tile_of(ti), next = ti + 4 < t1 ? ti + 4 : ti;
         bool ok_next;
-        const uint8_t *tn = tile_at(a, s, kvh, tile_of(next), ok_next);
+        const uint8_t *tn = tile_in<MODE>(a, s, kvh, tile_of(next), ok_next);
         f32x4 c[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -385,7 +376,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
         if (!low) __builtin_memcpy(red_o + (wave * 16 + r) * (D + 4) + 32 * g + 8 * h, o, 32);
     }
     __syncthreads();
-    const uint32_t pieces = T.count ? (T.count + chunk - 1) / chunk : 1;
+    const uint32_t pieces = MODE == kPrefix || MODE == kAfter ? 2 : T.count ? (T.count + chunk - 1) / chunk : 1;  // (2: a part of what a launch after this joins)
     const size_t all = (size_t)a.n_tok * a.n_heads;
     auto flat_of = [&](uint32_t rw) { return (size_t)(p.q0 + rw / a.group) * a.n_heads + kvh * a.group + rw % a.group; };
     auto out_of = [&](uint32_t rw) { return a.out + (size_t)(p.q0 + rw / a.group) * a.out_stride + (size_t)(kvh * a.group + rw % a.group) * D; };
@@ -420,7 +411,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
                 __builtin_amdgcn_raw_buffer_store_b64(__builtin_bit_cast(u32x2, (f32x2){M, L}), pm, (int)(8 * at), 0, kDevice);
         }
     }
-    if (pieces == 1) return;
+    if (MODE == kPrefix || MODE == kAfter || pieces == 1) return;
     // The pieces are joined in groups of a.join and the groups then into one, each by the workgroup that arrives
     // last: it finds the others' partial results complete (device-scope stores, waited for before the count) and
     // reads them with device-scope loads.  One workgroup reads a piece's rows in about 0.1 us, so two levels of
@@ -495,7 +486,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
 template <int D> struct TileLds {
     static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;
 };
-template <int D>
+template <int D, int MODE>
 __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
     constexpr int NK = D / 16, NN = D / 32, NU = D / 64;  // contraction steps of K q; channel blocks; 16-byte units
     constexpr int kAhead = D == 256 ? 3 : 1;  // more, where the registers do not cost a wave per SIMD
@@ -519,23 +510,24 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
         return at >= start(i) && at - start(i) < (p.nq * a.group + 127) / 128;
     };
     const uint32_t s = a.per ? at / a.per : sequence_of(a, at, start, holds), rt = at - (a.per ? s * a.per : start(s));
-    if (split == 0 && kvh == 0 && at < a.n_seq && threadIdx.x == 0 && span_of(a, at).bad) ah_record(a.status, ((unsigned long long)at << 8) + AH_ERR_CACHE_RANGE);
-    const Span p = span_of(a, s);
+    if (MODE != kPrefix && split == 0 && kvh == 0 && at < a.n_seq && threadIdx.x == 0 && span_in<MODE>(a, at, 0).bad)
+        ah_record(a.status, ((unsigned long long)at << 8) + AH_ERR_CACHE_RANGE);
+    const Span p = span_in<MODE>(a, s, kvh);
     const uint32_t rows = p.nq * a.group, row0 = rt * 128;
-    if (rt >= (rows + 127) / 128 || rows < a.least_rows) return;
-    const int32_t pos0 = p.ctx - (int32_t)p.nq;
+    if (rt >= (rows + 127) / 128 || (MODE == kAll && rows < a.least_rows)) return;
     const uint32_t last = row0 + 127 < rows ? row0 + 127 : rows - 1;
-    const Tiles T = tiles_of(a, pos0 + (int32_t)(row0 / a.group), pos0 + (int32_t)(last / a.group));
+    const Tiles T = tiles_in<MODE>(a, position_of<MODE>(p, row0 / a.group), position_of<MODE>(p, last / a.group));
     const uint32_t chunk = piece_of(a, T), t0 = split * chunk, t1 = t0 + chunk < T.count ? t0 + chunk : T.count;
-    if (split > 0 && t0 >= T.count) return;
+    if (MODE != kAfter && split > 0 && t0 >= T.count) return;
     // this wave's rows and the positions they span
     const uint32_t wrow = row0 + 32 * wave, row = wrow + c, tok = row / a.group, hq = kvh * a.group + row % a.group;
     const bool live = row < rows, any = wrow < rows;
     const uint32_t wlast = wrow + 31 < rows ? wrow + 31 : rows - 1;
-    const int32_t lo = pos0 + (int32_t)(wrow / a.group), hi = any ? pos0 + (int32_t)(wlast / a.group) : -1;
-    const int32_t pos = live ? pos0 + (int32_t)tok : -1;
+    const int32_t lo = position_of<MODE>(p, wrow / a.group), hi = any ? position_of<MODE>(p, wlast / a.group) : -1;
+    const int32_t pos = live ? position_of<MODE>(p, tok) : -1;
     // the keys below which the window hides one (for this row, and for the last of the rows), and the sinks
-    const int32_t low_key = a.window ? pos - (int32_t)a.window + 1 : 0, low_all = a.window ? hi - (int32_t)a.window + 1 : 0;
+    const int32_t low_key = MODE == kAfter ? (int32_t)a.first_key : a.window ? pos - (int32_t)a.window + 1 : 0;
+    const int32_t low_all = MODE == kAfter ? (int32_t)a.first_key : a.window ? hi - (int32_t)a.window + 1 : 0;
     const int32_t sink_key = (int32_t)a.sinks;
     auto tile_of = [&](uint32_t i) { return i < T.head ? i : T.tail + (i - T.head); };
 
@@ -799,7 +791,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
         }
     }
     l += xor_lanes(l, 32);
-    const uint32_t pieces = D == 64 && a.join && T.count ? (T.count + chunk - 1) / chunk : 1;
+    const uint32_t pieces = MODE == kAll && D == 64 && a.join && T.count ? (T.count + chunk - 1) / chunk : 1;
     if (D == 64 && pieces > 1) {
         // Few pieces are joined by the unit's workgroup that arrives last (as in attn_rows_kernel), each lane its own place
         // of all of them, in their order whichever is last: a launch less, but a memory round trip for each piece.
@@ -853,7 +845,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     }
     if (!live) return;
     const size_t flat = (size_t)(p.q0 + tok) * a.n_heads + hq, all = (size_t)a.n_tok * a.n_heads;
-    const bool part = a.splits > 1 && !(D == 64 && a.join);
+    const bool part = MODE != kAll || (a.splits > 1 && !(D == 64 && a.join));
     const float inv = part ? 1.0f : l > 0.0f || l != l ? 1.0f / l : 0.0f;
     float *dst = part ? a.part_o + (split * all + flat) * D : a.out + (size_t)(p.q0 + tok) * a.out_stride + (size_t)hq * D;
 #pragma unroll
@@ -912,24 +904,83 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     __builtin_memcpy(a.out + (size_t)tok * a.out_stride + (size_t)head * D + c, &sum, 16);
 }
 
+// Joins what kPrefix and kAfter leave: of every token of a sequence a.splits pieces, those of no weight passed over.
+template <int D>
+__global__ void __launch_bounds__(256) attn_meet_kernel(AttnArgs a) {
+    constexpr uint32_t kLanes = D / 4, kHeads = 64 / kLanes;
+    const uint32_t lane = threadIdx.x & 63, it = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t per = (a.n_heads + kHeads - 1) / kHeads, tok = it / per, head = (it - tok * per) * kHeads + lane / kLanes;
+    if (tok >= a.n_tok) return;
+    auto start = [&](uint32_t i) { return (uint32_t)a.q_start[i]; };
+    auto holds = [&](uint32_t i) {
+        const Span p = span_in<kAfter>(a, i, 0);
+        return tok >= p.q0 && tok - p.q0 < p.nq;
+    };
+    const Span p = span_in<kAfter>(a, sequence_of(a, tok, start, holds), 0);
+    if (tok < p.q0 || tok - p.q0 >= p.nq || head >= a.n_heads) return;
+    const uint32_t c = 4 * (lane % kLanes);
+    const size_t all = (size_t)a.n_tok * a.n_heads, flat = (size_t)tok * a.n_heads + head;
+    float M = kNoMax, L = 0.0f;
+#pragma unroll 4
+    for (uint32_t k = 0; k < a.splits; ++k) M = __builtin_fmaxf(M, a.part_ml[2 * (k * all + flat)]);
+    f32x4 sum = (f32x4)0.0f;
+#pragma unroll 4
+    for (uint32_t k = 0; k < a.splits; ++k) {
+        f32x2 ml;
+        f32x4 o;
+        __builtin_memcpy(&ml, a.part_ml + 2 * (k * all + flat), 8);
+        __builtin_memcpy(&o, a.part_o + (k * all + flat) * D + c, 16);
+        const float w = __builtin_amdgcn_exp2f(ml[0] - M);
+        L += ml[1] * w;
+        sum += o * w;
+    }
+    sum *= L > 0.0f || L != L ? 1.0f / L : 0.0f;
+    __builtin_memcpy(a.out + (size_t)tok * a.out_stride + (size_t)head * D + c, &sum, 16);
+}
+
 template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) * sizeof(float); }
 
-template <int D>
-hipError_t launch(const AttnArgs &a, hipStream_t stream) {
-    const dim3 grid(a.grid), block(256);
+template <int D, int MODE> void launch_rows(const AttnArgs &a, hipStream_t stream) {
+    if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false, MODE>), dim3(a.grid), dim3(256), attn_lds<D>(), stream, a);
+    else hipLaunchKernelGGL((attn_rows_kernel<D, true, MODE>), dim3(a.grid), dim3(256), attn_lds<D>(), stream, a);
+}
+template <int D, int MODE> void launch_tiles(const AttnArgs &a, hipStream_t stream) {
+    hipLaunchKernelGGL((attn_tile_kernel<D, MODE>), dim3(a.grid), dim3(256), 2 * TileLds<D>::kBytes, stream, a);
+}
+template <int D> uint32_t join_grid(const AttnArgs &a) { return (a.n_tok * ((a.n_heads + 256 / D - 1) / (256 / D)) + 3) / 4; }
+
+template <int D> hipError_t launch(const AttnArgs &a, hipStream_t stream) {
     if (a.rows != 128) {
-        if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false>), grid, block, attn_lds<D>(), stream, a);
-        else hipLaunchKernelGGL((attn_rows_kernel<D, true>), grid, block, attn_lds<D>(), stream, a);
+        launch_rows<D, kAll>(a, stream);
         return hipGetLastError();
     }
-    hipLaunchKernelGGL(attn_tile_kernel<D>, grid, block, 2 * TileLds<D>::kBytes, stream, a);
-    const uint32_t per = (a.n_heads + 256 / D - 1) / (256 / D);
-    if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3((a.n_tok * per + 3) / 4), block, 0, stream, a);
+    launch_tiles<D, kAll>(a, stream);
+    if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3(join_grid<D>(a)), dim3(256), 0, stream, a);
+    return hipGetLastError();
+}
+template <int D> hipError_t launch_shared(const AttnArgs &prefix, const AttnArgs &after, const AttnArgs &both, hipStream_t stream) {
+    if (prefix.rows == 128) launch_tiles<D, kPrefix>(prefix, stream);
+    else launch_rows<D, kPrefix>(prefix, stream);
+    if (after.rows == 128) launch_tiles<D, kAfter>(after, stream);
+    else launch_rows<D, kAfter>(after, stream);
+    hipLaunchKernelGGL(attn_meet_kernel<D>, dim3(join_grid<D>(both)), dim3(256), 0, stream, both);
+    return hipGetLastError();
+}
+template <int D> hipError_t launch_blocks(const AttnArgs &a, hipStream_t stream) {
+    launch_rows<D, kBlocks>(a, stream);
     return hipGetLastError();
 }
 
 template <class K> hipError_t allow_lds(K *k, size_t bytes) {
     return hipFuncSetAttribute(reinterpret_cast<const void *>(k), hipFuncAttributeMaxDynamicSharedMemorySize, (int)bytes);
+}
+template <int MODE> hipError_t allow_rows() {
+    const hipError_t e = allow_lds(attn_rows_kernel<256, false, MODE>, attn_lds<256>());
+    return e != hipSuccess ? e : allow_lds(attn_rows_kernel<256, true, MODE>, attn_lds<256>());
+}
+template <int MODE> hipError_t allow_tiles() {
+    const hipError_t e = allow_lds(attn_tile_kernel<128, MODE>, 2 * TileLds<128>::kBytes);
+    return e != hipSuccess ? e : allow_lds(attn_tile_kernel<256, MODE>, 2 * TileLds<256>::kBytes);
 }
 
 } // namespace
@@ -937,10 +988,19 @@ template <class K> hipError_t allow_lds(K *k, size_t bytes) {
 hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream) {
     return a.c.dim == 64 ? launch<64>(a, stream) : a.c.dim == 128 ? launch<128>(a, stream) : launch<256>(a, stream);
 }
+hipError_t ah_launch_attn_shared(const AttnArgs &p, const AttnArgs &s, const AttnArgs &both, hipStream_t stream) {
+    return p.c.dim == 64 ? launch_shared<64>(p, s, both, stream) : p.c.dim == 128 ? launch_shared<128>(p, s, both, stream) : launch_shared<256>(p, s, both, stream);
+}
+hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream) {
+    return a.c.dim == 64 ? launch_blocks<64>(a, stream) : a.c.dim == 128 ? launch_blocks<128>(a, stream) : launch_blocks<256>(a, stream);
+}
 
 hipError_t ah_attn_init_attrs() {
-    hipError_t e = allow_lds(attn_rows_kernel<256, false>, attn_lds<256>());
-    if (e == hipSuccess) e = allow_lds(attn_rows_kernel<256, true>, attn_lds<256>());
-    if (e == hipSuccess) e = allow_lds(attn_tile_kernel<128>, 2 * TileLds<128>::kBytes);
-    return e != hipSuccess ? e : allow_lds(attn_tile_kernel<256>, 2 * TileLds<256>::kBytes);
+    hipError_t e = allow_rows<kAll>();
+    if (e == hipSuccess) e = allow_rows<kPrefix>();
+    if (e == hipSuccess) e = allow_rows<kAfter>();
+    if (e == hipSuccess) e = allow_rows<kBlocks>();
+    if (e == hipSuccess) e = allow_tiles<kAll>();
+    if (e == hipSuccess) e = allow_tiles<kPrefix>();
+    return e != hipSuccess ? e : allow_tiles<kAfter>();
 }

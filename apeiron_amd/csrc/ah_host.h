@@ -109,3 +109,10 @@ inline int32_t ensure_scratch(ah_ctx *ctx, size_t bytes, void *stream) {
 }
 
 inline size_t align256(size_t v) { return (v + 255) & ~(size_t)255; }
+
+// Whether n rows of x and n of y share a byte, from each one's first to its last (rows `stride` floats apart).
+inline bool overlap(const float *x, size_t x_stride, size_t x_row, const float *y, size_t y_stride, size_t y_row, size_t n) {
+    if (!x || !y || n == 0) return false;
+    const uintptr_t x0 = reinterpret_cast<uintptr_t>(x), y0 = reinterpret_cast<uintptr_t>(y);
+    return x0 < y0 + ((n - 1) * y_stride + y_row) * sizeof(float) && y0 < x0 + ((n - 1) * x_stride + x_row) * sizeof(float);
+}

@@ -133,6 +133,31 @@ struct AttnArgs {
     uint32_t join;
     uint32_t *count;
     unsigned long long *status;
+    uint32_t first_key;  // of a batch behind a common prefix: its length
+    // of attention over blocks: for every (token, KV head) its keys (kNoList: no token of a sequence), then the first
+    // tiles (kv4_tile's, counted; kNoList: none to see) of its blocks of 1 << block_shift tiles
+    const uint32_t *list;
+    uint32_t list_stride, block_shift;
+};
+constexpr uint32_t kNoList = 0xffffffffu;
+constexpr uint32_t kLdsKeys = 16384;  // scores of a query's blocks that the choice keeps in LDS, at most
+
+// The choice of blocks (ah_blocks.hip): a's sequences, tokens, queries, table and scale.
+struct BlockArgs {
+    AttnArgs a;
+    const uint16_t *means;
+    uint32_t shift, top, first, last;  // positions of a block: 1 << shift
+    uint32_t *list;
+    int32_t *chosen;
+    uint64_t *keys;  // [token, KV head][most]: the scores' ranks, where they do not fit LDS
+    uint32_t most, lds_keys;
+};
+struct MeansArgs {
+    Kv4Ref c;
+    KvTokens t;
+    uint32_t shift;
+    uint16_t *means;
+    unsigned long long *status;
 };
 
 // What a row's scan and count leave for the launches after them (ah_sample.hip).
@@ -178,5 +203,9 @@ hipError_t ah_launch_rope(const RopeArgs &a, hipStream_t stream);
 hipError_t ah_launch_kv4_append(const AppendArgs &a, hipStream_t stream);
 hipError_t ah_launch_kv4_read(const KvReadArgs &a, hipStream_t stream);
 hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream);
+hipError_t ah_launch_attn_shared(const AttnArgs &prefix, const AttnArgs &after, const AttnArgs &both, hipStream_t stream);
+hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream);
+hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream);
+hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream);
 size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base);
 hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream);

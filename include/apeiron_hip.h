@@ -469,6 +469,82 @@ typedef struct ah_kv4_attn {
 int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, const float *d_q, size_t q_stride,
                         float *d_out, size_t out_stride, void *stream);
 
+/* ah_kv4_attn_dev for sequences that begin with the same prefix_len positions (args' window and sinks 0): those are
+ * read once for the whole batch.  d_prefix_table: their pages, [ceil(prefix_len / page_len)]; the positions from
+ * prefix_len on are read through d_table as ever (whose entries for pages before that are not read).  The result is what
+ * ah_kv4_attn_dev gives for tables that name the prefix's pages.  A sequence with tokens before the prefix's end is
+ * refused as one out of range.  prefix_len 0: ah_kv4_attn_dev.  d_out may not overlap d_q; at most 2^30 - 1 values of it. */
+int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, size_t prefix_len,
+                               const int32_t *d_prefix_table, const float *d_q, size_t q_stride, float *d_out,
+                               size_t out_stride, void *stream);
+
+/* Attention over a part of a long context: its blocks of block_len positions (a power of two, 32 to the cache's
+ * page_len).  A query at a position of block b sees, of the positions up to its own, those of
+ *   the blocks 0 .. n_first - 1 and b - n_last .. b, and
+ *   of the blocks between, the n_top whose score is highest (of equal scores the first): scale * sum_h q_h . mean, over
+ *   the queries h of the KV head, with the mean of the block's keys in the cache; every KV head chooses for itself.
+ * Scores are f64 (a block with a NaN or a page out of range scores lowest).  Everything else as ah_kv4_attn_dev, with
+ * args' window and sinks 0.  d_means: f16 [n_pages][page_len / block_len][n_kv_heads][head_dim] in the caller's memory,
+ * 16-byte aligned; ah_kv4_block_means_dev fills in the blocks whose last position is among the tokens (each block's f64
+ * mean, rounded to f32 and then to f16), after their append.  Only whole blocks are ever scored.
+ * d_chosen (optional): [n_tok][n_kv_heads][n_top], the blocks chosen by score, ascending, then -1.
+ * 1 <= n_top <= 4096, n_first and n_last <= 4096.  d_out may not overlap d_q.  Uses the context's scratch. */
+typedef struct ah_kv4_blocks {
+    size_t block_len, n_top, n_first, n_last;
+    const uint16_t *d_means;
+} ah_kv4_blocks;
+int32_t ah_kv4_block_means_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_tokens *tokens, size_t block_len,
+                               uint16_t *d_means, void *stream);
+int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, const ah_kv4_blocks *blocks,
+                               const float *d_q, size_t q_stride, float *d_out, size_t out_stride, int32_t *d_chosen,
+                               void *stream);
+
+/* ---- recurrent layers: a state of fixed size in place of a cache ----
+ *
+ * Sequence s has the tokens d_q_start[s] .. d_q_start[s + 1] - 1 (ascending, at most max_q each) and a state in the
+ * caller's memory: it is read from slot d_from[s] (negative: zeros) and left in slot d_to[s] (negative: dropped), which
+ * may be the same one; several sequences may begin from one slot.  A slot that a sequence writes may not be another's
+ * d_from or d_to: what those then hold or begin from is unspecified.  A sequence without tokens hands its state on.  A sequence
+ * whose tokens or slots are out of range is refused with AH_ERR_CACHE_RANGE and passed over; tokens of no sequence are not
+ * written.  Rows are *_stride floats apart, and outputs may not overlap inputs.  At most 65535 sequences.  A result that is
+ * not finite is refused with AH_ERR_NONFINITE_INPUT (ah_sync_status): the outputs and state of its sequence and head or
+ * channel, from its chunk of 64 tokens on, hold no values then. */
+typedef struct ah_state_seqs {
+    size_t n_seq, n_tok, max_q, n_slots;
+    const int32_t *d_q_start;     /* [n_seq + 1] */
+    const int32_t *d_from, *d_to; /* [n_seq] */
+} ah_state_seqs;
+
+/* The short causal convolution of every channel with its own weights, optionally with SiLU:
+ * y_t = act(bias + sum_i weight[i] x_(t - width + 1 + i)), where the inputs before the call's are the state
+ * [n_slots][width - 1][n_channels], the last one last.  width 2 to 8, at most 2^20 channels. */
+typedef struct ah_conv {
+    size_t n_channels, width;
+    const float *d_weight; /* [n_channels][width] */
+    const float *d_bias;   /* [n_channels]; NULL: none */
+    int32_t silu;
+    float *d_state;
+} ah_conv;
+int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *args, const float *d_x, size_t x_stride,
+                    float *d_y, size_t y_stride, void *stream);
+
+/* The gated delta rule.  Every head keeps S [k_dim][v_dim], f32, in the state [n_slots][n_heads][k_dim][v_dim]; a token does
+ *   S = e^g S;  S += k (beta (v - S^T k))^T;  out = scale S^T q.
+ * Head h takes q and k of head h / (n_heads / n_k_heads).  With d_a_log, g = -e^a_log log(1 + e^(a + dt_bias)) and
+ * beta = 1 / (1 + e^-b); without (NULL), a is g and b is beta.  norm_eps >= 0: q and k are divided by
+ * sqrt(their sum of squares + norm_eps) first; negative: taken as they are.  k_dim 64 or 128, v_dim 64, 128 or 256.  d_q,
+ * d_k: [n_tok] rows of n_k_heads heads, d_v, d_out: of n_heads, d_a, d_b: one value a head.  Uses the context's scratch
+ * (as ah_gemm_f32_dev, also for calls captured into a graph). */
+typedef struct ah_delta_rule {
+    size_t n_heads, n_k_heads, k_dim, v_dim;
+    const float *d_a_log, *d_dt_bias; /* [n_heads], both or neither */
+    float scale, norm_eps;
+    float *d_state;
+} ah_delta_rule;
+int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta_rule *args, const float *d_q, size_t q_stride,
+                          const float *d_k, size_t k_stride, const float *d_v, size_t v_stride, const float *d_a,
+                          size_t a_stride, const float *d_b, size_t b_stride, float *d_out, size_t out_stride, void *stream);
+
 /* One token per row of logits [n_rows][n_vocab] (rows row_stride floats apart; n_vocab <= 2^20, n_rows <=
  * 65536).  Uses the context's scratch (as ah_gemm_f32_dev, also for calls captured into a graph).  In the
  * order (logit descending, index ascending), with weights w = rint(2^32 exp((logit - largest) / T)): the
