@@ -64,6 +64,7 @@ double ah_few_cost(uint32_t type, uint32_t n_in, uint32_t kpad, uint32_t tok, ui
 hipError_t ah_few_init_attrs();
 hipError_t ah_attn_init_attrs();
 hipError_t ah_blocks_init_attrs();
+hipError_t ah_state_init_attrs();
 hipError_t ah_launch_few(uint32_t type, FewArgs &a, bool ffn, hipStream_t stream);
 hipError_t ah_probe_mfma(uint32_t kind, uint32_t cus, const uint32_t *d_seed, uint32_t *d_sink,
                          hipStream_t stream, double *tops);
@@ -1002,7 +1003,7 @@ int32_t ah_init(int32_t device, ah_ctx **out) {
         hipMalloc(&ctx->d_count, kCounts * sizeof(uint32_t)) != hipSuccess ||
         hipMemset(ctx->d_count, 0, kCounts * sizeof(uint32_t)) != hipSuccess ||
         ah_gemv_init_attrs() != hipSuccess || ah_few_init_attrs() != hipSuccess || ah_attn_init_attrs() != hipSuccess ||
-        ah_blocks_init_attrs() != hipSuccess) {
+        ah_blocks_init_attrs() != hipSuccess || ah_state_init_attrs() != hipSuccess) {
         delete ctx;
         return AH_ERR_HIP;
     }

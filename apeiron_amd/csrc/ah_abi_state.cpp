@@ -88,7 +88,23 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
     a.norm_eps = p->norm_eps;
     a.status = ctx->d_status;
     AH_HIP(ctx, hipSetDevice(ctx->device));
-    AH_HIP(ctx, ah_launch_delta(a, pick(ctx, stream)));
+    // A sequence of up to 8 tokens goes token by token, a longer one by chunks.  Sequences of one length all go the same way.
+    const size_t most_steps = 8;
+    const bool chunks = a.s.max_q > most_steps, even = a.s.n_seq == 1 || n == (size_t)a.s.n_seq * a.s.max_q;
+    a.chunk_from = !chunks ? 0xffffffffu : even ? 0 : (uint32_t)most_steps + 1;
+    if (chunks) {
+        // slots for the chunks: one for every 64 tokens and one more for every sequence, or one for every 8 tokens
+        const size_t by_seq = n / kDeltaChunk + a.s.n_seq, by_tokens = n / most_steps + 1;
+        a.slot_seq = even || by_seq <= by_tokens;
+        a.slot_shift = a.slot_seq ? 6 : 3;
+        const size_t slots = a.slot_seq ? by_seq : by_tokens;
+        if (slots * H > kMaxGrid || (size_t)a.s.n_seq * H * (dv / 16) > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
+        a.slots = (uint32_t)slots;
+        const int32_t st = ensure_scratch(ctx, slots * H * delta_block((uint32_t)dk, (uint32_t)dv).bytes, stream);
+        if (st) return st;
+        a.blocks = static_cast<uint8_t *>(ctx->scratch.p);
+    }
+    AH_HIP(ctx, ah_launch_delta(a, !chunks || !even, chunks, pick(ctx, stream)));
     return AH_OK;
 }
 

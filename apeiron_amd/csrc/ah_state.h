@@ -27,8 +27,28 @@ struct DeltaArgs {
     uint64_t q_stride, k_stride, v_stride, a_stride, b_stride, out_stride;
     uint32_t n_heads, group, k_dim, v_dim;  // group: heads that share a head of q and k
     float scale, norm_eps;                  // norm_eps < 0: q and k are taken as they are
+    // Sequences of chunk_from tokens or more go by chunks of 64, the others token by token.  What the chunks' preparation leaves
+    // is a block of delta_block_bytes for every (slot, head); sequence s has its chunks' slots from
+    // (q_start[s] >> slot_shift) + s * slot_seq on.
+    uint32_t chunk_from, slots, slot_shift, slot_seq;
+    uint8_t *blocks;
     unsigned long long *status;
 };
 
+constexpr uint32_t kDeltaChunk = 64;
+// A chunk's block: fragments (1 KB: 16 bytes of each lane, f16 operands of v_mfma_f32_16x16x32_f16) of W, of the decayed keys
+// and of P, each as a half that is the f16 value and one that is the rest; U0 as f32; factors.
+struct DeltaBlock {
+    uint32_t w, k, p, u, f, bytes;  // offsets
+};
+__host__ __device__ inline constexpr DeltaBlock delta_block(uint32_t dk, uint32_t dv) {
+    const uint32_t w = 0, k = w + 4 * (dk / 32) * 2048, p = k + (dk / 16) * 2 * 2048, u = p + 6 * 2048, f = u + (dv / 16) * 4096;
+    return {w, k, p, u, f, f + 1024};
+}
+// Factors, in floats: of o's rows; e^(the chunk's decay); W's largest magnitude by slices of 32 channels; the inverse scales of
+// W [tile of tokens][slice], of the keys by slice and of P by tile; q's scale by tile; U0's largest magnitude by columns.
+constexpr uint32_t kFRow = 0, kFDecay = 64, kFWMax = 68, kFW = 72, kFK = 88, kFP = 92, kFQ = 96, kFU = 100;
+
 hipError_t ah_launch_conv(const ConvArgs &a, hipStream_t stream);
-hipError_t ah_launch_delta(const DeltaArgs &a, hipStream_t stream);
+hipError_t ah_launch_delta(const DeltaArgs &a, bool steps, bool chunks, hipStream_t stream);
+hipError_t ah_state_init_attrs();

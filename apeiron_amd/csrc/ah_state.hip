@@ -141,7 +141,7 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
     if (s >= a.s.n_seq) return;
     const Seq p = seq_of(a.s, s);
     if (p.bad && vb == 0 && h == 0 && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
-    if (p.bad) return;
+    if (p.bad || p.nq >= a.chunk_from) return;
     const size_t tile = ((size_t)h * DK + R * r) * a.v_dim + 32 * vb + 4 * c, slot = (size_t)a.n_heads * DK * a.v_dim;
     f32x4 S[R];
     if (p.from >= 0) {
@@ -201,6 +201,597 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
     if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
 }
 
+// ---- the gated delta rule, by chunks -----------------------------------------------------------------
+//
+// With gamma_i the sum of g over a chunk's tokens up to i and D_ij = e^(gamma_i - gamma_j), the rule over 64 tokens is
+//   A_ij = beta_i D_ij k_i . k_j (j < i),  T = (1 + A)^-1,  W = T (beta e^gamma k),  U0 = T (beta v),
+//   U = U0 - W S,  o = scale (e^gamma q S + P U),  P_ij = D_ij q_i . k_j (j <= i),  S' = e^gamma_63 S + (e^(gamma_63 - gamma) k)^T U.
+// delta_prepare_kernel makes W, U0, P and the decayed keys of all chunks at once; delta_chain_kernel then walks a sequence's
+// chunks with S in registers, two products deep a chunk.  No exponent above a sum of g's is ever formed, and sums of g are f64.
+//   f32 by f16: every factor of a product is carried as hi + lo, two f16 of a value scaled by a power of two so that the largest
+// of its group (a tile, a slice, a chunk) lies in [2^13, 2^14): 22 bits, or 2^-38 of the group's largest.  Three products
+// (hi hi, hi lo, lo hi) are summed in the f32 accumulator, at 5 times the rate of the f32 matrix instructions.
+//   Layouts: a lane (r, h) = (lane & 15, lane >> 4) of a 16x16 product holds column r and rows 4 h + i of the result, and of an
+// operand row (or column) r and a quarter of the 32 values that are summed over.  Which those are is free as long as both
+// operands agree: rows 4 h + i of two neighbouring tiles.  So a result is the next product's operand where it lies.
+typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
+typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
+typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
+typedef float f32x2 __attribute__((ext_vector_type(2)));
+typedef uint32_t u32x2 __attribute__((ext_vector_type(2)));
+
+AH_DEV f32x4 mfma16(f16x8 a, f16x8 b, f32x4 c) { return __builtin_amdgcn_mfma_f32_16x16x32_f16(a, b, c, 0, 0, 0); }
+
+// Two halves of an operand.
+struct Frag {
+    u32x4 hi, lo;
+};
+AH_DEV f16x2 pack16(float a, float b) { return __builtin_convertvector((f32x2){a, b}, f16x2); }
+AH_DEV void split2(float a, float b, uint32_t &hi, uint32_t &lo) {
+    const f16x2 t = pack16(a, b);
+    hi = __builtin_bit_cast(uint32_t, t);
+    lo = __builtin_bit_cast(uint32_t, pack16(a - (float)t[0], b - (float)t[1]));
+}
+AH_DEV Frag split8(const float *x, float scale) {
+    Frag f;
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+        uint32_t hi, lo;
+        split2(x[2 * i] * scale, x[2 * i + 1] * scale, hi, lo);
+        f.hi[i] = hi;
+        f.lo[i] = lo;
+    }
+    return f;
+}
+AH_DEV f32x4 mm3(const Frag &a, const Frag &b, f32x4 c) {
+    c = mfma16(__builtin_bit_cast(f16x8, a.hi), __builtin_bit_cast(f16x8, b.hi), c);
+    c = mfma16(__builtin_bit_cast(f16x8, a.hi), __builtin_bit_cast(f16x8, b.lo), c);
+    return mfma16(__builtin_bit_cast(f16x8, a.lo), __builtin_bit_cast(f16x8, b.hi), c);
+}
+// The power of two that brings `top` into [2^13, 2^14), and its inverse.
+struct Scale {
+    float up, down;
+};
+AH_DEV Scale scale_of(float top) {
+    int e = (int)(__builtin_bit_cast(uint32_t, top) >> 23) - 127;
+    e = e < -100 ? -100 : e > 127 ? 127 : e;
+    return {__builtin_ldexpf(1.0f, 13 - e), __builtin_ldexpf(1.0f, e - 13)};
+}
+AH_DEV float wave_max(float v) {
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o, 64));
+    return v;
+}
+AH_DEV float top4(float top, f32x4 v) {
+#pragma unroll
+    for (int i = 0; i < 4; ++i) top = __builtin_fmaxf(top, __builtin_fabsf(v[i]));
+    return top;
+}
+// Of a tile of tokens and a step of 32 of them, the fragment's place among the six that a lower triangle has.
+AH_DEV constexpr uint32_t tri(uint32_t tile, uint32_t step) { return tile < 2 ? tile : 2 * tile - 2 + step; }
+
+// The chunk of a slot, and of which sequence: its first token, and how many there are (0: none).
+struct Chunk {
+    uint32_t s, tok0, live;
+};
+AH_DEV Chunk chunk_of(const DeltaArgs &a, uint32_t at) {
+    auto start = [&](uint32_t i) { return ((uint32_t)a.s.q_start[i] >> a.slot_shift) + i * a.slot_seq; };
+    auto holds = [&](uint32_t i) {
+        const Seq p = seq_of(a.s, i);
+        return !p.bad && p.nq >= a.chunk_from && at >= start(i) && at - start(i) < (p.nq + kDeltaChunk - 1) / kDeltaChunk;
+    };
+    const uint32_t s = sequence_among(a.s.q_start, a.s.n_seq, a.s.n_tok, at, start, holds);
+    if (!holds(s)) return {s, 0, 0};
+    const Seq p = seq_of(a.s, s);
+    const uint32_t first = kDeltaChunk * (at - start(s)), rest = p.nq - first;
+    return {s, p.q0 + first, rest < kDeltaChunk ? rest : kDeltaChunk};
+}
+
+// A product of 16x16 f32 blocks: x [16][ld] in LDS, y in registers as a result lies (lane (r, h): y[4 h + i][r]).
+AH_DEV f32x4 block_product(const float *x, uint32_t ld, f32x4 y, f32x4 c, uint32_t r, uint32_t h) {
+    f32x4 row;
+    __builtin_memcpy(&row, x + r * ld + 4 * h, 16);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) c = __builtin_amdgcn_mfma_f32_16x16x4f32(row[i], y[i], c, 0, 0, 0);
+    return c;
+}
+
+constexpr uint32_t kLd = 68;  // floats of a row of the chunk's triangle in LDS
+template <int DK> struct PrepareLds {
+    _Float16 kh[64][DK + 8], kl[64][DK + 8];
+    float A[64 * kLd];
+    u32x4 t[6][2][64];
+    double gamma[64];
+    float beta[64], fk[64], fw[64], fd[64], red[4], tinv[4], wtop[4];
+};
+template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel(DeltaArgs a) {
+    constexpr int NJ = DK / 16, NT = DK / 32;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
+    PrepareLds<DK> &L = *reinterpret_cast<PrepareLds<DK> *>(lds_bytes);
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t at = blockIdx.x / a.n_heads, hd = blockIdx.x - at * a.n_heads, kh = hd / a.group, dv = a.v_dim;
+    const Chunk c = chunk_of(a, at);
+    if (c.live == 0) return;
+    const DeltaBlock B = delta_block(DK, dv);
+    uint8_t *block = a.blocks + ((size_t)at * a.n_heads + hd) * B.bytes;
+    float *fac = reinterpret_cast<float *>(block + B.f);
+
+    // this wave's 16 rows of k and q, as operands lie: row r, channels 16 j + 4 h + i
+    const uint32_t row = 16 * w + r;
+    f32x4 kx[NJ], qx[NJ];
+    {
+        const size_t tok = c.tok0 + (row < c.live ? row : 0);
+        const float *k = a.k + tok * a.k_stride + (size_t)kh * DK + 4 * h, *q = a.q + tok * a.q_stride + (size_t)kh * DK + 4 * h;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            __builtin_memcpy(&kx[j], k + 16 * j, 16);
+            __builtin_memcpy(&qx[j], q + 16 * j, 16);
+        }
+        if (row >= c.live) {
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) kx[j] = qx[j] = (f32x4)0.0f;
+        }
+    }
+    // gates, a lane a token: gamma by a scan
+    float beta = 0.0f, g = 0.0f;
+    if (lane < c.live) {
+        g = decay_of(a, a.a[(size_t)(c.tok0 + lane) * a.a_stride + hd], hd);
+        g = g < -1000.0f ? -1000.0f : g;  // (e^g is 0 as well, and sums stay finite)
+        beta = rate_of(a, a.b[(size_t)(c.tok0 + lane) * a.b_stride + hd]);
+    }
+    double gamma = g;
+#pragma unroll
+    for (int o = 1; o < 64; o <<= 1) {
+        const double v = __shfl_up(gamma, o, 64);
+        gamma += (int)lane >= o ? v : 0.0;
+    }
+    float ktop = 0.0f, qtop = 0.0f, fk = 1.0f, fq = a.scale;
+#pragma unroll
+    for (int j = 0; j < NJ; ++j) {
+        ktop = top4(ktop, kx[j]);
+        qtop = top4(qtop, qx[j]);
+    }
+    if (a.norm_eps >= 0.0f) {
+        float kk = 0.0f, qq = 0.0f;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                kk = __builtin_fmaf(kx[j][i], kx[j][i], kk);
+                qq = __builtin_fmaf(qx[j][i], qx[j][i], qq);
+            }
+        kk += __shfl_xor(kk, 16, 64);
+        qq += __shfl_xor(qq, 16, 64);
+        kk += __shfl_xor(kk, 32, 64);
+        qq += __shfl_xor(qq, 32, 64);
+        fk = 1.0f / __builtin_sqrtf(kk + a.norm_eps);
+        fq *= 1.0f / __builtin_sqrtf(qq + a.norm_eps);
+    }
+    if (w == 0) {
+        L.gamma[lane] = gamma;
+        L.beta[lane] = beta;
+    }
+    if (h == 0) L.fk[row] = fk;
+    ktop = wave_max(ktop);
+    if (lane == 0) L.red[w] = ktop;
+    __syncthreads();
+    const Scale ks = scale_of(__builtin_fmaxf(__builtin_fmaxf(L.red[0], L.red[1]), __builtin_fmaxf(L.red[2], L.red[3]))), qs = scale_of(wave_max(qtop));
+    Frag kf[NT], qf[NT];
+#pragma unroll
+    for (int t = 0; t < NT; ++t) {
+        float x[8], y[8];
+        __builtin_memcpy(x, &kx[2 * t], 32);
+        __builtin_memcpy(y, &qx[2 * t], 32);
+        kf[t] = split8(x, ks.up);
+        qf[t] = split8(y, qs.up);
+#pragma unroll
+        for (int n = 0; n < 2; ++n) {
+            const u32x2 hi = {kf[t].hi[2 * n], kf[t].hi[2 * n + 1]}, lo = {kf[t].lo[2 * n], kf[t].lo[2 * n + 1]};
+            __builtin_memcpy(&L.kh[row][32 * t + 16 * n + 4 * h], &hi, 8);
+            __builtin_memcpy(&L.kl[row][32 * t + 16 * n + 4 * h], &lo, 8);
+        }
+    }
+    const double gr = L.gamma[row], all = L.gamma[63];
+    if (w == 0) {  // e^gamma of each token to W's keys, what is left of the chunk's decay to the state's
+        L.fw[lane] = beta * expf((float)gamma) * L.fk[lane];
+        L.fd[lane] = expf((float)(all - gamma)) * L.fk[lane];
+        if (lane == 0) fac[kFDecay] = expf((float)all);
+    }
+    if (h == 0) fac[kFRow + row] = fq * expf((float)gr);
+    if (lane == 0) fac[kFQ + w] = qs.up;
+    __syncthreads();
+
+    // k_j . k_i and k_j . q_i of this wave's tokens i and the tiles of j up to them: a lane has i = r, j = 16 t + 4 h + n
+    const float br = L.beta[row] * fk * ks.down * ks.down, pr = fq * ks.down * qs.down;
+    f32x4 p[4];
+#pragma unroll
+    for (uint32_t jt = 0; jt < 4; ++jt) {
+        p[jt] = (f32x4)0.0f;
+        if (jt > w) continue;
+        f32x4 kk = (f32x4)0.0f, kq = (f32x4)0.0f;
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            Frag f;
+            __builtin_memcpy(&f.hi, &L.kh[16 * jt + r][32 * t + 4 * h], 8);
+            __builtin_memcpy(reinterpret_cast<char *>(&f.hi) + 8, &L.kh[16 * jt + r][32 * t + 16 + 4 * h], 8);
+            __builtin_memcpy(&f.lo, &L.kl[16 * jt + r][32 * t + 4 * h], 8);
+            __builtin_memcpy(reinterpret_cast<char *>(&f.lo) + 8, &L.kl[16 * jt + r][32 * t + 16 + 4 * h], 8);
+            kk = mm3(f, kf[t], kk);
+            kq = mm3(f, qf[t], kq);
+        }
+        f32x4 aij;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) {
+            const uint32_t j = 16 * jt + 4 * h + n;
+            const float d = expf((float)(gr - L.gamma[j])) * L.fk[j];
+            aij[n] = j < row ? br * d * kk[n] : 0.0f;
+            p[jt][n] = j <= row ? pr * d * kq[n] : 0.0f;
+        }
+        __builtin_memcpy(&L.A[row * kLd + 16 * jt + 4 * h], &aij, 16);
+    }
+    __syncthreads();
+
+    // T = (1 + A)^-1 in place: the diagonal blocks by substitution, a lane a column; then blocks of 32, then the whole
+    {
+        float *D = &L.A[16 * w * kLd + 16 * w], x[16];
+#pragma unroll
+        for (int i = 0; i < 16; ++i) {
+            float v = i == (int)r ? 1.0f : 0.0f;
+#pragma unroll
+            for (int m = 0; m < i; ++m) v = __builtin_fmaf(-D[i * kLd + m], x[m], v);
+            x[i] = v;
+        }
+        if (h == 0) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) D[i * kLd + r] = x[i];
+        }
+    }
+    __syncthreads();
+    auto at_block = [&](uint32_t i, uint32_t j) { return &L.A[16 * i * kLd + 16 * j]; };
+    auto as_result = [&](const float *x) {  // a block as a result lies
+        f32x4 v;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) v[n] = x[(4 * h + n) * kLd + r];
+        return v;
+    };
+    auto put = [&](float *x, f32x4 v) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) x[(4 * h + n) * kLd + r] = v[n];
+    };
+    const f32x4 zero = (f32x4)0.0f;
+    if (w < 2) {
+        const uint32_t b = 2 * w;
+        const f32x4 y = block_product(at_block(b + 1, b), kLd, as_result(at_block(b, b)), zero, r, h);
+        put(at_block(b + 1, b), -block_product(at_block(b + 1, b + 1), kLd, y, zero, r, h));
+    }
+    __syncthreads();
+    {
+        const uint32_t col = w & 1, low = w >> 1;  // block (2 + low, col)
+        f32x4 z = zero;
+        for (uint32_t m = 0; m <= low; ++m) {
+            f32x4 y = zero;
+            for (uint32_t n = col; n < 2; ++n) y = block_product(at_block(2 + m, n), kLd, as_result(at_block(n, col)), y, r, h);
+            z = block_product(at_block(2 + low, 2 + m), kLd, y, z, r, h);
+        }
+        __syncthreads();
+        put(at_block(2 + low, col), -z);
+    }
+    __syncthreads();
+    {  // this wave's rows of T as operands
+        float x[2][8], top = 0.0f;
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const uint32_t tile = 2 * t + n / 4;
+                x[t][n] = tile <= w ? L.A[row * kLd + 16 * tile + 4 * h + (n & 3)] : 0.0f;
+                top = __builtin_fmaxf(top, __builtin_fabsf(x[t][n]));
+            }
+        const Scale s = scale_of(wave_max(top));
+        if (lane == 0) L.tinv[w] = s.down;
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t) {
+            if (t == 1 && w < 2) continue;
+            const Frag f = split8(x[t], s.up);
+            L.t[tri(w, t)][0][lane] = f.hi;
+            L.t[tri(w, t)][1][lane] = f.lo;
+        }
+    }
+    __syncthreads();
+    auto store_frag = [&](uint32_t to, const Frag &f) {
+        __builtin_memcpy(block + to + lane * 16, &f.hi, 16);
+        __builtin_memcpy(block + to + 1024 + lane * 16, &f.lo, 16);
+    };
+    auto t_frag = [&](uint32_t tile, uint32_t t) { return Frag{L.t[tri(tile, t)][0][lane], L.t[tri(tile, t)][1][lane]}; };
+    // P of this wave's tokens
+    {
+        float top = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) top = top4(top, p[t]);
+        const Scale s = scale_of(wave_max(top));
+        if (lane == 0) fac[kFP + w] = s.down;
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t) {
+            if (t == 1 && w < 2) continue;
+            float x[8];
+            __builtin_memcpy(x, &p[2 * t], 32);
+            store_frag(B.p + tri(w, t) * 2048, split8(x, s.up));
+        }
+    }
+    // 32 channels of the keys with the tokens as what is summed over: W's transpose (a lane has token r and channels 4 h + n),
+    // and the decayed keys
+    if (w < (uint32_t)NT) {
+        float x[2][2][8], fw[2][8], fd[2][8], wt = 0.0f, dt = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
+                fw[t][n] = L.fw[j];
+                fd[t][n] = L.fd[j];
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t ch = 32 * w + 16 * k + r;
+                    const float v = ((float)L.kh[j][ch] + (float)L.kl[j][ch]) * ks.down;
+                    x[k][t][n] = v;
+                    wt = __builtin_fmaxf(wt, __builtin_fabsf(v * fw[t][n]));
+                    dt = __builtin_fmaxf(dt, __builtin_fabsf(v * fd[t][n]));
+                }
+            }
+        const Scale ws = scale_of(wave_max(wt)), ds = scale_of(wave_max(dt));
+        if (lane == 0) fac[kFK + w] = ds.down;
+        Frag kw[2][2];
+#pragma unroll
+        for (int k = 0; k < 2; ++k)
+#pragma unroll
+            for (int t = 0; t < 2; ++t) {
+                float y[8], z[8];
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    y[n] = x[k][t][n] * fw[t][n];
+                    z[n] = x[k][t][n] * fd[t][n];
+                }
+                kw[k][t] = split8(y, ws.up);
+                store_frag(B.k + ((2 * w + k) * 2 + t) * 2048, split8(z, ds.up));
+            }
+        float most = 0.0f;
+#pragma unroll
+        for (uint32_t it = 0; it < 4; ++it) {
+            f32x4 v[2] = {zero, zero};
+#pragma unroll
+            for (uint32_t t = 0; t <= it / 2; ++t) {
+                const Frag f = t_frag(it, t);
+                v[0] = mm3(kw[0][t], f, v[0]);
+                v[1] = mm3(kw[1][t], f, v[1]);
+            }
+            const float down = ws.down * L.tinv[it];
+            v[0] *= down;
+            v[1] *= down;
+            const float top = wave_max(top4(top4(0.0f, v[0]), v[1]));
+            const Scale s = scale_of(top);
+            most = __builtin_fmaxf(most, top);
+            if (lane == 0) fac[kFW + 4 * it + w] = s.down;
+            float y[8];
+            __builtin_memcpy(y, v, 32);
+            store_frag(B.w + (it * NT + w) * 2048, split8(y, s.up));
+        }
+        if (lane == 0) fac[kFWMax + w] = most;
+    }
+    // U0: every fourth 16 columns of v
+    for (uint32_t cb = w; cb < dv / 16; cb += 4) {
+        float x[2][8], top = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
+                const float v = a.v[(size_t)(c.tok0 + (j < c.live ? j : 0)) * a.v_stride + (size_t)hd * dv + 16 * cb + r];
+                x[t][n] = j < c.live ? v * L.beta[j] : 0.0f;
+                top = __builtin_fmaxf(top, __builtin_fabsf(x[t][n]));
+            }
+        const Scale s = scale_of(wave_max(top));
+        const Frag vf[2] = {split8(x[0], s.up), split8(x[1], s.up)};
+        float most = 0.0f;
+#pragma unroll
+        for (uint32_t it = 0; it < 4; ++it) {
+            f32x4 u = zero;
+#pragma unroll
+            for (uint32_t t = 0; t <= it / 2; ++t) u = mm3(t_frag(it, t), vf[t], u);
+            u *= s.down * L.tinv[it];
+            most = top4(most, u);
+            __builtin_memcpy(block + B.u + (cb * 4 + it) * 1024 + lane * 16, &u, 16);
+        }
+        most = wave_max(most);
+        if (lane == 0) fac[kFU + cb] = most;
+    }
+}
+
+// A sequence's chunks in turn, for 16 columns of a head's S.  Waves 0 to 3 are the chain: wave w makes U of the tokens
+// 16 w .. 16 w + 15 (the first half of a chunk's time) and the rows 32 w .. 32 w + 31 of S (the second); what the others need goes
+// through LDS as operands.  Waves 4 to 7 make o of the same tokens: q S beside U, P U beside S.  Two barriers a chunk.
+//   What comes from memory is asked for as soon as its registers are free, a chunk ahead.
+template <int DK> __global__ void __launch_bounds__(512) delta_chain_kernel(DeltaArgs a) {
+    constexpr int NT = DK / 32;
+    __shared__ u32x4 sf[NT][2][64], uf[2][2][64];
+    __shared__ float sinv[4], stop[4], uinv;
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+    const uint32_t units = a.s.n_seq * a.n_heads, cb = blockIdx.x / units, unit = blockIdx.x - cb * units, s = unit / a.n_heads, hd = unit - s * a.n_heads;
+    const Seq p = seq_of(a.s, s);
+    if (p.bad && cb == 0 && hd == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
+    if (p.bad || p.nq < a.chunk_from) return;
+    const uint32_t chunks = (p.nq + kDeltaChunk - 1) / kDeltaChunk, dv = a.v_dim;
+    const DeltaBlock B = delta_block(DK, dv);
+    const size_t step = (size_t)a.n_heads * B.bytes, first = (((uint32_t)a.s.q_start[s] >> a.slot_shift) + s * a.slot_seq) * step + (size_t)hd * B.bytes;
+    auto block_of = [&](uint32_t n) { return a.blocks + first + (n < chunks ? n : chunks - 1) * step; };
+    auto frag = [&](const uint8_t *b) {
+        Frag f;
+        __builtin_memcpy(&f.hi, b + lane * 16, 16);
+        __builtin_memcpy(&f.lo, b + 1024 + lane * 16, 16);
+        return f;
+    };
+    bool odd = false;
+    if (wave < 4) {
+        const bool own = w < (uint32_t)NT;
+        const size_t tile = ((size_t)hd * DK + 32 * w + 4 * h) * dv + 16 * cb + r, slot = (size_t)a.n_heads * DK * dv;
+        f32x4 S[2] = {(f32x4)0.0f, (f32x4)0.0f};
+        if (own && p.from >= 0) {
+            const float *from = a.state + (size_t)p.from * slot + tile;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) S[k][i] = from[(size_t)(16 * k + i) * dv];
+        }
+        Frag W[NT], K[2][2];
+        f32x4 u0;
+        float winv[NT], bound[NT], utop, kinv, decay;
+        auto load_first = [&](uint32_t n) {
+            const uint8_t *b = block_of(n);
+            const float *f = reinterpret_cast<const float *>(b + B.f);
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                W[t] = frag(b + B.w + (w * NT + t) * 2048);
+                winv[t] = f[kFW + 4 * w + t];
+                bound[t] = 32.0f * f[kFWMax + t];
+            }
+            __builtin_memcpy(&u0, b + B.u + (cb * 4 + w) * 1024 + lane * 16, 16);
+            utop = f[kFU + cb];
+        };
+        auto load_second = [&](uint32_t n) {
+            const uint8_t *b = block_of(n);
+            const float *f = reinterpret_cast<const float *>(b + B.f);
+            decay = f[kFDecay];
+            kinv = f[kFK + (own ? w : 0)];
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int t = 0; t < 2; ++t) K[k][t] = frag(b + B.k + ((2 * (own ? w : 0) + k) * 2 + t) * 2048);
+        };
+        auto publish = [&] {  // this wave's rows of S
+            if (!own) return;
+            const float top = wave_max(top4(top4(0.0f, S[0]), S[1]));
+            const Scale c = scale_of(top);
+            float x[8];
+            __builtin_memcpy(x, S, 32);
+            const Frag f = split8(x, c.up);
+            sf[w][0][lane] = f.hi;
+            sf[w][1][lane] = f.lo;
+            if (lane == 0) {
+                sinv[w] = c.down;
+                stop[w] = top;
+            }
+        };
+        if (chunks) {
+            load_first(0);
+            load_second(0);
+        }
+        publish();
+        ah_lds_barrier();
+        for (uint32_t n = 0; n < chunks; ++n) {
+            f32x4 u = u0;
+            float top = utop;
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                const Frag f = {sf[t][0][lane], sf[t][1][lane]};
+                const f32x4 v = mm3(W[t], f, (f32x4)0.0f);
+                u -= v * (winv[t] * sinv[t]);
+                top = __builtin_fmaf(bound[t], stop[t], top);
+            }
+            // one scale for all of U: |U| is at most |U0| and 32 times the largest of W and S of each slice
+            const Scale c = scale_of(top);
+            u32x2 hi, lo;
+            uint32_t h0, h1, l0, l1;
+            split2(u[0] * c.up, u[1] * c.up, h0, l0);
+            split2(u[2] * c.up, u[3] * c.up, h1, l1);
+            hi = {h0, h1};
+            lo = {l0, l1};
+            __builtin_memcpy(reinterpret_cast<char *>(&uf[w >> 1][0][lane]) + 8 * (w & 1), &hi, 8);
+            __builtin_memcpy(reinterpret_cast<char *>(&uf[w >> 1][1][lane]) + 8 * (w & 1), &lo, 8);
+            if (threadIdx.x == 0) uinv = c.down;
+#pragma unroll
+            for (int i = 0; i < 4; ++i) odd = odd || !finite(u[i]);
+            load_first(n + 1);
+            ah_lds_barrier();
+            if (own) {
+                const Frag f[2] = {{uf[0][0][lane], uf[0][1][lane]}, {uf[1][0][lane], uf[1][1][lane]}};
+                const float down = kinv * c.down;
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const f32x4 v = mm3(K[k][1], f[1], mm3(K[k][0], f[0], (f32x4)0.0f));
+                    S[k] = S[k] * decay + v * down;
+                }
+            }
+            load_second(n + 1);
+            publish();
+            ah_lds_barrier();
+        }
+        if (own && p.to >= 0) {
+            float *to = a.state + (size_t)p.to * slot + tile;
+#pragma unroll
+            for (int k = 0; k < 2; ++k)
+#pragma unroll
+                for (int i = 0; i < 4; ++i) to[(size_t)(16 * k + i) * dv] = S[k][i];
+        }
+    } else {
+        f32x4 q[DK / 16], qf;
+        Frag P[2];
+        float qup, pinv;
+        const uint32_t kh = hd / a.group;
+        auto load_q = [&](uint32_t n) {
+            const uint32_t t = kDeltaChunk * n + 16 * w + r;
+            const float *x = a.q + (size_t)(p.q0 + (t < p.nq ? t : 0)) * a.q_stride + (size_t)kh * DK + 4 * h;
+#pragma unroll
+            for (int j = 0; j < DK / 16; ++j) __builtin_memcpy(&q[j], x + 16 * j, 16);
+            const float *f = reinterpret_cast<const float *>(block_of(n) + B.f);
+            qup = f[kFQ + w];
+            __builtin_memcpy(&qf, f + kFRow + 16 * w + 4 * h, 16);
+        };
+        auto load_p = [&](uint32_t n) {
+            const uint8_t *b = block_of(n);
+            pinv = reinterpret_cast<const float *>(b + B.f)[kFP + w];
+#pragma unroll
+            for (uint32_t t = 0; t < 2; ++t) P[t] = frag(b + B.p + tri(w, w < 2 ? 0 : t) * 2048);
+        };
+        if (chunks) {
+            load_q(0);
+            load_p(0);
+        }
+        ah_lds_barrier();
+        for (uint32_t n = 0; n < chunks; ++n) {
+            f32x4 o = (f32x4)0.0f;
+            const float qinv = 1.0f / qup;  // (a power of two)
+#pragma unroll
+            for (int t = 0; t < NT; ++t) {
+                float x[8];
+                __builtin_memcpy(x, &q[2 * t], 32);
+                const Frag f = {sf[t][0][lane], sf[t][1][lane]};
+                o += mm3(split8(x, qup), f, (f32x4)0.0f) * (qinv * sinv[t]);
+            }
+            o *= qf;
+            load_q(n + 1);
+            ah_lds_barrier();
+            f32x4 v = mm3(P[0], {uf[0][0][lane], uf[0][1][lane]}, (f32x4)0.0f);
+            if (w >= 2) v = mm3(P[1], {uf[1][0][lane], uf[1][1][lane]}, v);
+            o += v * (pinv * uinv);
+            load_p(n + 1);
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const uint32_t t = kDeltaChunk * n + 16 * w + 4 * h + i;
+                if (t < p.nq) {
+                    a.out[(size_t)(p.q0 + t) * a.out_stride + (size_t)hd * dv + 16 * cb + r] = o[i];
+                    odd = odd || !finite(o[i]);
+                }
+            }
+            ah_lds_barrier();
+        }
+    }
+    if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
+}
+
+template <int DK> void launch_chunks(const DeltaArgs &a, hipStream_t stream) {
+    hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(a.slots * a.n_heads), dim3(256), sizeof(PrepareLds<DK>), stream, a);
+    hipLaunchKernelGGL(delta_chain_kernel<DK>, dim3(a.s.n_seq * a.n_heads * (a.v_dim / 16)), dim3(512), 0, stream, a);
+}
+
 template <int W> hipError_t launch_conv(const ConvArgs &a, hipStream_t stream) {
     hipLaunchKernelGGL(conv_kernel<W>, dim3(a.tiles * ((a.n_ch + 1023) / 1024)), dim3(256), 0, stream, a);
     return hipGetLastError();
@@ -220,9 +811,21 @@ hipError_t ah_launch_conv(const ConvArgs &a, hipStream_t stream) {
     }
 }
 
-hipError_t ah_launch_delta(const DeltaArgs &a, hipStream_t stream) {
+hipError_t ah_launch_delta(const DeltaArgs &a, bool steps, bool chunks, hipStream_t stream) {
     const uint32_t units = a.s.n_seq * a.n_heads * (a.v_dim / 32);
-    if (a.k_dim == 64) hipLaunchKernelGGL(delta_step_kernel<64>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
-    else hipLaunchKernelGGL(delta_step_kernel<128>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
+    if (steps) {
+        if (a.k_dim == 64) hipLaunchKernelGGL(delta_step_kernel<64>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL(delta_step_kernel<128>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
+    }
+    if (chunks) {
+        if (a.k_dim == 64) launch_chunks<64>(a, stream);
+        else launch_chunks<128>(a, stream);
+    }
     return hipGetLastError();
+}
+
+hipError_t ah_state_init_attrs() {
+    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(delta_prepare_kernel<64>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PrepareLds<64>));
+    return e != hipSuccess ? e : hipFuncSetAttribute(reinterpret_cast<const void *>(delta_prepare_kernel<128>), hipFuncAttributeMaxDynamicSharedMemorySize,
+                                                     (int)sizeof(PrepareLds<128>));
 }
