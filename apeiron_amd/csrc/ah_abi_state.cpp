@@ -64,7 +64,7 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
               overlap(d_v, v_stride, H * dv, d_out, out_stride, H * dv, n) || overlap(d_a, a_stride, H, d_out, out_stride, H * dv, n) ||
               overlap(d_b, b_stride, H, d_out, out_stride, H * dv, n)))
         return AH_ERR_INVALID_ARG;
-    if ((size_t)a.s.n_seq * H * (dv / 32) > kMaxU32) return AH_ERR_INVALID_ARG;
+    if ((size_t)a.s.n_seq * H * (dv / 32) > kMaxU32 || out_stride > ((size_t)1 << 23)) return AH_ERR_INVALID_ARG;
     a.q = d_q;
     a.k = d_k;
     a.v = d_v;
@@ -100,6 +100,8 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
         const size_t slots = a.slot_seq ? by_seq : by_tokens;
         if (slots * H > kMaxGrid || (size_t)a.s.n_seq * H * (dv / 16) > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
         a.slots = (uint32_t)slots;
+        const size_t most = (size_t)a.s.n_seq * H * (dv / 16);
+        a.tiles = most >= 4 * (size_t)ctx->cu_count ? 4 : most >= 2 * (size_t)ctx->cu_count ? 2 : 1;
         const int32_t st = ensure_scratch(ctx, slots * H * delta_block((uint32_t)dk, (uint32_t)dv).bytes, stream);
         if (st) return st;
         a.blocks = static_cast<uint8_t *>(ctx->scratch.p);

@@ -31,22 +31,23 @@ struct DeltaArgs {
     // is a block of delta_block_bytes for every (slot, head); sequence s has its chunks' slots from
     // (q_start[s] >> slot_shift) + s * slot_seq on.
     uint32_t chunk_from, slots, slot_shift, slot_seq;
+    uint32_t tiles;  // of 16 columns of S for a workgroup of the chain: 1, 2 or 4
     uint8_t *blocks;
     unsigned long long *status;
 };
 
 constexpr uint32_t kDeltaChunk = 64;
-// A chunk's block: fragments (1 KB: 16 bytes of each lane, f16 operands of v_mfma_f32_16x16x32_f16) of W, of the decayed keys
-// and of P, each as a half that is the f16 value and one that is the rest; U0 as f32; factors.
+// A chunk's block: fragments (1 KB: 16 bytes of each lane, f16 operands of v_mfma_f32_16x16x32_f16) of W, of the decayed keys,
+// of q and of P, each as a half that is the f16 value and one that is the rest; U0 as f32; factors.
 struct DeltaBlock {
-    uint32_t w, k, p, u, f, bytes;  // offsets
+    uint32_t w, k, q, p, u, f, bytes;  // offsets
 };
 __host__ __device__ inline constexpr DeltaBlock delta_block(uint32_t dk, uint32_t dv) {
-    const uint32_t w = 0, k = w + 4 * (dk / 32) * 2048, p = k + (dk / 16) * 2 * 2048, u = p + 6 * 2048, f = u + (dv / 16) * 4096;
-    return {w, k, p, u, f, f + 1024};
+    const uint32_t rows = 4 * (dk / 32) * 2048, w = 0, k = w + rows, q = k + rows, p = q + rows, u = p + 6 * 2048, f = u + (dv / 16) * 4096;
+    return {w, k, q, p, u, f, f + 1024};
 }
 // Factors, in floats: of o's rows; e^(the chunk's decay); W's largest magnitude by slices of 32 channels; the inverse scales of
-// W [tile of tokens][slice], of the keys by slice and of P by tile; q's scale by tile; U0's largest magnitude by columns.
+// W [tile of tokens][slice], of the keys by slice, of P and of q by tile; U0's largest magnitude by columns.
 constexpr uint32_t kFRow = 0, kFDecay = 64, kFWMax = 68, kFW = 72, kFK = 88, kFP = 92, kFQ = 96, kFU = 100;
 
 hipError_t ah_launch_conv(const ConvArgs &a, hipStream_t stream);

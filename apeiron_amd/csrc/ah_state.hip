@@ -213,7 +213,8 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
 // (hi hi, hi lo, lo hi) are summed in the f32 accumulator, at 5 times the rate of the f32 matrix instructions.
 //   Layouts: a lane (r, h) = (lane & 15, lane >> 4) of a 16x16 product holds column r and rows 4 h + i of the result, and of an
 // operand row (or column) r and a quarter of the 32 values that are summed over.  Which those are is free as long as both
-// operands agree: rows 4 h + i of two neighbouring tiles.  So a result is the next product's operand where it lies.
+// operands agree: rows 4 h + i of two neighbouring tiles.  So a result is the next product's operand where it lies.  Row m of the
+// two tiles of a slice of 32 channels of S is channel 2 m of the slice in the one and 2 m + 1 in the other.
 typedef _Float16 f16x2 __attribute__((ext_vector_type(2)));
 typedef _Float16 f16x4 __attribute__((ext_vector_type(4)));
 typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
@@ -257,10 +258,16 @@ AH_DEV Scale scale_of(float top) {
     e = e < -100 ? -100 : e > 127 ? 127 : e;
     return {__builtin_ldexpf(1.0f, 13 - e), __builtin_ldexpf(1.0f, e - 13)};
 }
+template <int CTRL> AH_DEV float dpp(float v) {
+    return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
+}
+AH_DEV float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
 AH_DEV float wave_max(float v) {
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) v = __builtin_fmaxf(v, __shfl_xor(v, o, 64));
-    return v;
+    v = __builtin_fmaxf(v, dpp<0x121>(v));  // rotations by 1, 2, 4 and 8 of each 16 lanes
+    v = __builtin_fmaxf(v, dpp<0x122>(v));
+    v = __builtin_fmaxf(v, dpp<0x124>(v));
+    v = __builtin_fmaxf(v, dpp<0x128>(v));
+    return __builtin_fmaxf(__builtin_fmaxf(lane_of(v, 0), lane_of(v, 16)), __builtin_fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 AH_DEV float top4(float top, f32x4 v) {
 #pragma unroll
@@ -275,16 +282,30 @@ struct Chunk {
     uint32_t s, tok0, live;
 };
 AH_DEV Chunk chunk_of(const DeltaArgs &a, uint32_t at) {
-    auto start = [&](uint32_t i) { return ((uint32_t)a.s.q_start[i] >> a.slot_shift) + i * a.slot_seq; };
-    auto holds = [&](uint32_t i) {
-        const Seq p = seq_of(a.s, i);
-        return !p.bad && p.nq >= a.chunk_from && at >= start(i) && at - start(i) < (p.nq + kDeltaChunk - 1) / kDeltaChunk;
+    auto within = [&](const Seq &p, uint32_t i) {
+        const uint32_t first = ((uint32_t)p.q0 >> a.slot_shift) + i * a.slot_seq;
+        return !p.bad && p.nq >= a.chunk_from && at >= first && at - first < (p.nq + kDeltaChunk - 1) / kDeltaChunk;
     };
-    const uint32_t s = sequence_among(a.s.q_start, a.s.n_seq, a.s.n_tok, at, start, holds);
-    if (!holds(s)) return {s, 0, 0};
-    const Seq p = seq_of(a.s, s);
-    const uint32_t first = kDeltaChunk * (at - start(s)), rest = p.nq - first;
-    return {s, p.q0 + first, rest < kDeltaChunk ? rest : kDeltaChunk};
+    uint32_t s, q0, nq;
+    if (a.s.n_seq <= 64) {  // a lane a sequence: one round trip to memory
+        const uint32_t lane = threadIdx.x & 63, i = lane < a.s.n_seq ? lane : a.s.n_seq - 1;
+        const Seq p = seq_of(a.s, i);
+        const uint64_t found = __builtin_amdgcn_ballot_w64(within(p, i));
+        if (!found) return {0, 0, 0};
+        s = (uint32_t)__builtin_ctzll(found);
+        q0 = (uint32_t)__builtin_amdgcn_readlane((int)p.q0, (int)s);
+        nq = (uint32_t)__builtin_amdgcn_readlane((int)p.nq, (int)s);
+    } else {
+        auto first = [&](uint32_t i) { return ((uint32_t)a.s.q_start[i] >> a.slot_shift) + i * a.slot_seq; };
+        auto holds = [&](uint32_t i) { return within(seq_of(a.s, i), i); };
+        s = sequence_among(a.s.q_start, a.s.n_seq, a.s.n_tok, at, first, holds);
+        const Seq p = seq_of(a.s, s);
+        if (!within(p, s)) return {s, 0, 0};
+        q0 = p.q0;
+        nq = p.nq;
+    }
+    const uint32_t done = kDeltaChunk * (at - ((q0 >> a.slot_shift) + s * a.slot_seq)), rest = nq - done;
+    return {s, q0 + done, rest < kDeltaChunk ? rest : kDeltaChunk};
 }
 
 // A product of 16x16 f32 blocks: x [16][ld] in LDS, y in registers as a result lies (lane (r, h): y[4 h + i][r]).
@@ -297,15 +318,32 @@ AH_DEV f32x4 block_product(const float *x, uint32_t ld, f32x4 y, f32x4 c, uint32
 }
 
 constexpr uint32_t kLd = 68;  // floats of a row of the chunk's triangle in LDS
+// A wave's rows of q or k from memory: lanes side by side on a row, 16 bytes each.  (A lane for a row and its quarter, as operands
+// lie, takes 64 lines at once and four times as long.)
+template <int DK> struct Rows {
+    static constexpr uint32_t kLanes = DK / 4, kAtOnce = 64 / kLanes, kLoads = 16 / kAtOnce;  // of a row; rows of a load; loads of 16 rows
+    f32x4 x[kLoads];
+    static AH_DEV uint32_t row(uint32_t i, uint32_t lane) { return kAtOnce * i + lane / kLanes; }
+    static AH_DEV uint32_t col(uint32_t lane) { return 4 * (lane % kLanes); }
+};
+AH_DEV float sum16(float v) {  // over each 16 lanes
+    v += dpp<0x121>(v);
+    v += dpp<0x122>(v);
+    v += dpp<0x124>(v);
+    return v + dpp<0x128>(v);
+}
+
 template <int DK> struct PrepareLds {
     _Float16 kh[64][DK + 8], kl[64][DK + 8];
-    float A[64 * kLd];
-    u32x4 t[6][2][64];
+    union {
+        float A[64 * kLd];
+        u32x4 t[6][2][64];
+    };
     double gamma[64];
-    float beta[64], fk[64], fw[64], fd[64], red[4], tinv[4], wtop[4];
+    float beta[64], fk[64], fq[64], fw[64], fd[64], red[4], tinv[4];
 };
 template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel(DeltaArgs a) {
-    constexpr int NJ = DK / 16, NT = DK / 32;
+    constexpr int NT = DK / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
     PrepareLds<DK> &L = *reinterpret_cast<PrepareLds<DK> *>(lds_bytes);
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -316,22 +354,29 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
     uint8_t *block = a.blocks + ((size_t)at * a.n_heads + hd) * B.bytes;
     float *fac = reinterpret_cast<float *>(block + B.f);
 
-    // this wave's 16 rows of k and q, as operands lie: row r, channels 16 j + 4 h + i
-    const uint32_t row = 16 * w + r;
-    f32x4 kx[NJ], qx[NJ];
-    {
-        const size_t tok = c.tok0 + (row < c.live ? row : 0);
-        const float *k = a.k + tok * a.k_stride + (size_t)kh * DK + 4 * h, *q = a.q + tok * a.q_stride + (size_t)kh * DK + 4 * h;
+    typedef Rows<DK> R;
+    R k, q;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j) {
-            __builtin_memcpy(&kx[j], k + 16 * j, 16);
-            __builtin_memcpy(&qx[j], q + 16 * j, 16);
-        }
-        if (row >= c.live) {
-#pragma unroll
-            for (int j = 0; j < NJ; ++j) kx[j] = qx[j] = (f32x4)0.0f;
-        }
+    for (uint32_t i = 0; i < R::kLoads; ++i) {
+        const uint32_t t = 16 * w + R::row(i, lane);
+        const size_t tok = c.tok0 + (t < c.live ? t : 0), at_col = (size_t)kh * DK + R::col(lane);
+        __builtin_memcpy(&k.x[i], a.k + tok * a.k_stride + at_col, 16);
+        __builtin_memcpy(&q.x[i], a.q + tok * a.q_stride + at_col, 16);
     }
+    // v's first columns of this wave (every fourth 16), as operands that sum over the tokens
+    f32x4 vx[2][4];
+    auto load_v = [&](uint32_t cb0) {
+#pragma unroll
+        for (uint32_t m = 0; m < 2; ++m)
+#pragma unroll
+            for (uint32_t t = 0; t < 4; ++t)
+#pragma unroll
+                for (uint32_t n = 0; n < 4; ++n) {
+                    const uint32_t j = 16 * t + 4 * h + n, cb = cb0 + 4 * m;
+                    vx[m][t][n] = a.v[(size_t)(c.tok0 + (j < c.live ? j : 0)) * a.v_stride + (size_t)hd * dv + 16 * (cb < dv / 16 ? cb : 0) + r];
+                }
+    };
+    load_v(w);
     // gates, a lane a token: gamma by a scan
     float beta = 0.0f, g = 0.0f;
     if (lane < c.live) {
@@ -345,61 +390,90 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
         const double v = __shfl_up(gamma, o, 64);
         gamma += (int)lane >= o ? v : 0.0;
     }
-    float ktop = 0.0f, qtop = 0.0f, fk = 1.0f, fq = a.scale;
+    float ktop = 0.0f, qtop = 0.0f;
 #pragma unroll
-    for (int j = 0; j < NJ; ++j) {
-        ktop = top4(ktop, kx[j]);
-        qtop = top4(qtop, qx[j]);
-    }
-    if (a.norm_eps >= 0.0f) {
+    for (uint32_t i = 0; i < R::kLoads; ++i) {
+        const bool live = 16 * w + R::row(i, lane) < c.live;
+        __asm__("" : "+v"(k.x[i]), "+v"(q.x[i]));  // (the loads themselves stay outside the choice)
+        k.x[i] = live ? k.x[i] : (f32x4)0.0f;
+        q.x[i] = live ? q.x[i] : (f32x4)0.0f;
+        ktop = top4(ktop, k.x[i]);
+        qtop = top4(qtop, q.x[i]);
         float kk = 0.0f, qq = 0.0f;
 #pragma unroll
-        for (int j = 0; j < NJ; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                kk = __builtin_fmaf(kx[j][i], kx[j][i], kk);
-                qq = __builtin_fmaf(qx[j][i], qx[j][i], qq);
-            }
-        kk += __shfl_xor(kk, 16, 64);
-        qq += __shfl_xor(qq, 16, 64);
-        kk += __shfl_xor(kk, 32, 64);
-        qq += __shfl_xor(qq, 32, 64);
-        fk = 1.0f / __builtin_sqrtf(kk + a.norm_eps);
-        fq *= 1.0f / __builtin_sqrtf(qq + a.norm_eps);
+        for (int n = 0; n < 4; ++n) {
+            kk = __builtin_fmaf(k.x[i][n], k.x[i][n], kk);
+            qq = __builtin_fmaf(q.x[i][n], q.x[i][n], qq);
+        }
+        kk = sum16(kk);
+        qq = sum16(qq);
+        if (DK == 128) {
+            kk += __shfl_xor(kk, 16, 64);
+            qq += __shfl_xor(qq, 16, 64);
+        }
+        if (R::col(lane) == 0) {
+            const uint32_t t = 16 * w + R::row(i, lane);
+            const bool norm = a.norm_eps >= 0.0f;
+            L.fk[t] = !live ? 0.0f : norm ? 1.0f / __builtin_sqrtf(kk + a.norm_eps) : 1.0f;
+            L.fq[t] = !live ? 0.0f : norm ? a.scale / __builtin_sqrtf(qq + a.norm_eps) : a.scale;
+        }
     }
     if (w == 0) {
         L.gamma[lane] = gamma;
         L.beta[lane] = beta;
     }
-    if (h == 0) L.fk[row] = fk;
     ktop = wave_max(ktop);
     if (lane == 0) L.red[w] = ktop;
-    __syncthreads();
-    const Scale ks = scale_of(__builtin_fmaxf(__builtin_fmaxf(L.red[0], L.red[1]), __builtin_fmaxf(L.red[2], L.red[3]))), qs = scale_of(wave_max(qtop));
+    // q through this wave's rows of the keys' place: as an operand, eight channels a lane
+    const Scale qs = scale_of(wave_max(qtop));
+    auto put_rows = [&](const R &x, float up) {
+#pragma unroll
+        for (uint32_t i = 0; i < R::kLoads; ++i) {
+            const uint32_t t = 16 * w + R::row(i, lane), col = R::col(lane);
+            uint32_t hi[2], lo[2];
+            split2(x.x[i][0] * up, x.x[i][1] * up, hi[0], lo[0]);
+            split2(x.x[i][2] * up, x.x[i][3] * up, hi[1], lo[1]);
+            __builtin_memcpy(&L.kh[t][col], hi, 8);
+            __builtin_memcpy(&L.kl[t][col], lo, 8);
+        }
+    };
+    auto row_frag = [&](uint32_t t, int n) {
+        Frag f;
+        __builtin_memcpy(&f.hi, &L.kh[t][32 * n + 8 * h], 16);
+        __builtin_memcpy(&f.lo, &L.kl[t][32 * n + 8 * h], 16);
+        return f;
+    };
+    const uint32_t row = 16 * w + r;
     Frag kf[NT], qf[NT];
+    put_rows(q, qs.up);
+    __builtin_amdgcn_wave_barrier();
 #pragma unroll
     for (int t = 0; t < NT; ++t) {
-        float x[8], y[8];
-        __builtin_memcpy(x, &kx[2 * t], 32);
-        __builtin_memcpy(y, &qx[2 * t], 32);
-        kf[t] = split8(x, ks.up);
-        qf[t] = split8(y, qs.up);
-#pragma unroll
-        for (int n = 0; n < 2; ++n) {
-            const u32x2 hi = {kf[t].hi[2 * n], kf[t].hi[2 * n + 1]}, lo = {kf[t].lo[2 * n], kf[t].lo[2 * n + 1]};
-            __builtin_memcpy(&L.kh[row][32 * t + 16 * n + 4 * h], &hi, 8);
-            __builtin_memcpy(&L.kl[row][32 * t + 16 * n + 4 * h], &lo, 8);
-        }
+        qf[t] = row_frag(row, t);
+        // for the chain in the order of S: even channels, then odd ones
+        auto halves = [](u32x4 v) {
+            return (u32x4){__builtin_amdgcn_perm(v[1], v[0], 0x05040100), __builtin_amdgcn_perm(v[3], v[2], 0x05040100),
+                           __builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302)};
+        };
+        const u32x4 hi = halves(qf[t].hi), lo = halves(qf[t].lo);
+        __builtin_memcpy(block + B.q + (w * NT + t) * 2048 + lane * 16, &hi, 16);
+        __builtin_memcpy(block + B.q + (w * NT + t) * 2048 + 1024 + lane * 16, &lo, 16);
     }
+    __syncthreads();
+    const Scale ks = scale_of(__builtin_fmaxf(__builtin_fmaxf(L.red[0], L.red[1]), __builtin_fmaxf(L.red[2], L.red[3])));
+    put_rows(k, ks.up);
     const double gr = L.gamma[row], all = L.gamma[63];
+    const float fk = L.fk[row], fq = L.fq[row];
     if (w == 0) {  // e^gamma of each token to W's keys, what is left of the chunk's decay to the state's
         L.fw[lane] = beta * expf((float)gamma) * L.fk[lane];
         L.fd[lane] = expf((float)(all - gamma)) * L.fk[lane];
         if (lane == 0) fac[kFDecay] = expf((float)all);
     }
     if (h == 0) fac[kFRow + row] = fq * expf((float)gr);
-    if (lane == 0) fac[kFQ + w] = qs.up;
+    if (lane == 0) fac[kFQ + w] = qs.down;
     __syncthreads();
+#pragma unroll
+    for (int t = 0; t < NT; ++t) kf[t] = row_frag(row, t);
 
     // k_j . k_i and k_j . q_i of this wave's tokens i and the tiles of j up to them: a lane has i = r, j = 16 t + 4 h + n
     const float br = L.beta[row] * fk * ks.down * ks.down, pr = fq * ks.down * qs.down;
@@ -411,11 +485,7 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
         f32x4 kk = (f32x4)0.0f, kq = (f32x4)0.0f;
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
-            Frag f;
-            __builtin_memcpy(&f.hi, &L.kh[16 * jt + r][32 * t + 4 * h], 8);
-            __builtin_memcpy(reinterpret_cast<char *>(&f.hi) + 8, &L.kh[16 * jt + r][32 * t + 16 + 4 * h], 8);
-            __builtin_memcpy(&f.lo, &L.kl[16 * jt + r][32 * t + 4 * h], 8);
-            __builtin_memcpy(reinterpret_cast<char *>(&f.lo) + 8, &L.kl[16 * jt + r][32 * t + 16 + 4 * h], 8);
+            const Frag f = row_frag(16 * jt + r, t);
             kk = mm3(f, kf[t], kk);
             kq = mm3(f, qf[t], kq);
         }
@@ -489,6 +559,7 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
             }
         const Scale s = scale_of(wave_max(top));
         if (lane == 0) L.tinv[w] = s.down;
+        __syncthreads();
 #pragma unroll
         for (uint32_t t = 0; t < 2; ++t) {
             if (t == 1 && w < 2) continue;
@@ -529,10 +600,12 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
                 const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
                 fw[t][n] = L.fw[j];
                 fd[t][n] = L.fd[j];
+                f16x2 hi, lo;
+                __builtin_memcpy(&hi, &L.kh[j][32 * w + 2 * r], 4);
+                __builtin_memcpy(&lo, &L.kl[j][32 * w + 2 * r], 4);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const uint32_t ch = 32 * w + 16 * k + r;
-                    const float v = ((float)L.kh[j][ch] + (float)L.kl[j][ch]) * ks.down;
+                    const float v = ((float)hi[k] + (float)lo[k]) * ks.down;
                     x[k][t][n] = v;
                     wt = __builtin_fmaxf(wt, __builtin_fabsf(v * fw[t][n]));
                     dt = __builtin_fmaxf(dt, __builtin_fabsf(v * fd[t][n]));
@@ -578,48 +651,58 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
         if (lane == 0) fac[kFWMax + w] = most;
     }
     // U0: every fourth 16 columns of v
-    for (uint32_t cb = w; cb < dv / 16; cb += 4) {
-        float x[2][8], top = 0.0f;
+    for (uint32_t cb0 = w; cb0 < dv / 16; cb0 += 8) {
+        if (cb0 != w) load_v(cb0);
 #pragma unroll
-        for (int t = 0; t < 2; ++t)
+        for (uint32_t m = 0; m < 2; ++m) {
+            const uint32_t cb = cb0 + 4 * m;
+            if (cb >= dv / 16) continue;
+            float x[2][8], top = 0.0f;
 #pragma unroll
-            for (int n = 0; n < 8; ++n) {
-                const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
-                const float v = a.v[(size_t)(c.tok0 + (j < c.live ? j : 0)) * a.v_stride + (size_t)hd * dv + 16 * cb + r];
-                x[t][n] = j < c.live ? v * L.beta[j] : 0.0f;
-                top = __builtin_fmaxf(top, __builtin_fabsf(x[t][n]));
+            for (int t = 0; t < 2; ++t)
+#pragma unroll
+                for (int n = 0; n < 8; ++n) {
+                    const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
+                    float v = vx[m][2 * t + n / 4][n & 3];
+                    __asm__("" : "+v"(v));  // (the load itself stays outside the choice)
+                    x[t][n] = j < c.live ? v * L.beta[j] : 0.0f;
+                    top = __builtin_fmaxf(top, __builtin_fabsf(x[t][n]));
+                }
+            const Scale s = scale_of(wave_max(top));
+            const Frag vf[2] = {split8(x[0], s.up), split8(x[1], s.up)};
+            float most = 0.0f;
+#pragma unroll
+            for (uint32_t it = 0; it < 4; ++it) {
+                f32x4 u = zero;
+#pragma unroll
+                for (uint32_t t = 0; t <= it / 2; ++t) u = mm3(t_frag(it, t), vf[t], u);
+                u *= s.down * L.tinv[it];
+                most = top4(most, u);
+                __builtin_memcpy(block + B.u + (cb * 4 + it) * 1024 + lane * 16, &u, 16);
             }
-        const Scale s = scale_of(wave_max(top));
-        const Frag vf[2] = {split8(x[0], s.up), split8(x[1], s.up)};
-        float most = 0.0f;
-#pragma unroll
-        for (uint32_t it = 0; it < 4; ++it) {
-            f32x4 u = zero;
-#pragma unroll
-            for (uint32_t t = 0; t <= it / 2; ++t) u = mm3(t_frag(it, t), vf[t], u);
-            u *= s.down * L.tinv[it];
-            most = top4(most, u);
-            __builtin_memcpy(block + B.u + (cb * 4 + it) * 1024 + lane * 16, &u, 16);
+            most = wave_max(most);
+            if (lane == 0) fac[kFU + cb] = most;
         }
-        most = wave_max(most);
-        if (lane == 0) fac[kFU + cb] = most;
     }
 }
 
-// A sequence's chunks in turn, for 16 columns of a head's S.  Waves 0 to 3 are the chain: wave w makes U of the tokens
-// 16 w .. 16 w + 15 (the first half of a chunk's time) and the rows 32 w .. 32 w + 31 of S (the second); what the others need goes
+// A sequence's chunks in turn, for NC times 16 columns of a head's S.  Waves 0 to 3 are the chain: wave w makes U of the tokens
+// 16 w .. 16 w + 15 (the first half of a chunk's time) and the rows of slice w of S (the second); what the others need goes
 // through LDS as operands.  Waves 4 to 7 make o of the same tokens: q S beside U, P U beside S.  Two barriers a chunk.
-//   What comes from memory is asked for as soon as its registers are free, a chunk ahead.
-template <int DK> __global__ void __launch_bounds__(512) delta_chain_kernel(DeltaArgs a) {
+//   What comes from memory is asked for two chunks ahead, and touched a few chunks before that, each of a head's workgroups a
+// part, so that it waits in the XCD's L2.
+template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_kernel(DeltaArgs a) {
     constexpr int NT = DK / 32;
-    __shared__ u32x4 sf[NT][2][64], uf[2][2][64];
-    __shared__ float sinv[4], stop[4], uinv;
+    constexpr uint32_t kTouch = 4;  // chunks
+    __shared__ u32x4 sf[NC][NT][2][64], uf[NC][2][2][64];
+    __shared__ float sinv[NC][4], stop[NC][4], uinv[NC];
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
-    const uint32_t units = a.s.n_seq * a.n_heads, cb = blockIdx.x / units, unit = blockIdx.x - cb * units, s = unit / a.n_heads, hd = unit - s * a.n_heads;
+    // columns slowest: a head's workgroups go to one XCD (they go to the eight in turn) wherever eight divides the heads
+    const uint32_t units = a.s.n_seq * a.n_heads, part = blockIdx.x / units, unit = blockIdx.x - part * units, s = unit / a.n_heads, hd = unit - s * a.n_heads;
     const Seq p = seq_of(a.s, s);
-    if (p.bad && cb == 0 && hd == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
+    if (p.bad && part == 0 && hd == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
     if (p.bad || p.nq < a.chunk_from) return;
-    const uint32_t chunks = (p.nq + kDeltaChunk - 1) / kDeltaChunk, dv = a.v_dim;
+    const uint32_t chunks = (p.nq + kDeltaChunk - 1) / kDeltaChunk, dv = a.v_dim, cb = part * NC;
     const DeltaBlock B = delta_block(DK, dv);
     const size_t step = (size_t)a.n_heads * B.bytes, first = (((uint32_t)a.s.q_start[s] >> a.slot_shift) + s * a.slot_seq) * step + (size_t)hd * B.bytes;
     auto block_of = [&](uint32_t n) { return a.blocks + first + (n < chunks ? n : chunks - 1) * step; };
@@ -632,164 +715,221 @@ template <int DK> __global__ void __launch_bounds__(512) delta_chain_kernel(Delt
     bool odd = false;
     if (wave < 4) {
         const bool own = w < (uint32_t)NT;
-        const size_t tile = ((size_t)hd * DK + 32 * w + 4 * h) * dv + 16 * cb + r, slot = (size_t)a.n_heads * DK * dv;
-        f32x4 S[2] = {(f32x4)0.0f, (f32x4)0.0f};
+        const size_t tile = ((size_t)hd * DK + 32 * w + 8 * h) * dv + 16 * cb + r, slot = (size_t)a.n_heads * DK * dv;
+        f32x4 S[NC][2];
+#pragma unroll
+        for (int c = 0; c < NC; ++c) S[c][0] = S[c][1] = (f32x4)0.0f;
         if (own && p.from >= 0) {
             const float *from = a.state + (size_t)p.from * slot + tile;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) S[k][i] = from[(size_t)(16 * k + i) * dv];
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) S[c][k][i] = from[(size_t)(2 * i + k) * dv + 16 * c];
         }
-        Frag W[NT], K[2][2];
-        f32x4 u0;
-        float winv[NT], bound[NT], utop, kinv, decay;
-        auto load_first = [&](uint32_t n) {
+        // of a chunk: W, U0 and the factors (a lane each) for the first half of its time, the keys for the second
+        struct Ahead {
+            Frag W[NT], K[2][2];
+            f32x4 u0[NC];
+            float f;
+        } ahead[2];
+        auto load_first = [&](uint32_t n, Ahead &x) {
             const uint8_t *b = block_of(n);
-            const float *f = reinterpret_cast<const float *>(b + B.f);
 #pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                W[t] = frag(b + B.w + (w * NT + t) * 2048);
-                winv[t] = f[kFW + 4 * w + t];
-                bound[t] = 32.0f * f[kFWMax + t];
-            }
-            __builtin_memcpy(&u0, b + B.u + (cb * 4 + w) * 1024 + lane * 16, 16);
-            utop = f[kFU + cb];
+            for (int t = 0; t < NT; ++t) x.W[t] = frag(b + B.w + (w * NT + t) * 2048);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) __builtin_memcpy(&x.u0[c], b + B.u + ((cb + c) * 4 + w) * 1024 + lane * 16, 16);
         };
-        auto load_second = [&](uint32_t n) {
+        auto load_second = [&](uint32_t n, Ahead &x) {
             const uint8_t *b = block_of(n);
-            const float *f = reinterpret_cast<const float *>(b + B.f);
-            decay = f[kFDecay];
-            kinv = f[kFK + (own ? w : 0)];
 #pragma unroll
             for (int k = 0; k < 2; ++k)
 #pragma unroll
-                for (int t = 0; t < 2; ++t) K[k][t] = frag(b + B.k + ((2 * (own ? w : 0) + k) * 2 + t) * 2048);
+                for (int t = 0; t < 2; ++t) x.K[k][t] = frag(b + B.k + ((2 * (own ? w : 0) + k) * 2 + t) * 2048);
+            x.f = reinterpret_cast<const float *>(b + B.f)[64 + lane];
         };
         auto publish = [&] {  // this wave's rows of S
             if (!own) return;
-            const float top = wave_max(top4(top4(0.0f, S[0]), S[1]));
-            const Scale c = scale_of(top);
-            float x[8];
-            __builtin_memcpy(x, S, 32);
-            const Frag f = split8(x, c.up);
-            sf[w][0][lane] = f.hi;
-            sf[w][1][lane] = f.lo;
-            if (lane == 0) {
-                sinv[w] = c.down;
-                stop[w] = top;
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                const float top = wave_max(top4(top4(0.0f, S[c][0]), S[c][1]));
+                const Scale z = scale_of(top);
+                float x[8];
+                __builtin_memcpy(x, S[c], 32);
+                const Frag f = split8(x, z.up);
+                sf[c][w][0][lane] = f.hi;
+                sf[c][w][1][lane] = f.lo;
+                if (lane == 0) {
+                    sinv[c][w] = z.down;
+                    stop[c][w] = top;
+                }
             }
         };
+        auto chunk = [&](uint32_t n, Ahead &x) {
+            float udown[NC];
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                f32x4 u = x.u0[c];
+                float top = lane_of(x.f, kFU - 64 + cb + c);
+#pragma unroll
+                for (int t = 0; t < NT; ++t) {
+                    const Frag f = {sf[c][t][0][lane], sf[c][t][1][lane]};
+                    const f32x4 v = mm3(x.W[t], f, (f32x4)0.0f);
+                    u -= v * (lane_of(x.f, kFW - 64 + 4 * w + t) * sinv[c][t]);
+                    top = __builtin_fmaf(32.0f * lane_of(x.f, kFWMax - 64 + t), stop[c][t], top);
+                }
+                // one scale for all of U: |U| is at most |U0| and 32 times the largest of W and S of each slice
+                const Scale z = scale_of(top);
+                uint32_t hi[2], lo[2];
+                split2(u[0] * z.up, u[1] * z.up, hi[0], lo[0]);
+                split2(u[2] * z.up, u[3] * z.up, hi[1], lo[1]);
+                __builtin_memcpy(reinterpret_cast<char *>(&uf[c][w >> 1][0][lane]) + 8 * (w & 1), hi, 8);
+                __builtin_memcpy(reinterpret_cast<char *>(&uf[c][w >> 1][1][lane]) + 8 * (w & 1), lo, 8);
+                if (threadIdx.x == 0) uinv[c] = z.down;
+                udown[c] = z.down;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) odd = odd || !finite(u[i]);
+            }
+            load_first(n + 2, x);
+            ah_lds_barrier();
+            if (own) {
+                const float decay = lane_of(x.f, kFDecay - 64), kdown = lane_of(x.f, kFK - 64 + w);
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const Frag f[2] = {{uf[c][0][0][lane], uf[c][0][1][lane]}, {uf[c][1][0][lane], uf[c][1][1][lane]}};
+#pragma unroll
+                    for (int k = 0; k < 2; ++k) {
+                        const f32x4 v = mm3(x.K[k][1], f[1], mm3(x.K[k][0], f[0], (f32x4)0.0f));
+                        S[c][k] = S[c][k] * decay + v * (kdown * udown[c]);
+                    }
+                }
+            }
+            load_second(n + 2, x);
+            publish();
+            ah_lds_barrier();
+        };
         if (chunks) {
-            load_first(0);
-            load_second(0);
+#pragma unroll
+            for (uint32_t n = 0; n < 2; ++n) {
+                load_first(n, ahead[n]);
+                __builtin_amdgcn_sched_barrier(0);
+                load_second(n, ahead[n]);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
         publish();
         ah_lds_barrier();
-        for (uint32_t n = 0; n < chunks; ++n) {
-            f32x4 u = u0;
-            float top = utop;
-#pragma unroll
-            for (int t = 0; t < NT; ++t) {
-                const Frag f = {sf[t][0][lane], sf[t][1][lane]};
-                const f32x4 v = mm3(W[t], f, (f32x4)0.0f);
-                u -= v * (winv[t] * sinv[t]);
-                top = __builtin_fmaf(bound[t], stop[t], top);
-            }
-            // one scale for all of U: |U| is at most |U0| and 32 times the largest of W and S of each slice
-            const Scale c = scale_of(top);
-            u32x2 hi, lo;
-            uint32_t h0, h1, l0, l1;
-            split2(u[0] * c.up, u[1] * c.up, h0, l0);
-            split2(u[2] * c.up, u[3] * c.up, h1, l1);
-            hi = {h0, h1};
-            lo = {l0, l1};
-            __builtin_memcpy(reinterpret_cast<char *>(&uf[w >> 1][0][lane]) + 8 * (w & 1), &hi, 8);
-            __builtin_memcpy(reinterpret_cast<char *>(&uf[w >> 1][1][lane]) + 8 * (w & 1), &lo, 8);
-            if (threadIdx.x == 0) uinv = c.down;
-#pragma unroll
-            for (int i = 0; i < 4; ++i) odd = odd || !finite(u[i]);
-            load_first(n + 1);
-            ah_lds_barrier();
-            if (own) {
-                const Frag f[2] = {{uf[0][0][lane], uf[0][1][lane]}, {uf[1][0][lane], uf[1][1][lane]}};
-                const float down = kinv * c.down;
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const f32x4 v = mm3(K[k][1], f[1], mm3(K[k][0], f[0], (f32x4)0.0f));
-                    S[k] = S[k] * decay + v * down;
-                }
-            }
-            load_second(n + 1);
-            publish();
-            ah_lds_barrier();
+        for (uint32_t n = 0; n + 1 < chunks; n += 2) {
+            chunk(n, ahead[0]);
+            chunk(n + 1, ahead[1]);
         }
+        if (chunks & 1) chunk(chunks - 1, ahead[0]);
         if (own && p.to >= 0) {
             float *to = a.state + (size_t)p.to * slot + tile;
 #pragma unroll
-            for (int k = 0; k < 2; ++k)
+            for (int c = 0; c < NC; ++c)
 #pragma unroll
-                for (int i = 0; i < 4; ++i) to[(size_t)(16 * k + i) * dv] = S[k][i];
+                for (int k = 0; k < 2; ++k)
+#pragma unroll
+                    for (int i = 0; i < 4; ++i) to[(size_t)(2 * i + k) * dv + 16 * c] = S[c][k][i];
         }
     } else {
-        f32x4 q[DK / 16], qf;
-        Frag P[2];
-        float qup, pinv;
-        const uint32_t kh = hd / a.group;
-        auto load_q = [&](uint32_t n) {
-            const uint32_t t = kDeltaChunk * n + 16 * w + r;
-            const float *x = a.q + (size_t)(p.q0 + (t < p.nq ? t : 0)) * a.q_stride + (size_t)kh * DK + 4 * h;
-#pragma unroll
-            for (int j = 0; j < DK / 16; ++j) __builtin_memcpy(&q[j], x + 16 * j, 16);
-            const float *f = reinterpret_cast<const float *>(block_of(n) + B.f);
-            qup = f[kFQ + w];
-            __builtin_memcpy(&qf, f + kFRow + 16 * w + 4 * h, 16);
-        };
-        auto load_p = [&](uint32_t n) {
+        struct Ahead {
+            Frag Q[NT], P[2];
+            f32x4 qf;
+            float f;
+            uint32_t touched;
+        } ahead[2];
+        auto load_first = [&](uint32_t n, Ahead &x) {
             const uint8_t *b = block_of(n);
-            pinv = reinterpret_cast<const float *>(b + B.f)[kFP + w];
 #pragma unroll
-            for (uint32_t t = 0; t < 2; ++t) P[t] = frag(b + B.p + tri(w, w < 2 ? 0 : t) * 2048);
+            for (int t = 0; t < NT; ++t) x.Q[t] = frag(b + B.q + (w * NT + t) * 2048);
         };
-        if (chunks) {
-            load_q(0);
-            load_p(0);
-        }
-        ah_lds_barrier();
-        for (uint32_t n = 0; n < chunks; ++n) {
-            f32x4 o = (f32x4)0.0f;
-            const float qinv = 1.0f / qup;  // (a power of two)
+        auto load_second = [&](uint32_t n, Ahead &x) {
+            const uint8_t *b = block_of(n);
+            __builtin_memcpy(&x.qf, reinterpret_cast<const float *>(b + B.f) + kFRow + 16 * w + 4 * h, 16);
+#pragma unroll
+            for (uint32_t t = 0; t < 2; ++t) x.P[t] = frag(b + B.p + tri(w, w < 2 ? 0 : t) * 2048);
+            x.f = reinterpret_cast<const float *>(b + B.f)[64 + lane];
+        };
+        // A line of 128 bytes for each lane, of what all of a head's workgroups read: each takes a part, each wave of it a fourth.
+        const uint32_t parts = dv / (16 * NC), lines = B.u / 128, each = (lines + 4 * parts - 1) / (4 * parts);
+        auto touch = [&](uint32_t n) {
+            uint32_t v;
+            const uint32_t at = (4 * part + w) * each + (lane < each ? lane : 0);
+            __builtin_memcpy(&v, block_of(n) + 128 * (at < lines ? at : lines - 1), 4);
+            return v;
+        };
+        auto chunk = [&](uint32_t n, Ahead &x) {
+            f32x4 o[NC];
+            const float qinv = lane_of(x.f, kFQ - 64 + w);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c] = (f32x4)0.0f;
 #pragma unroll
             for (int t = 0; t < NT; ++t) {
-                float x[8];
-                __builtin_memcpy(x, &q[2 * t], 32);
-                const Frag f = {sf[t][0][lane], sf[t][1][lane]};
-                o += mm3(split8(x, qup), f, (f32x4)0.0f) * (qinv * sinv[t]);
-            }
-            o *= qf;
-            load_q(n + 1);
-            ah_lds_barrier();
-            f32x4 v = mm3(P[0], {uf[0][0][lane], uf[0][1][lane]}, (f32x4)0.0f);
-            if (w >= 2) v = mm3(P[1], {uf[1][0][lane], uf[1][1][lane]}, v);
-            o += v * (pinv * uinv);
-            load_p(n + 1);
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t t = kDeltaChunk * n + 16 * w + 4 * h + i;
-                if (t < p.nq) {
-                    a.out[(size_t)(p.q0 + t) * a.out_stride + (size_t)hd * dv + 16 * cb + r] = o[i];
-                    odd = odd || !finite(o[i]);
+                for (int c = 0; c < NC; ++c) {
+                    const Frag f = {sf[c][t][0][lane], sf[c][t][1][lane]};
+                    o[c] += mm3(x.Q[t], f, (f32x4)0.0f) * (qinv * sinv[c][t]);
                 }
             }
+#pragma unroll
+            for (int c = 0; c < NC; ++c) o[c] *= x.qf;
+            load_first(n + 2, x);
             ah_lds_barrier();
+            const float pinv = lane_of(x.f, kFP - 64 + w);
+#pragma unroll
+            for (int c = 0; c < NC; ++c) {
+                f32x4 v = mm3(x.P[0], {uf[c][0][0][lane], uf[c][0][1][lane]}, (f32x4)0.0f);
+                if (w >= 2) v = mm3(x.P[1], {uf[c][1][0][lane], uf[c][1][1][lane]}, v);
+                o[c] += v * (pinv * uinv[c]);
+            }
+            load_second(n + 2, x);
+            // (range-checked stores: a branch around them would have every later wait for loads wait for them too)
+            const uint32_t live = p.nq - kDeltaChunk * n < kDeltaChunk ? p.nq - kDeltaChunk * n : kDeltaChunk, stride = (uint32_t)a.out_stride;
+            const __amdgpu_buffer_rsrc_t to = ah_rsrc(a.out + (size_t)(p.q0 + kDeltaChunk * n) * a.out_stride + (size_t)hd * dv + 16 * cb, 4 * ((live - 1) * stride + 16 * NC));
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+#pragma unroll
+                for (int c = 0; c < NC; ++c) {
+                    const uint32_t t = 16 * w + 4 * h + i;
+                    const float y = o[c][i];
+                    __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, y), to, (int)(4 * (t * stride + 16 * c + r)), 0, 0);
+                    odd = odd || (t < live && !finite(y));
+                }
+            __asm__ volatile("" ::"v"(x.touched));
+            x.touched = touch(n + kTouch);
+            ah_lds_barrier();
+        };
+        if (chunks) {
+#pragma unroll
+            for (uint32_t n = 0; n < 2; ++n) {
+                load_first(n, ahead[n]);
+                __builtin_amdgcn_sched_barrier(0);
+                load_second(n, ahead[n]);
+                ahead[n].touched = touch(n + 2);
+                __builtin_amdgcn_sched_barrier(0);
+            }
         }
+        ah_lds_barrier();
+        for (uint32_t n = 0; n + 1 < chunks; n += 2) {
+            chunk(n, ahead[0]);
+            chunk(n + 1, ahead[1]);
+        }
+        if (chunks & 1) chunk(chunks - 1, ahead[0]);
     }
     if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
 }
 
+template <int DK, int NC> void launch_chain(const DeltaArgs &a, hipStream_t stream) {
+    hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.s.n_seq * a.n_heads * (a.v_dim / (16 * NC))), dim3(512), 0, stream, a);
+}
 template <int DK> void launch_chunks(const DeltaArgs &a, hipStream_t stream) {
     hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(a.slots * a.n_heads), dim3(256), sizeof(PrepareLds<DK>), stream, a);
-    hipLaunchKernelGGL(delta_chain_kernel<DK>, dim3(a.s.n_seq * a.n_heads * (a.v_dim / 16)), dim3(512), 0, stream, a);
+    if (a.tiles == 1) launch_chain<DK, 1>(a, stream);
+    else if (a.tiles == 2) launch_chain<DK, 2>(a, stream);
+    else launch_chain<DK, 4>(a, stream);
 }
 
 template <int W> hipError_t launch_conv(const ConvArgs &a, hipStream_t stream) {
