@@ -5,6 +5,7 @@
 namespace {
 
 constexpr size_t kMaxU32 = 0x7fffffff, kMaxGrid = 0xffffffffu / 256;  // (workgroups of 256 threads: under 2^32 threads)
+constexpr size_t kMaxStride = (size_t)1 << 23;  // floats: 64 rows and more within a range-checked resource's 32 bits
 
 // The sequences of a call; false where they are refused.
 bool seqs_of(const ah_state_seqs *p, StateSeqs &s) {
@@ -24,7 +25,7 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *p, co
     ConvArgs a = {};
     if (!seqs_of(seqs, a.s) || !p->d_weight || !p->d_state) return AH_ERR_INVALID_ARG;
     const size_t C = p->n_channels, n_tok = a.s.n_tok;
-    if (n_tok && (!d_x || !d_y || x_stride < C || y_stride < C || overlap(d_x, x_stride, C, d_y, y_stride, C, n_tok))) return AH_ERR_INVALID_ARG;
+    if (n_tok && (!d_x || !d_y || x_stride < C || y_stride < C || x_stride > kMaxStride || y_stride > kMaxStride || overlap(d_x, x_stride, C, d_y, y_stride, C, n_tok))) return AH_ERR_INVALID_ARG;
     a.x = d_x;
     a.y = d_y;
     a.x_stride = x_stride;
@@ -37,10 +38,14 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *p, co
     a.silu = p->silu != 0;
     a.status = ctx->d_status;
     const size_t blocks = (C + 1023) / 1024, max_q = a.s.max_q ? a.s.max_q : 1;
-    a.tile = 32;
+    // Tiles of 32 tokens; of 16 or 8 where those leave the CUs without four workgroups each.
     const bool even = n_tok == (size_t)a.s.n_seq * a.s.max_q || a.s.n_seq == 1;
-    a.per = even ? (uint32_t)((max_q + a.tile - 1) / a.tile) : 0;
-    const size_t tiles = even ? (size_t)a.per * a.s.n_seq : n_tok / a.tile + a.s.n_seq;
+    size_t tiles = 0;
+    for (a.tile = 32;; a.tile /= 2) {
+        a.per = even ? (uint32_t)((max_q + a.tile - 1) / a.tile) : 0;
+        tiles = even ? (size_t)a.per * a.s.n_seq : n_tok / a.tile + a.s.n_seq;
+        if (a.tile == 8 || tiles * blocks >= 4 * (size_t)ctx->cu_count) break;
+    }
     if (tiles > kMaxGrid / blocks) return AH_ERR_INVALID_ARG;
     a.tiles = (uint32_t)tiles;
     AH_HIP(ctx, hipSetDevice(ctx->device));
@@ -64,7 +69,7 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
               overlap(d_v, v_stride, H * dv, d_out, out_stride, H * dv, n) || overlap(d_a, a_stride, H, d_out, out_stride, H * dv, n) ||
               overlap(d_b, b_stride, H, d_out, out_stride, H * dv, n)))
         return AH_ERR_INVALID_ARG;
-    if ((size_t)a.s.n_seq * H * (dv / 32) > kMaxU32 || out_stride > ((size_t)1 << 23)) return AH_ERR_INVALID_ARG;
+    if ((size_t)a.s.n_seq * H * (dv / 32) > kMaxU32 || out_stride > kMaxStride) return AH_ERR_INVALID_ARG;
     a.q = d_q;
     a.k = d_k;
     a.v = d_v;
@@ -101,7 +106,7 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
         if (slots * H > kMaxGrid || (size_t)a.s.n_seq * H * (dv / 16) > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
         a.slots = (uint32_t)slots;
         const size_t most = (size_t)a.s.n_seq * H * (dv / 16);
-        a.tiles = most >= 4 * (size_t)ctx->cu_count ? 4 : most >= 2 * (size_t)ctx->cu_count ? 2 : 1;
+        a.tiles = most >= 4 * (size_t)ctx->cu_count ? 4 : most > (size_t)ctx->cu_count ? 2 : 1;
         const int32_t st = ensure_scratch(ctx, slots * H * delta_block((uint32_t)dk, (uint32_t)dv).bytes, stream);
         if (st) return st;
         a.blocks = static_cast<uint8_t *>(ctx->scratch.p);

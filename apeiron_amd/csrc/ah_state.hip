@@ -31,91 +31,96 @@ AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 // ---- the short causal convolution --------------------------------------------------------------------
 //
 // y_t = act(bias + sum_i w_i x_(t - W + 1 + i)), a lane four channels of a tile of consecutive tokens: it keeps the
-// W - 1 rows before the next one in registers, so a row is read once a tile and the rows before a tile once more.  The
-// tile that holds a sequence's first token alone reads the state and also writes the new one, so that both may lie in
-// the same slot.
-AH_DEV void load4(float *v, const float *p, uint32_t take) {
+// W - 1 rows before the next one in registers and has eight rows on their way, so a row is read once a tile and the rows before a
+// tile once more.  The tile that holds a sequence's first token alone reads the state and also writes the new one, so that both
+// may lie in the same slot.  Rows come and go through range-checked resources: no branch stands between the loads.
+AH_DEV f32x4 ld4(__amdgpu_buffer_rsrc_t r, uint32_t at) { return __builtin_bit_cast(f32x4, ah_ld128(r, 4 * at)); }
+AH_DEV void st4(__amdgpu_buffer_rsrc_t r, uint32_t at, f32x4 v, uint32_t take) {
     if (take == 4) {
-        __builtin_memcpy(v, p, 16);
+        __builtin_amdgcn_raw_buffer_store_b128(__builtin_bit_cast(u32x4, v), r, (int)(4 * at), 0, 0);
         return;
     }
 #pragma unroll
-    for (uint32_t i = 0; i < 4; ++i) v[i] = i < take ? p[i] : 0.0f;
-}
-AH_DEV void store4(float *p, const float *v, uint32_t take) {
-    if (take == 4) {
-        __builtin_memcpy(p, v, 16);
-        return;
+    for (uint32_t i = 0; i < 3; ++i) {
+        const float x = v[i];
+        if (i < take) __builtin_amdgcn_raw_buffer_store_b32(__builtin_bit_cast(uint32_t, x), r, (int)(4 * (at + i)), 0, 0);
     }
-#pragma unroll
-    for (uint32_t i = 0; i < 4; ++i)
-        if (i < take) p[i] = v[i];
 }
 
 template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) {
+    constexpr uint32_t kRows = 8;  // on their way
     const uint32_t at = blockIdx.x % a.tiles, block = blockIdx.x / a.tiles, c0 = 4 * (block * 256 + threadIdx.x);
+    const uint32_t take = c0 >= a.n_ch ? 0 : a.n_ch - c0 < 4 ? a.n_ch - c0 : 4;
+    const __amdgpu_buffer_rsrc_t wr = ah_rsrc(a.weight, 4 * a.n_ch * W);
+    float w[4 * W];
+#pragma unroll
+    for (int j = 0; j < W; ++j) {
+        const f32x4 v = ld4(wr, c0 * W + 4 * j);
+        __builtin_memcpy(w + 4 * j, &v, 16);
+    }
+    f32x4 bias = (f32x4)0.0f;
+    if (a.bias) bias = ld4(ah_rsrc(a.bias, 4 * a.n_ch), c0);
     auto start = [&](uint32_t i) { return (uint32_t)a.s.q_start[i] / a.tile + i; };
     auto holds = [&](uint32_t i) {
         const Seq p = seq_of(a.s, i);
         return !p.bad && at >= start(i) && at - start(i) < (p.nq ? (p.nq + a.tile - 1) / a.tile : 1);
     };
     const uint32_t s = a.per ? at / a.per : sequence_among(a.s.q_start, a.s.n_seq, a.s.n_tok, at, start, holds), n = at - (a.per ? s * a.per : start(s));
+    const Seq p = seq_of(a.s, s);
+    const uint32_t t0 = n * a.tile;
+    if (!p.bad && (n == 0 || t0 < p.nq)) {
+        const uint32_t rows = t0 >= p.nq ? 0 : p.nq - t0 < a.tile ? p.nq - t0 : a.tile, x_stride = (uint32_t)a.x_stride, y_stride = (uint32_t)a.y_stride;
+        const uint32_t back = n ? W - 1 : 0;  // rows of the tile before this one (a tile has at least as many)
+        const __amdgpu_buffer_rsrc_t xr = ah_rsrc(a.x + (size_t)(p.q0 + t0 - back) * a.x_stride, rows + back ? 4 * ((rows + back - 1) * x_stride + a.n_ch) : 0);
+        const __amdgpu_buffer_rsrc_t yr = ah_rsrc(a.y + (size_t)(p.q0 + t0) * a.y_stride, rows ? 4 * ((rows - 1) * y_stride + a.n_ch) : 0);
+        const uint32_t slot = 4 * (W - 1) * a.n_ch;
+        const __amdgpu_buffer_rsrc_t old = ah_rsrc(a.state + (size_t)(p.from < 0 ? 0 : p.from) * (W - 1) * a.n_ch, p.from < 0 ? 0 : slot);
+        f32x4 row[W - 1], ahead[kRows];
+#pragma unroll
+        for (uint32_t j = 0; j < W - 1; ++j) row[j] = n ? ld4(xr, j * x_stride + c0) : ld4(old, j * a.n_ch + c0);
+#pragma unroll
+        for (uint32_t j = 0; j < kRows; ++j) ahead[j] = ld4(xr, (back + j) * x_stride + c0);
+        if (n == 0 && p.to >= 0) {  // the last W - 1 of the state's rows and the sequence's
+            const __amdgpu_buffer_rsrc_t to = ah_rsrc(a.state + (size_t)p.to * (W - 1) * a.n_ch, slot);
+            const uint32_t first = p.nq < W - 1 ? 0 : p.nq - (W - 1);
+            const __amdgpu_buffer_rsrc_t end = ah_rsrc(a.x + (size_t)(p.q0 + first) * a.x_stride, p.nq ? 4 * ((p.nq - first - 1) * x_stride + a.n_ch) : 0);
+            f32x4 kept[W - 1];
+#pragma unroll
+            for (uint32_t j = 0; j < W - 1; ++j)  // row nq + j of both, one after the other
+                kept[j] = p.nq + j < W - 1 ? ld4(old, (p.nq + j) * a.n_ch + c0) : ld4(end, (p.nq + j - (W - 1) - first) * x_stride + c0);
+#pragma unroll
+            for (uint32_t j = 0; j < W - 1; ++j) st4(to, j * a.n_ch + c0, kept[j], take);
+        }
+        bool odd = false;
+        for (uint32_t t = 0; t < rows; t += kRows) {
+            f32x4 now[kRows];
+#pragma unroll
+            for (uint32_t j = 0; j < kRows; ++j) now[j] = ahead[j];
+#pragma unroll
+            for (uint32_t j = 0; j < kRows; ++j) ahead[j] = ld4(xr, (back + t + kRows + j) * x_stride + c0);
+#pragma unroll
+            for (uint32_t j = 0; j < kRows; ++j) {
+                f32x4 out;
+#pragma unroll
+                for (int i = 0; i < 4; ++i) {
+                    float v = bias[i];
+#pragma unroll
+                    for (int k = 0; k < W - 1; ++k) v = __builtin_fmaf(w[i * W + k], row[k][i], v);
+                    v = __builtin_fmaf(w[i * W + W - 1], now[j][i], v);
+                    odd = odd || ((uint32_t)i < take && t + j < rows && !finite(v));
+                    out[i] = a.silu ? v / (1.0f + expf(-v)) : v;
+                }
+                if (t + j < rows) st4(yr, (t + j) * y_stride + c0, out, take);
+#pragma unroll
+                for (int k = 0; k + 1 < W - 1; ++k) row[k] = row[k + 1];
+                row[W - 2] = now[j];
+            }
+        }
+        if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
+    }
     if (block == 0 && threadIdx.x == 0)
         for (uint32_t i = at; i < a.s.n_seq; i += a.tiles)
             if (seq_of(a.s, i).bad) ah_record(a.status, ((unsigned long long)i << 8) + kKeyRange);
-    const Seq p = seq_of(a.s, s);
-    const uint32_t t0 = n * a.tile, take = c0 >= a.n_ch ? 0 : a.n_ch - c0 < 4 ? a.n_ch - c0 : 4;
-    if (p.bad || take == 0 || (n && t0 >= p.nq)) return;
-    const uint32_t t1 = t0 + a.tile < p.nq ? t0 + a.tile : p.nq;
-    const float *x = a.x + (size_t)p.q0 * a.x_stride + c0;
-    float w[4][W], bias[4] = {0.0f, 0.0f, 0.0f, 0.0f}, row[W][4];
-#pragma unroll
-    for (int i = 0; i < 4; ++i)
-#pragma unroll
-        for (int j = 0; j < W; ++j) w[i][j] = i < (int)take ? a.weight[(size_t)(c0 + i) * W + j] : 0.0f;
-    if (a.bias) load4(bias, a.bias + c0, take);
-    // rows before the tile: of the sequence, or of the state (row W - 1 - j of it stands j places before the first token)
-    const float *old = a.state + (size_t)(p.from < 0 ? 0 : p.from) * (W - 1) * a.n_ch + c0;
-    auto before = [&](float *v, int64_t t) {  // row t of the sequence, t >= 1 - W
-        if (t >= 0) load4(v, x + (size_t)t * a.x_stride, take);
-        else if (p.from >= 0) load4(v, old + (size_t)(W - 1 + t) * a.n_ch, take);
-        else
-#pragma unroll
-            for (int i = 0; i < 4; ++i) v[i] = 0.0f;
-    };
-#pragma unroll
-    for (int j = 0; j < W - 1; ++j) before(row[j], (int64_t)t0 - (W - 1) + j);
-    float kept[W - 1][4];
-    const bool keep = n == 0 && p.to >= 0;
-    if (keep) {
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) before(kept[j], (int64_t)p.nq - (W - 1) + j);
-    }
-    float *y = a.y + (size_t)p.q0 * a.y_stride + c0;
-    bool odd = false;
-    for (uint32_t t = t0; t < t1; ++t) {
-        load4(row[W - 1], x + (size_t)t * a.x_stride, take);
-        float out[4];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float v = bias[i];
-#pragma unroll
-            for (int j = 0; j < W; ++j) v = __builtin_fmaf(w[i][j], row[j][i], v);
-            odd = odd || !finite(v);
-            out[i] = a.silu ? v / (1.0f + expf(-v)) : v;
-        }
-        store4(y + (size_t)t * a.y_stride, out, take);
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j)
-#pragma unroll
-            for (int i = 0; i < 4; ++i) row[j][i] = row[j + 1][i];
-    }
-    if (keep) {
-        float *to = a.state + (size_t)p.to * (W - 1) * a.n_ch + c0;
-#pragma unroll
-        for (int j = 0; j < W - 1; ++j) store4(to + (size_t)j * a.n_ch, kept[j], take);
-    }
-    if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
 }
 
 // ---- the gated delta rule ----------------------------------------------------------------------------

@@ -506,7 +506,8 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
  * may be the same one; several sequences may begin from one slot.  A slot that a sequence writes may not be another's
  * d_from or d_to: what those then hold or begin from is unspecified.  A sequence without tokens hands its state on.  A sequence
  * whose tokens or slots are out of range is refused with AH_ERR_CACHE_RANGE and passed over; tokens of no sequence are not
- * written.  Rows are *_stride floats apart, and outputs may not overlap inputs.  At most 65535 sequences.  A result that is
+ * written.  Rows are *_stride floats apart (outputs' and the convolution's at most 2^23), and outputs may not overlap inputs.
+ * At most 65535 sequences.  A result that is
  * not finite is refused with AH_ERR_NONFINITE_INPUT (ah_sync_status): the outputs and state of its sequence and head or
  * channel, from its chunk of 64 tokens on, hold no values then. */
 typedef struct ah_state_seqs {
