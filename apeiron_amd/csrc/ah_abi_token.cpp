@@ -507,10 +507,14 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     a.block_shift = b.shift - 5;
     b.most = (uint32_t)all;
     b.lds_keys = (uint32_t)(all < kLdsKeys ? all : kLdsKeys);
+    // A few tokens of a sequence and more are chosen for together, where 16 tokens' scores fit LDS.
+    const bool together = a.max_q >= 4 && 16 * (a.c.dim + 2 + all + 1) <= kLdsKeys;
+    b.tiles = together ? a.n_tok / 16 + a.n_seq : 0;
+    if ((size_t)b.tiles * a.c.n_kv > max_grid(1024) || (!together && units > max_grid(1024))) return AH_ERR_INVALID_ARG;
     const size_t keys_at = align256(units * a.list_stride * sizeof(uint32_t)), kept = keys_at + (all > kLdsKeys ? align256(units * all * sizeof(uint64_t)) : 0);
     AttnArgs rows = a;
     rows.n_seq = a.n_tok;  // every token for itself
-    rows.max_q = 1;
+    rows.seqs = together ? a.n_seq : 0;
     const int32_t st = attn_rows_plan(ctx, rows, entries << a.block_shift, a.group, kept, stream);
     if (st) return st;
     b.list = static_cast<uint32_t *>(ctx->scratch.p);

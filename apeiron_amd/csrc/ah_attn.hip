@@ -96,7 +96,16 @@ template <int MODE> AH_DEV Span span_in(const AttnArgs &a, uint32_t s, uint32_t 
     if (MODE == kPrefix) return {0, a.n_tok, (int32_t)a.first_key, false};
     if (MODE == kBlocks) {  // [0] of a list: its keys, kNoList where the token is no sequence's
         const uint32_t keys = a.list[((size_t)s * a.c.n_kv + kvh) * a.list_stride];
-        return {s, keys == kNoList ? 0u : 1u, keys == kNoList ? 0 : (int32_t)keys, keys == kNoList};
+        bool none = a.seqs == 0 && keys == kNoList;
+        if (a.seqs) {
+            none = true;
+            for (uint32_t base = 0; none && base < a.seqs; base += 64) {
+                const uint32_t i = base + (threadIdx.x & 63);
+                const Span p = span_of(a, i < a.seqs ? i : 0);
+                none = !__builtin_amdgcn_ballot_w64(i < a.seqs && s >= p.q0 && s - p.q0 < p.nq);
+            }
+        }
+        return {s, none ? 0u : 1u, none ? 0 : (int32_t)keys, none};
     }
     Span p = span_of(a, s);
     if (MODE == kAfter && !p.bad && (uint32_t)(p.ctx - (int32_t)p.nq) < a.first_key) p = {0, 0, 0, true};

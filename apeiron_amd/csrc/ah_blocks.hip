@@ -31,6 +31,7 @@ template <int D> __global__ void __launch_bounds__(256) block_means_kernel(Means
     const uint32_t in = (uint32_t)pos & ((1u << a.c.page_shift) - 1), first = in + 1 - len;  // of the page's positions
     for (uint32_t h = threadIdx.x >> 6; h < a.c.n_kv; h += blockDim.x >> 6) {
         double sum[8] = {};
+#pragma unroll 8
         for (uint32_t i = ph; i < len; i += P) {
             const uint32_t at = first + i, t = at & 31;
             const uint8_t *tile = a.c.base + kv4_tile(a.c, page, h, at >> 5);
@@ -57,26 +58,160 @@ template <int D> __global__ void __launch_bounds__(256) block_means_kernel(Means
 
 // ---- the choice --------------------------------------------------------------------------------------
 //
-// A workgroup for a (token, KV head).  The query at position p of block b reads the blocks 0 .. first - 1, b - last .. b
-// and, of those between, the `top` of the highest score scale sum_h q_h . mean (h over the KV head's queries; of equal ones
-// the first).  Scores are f64: the order of two blocks is the formula's, not the rounding's.  They are ranked as whole
-// numbers of the same order; the top-th is found bit by bit from the highest one in which any two differ.
-
+// The query at position p of block b reads the blocks 0 .. first - 1, b - last .. b and, of those between, the `top` of the
+// highest score scale sum_h q_h . mean (h over the KV head's queries; of equal ones the first).  Scores are f64: the order of two
+// blocks is the formula's, not the rounding's.  They are ranked as whole numbers of the same order.
 AH_DEV uint64_t rank_of(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);  // (-0 is 0)
     return v != v ? 0 : b >> 63 ? ~b : b | 1ull << 63;
 }
+AH_DEV uint32_t count(bool x) { return (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x)); }
+AH_DEV uint32_t before(bool x) {  // lanes below this one where x is true
+    const uint64_t m = __builtin_amdgcn_ballot_w64(x);
+    return __builtin_amdgcn_mbcnt_hi((uint32_t)(m >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)m, 0));
+}
+// The largest T with at least `top` keys >= T, bit by bit: many(x) counts the keys >= x; found: how many are >= T.  As soon as
+// those are just `top`, the rest of the bits does not matter.
+template <class F> AH_DEV uint64_t threshold(uint32_t top, uint32_t n, F many, uint32_t &found) {
+    uint64_t T = 0;
+    found = n;
+    for (int bit = 63; bit >= 0 && found != top; --bit) {
+        const uint32_t c = many(T | 1ull << bit);
+        if (c >= top) {
+            T |= 1ull << bit;
+            found = c;
+        }
+    }
+    return T;
+}
 
-template <int D> __global__ void __launch_bounds__(256) block_choice_kernel(BlockArgs b) {
-    constexpr uint32_t L = D / 8, kPer = 64 / L, kAhead = 4;  // lanes of a block's mean, blocks of a wave
-    extern __shared__ uint64_t lds_keys[];  // [b.lds_keys]
-    __shared__ uint64_t red[2][4];
-    __shared__ uint32_t cnt[2][4], cnt2[2][4];
+AH_DEV void record_bad(const BlockArgs &b, uint32_t at, uint32_t of) {  // sequences out of range: every of-th from at on
+    for (uint32_t i = at; i < b.a.n_seq; i += of)
+        if (span_of(b.a, i).bad) ah_record(b.a.status, ((unsigned long long)i << 8) + kKeyCache);
+}
+
+// What a (token, KV head) reads and where it stands in the cache.
+struct Query {
+    uint32_t s, own, n;  // its sequence and block; blocks to choose among, from b.first on
+    int32_t pos;
+};
+AH_DEV Query query_of(const BlockArgs &b, const Span &p, uint32_t s, uint32_t tok) {
+    Query x;
+    x.s = s;
+    x.pos = p.ctx - (int32_t)p.nq + (int32_t)(tok - p.q0);
+    x.own = x.pos < 0 ? 0 : (uint32_t)x.pos >> b.shift;
+    x.n = x.own > b.first + (uint64_t)b.last ? x.own - b.last - b.first : 0;
+    return x;
+}
+AH_DEV uint32_t page_of(const BlockArgs &b, uint32_t s, uint32_t block) {
+    return (uint32_t)b.a.table[(size_t)s * b.a.table_stride + (block >> (b.a.c.page_shift - b.shift))];
+}
+AH_DEV size_t mean_at(const BlockArgs &b, uint32_t page, uint32_t kvh, uint32_t block) {  // the place of a block's mean, in heads
+    const uint32_t per = b.a.c.page_shift - b.shift;
+    return (((size_t)page << per) + (block & ((1u << per) - 1))) * b.a.c.n_kv + kvh;
+}
+// A block's first tile, as attention's list has it.
+AH_DEV uint32_t entry_of(const BlockArgs &b, uint32_t s, uint32_t kvh, uint32_t block) {
+    const Kv4Ref &c = b.a.c;
+    const uint32_t page = page_of(b, s, block), per = c.page_shift - b.shift;
+    if (page >= c.n_pages) {
+        ah_record(b.a.status, ((unsigned long long)s << 8) + kKeyCache);
+        return kNoList;
+    }
+    return ((page * c.n_kv + kvh) << (c.page_shift - 5)) + ((block & ((1u << per) - 1)) << (b.shift - 5));
+}
+// What a query reads without a choice, by `lanes` lanes; true where that is all.
+AH_DEV bool list_fixed(const BlockArgs &b, const Query &x, uint32_t kvh, uint32_t *list, int32_t *chosen, uint32_t lane, uint32_t lanes) {
+    if (x.n <= b.top) {
+        const uint32_t all = x.pos < 0 ? 0 : x.own + 1;
+        for (uint32_t i = lane; i < all; i += lanes) list[1 + i] = entry_of(b, x.s, kvh, i);
+        if (lane == 0) list[0] = (uint32_t)(x.pos + 1);
+        if (chosen)
+            for (uint32_t i = lane; i < b.top; i += lanes) chosen[i] = i < x.n ? (int32_t)(b.first + i) : -1;
+        return true;
+    }
+    for (uint32_t i = lane; i < b.first; i += lanes) list[1 + i] = entry_of(b, x.s, kvh, i);
+    for (uint32_t i = lane; i <= b.last; i += lanes) list[1 + b.first + b.top + i] = entry_of(b, x.s, kvh, x.own - b.last + i);
+    if (lane == 0) list[0] = ((b.first + b.top + b.last) << b.shift) + ((uint32_t)x.pos & ((1u << b.shift) - 1)) + 1;
+    return false;
+}
+
+// The choice among n > top keys by one wave: emit(place, block) for the chosen ones, ascending.  With top at most 64, the top-th of
+// the lanes' largest keys bounds the top-th of all from below, and few keys pass it; where no more than 64 do, a lane each,
+// the rest is ballots.  false: it is left to many_keys.
+template <class K, class E> AH_DEV bool few_keys(uint32_t n, uint32_t top, uint64_t *room, K key_at, E emit) {
+    if (top > 64) return false;
+    const uint32_t lane = threadIdx.x & 63;
+    uint64_t most = 0;
+    for (uint32_t i = lane; i < n; i += 64) {
+        const uint64_t k = key_at(i);
+        most = k > most ? k : most;
+    }
+    uint32_t found;
+    const uint64_t bound = threshold(top, 64, [&](uint64_t x) { return count(most >= x); }, found);
+    uint32_t c = 0;
+    for (uint32_t base = 0; base < n; base += 64) {
+        const uint64_t k = base + lane < n ? key_at(base + lane) : 0;
+        const bool in = base + lane < n && k >= bound;
+        const uint32_t at = c + before(in);
+        if (in && at < 64) {
+            room[at] = k;
+            room[64 + at] = base + lane;
+        }
+        c += count(in);
+    }
+    if (c > 64) return false;
+    __builtin_amdgcn_wave_barrier();
+    const uint64_t k = lane < c ? room[lane] : 0;
+    const uint64_t T = threshold(top, c, [&](uint64_t x) { return count(lane < c && k >= x); }, found);
+    const bool above = lane < c && k > T, same = lane < c && k == T;
+    const uint32_t ties = top - count(above);
+    const bool in = above || (same && before(same) < ties);
+    if (in) emit(before(in), (uint32_t)room[64 + lane]);
+    return true;
+}
+// Any n and top, `waves` waves together (one: no barriers): many(x) counts the keys >= x over all of them.
+template <class K, class E, class M> AH_DEV void many_keys(uint32_t n, uint32_t top, K key_at, E emit, M many) {
+    uint32_t found;
+    const uint64_t T = threshold(top, n, many, found);
+    const uint32_t above = found == top || T == ~0ull ? 0 : many(T + 1);
+    const uint32_t lane = threadIdx.x & 63, ties = top - above;
+    uint32_t gt = 0, eq = 0;
+    for (uint32_t base = 0; base < n; base += 64) {
+        const uint64_t k = base + lane < n ? key_at(base + lane) : 0;
+        const bool x = base + lane < n && found != top && k > T, y = base + lane < n && (found == top ? k >= T : k == T);
+        const uint32_t g = gt + before(x), e = eq + before(y);
+        if (x || (y && e < ties)) emit(g + (e < ties ? e : ties), base + lane);
+        gt += count(x);
+        eq += count(y);
+    }
+}
+
+// A workgroup of 16 waves for a (token, KV head).  Scores: D / 8 lanes a block, eight channels each, the means of four blocks a
+// lane on their way.
+constexpr uint32_t kOneThreads = 1024;
+template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_kernel(BlockArgs b) {
+    constexpr uint32_t L = D / 8, kPer = 64 / L, kWaves = kOneThreads / 64, kAhead = 4;  // lanes of a block's mean, blocks of a wave
+    extern __shared__ uint64_t lds_keys[];                                              // [b.lds_keys]
+    __shared__ uint64_t room[128];
+    __shared__ uint32_t cnt[2][kWaves], done;
     const AttnArgs &a = b.a;
     const uint32_t unit = blockIdx.x, tok = unit / a.c.n_kv, kvh = unit - tok * a.c.n_kv, tid = threadIdx.x, lane = tid & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6);
-    for (uint32_t i = unit * 256 + tid; i < a.n_seq; i += gridDim.x * 256)
-        if (span_of(a, i).bad) ah_record(a.status, ((unsigned long long)i << 8) + kKeyCache);
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane % L;
+    // q's sum over the heads, before the sequence is known
+    double q[8] = {};
+    {
+        const float *x = a.q + (size_t)tok * a.q_stride + (size_t)kvh * a.group * D + 8 * g;
+#pragma unroll 4
+        for (uint32_t h = 0; h < a.group; ++h) {
+            float v[8];
+            __builtin_memcpy(v, x + (size_t)h * D, 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) q[i] += (double)v[i];
+        }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] *= (double)a.scale;
+    }
     auto start = [&](uint32_t i) { return (uint32_t)a.q_start[i]; };
     auto holds = [&](uint32_t i) {
         const Span p = span_of(a, i);
@@ -88,149 +223,152 @@ template <int D> __global__ void __launch_bounds__(256) block_choice_kernel(Bloc
     int32_t *chosen = b.chosen ? b.chosen + (size_t)unit * b.top : nullptr;
     if (tok < p.q0 || tok - p.q0 >= p.nq) {
         if (tid == 0) list[0] = kNoList;
+        if (tid == 0) record_bad(b, unit, gridDim.x);
         return;
     }
-    const int32_t pos = p.ctx - (int32_t)p.nq + (int32_t)(tok - p.q0);
-    const uint32_t own = pos < 0 ? 0 : (uint32_t)pos >> b.shift;
-    const uint32_t n = own > b.first + (uint64_t)b.last ? own - b.last - b.first : 0;  // blocks to choose among, from b.first on
-    const uint32_t per = a.c.page_shift - b.shift;                                     // (log2) blocks of a page
-    const int32_t *table = a.table + (size_t)s * a.table_stride;
-    auto page_of = [&](uint32_t block) { return (uint32_t)table[block >> per]; };
-    auto entry = [&](uint32_t block) {
-        const uint32_t page = page_of(block);
-        if (page >= a.c.n_pages) {
-            ah_record(a.status, ((unsigned long long)s << 8) + kKeyCache);
-            return kNoList;
-        }
-        return ((page * a.c.n_kv + kvh) << (a.c.page_shift - 5)) + ((block & ((1u << per) - 1)) << (b.shift - 5));
-    };
-    if (n <= b.top) {  // all of them
-        const uint32_t all = pos < 0 ? 0 : own + 1;
-        for (uint32_t i = tid; i < all; i += 256) list[1 + i] = entry(i);
-        if (tid == 0) list[0] = pos < 0 ? 0 : (uint32_t)pos + 1;
-        if (chosen)
-            for (uint32_t i = tid; i < b.top; i += 256) chosen[i] = i < n ? (int32_t)(b.first + i) : -1;
-        return;
-    }
+    const Query x = query_of(b, p, s, tok);
+    const uint32_t n = x.n;
     const bool in_lds = n <= b.lds_keys;
     uint64_t *far = b.keys + (size_t)unit * b.most;
     auto key_at = [&](uint32_t i) { return in_lds ? lds_keys[i] : far[i]; };
-
-    // scores: L lanes a block, eight channels each
-    const uint32_t g = lane % L, first = wave * kPer + lane / L;
-    double q[8] = {};
-    {
-        const float *x = a.q + (size_t)tok * a.q_stride + (size_t)kvh * a.group * D + 8 * g;
-        for (uint32_t h = 0; h < a.group; ++h) {
-            float v[8];
-            __builtin_memcpy(v, x + (size_t)h * D, 32);
+    auto emit = [&](uint32_t at, uint32_t i) {
+        list[1 + b.first + at] = entry_of(b, s, kvh, b.first + i);
+        if (chosen) chosen[at] = (int32_t)(b.first + i);
+    };
+    if (n > b.top) {
+        const uint32_t first = wave * kPer + lane / L, step = kWaves * kPer;
+        for (uint32_t base = 0; base < n; base += step * kAhead) {
+            f16x8 m[kAhead];
+            uint32_t page[kAhead];
 #pragma unroll
-            for (int i = 0; i < 8; ++i) q[i] += (double)v[i];
-        }
+            for (uint32_t j = 0; j < kAhead; ++j) {
+                const uint32_t i = base + j * step + first;
+                page[j] = page_of(b, s, b.first + (i < n ? i : n - 1));
+            }
 #pragma unroll
-        for (int i = 0; i < 8; ++i) q[i] *= (double)a.scale;
-    }
-    uint64_t any = 0, every = ~0ull;
-    for (uint32_t base = 0; base < n; base += 4 * kPer * kAhead) {
-        f16x8 m[kAhead];
-        bool ok[kAhead];
+            for (uint32_t j = 0; j < kAhead; ++j) {
+                const uint32_t i = base + j * step + first;
+                __builtin_memcpy(&m[j], b.means + mean_at(b, page[j] < a.c.n_pages ? page[j] : 0, kvh, b.first + (i < n ? i : n - 1)) * D + 8 * g, 16);
+            }
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; ++j) {
-            const uint32_t i = base + j * 4 * kPer + first, block = b.first + (i < n ? i : n - 1);
-            const uint32_t page = page_of(block);
-            ok[j] = page < a.c.n_pages;
-            const size_t at = ((size_t)(ok[j] ? page : 0) << per) + (block & ((1u << per) - 1));
-            __builtin_memcpy(&m[j], b.means + (at * a.c.n_kv + kvh) * D + 8 * g, 16);
-        }
+            for (uint32_t j = 0; j < kAhead; ++j) {
+                const uint32_t i = base + j * step + first;
+                double v = 0.0;
 #pragma unroll
-        for (uint32_t j = 0; j < kAhead; ++j) {
-            const uint32_t i = base + j * 4 * kPer + first;
-            double v = 0.0;
+                for (int c = 0; c < 8; ++c) v = __builtin_fma(q[c], (double)(float)m[j][c], v);
 #pragma unroll
-            for (int c = 0; c < 8; ++c) v = __builtin_fma(q[c], (double)(float)m[j][c], v);
-#pragma unroll
-            for (uint32_t o = 1; o < L; o <<= 1) v += __shfl_xor(v, (int)o, 64);
-            const uint64_t key = ok[j] ? rank_of(v) : 0;
-            if (i < n) {
-                if (g == 0) {
+                for (uint32_t o = 1; o < L; o <<= 1) v += __shfl_xor(v, (int)o, 64);
+                const uint64_t key = page[j] < a.c.n_pages ? rank_of(v) : 0;
+                if (i < n && g == 0) {
                     if (in_lds) lds_keys[i] = key;
                     else far[i] = key;
                 }
-                any |= key;
-                every &= key;
             }
         }
+        __syncthreads();
+        if (wave == 0) {
+            const bool all = few_keys(n, b.top, room, key_at, emit);
+            if (lane == 0) done = all;
+        }
     }
-#pragma unroll
-    for (uint32_t o = L; o < 64; o <<= 1) {
-        any |= __shfl_xor(any, (int)o, 64);
-        every &= __shfl_xor(every, (int)o, 64);
+    if (wave == 1) {
+        (void)list_fixed(b, x, kvh, list, chosen, lane, 64);
+        if (lane == 0) record_bad(b, unit, gridDim.x);
     }
-    if (lane == 0) {
-        red[0][wave] = any;
-        red[1][wave] = every;
-    }
+    if (n <= b.top) return;
     __syncthreads();
-    any = red[0][0] | red[0][1] | red[0][2] | red[0][3];
-    every = red[1][0] & red[1][1] & red[1][2] & red[1][3];
+    if (done) return;
     uint32_t turn = 0;
-    auto count = [&](uint64_t at_least) {  // keys >= at_least
+    auto many = [&](uint64_t at_least) {
         uint32_t c = 0;
-        for (uint32_t i = tid; i < n; i += 256) c += key_at(i) >= at_least;
-#pragma unroll
-        for (uint32_t o = 1; o < 64; o <<= 1) c += (uint32_t)__shfl_xor((int)c, (int)o, 64);
+        for (uint32_t base = 64 * wave; base < n; base += kOneThreads) c += count(base + lane < n && key_at(base + lane) >= at_least);
         if (lane == 0) cnt[turn][wave] = c;
         __syncthreads();
-        c = cnt[turn][0] + cnt[turn][1] + cnt[turn][2] + cnt[turn][3];
+        c = 0;
+#pragma unroll
+        for (uint32_t w = 0; w < kWaves; ++w) c += cnt[turn][w];
         turn ^= 1;
         return c;
     };
-    // the largest T with at least `top` keys >= T
-    uint64_t T = every;
-    uint32_t found = n;
-    if (any != every) {
-        int bit = 63 - __builtin_clzll(any ^ every);
-        T = every & ~((2ull << bit) - 1);
-        for (; bit >= 0 && found != b.top; --bit) {
-            const uint64_t to = T | 1ull << bit;
-            const uint32_t c = count(to);
-            if (c >= b.top) {
-                T = to;
-                found = c;
-            }
-        }
-    }
-    const uint32_t above = found == b.top ? 0 : T == ~0ull ? 0 : count(T + 1), ties = found == b.top ? b.top : b.top - above;
-    // keys above T, and the first `ties` that equal it (all from T on, where there are just as many)
-    uint32_t gt0 = 0, eq0 = 0;
-    for (uint32_t base = 0; base < n; base += 256) {
-        const uint32_t i = base + tid;
-        const uint64_t key = i < n ? key_at(i) : 0;
-        const bool gt = i < n && found != b.top && key > T, eq = i < n && (found == b.top ? key >= T : key == T);
-        const uint64_t bg = __builtin_amdgcn_ballot_w64(gt), be = __builtin_amdgcn_ballot_w64(eq), below = (1ull << lane) - 1;
-        if (lane == 0) {
-            cnt[turn][wave] = (uint32_t)__builtin_popcountll(bg);
-            cnt2[turn][wave] = (uint32_t)__builtin_popcountll(be);
+    many_keys(n, b.top, key_at, [&](uint32_t at, uint32_t i) {
+        if (wave == 0) emit(at, i);
+    }, many);
+}
+
+// A workgroup for 16 tokens of a sequence and a KV head: scores of 16 blocks and the 16 tokens by f64 matrix products (lane
+// (r, h): token r, blocks h + 4 i of the result), then a token's choice by one wave.
+constexpr uint32_t kSomeWaves = 8;
+template <int D> __global__ void __launch_bounds__(64 * kSomeWaves) block_choices_kernel(BlockArgs b) {
+    typedef double f64x4 __attribute__((ext_vector_type(4)));
+    constexpr int Q = D / 4;  // channels of a lane's quarter
+    extern __shared__ uint64_t lds[];
+    __shared__ uint64_t room[kSomeWaves][128];
+    const AttnArgs &a = b.a;
+    const uint32_t at = blockIdx.x / a.c.n_kv, kvh = blockIdx.x - at * a.c.n_kv, lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    double *qs = reinterpret_cast<double *>(lds);  // [16][D + 2]
+    uint64_t *keys = lds + 16 * (D + 2);           // [16][stride]
+    const uint32_t stride = b.lds_keys + 1;
+    if (kvh == 0 && threadIdx.x == 0) record_bad(b, at, b.tiles);
+    auto start = [&](uint32_t i) { return (uint32_t)a.q_start[i] / 16 + i; };
+    auto holds = [&](uint32_t i) {
+        const Span p = span_of(a, i);
+        return at >= start(i) && at - start(i) < (p.nq + 15) / 16;
+    };
+    const uint32_t s = sequence_of(a, at, start, holds);
+    const Span p = span_of(a, s);
+    const uint32_t tile = at - start(s);
+    if (tile >= (p.nq + 15) / 16) return;
+    const uint32_t tok0 = p.q0 + 16 * tile, live = p.nq - 16 * tile < 16 ? p.nq - 16 * tile : 16;
+    const uint32_t most = query_of(b, p, s, tok0 + live - 1).n;  // (the last token's: the most)
+    if (most > b.top) {
+        for (uint32_t i = threadIdx.x; i < 16 * D; i += 64 * kSomeWaves) {
+            const uint32_t t = i / D, c = i % D;
+            const float *x = a.q + (size_t)(tok0 + (t < live ? t : 0)) * a.q_stride + (size_t)kvh * a.group * D + c;
+            double v = 0.0;
+#pragma unroll 8
+            for (uint32_t g = 0; g < a.group; ++g) v += (double)x[(size_t)g * D];
+            qs[t * (D + 2) + c] = v * (double)a.scale;
         }
         __syncthreads();
-        uint32_t g_at = gt0 + (uint32_t)__builtin_popcountll(bg & below), e_at = eq0 + (uint32_t)__builtin_popcountll(be & below);
+        double q[Q];
 #pragma unroll
-        for (uint32_t w = 0; w < 4; ++w) {
-            g_at += w < wave ? cnt[turn][w] : 0;
-            e_at += w < wave ? cnt2[turn][w] : 0;
-            gt0 += cnt[turn][w];
-            eq0 += cnt2[turn][w];
+        for (int i = 0; i < Q; ++i) q[i] = qs[r * (D + 2) + h * Q + i];
+        for (uint32_t base = 16 * wave; base < most; base += 16 * kSomeWaves) {
+            const uint32_t i = base + r, block = b.first + (i < most ? i : most - 1), page = page_of(b, s, block);
+            const bool ok = page < a.c.n_pages;
+            _Float16 m[Q];
+            __builtin_memcpy(m, b.means + mean_at(b, ok ? page : 0, kvh, block) * D + h * Q, 2 * Q);
+            f64x4 v = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+            for (int c = 0; c < Q; ++c) v = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)m[c], q[c], v, 0, 0, 0);
+            const uint32_t good = (uint32_t)__builtin_amdgcn_ballot_w64(ok);  // of the blocks: lanes 0 to 15
+#pragma unroll
+            for (int n = 0; n < 4; ++n) {
+                const uint32_t j = h + 4 * n;
+                if (base + j < most) keys[r * stride + base + j] = good >> j & 1 ? rank_of(v[n]) : 0;
+            }
         }
-        turn ^= 1;
-        if (gt || (eq && e_at < ties)) {
-            const uint32_t at = g_at + (e_at < ties ? e_at : ties);
-            list[1 + b.first + at] = entry(b.first + i);
-            if (chosen) chosen[at] = (int32_t)(b.first + i);
-        }
+        __syncthreads();
     }
-    for (uint32_t i = tid; i < b.first; i += 256) list[1 + i] = entry(i);
-    for (uint32_t i = tid; i <= b.last; i += 256) list[1 + b.first + b.top + i] = entry(own - b.last + i);
-    if (tid == 0) list[0] = ((b.first + b.top + b.last) << b.shift) + ((uint32_t)pos & ((1u << b.shift) - 1)) + 1;
+    for (uint32_t t = wave; t < live; t += kSomeWaves) {
+        const uint32_t tok = tok0 + t, unit = tok * a.c.n_kv + kvh;
+        const Query x = query_of(b, p, s, tok);
+        uint32_t *list = b.list + (size_t)unit * a.list_stride;
+        int32_t *chosen = b.chosen ? b.chosen + (size_t)unit * b.top : nullptr;
+        if (list_fixed(b, x, kvh, list, chosen, lane, 64)) continue;
+        auto key_at = [&](uint32_t i) { return keys[t * stride + i]; };
+        auto emit = [&](uint32_t to, uint32_t i) {
+            list[1 + b.first + to] = entry_of(b, s, kvh, b.first + i);
+            if (chosen) chosen[to] = (int32_t)(b.first + i);
+        };
+        if (few_keys(x.n, b.top, room[wave], key_at, emit)) continue;
+        many_keys(x.n, b.top, key_at, emit, [&](uint64_t at_least) {
+            uint32_t c = 0;
+            for (uint32_t i = lane; i < (x.n + 63) / 64 * 64; i += 64) c += count(i < x.n && key_at(i) >= at_least);
+            return c;
+        });
+    }
 }
 
 } // namespace
@@ -243,19 +381,26 @@ hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream) {
     return hipGetLastError();
 }
 
+template <int D> void launch_choice(const BlockArgs &a, hipStream_t stream) {
+    if (!a.tiles) {
+        hipLaunchKernelGGL(block_choice_kernel<D>, dim3(a.a.n_tok * a.a.c.n_kv), dim3(kOneThreads), a.lds_keys * sizeof(uint64_t), stream, a);
+        return;
+    }
+    hipLaunchKernelGGL(block_choices_kernel<D>, dim3(a.tiles * a.a.c.n_kv), dim3(64 * kSomeWaves), 16 * (D + 2 + a.lds_keys + 1) * sizeof(uint64_t), stream, a);
+}
+
 hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream) {
-    const dim3 grid(a.a.n_tok * a.a.c.n_kv), block(256);
-    const size_t lds = a.lds_keys * sizeof(uint64_t);
-    if (a.a.c.dim == 64) hipLaunchKernelGGL(block_choice_kernel<64>, grid, block, lds, stream, a);
-    else if (a.a.c.dim == 128) hipLaunchKernelGGL(block_choice_kernel<128>, grid, block, lds, stream, a);
-    else hipLaunchKernelGGL(block_choice_kernel<256>, grid, block, lds, stream, a);
+    if (a.a.c.dim == 64) launch_choice<64>(a, stream);
+    else if (a.a.c.dim == 128) launch_choice<128>(a, stream);
+    else launch_choice<256>(a, stream);
     return hipGetLastError();
 }
 
 hipError_t ah_blocks_init_attrs() {
     const int most = (int)(kLdsKeys * sizeof(uint64_t));
     hipError_t e = hipSuccess;
-    for (const void *k : {(const void *)block_choice_kernel<64>, (const void *)block_choice_kernel<128>, (const void *)block_choice_kernel<256>})
+    for (const void *k : {(const void *)block_choice_kernel<64>, (const void *)block_choice_kernel<128>, (const void *)block_choice_kernel<256>,
+                          (const void *)block_choices_kernel<64>, (const void *)block_choices_kernel<128>, (const void *)block_choices_kernel<256>})
         if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, most);
     return e;
 }

@@ -138,6 +138,7 @@ struct AttnArgs {
     // tiles (kv4_tile's, counted; kNoList: none to see) of its blocks of 1 << block_shift tiles
     const uint32_t *list;
     uint32_t list_stride, block_shift;
+    uint32_t seqs;  // where tokens of no sequence have no list: the sequences to look a token up among (n_seq: the tokens)
 };
 constexpr uint32_t kNoList = 0xffffffffu;
 constexpr uint32_t kLdsKeys = 16384;  // scores of a query's blocks that the choice keeps in LDS, at most
@@ -151,6 +152,7 @@ struct BlockArgs {
     int32_t *chosen;
     uint64_t *keys;  // [token, KV head][most]: the scores' ranks, where they do not fit LDS
     uint32_t most, lds_keys;
+    uint32_t tiles;  // numbers of groups of 16 tokens of a sequence, chosen for together; 0: every token by itself
 };
 struct MeansArgs {
     Kv4Ref c;
