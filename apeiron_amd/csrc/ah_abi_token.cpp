@@ -512,16 +512,25 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     b.tiles = together ? a.n_tok / 16 + a.n_seq : 0;
     if ((size_t)b.tiles * a.c.n_kv > max_grid(1024) || (!together && units > max_grid(1024))) return AH_ERR_INVALID_ARG;
     const size_t keys_at = align256(units * a.list_stride * sizeof(uint32_t)), kept = keys_at + (all > kLdsKeys ? align256(units * all * sizeof(uint64_t)) : 0);
+    // Up to eight queries a KV head, and lists enough for four waves a CU and more: a wave each.
+    const bool alone = a.group <= 8 && together && units >= 4 * (size_t)ctx->cu_count;
+    a.seqs = together ? a.n_seq : 0;
     AttnArgs rows = a;
-    rows.n_seq = a.n_tok;  // every token for itself
-    rows.seqs = together ? a.n_seq : 0;
-    const int32_t st = attn_rows_plan(ctx, rows, entries << a.block_shift, a.group, kept, stream);
+    int32_t st;
+    if (alone) {
+        AH_HIP(ctx, hipSetDevice(ctx->device));
+        st = ensure_scratch(ctx, kept, stream);
+    } else {
+        rows.n_seq = a.n_tok;  // every token for itself
+        st = attn_rows_plan(ctx, rows, entries << a.block_shift, a.group, kept, stream);
+    }
     if (st) return st;
     b.list = static_cast<uint32_t *>(ctx->scratch.p);
     b.keys = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(ctx->scratch.p) + keys_at);
     rows.list = b.list;
     AH_HIP(ctx, ah_launch_block_choice(b, pick(ctx, stream)));
-    AH_HIP(ctx, ah_launch_attn_blocks(rows, pick(ctx, stream)));
+    if (alone) AH_HIP(ctx, ah_launch_attend_lists(rows, pick(ctx, stream)));
+    else AH_HIP(ctx, ah_launch_attn_blocks(rows, pick(ctx, stream)));
     return AH_OK;
 }
 

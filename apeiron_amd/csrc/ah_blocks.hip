@@ -4,8 +4,6 @@
 
 namespace {
 
-typedef _Float16 f16x8 __attribute__((ext_vector_type(8)));
-
 constexpr unsigned long long kKeyCache = AH_ERR_CACHE_RANGE;
 
 // ---- means -----------------------------------------------------------------------------------------
@@ -64,6 +62,12 @@ template <int D> __global__ void __launch_bounds__(256) block_means_kernel(Means
 AH_DEV uint64_t rank_of(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);  // (-0 is 0)
     return v != v ? 0 : b >> 63 ? ~b : b | 1ull << 63;
+}
+template <int CTRL> AH_DEV double dpp64(double v) {
+    const uint64_t b = __builtin_bit_cast(uint64_t, v);
+    const uint32_t lo = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)b, CTRL, 0xF, 0xF, true);
+    const uint32_t hi = (uint32_t)__builtin_amdgcn_update_dpp(0, (int)(uint32_t)(b >> 32), CTRL, 0xF, 0xF, true);
+    return __builtin_bit_cast(double, (uint64_t)hi << 32 | lo);
 }
 AH_DEV uint32_t count(bool x) { return (uint32_t)__builtin_popcountll(__builtin_amdgcn_ballot_w64(x)); }
 AH_DEV uint32_t before(bool x) {  // lanes below this one where x is true
@@ -140,31 +144,45 @@ AH_DEV bool list_fixed(const BlockArgs &b, const Query &x, uint32_t kvh, uint32_
 // the lanes' largest keys bounds the top-th of all from below, and few keys pass it; where no more than 64 do, a lane each,
 // the rest is ballots.  false: it is left to many_keys.
 template <class K, class E> AH_DEV bool few_keys(uint32_t n, uint32_t top, uint64_t *room, K key_at, E emit) {
+    constexpr uint32_t kBatch = 8;  // keys of a lane on their way
     if (top > 64) return false;
     const uint32_t lane = threadIdx.x & 63;
-    uint64_t most = 0;
-    for (uint32_t i = lane; i < n; i += 64) {
-        const uint64_t k = key_at(i);
-        most = k > most ? k : most;
+    uint64_t most = 0, k[kBatch];
+    auto batch = [&](uint32_t base) {
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t i = base + 64 * j + lane;
+            k[j] = key_at(i < n ? i : n - 1);
+            k[j] = i < n ? k[j] : 0;
+        }
+    };
+    for (uint32_t base = 0; base < n; base += 64 * kBatch) {
+        batch(base);
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) most = k[j] > most ? k[j] : most;
     }
     uint32_t found;
     const uint64_t bound = threshold(top, 64, [&](uint64_t x) { return count(most >= x); }, found);
     uint32_t c = 0;
-    for (uint32_t base = 0; base < n; base += 64) {
-        const uint64_t k = base + lane < n ? key_at(base + lane) : 0;
-        const bool in = base + lane < n && k >= bound;
-        const uint32_t at = c + before(in);
-        if (in && at < 64) {
-            room[at] = k;
-            room[64 + at] = base + lane;
+    for (uint32_t base = 0; base < n; base += 64 * kBatch) {
+        if (n > 64 * kBatch) batch(base);
+#pragma unroll
+        for (uint32_t j = 0; j < kBatch; ++j) {
+            const uint32_t i = base + 64 * j + lane;
+            const bool in = i < n && k[j] >= bound;
+            const uint32_t at = c + before(in);
+            if (in && at < 64) {
+                room[at] = k[j];
+                room[64 + at] = i;
+            }
+            c += count(in);
         }
-        c += count(in);
     }
     if (c > 64) return false;
     __builtin_amdgcn_wave_barrier();
-    const uint64_t k = lane < c ? room[lane] : 0;
-    const uint64_t T = threshold(top, c, [&](uint64_t x) { return count(lane < c && k >= x); }, found);
-    const bool above = lane < c && k > T, same = lane < c && k == T;
+    const uint64_t mine = lane < c ? room[lane] : 0;
+    const uint64_t T = threshold(top, c, [&](uint64_t x) { return count(lane < c && mine >= x); }, found);
+    const bool above = lane < c && mine > T, same = lane < c && mine == T;
     const uint32_t ties = top - count(above);
     const bool in = above || (same && before(same) < ties);
     if (in) emit(before(in), (uint32_t)room[64 + lane]);
@@ -187,22 +205,22 @@ template <class K, class E, class M> AH_DEV void many_keys(uint32_t n, uint32_t 
     }
 }
 
-// A workgroup of 16 waves for a (token, KV head).  Scores: D / 8 lanes a block, eight channels each, the means of four blocks a
-// lane on their way.
-constexpr uint32_t kOneThreads = 1024;
-template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_kernel(BlockArgs b) {
-    constexpr uint32_t L = D / 8, kPer = 64 / L, kWaves = kOneThreads / 64, kAhead = 4;  // lanes of a block's mean, blocks of a wave
-    extern __shared__ uint64_t lds_keys[];                                              // [b.lds_keys]
-    __shared__ uint64_t room[128];
-    __shared__ uint32_t cnt[2][kWaves], done;
+// The choice for a (token, KV head) by a workgroup of W waves, into `list` (as attention's, kNoList where the token is no
+// sequence's).  Scores: D / 8 lanes a block, eight channels each, the means of several blocks a lane on their way.
+template <int W> struct ChoiceLds {
+    uint64_t room[128];
+    uint32_t cnt[2][W], done;
+};
+template <int D, int W> AH_DEV void choose(const BlockArgs &b, uint32_t unit, uint32_t *list, uint64_t *lds_keys, ChoiceLds<W> &L) {
+    constexpr uint32_t kLanes = D / 8, kPer = 64 / kLanes, kAhead = W >= 16 ? 4 : 8;  // lanes of a block's mean, blocks of a wave
     const AttnArgs &a = b.a;
-    const uint32_t unit = blockIdx.x, tok = unit / a.c.n_kv, kvh = unit - tok * a.c.n_kv, tid = threadIdx.x, lane = tid & 63;
-    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane % L;
+    const uint32_t tok = unit / a.c.n_kv, kvh = unit - tok * a.c.n_kv, tid = threadIdx.x, lane = tid & 63;
+    const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane % kLanes;
     // q's sum over the heads, before the sequence is known
     double q[8] = {};
     {
         const float *x = a.q + (size_t)tok * a.q_stride + (size_t)kvh * a.group * D + 8 * g;
-#pragma unroll 4
+#pragma unroll 8
         for (uint32_t h = 0; h < a.group; ++h) {
             float v[8];
             __builtin_memcpy(v, x + (size_t)h * D, 32);
@@ -219,7 +237,6 @@ template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_ker
     };
     const uint32_t s = sequence_of(a, tok, start, holds);
     const Span p = span_of(a, s);
-    uint32_t *list = b.list + (size_t)unit * a.list_stride;
     int32_t *chosen = b.chosen ? b.chosen + (size_t)unit * b.top : nullptr;
     if (tok < p.q0 || tok - p.q0 >= p.nq) {
         if (tid == 0) list[0] = kNoList;
@@ -236,7 +253,7 @@ template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_ker
         if (chosen) chosen[at] = (int32_t)(b.first + i);
     };
     if (n > b.top) {
-        const uint32_t first = wave * kPer + lane / L, step = kWaves * kPer;
+        const uint32_t first = wave * kPer + lane / kLanes, step = W * kPer;
         for (uint32_t base = 0; base < n; base += step * kAhead) {
             f16x8 m[kAhead];
             uint32_t page[kAhead];
@@ -256,8 +273,11 @@ template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_ker
                 double v = 0.0;
 #pragma unroll
                 for (int c = 0; c < 8; ++c) v = __builtin_fma(q[c], (double)(float)m[j][c], v);
-#pragma unroll
-                for (uint32_t o = 1; o < L; o <<= 1) v += __shfl_xor(v, (int)o, 64);
+                v += dpp64<0xB1>(v);   // lanes 1 0 3 2
+                v += dpp64<0x4E>(v);   // lanes 2 3 0 1
+                v += dpp64<0x141>(v);  // the other half of eight, mirrored
+                if (kLanes >= 16) v += dpp64<0x140>(v);  // of sixteen
+                if (kLanes == 32) v += __shfl_xor(v, 16, 64);
                 const uint64_t key = page[j] < a.c.n_pages ? rank_of(v) : 0;
                 if (i < n && g == 0) {
                     if (in_lds) lds_keys[i] = key;
@@ -267,8 +287,8 @@ template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_ker
         }
         __syncthreads();
         if (wave == 0) {
-            const bool all = few_keys(n, b.top, room, key_at, emit);
-            if (lane == 0) done = all;
+            const bool all = few_keys(n, b.top, L.room, key_at, emit);
+            if (lane == 0) L.done = all;
         }
     }
     if (wave == 1) {
@@ -277,22 +297,27 @@ template <int D> __global__ void __launch_bounds__(kOneThreads) block_choice_ker
     }
     if (n <= b.top) return;
     __syncthreads();
-    if (done) return;
+    if (L.done) return;
     uint32_t turn = 0;
     auto many = [&](uint64_t at_least) {
         uint32_t c = 0;
-        for (uint32_t base = 64 * wave; base < n; base += kOneThreads) c += count(base + lane < n && key_at(base + lane) >= at_least);
-        if (lane == 0) cnt[turn][wave] = c;
+        for (uint32_t base = 64 * wave; base < n; base += 64 * W) c += count(base + lane < n && key_at(base + lane) >= at_least);
+        if (lane == 0) L.cnt[turn][wave] = c;
         __syncthreads();
         c = 0;
 #pragma unroll
-        for (uint32_t w = 0; w < kWaves; ++w) c += cnt[turn][w];
+        for (uint32_t w = 0; w < W; ++w) c += L.cnt[turn][w];
         turn ^= 1;
         return c;
     };
     many_keys(n, b.top, key_at, [&](uint32_t at, uint32_t i) {
         if (wave == 0) emit(at, i);
     }, many);
+}
+template <int D> __global__ void __launch_bounds__(1024) block_choice_kernel(BlockArgs b) {
+    extern __shared__ uint64_t lds_keys[];  // [b.lds_keys]
+    __shared__ ChoiceLds<16> L;
+    choose<D, 16>(b, blockIdx.x, b.list + (size_t)blockIdx.x * b.a.list_stride, lds_keys, L);
 }
 
 // A workgroup for 16 tokens of a sequence and a KV head: scores of 16 blocks and the 16 tokens by f64 matrix products (lane
@@ -371,6 +396,155 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves) block_choice
     }
 }
 
+// ---- attention over a list of blocks ---------------------------------------------------------------------
+//
+// attn_rows_kernel's eight packed rows (ah_attn.hip), all of one token: the KV head's queries see the same keys, 0 .. keys - 1 of
+// the listed blocks one after the other, so only the last tile needs a mask.  A wave takes a whole list: with enough of them
+// nobody needs to be met.
+template <int D, class T> AH_DEV void attend_rows(const AttnArgs &a, uint32_t tok, uint32_t kvh, uint32_t keys, T tile_at) {
+    constexpr int NJ = D / 32;
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, row = r & 7;
+    const uint32_t tiles = (keys + 31) / 32;
+    const bool live = row < a.group, low = r >= 8;
+    KTile<D> k;
+    VTile<D> v;
+    bool ok = true;
+    if (tiles) {
+        const uint8_t *t = tile_at(0, ok);
+        k.load(t, r, h);
+        v.load(t, r, h);
+    }
+    f16x8 qh[NJ];
+    float f;
+    {
+        const float *q = a.q + (size_t)tok * a.q_stride + (size_t)(kvh * a.group + (live ? row : 0)) * D + h * (D / 4);
+        float x[NJ][8], top = 0.0f, up;
+#pragma unroll
+        for (int j = 0; j < NJ; ++j) {
+            __builtin_memcpy(x[j], q + 8 * j, 32);
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                x[j][i] = live ? x[j][i] : 0.0f;
+                top = __builtin_fmaxf(top, __builtin_fabsf(x[j][i]));
+            }
+        }
+        top = __builtin_fmaxf(top, xor_lanes(top, 16));
+        top = __builtin_fmaxf(top, xor_lanes(top, 32));
+        q_scale(a.scale, top, up, f);
+#pragma unroll
+        for (int j = 0; j < NJ; ++j)
+#pragma unroll
+            for (int i = 0; i < 8; ++i) {
+                const float y = x[j][i] * up;
+                const _Float16 hv = (_Float16)y;
+                qh[j][i] = low ? (_Float16)(y - (float)hv) : hv;
+            }
+    }
+    f32x4 acc[NJ][2];
+#pragma unroll
+    for (int g = 0; g < NJ; ++g) acc[g][0] = acc[g][1] = (f32x4)0.0f;
+    float m = kNoMax, l = 0.0f;
+    const Masks mk;
+    const float minus_low = low ? -1.0f : 0.0f;
+    for (uint32_t ti = 0; ti < tiles; ++ti) {
+        bool ok_next;
+        const uint8_t *tn = tile_at(ti + 1 < tiles ? ti + 1 : ti, ok_next);
+        f32x4 c[2];
+#pragma unroll
+        for (int half = 0; half < 2; ++half) {
+            c[half] = (f32x4)0.0f;
+#pragma unroll
+            for (int j = 0; j < NJ; ++j) c[half] = mfma16(k_frag(k.code(half, j), k.scale(half, j), mk), qh[j], c[half]);
+        }
+        k.load(tn, r, h);
+        float x[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const float y = c[i >> 2][i & 3];
+            x[i] = y + ror8(y);
+        }
+        if (!ok || 32 * ti + 32 > keys) {
+            const uint32_t end = ok ? keys : 0;
+#pragma unroll
+            for (int i = 0; i < 8; ++i) x[i] = 32 * ti + 16 * (i >> 2) + 4 * h + (i & 3) < end ? x[i] : -__builtin_inff();
+        }
+        float top = x[0];
+#pragma unroll
+        for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
+        top *= f;
+        if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0ull) {
+            top = __builtin_fmaxf(top, xor_lanes(top, 16));
+            top = __builtin_fmaxf(top, xor_lanes(top, 32));
+            const float up = __builtin_fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - up);
+            m = up;
+            l *= alpha;
+#pragma unroll
+            for (int g = 0; g < NJ; ++g) {
+                acc[g][0] *= alpha;
+                acc[g][1] *= alpha;
+            }
+        }
+        const float base = kUp - m;
+        float ls = 0.0f;
+        f16x2 pl[4];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], f, base)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], f, base));
+            ls = i ? ls + e0 : e0;
+            ls += e1;
+            const f16x2 ph = pack16(e0, e1);
+            pl[i] = pack16(__builtin_fmaf((float)ph[0], minus_low, e0), __builtin_fmaf((float)ph[1], minus_low, e1));
+        }
+        l += ls;
+        const f16x8 pf = join8(pl[0], pl[1], pl[2], pl[3]);
+#pragma unroll
+        for (int g = 0; g < NJ; ++g) {
+            f16x8 even, odd;
+            v_frags(v.w[g >> 1][2 * (g & 1)], v.w[g >> 1][2 * (g & 1) + 1], v.d[g], mk, even, odd);
+            acc[g][0] = mfma16(even, pf, acc[g][0]);
+            acc[g][1] = mfma16(odd, pf, acc[g][1]);
+        }
+        v.load(tn, r, h);
+        ok = ok_next;
+    }
+    l += xor_lanes(l, 16);
+    l += xor_lanes(l, 32);
+    float *out = a.out + (size_t)tok * a.out_stride + (size_t)kvh * a.group * D;
+    const float inv = l > 0.0f || l != l ? 1.0f / l : 0.0f;
+#pragma unroll
+    for (int g = 0; g < NJ; ++g) {
+        float o[8];
+#pragma unroll
+        for (int i = 0; i < 4; ++i) {
+            const float e = acc[g][0][i], d = acc[g][1][i];
+            o[2 * i] = (e + ror8(e)) * inv;
+            o[2 * i + 1] = (d + ror8(d)) * inv;
+        }
+        if (!low && live) __builtin_memcpy(out + (size_t)row * D + 32 * g + 8 * h, o, 32);
+    }
+}
+
+// A wave a (token, KV head), four of them a workgroup.
+template <int D> __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attend_lists_kernel(AttnArgs a) {
+    const uint32_t unit = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), tok = unit / a.c.n_kv, kvh = unit - tok * a.c.n_kv;
+    if (tok >= a.n_tok) return;
+    bool none = true;
+    for (uint32_t base = 0; none && base < a.seqs; base += 64) {
+        const uint32_t i = base + (threadIdx.x & 63);
+        const Span p = span_of(a, i < a.seqs ? i : 0);
+        none = !__builtin_amdgcn_ballot_w64(i < a.seqs && tok >= p.q0 && tok - p.q0 < p.nq);
+    }
+    if (none) return;
+    typedef const uint32_t __attribute__((address_space(4))) *cptr;
+    const cptr list = (cptr)(uintptr_t)(a.list + (size_t)unit * a.list_stride);
+    auto tile_at = [&](uint32_t tile, bool &ok) {
+        const uint32_t at = list[1 + (tile >> a.block_shift)];
+        ok = at != kNoList;
+        return (const uint8_t *)a.c.base + (uint64_t)((ok ? at : 0) + (tile & ((1u << a.block_shift) - 1))) * (36u * D);
+    };
+    attend_rows<D>(a, tok, kvh, list[0], tile_at);
+}
+
 } // namespace
 
 hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream) {
@@ -383,7 +557,7 @@ hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream) {
 
 template <int D> void launch_choice(const BlockArgs &a, hipStream_t stream) {
     if (!a.tiles) {
-        hipLaunchKernelGGL(block_choice_kernel<D>, dim3(a.a.n_tok * a.a.c.n_kv), dim3(kOneThreads), a.lds_keys * sizeof(uint64_t), stream, a);
+        hipLaunchKernelGGL(block_choice_kernel<D>, dim3(a.a.n_tok * a.a.c.n_kv), dim3(1024), a.lds_keys * sizeof(uint64_t), stream, a);
         return;
     }
     hipLaunchKernelGGL(block_choices_kernel<D>, dim3(a.tiles * a.a.c.n_kv), dim3(64 * kSomeWaves), 16 * (D + 2 + a.lds_keys + 1) * sizeof(uint64_t), stream, a);
@@ -393,6 +567,14 @@ hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream) {
     if (a.a.c.dim == 64) launch_choice<64>(a, stream);
     else if (a.a.c.dim == 128) launch_choice<128>(a, stream);
     else launch_choice<256>(a, stream);
+    return hipGetLastError();
+}
+
+hipError_t ah_launch_attend_lists(const AttnArgs &a, hipStream_t stream) {
+    const dim3 grid((a.n_tok * a.c.n_kv + 3) / 4), block(256);
+    if (a.c.dim == 64) hipLaunchKernelGGL(attend_lists_kernel<64>, grid, block, 0, stream, a);
+    else if (a.c.dim == 128) hipLaunchKernelGGL(attend_lists_kernel<128>, grid, block, 0, stream, a);
+    else hipLaunchKernelGGL(attend_lists_kernel<256>, grid, block, 0, stream, a);
     return hipGetLastError();
 }
 

@@ -209,5 +209,6 @@ hipError_t ah_launch_attn_shared(const AttnArgs &prefix, const AttnArgs &after, 
 hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream);
 hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream);
 hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream);
+hipError_t ah_launch_attend_lists(const AttnArgs &a, hipStream_t stream);
 size_t ah_sample_plan(SampleArgs &a, uint32_t cus, uint8_t *base);
 hipError_t ah_launch_sample(const SampleArgs &a, hipStream_t stream);
