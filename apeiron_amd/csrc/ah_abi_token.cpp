@@ -423,26 +423,40 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     a.first_key = (uint32_t)prefix_len;
     AttnArgs pre = a, own = a;
     const size_t kv = a.c.n_kv, cus = (size_t)ctx->cu_count, most = most_pieces(a, rows);
-    // n pieces of `tiles` tiles for `units` workgroups: as many as fill `places`, at least `least` tiles each.
-    auto cut = [&](AttnArgs &x, size_t units, size_t tiles, size_t places, size_t least) {
-        size_t n = places / units, fit = (tiles + least - 1) / least;
-        n = n < fit ? n : fit;
+    auto cut = [&](AttnArgs &x, size_t units, size_t tiles, size_t n) {  // into n pieces
         n = n < most / 2 ? n : most / 2;
         n = n < 1 ? 1 : n;
         const size_t chunk = tiles ? (tiles + n - 1) / n : 1;
         x.chunk = (uint32_t)chunk;
         x.splits = (uint32_t)(tiles ? (tiles + chunk - 1) / chunk : 1);
         x.grid = (uint32_t)(units * x.splits);
-        return units <= max_grid(256) / x.splits;
+        return units <= max_grid(256) / 2 / x.splits;
     };
     // The prefix: the whole batch as one sequence.
     pre.n_seq = 1;
     pre.table = d_prefix_table;
     pre.table_stride = (uint32_t)((prefix_len - 1) >> a.c.page_shift) + 1;
-    pre.rows = batch <= 8 ? 8 : batch <= 128 ? 16 : 128;
-    const size_t held = a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1, units = (batch + pre.rows - 1) / pre.rows;
+    pre.rows = batch <= 128 ? 16 : 128;
+    const size_t units = (batch + pre.rows - 1) / pre.rows, all = (prefix_len + 31) / 32;
     pre.per = (uint32_t)units;
-    if (!cut(pre, units * kv, (prefix_len + 31) / 32, pre.rows == 128 ? held * cus : 2 * cus, 4)) return AH_ERR_INVALID_ARG;
+    // Pieces by the time that they take, as attn_tiles has it: workgroups in rounds, and a piece's results written and read.
+    const size_t held = pre.rows != 128 ? 4 : a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1;
+    const double tile = pre.rows == 128 ? a.c.dim * 0.0077 : 0.18, alone = pre.rows == 128 ? 1.4 * tile : 0.18, start = 5.0, join = (double)rows * a.c.dim * 8.0 / 4e6 + 0.05;
+    size_t pieces = 1;
+    double best = 0.0;
+    for (size_t n = 1; n <= (all + 3) / 4 && n <= 256; ++n) {
+        const size_t wgs = units * kv * n, full = wgs / (held * cus), rest = wgs % (held * cus), per_piece = (all + n - 1) / n;
+        auto round = [&](size_t m) {
+            const double t = (double)((m + cus - 1) / cus) * tile;
+            return (double)per_piece * (t > alone ? t : alone) + start;
+        };
+        const double t = (double)full * round(held * cus) + (rest ? round(rest) : 0.0) + (double)n * join;
+        if (n == 1 || t < best) {
+            best = t;
+            pieces = n;
+        }
+    }
+    if (!cut(pre, units * kv, all, pieces)) return AH_ERR_INVALID_ARG;
     // What follows it: each sequence for itself.
     const size_t per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
     const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
@@ -453,7 +467,10 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         own.per = (size_t)a.n_tok == (size_t)a.n_seq * a.max_q || a.n_seq == 1 ? (uint32_t)((per_seq + 127) / 128) : 0;
         own_units = (own.per ? (size_t)own.per * a.n_seq : ((size_t)a.n_tok * a.group >> 7) + a.n_seq) * kv;
     }
-    if (!cut(own, own_units, tiles, 2 * cus, 4)) return AH_ERR_INVALID_ARG;
+    // (four tiles a piece or more: a wave each)
+    size_t fill = 2 * cus / own_units;
+    fill = fill < (tiles + 3) / 4 ? fill : (tiles + 3) / 4;
+    if (!cut(own, own_units, tiles, fill)) return AH_ERR_INVALID_ARG;
     a.splits = pre.splits + own.splits;
     AH_HIP(ctx, hipSetDevice(ctx->device));
     const int32_t st = attn_scratch(ctx, a, rows, 0, stream);

@@ -106,8 +106,7 @@ template <int MODE> AH_DEV const uint8_t *tile_in(const AttnArgs &a, uint32_t s,
 // page's index, a tile, the partial results' way to the last workgroup and back (4001 keys: 9.8 us).  A unit
 // over all keys in one workgroup, joined by nobody, costs 0.7 us a tile and wave; a second launch for the join
 // 5 us more; equal shares of all units' tiles for every workgroup (two units in one) up to 10.
-template <int D, bool PACK, int MODE>
-__global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_rows_kernel(AttnArgs a) {
+template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, uint32_t block, uint32_t grid) {
     constexpr int NJ = D / 32;  // contraction steps of K q, and blocks of channels
     constexpr uint32_t R = PACK ? 8 : 16;
     extern __shared__ float lds[];
@@ -119,7 +118,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
     // pieces run slowest: the workgroups without work (pieces past a short context) are the last ones, and
     // every XCD (workgroups go to them in turn) gets its share of those with work; a context's pieces go
     // round the XCDs
-    const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units, unit = (blockIdx.x - split * units + split) % units;
+    const uint32_t units = grid / a.splits, split = block / units, unit = (block - split * units + split) % units;
     const uint32_t per = units / a.n_seq, s = unit / per, rest = unit - s * per, rt = rest / a.c.n_kv, kvh = rest - rt * a.c.n_kv;
     const Span p = span_in<MODE>(a, s, kvh);
     if (MODE != kBlocks && p.bad && split == 0 && rest == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
@@ -377,6 +376,10 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
     }
     if (groups > 1 && arrive(a.count + unit, groups)) join(0, a.join, groups, true);
 }
+template <int D, bool PACK, int MODE>
+__global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_rows_kernel(AttnArgs a) {
+    attn_rows<D, PACK, MODE>(a, blockIdx.x, gridDim.x);
+}
 
 // Chunks of tokens: 128 rows (token, head of the group) a workgroup, 32 a wave as the columns of 32x32 products,
 // over 64 keys at a time.  The four waves turn a tile's codes into f16 in LDS together (once for 128 rows), in
@@ -396,8 +399,7 @@ __global__ void __launch_bounds__(256, D == 256 ? 2 : D == 128 ? 3 : 4) attn_row
 template <int D> struct TileLds {
     static constexpr int kK = 2 * D + 16, kV = 144, kBytes = 64 * kK + D * kV;
 };
-template <int D, int MODE>
-__global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
+template <int D, int MODE> AH_DEV void attn_tiles(const AttnArgs &a, uint32_t block, uint32_t grid) {
     constexpr int NK = D / 16, NN = D / 32, NU = D / 64;  // contraction steps of K q; channel blocks; 16-byte units
     constexpr int kAhead = D == 256 ? 3 : 1;  // more, where the registers do not cost a wave per SIMD
     typedef TileLds<D> Lds;
@@ -407,8 +409,8 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     // Pieces slowest; then the last rows first: with a causal mask they have the most keys.  Even sequences have `per`
     // units of 128 rows each.  Of uneven ones, sequence s has its units from start(s) on: floor of its first row / 128,
     // and one more for each sequence before it, so that few numbers have no rows.
-    const uint32_t units = gridDim.x / a.splits, split = blockIdx.x / units;
-    uint32_t unit = blockIdx.x - split * units;
+    const uint32_t units = grid / a.splits, split = block / units;
+    uint32_t unit = block - split * units;
     if (a.per && a.n_seq > 1) {  // workgroups go to the eight XCDs in turn: neighbouring units to one, whose L2 they share
         const uint32_t x = unit & 7, more = units & 7;
         unit = x * (units / 8) + (x < more ? x : more) + unit / 8;
@@ -724,7 +726,7 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
         __syncthreads();
         uint32_t *turn = reinterpret_cast<uint32_t *>(tile_lds);
         if (threadIdx.x == 0) {
-            uint32_t *counter = a.count + (blockIdx.x - split * units);
+            uint32_t *counter = a.count + (block - split * units);
             const uint32_t n = __hip_atomic_fetch_add(counter, 1u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             if (n == pieces - 1) __hip_atomic_store(counter, 0u, __ATOMIC_RELAXED, __HIP_MEMORY_SCOPE_AGENT);
             *turn = n;
@@ -772,6 +774,18 @@ __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile
     }
 }
 
+template <int D, int MODE> __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
+    attn_tiles<D, MODE>(a, blockIdx.x, gridDim.x);
+}
+// A common prefix, by 16 or 128 rows of the whole batch, and beside it in the same launch what each sequence has after it, by 8
+// or 16: the one alone leaves CUs without work at its end, and a launch more costs 5 us.
+template <int D, bool TILES, bool PACK>
+__global__ void __launch_bounds__(256, TILES ? (D == 64 ? 3 : D == 128 ? 2 : 1) : D == 256 ? 2 : D == 128 ? 3 : 4) attn_shared_kernel(AttnArgs prefix, AttnArgs after) {
+    if (blockIdx.x >= prefix.grid) attn_rows<D, PACK, kAfter>(after, blockIdx.x - prefix.grid, after.grid);
+    else if (TILES) attn_tiles<D, kPrefix>(prefix, blockIdx.x, prefix.grid);
+    else attn_rows<D, false, kPrefix>(prefix, blockIdx.x, prefix.grid);
+}
+
 // Joins the pieces of attn_tile_kernel's contexts: a wave takes 256 / D heads of a token, four channels a lane.  A piece
 // past a row's keys was never written; which those are follows from the same tiles_of.  Bound by the partial results'
 // bytes.
@@ -814,35 +828,63 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
     __builtin_memcpy(a.out + (size_t)tok * a.out_stride + (size_t)head * D + c, &sum, 16);
 }
 
-// Joins what kPrefix and kAfter leave: of every token of a sequence a.splits pieces, those of no weight passed over.
+// Joins what kPrefix and kAfter leave, a.splits pieces of every token of a sequence: a workgroup takes 256 / D heads of a token,
+// each of its waves every fourth piece, eight of them on their way, and they meet in LDS.
 template <int D>
 __global__ void __launch_bounds__(256) attn_meet_kernel(AttnArgs a) {
-    constexpr uint32_t kLanes = D / 4, kHeads = 64 / kLanes;
-    const uint32_t lane = threadIdx.x & 63, it = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
-    const uint32_t per = (a.n_heads + kHeads - 1) / kHeads, tok = it / per, head = (it - tok * per) * kHeads + lane / kLanes;
-    if (tok >= a.n_tok) return;
+    constexpr uint32_t kLanes = D / 4, kHeads = 64 / kLanes, kAhead = 8;
+    __shared__ f32x4 red[4][64];
+    __shared__ f32x2 red_ml[4][64];
+    const uint32_t lane = threadIdx.x & 63, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t per = (a.n_heads + kHeads - 1) / kHeads, tok = blockIdx.x / per, head = (blockIdx.x - tok * per) * kHeads + lane / kLanes;
     auto start = [&](uint32_t i) { return (uint32_t)a.q_start[i]; };
     auto holds = [&](uint32_t i) {
         const Span p = span_in<kAfter>(a, i, 0);
         return tok >= p.q0 && tok - p.q0 < p.nq;
     };
-    const Span p = span_in<kAfter>(a, sequence_of(a, tok, start, holds), 0);
-    if (tok < p.q0 || tok - p.q0 >= p.nq || head >= a.n_heads) return;
+    const size_t all = (size_t)a.n_tok * a.n_heads, flat = (size_t)tok * a.n_heads + (head < a.n_heads ? head : 0);
     const uint32_t c = 4 * (lane % kLanes);
-    const size_t all = (size_t)a.n_tok * a.n_heads, flat = (size_t)tok * a.n_heads + head;
     float M = kNoMax, L = 0.0f;
-#pragma unroll 4
-    for (uint32_t k = 0; k < a.splits; ++k) M = __builtin_fmaxf(M, a.part_ml[2 * (k * all + flat)]);
     f32x4 sum = (f32x4)0.0f;
-#pragma unroll 4
-    for (uint32_t k = 0; k < a.splits; ++k) {
-        f32x2 ml;
-        f32x4 o;
-        __builtin_memcpy(&ml, a.part_ml + 2 * (k * all + flat), 8);
-        __builtin_memcpy(&o, a.part_o + (k * all + flat) * D + c, 16);
-        const float w = __builtin_amdgcn_exp2f(ml[0] - M);
-        L += ml[1] * w;
-        sum += o * w;
+    for (uint32_t k0 = wave; k0 < a.splits; k0 += 4 * kAhead) {
+        f32x2 ml[kAhead];
+        f32x4 o[kAhead];
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const uint32_t k = k0 + 4 * j < a.splits ? k0 + 4 * j : k0;
+            __builtin_memcpy(&ml[j], a.part_ml + 2 * (k * all + flat), 8);
+            __builtin_memcpy(&o[j], a.part_o + (k * all + flat) * D + c, 16);
+        }
+        float top = M;
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) top = __builtin_fmaxf(top, ml[j][0]);
+        const float keep = __builtin_amdgcn_exp2f(M - top);
+        L *= keep;
+        sum *= keep;
+        M = top;
+#pragma unroll
+        for (uint32_t j = 0; j < kAhead; ++j) {
+            const float w = k0 + 4 * j < a.splits ? __builtin_amdgcn_exp2f(ml[j][0] - M) : 0.0f;
+            if (k0 + 4 * j < a.splits) {
+                L += ml[j][1] * w;
+                sum += o[j] * w;
+            }
+        }
+    }
+    red[wave][lane] = sum;
+    red_ml[wave][lane] = (f32x2){M, L};
+    const Span p = span_in<kAfter>(a, sequence_of(a, tok, start, holds), 0);
+    __syncthreads();
+    if (wave != 0 || tok < p.q0 || tok - p.q0 >= p.nq || head >= a.n_heads) return;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, red_ml[w][lane][0]);
+    L = 0.0f;
+    sum = (f32x4)0.0f;
+#pragma unroll
+    for (int w = 0; w < 4; ++w) {
+        const float x = __builtin_amdgcn_exp2f(red_ml[w][lane][0] - M);
+        L += red_ml[w][lane][1] * x;
+        sum += red[w][lane] * x;
     }
     sum *= L > 0.0f || L != L ? 1.0f / L : 0.0f;
     __builtin_memcpy(a.out + (size_t)tok * a.out_stride + (size_t)head * D + c, &sum, 16);
@@ -868,12 +910,20 @@ template <int D> hipError_t launch(const AttnArgs &a, hipStream_t stream) {
     if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3(join_grid<D>(a)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
+template <int D, bool TILES, bool PACK> void launch_both(const AttnArgs &prefix, const AttnArgs &after, hipStream_t stream) {
+    constexpr size_t tiles = 2 * TileLds<D>::kBytes, lds = TILES && tiles > attn_lds<D>() ? tiles : attn_lds<D>();
+    hipLaunchKernelGGL((attn_shared_kernel<D, TILES, PACK>), dim3(prefix.grid + after.grid), dim3(256), lds, stream, prefix, after);
+}
 template <int D> hipError_t launch_shared(const AttnArgs &prefix, const AttnArgs &after, const AttnArgs &both, hipStream_t stream) {
-    if (prefix.rows == 128) launch_tiles<D, kPrefix>(prefix, stream);
-    else launch_rows<D, kPrefix>(prefix, stream);
-    if (after.rows == 128) launch_tiles<D, kAfter>(after, stream);
-    else launch_rows<D, kAfter>(after, stream);
-    hipLaunchKernelGGL(attn_meet_kernel<D>, dim3(join_grid<D>(both)), dim3(256), 0, stream, both);
+    if (after.rows == 128) {
+        launch_tiles<D, kPrefix>(prefix, stream);
+        launch_tiles<D, kAfter>(after, stream);
+    } else if (prefix.rows == 128) {
+        after.rows == 16 ? launch_both<D, true, false>(prefix, after, stream) : launch_both<D, true, true>(prefix, after, stream);
+    } else {
+        after.rows == 16 ? launch_both<D, false, false>(prefix, after, stream) : launch_both<D, false, true>(prefix, after, stream);
+    }
+    hipLaunchKernelGGL(attn_meet_kernel<D>, dim3(both.n_tok * ((both.n_heads + 256 / D - 1) / (256 / D))), dim3(256), 0, stream, both);
     return hipGetLastError();
 }
 template <int D> hipError_t launch_blocks(const AttnArgs &a, hipStream_t stream) {
@@ -905,12 +955,21 @@ hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream) {
     return a.c.dim == 64 ? launch_blocks<64>(a, stream) : a.c.dim == 128 ? launch_blocks<128>(a, stream) : launch_blocks<256>(a, stream);
 }
 
+template <int D> hipError_t allow_shared() {
+    const size_t most = 2 * TileLds<D>::kBytes > attn_lds<D>() ? 2 * TileLds<D>::kBytes : attn_lds<D>();
+    hipError_t e = allow_lds(attn_shared_kernel<D, false, false>, most);
+    if (e == hipSuccess) e = allow_lds(attn_shared_kernel<D, false, true>, most);
+    if (e == hipSuccess) e = allow_lds(attn_shared_kernel<D, true, false>, most);
+    return e != hipSuccess ? e : allow_lds(attn_shared_kernel<D, true, true>, most);
+}
+
 hipError_t ah_attn_init_attrs() {
     hipError_t e = allow_rows<kAll>();
-    if (e == hipSuccess) e = allow_rows<kPrefix>();
-    if (e == hipSuccess) e = allow_rows<kAfter>();
     if (e == hipSuccess) e = allow_rows<kBlocks>();
     if (e == hipSuccess) e = allow_tiles<kAll>();
     if (e == hipSuccess) e = allow_tiles<kPrefix>();
-    return e != hipSuccess ? e : allow_tiles<kAfter>();
+    if (e == hipSuccess) e = allow_tiles<kAfter>();
+    if (e == hipSuccess) e = allow_shared<64>();
+    if (e == hipSuccess) e = allow_shared<128>();
+    return e != hipSuccess ? e : allow_shared<256>();
 }
