@@ -26,6 +26,17 @@ AH_DEV Seq seq_of(const StateSeqs &a, uint32_t s) {
     return p;
 }
 
+// v / (1 + e^-v).  e^-v = 2^t (1 + r ln 2), t the f32 product v log2(e) and r what that rounding and log2(e)'s left out, a few
+// last places of t; the quotient by v_rcp_f32 with a Newton step.  Within 4 2^-24 of the result (5 x 1021 tokens of 4099 channels
+// with a library exponential and division: 41 us for 39).
+AH_DEV float silu(float v) {
+    constexpr float kHi = -1.44269502162933349609f, kLo = -1.92596299112661746887e-8f, kLn2 = 0.69314718f;
+    const float t = v * kHi, r = __builtin_fmaf(v, kHi, -t) + v * kLo;
+    float e = __builtin_amdgcn_exp2f(t);
+    e = __builtin_fmaf(e, __builtin_fabsf(t) < 126.0f ? r * kLn2 : 0.0f, e);
+    const float d = 1.0f + e, q = __builtin_amdgcn_rcpf(d), y = v * q;
+    return d < 0x1p100f ? __builtin_fmaf(__builtin_fmaf(-d, y, v), q, y) : y;
+}
 AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 
 // ---- the short causal convolution --------------------------------------------------------------------
@@ -108,7 +119,7 @@ template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) 
                     for (int k = 0; k < W - 1; ++k) v = __builtin_fmaf(w[i * W + k], row[k][i], v);
                     v = __builtin_fmaf(w[i * W + W - 1], now[j][i], v);
                     odd = odd || ((uint32_t)i < take && t + j < rows && !finite(v));
-                    out[i] = a.silu ? v / (1.0f + expf(-v)) : v;
+                    out[i] = a.silu ? silu(v) : v;
                 }
                 if (t + j < rows) st4(yr, (t + j) * y_stride + c0, out, take);
 #pragma unroll
@@ -347,91 +358,68 @@ template <int DK> struct PrepareLds {
     double gamma[64];
     float beta[64], fk[64], fq[64], fw[64], fd[64], red[4], tinv[4];
 };
-template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel(DeltaArgs a) {
+// Eight waves a chunk and head.  Waves 0 to 3 have the keys and beta_i k_i . k_j of 16 tokens i each, and make T of them; waves 4 to
+// 7 have q of the same tokens, P and q's fragments.  W and U0 are shared by all.  Barriers wait for LDS alone: loads and stores stay
+// on their way.
+template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel(DeltaArgs a) {
     constexpr int NT = DK / 32;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
     PrepareLds<DK> &L = *reinterpret_cast<PrepareLds<DK> *>(lds_bytes);
-    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, w = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
+    const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
+    const bool keys = wave < 4;
     const uint32_t at = blockIdx.x / a.n_heads, hd = blockIdx.x - at * a.n_heads, kh = hd / a.group, dv = a.v_dim;
     const Chunk c = chunk_of(a, at);
     if (c.live == 0) return;
     const DeltaBlock B = delta_block(DK, dv);
     uint8_t *block = a.blocks + ((size_t)at * a.n_heads + hd) * B.bytes;
     float *fac = reinterpret_cast<float *>(block + B.f);
-
     typedef Rows<DK> R;
-    R k, q;
+    R x;
+    {
+        const float *from = keys ? a.k : a.q;
+        const size_t stride = keys ? a.k_stride : a.q_stride;
 #pragma unroll
-    for (uint32_t i = 0; i < R::kLoads; ++i) {
-        const uint32_t t = 16 * w + R::row(i, lane);
-        const size_t tok = c.tok0 + (t < c.live ? t : 0), at_col = (size_t)kh * DK + R::col(lane);
-        __builtin_memcpy(&k.x[i], a.k + tok * a.k_stride + at_col, 16);
-        __builtin_memcpy(&q.x[i], a.q + tok * a.q_stride + at_col, 16);
-    }
-    // v's first columns of this wave (every fourth 16), as operands that sum over the tokens
-    f32x4 vx[2][4];
-    auto load_v = [&](uint32_t cb0) {
-#pragma unroll
-        for (uint32_t m = 0; m < 2; ++m)
-#pragma unroll
-            for (uint32_t t = 0; t < 4; ++t)
-#pragma unroll
-                for (uint32_t n = 0; n < 4; ++n) {
-                    const uint32_t j = 16 * t + 4 * h + n, cb = cb0 + 4 * m;
-                    vx[m][t][n] = a.v[(size_t)(c.tok0 + (j < c.live ? j : 0)) * a.v_stride + (size_t)hd * dv + 16 * (cb < dv / 16 ? cb : 0) + r];
-                }
-    };
-    load_v(w);
-    // gates, a lane a token: gamma by a scan
-    float beta = 0.0f, g = 0.0f;
-    if (lane < c.live) {
-        g = decay_of(a, a.a[(size_t)(c.tok0 + lane) * a.a_stride + hd], hd);
-        g = g < -1000.0f ? -1000.0f : g;  // (e^g is 0 as well, and sums stay finite)
-        beta = rate_of(a, a.b[(size_t)(c.tok0 + lane) * a.b_stride + hd]);
-    }
-    double gamma = g;
-#pragma unroll
-    for (int o = 1; o < 64; o <<= 1) {
-        const double v = __shfl_up(gamma, o, 64);
-        gamma += (int)lane >= o ? v : 0.0;
-    }
-    float ktop = 0.0f, qtop = 0.0f;
-#pragma unroll
-    for (uint32_t i = 0; i < R::kLoads; ++i) {
-        const bool live = 16 * w + R::row(i, lane) < c.live;
-        __asm__("" : "+v"(k.x[i]), "+v"(q.x[i]));  // (the loads themselves stay outside the choice)
-        k.x[i] = live ? k.x[i] : (f32x4)0.0f;
-        q.x[i] = live ? q.x[i] : (f32x4)0.0f;
-        ktop = top4(ktop, k.x[i]);
-        qtop = top4(qtop, q.x[i]);
-        float kk = 0.0f, qq = 0.0f;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) {
-            kk = __builtin_fmaf(k.x[i][n], k.x[i][n], kk);
-            qq = __builtin_fmaf(q.x[i][n], q.x[i][n], qq);
-        }
-        kk = sum16(kk);
-        qq = sum16(qq);
-        if (DK == 128) {
-            kk += __shfl_xor(kk, 16, 64);
-            qq += __shfl_xor(qq, 16, 64);
-        }
-        if (R::col(lane) == 0) {
+        for (uint32_t i = 0; i < R::kLoads; ++i) {
             const uint32_t t = 16 * w + R::row(i, lane);
-            const bool norm = a.norm_eps >= 0.0f;
-            L.fk[t] = !live ? 0.0f : norm ? 1.0f / __builtin_sqrtf(kk + a.norm_eps) : 1.0f;
-            L.fq[t] = !live ? 0.0f : norm ? a.scale / __builtin_sqrtf(qq + a.norm_eps) : a.scale;
+            __builtin_memcpy(&x.x[i], from + (size_t)(c.tok0 + (t < c.live ? t : 0)) * stride + (size_t)kh * DK + R::col(lane), 16);
         }
     }
-    if (w == 0) {
+    if (wave == 7) {  // gates, a lane a token: gamma by a scan
+        float beta = 0.0f, g = 0.0f;
+        if (lane < c.live) {
+            g = decay_of(a, a.a[(size_t)(c.tok0 + lane) * a.a_stride + hd], hd);
+            g = g < -1000.0f ? -1000.0f : g;  // (e^g is 0 as well, and sums stay finite)
+            beta = rate_of(a, a.b[(size_t)(c.tok0 + lane) * a.b_stride + hd]);
+        }
+        double gamma = g;
+#pragma unroll
+        for (int o = 1; o < 64; o <<= 1) {
+            const double v = __shfl_up(gamma, o, 64);
+            gamma += (int)lane >= o ? v : 0.0;
+        }
         L.gamma[lane] = gamma;
         L.beta[lane] = beta;
     }
-    ktop = wave_max(ktop);
-    if (lane == 0) L.red[w] = ktop;
-    // q through this wave's rows of the keys' place: as an operand, eight channels a lane
-    const Scale qs = scale_of(wave_max(qtop));
-    auto put_rows = [&](const R &x, float up) {
+    float top = 0.0f;
+#pragma unroll
+    for (uint32_t i = 0; i < R::kLoads; ++i) {
+        const uint32_t t = 16 * w + R::row(i, lane);
+        __asm__("" : "+v"(x.x[i]));  // (the loads themselves stay outside the choice)
+        x.x[i] = t < c.live ? x.x[i] : (f32x4)0.0f;
+        top = top4(top, x.x[i]);
+        float sum = 0.0f;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) sum = __builtin_fmaf(x.x[i][n], x.x[i][n], sum);
+        sum = sum16(sum);
+        if (DK == 128) sum += __shfl_xor(sum, 16, 64);
+        if (R::col(lane) == 0) {
+            const float f = keys ? 1.0f : a.scale, v = a.norm_eps >= 0.0f ? f / __builtin_sqrtf(sum + a.norm_eps) : f;
+            (keys ? L.fk : L.fq)[t] = t < c.live ? v : 0.0f;
+        }
+    }
+    top = wave_max(top);
+    if (keys && lane == 0) L.red[w] = top;
+    auto put_rows = [&](float up) {
 #pragma unroll
         for (uint32_t i = 0; i < R::kLoads; ++i) {
             const uint32_t t = 16 * w + R::row(i, lane), col = R::col(lane);
@@ -442,162 +430,184 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
             __builtin_memcpy(&L.kl[t][col], lo, 8);
         }
     };
-    auto row_frag = [&](uint32_t t, int n) {
+    auto row_frag = [&](uint32_t t, int n) {  // eight channels a lane
         Frag f;
         __builtin_memcpy(&f.hi, &L.kh[t][32 * n + 8 * h], 16);
         __builtin_memcpy(&f.lo, &L.kl[t][32 * n + 8 * h], 16);
         return f;
     };
+    auto store_frag = [&](uint32_t to, const Frag &f) {
+        __builtin_memcpy(block + to + lane * 16, &f.hi, 16);
+        __builtin_memcpy(block + to + 1024 + lane * 16, &f.lo, 16);
+    };
     const uint32_t row = 16 * w + r;
-    Frag kf[NT], qf[NT];
-    put_rows(q, qs.up);
-    __builtin_amdgcn_wave_barrier();
+    Frag f[NT];  // of the wave's rows
+    const Scale qs = scale_of(top);
+    if (!keys) {  // through the keys' place, before they are there
+        put_rows(qs.up);
+        __builtin_amdgcn_wave_barrier();
 #pragma unroll
-    for (int t = 0; t < NT; ++t) {
-        qf[t] = row_frag(row, t);
-        // for the chain in the order of S: even channels, then odd ones
-        auto halves = [](u32x4 v) {
-            return (u32x4){__builtin_amdgcn_perm(v[1], v[0], 0x05040100), __builtin_amdgcn_perm(v[3], v[2], 0x05040100),
-                           __builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302)};
-        };
-        const u32x4 hi = halves(qf[t].hi), lo = halves(qf[t].lo);
-        __builtin_memcpy(block + B.q + (w * NT + t) * 2048 + lane * 16, &hi, 16);
-        __builtin_memcpy(block + B.q + (w * NT + t) * 2048 + 1024 + lane * 16, &lo, 16);
+        for (int t = 0; t < NT; ++t) {
+            f[t] = row_frag(row, t);
+            // for the chain in the order of S: even channels, then odd ones
+            auto halves = [](u32x4 v) {
+                return (u32x4){__builtin_amdgcn_perm(v[1], v[0], 0x05040100), __builtin_amdgcn_perm(v[3], v[2], 0x05040100),
+                               __builtin_amdgcn_perm(v[1], v[0], 0x07060302), __builtin_amdgcn_perm(v[3], v[2], 0x07060302)};
+            };
+            store_frag(B.q + (w * NT + t) * 2048, {halves(f[t].hi), halves(f[t].lo)});
+        }
+        if (lane == 0) fac[kFQ + w] = qs.down;
     }
-    __syncthreads();
+    ah_lds_barrier();
     const Scale ks = scale_of(__builtin_fmaxf(__builtin_fmaxf(L.red[0], L.red[1]), __builtin_fmaxf(L.red[2], L.red[3])));
-    put_rows(k, ks.up);
     const double gr = L.gamma[row], all = L.gamma[63];
-    const float fk = L.fk[row], fq = L.fq[row];
-    if (w == 0) {  // e^gamma of each token to W's keys, what is left of the chunk's decay to the state's
-        L.fw[lane] = beta * expf((float)gamma) * L.fk[lane];
+    if (keys) put_rows(ks.up);
+    else if (h == 0) fac[kFRow + row] = L.fq[row] * expf((float)gr);
+    if (wave == 4) {  // e^gamma of each token to W's keys, what is left of the chunk's decay to the state's
+        const double gamma = L.gamma[lane];
+        L.fw[lane] = L.beta[lane] * expf((float)gamma) * L.fk[lane];
         L.fd[lane] = expf((float)(all - gamma)) * L.fk[lane];
         if (lane == 0) fac[kFDecay] = expf((float)all);
     }
-    if (h == 0) fac[kFRow + row] = fq * expf((float)gr);
-    if (lane == 0) fac[kFQ + w] = qs.down;
-    __syncthreads();
-#pragma unroll
-    for (int t = 0; t < NT; ++t) kf[t] = row_frag(row, t);
+    ah_lds_barrier();
 
-    // k_j . k_i and k_j . q_i of this wave's tokens i and the tiles of j up to them: a lane has i = r, j = 16 t + 4 h + n
-    const float br = L.beta[row] * fk * ks.down * ks.down, pr = fq * ks.down * qs.down;
+    // k_j . k_i or k_j . q_i of the wave's tokens i and the tiles of j up to them: a lane has i = r, j = 16 t + 4 h + n
+    if (keys) {
+#pragma unroll
+        for (int t = 0; t < NT; ++t) f[t] = row_frag(row, t);
+    }
+    const uint32_t end = keys ? row : row + 1;
+    const float fr = keys ? L.beta[row] * L.fk[row] * ks.down * ks.down : L.fq[row] * ks.down * qs.down;
     f32x4 p[4];
 #pragma unroll
     for (uint32_t jt = 0; jt < 4; ++jt) {
         p[jt] = (f32x4)0.0f;
         if (jt > w) continue;
-        f32x4 kk = (f32x4)0.0f, kq = (f32x4)0.0f;
-#pragma unroll
-        for (int t = 0; t < NT; ++t) {
-            const Frag f = row_frag(16 * jt + r, t);
-            kk = mm3(f, kf[t], kk);
-            kq = mm3(f, qf[t], kq);
-        }
-        f32x4 aij;
+        float d[4];  // (formed for every lane: a branch for each would wait for each one's factors in turn)
 #pragma unroll
         for (int n = 0; n < 4; ++n) {
             const uint32_t j = 16 * jt + 4 * h + n;
-            const float d = expf((float)(gr - L.gamma[j])) * L.fk[j];
-            aij[n] = j < row ? br * d * kk[n] : 0.0f;
-            p[jt][n] = j <= row ? pr * d * kq[n] : 0.0f;
+            d[n] = fr * expf((float)(gr - L.gamma[j])) * L.fk[j];
+            __asm__("" : "+v"(d[n]));
         }
-        __builtin_memcpy(&L.A[row * kLd + 16 * jt + 4 * h], &aij, 16);
+        f32x4 v = (f32x4)0.0f, v1 = (f32x4)0.0f, v2 = (f32x4)0.0f;  // mm3's three sums, side by side
+#pragma unroll
+        for (int t = 0; t < NT; ++t) {
+            const Frag g = row_frag(16 * jt + r, t);
+            v = mfma16(__builtin_bit_cast(f16x8, g.hi), __builtin_bit_cast(f16x8, f[t].hi), v);
+            v1 = mfma16(__builtin_bit_cast(f16x8, g.hi), __builtin_bit_cast(f16x8, f[t].lo), v1);
+            v2 = mfma16(__builtin_bit_cast(f16x8, g.lo), __builtin_bit_cast(f16x8, f[t].hi), v2);
+        }
+        v += v1 + v2;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) p[jt][n] = 16 * jt + 4 * h + n < end ? d[n] * v[n] : 0.0f;
+        if (keys) __builtin_memcpy(&L.A[row * kLd + 16 * jt + 4 * h], &p[jt], 16);
     }
-    __syncthreads();
+    // v's columns of this wave (every eighth 16), as operands that sum over the tokens: on their way while T is made
+    f32x4 vx[4];
+    auto load_v = [&](uint32_t cb) {
+#pragma unroll
+        for (uint32_t t = 0; t < 4; ++t)
+#pragma unroll
+            for (uint32_t n = 0; n < 4; ++n) {
+                const uint32_t j = 16 * t + 4 * h + n;
+                vx[t][n] = a.v[(size_t)(c.tok0 + (j < c.live ? j : 0)) * a.v_stride + (size_t)hd * dv + 16 * cb + r];
+            }
+    };
+    const uint32_t cb_first = dv == 64 ? w : wave;  // (of four columns of tiles, the waves 4 to 7 take one each)
+    const bool has_v = dv > 64 || !keys;
+    if (has_v) load_v(cb_first);
+    ah_lds_barrier();
 
     // T = (1 + A)^-1 in place: the diagonal blocks by substitution, a lane a column; then blocks of 32, then the whole
-    {
-        float *D = &L.A[16 * w * kLd + 16 * w], x[16];
+    const f32x4 zero = (f32x4)0.0f;
+    auto at_block = [&](uint32_t i, uint32_t j) { return &L.A[16 * i * kLd + 16 * j]; };
+    auto as_result = [&](const float *y) {  // a block as a result lies
+        f32x4 v;
+#pragma unroll
+        for (int n = 0; n < 4; ++n) v[n] = y[(4 * h + n) * kLd + r];
+        return v;
+    };
+    auto put = [&](float *y, f32x4 v) {
+#pragma unroll
+        for (int n = 0; n < 4; ++n) y[(4 * h + n) * kLd + r] = v[n];
+    };
+    if (keys) {
+        float *D = &L.A[16 * w * kLd + 16 * w], y[16];
 #pragma unroll
         for (int i = 0; i < 16; ++i) {
             float v = i == (int)r ? 1.0f : 0.0f;
 #pragma unroll
-            for (int m = 0; m < i; ++m) v = __builtin_fmaf(-D[i * kLd + m], x[m], v);
-            x[i] = v;
+            for (int m = 0; m < i; ++m) v = __builtin_fmaf(-D[i * kLd + m], y[m], v);
+            y[i] = v;
         }
         if (h == 0) {
 #pragma unroll
-            for (int i = 0; i < 16; ++i) D[i * kLd + r] = x[i];
+            for (int i = 0; i < 16; ++i) D[i * kLd + r] = y[i];
+        }
+    } else {  // P of the wave's tokens
+        float most = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 4; ++t) most = top4(most, p[t]);
+        const Scale s = scale_of(wave_max(most));
+        if (lane == 0) fac[kFP + w] = s.down;
+#pragma unroll
+        for (uint32_t t = 0; t < 2; ++t) {
+            if (t == 1 && w < 2) continue;
+            float y[8];
+            __builtin_memcpy(y, &p[2 * t], 32);
+            store_frag(B.p + tri(w, t) * 2048, split8(y, s.up));
         }
     }
-    __syncthreads();
-    auto at_block = [&](uint32_t i, uint32_t j) { return &L.A[16 * i * kLd + 16 * j]; };
-    auto as_result = [&](const float *x) {  // a block as a result lies
-        f32x4 v;
-#pragma unroll
-        for (int n = 0; n < 4; ++n) v[n] = x[(4 * h + n) * kLd + r];
-        return v;
-    };
-    auto put = [&](float *x, f32x4 v) {
-#pragma unroll
-        for (int n = 0; n < 4; ++n) x[(4 * h + n) * kLd + r] = v[n];
-    };
-    const f32x4 zero = (f32x4)0.0f;
-    if (w < 2) {
+    ah_lds_barrier();
+    if (wave < 2) {
         const uint32_t b = 2 * w;
         const f32x4 y = block_product(at_block(b + 1, b), kLd, as_result(at_block(b, b)), zero, r, h);
         put(at_block(b + 1, b), -block_product(at_block(b + 1, b + 1), kLd, y, zero, r, h));
     }
-    __syncthreads();
-    {
-        const uint32_t col = w & 1, low = w >> 1;  // block (2 + low, col)
-        f32x4 z = zero;
+    ah_lds_barrier();
+    f32x4 z = zero;
+    const uint32_t col = w & 1, low = w >> 1;  // block (2 + low, col)
+    if (keys) {
         for (uint32_t m = 0; m <= low; ++m) {
             f32x4 y = zero;
             for (uint32_t n = col; n < 2; ++n) y = block_product(at_block(2 + m, n), kLd, as_result(at_block(n, col)), y, r, h);
             z = block_product(at_block(2 + low, 2 + m), kLd, y, z, r, h);
         }
-        __syncthreads();
-        put(at_block(2 + low, col), -z);
     }
-    __syncthreads();
-    {  // this wave's rows of T as operands
-        float x[2][8], top = 0.0f;
+    ah_lds_barrier();
+    if (keys) put(at_block(2 + low, col), -z);
+    ah_lds_barrier();
+    {  // the wave's rows of T as operands, in T's place
+        float y[2][8], most = 0.0f;
 #pragma unroll
         for (uint32_t t = 0; t < 2; ++t)
 #pragma unroll
             for (int n = 0; n < 8; ++n) {
                 const uint32_t tile = 2 * t + n / 4;
-                x[t][n] = tile <= w ? L.A[row * kLd + 16 * tile + 4 * h + (n & 3)] : 0.0f;
-                top = __builtin_fmaxf(top, __builtin_fabsf(x[t][n]));
+                y[t][n] = keys && tile <= w ? L.A[row * kLd + 16 * tile + 4 * h + (n & 3)] : 0.0f;
+                most = __builtin_fmaxf(most, __builtin_fabsf(y[t][n]));
             }
-        const Scale s = scale_of(wave_max(top));
-        if (lane == 0) L.tinv[w] = s.down;
-        __syncthreads();
+        const Scale s = scale_of(wave_max(most));
+        ah_lds_barrier();
+        if (keys) {
+            if (lane == 0) L.tinv[w] = s.down;
 #pragma unroll
-        for (uint32_t t = 0; t < 2; ++t) {
-            if (t == 1 && w < 2) continue;
-            const Frag f = split8(x[t], s.up);
-            L.t[tri(w, t)][0][lane] = f.hi;
-            L.t[tri(w, t)][1][lane] = f.lo;
+            for (uint32_t t = 0; t < 2; ++t) {
+                if (t == 1 && w < 2) continue;
+                const Frag g = split8(y[t], s.up);
+                L.t[tri(w, t)][0][lane] = g.hi;
+                L.t[tri(w, t)][1][lane] = g.lo;
+            }
         }
     }
-    __syncthreads();
-    auto store_frag = [&](uint32_t to, const Frag &f) {
-        __builtin_memcpy(block + to + lane * 16, &f.hi, 16);
-        __builtin_memcpy(block + to + 1024 + lane * 16, &f.lo, 16);
-    };
+    ah_lds_barrier();
     auto t_frag = [&](uint32_t tile, uint32_t t) { return Frag{L.t[tri(tile, t)][0][lane], L.t[tri(tile, t)][1][lane]}; };
-    // P of this wave's tokens
-    {
-        float top = 0.0f;
-#pragma unroll
-        for (int t = 0; t < 4; ++t) top = top4(top, p[t]);
-        const Scale s = scale_of(wave_max(top));
-        if (lane == 0) fac[kFP + w] = s.down;
-#pragma unroll
-        for (uint32_t t = 0; t < 2; ++t) {
-            if (t == 1 && w < 2) continue;
-            float x[8];
-            __builtin_memcpy(x, &p[2 * t], 32);
-            store_frag(B.p + tri(w, t) * 2048, split8(x, s.up));
-        }
-    }
-    // 32 channels of the keys with the tokens as what is summed over: W's transpose (a lane has token r and channels 4 h + n),
-    // and the decayed keys
+    // A slice of 32 channels of the keys, by two waves (w and w + 4), with the tokens as what is summed over: W's transpose (a lane
+    // has token r and channels 4 h + n) of two tiles of tokens each, and the decayed keys of every other channel each.
     if (w < (uint32_t)NT) {
-        float x[2][2][8], fw[2][8], fd[2][8], wt = 0.0f, dt = 0.0f;
+        const uint32_t half = wave >> 2;
+        float y[2][2][8], fw[2][8], fd[2][8], wt = 0.0f, dt = 0.0f;
 #pragma unroll
         for (int t = 0; t < 2; ++t)
 #pragma unroll
@@ -611,83 +621,79 @@ template <int DK> __global__ void __launch_bounds__(256, 2) delta_prepare_kernel
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
                     const float v = ((float)hi[k] + (float)lo[k]) * ks.down;
-                    x[k][t][n] = v;
+                    y[k][t][n] = v;
                     wt = __builtin_fmaxf(wt, __builtin_fabsf(v * fw[t][n]));
                     dt = __builtin_fmaxf(dt, __builtin_fabsf(v * fd[t][n]));
                 }
             }
         const Scale ws = scale_of(wave_max(wt)), ds = scale_of(wave_max(dt));
-        if (lane == 0) fac[kFK + w] = ds.down;
+        if (lane == 0 && half == 0) fac[kFK + w] = ds.down;
         Frag kw[2][2];
 #pragma unroll
-        for (int k = 0; k < 2; ++k)
+        for (int t = 0; t < 2; ++t) {
+            float u[8];
 #pragma unroll
-            for (int t = 0; t < 2; ++t) {
-                float y[8], z[8];
+            for (int k = 0; k < 2; ++k) {
 #pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    y[n] = x[k][t][n] * fw[t][n];
-                    z[n] = x[k][t][n] * fd[t][n];
-                }
-                kw[k][t] = split8(y, ws.up);
-                store_frag(B.k + ((2 * w + k) * 2 + t) * 2048, split8(z, ds.up));
+                for (int n = 0; n < 8; ++n) u[n] = y[k][t][n] * fw[t][n];
+                kw[k][t] = split8(u, ws.up);
             }
-        float most = 0.0f;
 #pragma unroll
-        for (uint32_t it = 0; it < 4; ++it) {
+            for (int n = 0; n < 8; ++n) u[n] = (half ? y[1][t][n] : y[0][t][n]) * fd[t][n];
+            store_frag(B.k + ((2 * w + half) * 2 + t) * 2048, split8(u, ds.up));
+        }
+#pragma unroll
+        for (uint32_t n = 0; n < 2; ++n) {
+            const uint32_t it = n ? 3 - half : half;  // (0 and 3, 1 and 2: three steps each)
             f32x4 v[2] = {zero, zero};
 #pragma unroll
-            for (uint32_t t = 0; t <= it / 2; ++t) {
-                const Frag f = t_frag(it, t);
-                v[0] = mm3(kw[0][t], f, v[0]);
-                v[1] = mm3(kw[1][t], f, v[1]);
+            for (uint32_t t = 0; t <= n; ++t) {
+                const Frag g = t_frag(it, t);
+                v[0] = mm3(kw[0][t], g, v[0]);
+                v[1] = mm3(kw[1][t], g, v[1]);
             }
             const float down = ws.down * L.tinv[it];
             v[0] *= down;
             v[1] *= down;
-            const float top = wave_max(top4(top4(0.0f, v[0]), v[1]));
-            const Scale s = scale_of(top);
-            most = __builtin_fmaxf(most, top);
-            if (lane == 0) fac[kFW + 4 * it + w] = s.down;
-            float y[8];
-            __builtin_memcpy(y, v, 32);
-            store_frag(B.w + (it * NT + w) * 2048, split8(y, s.up));
-        }
-        if (lane == 0) fac[kFWMax + w] = most;
-    }
-    // U0: every fourth 16 columns of v
-    for (uint32_t cb0 = w; cb0 < dv / 16; cb0 += 8) {
-        if (cb0 != w) load_v(cb0);
-#pragma unroll
-        for (uint32_t m = 0; m < 2; ++m) {
-            const uint32_t cb = cb0 + 4 * m;
-            if (cb >= dv / 16) continue;
-            float x[2][8], top = 0.0f;
-#pragma unroll
-            for (int t = 0; t < 2; ++t)
-#pragma unroll
-                for (int n = 0; n < 8; ++n) {
-                    const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
-                    float v = vx[m][2 * t + n / 4][n & 3];
-                    __asm__("" : "+v"(v));  // (the load itself stays outside the choice)
-                    x[t][n] = j < c.live ? v * L.beta[j] : 0.0f;
-                    top = __builtin_fmaxf(top, __builtin_fabsf(x[t][n]));
-                }
-            const Scale s = scale_of(wave_max(top));
-            const Frag vf[2] = {split8(x[0], s.up), split8(x[1], s.up)};
-            float most = 0.0f;
-#pragma unroll
-            for (uint32_t it = 0; it < 4; ++it) {
-                f32x4 u = zero;
-#pragma unroll
-                for (uint32_t t = 0; t <= it / 2; ++t) u = mm3(t_frag(it, t), vf[t], u);
-                u *= s.down * L.tinv[it];
-                most = top4(most, u);
-                __builtin_memcpy(block + B.u + (cb * 4 + it) * 1024 + lane * 16, &u, 16);
+            const float most = wave_max(top4(top4(0.0f, v[0]), v[1]));
+            const Scale s = scale_of(most);
+            if (lane == 0) {
+                fac[kFW + 4 * it + w] = s.down;
+                fac[kFWMax + 4 * it + w] = most;
             }
-            most = wave_max(most);
-            if (lane == 0) fac[kFU + cb] = most;
+            float u[8];
+            __builtin_memcpy(u, v, 32);
+            store_frag(B.w + (it * NT + w) * 2048, split8(u, s.up));
         }
+    }
+    // U0
+    for (uint32_t cb = cb_first; has_v && cb < dv / 16; cb += 8) {
+        if (cb != cb_first) load_v(cb);
+        float y[2][8], most = 0.0f;
+#pragma unroll
+        for (int t = 0; t < 2; ++t)
+#pragma unroll
+            for (int n = 0; n < 8; ++n) {
+                const uint32_t j = 32 * t + 16 * (n / 4) + 4 * h + (n & 3);
+                float v = vx[2 * t + n / 4][n & 3];
+                __asm__("" : "+v"(v));  // (the load itself stays outside the choice)
+                y[t][n] = j < c.live ? v * L.beta[j] : 0.0f;
+                most = __builtin_fmaxf(most, __builtin_fabsf(y[t][n]));
+            }
+        const Scale s = scale_of(wave_max(most));
+        const Frag vf[2] = {split8(y[0], s.up), split8(y[1], s.up)};
+        most = 0.0f;
+#pragma unroll
+        for (uint32_t it = 0; it < 4; ++it) {
+            f32x4 u = zero;
+#pragma unroll
+            for (uint32_t t = 0; t <= it / 2; ++t) u = mm3(t_frag(it, t), vf[t], u);
+            u *= s.down * L.tinv[it];
+            most = top4(most, u);
+            __builtin_memcpy(block + B.u + (cb * 4 + it) * 1024 + lane * 16, &u, 16);
+        }
+        most = wave_max(most);
+        if (lane == 0) fac[kFU + cb] = most;
     }
 }
 
@@ -737,7 +743,7 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
         struct Ahead {
             Frag W[NT], K[2][2];
             f32x4 u0[NC];
-            float f;
+            float f, wmax;
         } ahead[2];
         auto load_first = [&](uint32_t n, Ahead &x) {
             const uint8_t *b = block_of(n);
@@ -773,6 +779,9 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
         };
         auto chunk = [&](uint32_t n, Ahead &x) {
             float udown[NC];
+            // the largest of W of each slice: of the four tiles' factors, four lanes each
+            x.wmax = __builtin_fmaxf(x.f, dpp<0x124>(x.f));
+            x.wmax = __builtin_fmaxf(x.wmax, dpp<0x128>(x.wmax));
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 f32x4 u = x.u0[c];
@@ -782,7 +791,7 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
                     const Frag f = {sf[c][t][0][lane], sf[c][t][1][lane]};
                     const f32x4 v = mm3(x.W[t], f, (f32x4)0.0f);
                     u -= v * (lane_of(x.f, kFW - 64 + 4 * w + t) * sinv[c][t]);
-                    top = __builtin_fmaf(32.0f * lane_of(x.f, kFWMax - 64 + t), stop[c][t], top);
+                    top = __builtin_fmaf(32.0f * lane_of(x.wmax, t), stop[c][t], top);
                 }
                 // one scale for all of U: |U| is at most |U0| and 32 times the largest of W and S of each slice
                 const Scale z = scale_of(top);
@@ -931,7 +940,7 @@ template <int DK, int NC> void launch_chain(const DeltaArgs &a, hipStream_t stre
     hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.s.n_seq * a.n_heads * (a.v_dim / (16 * NC))), dim3(512), 0, stream, a);
 }
 template <int DK> void launch_chunks(const DeltaArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(a.slots * a.n_heads), dim3(256), sizeof(PrepareLds<DK>), stream, a);
+    hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(a.slots * a.n_heads), dim3(512), sizeof(PrepareLds<DK>), stream, a);
     if (a.tiles == 1) launch_chain<DK, 1>(a, stream);
     else if (a.tiles == 2) launch_chain<DK, 2>(a, stream);
     else launch_chain<DK, 4>(a, stream);
