@@ -140,9 +140,34 @@ AH_DEV bool list_fixed(const BlockArgs &b, const Query &x, uint32_t kvh, uint32_
     return false;
 }
 
+// The `top` largest of the keys of lanes in `valid` (of equal ones the first), by the bits from the highest on: `alive` are the
+// lanes still equal to the top-th as far as the bits go.  least: nothing chosen is smaller.
+AH_DEV bool largest(uint64_t key, uint64_t valid, uint32_t top, uint64_t &least) {
+    uint64_t alive = valid, taken = 0, prefix = 0;
+    uint32_t need = top;
+#pragma unroll
+    for (int word = 1; word >= 0; --word) {
+        const uint32_t v = (uint32_t)(key >> (32 * word));
+        for (int bit = 31; bit >= 0 && (uint32_t)__builtin_popcountll(alive) != need; --bit) {
+            const uint64_t ones = __builtin_amdgcn_ballot_w64((v >> bit & 1u) != 0) & alive;
+            const uint32_t c = (uint32_t)__builtin_popcountll(ones);
+            if (c >= need) {
+                alive = ones;
+                prefix |= 1ull << (32 * word + bit);
+            } else {
+                taken |= ones;
+                need -= c;
+                alive &= ~ones;
+            }
+        }
+    }
+    least = prefix;
+    const uint64_t me = 1ull << (threadIdx.x & 63);
+    return (taken & me) || ((alive & me) && __builtin_amdgcn_mbcnt_hi((uint32_t)(alive >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)alive, 0)) < need);
+}
 // The choice among n > top keys by one wave: emit(place, block) for the chosen ones, ascending.  With top at most 64, the top-th of
 // the lanes' largest keys bounds the top-th of all from below, and few keys pass it; where no more than 64 do, a lane each,
-// the rest is ballots.  false: it is left to many_keys.
+// those are chosen among.  false: it is left to many_keys.
 template <class K, class E> AH_DEV bool few_keys(uint32_t n, uint32_t top, uint64_t *room, K key_at, E emit) {
     constexpr uint32_t kBatch = 8;  // keys of a lane on their way
     if (top > 64) return false;
@@ -161,8 +186,8 @@ template <class K, class E> AH_DEV bool few_keys(uint32_t n, uint32_t top, uint6
 #pragma unroll
         for (uint32_t j = 0; j < kBatch; ++j) most = k[j] > most ? k[j] : most;
     }
-    uint32_t found;
-    const uint64_t bound = threshold(top, 64, [&](uint64_t x) { return count(most >= x); }, found);
+    uint64_t bound, least;
+    (void)largest(most, ~0ull, top, bound);
     uint32_t c = 0;
     for (uint32_t base = 0; base < n; base += 64 * kBatch) {
         if (n > 64 * kBatch) batch(base);
@@ -180,11 +205,7 @@ template <class K, class E> AH_DEV bool few_keys(uint32_t n, uint32_t top, uint6
     }
     if (c > 64) return false;
     __builtin_amdgcn_wave_barrier();
-    const uint64_t mine = lane < c ? room[lane] : 0;
-    const uint64_t T = threshold(top, c, [&](uint64_t x) { return count(lane < c && mine >= x); }, found);
-    const bool above = lane < c && mine > T, same = lane < c && mine == T;
-    const uint32_t ties = top - count(above);
-    const bool in = above || (same && before(same) < ties);
+    const bool in = largest(lane < c ? room[lane] : 0, c == 64 ? ~0ull : (1ull << c) - 1, top, least);
     if (in) emit(before(in), (uint32_t)room[64 + lane]);
     return true;
 }
@@ -322,12 +343,12 @@ template <int D> __global__ void __launch_bounds__(1024) block_choice_kernel(Blo
 
 // A workgroup for 16 tokens of a sequence and a KV head: scores of 16 blocks and the 16 tokens by f64 matrix products (lane
 // (r, h): token r, blocks h + 4 i of the result), then a token's choice by one wave.
-constexpr uint32_t kSomeWaves = 8;
-template <int D> __global__ void __launch_bounds__(64 * kSomeWaves) block_choices_kernel(BlockArgs b) {
+template <int D> constexpr uint32_t kSomeWaves = D == 256 ? 8 : 16;  // (as many as the registers allow)
+template <int D> __global__ void __launch_bounds__(64 * kSomeWaves<D>) block_choices_kernel(BlockArgs b) {
     typedef double f64x4 __attribute__((ext_vector_type(4)));
     constexpr int Q = D / 4;  // channels of a lane's quarter
     extern __shared__ uint64_t lds[];
-    __shared__ uint64_t room[kSomeWaves][128];
+    __shared__ uint64_t room[kSomeWaves<D>][128];
     const AttnArgs &a = b.a;
     const uint32_t at = blockIdx.x / a.c.n_kv, kvh = blockIdx.x - at * a.c.n_kv, lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
@@ -347,7 +368,7 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves) block_choice
     const uint32_t tok0 = p.q0 + 16 * tile, live = p.nq - 16 * tile < 16 ? p.nq - 16 * tile : 16;
     const uint32_t most = query_of(b, p, s, tok0 + live - 1).n;  // (the last token's: the most)
     if (most > b.top) {
-        for (uint32_t i = threadIdx.x; i < 16 * D; i += 64 * kSomeWaves) {
+        for (uint32_t i = threadIdx.x; i < 16 * D; i += 64 * kSomeWaves<D>) {
             const uint32_t t = i / D, c = i % D;
             const float *x = a.q + (size_t)(tok0 + (t < live ? t : 0)) * a.q_stride + (size_t)kvh * a.group * D + c;
             double v = 0.0;
@@ -359,7 +380,7 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves) block_choice
         double q[Q];
 #pragma unroll
         for (int i = 0; i < Q; ++i) q[i] = qs[r * (D + 2) + h * Q + i];
-        for (uint32_t base = 16 * wave; base < most; base += 16 * kSomeWaves) {
+        for (uint32_t base = 16 * wave; base < most; base += 16 * kSomeWaves<D>) {
             const uint32_t i = base + r, block = b.first + (i < most ? i : most - 1), page = page_of(b, s, block);
             const bool ok = page < a.c.n_pages;
             _Float16 m[Q];
@@ -376,7 +397,7 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves) block_choice
         }
         __syncthreads();
     }
-    for (uint32_t t = wave; t < live; t += kSomeWaves) {
+    for (uint32_t t = wave; t < live; t += kSomeWaves<D>) {
         const uint32_t tok = tok0 + t, unit = tok * a.c.n_kv + kvh;
         const Query x = query_of(b, p, s, tok);
         uint32_t *list = b.list + (size_t)unit * a.list_stride;
@@ -560,7 +581,7 @@ template <int D> void launch_choice(const BlockArgs &a, hipStream_t stream) {
         hipLaunchKernelGGL(block_choice_kernel<D>, dim3(a.a.n_tok * a.a.c.n_kv), dim3(1024), a.lds_keys * sizeof(uint64_t), stream, a);
         return;
     }
-    hipLaunchKernelGGL(block_choices_kernel<D>, dim3(a.tiles * a.a.c.n_kv), dim3(64 * kSomeWaves), 16 * (D + 2 + a.lds_keys + 1) * sizeof(uint64_t), stream, a);
+    hipLaunchKernelGGL(block_choices_kernel<D>, dim3(a.tiles * a.a.c.n_kv), dim3(64 * kSomeWaves<D>), 16 * (D + 2 + a.lds_keys + 1) * sizeof(uint64_t), stream, a);
 }
 
 hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream) {
