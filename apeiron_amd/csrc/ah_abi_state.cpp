@@ -38,14 +38,9 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *p, co
     a.silu = p->silu != 0;
     a.status = ctx->d_status;
     const size_t blocks = (C + 1023) / 1024, max_q = a.s.max_q ? a.s.max_q : 1;
-    // Tiles of 32 tokens; of 16 or 8 where those leave the CUs without four workgroups each.
     const bool even = n_tok == (size_t)a.s.n_seq * a.s.max_q || a.s.n_seq == 1;
-    size_t tiles = 0;
-    for (a.tile = 32;; a.tile /= 2) {
-        a.per = even ? (uint32_t)((max_q + a.tile - 1) / a.tile) : 0;
-        tiles = even ? (size_t)a.per * a.s.n_seq : n_tok / a.tile + a.s.n_seq;
-        if (a.tile == 8 || tiles * blocks >= 4 * (size_t)ctx->cu_count) break;
-    }
+    a.per = even ? (uint32_t)((max_q + kConvTile - 1) / kConvTile) : 0;
+    const size_t tiles = even ? (size_t)a.per * a.s.n_seq : n_tok / kConvTile + a.s.n_seq;
     if (tiles > kMaxGrid / blocks) return AH_ERR_INVALID_ARG;
     a.tiles = (uint32_t)tiles;
     AH_HIP(ctx, hipSetDevice(ctx->device));
@@ -93,23 +88,45 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
     a.norm_eps = p->norm_eps;
     a.status = ctx->d_status;
     AH_HIP(ctx, hipSetDevice(ctx->device));
-    // A sequence of up to 8 tokens goes token by token, a longer one by chunks.  Sequences of one length all go the same way.
-    const size_t most_steps = 8;
+    // A sequence of up to 8 tokens goes token by token, a longer one by chunks; the bound is 16 tokens where the batch gives
+    // every CU a head and 24 where it gives two.  (Heads of 128 x 128, us by tokens and by chunks: 16 heads, 8 tokens 24.6 and
+    // 23.9, 16 tokens 42 and 24; 256 heads, 16 tokens 51 and 57, 24 tokens 70 and 58; 512 heads, 24 tokens 76 and 90; 1024
+    // heads, 16 tokens 110 and 165, 32 tokens 193 and 171.)  Sequences of one length all go the same way.
+    const size_t cus = (size_t)ctx->cu_count, units = (size_t)a.s.n_seq * H, most_steps = units < cus ? 8 : units < 2 * cus ? 16 : 24;
     const bool chunks = a.s.max_q > most_steps, even = a.s.n_seq == 1 || n == (size_t)a.s.n_seq * a.s.max_q;
     a.chunk_from = !chunks ? 0xffffffffu : even ? 0 : (uint32_t)most_steps + 1;
     if (chunks) {
-        // slots for the chunks: one for every 64 tokens and one more for every sequence, or one for every 8 tokens
-        const size_t by_seq = n / kDeltaChunk + a.s.n_seq, by_tokens = n / most_steps + 1;
-        a.slot_seq = even || by_seq <= by_tokens;
-        a.slot_shift = a.slot_seq ? 6 : 3;
-        const size_t slots = a.slot_seq ? by_seq : by_tokens;
-        if (slots * H > kMaxGrid || (size_t)a.s.n_seq * H * (dv / 16) > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
-        a.slots = (uint32_t)slots;
-        const size_t most = (size_t)a.s.n_seq * H * (dv / 16);
-        a.tiles = most >= 4 * (size_t)ctx->cu_count ? 4 : most > (size_t)ctx->cu_count ? 2 : 1;
-        const int32_t st = ensure_scratch(ctx, slots * H * delta_block((uint32_t)dk, (uint32_t)dv).bytes, stream);
+        const size_t bytes = delta_block((uint32_t)dk, (uint32_t)dv).bytes, columns = units * (dv / 16), per = (a.s.max_q + kDeltaChunk - 1) / kDeltaChunk;
+        // A workgroup of the chain takes 16 columns of S; 32 or 64 where there are more of them than CUs and then than fill eight
+        // rounds: a chunk's block is read by fewer workgroups.  (16 heads of 128 x 128, us with 16, 32, 64: 1 x 64 tokens 25,
+        // 25, 30; 2 x 301 35, 39, 52; 5 x 301 66, 62, 63; 4 x 2048 274, 205, 336; 8 x 1024 326, 241, 246; 16 x 512 410, 284,
+        // 269; columns of 64: 64 x 512 1189, 801, 692.)
+        a.tiles = columns >= 8 * cus ? 4 : columns > cus ? 2 : 1;
+        // All chunks are prepared at once, or, where the chain leaves half of the CUs without work and the blocks would not
+        // stay in the 256 MB of the last cache, by groups of as many as give every CU one, the next group's preparation beside a
+        // group's chain.  (us at once and by groups: 16 heads, 4096 tokens (148 MB) 151 and 160, 6144 249 and 232, 8192 348 and
+        // 304, 32768 1275 and 1169; 8 heads, 8192 tokens 239 and 234, 12000 374 and 332, 16384 554 and 444.)
+        const size_t half = (cus + units - 1) / units;
+        size_t need;
+        if (even && columns <= cus / 2 && per * units * bytes > ((size_t)192 << 20)) {
+            a.ring = 2 * (uint32_t)half;
+            need = align256(a.s.n_seq * (size_t)a.ring * H * bytes) + units * dk * dv * sizeof(float);
+        } else {
+            // Slots for the chunks: one for every 64 tokens and one more for every sequence, or one for every 8 tokens, which is
+            // fewer where most sequences have a few tokens (1024 of one token and one of 512, 8 heads: 0.2 GB rather than 1.2,
+            // the time is the same).
+            const size_t by_seq = n / kDeltaChunk + a.s.n_seq, by_tokens = n / 8 + 1;
+            a.slot_seq = even || by_seq <= by_tokens;
+            a.slot_shift = a.slot_seq ? 6 : 3;
+            const size_t slots = a.slot_seq ? by_seq : by_tokens;
+            if (slots * H > kMaxGrid / 2 || columns > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
+            a.slots = (uint32_t)slots;
+            need = slots * H * bytes;
+        }
+        const int32_t st = ensure_scratch(ctx, need, stream);
         if (st) return st;
         a.blocks = static_cast<uint8_t *>(ctx->scratch.p);
+        if (a.ring) a.carry = reinterpret_cast<float *>(a.blocks + align256(a.s.n_seq * (size_t)a.ring * H * bytes));
     }
     AH_HIP(ctx, ah_launch_delta(a, !chunks || !even, chunks, pick(ctx, stream)));
     return AH_OK;

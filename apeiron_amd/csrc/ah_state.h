@@ -9,14 +9,14 @@ struct StateSeqs {
     uint32_t n_seq, n_tok, max_q, n_slots;
 };
 
-constexpr uint32_t kConvMaxWidth = 8;
+constexpr uint32_t kConvMaxWidth = 8, kConvTile = 8;  // tokens of a workgroup: W - 1 at least
 struct ConvArgs {
     StateSeqs s;
     const float *x, *weight, *bias;
     float *y, *state;
     uint64_t x_stride, y_stride;
     uint32_t n_ch, width, silu;
-    uint32_t tile, tiles, per;  // tokens of a workgroup, numbers that workgroups of tokens have, those of every sequence (0: they differ)
+    uint32_t tiles, per;  // numbers that tiles of tokens have, those of every sequence (0: they differ)
     unsigned long long *status;
 };
 
@@ -33,6 +33,10 @@ struct DeltaArgs {
     uint32_t chunk_from, slots, slot_shift, slot_seq;
     uint32_t tiles;  // of 16 columns of S for a workgroup of the chain: 1, 2 or 4
     uint8_t *blocks;
+    // By groups of ring / 2 chunks (0: all at once): what a launch's chain begins with, its workgroups, the first chunk that it
+    // prepares, and S of every (sequence, head) between two launches.
+    uint32_t ring, begin, chain_grid, prepared;
+    float *carry;
     unsigned long long *status;
 };
 

@@ -41,10 +41,14 @@ AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 
 // ---- the short causal convolution --------------------------------------------------------------------
 //
-// y_t = act(bias + sum_i w_i x_(t - W + 1 + i)), a lane four channels of a tile of consecutive tokens: it keeps the
-// W - 1 rows before the next one in registers and has eight rows on their way, so a row is read once a tile and the rows before a
-// tile once more.  The tile that holds a sequence's first token alone reads the state and also writes the new one, so that both
-// may lie in the same slot.  Rows come and go through range-checked resources: no branch stands between the loads.
+// y_t = act(bias + sum_i w_i x_(t - W + 1 + i)).  A lane has four channels of a tile of eight tokens: it asks for the tile's
+// rows and the W - 1 before them at once, so that no load waits for another.  Bytes bound it: x once, y once; the rows
+// before a tile come from L2 a second time.  (64 to 8192 tokens of 1024 to 6144 channels: tiles of 8 86 us, of 16 91, of 32 93 at
+// 8192 x 6144, 13.9, 15.9 and 21.9 at 512 x 6144, the smallest never behind by more than the noise.)  8192 x 6144 takes 86 us,
+// 4.7 TB/s of the 5.0 that a copy reaches; a token of 64 sequences 2.9 us.  The tile that holds a sequence's first token
+// alone reads the state and also writes the new one, so that both may lie in the same slot.  Rows come and go through
+// range-checked resources: no branch stands between the loads.
+static_assert(kConvTile >= kConvMaxWidth - 1, "the rows before a tile lie in the one before it");
 AH_DEV f32x4 ld4(__amdgpu_buffer_rsrc_t r, uint32_t at) { return __builtin_bit_cast(f32x4, ah_ld128(r, 4 * at)); }
 AH_DEV void st4(__amdgpu_buffer_rsrc_t r, uint32_t at, f32x4 v, uint32_t take) {
     if (take == 4) {
@@ -59,7 +63,6 @@ AH_DEV void st4(__amdgpu_buffer_rsrc_t r, uint32_t at, f32x4 v, uint32_t take) {
 }
 
 template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) {
-    constexpr uint32_t kRows = 8;  // on their way
     const uint32_t at = blockIdx.x % a.tiles, block = blockIdx.x / a.tiles, c0 = 4 * (block * 256 + threadIdx.x);
     const uint32_t take = c0 >= a.n_ch ? 0 : a.n_ch - c0 < 4 ? a.n_ch - c0 : 4;
     const __amdgpu_buffer_rsrc_t wr = ah_rsrc(a.weight, 4 * a.n_ch * W);
@@ -71,26 +74,26 @@ template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) 
     }
     f32x4 bias = (f32x4)0.0f;
     if (a.bias) bias = ld4(ah_rsrc(a.bias, 4 * a.n_ch), c0);
-    auto start = [&](uint32_t i) { return (uint32_t)a.s.q_start[i] / a.tile + i; };
+    auto start = [&](uint32_t i) { return (uint32_t)a.s.q_start[i] / kConvTile + i; };
     auto holds = [&](uint32_t i) {
         const Seq p = seq_of(a.s, i);
-        return !p.bad && at >= start(i) && at - start(i) < (p.nq ? (p.nq + a.tile - 1) / a.tile : 1);
+        return !p.bad && at >= start(i) && at - start(i) < (p.nq ? (p.nq + kConvTile - 1) / kConvTile : 1);
     };
     const uint32_t s = a.per ? at / a.per : sequence_among(a.s.q_start, a.s.n_seq, a.s.n_tok, at, start, holds), n = at - (a.per ? s * a.per : start(s));
     const Seq p = seq_of(a.s, s);
-    const uint32_t t0 = n * a.tile;
+    const uint32_t t0 = n * kConvTile;
     if (!p.bad && (n == 0 || t0 < p.nq)) {
-        const uint32_t rows = t0 >= p.nq ? 0 : p.nq - t0 < a.tile ? p.nq - t0 : a.tile, x_stride = (uint32_t)a.x_stride, y_stride = (uint32_t)a.y_stride;
+        const uint32_t rows = t0 >= p.nq ? 0 : p.nq - t0 < kConvTile ? p.nq - t0 : kConvTile, x_stride = (uint32_t)a.x_stride, y_stride = (uint32_t)a.y_stride;
         const uint32_t back = n ? W - 1 : 0;  // rows of the tile before this one (a tile has at least as many)
         const __amdgpu_buffer_rsrc_t xr = ah_rsrc(a.x + (size_t)(p.q0 + t0 - back) * a.x_stride, rows + back ? 4 * ((rows + back - 1) * x_stride + a.n_ch) : 0);
         const __amdgpu_buffer_rsrc_t yr = ah_rsrc(a.y + (size_t)(p.q0 + t0) * a.y_stride, rows ? 4 * ((rows - 1) * y_stride + a.n_ch) : 0);
         const uint32_t slot = 4 * (W - 1) * a.n_ch;
         const __amdgpu_buffer_rsrc_t old = ah_rsrc(a.state + (size_t)(p.from < 0 ? 0 : p.from) * (W - 1) * a.n_ch, p.from < 0 ? 0 : slot);
-        f32x4 row[W - 1], ahead[kRows];
+        f32x4 row[W - 1], now[kConvTile];
 #pragma unroll
         for (uint32_t j = 0; j < W - 1; ++j) row[j] = n ? ld4(xr, j * x_stride + c0) : ld4(old, j * a.n_ch + c0);
 #pragma unroll
-        for (uint32_t j = 0; j < kRows; ++j) ahead[j] = ld4(xr, (back + j) * x_stride + c0);
+        for (uint32_t j = 0; j < kConvTile; ++j) now[j] = ld4(xr, (back + j) * x_stride + c0);
         if (n == 0 && p.to >= 0) {  // the last W - 1 of the state's rows and the sequence's
             const __amdgpu_buffer_rsrc_t to = ah_rsrc(a.state + (size_t)p.to * (W - 1) * a.n_ch, slot);
             const uint32_t first = p.nq < W - 1 ? 0 : p.nq - (W - 1);
@@ -103,29 +106,22 @@ template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) 
             for (uint32_t j = 0; j < W - 1; ++j) st4(to, j * a.n_ch + c0, kept[j], take);
         }
         bool odd = false;
-        for (uint32_t t = 0; t < rows; t += kRows) {
-            f32x4 now[kRows];
 #pragma unroll
-            for (uint32_t j = 0; j < kRows; ++j) now[j] = ahead[j];
+        for (uint32_t j = 0; j < kConvTile; ++j) {
+            f32x4 out;
 #pragma unroll
-            for (uint32_t j = 0; j < kRows; ++j) ahead[j] = ld4(xr, (back + t + kRows + j) * x_stride + c0);
+            for (int i = 0; i < 4; ++i) {
+                float v = bias[i];
 #pragma unroll
-            for (uint32_t j = 0; j < kRows; ++j) {
-                f32x4 out;
-#pragma unroll
-                for (int i = 0; i < 4; ++i) {
-                    float v = bias[i];
-#pragma unroll
-                    for (int k = 0; k < W - 1; ++k) v = __builtin_fmaf(w[i * W + k], row[k][i], v);
-                    v = __builtin_fmaf(w[i * W + W - 1], now[j][i], v);
-                    odd = odd || ((uint32_t)i < take && t + j < rows && !finite(v));
-                    out[i] = a.silu ? silu(v) : v;
-                }
-                if (t + j < rows) st4(yr, (t + j) * y_stride + c0, out, take);
-#pragma unroll
-                for (int k = 0; k + 1 < W - 1; ++k) row[k] = row[k + 1];
-                row[W - 2] = now[j];
+                for (int k = 0; k < W - 1; ++k) v = __builtin_fmaf(w[i * W + k], row[k][i], v);
+                v = __builtin_fmaf(w[i * W + W - 1], now[j][i], v);
+                odd = odd || ((uint32_t)i < take && j < rows && !finite(v));
+                out[i] = a.silu ? silu(v) : v;
             }
+            if (j < rows) st4(yr, j * y_stride + c0, out, take);
+#pragma unroll
+            for (int k = 0; k + 1 < W - 1; ++k) row[k] = row[k + 1];
+            row[W - 2] = now[j];
         }
         if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
     }
@@ -361,17 +357,12 @@ template <int DK> struct PrepareLds {
 // Eight waves a chunk and head.  Waves 0 to 3 have the keys and beta_i k_i . k_j of 16 tokens i each, and make T of them; waves 4 to
 // 7 have q of the same tokens, P and q's fragments.  W and U0 are shared by all.  Barriers wait for LDS alone: loads and stores stay
 // on their way.
-template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel(DeltaArgs a) {
+template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32_t hd, uint8_t *block, PrepareLds<DK> &L) {
     constexpr int NT = DK / 32;
-    extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
-    PrepareLds<DK> &L = *reinterpret_cast<PrepareLds<DK> *>(lds_bytes);
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
     const bool keys = wave < 4;
-    const uint32_t at = blockIdx.x / a.n_heads, hd = blockIdx.x - at * a.n_heads, kh = hd / a.group, dv = a.v_dim;
-    const Chunk c = chunk_of(a, at);
-    if (c.live == 0) return;
+    const uint32_t kh = hd / a.group, dv = a.v_dim;
     const DeltaBlock B = delta_block(DK, dv);
-    uint8_t *block = a.blocks + ((size_t)at * a.n_heads + hd) * B.bytes;
     float *fac = reinterpret_cast<float *>(block + B.f);
     typedef Rows<DK> R;
     R x;
@@ -696,42 +687,65 @@ template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel
         if (lane == 0) fac[kFU + cb] = most;
     }
 }
+template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel(DeltaArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
+    const uint32_t at = blockIdx.x / a.n_heads, hd = blockIdx.x - at * a.n_heads;
+    const Chunk c = chunk_of(a, at);
+    if (c.live) prepare<DK>(a, c, hd, a.blocks + ((size_t)at * a.n_heads + hd) * delta_block(DK, a.v_dim).bytes, *reinterpret_cast<PrepareLds<DK> *>(lds_bytes));
+}
 
 // A sequence's chunks in turn, for NC times 16 columns of a head's S.  Waves 0 to 3 are the chain: wave w makes U of the tokens
 // 16 w .. 16 w + 15 (the first half of a chunk's time) and the rows of slice w of S (the second); what the others need goes
 // through LDS as operands.  Waves 4 to 7 make o of the same tokens: q S beside U, P U beside S.  Two barriers a chunk.
 //   What comes from memory is asked for two chunks ahead, and touched a few chunks before that, each of a head's workgroups a
 // part, so that it waits in the XCD's L2.
-template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_kernel(DeltaArgs a) {
+template <int DK, int NC> struct ChainLds {
+    u32x4 sf[NC][DK / 32][2][64], uf[NC][2][2][64];
+    float sinv[NC][4], stop[NC][4], uinv[NC];
+};
+template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC> &L) {
     constexpr int NT = DK / 32;
     constexpr uint32_t kTouch = 4;  // chunks
-    __shared__ u32x4 sf[NC][NT][2][64], uf[NC][2][2][64];
-    __shared__ float sinv[NC][4], stop[NC][4], uinv[NC];
+    auto &sf = L.sf;
+    auto &uf = L.uf;
+    auto &sinv = L.sinv;
+    auto &stop = L.stop;
+    auto &uinv = L.uinv;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
     // columns slowest: a head's workgroups go to one XCD (they go to the eight in turn) wherever eight divides the heads
     const uint32_t units = a.s.n_seq * a.n_heads, part = blockIdx.x / units, unit = blockIdx.x - part * units, s = unit / a.n_heads, hd = unit - s * a.n_heads;
     const Seq p = seq_of(a.s, s);
     if (p.bad && part == 0 && hd == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
     if (p.bad || p.nq < a.chunk_from) return;
-    const uint32_t chunks = (p.nq + kDeltaChunk - 1) / kDeltaChunk, dv = a.v_dim, cb = part * NC;
+    // this launch's chunks: begin .. chunks - 1 of `whole`
+    const uint32_t whole = (p.nq + kDeltaChunk - 1) / kDeltaChunk, begin = a.ring ? a.begin : 0, end = a.ring ? a.begin + a.ring / 2 : whole;
+    const uint32_t chunks = whole < end ? whole : end, dv = a.v_dim, cb = part * NC;
+    if (begin && begin >= whole) return;
     const DeltaBlock B = delta_block(DK, dv);
-    const size_t step = (size_t)a.n_heads * B.bytes, first = (((uint32_t)a.s.q_start[s] >> a.slot_shift) + s * a.slot_seq) * step + (size_t)hd * B.bytes;
-    auto block_of = [&](uint32_t n) { return a.blocks + first + (n < chunks ? n : chunks - 1) * step; };
+    const size_t step = (size_t)a.n_heads * B.bytes, first = (a.ring ? s * a.ring : ((uint32_t)a.s.q_start[s] >> a.slot_shift) + s * a.slot_seq) * step + (size_t)hd * B.bytes;
+    auto block_of = [&](uint32_t n) {
+        const uint32_t m = n < chunks ? n : chunks - 1;
+        return a.blocks + first + (a.ring ? m % a.ring : m) * step;
+    };
     auto frag = [&](const uint8_t *b) {
         Frag f;
         __builtin_memcpy(&f.hi, b + lane * 16, 16);
         __builtin_memcpy(&f.lo, b + 1024 + lane * 16, 16);
         return f;
     };
+    // S between a sequence's launches
+    float *carry = a.carry + (size_t)unit * DK * dv;
+    const float *old = begin ? carry : p.from >= 0 ? a.state + ((size_t)p.from * a.n_heads + hd) * DK * dv : nullptr;
+    float *now = chunks < whole ? carry : p.to >= 0 ? a.state + ((size_t)p.to * a.n_heads + hd) * DK * dv : nullptr;
     bool odd = false;
     if (wave < 4) {
         const bool own = w < (uint32_t)NT;
-        const size_t tile = ((size_t)hd * DK + 32 * w + 8 * h) * dv + 16 * cb + r, slot = (size_t)a.n_heads * DK * dv;
+        const size_t tile = (size_t)(32 * w + 8 * h) * dv + 16 * cb + r;
         f32x4 S[NC][2];
 #pragma unroll
         for (int c = 0; c < NC; ++c) S[c][0] = S[c][1] = (f32x4)0.0f;
-        if (own && p.from >= 0) {
-            const float *from = a.state + (size_t)p.from * slot + tile;
+        if (own && old) {
+            const float *from = old + tile;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -823,24 +837,24 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
             publish();
             ah_lds_barrier();
         };
-        if (chunks) {
+        if (chunks > begin) {
 #pragma unroll
             for (uint32_t n = 0; n < 2; ++n) {
-                load_first(n, ahead[n]);
+                load_first(begin + n, ahead[n]);
                 __builtin_amdgcn_sched_barrier(0);
-                load_second(n, ahead[n]);
+                load_second(begin + n, ahead[n]);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         publish();
         ah_lds_barrier();
-        for (uint32_t n = 0; n + 1 < chunks; n += 2) {
+        for (uint32_t n = begin; n + 1 < chunks; n += 2) {
             chunk(n, ahead[0]);
             chunk(n + 1, ahead[1]);
         }
-        if (chunks & 1) chunk(chunks - 1, ahead[0]);
-        if (own && p.to >= 0) {
-            float *to = a.state + (size_t)p.to * slot + tile;
+        if ((chunks - begin) & 1) chunk(chunks - 1, ahead[0]);
+        if (own && now) {
+            float *to = now + tile;
 #pragma unroll
             for (int c = 0; c < NC; ++c)
 #pragma unroll
@@ -916,30 +930,67 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
             x.touched = touch(n + kTouch);
             ah_lds_barrier();
         };
-        if (chunks) {
+        if (chunks > begin) {
 #pragma unroll
             for (uint32_t n = 0; n < 2; ++n) {
-                load_first(n, ahead[n]);
+                load_first(begin + n, ahead[n]);
                 __builtin_amdgcn_sched_barrier(0);
-                load_second(n, ahead[n]);
-                ahead[n].touched = touch(n + 2);
+                load_second(begin + n, ahead[n]);
+                ahead[n].touched = touch(begin + n + 2);
                 __builtin_amdgcn_sched_barrier(0);
             }
         }
         ah_lds_barrier();
-        for (uint32_t n = 0; n + 1 < chunks; n += 2) {
+        for (uint32_t n = begin; n + 1 < chunks; n += 2) {
             chunk(n, ahead[0]);
             chunk(n + 1, ahead[1]);
         }
-        if (chunks & 1) chunk(chunks - 1, ahead[0]);
+        if ((chunks - begin) & 1) chunk(chunks - 1, ahead[0]);
     }
     if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
+}
+template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_kernel(DeltaArgs a) {
+    __shared__ ChainLds<DK, NC> L;
+    chain<DK, NC>(a, L);
+}
+// The chain of one group of chunks beside the preparation of the next, where the chain leaves CUs to it: every sequence's chunks
+// begin .. begin + ring / 2 - 1 and, by the workgroups after the chain's, the ring / 2 after those.  The blocks of two groups
+// are there at once, [sequence][ring][head].
+template <int DK> __global__ void __launch_bounds__(512) delta_both_kernel(DeltaArgs a) {
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
+    __shared__ ChainLds<DK, 1> L;
+    if (blockIdx.x < a.chain_grid) {
+        chain<DK, 1>(a, L);
+        return;
+    }
+    const uint32_t half = a.ring / 2, at = blockIdx.x - a.chain_grid, hd = at % a.n_heads, i = at / a.n_heads, s = i / half, n = a.prepared + i % half;
+    const Seq p = seq_of(a.s, s);
+    if (p.bad || kDeltaChunk * n >= p.nq) return;
+    const uint32_t rest = p.nq - kDeltaChunk * n;
+    const Chunk c = {s, p.q0 + kDeltaChunk * n, rest < kDeltaChunk ? rest : kDeltaChunk};
+    prepare<DK>(a, c, hd, a.blocks + (((size_t)s * a.ring + n % a.ring) * a.n_heads + hd) * delta_block(DK, a.v_dim).bytes,
+                *reinterpret_cast<PrepareLds<DK> *>(lds_bytes));
 }
 
 template <int DK, int NC> void launch_chain(const DeltaArgs &a, hipStream_t stream) {
     hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.s.n_seq * a.n_heads * (a.v_dim / (16 * NC))), dim3(512), 0, stream, a);
 }
+// Groups of chunks: each launch has the chain of one and the preparation of the next.
+template <int DK> void launch_groups(DeltaArgs a, hipStream_t stream) {
+    const uint32_t half = a.ring / 2, all = (a.s.max_q + kDeltaChunk - 1) / kDeltaChunk, groups = (all + half - 1) / half;
+    const uint32_t chain_grid = a.s.n_seq * a.n_heads * (a.v_dim / 16), prepare_grid = a.s.n_seq * half * a.n_heads;
+    for (uint32_t g = 0; g <= groups; ++g) {
+        a.begin = g ? (g - 1) * half : 0;
+        a.chain_grid = g ? chain_grid : 0;
+        a.prepared = g * half;
+        hipLaunchKernelGGL(delta_both_kernel<DK>, dim3(a.chain_grid + (g < groups ? prepare_grid : 0)), dim3(512), sizeof(PrepareLds<DK>), stream, a);
+    }
+}
 template <int DK> void launch_chunks(const DeltaArgs &a, hipStream_t stream) {
+    if (a.ring) {
+        launch_groups<DK>(a, stream);
+        return;
+    }
     hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(a.slots * a.n_heads), dim3(512), sizeof(PrepareLds<DK>), stream, a);
     if (a.tiles == 1) launch_chain<DK, 1>(a, stream);
     else if (a.tiles == 2) launch_chain<DK, 2>(a, stream);
@@ -979,7 +1030,10 @@ hipError_t ah_launch_delta(const DeltaArgs &a, bool steps, bool chunks, hipStrea
 }
 
 hipError_t ah_state_init_attrs() {
-    const hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void *>(delta_prepare_kernel<64>), hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PrepareLds<64>));
-    return e != hipSuccess ? e : hipFuncSetAttribute(reinterpret_cast<const void *>(delta_prepare_kernel<128>), hipFuncAttributeMaxDynamicSharedMemorySize,
-                                                     (int)sizeof(PrepareLds<128>));
+    hipError_t e = hipSuccess;
+    for (const void *k : {(const void *)delta_prepare_kernel<64>, (const void *)delta_both_kernel<64>})
+        if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PrepareLds<64>));
+    for (const void *k : {(const void *)delta_prepare_kernel<128>, (const void *)delta_both_kernel<128>})
+        if (e == hipSuccess) e = hipFuncSetAttribute(k, hipFuncAttributeMaxDynamicSharedMemorySize, (int)sizeof(PrepareLds<128>));
+    return e;
 }
