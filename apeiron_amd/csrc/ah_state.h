@@ -33,9 +33,10 @@ struct DeltaArgs {
     uint32_t chunk_from, slots, slot_shift, slot_seq;
     uint32_t tiles;  // of 16 columns of S for a workgroup of the chain: 1, 2 or 4
     uint8_t *blocks;
-    // By groups of ring / 2 chunks (0: all at once): what a launch's chain begins with, its workgroups, the first chunk that it
-    // prepares, and S of every (sequence, head) between two launches.
-    uint32_t ring, begin, chain_grid, prepared;
+    uint32_t chain_grid;  // workgroups of the chain; a launch may have others after them
+    // By groups of ring / 2 chunks (0: all at once): what a launch's chain begins with, the first chunk that it prepares, and S
+    // of every (sequence, head) between two launches.
+    uint32_t ring, begin, prepared;
     float *carry;
     unsigned long long *status;
 };

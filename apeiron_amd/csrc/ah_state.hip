@@ -145,10 +145,9 @@ AH_DEV float softplus(float x) { return __builtin_fmaxf(x, 0.0f) + log1pf(expf(-
 AH_DEV float decay_of(const DeltaArgs &a, float x, uint32_t h) { return a.a_log ? -expf(a.a_log[h]) * softplus(x + a.dt_bias[h]) : x; }
 AH_DEV float rate_of(const DeltaArgs &a, float x) { return a.a_log ? 1.0f / (1.0f + expf(-x)) : x; }
 
-template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(DeltaArgs a) {
+template <int DK> AH_DEV void steps(const DeltaArgs &a, uint32_t unit) {  // a wave's (sequence, head, 32 columns)
     constexpr int R = DK / 8;
-    const uint32_t lane = threadIdx.x & 63, r = lane >> 3, c = lane & 7;
-    const uint32_t unit = 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), nvb = a.v_dim / 32;
+    const uint32_t lane = threadIdx.x & 63, r = lane >> 3, c = lane & 7, nvb = a.v_dim / 32;
     const uint32_t vb = unit % nvb, h = unit / nvb % a.n_heads, s = unit / nvb / a.n_heads;
     if (s >= a.s.n_seq) return;
     const Seq p = seq_of(a.s, s);
@@ -211,6 +210,10 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
         for (int i = 0; i < R; ++i) __builtin_memcpy(to + (size_t)i * a.v_dim, &S[i], 16);
     }
     if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
+}
+
+template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(DeltaArgs a) {
+    steps<DK>(a, 4 * blockIdx.x + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 }
 
 // ---- the gated delta rule, by chunks -----------------------------------------------------------------
@@ -951,7 +954,8 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
 }
 template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_kernel(DeltaArgs a) {
     __shared__ ChainLds<DK, NC> L;
-    chain<DK, NC>(a, L);
+    if (blockIdx.x < a.chain_grid) chain<DK, NC>(a, L);
+    else steps<DK>(a, 8 * (blockIdx.x - a.chain_grid) + __builtin_amdgcn_readfirstlane(threadIdx.x >> 6));
 }
 // The chain of one group of chunks beside the preparation of the next, where the chain leaves CUs to it: every sequence's chunks
 // begin .. begin + ring / 2 - 1 and, by the workgroups after the chain's, the ring / 2 after those.  The blocks of two groups
@@ -972,8 +976,11 @@ template <int DK> __global__ void __launch_bounds__(512) delta_both_kernel(Delta
                 *reinterpret_cast<PrepareLds<DK> *>(lds_bytes));
 }
 
-template <int DK, int NC> void launch_chain(const DeltaArgs &a, hipStream_t stream) {
-    hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.s.n_seq * a.n_heads * (a.v_dim / (16 * NC))), dim3(512), 0, stream, a);
+// The chain, and in the workgroups after it, where the lengths differ, the sequences that go token by token.
+template <int DK, int NC> void launch_chain(DeltaArgs a, bool mixed, hipStream_t stream) {
+    const uint32_t units = a.s.n_seq * a.n_heads;
+    a.chain_grid = units * (a.v_dim / (16 * NC));
+    hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.chain_grid + (mixed ? (units * (a.v_dim / 32) + 7) / 8 : 0)), dim3(512), 0, stream, a);
 }
 // Groups of chunks: each launch has the chain of one and the preparation of the next.
 template <int DK> void launch_groups(DeltaArgs a, hipStream_t stream) {
@@ -986,15 +993,15 @@ template <int DK> void launch_groups(DeltaArgs a, hipStream_t stream) {
         hipLaunchKernelGGL(delta_both_kernel<DK>, dim3(a.chain_grid + (g < groups ? prepare_grid : 0)), dim3(512), sizeof(PrepareLds<DK>), stream, a);
     }
 }
-template <int DK> void launch_chunks(const DeltaArgs &a, hipStream_t stream) {
+template <int DK> void launch_chunks(const DeltaArgs &a, bool mixed, hipStream_t stream) {
     if (a.ring) {
         launch_groups<DK>(a, stream);
         return;
     }
     hipLaunchKernelGGL(delta_prepare_kernel<DK>, dim3(a.slots * a.n_heads), dim3(512), sizeof(PrepareLds<DK>), stream, a);
-    if (a.tiles == 1) launch_chain<DK, 1>(a, stream);
-    else if (a.tiles == 2) launch_chain<DK, 2>(a, stream);
-    else launch_chain<DK, 4>(a, stream);
+    if (a.tiles == 1) launch_chain<DK, 1>(a, mixed, stream);
+    else if (a.tiles == 2) launch_chain<DK, 2>(a, mixed, stream);
+    else launch_chain<DK, 4>(a, mixed, stream);
 }
 
 template <int W> hipError_t launch_conv(const ConvArgs &a, hipStream_t stream) {
@@ -1017,15 +1024,14 @@ hipError_t ah_launch_conv(const ConvArgs &a, hipStream_t stream) {
 }
 
 hipError_t ah_launch_delta(const DeltaArgs &a, bool steps, bool chunks, hipStream_t stream) {
-    const uint32_t units = a.s.n_seq * a.n_heads * (a.v_dim / 32);
-    if (steps) {
-        if (a.k_dim == 64) hipLaunchKernelGGL(delta_step_kernel<64>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
-        else hipLaunchKernelGGL(delta_step_kernel<128>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
-    }
     if (chunks) {
-        if (a.k_dim == 64) launch_chunks<64>(a, stream);
-        else launch_chunks<128>(a, stream);
+        if (a.k_dim == 64) launch_chunks<64>(a, steps, stream);
+        else launch_chunks<128>(a, steps, stream);
+        return hipGetLastError();
     }
+    const uint32_t units = a.s.n_seq * a.n_heads * (a.v_dim / 32);
+    if (a.k_dim == 64) hipLaunchKernelGGL(delta_step_kernel<64>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
+    else hipLaunchKernelGGL(delta_step_kernel<128>, dim3((units + 3) / 4), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
 
