@@ -432,11 +432,14 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         x.grid = (uint32_t)(units * x.splits);
         return units <= max_grid(256) / 2 / x.splits;
     };
-    // The prefix: the whole batch as one sequence.
+    // The prefix: the whole batch as one sequence, by units of 16 rows, or of 128 with the tiles in LDS once there are many (2 KV
+    // heads behind 8192 keys, rows of a KV head, 16 and 128 a unit, us: heads of 128, 48 rows 17 and 21, 384 28 and 37, 768 37
+    // and 43, 1536 55 and 61, 1764 72 and 60; of 64, 1400 36 and 38, 1715 48 and 41; of 256, 1024 66 and 80, 1568 94 and 95,
+    // 1960 113 and 108).
     pre.n_seq = 1;
     pre.table = d_prefix_table;
     pre.table_stride = (uint32_t)((prefix_len - 1) >> a.c.page_shift) + 1;
-    pre.rows = batch <= 128 ? 16 : 128;
+    pre.rows = batch <= 1536 ? 16 : 128;
     const size_t units = (batch + pre.rows - 1) / pre.rows, all = (prefix_len + 31) / 32;
     pre.per = (uint32_t)units;
     // Pieces by the time that they take, as attn_tiles has it: workgroups in rounds, and a piece's results written and read.
@@ -457,12 +460,15 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         }
     }
     if (!cut(pre, units * kv, all, pieces)) return AH_ERR_INVALID_ARG;
-    // What follows it: each sequence for itself.
+    // What follows it: each sequence for itself, by units of 8 or 16 rows, or of 128 from twelve of 16 a CU on (2 KV heads of 128,
+    // sequences x tokens and their keys, units, us by 16 and by 128: 16 x 128 of 128 1536 100 and 112; 64 x 49 of 2048 2432 181
+    // and 186; 16 x 256 of 256 3072 191 and 189; 32 x 128 of 128 3072 109 and 103; 32 x 256 of 256 6144 213 and 189; 16 x 512 of
+    // 512 6144 242 and 198).
     const size_t per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
     const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
     own.rows = per_seq <= 8 ? 8 : 16;
     size_t own_units = (per_seq + own.rows - 1) / own.rows * kv * a.n_seq;
-    if (per_seq > 128 && tiles > 64) {
+    if (own_units >= 12 * cus) {
         own.rows = 128;
         own.per = (size_t)a.n_tok == (size_t)a.n_seq * a.max_q || a.n_seq == 1 ? (uint32_t)((per_seq + 127) / 128) : 0;
         own_units = (own.per ? (size_t)own.per * a.n_seq : ((size_t)a.n_tok * a.group >> 7) + a.n_seq) * kv;
@@ -524,12 +530,17 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     a.block_shift = b.shift - 5;
     b.most = (uint32_t)all;
     b.lds_keys = (uint32_t)(all < kLdsKeys ? all : kLdsKeys);
-    // A few tokens of a sequence and more are chosen for together, where 16 tokens' scores fit LDS.
-    const bool together = a.max_q >= 4 && 16 * (a.c.dim + 2 + all + 1) <= kLdsKeys;
+    // Where 16 tokens' scores fit LDS, 16 tokens of a sequence are chosen for together once every CU has two (token, KV
+    // head)s (four with heads of 256, whose workgroups are smaller).  2 KV heads, 8192 keys, us a token for itself and together:
+    // heads of 128, 128 tokens of a sequence 35 and 42, 256 51 and 51, 512 88 and 62, 64 x 4 55 and 50; of 256, 256 tokens 71
+    // and 81, 512 124 and 97.  (Tiles of one or two tokens: 512 x 1 104 and 112, 128 x 2 56 and 62.)
+    const bool together = a.max_q >= 4 && units >= (a.c.dim == 256 ? 4 : 2) * (size_t)ctx->cu_count && 16 * (a.c.dim + 2 + all + 1) <= kLdsKeys;
     b.tiles = together ? a.n_tok / 16 + a.n_seq : 0;
     if ((size_t)b.tiles * a.c.n_kv > max_grid(1024) || (!together && units > max_grid(1024))) return AH_ERR_INVALID_ARG;
     const size_t keys_at = align256(units * a.list_stride * sizeof(uint32_t)), kept = keys_at + (all > kLdsKeys ? align256(units * all * sizeof(uint64_t)) : 0);
-    // Up to eight queries a KV head, and lists enough for four waves a CU and more: a wave each.
+    // Up to eight queries a KV head, and lists enough for four waves a CU and more: a wave each.  (us with a wave each and in
+    // pieces, 2 KV heads, lists of 1152 keys: heads of 64, 512 lists 46 and 39, 1024 49 and 52; of 128 61 and 53, 63 and 74; of
+    // 256 94 and 83, 98 and 119.)
     const bool alone = a.group <= 8 && together && units >= 4 * (size_t)ctx->cu_count;
     a.seqs = together ? a.n_seq : 0;
     AttnArgs rows = a;

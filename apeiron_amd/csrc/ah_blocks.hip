@@ -129,7 +129,7 @@ AH_DEV bool list_fixed(const BlockArgs &b, const Query &x, uint32_t kvh, uint32_
     if (x.n <= b.top) {
         const uint32_t all = x.pos < 0 ? 0 : x.own + 1;
         for (uint32_t i = lane; i < all; i += lanes) list[1 + i] = entry_of(b, x.s, kvh, i);
-        if (lane == 0) list[0] = (uint32_t)(x.pos + 1);
+        if (lane == 0) list[0] = x.pos < 0 ? 0 : (uint32_t)x.pos + 1;
         if (chosen)
             for (uint32_t i = lane; i < b.top; i += lanes) chosen[i] = i < x.n ? (int32_t)(b.first + i) : -1;
         return true;

@@ -158,6 +158,37 @@ def test_shared_prefix_of_large_scores_and_longer_contexts_than_planned(dev, dim
             compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], np.broadcast_to(see, (B.qs[s], 2, ctx[s])), B.scale)
 
 
+MANY = [  # (head_dim, KV heads, queries of each, tokens, what follows the prefix of each sequence, prefix)
+    (64, 1, 7, [50, 1, 0, 128, 64], [60, 1, 5, 128, 200], 133), (128, 1, 6, [90, 100, 70], [90, 100, 300], 640), (256, 2, 3, [300, 220], [333, 250], 31),
+    (64, 4, 16, [32, 31, 1, 0, 20] * 5, [32, 31, 1, 3, 90] * 5, 100), (128, 4, 16, [32] * 24, [32 + i % 3 for i in range(24)], 65),
+    (256, 8, 16, [16, 3, 16, 1] * 6, [16, 20, 70, 1] * 6, 64)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kv,G,qs,after,prefix", MANY)
+def test_shared_prefix_of_many_rows(dev, dim, kv, G, qs, after, prefix):  # noqa: F811
+    """More than 1536 rows of a KV head behind the prefix, and sequences of many rows."""
+    ctx = [prefix + n for n in after]
+    B = Batch(dev, qs, ctx, kv, G, dim, 32, prefix=prefix, seed=dim, pad=3)
+    status, out = B.shared()
+    assert status == OK and (out[:, B.heads * dim:] == 7).all()
+    for s in range(len(qs)):
+        if qs[s]:
+            see = np.arange(ctx[s]) <= B.positions(s)[:, None, None]
+            compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], np.broadcast_to(see, (qs[s], kv, ctx[s])), B.scale)
+    good = out
+    for value in (-1, prefix + qs[0] - 1, 10 ** 6):  # the first out of range: the others as before
+        status, out = B.shared(ctx=[value] + ctx[1:])
+        assert status == CACHE and (out[: qs[0]] == 7).all() and np.array_equal(out[qs[0]:], good[qs[0]:])
+    start = B.start.copy()
+    start[1] = sum(qs) + 1
+    status, out = B.shared(start=start)
+    assert status == CACHE and (out[: qs[0] + qs[1]] == 7).all() and np.array_equal(out[qs[0] + qs[1]:], good[qs[0] + qs[1]:])
+    B.q = np.concatenate([B.q, np.full((40, B.width), np.nan, np.float32)])  # rows of no sequence
+    status, out = B.shared()
+    assert status == OK and (out[-40:] == 7).all() and np.isfinite(out).all()
+
+
 @pytest.mark.gpu
 def test_shared_prefix_of_none_is_the_plain_call(dev):  # noqa: F811
     B = Batch(dev, [1, 40], [300, 500], 2, 4, 64, 32, seed=1)
@@ -282,6 +313,49 @@ def test_blocks_that_hold_everything_are_the_whole_context(dev):  # noqa: F811
         compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], np.broadcast_to(see, (B.qs[s], 2, B.ctxs[s])), B.scale)
         own = B.positions(s) // 64
         assert np.array_equal(chosen[B.start[s]:B.start[s + 1], 0], np.where(np.arange(32) < own[:, None], np.arange(32), -1))
+
+
+MANY_TOKENS = [  # (head_dim, KV heads, queries of each, tokens, contexts, page, block, top, first, last)
+    (64, 2, 7, [1, 300, 5, 0, 40], [800, 900, 5, 40, 1200], 64, 32, 5, 1, 1), (128, 2, 6, [520], [1531], 64, 64, 4, 0, 2), (128, 8, 1, [4] * 20, [1000 + 7 * i for i in range(20)], 128, 128, 2, 1, 0),
+    (128, 2, 3, [70, 250], [3000, 260], 32, 32, 30, 2, 3), (256, 4, 2, [100, 1, 17, 200], [100, 700, 900, 1100], 64, 32, 6, 0, 0), (64, 3, 9, [200, 201], [700, 800], 32, 32, 65, 1, 0),
+    (64, 2, 8, [2, 600], [2000, 640], 1024, 64, 3, 1, 1)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kv,G,qs,ctx,page,block,top,first,last", MANY_TOKENS)
+def test_blocks_of_many_tokens(dev, dim, kv, G, qs, ctx, page, block, top, first, last):  # noqa: F811
+    """Two (token, KV head)s a CU and more, four and more: 16 tokens' choice together, a wave a list."""
+    B = Batch(dev, qs, ctx, kv, G, dim, page, seed=dim + kv, pad=4)
+    means = B.means(block)
+    status, out, chosen = B.blocks(means, block, top, first, last)
+    assert status == OK and (out[:, B.heads * dim:] == 7).all()
+    for s in range(len(qs)):
+        if qs[s]:
+            want, see = B.choose(s, block, top, first, last)
+            assert np.array_equal(chosen[B.start[s]:B.start[s + 1]], want)
+            compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], see, B.scale)
+    good, picked, edge = out, chosen, qs[0]
+    for value in (-1, 10 ** 6):  # the first out of range: the others as before
+        status, out, chosen = B.blocks(means, block, top, first, last, ctx=[value] + ctx[1:])
+        assert status == CACHE and (out[:edge] == 7).all() and np.array_equal(out[edge:], good[edge:]) and np.array_equal(chosen[edge:], picked[edge:])
+    B.q = np.concatenate([B.q, np.full((40, B.width), np.nan, np.float32)])  # rows of no sequence
+    status, out, chosen = B.blocks(means, block, top, first, last)
+    assert status == OK and (out[-40:] == 7).all() and (chosen[-40:] == -7).all() and np.array_equal(out[:-40], good) and np.array_equal(chosen[:-40], picked)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,G,qs,ctx", [(128, 6, [40], [3]), (256, 3, [1, 70, 5], [0, 2, 40]), (64, 7, [300, 40], [20, 0]), (128, 4, [600], [130]), (64, 8, [520, 30], [3, 100]),
+                                          (256, 2, [520], [1]), (128, 9, [520], [260])])
+def test_blocks_of_more_tokens_than_positions(dev, dim, G, qs, ctx):  # noqa: F811
+    """Tokens before position 0 see nothing and choose nothing."""
+    B = Batch(dev, qs, ctx, 2, G, dim, 64, seed=dim)
+    status, out, chosen = B.blocks(B.means(32), 32, 2, 1, 0)
+    assert status == OK
+    for s in range(len(qs)):
+        want, see = B.choose(s, 32, 2, 1, 0)
+        assert np.array_equal(chosen[B.start[s]:B.start[s + 1]], want) and (B.rows(s, out)[B.positions(s) < 0] == 0).all()
+        if ctx[s]:
+            compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], see, B.scale)
 
 
 @pytest.mark.gpu

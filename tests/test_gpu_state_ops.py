@@ -291,6 +291,114 @@ def test_delta_rule_is_the_same_each_time_in_any_batch_and_on_any_stream(dev):  
         close(s, want, delta_bound(128, qs[i]), per=(0, 1))
 
 
+def on_the_gpu(R, src, dst):
+    """R.reference for thousands of tokens: the same steps in f64 tensors of the GPU."""
+    f = lambda x: cuda(x).double()  # noqa: E731
+    q, k, v, a, b, state = f(R.q), f(R.k), f(R.v), f(R.a), f(R.b), f(R.state)
+    r = v.shape[1] // q.shape[1]
+    q, k = (x / torch.sqrt((x * x).sum(-1, keepdim=True) + R.eps) for x in (q, k))
+    q, k = q.repeat_interleave(r, 1), k.repeat_interleave(r, 1)
+    keep, b = torch.exp(-torch.exp(f(R.A)) * torch.nn.functional.softplus(a + f(R.dt))), torch.sigmoid(b)
+    out, mag, old = torch.zeros_like(v), torch.zeros_like(v), state.clone()
+    for s, (at, n) in enumerate(zip(starts(R.qs), R.qs)):
+        S = old[src[s]].clone() if src[s] >= 0 else torch.zeros_like(old[0])
+        for t in range(at, at + n):
+            S *= keep[t, :, None, None]
+            u = b[t, :, None] * (v[t] - (S * k[t, :, :, None]).sum(1))
+            S += k[t, :, :, None] * u[:, None, :]
+            o = S * q[t, :, :, None]
+            out[t], mag[t] = o.sum(1) * R.scale, torch.sqrt((o * o).sum(1)) * R.scale
+        if dst[s] >= 0:
+            state[dst[s]] = S
+    return out.cpu().numpy(), state.cpu().numpy(), mag.cpu().numpy()
+
+
+# (heads of q and k, heads, k_dim, v_dim, tokens; the arrays' rows): sequences whose chunks' blocks come to 192 MB and more
+LONG = [(8, 16, 128, 128, [5700], 5700), (8, 8, 128, 128, [5610, 5610], 11220), (8, 8, 128, 128, [5600, 90], 11200), (16, 32, 64, 64, [5200], 5200),
+        (4, 8, 64, 256, [12700], 12700), (4, 16, 128, 128, [130], 8000)]
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,H,dk,dv,qs,rows", LONG)
+def test_delta_rule_of_long_sequences(dev, K, H, dk, dv, qs, rows):  # noqa: F811
+    """Chunks in groups; rows behind the last sequence, in a batch that could be even, stay as they were."""
+    n, longest = sum(qs), max(rows // len(qs), max(qs))
+    R = Rule([rows], K, H, dk, dv, seed=rows, slots=4)
+    src, dst = ([3], [0]) if len(qs) == 1 else ([1, -1], [1, 0])  # (the first of two in place)
+    R.qs = qs
+    status, out, state = R(dev, src, dst, max_q=longest)
+    assert status == OK and (out[n:] == 7).all()
+    ref, want, mag = on_the_gpu(R, src, dst)
+    close(out[:n], ref[:n], delta_bound(dk, max(qs)), per=(1,), mag=mag[:n])
+    close(state, want, delta_bound(dk, max(qs)), per=(0, 1))
+    if len(qs) == 2:  # one of them out of range: the other as before
+        first, second = slice(0, qs[0]), slice(qs[0], n)
+        for a, b, good, bad, slot, left in (([4, -1], dst, second, first, 0, 1), (src, [1, 4], first, second, 1, 0)):
+            status, o, s = R(dev, a, b, max_q=longest)
+            assert status == CACHE and np.array_equal(o[good], out[good]) and (o[bad] == 7).all()
+            assert np.array_equal(s[slot], state[slot]) and np.array_equal(s[left], R.state[left])
+        x = R.v.copy()
+        R.v[qs[0] - 70, 2, 5] = np.nan  # (in the first's last chunks: its earlier outputs and the other's are as before)
+        status, o, s = R(dev, src, dst, max_q=longest)
+        R.v = x
+        same = np.ones(o.shape, bool)
+        same[(qs[0] - 70) // 64 * 64:qs[0], 2] = False
+        assert status == NONFINITE and np.array_equal(o[same], out[same]) and np.array_equal(s[0], state[0])
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 256), (128, 64)])
+@pytest.mark.parametrize("H,qs", [(64, [24, 25, 90, 1, 130, 0, 65, 24, 2]), (64, [25] * 8), (64, [24] * 8), (48, [16, 17, 3, 100, 15, 1]), (3, [1] * 40 + [70, 1, 1, 9, 66, 8])])
+def test_delta_rule_of_many_heads(dev, dk, dv, H, qs):  # noqa: F811
+    """The lengths around which sequences go by tokens or by chunks, the chain's wider columns, many single tokens."""
+    R = Rule(qs, H // 3 if H % 3 == 0 else H // 2, H, dk, dv, seed=H + dk, slots=len(qs) + 2)
+    src, dst = [i if i % 3 else -1 for i in range(len(qs))], [i if i % 5 else -1 for i in range(len(qs))]
+    status, out, state = R(dev, src, dst)
+    ref, want, mag = on_the_gpu(R, src, dst)
+    assert status == OK
+    close(out, ref, delta_bound(dk, max(qs)), mag=mag)
+    close(state, want, delta_bound(dk, max(qs)))
+
+
+@pytest.mark.gpu
+def test_a_group_of_chunks_replayed_as_a_graph(dev):  # noqa: F811
+    """A long sequence captured: what passes from launch to launch in the scratch is made anew by every replay."""
+    d2, n, H = chart.Device(0), 5700, 16
+    rng = np.random.default_rng(2)
+    f32 = lambda *s: cuda(rng.standard_normal(s).astype(np.float32))  # noqa: E731
+    x, ab, out, state = f32(n, 3 * H * 128), f32(n, 2 * H), torch.zeros(n, H * 128, device="cuda"), f32(2, H, 128, 128)
+    gate, kept, i = (f32(H), f32(H) - 4), state.clone(), cuda(np.array([0, n, 0, 1], np.int32))
+
+    def run(d):
+        chart.delta_rule_dev(d, ptr(x), ptr(x) + 4 * H * 128, ptr(x) + 8 * H * 128, ptr(ab), ptr(ab) + 4 * H, ptr(out), n_heads=H, n_k_heads=H, k_dim=128, v_dim=128,
+                             a_log_ptr=ptr(gate[0]), dt_bias_ptr=ptr(gate[1]), scale=0.1, norm_eps=1e-6, state_ptr=ptr(state), q_stride=3 * H * 128, k_stride=3 * H * 128,
+                             v_stride=3 * H * 128, a_stride=2 * H, b_stride=2 * H, n_seq=1, n_tok=n, max_q=n, n_slots=2, q_start_ptr=ptr(i), from_ptr=ptr(i) + 8,
+                             to_ptr=ptr(i) + 8, stream=stream())
+
+    want = []
+    for _ in range(3):
+        run(dev)
+        torch.cuda.synchronize()
+        want.append((out.clone(), state.clone()))
+    state.copy_(kept)
+    run(d2)
+    torch.cuda.synchronize()
+    state.copy_(kept)
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        run(d2)
+    state.copy_(kept)
+    other = Rule([300, 200], 2, 4, 128, 128, seed=3, slots=2)
+    for o, s in want:
+        graph.replay()
+        torch.cuda.synchronize()
+        assert torch.equal(out, o) and torch.equal(state, s)
+        out.zero_()
+        assert other(d2, [0, 1], [0, 1])[0] == OK
+    assert d2.sync_status(stream()) == OK
+    d2.close()
+
+
 @pytest.mark.gpu
 def test_delta_rule_out_of_range_and_not_finite(dev):  # noqa: F811
     qs, src, dst = [70, 3, 129, 1], [0, 1, 2, 3], [0, 1, 2, 3]
