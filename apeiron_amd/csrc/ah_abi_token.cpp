@@ -432,19 +432,33 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         x.grid = (uint32_t)(units * x.splits);
         return units <= max_grid(256) / 2 / x.splits;
     };
-    // The prefix: the whole batch as one sequence, by units of 16 rows, or of 128 with the tiles in LDS once there are many (2 KV
-    // heads behind 8192 keys, rows of a KV head, 16 and 128 a unit, us: heads of 128, 48 rows 17 and 21, 384 28 and 37, 768 37
-    // and 43, 1536 55 and 61, 1764 72 and 60; of 64, 1400 36 and 38, 1715 48 and 41; of 256, 1024 66 and 80, 1568 94 and 95,
-    // 1960 113 and 108).
+    // What follows the prefix: each sequence for itself, by units of 8 or 16 rows, or of 128 where its rows are many and the units
+    // of 16 twelve a CU and more (2 KV heads of 128, sequences x tokens and their keys, units, us by 16 and by 128: 16 x 128 of
+    // 128 1536 100 and 112; 64 x 49 of 2048 2432 181 and 186; 32 x 128 of 128 12 a CU 109 and 103; 32 x 256 of 256 6144 213
+    // and 189; 16 x 512 of 512 6144 242 and 198).
+    const size_t per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
+    const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
+    own.rows = per_seq <= 8 ? 8 : 16;
+    size_t own_units = (per_seq + own.rows - 1) / own.rows * kv * a.n_seq;
+    if (per_seq > 128 && own_units >= 12 * cus) {
+        own.rows = 128;
+        own.per = (size_t)a.n_tok == (size_t)a.n_seq * a.max_q || a.n_seq == 1 ? (uint32_t)((per_seq + 127) / 128) : 0;
+        own_units = (own.per ? (size_t)own.per * a.n_seq : ((size_t)a.n_tok * a.group >> 7) + a.n_seq) * kv;
+    }
+    // The prefix: the whole batch as one sequence.  Units of 16 rows; of 32, for heads of 128, from 2^23 rows x keys on (a
+    // tile's codes are converted for twice the rows, by half as many waves); of 128, with the tiles in LDS, where the rows are many
+    // more.  2 KV heads behind 8192 keys, rows of a KV head, us by 16, 32, 128: heads of 128, 48 rows 16, 19, 22; 384 26, 27, 36; 768
+    // 38, 36, 44; 1764 71, 58, 60; 2352 81, 67, 68; 4704 133, 115, 113; 384 rows behind 16384 keys 39, 34, 47, behind 2048 17,
+    // 20, 23; of 64 (16 and 128) 1400 36 and 38, 1715 48 and 41; of 256 1024 66 and 80, 1568 94 and 95, 1960 113 and 108.
     pre.n_seq = 1;
     pre.table = d_prefix_table;
     pre.table_stride = (uint32_t)((prefix_len - 1) >> a.c.page_shift) + 1;
-    pre.rows = batch <= 1536 ? 16 : 128;
+    pre.rows = own.rows == 128 || batch > (a.c.dim == 128 ? 2560 : 1536) ? 128 : a.c.dim == 128 && batch * kv * prefix_len >= (size_t)1 << 23 ? 32 : 16;
     const size_t units = (batch + pre.rows - 1) / pre.rows, all = (prefix_len + 31) / 32;
     pre.per = (uint32_t)units;
     // Pieces by the time that they take, as attn_tiles has it: workgroups in rounds, and a piece's results written and read.
-    const size_t held = pre.rows != 128 ? 4 : a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1;
-    const double tile = pre.rows == 128 ? a.c.dim * 0.0077 : 0.18, alone = pre.rows == 128 ? 1.4 * tile : 0.18, start = 5.0, join = (double)rows * a.c.dim * 8.0 / 4e6 + 0.05;
+    const size_t held = pre.rows == 16 ? 4 : a.c.dim == 64 ? 3 : a.c.dim == 128 ? 2 : 1;
+    const double tile = pre.rows == 128 ? a.c.dim * 0.0077 : pre.rows == 32 ? 0.22 : 0.18, alone = pre.rows == 128 ? 1.4 * tile : tile, start = 5.0, join = (double)rows * a.c.dim * 8.0 / 4e6 + 0.05;
     size_t pieces = 1;
     double best = 0.0;
     for (size_t n = 1; n <= (all + 3) / 4 && n <= 256; ++n) {
@@ -460,19 +474,6 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         }
     }
     if (!cut(pre, units * kv, all, pieces)) return AH_ERR_INVALID_ARG;
-    // What follows it: each sequence for itself, by units of 8 or 16 rows, or of 128 from twelve of 16 a CU on (2 KV heads of 128,
-    // sequences x tokens and their keys, units, us by 16 and by 128: 16 x 128 of 128 1536 100 and 112; 64 x 49 of 2048 2432 181
-    // and 186; 16 x 256 of 256 3072 191 and 189; 32 x 128 of 128 3072 109 and 103; 32 x 256 of 256 6144 213 and 189; 16 x 512 of
-    // 512 6144 242 and 198).
-    const size_t per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
-    const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
-    own.rows = per_seq <= 8 ? 8 : 16;
-    size_t own_units = (per_seq + own.rows - 1) / own.rows * kv * a.n_seq;
-    if (own_units >= 12 * cus) {
-        own.rows = 128;
-        own.per = (size_t)a.n_tok == (size_t)a.n_seq * a.max_q || a.n_seq == 1 ? (uint32_t)((per_seq + 127) / 128) : 0;
-        own_units = (own.per ? (size_t)own.per * a.n_seq : ((size_t)a.n_tok * a.group >> 7) + a.n_seq) * kv;
-    }
     // (four tiles a piece or more: a wave each)
     size_t fill = 2 * cus / own_units;
     fill = fill < (tiles + 3) / 4 ? fill : (tiles + 3) / 4;

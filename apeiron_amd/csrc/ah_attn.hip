@@ -98,7 +98,7 @@ template <int MODE> AH_DEV const uint8_t *tile_in(const AttnArgs &a, uint32_t s,
 // lane (r, h) holds the scores of column r, tokens 4 h + i of both half-tiles.
 //   PACK: 8 rows, column r the hi half of row r & 7 for r < 8 and the lo half for r >= 8: one product gives
 //   both (they meet by a rotation of the columns), half the matrix work where a call has few rows.
-//   Otherwise 16 rows and a product for each half.
+//   Otherwise 16 rows, or C times 16, whose columns share a tile's converted codes, and a product for each half.
 // A tile's K is used first and its V last, so the next tile's K loads go out as soon as the scores are
 // formed and its V loads as soon as the output is: a wave always has half a tile on its way.
 //   What bounds it: for many keys in all the cache's bytes (64 sequences of 1 to 16384 keys, 12 heads of 128 over
@@ -106,13 +106,14 @@ template <int MODE> AH_DEV const uint8_t *tile_in(const AttnArgs &a, uint32_t s,
 // page's index, a tile, the partial results' way to the last workgroup and back (4001 keys: 9.8 us).  A unit
 // over all keys in one workgroup, joined by nobody, costs 0.7 us a tile and wave; a second launch for the join
 // 5 us more; equal shares of all units' tiles for every workgroup (two units in one) up to 10.
-template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, uint32_t block, uint32_t grid) {
+template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const AttnArgs &a, uint32_t block, uint32_t grid) {
     constexpr int NJ = D / 32;  // contraction steps of K q, and blocks of channels
-    constexpr uint32_t R = PACK ? 8 : 16;
+    constexpr uint32_t R = PACK ? 8 : 16 * C, kRed = 16 * C;
+    static_assert(C == 1 || (!PACK && MODE == kPrefix), "more columns are for rows that all see the same keys");
     extern __shared__ float lds[];
-    float *red_o = lds;                   // [4][16][D + 4]
-    float *red_m = lds + 4 * 16 * (D + 4);  // [4][16], then the sums
-    float *red_l = red_m + 64;
+    float *red_o = lds;                   // [4][16 C][D + 4]
+    float *red_m = lds + 4 * kRed * (D + 4);  // [4][16 C], then the sums
+    float *red_l = red_m + 4 * kRed;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6);
     // pieces run slowest: the workgroups without work (pieces past a short context) are the last ones, and
@@ -124,7 +125,7 @@ template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, u
     if (MODE != kBlocks && p.bad && split == 0 && rest == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
     const uint32_t rows = p.nq * a.group, row0 = rt * R;
     if (row0 >= rows || (MODE == kAll && rows > a.most_rows)) return;
-    const uint32_t row = row0 + r % R, tok = row / a.group, hq = kvh * a.group + row % a.group;
+    const uint32_t row = row0 + r % R, tok = row / a.group;
     const bool live = row < rows, low = PACK && r >= 8;
     const uint32_t last = row0 + R - 1 < rows ? row0 + R - 1 : rows - 1;
     const int32_t lo = position_of<MODE>(p, row0 / a.group), hi = position_of<MODE>(p, last / a.group);
@@ -150,14 +151,17 @@ template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, u
     }
 
     // q, scaled by a power of two so that its largest magnitude is in [2^13, 2^14), as hi + lo
-    f16x8 qh[NJ], ql[PACK ? 1 : NJ];
-    float f;
-    {
-        const float *q = a.q + (size_t)(p.q0 + tok) * a.q_stride + (size_t)hq * D + h * (D / 4);
+    f16x8 qh[C][NJ], ql[C][PACK ? 1 : NJ];
+    float f[C];
+#pragma unroll
+    for (int n = 0; n < C; ++n) {
+        const uint32_t rw = row + 16 * n, tk = rw / a.group, hq = kvh * a.group + rw % a.group;
+        const bool there = rw < rows;
+        const float *q = a.q + (size_t)(p.q0 + tk) * a.q_stride + (size_t)hq * D + h * (D / 4);
         float x[NJ][8], top = 0.0f;
 #pragma unroll
         for (int j = 0; j < NJ; ++j) {
-            if (live) __builtin_memcpy(x[j], q + 8 * j, 32);
+            if (there) __builtin_memcpy(x[j], q + 8 * j, 32);
             else
 #pragma unroll
                 for (int i = 0; i < 8; ++i) x[j][i] = 0.0f;
@@ -167,99 +171,116 @@ template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, u
         top = __builtin_fmaxf(top, xor_lanes(top, 16));
         top = __builtin_fmaxf(top, xor_lanes(top, 32));
         float sign;
-        q_scale(a.scale, top, sign, f);
+        q_scale(a.scale, top, sign, f[n]);
 #pragma unroll
         for (int j = 0; j < NJ; ++j)
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
                 const float y = x[j][i] * sign;
                 const _Float16 hv = (_Float16)y, lv = (_Float16)(y - (float)hv);
-                qh[j][i] = low ? lv : hv;
-                if (!PACK) ql[j][i] = lv;
+                qh[n][j][i] = low ? lv : hv;
+                if (!PACK) ql[n][j][i] = lv;
             }
     }
 
-    f32x4 acc[NJ][2];
+    f32x4 acc[C][NJ][2];
+    float m[C], l[C];
 #pragma unroll
-    for (int g = 0; g < NJ; ++g) acc[g][0] = acc[g][1] = (f32x4)0.0f;
-    float m = kNoMax, l = 0.0f;
+    for (int n = 0; n < C; ++n) {
+#pragma unroll
+        for (int g = 0; g < NJ; ++g) acc[n][g][0] = acc[n][g][1] = (f32x4)0.0f;
+        m[n] = kNoMax;
+        l[n] = 0.0f;
+    }
     const Masks mk;
     const float minus_low = low ? -1.0f : 0.0f;
     for (; ti < t1; ti += 4) {
         const uint32_t tile = tile_of(ti), next = ti + 4 < t1 ? ti + 4 : ti;
         bool ok_next;
         const uint8_t *tn = tile_in<MODE>(a, s, kvh, tile_of(next), ok_next);
-        f32x4 c[2];
+        f32x4 c[C][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            c[half] = (f32x4)0.0f;
+#pragma unroll
+            for (int n = 0; n < C; ++n) c[n][half] = (f32x4)0.0f;
 #pragma unroll
             for (int j = 0; j < NJ; ++j) {
                 const f16x8 kf = k_frag(k.code(half, j), k.scale(half, j), mk);
-                c[half] = mfma16(kf, qh[j], c[half]);
-                if (!PACK) c[half] = mfma16(kf, ql[j], c[half]);
+#pragma unroll
+                for (int n = 0; n < C; ++n) {
+                    c[n][half] = mfma16(kf, qh[n][j], c[n][half]);
+                    if (!PACK) c[n][half] = mfma16(kf, ql[n][j], c[n][half]);
+                }
             }
         }
         k.load(tn, r, h);
-        float x[8];
-#pragma unroll
-        for (int i = 0; i < 8; ++i) {
-            const float y = c[i >> 2][i & 3];
-            x[i] = PACK ? y + ror8(y) : y;
-        }
+        f16x8 pf[C], pg[C];
         const int32_t first = (int32_t)(tile * 32);
         // a tile that every row sees whole needs no mask
         const bool whole = ok && first + 31 <= lo && (first >= low_all || first + 32 <= sink_key);
-        if (!whole) {
-            if (!ok && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
-            const int32_t top_key = ok ? pos : -1;
+        if (!whole && !ok && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
+#pragma unroll
+        for (int n = 0; n < C; ++n) {
+            float x[8];
 #pragma unroll
             for (int i = 0; i < 8; ++i) {
-                const int32_t key = first + 16 * (i >> 2) + 4 * (int32_t)h + (i & 3);
-                const bool see = key <= top_key && (key >= low_key || key < sink_key);
-                x[i] = see ? x[i] : -__builtin_inff();
+                const float y = c[n][i >> 2][i & 3];
+                x[i] = PACK ? y + ror8(y) : y;
             }
-        }
-        float top = x[0];
+            if (!whole) {
+                const int32_t top_key = ok ? C == 1 ? pos : row + 16 * n < rows ? position_of<MODE>(p, 0) : -1 : -1;
 #pragma unroll
-        for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
-        top *= f;
-        if (__builtin_amdgcn_ballot_w64(top > m + kSlack) != 0ull) {
-            top = __builtin_fmaxf(top, xor_lanes(top, 16));
-            top = __builtin_fmaxf(top, xor_lanes(top, 32));
-            const float up = __builtin_fmaxf(m, top), alpha = __builtin_amdgcn_exp2f(m - up);
-            m = up;
-            l *= alpha;
-#pragma unroll
-            for (int g = 0; g < NJ; ++g) {
-                acc[g][0] *= alpha;
-                acc[g][1] *= alpha;
+                for (int i = 0; i < 8; ++i) {
+                    const int32_t key = first + 16 * (i >> 2) + 4 * (int32_t)h + (i & 3);
+                    const bool see = key <= top_key && (key >= low_key || key < sink_key);
+                    x[i] = see ? x[i] : -__builtin_inff();
+                }
             }
-        }
-        const float base = kUp - m;
-        float ls = 0.0f;  // the tile's weights, as in attn_tile_kernel
-        f16x2 ph[4], pl[4];
+            float top = x[0];
 #pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], f, base)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], f, base));
-            ls = i ? ls + e0 : e0;
-            ls += e1;
-            ph[i] = pack16(e0, e1);
-            // what is left of p past its hi half; a packed column takes that or p itself
-            const float k = PACK ? minus_low : -1.0f;
-            pl[i] = pack16(__builtin_fmaf((float)ph[i][0], k, e0), __builtin_fmaf((float)ph[i][1], k, e1));
+            for (int i = 1; i < 8; ++i) top = __builtin_fmaxf(top, x[i]);
+            top *= f[n];
+            if (__builtin_amdgcn_ballot_w64(top > m[n] + kSlack) != 0ull) {
+                top = __builtin_fmaxf(top, xor_lanes(top, 16));
+                top = __builtin_fmaxf(top, xor_lanes(top, 32));
+                const float up = __builtin_fmaxf(m[n], top), alpha = __builtin_amdgcn_exp2f(m[n] - up);
+                m[n] = up;
+                l[n] *= alpha;
+#pragma unroll
+                for (int g = 0; g < NJ; ++g) {
+                    acc[n][g][0] *= alpha;
+                    acc[n][g][1] *= alpha;
+                }
+            }
+            const float base = kUp - m[n];
+            float ls = 0.0f;  // the tile's weights, as in attn_tile_kernel
+            f16x2 ph[4], pl[4];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                float e0 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i], f[n], base)), e1 = __builtin_amdgcn_exp2f(__builtin_fmaf(x[2 * i + 1], f[n], base));
+                ls = i ? ls + e0 : e0;
+                ls += e1;
+                ph[i] = pack16(e0, e1);
+                // what is left of p past its hi half; a packed column takes that or p itself
+                const float k = PACK ? minus_low : -1.0f;
+                pl[i] = pack16(__builtin_fmaf((float)ph[i][0], k, e0), __builtin_fmaf((float)ph[i][1], k, e1));
+            }
+            l[n] += ls;
+            pg[n] = join8(pl[0], pl[1], pl[2], pl[3]);
+            pf[n] = PACK ? pg[n] : join8(ph[0], ph[1], ph[2], ph[3]);
         }
-        l += ls;
-        const f16x8 pg = join8(pl[0], pl[1], pl[2], pl[3]), pf = PACK ? pg : join8(ph[0], ph[1], ph[2], ph[3]);
 #pragma unroll
         for (int g = 0; g < NJ; ++g) {
             f16x8 even, odd;
             v_frags(v.w[g >> 1][2 * (g & 1)], v.w[g >> 1][2 * (g & 1) + 1], v.d[g], mk, even, odd);
-            acc[g][0] = mfma16(even, pf, acc[g][0]);
-            acc[g][1] = mfma16(odd, pf, acc[g][1]);
-            if (!PACK) {
-                acc[g][0] = mfma16(even, pg, acc[g][0]);
-                acc[g][1] = mfma16(odd, pg, acc[g][1]);
+#pragma unroll
+            for (int n = 0; n < C; ++n) {
+                acc[n][g][0] = mfma16(even, pf[n], acc[n][g][0]);
+                acc[n][g][1] = mfma16(odd, pf[n], acc[n][g][1]);
+                if (!PACK) {
+                    acc[n][g][0] = mfma16(even, pg[n], acc[n][g][0]);
+                    acc[n][g][1] = mfma16(odd, pg[n], acc[n][g][1]);
+                }
             }
         }
         v.load(tn, r, h);
@@ -267,22 +288,25 @@ template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, u
     }
 
     // the lanes' sums of a column, then the four waves
-    l += xor_lanes(l, 16);
-    l += xor_lanes(l, 32);
-    if (h == 0 && !low) {
-        red_m[wave * 16 + r] = m;
-        red_l[wave * 16 + r] = l;
-    }
 #pragma unroll
-    for (int g = 0; g < NJ; ++g) {
-        float o[8];
-#pragma unroll
-        for (int i = 0; i < 4; ++i) {
-            const float e = acc[g][0][i], d = acc[g][1][i];
-            o[2 * i] = PACK ? e + ror8(e) : e;
-            o[2 * i + 1] = PACK ? d + ror8(d) : d;
+    for (int n = 0; n < C; ++n) {
+        l[n] += xor_lanes(l[n], 16);
+        l[n] += xor_lanes(l[n], 32);
+        if (h == 0 && !low) {
+            red_m[wave * kRed + 16 * n + r] = m[n];
+            red_l[wave * kRed + 16 * n + r] = l[n];
         }
-        if (!low) __builtin_memcpy(red_o + (wave * 16 + r) * (D + 4) + 32 * g + 8 * h, o, 32);
+#pragma unroll
+        for (int g = 0; g < NJ; ++g) {
+            float o[8];
+#pragma unroll
+            for (int i = 0; i < 4; ++i) {
+                const float e = acc[n][g][0][i], d = acc[n][g][1][i];
+                o[2 * i] = PACK ? e + ror8(e) : e;
+                o[2 * i + 1] = PACK ? d + ror8(d) : d;
+            }
+            if (!low) __builtin_memcpy(red_o + (wave * kRed + 16 * n + r) * (D + 4) + 32 * g + 8 * h, o, 32);
+        }
     }
     __syncthreads();
     const uint32_t pieces = MODE == kPrefix || MODE == kAfter ? 2 : T.count ? (T.count + chunk - 1) / chunk : 1;  // (2: a part of what a launch after this joins)
@@ -291,16 +315,17 @@ template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, u
     auto out_of = [&](uint32_t rw) { return a.out + (size_t)(p.q0 + rw / a.group) * a.out_stride + (size_t)(kvh * a.group + rw % a.group) * D; };
     const uint32_t n_rows = last - row0 + 1;
     const __amdgpu_buffer_rsrc_t po = ah_rsrc(a.part_o, (uint32_t)(a.splits * all * D * 4)), pm = ah_rsrc(a.part_ml, (uint32_t)(a.splits * all * 8));
-    {
-        const uint32_t rr = threadIdx.x >> 4;
+#pragma unroll
+    for (int n = 0; n < C; ++n) {
+        const uint32_t rr = 16 * n + (threadIdx.x >> 4);
         if (rr < n_rows) {
             float M = kNoMax, L = 0.0f, w4[4];
 #pragma unroll
-            for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, red_m[w * 16 + rr]);
+            for (int w = 0; w < 4; ++w) M = __builtin_fmaxf(M, red_m[w * kRed + rr]);
 #pragma unroll
             for (int w = 0; w < 4; ++w) {
-                w4[w] = __builtin_amdgcn_exp2f(red_m[w * 16 + rr] - M);
-                L += red_l[w * 16 + rr] * w4[w];
+                w4[w] = __builtin_amdgcn_exp2f(red_m[w * kRed + rr] - M);
+                L += red_l[w * kRed + rr] * w4[w];
             }
             const float inv = pieces > 1 ? 1.0f : L > 0.0f || L != L ? 1.0f / L : 0.0f;
             const size_t at = split * all + flat_of(row0 + rr);
@@ -309,7 +334,7 @@ template <int D, bool PACK, int MODE> AH_DEV void attn_rows(const AttnArgs &a, u
 #pragma unroll
                 for (int w = 0; w < 4; ++w) {
                     f32x4 y;
-                    __builtin_memcpy(&y, red_o + (w * 16 + rr) * (D + 4) + c, 16);
+                    __builtin_memcpy(&y, red_o + (w * kRed + rr) * (D + 4) + c, 16);
                     o += y * w4[w];
                 }
                 o *= inv;
@@ -777,13 +802,15 @@ template <int D, int MODE> AH_DEV void attn_tiles(const AttnArgs &a, uint32_t bl
 template <int D, int MODE> __global__ void __launch_bounds__(256, D == 64 ? 3 : D == 128 ? 2 : 1) attn_tile_kernel(AttnArgs a) {
     attn_tiles<D, MODE>(a, blockIdx.x, gridDim.x);
 }
-// A common prefix, by 16 or 128 rows of the whole batch, and beside it in the same launch what each sequence has after it, by 8
-// or 16: the one alone leaves CUs without work at its end, and a launch more costs 5 us.
-template <int D, bool TILES, bool PACK>
-__global__ void __launch_bounds__(256, TILES ? (D == 64 ? 3 : D == 128 ? 2 : 1) : D == 256 ? 2 : D == 128 ? 3 : 4) attn_shared_kernel(AttnArgs prefix, AttnArgs after) {
+// A common prefix, by 16, 32 or 128 rows of the whole batch, and beside it in the same launch what each sequence has after it, by 8
+// or 16: the one alone leaves CUs without work at its end, and a launch more costs 5 us.  What bounds the units of 16 and 32 is
+// the vector work of converting codes and of the exponentials: of 12 heads of 128 over 2 of 64 sequences behind 16384 keys, 6.4
+// MB and 12.9 GFLOP, 26 with the halves, in 33 us (by 16 rows 37, by 128 47).
+template <int D, int ROWS, bool PACK>
+__global__ void __launch_bounds__(256, ROWS == 16 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : D == 64 ? 3 : D == 128 ? 2 : 1) attn_shared_kernel(AttnArgs prefix, AttnArgs after) {
     if (blockIdx.x >= prefix.grid) attn_rows<D, PACK, kAfter>(after, blockIdx.x - prefix.grid, after.grid);
-    else if (TILES) attn_tiles<D, kPrefix>(prefix, blockIdx.x, prefix.grid);
-    else attn_rows<D, false, kPrefix>(prefix, blockIdx.x, prefix.grid);
+    else if (ROWS == 128) attn_tiles<D, kPrefix>(prefix, blockIdx.x, prefix.grid);
+    else attn_rows<D, false, kPrefix, ROWS == 32 ? 2 : 1>(prefix, blockIdx.x, prefix.grid);
 }
 
 // Joins the pieces of attn_tile_kernel's contexts: a wave takes 256 / D heads of a token, four channels a lane.  A piece
@@ -890,7 +917,7 @@ __global__ void __launch_bounds__(256) attn_meet_kernel(AttnArgs a) {
     __builtin_memcpy(a.out + (size_t)tok * a.out_stride + (size_t)head * D + c, &sum, 16);
 }
 
-template <int D> constexpr size_t attn_lds() { return (4 * 16 * (D + 4) + 128) * sizeof(float); }
+template <int D, int C = 1> constexpr size_t attn_lds() { return C * (4 * 16 * (D + 4) + 128) * sizeof(float); }
 
 template <int D, int MODE> void launch_rows(const AttnArgs &a, hipStream_t stream) {
     if (a.rows == 16) hipLaunchKernelGGL((attn_rows_kernel<D, false, MODE>), dim3(a.grid), dim3(256), attn_lds<D>(), stream, a);
@@ -910,18 +937,24 @@ template <int D> hipError_t launch(const AttnArgs &a, hipStream_t stream) {
     if (a.splits > 1 && !a.join) hipLaunchKernelGGL(attn_join_kernel<D>, dim3(join_grid<D>(a)), dim3(256), 0, stream, a);
     return hipGetLastError();
 }
-template <int D, bool TILES, bool PACK> void launch_both(const AttnArgs &prefix, const AttnArgs &after, hipStream_t stream) {
-    constexpr size_t tiles = 2 * TileLds<D>::kBytes, lds = TILES && tiles > attn_lds<D>() ? tiles : attn_lds<D>();
-    hipLaunchKernelGGL((attn_shared_kernel<D, TILES, PACK>), dim3(prefix.grid + after.grid), dim3(256), lds, stream, prefix, after);
+template <int D, int ROWS> constexpr size_t shared_lds() {
+    return ROWS == 128 ? (2 * TileLds<D>::kBytes > attn_lds<D>() ? 2 * TileLds<D>::kBytes : attn_lds<D>()) : attn_lds<D, ROWS / 16>();
+}
+template <int D, int ROWS> void launch_both(const AttnArgs &prefix, const AttnArgs &after, hipStream_t stream) {
+    const dim3 grid(prefix.grid + after.grid);
+    if (after.rows == 16) hipLaunchKernelGGL((attn_shared_kernel<D, ROWS, false>), grid, dim3(256), (shared_lds<D, ROWS>()), stream, prefix, after);
+    else hipLaunchKernelGGL((attn_shared_kernel<D, ROWS, true>), grid, dim3(256), (shared_lds<D, ROWS>()), stream, prefix, after);
 }
 template <int D> hipError_t launch_shared(const AttnArgs &prefix, const AttnArgs &after, const AttnArgs &both, hipStream_t stream) {
     if (after.rows == 128) {
         launch_tiles<D, kPrefix>(prefix, stream);
         launch_tiles<D, kAfter>(after, stream);
     } else if (prefix.rows == 128) {
-        after.rows == 16 ? launch_both<D, true, false>(prefix, after, stream) : launch_both<D, true, true>(prefix, after, stream);
+        launch_both<D, 128>(prefix, after, stream);
+    } else if (D == 128 && prefix.rows == 32) {
+        launch_both<D, D == 128 ? 32 : 16>(prefix, after, stream);
     } else {
-        after.rows == 16 ? launch_both<D, false, false>(prefix, after, stream) : launch_both<D, false, true>(prefix, after, stream);
+        launch_both<D, 16>(prefix, after, stream);
     }
     hipLaunchKernelGGL(attn_meet_kernel<D>, dim3(both.n_tok * ((both.n_heads + 256 / D - 1) / (256 / D))), dim3(256), 0, stream, both);
     return hipGetLastError();
@@ -955,12 +988,14 @@ hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream) {
     return a.c.dim == 64 ? launch_blocks<64>(a, stream) : a.c.dim == 128 ? launch_blocks<128>(a, stream) : launch_blocks<256>(a, stream);
 }
 
+template <int D, int ROWS> hipError_t allow_both() {
+    const hipError_t e = allow_lds(attn_shared_kernel<D, ROWS, false>, shared_lds<D, ROWS>());
+    return e != hipSuccess ? e : allow_lds(attn_shared_kernel<D, ROWS, true>, shared_lds<D, ROWS>());
+}
 template <int D> hipError_t allow_shared() {
-    const size_t most = 2 * TileLds<D>::kBytes > attn_lds<D>() ? 2 * TileLds<D>::kBytes : attn_lds<D>();
-    hipError_t e = allow_lds(attn_shared_kernel<D, false, false>, most);
-    if (e == hipSuccess) e = allow_lds(attn_shared_kernel<D, false, true>, most);
-    if (e == hipSuccess) e = allow_lds(attn_shared_kernel<D, true, false>, most);
-    return e != hipSuccess ? e : allow_lds(attn_shared_kernel<D, true, true>, most);
+    hipError_t e = allow_both<D, 16>();
+    if (e == hipSuccess && D == 128) e = allow_both<D, D == 128 ? 32 : 16>();
+    return e != hipSuccess ? e : allow_both<D, 128>();
 }
 
 hipError_t ah_attn_init_attrs() {

@@ -125,9 +125,14 @@ template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) 
         }
         if (odd) ah_record(a.status, ((unsigned long long)s << 8) + kKeyNonFinite);
     }
-    if (block == 0 && threadIdx.x == 0)
-        for (uint32_t i = at; i < a.s.n_seq; i += a.tiles)
-            if (seq_of(a.s, i).bad) ah_record(a.status, ((unsigned long long)i << 8) + kKeyRange);
+    if (block == 0 && threadIdx.x == 0) {
+        if (a.per) {
+            if (p.bad && n == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
+        } else {  // (a sequence out of range has no tile)
+            for (uint32_t i = at; i < a.s.n_seq; i += a.tiles)
+                if (seq_of(a.s, i).bad) ah_record(a.status, ((unsigned long long)i << 8) + kKeyRange);
+        }
+    }
 }
 
 // ---- the gated delta rule ----------------------------------------------------------------------------

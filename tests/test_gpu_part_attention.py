@@ -161,7 +161,8 @@ def test_shared_prefix_of_large_scores_and_longer_contexts_than_planned(dev, dim
 MANY = [  # (head_dim, KV heads, queries of each, tokens, what follows the prefix of each sequence, prefix)
     (64, 1, 7, [50, 1, 0, 128, 64], [60, 1, 5, 128, 200], 133), (128, 1, 6, [90, 100, 70], [90, 100, 300], 640), (256, 2, 3, [300, 220], [333, 250], 31),
     (64, 4, 16, [32, 31, 1, 0, 20] * 5, [32, 31, 1, 3, 90] * 5, 100), (128, 4, 16, [32] * 24, [32 + i % 3 for i in range(24)], 65),
-    (256, 8, 16, [16, 3, 16, 1] * 6, [16, 20, 70, 1] * 6, 64)]
+    (256, 8, 16, [16, 3, 16, 1] * 6, [16, 20, 70, 1] * 6, 64), (64, 64, 10, [16, 2, 13, 1, 16], [16, 2, 40, 1, 17], 40), (64, 32, 1, [1] * 110, [1 + i % 9 for i in range(110)], 33),
+    (128, 2, 16, [17] * 9 + [1], [20] * 9 + [300], 2000), (128, 1, 6, [90, 1, 100, 60], [90, 1, 300, 64], 5700)]
 
 
 @pytest.mark.gpu
