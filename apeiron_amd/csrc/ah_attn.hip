@@ -805,7 +805,9 @@ template <int D, int MODE> __global__ void __launch_bounds__(256, D == 64 ? 3 : 
 // A common prefix, by 16, 32 or 128 rows of the whole batch, and beside it in the same launch what each sequence has after it, by 8
 // or 16: the one alone leaves CUs without work at its end, and a launch more costs 5 us.  What bounds the units of 16 and 32 is
 // the vector work of converting codes and of the exponentials: of 12 heads of 128 over 2 of 64 sequences behind 16384 keys, 6.4
-// MB and 12.9 GFLOP, 26 with the halves, in 33 us (by 16 rows 37, by 128 47).
+// MB and 6.6 GFLOP, 13 with the halves, in 28 us (by 16 rows 31, by 128 35): vector work takes 57% of a SIMD's cycles while a
+// CU works, products 24%.  By 128 rows (16 sequences of 25 to 49 tokens behind 8003 keys, 30 GFLOP, 60 with the halves, 82 us)
+// 42% and 39%.
 template <int D, int ROWS, bool PACK>
 __global__ void __launch_bounds__(256, ROWS == 16 ? (D == 256 ? 2 : D == 128 ? 3 : 4) : D == 64 ? 3 : D == 128 ? 2 : 1) attn_shared_kernel(AttnArgs prefix, AttnArgs after) {
     if (blockIdx.x >= prefix.grid) attn_rows<D, PACK, kAfter>(after, blockIdx.x - prefix.grid, after.grid);
@@ -856,7 +858,8 @@ __global__ void __launch_bounds__(256) attn_join_kernel(AttnArgs a) {
 }
 
 // Joins what kPrefix and kAfter leave, a.splits pieces of every token of a sequence: a workgroup takes 256 / D heads of a token,
-// each of its waves every fourth piece, eight of them on their way, and they meet in LDS.
+// each of its waves every fourth piece, eight of them on their way, and they meet in LDS.  Bound by the launch and the partial
+// results' bytes: 64 tokens of 12 heads of 128 4.7 us, 608 tokens, 37 MB, 11 us.
 template <int D>
 __global__ void __launch_bounds__(256) attn_meet_kernel(AttnArgs a) {
     constexpr uint32_t kLanes = D / 4, kHeads = 64 / kLanes, kAhead = 8;

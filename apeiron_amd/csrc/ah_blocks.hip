@@ -1,5 +1,6 @@
 // ah_blocks.hip -- the choice of blocks for attention over parts of a long context in the paged 4-bit cache (layout:
-// ah_kv4.h): the means of the blocks' keys, and for every (token, KV head) the blocks that its queries score highest.
+// ah_kv4.h): the means of the blocks' keys, for every (token, KV head) the blocks that its queries score highest, and
+// attention over many such lists (over few it is attn_rows_kernel's).
 #include "ah_attn.h"
 
 namespace {
@@ -11,7 +12,10 @@ constexpr unsigned long long kKeyCache = AH_ERR_CACHE_RANGE;
 // A block whose last position is among the tokens: the mean of its keys, a wave a KV head.  Lane (p, g) sums the eight
 // channels of group g over every (64 / (D / 8))-th position from p on, in f64: the cache's values have eleven
 // significant bits between 2^-24 and 2^16, so the sums are exact in any order, and a block's mean is the same however
-// its positions came.  It is rounded to f32 and then to f16.
+// its positions came.  It is rounded to f32 and then to f16: half a step of f16 in a mean moves a score by 2^-11 of |q| |k|, and a
+// mean is 16-bit in memory because the choice reads all of them (16.8 MB for 64 contexts of 32768 keys of 2 heads of 128).
+//   What bounds it: a workgroup a token, nearly all of which end no block: the launch and one round trip to learn that, another for
+// the page, one for the block (64 single tokens 4.2 to 5.2 us); 2039 tokens of a prompt 7.4.
 template <int D> __global__ void __launch_bounds__(256) block_means_kernel(MeansArgs a) {
     constexpr uint32_t G = D / 8, P = 64 / G;
     const uint32_t tok = blockIdx.x, lane = threadIdx.x & 63, g = lane % G, ph = lane / G;
@@ -59,6 +63,10 @@ template <int D> __global__ void __launch_bounds__(256) block_means_kernel(Means
 // The query at position p of block b reads the blocks 0 .. first - 1, b - last .. b and, of those between, the `top` of the
 // highest score scale sum_h q_h . mean (h over the KV head's queries; of equal ones the first).  Scores are f64: the order of two
 // blocks is the formula's, not the rounding's.  They are ranked as whole numbers of the same order.
+//   What bounds it: for a token by itself round trips and barriers (512 means a KV head of 32768 keys: 11 us for one token, of which
+// means and scores 4, the choice by one wave 4; 64 such tokens 13), for many f64 products and one wave's choice a token (2039
+// tokens of up to 250 blocks 16.5 us).  Bits counted over a workgroup with a barrier each: 41 us for 25 of a token's
+// whole call.  In one launch with the attention, which then has a CU for a token, it took as long as in two.
 AH_DEV uint64_t rank_of(double v) {
     const uint64_t b = __builtin_bit_cast(uint64_t, v + 0.0);  // (-0 is 0)
     return v != v ? 0 : b >> 63 ? ~b : b | 1ull << 63;
@@ -227,7 +235,8 @@ template <class K, class E, class M> AH_DEV void many_keys(uint32_t n, uint32_t 
 }
 
 // The choice for a (token, KV head) by a workgroup of W waves, into `list` (as attention's, kNoList where the token is no
-// sequence's).  Scores: D / 8 lanes a block, eight channels each, the means of several blocks a lane on their way.
+// sequence's).  Scores: D / 8 lanes a block, eight channels each, the means of several blocks a lane on their way (a load touches
+// few lines; with a lane for a whole mean it touches 64).  16 waves: all blocks of 32768 keys are on their way at once.
 template <int W> struct ChoiceLds {
     uint64_t room[128];
     uint32_t cnt[2][W], done;
@@ -342,7 +351,8 @@ template <int D> __global__ void __launch_bounds__(1024) block_choice_kernel(Blo
 }
 
 // A workgroup for 16 tokens of a sequence and a KV head: scores of 16 blocks and the 16 tokens by f64 matrix products (lane
-// (r, h): token r, blocks h + 4 i of the result), then a token's choice by one wave.
+// (r, h): token r, blocks h + 4 i of the result), then a token's choice by one wave: the means are read once for 16 tokens, and no
+// barrier stands inside a choice.  16 waves rather than 4: 2039 tokens of 16001 keys 16.5 us for 20.
 template <int D> constexpr uint32_t kSomeWaves = D == 256 ? 8 : 16;  // (as many as the registers allow)
 template <int D> __global__ void __launch_bounds__(64 * kSomeWaves<D>) block_choices_kernel(BlockArgs b) {
     typedef double f64x4 __attribute__((ext_vector_type(4)));
@@ -422,6 +432,9 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves<D>) block_cho
 // attn_rows_kernel's eight packed rows (ah_attn.hip), all of one token: the KV head's queries see the same keys, 0 .. keys - 1 of
 // the listed blocks one after the other, so only the last tile needs a mask.  A wave takes a whole list: with enough of them
 // nobody needs to be met.
+//   What bounds it: vector work, 88% of a SIMD's cycles while a CU works (210 instructions a tile of 32 keys of 64 channels: a
+// list is one token's, so its queries alone share what converting the codes costs).  2039 tokens, 7 heads over 2, lists of up to
+// 1184 keys, 8.8 GFLOP: 72 us.
 template <int D, class T> AH_DEV void attend_rows(const AttnArgs &a, uint32_t tok, uint32_t kvh, uint32_t keys, T tile_at) {
     constexpr int NJ = D / 32;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, row = r & 7;

@@ -1,6 +1,6 @@
 // ah_kv4.h -- the paged 4-bit key/value cache: its layout in memory, and the launch arguments of the
-// operators between a token's projections (ah_token.hip, ah_attn.hip, ah_sample.hip), planned by
-// ah_abi_token.cpp.
+// operators between a token's projections (ah_token.hip, ah_attn.hip, ah_blocks.hip, ah_sample.hip), planned
+// by ah_abi_token.cpp.
 //
 // A block is 32 channels of one token and KV head.  With m its element of largest magnitude (the
 // positive one of two), d is the f16 number of 8 significant bits nearest to -m / 8, the code of x

@@ -45,7 +45,8 @@ AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 // rows and the W - 1 before them at once, so that no load waits for another.  Bytes bound it: x once, y once; the rows
 // before a tile come from L2 a second time.  (64 to 8192 tokens of 1024 to 6144 channels: tiles of 8 86 us, of 16 91, of 32 93 at
 // 8192 x 6144, 13.9, 15.9 and 21.9 at 512 x 6144, the smallest never behind by more than the noise.)  8192 x 6144 takes 86 us,
-// 4.7 TB/s of the 5.0 that a copy reaches; a token of 64 sequences 2.9 us.  The tile that holds a sequence's first token
+// 4.7 TB/s of the 5.0 that a copy reaches, 3831 tokens of 4099 channels 33.5 us, 4.0 TB/s (rows off the 16-byte grid); a token of
+// 64 sequences, 12.7 MB, 8.4 us: a launch, the sequence's numbers, its rows and the writes, one after the other.  The tile that holds a sequence's first token
 // alone reads the state and also writes the new one, so that both may lie in the same slot.  Rows come and go through
 // range-checked resources: no branch stands between the loads.
 static_assert(kConvTile >= kConvMaxWidth - 1, "the rows before a tile lie in the one before it");
@@ -139,7 +140,10 @@ template <int W> __global__ void __launch_bounds__(256) conv_kernel(ConvArgs a) 
 //
 // Token by token, with a head's S [k_dim][v_dim] in registers: S = e^g S, u = beta (v - S^T k), S += k u^T,
 // o = scale S^T q.  A wave takes 32 columns of S: lane (r, c) = (lane >> 3, lane & 7) rows R r .. R r + R - 1 of columns
-// 4 c .. 4 c + 3.
+// 4 c .. 4 c + 3, so that a row's 32 columns are a line and the sums over rows cross eight lanes; columns do not depend on each
+// other, and every one of them forms the token's norms, decay and rate anew rather than wait for one that does.
+//   What bounds it: S's bytes, read once and written once (a token of 64 sequences, 16 heads of 128 x 128, 136 MB: 24 us, 5.6 TB/s,
+// some of it from the last cache); a few tokens of few heads their chain, 2.2 us a token (rows, three sums, S's update).
 AH_DEV float sum_rows(float v) {  // over the eight lanes of a column
     v += __shfl_xor(v, 8, 64);
     v += __shfl_xor(v, 16, 64);
@@ -228,6 +232,9 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
 //   U = U0 - W S,  o = scale (e^gamma q S + P U),  P_ij = D_ij q_i . k_j (j <= i),  S' = e^gamma_63 S + (e^(gamma_63 - gamma) k)^T U.
 // delta_prepare_kernel makes W, U0, P and the decayed keys of all chunks at once; delta_chain_kernel then walks a sequence's
 // chunks with S in registers, two products deep a chunk.  No exponent above a sum of g's is ever formed, and sums of g are f64.
+//   Token by token a head's S passes registers once a token (8192 tokens of 16 heads: 20.7 ms); by chunks of 64 it takes 6 dk dv
+// products of 64 tokens on the matrix cores and a chain 64 times shorter (301 us).  Shorter chunks have a longer chain, longer
+// ones more of the triangle (T by recursion: 64 is four tiles of 16).
 //   f32 by f16: every factor of a product is carried as hi + lo, two f16 of a value scaled by a power of two so that the largest
 // of its group (a tile, a slice, a chunk) lies in [2^13, 2^14): 22 bits, or 2^-38 of the group's largest.  Three products
 // (hi hi, hi lo, lo hi) are summed in the f32 accumulator, at 5 times the rate of the f32 matrix instructions.
@@ -364,7 +371,9 @@ template <int DK> struct PrepareLds {
 };
 // Eight waves a chunk and head.  Waves 0 to 3 have the keys and beta_i k_i . k_j of 16 tokens i each, and make T of them; waves 4 to
 // 7 have q of the same tokens, P and q's fragments.  W and U0 are shared by all.  Barriers wait for LDS alone: loads and stores stay
-// on their way.
+// on their way.  What bounds it is vector work beside the waits at barriers (58% of a SIMD's cycles while a CU works, products 9%):
+// halves of every factor, T's recursion, the scales.  A chunk and head of 128 x 128 takes 26 us where two share a CU (5 x 301
+// tokens, 16 heads), 2048 of them 110.
 template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32_t hd, uint8_t *block, PrepareLds<DK> &L) {
     constexpr int NT = DK / 32;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
@@ -707,6 +716,10 @@ template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel
 // through LDS as operands.  Waves 4 to 7 make o of the same tokens: q S beside U, P U beside S.  Two barriers a chunk.
 //   What comes from memory is asked for two chunks ahead, and touched a few chunks before that, each of a head's workgroups a
 // part, so that it waits in the XCD's L2.
+//   What bounds it is that chain of two products, their scales and halves, and two barriers: 1.9 us a chunk of 128 x 128 where the
+// blocks lie in the last cache (8192 tokens of 16 heads: 128 workgroups of 256 CUs, 238 us), whatever the columns; more columns
+// a workgroup take longer a chunk and read a block fewer times.  In 5 x 301 tokens (NC 2, 28 us) products take 16% of a SIMD's
+// cycles while a CU works, vector work 27%, and the waves wait 37% of theirs.
 template <int DK, int NC> struct ChainLds {
     u32x4 sf[NC][DK / 32][2][64], uf[NC][2][2][64];
     float sinv[NC][4], stop[NC][4], uinv[NC];
@@ -964,7 +977,8 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
 }
 // The chain of one group of chunks beside the preparation of the next, where the chain leaves CUs to it: every sequence's chunks
 // begin .. begin + ring / 2 - 1 and, by the workgroups after the chain's, the ring / 2 after those.  The blocks of two groups
-// are there at once, [sequence][ring][head].
+// are there at once, [sequence][ring][head].  A launch of 16 chunks of 16 heads takes 38 us: 30 of chain, and 256 preparations
+// in the 128 CUs that it leaves, one a CU (the chain's registers leave a CU no room for two).
 template <int DK> __global__ void __launch_bounds__(512) delta_both_kernel(DeltaArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
     __shared__ ChainLds<DK, 1> L;

@@ -60,7 +60,7 @@ extern "C" {
 #define AH_ERR_OUT_OF_MEMORY 23
 #define AH_ERR_SCRATCH_LIMIT 24       /* a no-alloc call needs more than its fixed scratch  */
 #define AH_ERR_SEQ_TIMEOUT 25         /* a sequence's grid barrier waited past its limit    */
-#define AH_ERR_CACHE_RANGE 27         /* a sequence, position or page outside the 4-bit cache */
+#define AH_ERR_CACHE_RANGE 27         /* a sequence, position, page or slot outside its range */
 
 /* ggml type ids (format/quant.rs:20-49) */
 #define AH_GGML_Q5_0 6   /* format/quant.rs:28-29, :261-297 */
@@ -507,9 +507,8 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
  * d_from or d_to: what those then hold or begin from is unspecified.  A sequence without tokens hands its state on.  A sequence
  * whose tokens or slots are out of range is refused with AH_ERR_CACHE_RANGE and passed over; tokens of no sequence are not
  * written.  Rows are *_stride floats apart (outputs' and the convolution's at most 2^23), and outputs may not overlap inputs.
- * At most 65535 sequences.  A result that is
- * not finite is refused with AH_ERR_NONFINITE_INPUT (ah_sync_status): the outputs and state of its sequence and head or
- * channel, from its chunk of 64 tokens on, hold no values then. */
+ * At most 65535 sequences.  A result that is not finite is refused with AH_ERR_NONFINITE_INPUT (ah_sync_status): the
+ * outputs and state of its sequence and head or channel, from its chunk of 64 tokens on, hold no values then. */
 typedef struct ah_state_seqs {
     size_t n_seq, n_tok, max_q, n_slots;
     const int32_t *d_q_start;     /* [n_seq + 1] */
