@@ -421,8 +421,22 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         overlap(d_q, q_stride, a.n_heads * a.c.dim, d_out, out_stride, a.n_heads * a.c.dim, a.n_tok))
         return AH_ERR_INVALID_ARG;
     a.first_key = (uint32_t)prefix_len;
+    const size_t kv = a.c.n_kv, per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
+    const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
+    // A short prefix of few sequences, each reads for itself: it costs less than a second launch and the join.  (Single tokens of 14
+    // heads of 64 over 2, us a call for itself and together: 8 behind 2048 keys 12.9 and 15.9, 16 behind 4096 13.6 and 15.6, 64
+    // behind 512 12.3 and 14.6, 32 behind 2048 and 512 more 15.1 and 14.8, 4 behind 16384 16.9 and 15.1; 12 of 128 over 2: 8 behind
+    // 2048 14.2 and 16.2, 16 behind 4096 17.5 and 17.1, 8 behind 8192 19.5 and 15.9; 32 over 8: 16 behind 2048 19.7 and 16.0.
+    // Heads of 256 gain nothing.)
+    if (a.c.dim < 256 && prefix_len <= 4096 && a.n_seq * ((per_seq + 15) / 16) * kv * a.c.dim * prefix_len <= (size_t)1 << 23) {
+        a.first_table = d_prefix_table;
+        const int32_t st = attn_rows_plan(ctx, a, (prefix_len + 31) / 32 + tiles, per_seq, 0, stream);
+        if (st) return st;
+        AH_HIP(ctx, ah_launch_attn_some(a, pick(ctx, stream)));
+        return AH_OK;
+    }
     AttnArgs pre = a, own = a;
-    const size_t kv = a.c.n_kv, cus = (size_t)ctx->cu_count, most = most_pieces(a, rows);
+    const size_t cus = (size_t)ctx->cu_count, most = most_pieces(a, rows);
     auto cut = [&](AttnArgs &x, size_t units, size_t tiles, size_t n) {  // into n pieces
         n = n < most / 2 ? n : most / 2;
         n = n < 1 ? 1 : n;
@@ -436,8 +450,6 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     // of 16 twelve a CU and more (2 KV heads of 128, sequences x tokens and their keys, units, us by 16 and by 128: 16 x 128 of
     // 128 1536 100 and 112; 64 x 49 of 2048 2432 181 and 186; 32 x 128 of 128 12 a CU 109 and 103; 32 x 256 of 256 6144 213
     // and 189; 16 x 512 of 512 6144 242 and 198).
-    const size_t per_seq = (size_t)a.max_q * a.group, room = (size_t)a.table_stride << a.c.page_shift;
-    const size_t end = p->max_ctx < room ? p->max_ctx : room, tiles = end > prefix_len ? (end + 31) / 32 - prefix_len / 32 : 0;
     own.rows = per_seq <= 8 ? 8 : 16;
     size_t own_units = (per_seq + own.rows - 1) / own.rows * kv * a.n_seq;
     if (per_seq > 128 && own_units >= 12 * cus) {
@@ -559,7 +571,7 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     rows.list = b.list;
     AH_HIP(ctx, ah_launch_block_choice(b, pick(ctx, stream)));
     if (alone) AH_HIP(ctx, ah_launch_attend_lists(rows, pick(ctx, stream)));
-    else AH_HIP(ctx, ah_launch_attn_blocks(rows, pick(ctx, stream)));
+    else AH_HIP(ctx, ah_launch_attn_some(rows, pick(ctx, stream)));
     return AH_OK;
 }
 

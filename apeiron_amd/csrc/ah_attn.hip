@@ -34,9 +34,10 @@ AH_DEV Tiles tiles_of(const AttnArgs &a, int32_t lo, int32_t hi) {
 //   kAll: the positions that a query sees, in its sequence's pages;
 //   kPrefix: every row the first first_key positions, in the pages of one table: the whole batch as one sequence;
 //   kAfter: as kAll, from position first_key on;
+//   kTwo: as kAll, the positions below first_key in the pages of a table of their own, for each sequence anew;
 //   kBlocks: every (token, KV head) the blocks that it has a list of, as if they stood one after the other.
 // kPrefix and kAfter leave their pieces for attn_meet_kernel, pieces of kAfter without a key with no weight.
-enum { kAll, kPrefix, kAfter, kBlocks };
+enum { kAll, kPrefix, kAfter, kBlocks, kTwo };
 template <int MODE> AH_DEV Span span_in(const AttnArgs &a, uint32_t s, uint32_t kvh) {
     if (MODE == kPrefix) return {0, a.n_tok, (int32_t)a.first_key, false};
     if (MODE == kBlocks) {  // [0] of a list: its keys, kNoList where the token is no sequence's
@@ -53,19 +54,19 @@ template <int MODE> AH_DEV Span span_in(const AttnArgs &a, uint32_t s, uint32_t 
         return {s, none ? 0u : 1u, none ? 0 : (int32_t)keys, none};
     }
     Span p = span_of(a, s);
-    if (MODE == kAfter && !p.bad && (uint32_t)(p.ctx - (int32_t)p.nq) < a.first_key) p = {0, 0, 0, true};
+    if ((MODE == kAfter || MODE == kTwo) && !p.bad && (uint32_t)(p.ctx - (int32_t)p.nq) < a.first_key) p = {0, 0, 0, true};
     return p;
 }
 template <int MODE> AH_DEV int32_t position_of(const Span &p, uint32_t tok) {  // of a span's token
     return MODE == kPrefix ? p.ctx - 1 : p.ctx - (int32_t)p.nq + (int32_t)tok;
 }
 template <int MODE> AH_DEV Tiles tiles_in(const AttnArgs &a, int32_t lo, int32_t hi) {
-    if (MODE != kAfter) return tiles_of(a, lo, hi);
+    if (MODE != kAfter && MODE != kTwo) return tiles_of(a, lo, hi);
     Tiles t;
     t.end = hi < 0 ? 0 : ((uint32_t)hi >> 5) + 1;
-    t.head = 0;
+    t.head = MODE == kTwo ? (a.first_key >> 5) + ((a.first_key & 31) != 0) : 0;  // (a tile may be in both)
     t.tail = a.first_key >> 5;
-    t.count = t.end > t.tail ? t.end - t.tail : 0;
+    t.count = t.head + (t.end > t.tail ? t.end - t.tail : 0);
     return t;
 }
 
@@ -75,18 +76,19 @@ AH_DEV uint32_t piece_of(const AttnArgs &a, const Tiles &t) {
     return need > a.chunk ? need : a.chunk;
 }
 
-// Byte offset in the cache of tile `tile` of sequence s for head kvh, through the page table; `ok` false where
+// Tile `tile` for head kvh in the cache, through a sequence's row of the page table; `ok` false where
 // the page is outside.  The index is read through the scalar cache: it is the same for the whole wave.
-AH_DEV const uint8_t *tile_at(const AttnArgs &a, uint32_t s, uint32_t kvh, uint32_t tile, bool &ok) {
+AH_DEV const uint8_t *tile_at(const AttnArgs &a, const int32_t *table, uint32_t kvh, uint32_t tile, bool &ok) {
     typedef const int32_t __attribute__((address_space(4))) *cptr;
     const uint32_t in = a.c.page_shift - 5, pi = tile >> in;
-    const uint32_t page = (uint32_t)((cptr)(uintptr_t)a.table)[(size_t)s * a.table_stride + pi];
+    const uint32_t page = (uint32_t)((cptr)(uintptr_t)table)[pi];
     ok = page < a.c.n_pages;
     return a.c.base + kv4_tile(a.c, ok ? page : 0, kvh, tile & ((1u << in) - 1));
 }
 
-template <int MODE> AH_DEV const uint8_t *tile_in(const AttnArgs &a, uint32_t s, uint32_t kvh, uint32_t tile, bool &ok) {
-    if (MODE != kBlocks) return tile_at(a, s, kvh, tile, ok);
+// (prefix: of kTwo, a tile of the first table)
+template <int MODE> AH_DEV const uint8_t *tile_in(const AttnArgs &a, uint32_t s, uint32_t kvh, uint32_t tile, bool &ok, bool prefix = false) {
+    if (MODE != kBlocks) return tile_at(a, MODE == kTwo && prefix ? a.first_table : a.table + (size_t)s * a.table_stride, kvh, tile, ok);
     typedef const uint32_t __attribute__((address_space(4))) *cptr;
     const uint32_t at = ((cptr)(uintptr_t)a.list)[((size_t)s * a.c.n_kv + kvh) * a.list_stride + 1 + (tile >> a.block_shift)];
     ok = at != kNoList;
@@ -131,8 +133,8 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
     const int32_t lo = position_of<MODE>(p, row0 / a.group), hi = position_of<MODE>(p, last / a.group);
     const int32_t pos = live ? position_of<MODE>(p, tok) : -1;
     // the keys below which the window hides one (for this row, and for the last of the rows), and the sinks
-    const int32_t low_key = MODE == kAfter ? (int32_t)a.first_key : a.window ? pos - (int32_t)a.window + 1 : 0;
-    const int32_t low_all = MODE == kAfter ? (int32_t)a.first_key : a.window ? hi - (int32_t)a.window + 1 : 0;
+    const int32_t low_key = MODE == kAfter || MODE == kTwo ? (int32_t)a.first_key : a.window ? pos - (int32_t)a.window + 1 : 0;
+    const int32_t low_all = MODE == kAfter || MODE == kTwo ? (int32_t)a.first_key : a.window ? hi - (int32_t)a.window + 1 : 0;
     const int32_t sink_key = (int32_t)a.sinks;
     const Tiles T = tiles_in<MODE>(a, lo, hi);
     const uint32_t chunk = piece_of(a, T), t0 = split * chunk, t1 = t0 + chunk < T.count ? t0 + chunk : T.count;
@@ -145,7 +147,7 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
     uint32_t ti = t0 + wave;
     auto tile_of = [&](uint32_t i) { return i < T.head ? i : T.tail + (i - T.head); };
     if (ti < t1) {
-        const uint8_t *t = tile_in<MODE>(a, s, kvh, tile_of(ti), ok);
+        const uint8_t *t = tile_in<MODE>(a, s, kvh, tile_of(ti), ok, ti < T.head);
         k.load(t, r, h);
         v.load(t, r, h);
     }
@@ -197,7 +199,7 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
     for (; ti < t1; ti += 4) {
         const uint32_t tile = tile_of(ti), next = ti + 4 < t1 ? ti + 4 : ti;
         bool ok_next;
-        const uint8_t *tn = tile_in<MODE>(a, s, kvh, tile_of(next), ok_next);
+        const uint8_t *tn = tile_in<MODE>(a, s, kvh, tile_of(next), ok_next, next < T.head);
         f32x4 c[C][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
@@ -217,7 +219,8 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
         f16x8 pf[C], pg[C];
         const int32_t first = (int32_t)(tile * 32);
         // a tile that every row sees whole needs no mask
-        const bool whole = ok && first + 31 <= lo && (first >= low_all || first + 32 <= sink_key);
+        const bool prefix = MODE == kTwo && ti < T.head;
+        const bool whole = ok && (prefix ? first + 31 < (int32_t)a.first_key : first + 31 <= lo && (first >= low_all || first + 32 <= sink_key));
         if (!whole && !ok && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
 #pragma unroll
         for (int n = 0; n < C; ++n) {
@@ -232,7 +235,7 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
 #pragma unroll
                 for (int i = 0; i < 8; ++i) {
                     const int32_t key = first + 16 * (i >> 2) + 4 * (int32_t)h + (i & 3);
-                    const bool see = key <= top_key && (key >= low_key || key < sink_key);
+                    const bool see = key <= top_key && (prefix ? key < (int32_t)a.first_key : key >= low_key || key < sink_key);
                     x[i] = see ? x[i] : -__builtin_inff();
                 }
             }
@@ -483,7 +486,7 @@ template <int D, int MODE> AH_DEV void attn_tiles(const AttnArgs &a, uint32_t bl
 #pragma unroll
         for (uint32_t j = 0; j < 2; ++j) {
             bool ok;
-            base[j] = tile_at(a, s, kvh, tile_of(ti + j < t1 ? ti + j : t1 - 1), ok);
+            base[j] = tile_at(a, a.table + (size_t)s * a.table_stride, kvh, tile_of(ti + j < t1 ? ti + j : t1 - 1), ok);
             if (!ok || ti + j >= t1) bad |= 1u << j;
             if (!ok && ti + j < t1 && lane == 0) ah_record(a.status, ((unsigned long long)s << 8) + AH_ERR_CACHE_RANGE);
         }
@@ -962,8 +965,9 @@ template <int D> hipError_t launch_shared(const AttnArgs &prefix, const AttnArgs
     hipLaunchKernelGGL(attn_meet_kernel<D>, dim3(both.n_tok * ((both.n_heads + 256 / D - 1) / (256 / D))), dim3(256), 0, stream, both);
     return hipGetLastError();
 }
-template <int D> hipError_t launch_blocks(const AttnArgs &a, hipStream_t stream) {
-    launch_rows<D, kBlocks>(a, stream);
+template <int D> hipError_t launch_some(const AttnArgs &a, hipStream_t stream) {
+    if (D < 256 && a.first_table) launch_rows<D, D < 256 ? kTwo : kBlocks>(a, stream);
+    else launch_rows<D, kBlocks>(a, stream);
     return hipGetLastError();
 }
 
@@ -987,8 +991,8 @@ hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream) {
 hipError_t ah_launch_attn_shared(const AttnArgs &p, const AttnArgs &s, const AttnArgs &both, hipStream_t stream) {
     return p.c.dim == 64 ? launch_shared<64>(p, s, both, stream) : p.c.dim == 128 ? launch_shared<128>(p, s, both, stream) : launch_shared<256>(p, s, both, stream);
 }
-hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream) {
-    return a.c.dim == 64 ? launch_blocks<64>(a, stream) : a.c.dim == 128 ? launch_blocks<128>(a, stream) : launch_blocks<256>(a, stream);
+hipError_t ah_launch_attn_some(const AttnArgs &a, hipStream_t stream) {
+    return a.c.dim == 64 ? launch_some<64>(a, stream) : a.c.dim == 128 ? launch_some<128>(a, stream) : launch_some<256>(a, stream);
 }
 
 template <int D, int ROWS> hipError_t allow_both() {

@@ -133,7 +133,8 @@ struct AttnArgs {
     uint32_t join;
     uint32_t *count;
     unsigned long long *status;
-    uint32_t first_key;  // of a batch behind a common prefix: its length
+    uint32_t first_key;          // of a batch behind a common prefix: its length
+    const int32_t *first_table;  // its pages, where each sequence reads it for itself
     // of attention over blocks: for every (token, KV head) its keys (kNoList: no token of a sequence), then the first
     // tiles (kv4_tile's, counted; kNoList: none to see) of its blocks of 1 << block_shift tiles
     const uint32_t *list;
@@ -206,7 +207,7 @@ hipError_t ah_launch_kv4_append(const AppendArgs &a, hipStream_t stream);
 hipError_t ah_launch_kv4_read(const KvReadArgs &a, hipStream_t stream);
 hipError_t ah_launch_attn(const AttnArgs &a, hipStream_t stream);
 hipError_t ah_launch_attn_shared(const AttnArgs &prefix, const AttnArgs &after, const AttnArgs &both, hipStream_t stream);
-hipError_t ah_launch_attn_blocks(const AttnArgs &a, hipStream_t stream);
+hipError_t ah_launch_attn_some(const AttnArgs &a, hipStream_t stream);  // over lists of blocks, or (first_table) two tables
 hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream);
 hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream);
 hipError_t ah_launch_attend_lists(const AttnArgs &a, hipStream_t stream);

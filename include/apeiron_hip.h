@@ -470,10 +470,11 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *arg
                         float *d_out, size_t out_stride, void *stream);
 
 /* ah_kv4_attn_dev for sequences that begin with the same prefix_len positions (args' window and sinks 0): those are
- * read once for the whole batch.  d_prefix_table: their pages, [ceil(prefix_len / page_len)]; the positions from
- * prefix_len on are read through d_table as ever (whose entries for pages before that are not read).  The result is what
- * ah_kv4_attn_dev gives for tables that name the prefix's pages.  A sequence with tokens before the prefix's end is
- * refused as one out of range.  prefix_len 0: ah_kv4_attn_dev.  d_out may not overlap d_q; at most 2^30 - 1 values of it. */
+ * read once for the whole batch (or, a short prefix of few sequences, by each).  d_prefix_table: their pages,
+ * [ceil(prefix_len / page_len)]; the positions from prefix_len on are read through d_table as ever (whose entries for pages
+ * before that are not read).  The result is what ah_kv4_attn_dev gives for tables that name the prefix's pages.  A sequence
+ * with tokens before the prefix's end is refused as one out of range.  prefix_len 0: ah_kv4_attn_dev.  d_out may not
+ * overlap d_q; at most 2^30 - 1 values of it.  Uses the context's scratch. */
 int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, size_t prefix_len,
                                const int32_t *d_prefix_table, const float *d_q, size_t q_stride, float *d_out,
                                size_t out_stride, void *stream);
@@ -534,7 +535,8 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *args,
  * beta = 1 / (1 + e^-b); without (NULL), a is g and b is beta.  norm_eps >= 0: q and k are divided by
  * sqrt(their sum of squares + norm_eps) first; negative: taken as they are.  k_dim 64 or 128, v_dim 64, 128 or 256.  d_q,
  * d_k: [n_tok] rows of n_k_heads heads, d_v, d_out: of n_heads, d_a, d_b: one value a head.  Uses the context's scratch
- * (as ah_gemm_f32_dev, also for calls captured into a graph). */
+ * (as ah_gemm_f32_dev, also for calls captured into a graph): 768 k_dim + 256 v_dim + 13 KB for every 64 tokens and head
+ * and for every sequence and head, less where few sequences are long. */
 typedef struct ah_delta_rule {
     size_t n_heads, n_k_heads, k_dim, v_dim;
     const float *d_a_log, *d_dt_bias; /* [n_heads], both or neither */

@@ -191,6 +191,35 @@ def test_shared_prefix_of_many_rows(dev, dim, kv, G, qs, after, prefix):  # noqa
 
 
 @pytest.mark.gpu
+@pytest.mark.parametrize("dim,kv,G,pad", [(64, 2, 7, 0), (128, 2, 6, 4), (64, 1, 1, 1), (128, 1, 19, 0), (128, 4, 2, 2)])
+@pytest.mark.parametrize("qs,after,prefix", [([1, 1, 1], [6, 1, 36], 4097), ([1] * 9, [1 + 7 * i for i in range(9)], 4128), ([5, 0, 33, 1, 17], [11, 2, 71, 1, 17], 5000), ([1] * 40, [1 + i for i in range(40)], 4100)])
+def test_a_long_shared_prefix(dev, dim, kv, G, pad, qs, after, prefix):  # noqa: F811
+    """Past the lengths that a sequence reads for itself."""
+    ctx = [prefix + n for n in after]
+    B = Batch(dev, qs, ctx, kv, G, dim, 64, prefix=prefix, seed=dim, pad=pad)
+    table = B.P.table.clone()
+    first = table[0, : -(-prefix // 64)].clone()
+    table[:, : prefix // 64] = 1 << 30  # the sequences' own entries before the prefix's end are not read
+    status, out = B.shared(prefix_table=first, table=table)
+    assert status == OK and (out[:, B.heads * dim:] == 7).all()
+    for s in range(len(qs)):
+        if qs[s]:
+            see = np.arange(ctx[s]) <= B.positions(s)[:, None, None]
+            compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], np.broadcast_to(see, (qs[s], kv, ctx[s])), B.scale)
+    # a page of the prefix out of range: its positions are not seen; a context inside the prefix: passed over
+    good, first[3] = out, -1
+    status, out = B.shared(prefix_table=first, table=table)
+    assert status == CACHE
+    for s in range(len(qs)):
+        if qs[s]:
+            see = (np.arange(ctx[s]) <= B.positions(s)[:, None, None]) & (np.arange(ctx[s]) // 64 != 3)
+            compare(B.rows(s, out), B.rows(s, B.q), B.k[s], B.v[s], np.broadcast_to(see, (qs[s], kv, ctx[s])), B.scale)
+    first[3] = B.P.table[0, 3]
+    status, out = B.shared(prefix_table=first, table=table, ctx=[prefix + qs[0] - 1] + ctx[1:])
+    assert status == CACHE and (out[: qs[0]] == 7).all() and np.array_equal(out[qs[0]:], good[qs[0]:])
+
+
+@pytest.mark.gpu
 def test_shared_prefix_of_none_is_the_plain_call(dev):  # noqa: F811
     B = Batch(dev, [1, 40], [300, 500], 2, 4, 64, 32, seed=1)
     assert np.array_equal(B.shared(prefix=0)[1], B.plain()[1])
