@@ -203,8 +203,10 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
         f32x4 c[C][2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
-            // The lo halves' products apart: a score is rounded half as often at its own size.  Of 1000 calls behind a prefix
-            // 0 and 8 were over 1e-6 off with and without (plain f32 operations 268), for 2% of the time.  (kAll stays as it was.)
+            // The lo halves' products, or packed the second half of the channels', apart: a score is rounded half as often at its
+            // own size.  Of 1000 calls behind a prefix 0 and 8 were over 1e-6 off with and without (plain f32 operations 268), for
+            // 2% of the time.  (kAll stays as it was.)
+            constexpr bool kApart = MODE != kAll && (!PACK || D > 64);
             f32x4 rest[C];
 #pragma unroll
             for (int n = 0; n < C; ++n) c[n][half] = rest[n] = (f32x4)0.0f;
@@ -213,12 +215,13 @@ template <int D, bool PACK, int MODE, int C = 1> AH_DEV void attn_rows(const Att
                 const f16x8 kf = k_frag(k.code(half, j), k.scale(half, j), mk);
 #pragma unroll
                 for (int n = 0; n < C; ++n) {
-                    c[n][half] = mfma16(kf, qh[n][j], c[n][half]);
-                    if (!PACK && MODE == kAll) c[n][half] = mfma16(kf, ql[n][j], c[n][half]);
-                    if (!PACK && MODE != kAll) rest[n] = mfma16(kf, ql[n][j], rest[n]);
+                    if (PACK && kApart && j >= NJ / 2) rest[n] = mfma16(kf, qh[n][j], rest[n]);
+                    else c[n][half] = mfma16(kf, qh[n][j], c[n][half]);
+                    if (!PACK && !kApart) c[n][half] = mfma16(kf, ql[n][j], c[n][half]);
+                    if (!PACK && kApart) rest[n] = mfma16(kf, ql[n][j], rest[n]);
                 }
             }
-            if (!PACK && MODE != kAll)
+            if (kApart)
 #pragma unroll
                 for (int n = 0; n < C; ++n) c[n][half] += rest[n];
         }

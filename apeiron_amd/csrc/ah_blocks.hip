@@ -486,9 +486,14 @@ template <int D, class T> AH_DEV void attend_rows(const AttnArgs &a, uint32_t to
         f32x4 c[2];
 #pragma unroll
         for (int half = 0; half < 2; ++half) {
+            f32x4 rest = (f32x4)0.0f;  // (as in attn_rows)
             c[half] = (f32x4)0.0f;
 #pragma unroll
-            for (int j = 0; j < NJ; ++j) c[half] = mfma16(k_frag(k.code(half, j), k.scale(half, j), mk), qh[j], c[half]);
+            for (int j = 0; j < NJ; ++j) {
+                f32x4 &to = D > 64 && j >= NJ / 2 ? rest : c[half];
+                to = mfma16(k_frag(k.code(half, j), k.scale(half, j), mk), qh[j], to);
+            }
+            if (D > 64) c[half] += rest;
         }
         k.load(tn, r, h);
         float x[8];
