@@ -201,3 +201,68 @@ def test_a_hybrid_model_serves_a_batch_behind_a_common_prompt(dev, prompts):  # 
         for c in model.cache:
             c.free()
     d.close()
+
+
+def prompt_pass(M, prompts):
+    """What a pass over prompts behind the prefix needs, and the pass: from slot 0 and the prefix's pages, so that it may be repeated."""
+    M.run(M.x[0][:PREFIX].contiguous(), M.arrays([PREFIX], [PREFIX], [-1], [0]), 0)
+    t = M.arrays(prompts, [PREFIX + p for p in prompts], [0] * M.n, [s + 1 for s in range(M.n)])
+    x = torch.cat([M.x[s][PREFIX:PREFIX + p] for s, p in enumerate(prompts)])
+    torch.cuda.synchronize()
+    return lambda: M.run(x, t, PREFIX)
+
+
+@pytest.mark.gpu
+def test_two_contexts_at_once_on_two_streams(dev):  # noqa: F811
+    """Contexts have scratch of their own: passes that run at the same time leave what each leaves alone."""
+    devices, streams, kinds = [chart.Device(0), chart.Device(0)], [torch.cuda.Stream(), torch.cuda.Stream()], ([300, 2, 150], [64, 64, 64, 64, 64])
+    models = [Model(d, p) for d, p in zip(devices, kinds)]
+    passes = [prompt_pass(M, p) for M, p in zip(models, kinds)]
+    want = []
+    for M, go in zip(models, passes):
+        x, pick = go()
+        torch.cuda.synchronize()
+        want.append((x.clone(), pick.clone(), M.state.clone(), M.tail.clone()))
+    for _ in range(5):
+        got = []
+        for st, go in zip(streams, passes):
+            with torch.cuda.stream(st):
+                got.append(go())
+        torch.cuda.synchronize()
+        for M, (x, pick), (x0, pick0, state, tail) in zip(models, got, want):
+            assert torch.equal(x, x0) and torch.equal(pick, pick0) and torch.equal(M.state, state) and torch.equal(M.tail, tail)
+    for d, M, st in zip(devices, models, streams):
+        assert d.sync_status(st.cuda_stream) == OK
+        for c in M.cache:
+            c.free()
+        d.close()
+
+
+@pytest.mark.gpu
+def test_two_graphs_share_a_contexts_scratch(dev):  # noqa: F811
+    """Captured one after the other, the second growing the scratch; replayed in turn, with eager passes between."""
+    d, kinds = chart.Device(0), ([3, 40, 1], [500, 300, 64])
+    models = [Model(d, p) for p in kinds]
+    passes = [prompt_pass(M, p) for M, p in zip(models, kinds)]
+    want, graphs, outs = [], [], []
+    for M, go in zip(models, passes):
+        x, pick = go()
+        torch.cuda.synchronize()
+        want.append((x.clone(), pick.clone(), M.state.clone()))
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            outs.append(go())
+        graphs.append(graph)
+    for turn in range(4):
+        for M, graph, out, (x, pick, state), go in zip(models, graphs, outs, want, passes):
+            out[0].zero_(), out[1].zero_(), M.state[1:].zero_()
+            graph.replay()
+            torch.cuda.synchronize()
+            assert torch.equal(out[0], x) and torch.equal(out[1], pick) and torch.equal(M.state, state), turn
+            if turn == 2:
+                go()
+    assert d.sync_status(stream()) == OK
+    for M in models:
+        for c in M.cache:
+            c.free()
+    d.close()
