@@ -96,12 +96,16 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
     const bool chunks = a.s.max_q > most_steps, even = a.s.n_seq == 1 || n == (size_t)a.s.n_seq * a.s.max_q;
     a.chunk_from = !chunks ? 0xffffffffu : even ? 0 : (uint32_t)most_steps + 1;
     if (chunks) {
-        const size_t bytes = delta_block((uint32_t)dk, (uint32_t)dv).bytes, columns = units * (dv / 16), per = (a.s.max_q + kDeltaChunk - 1) / kDeltaChunk;
-        // A workgroup of the chain takes 16 columns of S; 32 or 64 where there are more of them than CUs and then than fill eight
+        // (uneven: at most `longs` sequences go by chunks, and as many of the longest would have the batch's tokens)
+        const size_t longest = n / (most_steps + 1), longs = even || longest > a.s.n_seq ? a.s.n_seq : longest, as_long = (n + a.s.max_q - 1) / a.s.max_q;
+        const size_t columns = (even ? a.s.n_seq : as_long) * H * (dv / 16), bytes = delta_block((uint32_t)dk, (uint32_t)dv).bytes, per = (a.s.max_q + kDeltaChunk - 1) / kDeltaChunk;
+        // A workgroup of the chain takes 16 columns of S; 32 or 64 where there are more of them than CUs and then than fill six
         // rounds: a chunk's block is read by fewer workgroups.  (16 heads of 128 x 128, us with 16, 32, 64: 1 x 64 tokens 25,
         // 25, 30; 2 x 301 35, 39, 52; 5 x 301 66, 62, 63; 4 x 2048 274, 205, 336; 8 x 1024 326, 241, 246; 16 x 512 410, 284,
-        // 269; columns of 64: 64 x 512 1189, 801, 692.)
-        a.tiles = columns >= 8 * cus ? 4 : columns > cus ? 2 : 1;
+        // 269; columns of 64: 64 x 512 1189, 801, 692.  Uneven, one of 512 among 16 single tokens 53, 46, 67, among 64 70, 62, 83, among
+        // 256 166, 146, 146; 16 of up to 301 220, 157, 143.)
+        a.longs = (uint32_t)longs;
+        a.tiles = columns >= 6 * cus ? 4 : columns > cus || (!even && columns == cus) ? 2 : 1;
         // All chunks are prepared at once, or, where the chain leaves half of the CUs without work and the blocks would not
         // stay in the 256 MB of the last cache, by groups of as many as give every CU one, the next group's preparation beside a
         // group's chain.  (us at once and by groups: 16 heads, 4096 tokens (148 MB) 151 and 160, 6144 249 and 232, 8192 348 and
@@ -119,7 +123,7 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
             a.slot_seq = even || by_seq <= by_tokens;
             a.slot_shift = a.slot_seq ? 6 : 3;
             const size_t slots = a.slot_seq ? by_seq : by_tokens;
-            if (slots * H > kMaxGrid / 2 || columns > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
+            if (slots * H > kMaxGrid / 2 || units * (dv / 16) > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
             a.slots = (uint32_t)slots;
             need = slots * H * bytes;
         }

@@ -30,7 +30,7 @@ struct DeltaArgs {
     // Sequences of chunk_from tokens or more go by chunks of 64, the others token by token.  What the chunks' preparation leaves
     // is a block of delta_block_bytes for every (slot, head); sequence s has its chunks' slots from
     // (q_start[s] >> slot_shift) + s * slot_seq on.
-    uint32_t chunk_from, slots, slot_shift, slot_seq;
+    uint32_t chunk_from, longs, slots, slot_shift, slot_seq;  // longs: at most so many go by chunks
     uint32_t tiles;  // of 16 columns of S for a workgroup of the chain: 1, 2 or 4
     uint8_t *blocks;
     uint32_t chain_grid;  // workgroups of the chain; a launch may have others after them

@@ -720,6 +720,25 @@ template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel
 // blocks lie in the last cache (8192 tokens of 16 heads: 128 workgroups of 256 CUs, 238 us), whatever the columns; more columns
 // a workgroup take longer a chunk and read a block fewer times.  In 5 x 301 tokens (NC 2, 28 us) products take 16% of a SIMD's
 // cycles while a CU works, vector work 27%, and the waves wait 37% of theirs.
+// The nth sequence that goes by chunks, from the lanes that look for it; n_seq if there is none.  (Workgroups for every sequence of a batch of mostly single tokens
+// ended at once, but took as long to start as the others: one of 512 tokens among 256 158 us for 146, among 16 67 for 46.)
+AH_DEV uint32_t nth_long(const DeltaArgs &a, uint32_t nth, Seq &found) {
+    for (uint32_t base = 0; base < a.s.n_seq; base += 64) {
+        const uint32_t i = base + (threadIdx.x & 63);
+        const Seq p = seq_of(a.s, i < a.s.n_seq ? i : a.s.n_seq - 1);
+        const uint64_t all = __builtin_amdgcn_ballot_w64(i < a.s.n_seq && !p.bad && p.nq >= a.chunk_from);
+        const uint32_t n = (uint32_t)__builtin_popcountll(all);
+        if (nth < n) {
+            const bool me = (all >> (threadIdx.x & 63) & 1) && __builtin_amdgcn_mbcnt_hi((uint32_t)(all >> 32), __builtin_amdgcn_mbcnt_lo((uint32_t)all, 0)) == nth;
+            const int at = __builtin_ctzll(__builtin_amdgcn_ballot_w64(me));
+            found = {(uint32_t)__builtin_amdgcn_readlane((int)p.q0, at), (uint32_t)__builtin_amdgcn_readlane((int)p.nq, at), __builtin_amdgcn_readlane(p.from, at),
+                     __builtin_amdgcn_readlane(p.to, at), false};
+            return base + (uint32_t)at;
+        }
+        nth -= n;
+    }
+    return a.s.n_seq;
+}
 template <int DK, int NC> struct ChainLds {
     u32x4 sf[NC][DK / 32][2][64], uf[NC][2][2][64];
     float sinv[NC][4], stop[NC][4], uinv[NC];
@@ -734,16 +753,20 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
     auto &uinv = L.uinv;
     const uint32_t lane = threadIdx.x & 63, r = lane & 15, h = lane >> 4, wave = __builtin_amdgcn_readfirstlane(threadIdx.x >> 6), w = wave & 3;
     // columns slowest: a head's workgroups go to one XCD (they go to the eight in turn) wherever eight divides the heads
-    const uint32_t units = a.s.n_seq * a.n_heads, part = blockIdx.x / units, unit = blockIdx.x - part * units, s = unit / a.n_heads, hd = unit - s * a.n_heads;
-    const Seq p = seq_of(a.s, s);
+    const uint32_t units = a.longs * a.n_heads, part = blockIdx.x / units, unit = blockIdx.x - part * units, nth = unit / a.n_heads, hd = unit - nth * a.n_heads;
+    Seq p;
+    uint32_t s = nth;
+    if (a.chunk_from) s = nth_long(a, nth, p);
+    else p = seq_of(a.s, s);
+    if (s >= a.s.n_seq) return;
     if (p.bad && part == 0 && hd == 0 && threadIdx.x == 0) ah_record(a.status, ((unsigned long long)s << 8) + kKeyRange);
-    if (p.bad || p.nq < a.chunk_from) return;
+    if (p.bad) return;
     // this launch's chunks: begin .. chunks - 1 of `whole`
     const uint32_t whole = (p.nq + kDeltaChunk - 1) / kDeltaChunk, begin = a.ring ? a.begin : 0, end = a.ring ? a.begin + a.ring / 2 : whole;
     const uint32_t chunks = whole < end ? whole : end, dv = a.v_dim, cb = part * NC;
     if (begin && begin >= whole) return;
     const DeltaBlock B = delta_block(DK, dv);
-    const size_t step = (size_t)a.n_heads * B.bytes, first = (a.ring ? s * a.ring : ((uint32_t)a.s.q_start[s] >> a.slot_shift) + s * a.slot_seq) * step + (size_t)hd * B.bytes;
+    const size_t step = (size_t)a.n_heads * B.bytes, first = (a.ring ? s * a.ring : (p.q0 >> a.slot_shift) + s * a.slot_seq) * step + (size_t)hd * B.bytes;
     auto block_of = [&](uint32_t n) {
         const uint32_t m = n < chunks ? n : chunks - 1;
         return a.blocks + first + (a.ring ? m % a.ring : m) * step;
@@ -997,9 +1020,8 @@ template <int DK> __global__ void __launch_bounds__(512) delta_both_kernel(Delta
 
 // The chain, and in the workgroups after it, where the lengths differ, the sequences that go token by token.
 template <int DK, int NC> void launch_chain(DeltaArgs a, bool mixed, hipStream_t stream) {
-    const uint32_t units = a.s.n_seq * a.n_heads;
-    a.chain_grid = units * (a.v_dim / (16 * NC));
-    hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.chain_grid + (mixed ? (units * (a.v_dim / 32) + 7) / 8 : 0)), dim3(512), 0, stream, a);
+    a.chain_grid = a.longs * a.n_heads * (a.v_dim / (16 * NC));
+    hipLaunchKernelGGL((delta_chain_kernel<DK, NC>), dim3(a.chain_grid + (mixed ? (a.s.n_seq * a.n_heads * (a.v_dim / 32) + 7) / 8 : 0)), dim3(512), 0, stream, a);
 }
 // Groups of chunks: each launch has the chain of one and the preparation of the next.
 template <int DK> void launch_groups(DeltaArgs a, hipStream_t stream) {

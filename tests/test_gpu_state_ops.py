@@ -348,7 +348,7 @@ def test_delta_rule_of_long_sequences(dev, K, H, dk, dv, qs, rows):  # noqa: F81
 
 @pytest.mark.gpu
 @pytest.mark.parametrize("dk,dv", [(64, 64), (128, 128), (64, 256), (128, 64)])
-@pytest.mark.parametrize("H,qs", [(64, [24, 25, 90, 1, 130, 0, 65, 24, 2]), (64, [25] * 8), (64, [24] * 8), (48, [16, 17, 3, 100, 15, 1]), (3, [1] * 40 + [70, 1, 1, 9, 66, 8])])
+@pytest.mark.parametrize("H,qs", [(64, [24, 25, 90, 1, 130, 0, 65, 24, 2]), (64, [25] * 8), (64, [24] * 8), (48, [16, 17, 3, 100, 15, 1]), (3, [1] * 40 + [70, 1, 1, 9, 66, 8]), (4, [1] * 100 + [70] + [2, 0] * 30 + [130, 17, 90] + [1] * 70 + [65]), (2, [33] * 70 + [1, 200])])
 def test_delta_rule_of_many_heads(dev, dk, dv, H, qs):  # noqa: F811
     """The lengths around which sequences go by tokens or by chunks, the chain's wider columns, many single tokens."""
     R = Rule(qs, H // 3 if H % 3 == 0 else H // 2, H, dk, dv, seed=H + dk, slots=len(qs) + 2)
