@@ -27,15 +27,23 @@ AH_DEV Seq seq_of(const StateSeqs &a, uint32_t s) {
 }
 
 // v / (1 + e^-v).  e^-v = 2^t (1 + r ln 2), t the f32 product v log2(e) and r what that rounding and log2(e)'s left out, a few
-// last places of t; the quotient by v_rcp_f32 with a Newton step.  Within 4 2^-24 of the result (5 x 1021 tokens of 4099 channels
-// with a library exponential and division: 41 us for 39).
+// last places of t; the quotient by v_rcp_f32 with a Newton step.  Past t = 100 the power is formed 2^-64 times as large (1 + it is
+// it) and the quotient multiplied by as much, so that neither it nor v_rcp_f32's result leaves f32's normal numbers; below -130
+// the result is -0 as it is there.  Within 6 2^-24 of the result, or half of f32's smallest number.  (5 x 1021 tokens of 4099
+// channels with a library exponential and division: 41 us for 39.)
 AH_DEV float silu(float v) {
     constexpr float kHi = -1.44269502162933349609f, kLo = -1.92596299112661746887e-8f, kLn2 = 0.69314718f;
-    const float t = v * kHi, r = __builtin_fmaf(v, kHi, -t) + v * kLo;
-    float e = __builtin_amdgcn_exp2f(t);
-    e = __builtin_fmaf(e, __builtin_fabsf(t) < 126.0f ? r * kLn2 : 0.0f, e);
-    const float d = 1.0f + e, q = __builtin_amdgcn_rcpf(d), y = v * q;
-    return d < 0x1p100f ? __builtin_fmaf(__builtin_fmaf(-d, y, v), q, y) : y;
+    const float w = v < -130.0f ? -130.0f : v;
+    float t = w * kHi;
+    __asm__("" : "+v"(t));  // (t - 64 of the rounded product, which r belongs to: no fused w kHi - 64)
+    const float r = __builtin_fmaf(w, kHi, -t) + w * kLo;
+    const bool far = t > 100.0f;
+    float e = __builtin_amdgcn_exp2f(far ? t - 64.0f : t);
+    e = __builtin_fmaf(e, t > -126.0f ? r * kLn2 : 0.0f, e);
+    const float d = 1.0f + e, q = __builtin_amdgcn_rcpf(d);
+    float y = w * q;
+    y = __builtin_fmaf(__builtin_fmaf(-d, y, w), q, y);
+    return far ? y * 0x1p-64f : y;
 }
 AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
 

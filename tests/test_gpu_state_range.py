@@ -1,0 +1,35 @@
+"""The recurrent layer's operators over the whole range of their inputs: activations far from zero.
+
+Tolerances (u = 2^-24, f32's rounding):
+  SiLU   v / (1 + e^-v): the exponential takes up to 2 u (v_exp_f32's last place) and two roundings, the sum, the quotient's
+         product and its Newton step one each: 6 u of the result, and half of f32's smallest number (2^-150), where it is
+         below the normal ones.  With a bias of zero and one weight of one the value before it is the input itself.
+"""
+import numpy as np
+import pytest
+
+from test_gpu_state_ops import OK, U, conv, dev  # noqa: F401
+
+torch = pytest.importorskip("torch")
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qs", [[1] * 40, [40], [9, 1, 30]])
+def test_silu_of_any_finite_value(dev, qs):  # noqa: F811
+    rng = np.random.default_rng(len(qs))
+    C = 130
+    x = rng.uniform(-110, 110, (40, C)).astype(np.float32)
+    x[0] = rng.uniform(-89, -87, C)
+    x[1] = rng.uniform(-75, -68, C)
+    edges = [88, 88.73, 89, 100, 104, 126, 128, 130, 1e4, 1e30, 3e38, 3.4028234663852886e38, 2.0 ** -126, 1e-45, 0]
+    x[2, :30] = np.float32(edges + [-v for v in edges])
+    x[3], x[4] = -np.exp(rng.uniform(0, 88, C)), np.exp(rng.uniform(0, 88, C))
+    w = np.zeros((C, 4), np.float32)
+    w[:, 3] = 1
+    src = list(range(len(qs)))
+    status, y, _ = conv(dev, x, w, None, True, qs, src, src, np.zeros((len(qs), 3, C), np.float32))
+    v = x.astype(np.float64)
+    with np.errstate(over="ignore"):
+        ref = v / (1 + np.exp(-v))
+    assert status == OK
+    assert (np.abs(y - ref) <= 6 * U * np.abs(ref) + 2.0 ** -150).all()
