@@ -54,7 +54,7 @@ template <int MODE> AH_DEV Span span_in(const AttnArgs &a, uint32_t s, uint32_t 
         return {s, none ? 0u : 1u, none ? 0 : (int32_t)keys, none};
     }
     Span p = span_of(a, s);
-    if ((MODE == kAfter || MODE == kTwo) && !p.bad && p.ctx - (int32_t)p.nq < (int32_t)a.first_key) p = {0, 0, 0, true};
+    if ((MODE == kAfter || MODE == kTwo) && p.nq && p.ctx - (int32_t)p.nq < (int32_t)a.first_key) p = {0, 0, 0, true};
     return p;
 }
 template <int MODE> AH_DEV int32_t position_of(const Span &p, uint32_t tok) {  // of a span's token

@@ -473,7 +473,8 @@ int32_t ah_kv4_attn_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *arg
  * read once for the whole batch (or, a short prefix of few sequences, by each).  d_prefix_table: their pages,
  * [ceil(prefix_len / page_len)]; the positions from prefix_len on are read through d_table as ever (whose entries for pages
  * before that are not read).  The result is what ah_kv4_attn_dev gives for tables that name the prefix's pages.  A sequence
- * with tokens before the prefix's end is refused as one out of range.  prefix_len 0: ah_kv4_attn_dev.  d_out may not
+ * with tokens before the prefix's end (of fewer positions than tokens too) is refused as one out of range; one without tokens
+ * may have any context.  prefix_len 0: ah_kv4_attn_dev.  d_out may not
  * overlap d_q; at most 2^30 - 1 values of it.  Uses the context's scratch. */
 int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_attn *args, size_t prefix_len,
                                const int32_t *d_prefix_table, const float *d_q, size_t q_stride, float *d_out,

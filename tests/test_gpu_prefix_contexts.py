@@ -1,4 +1,4 @@
-"""Sequences behind a common prefix whose contexts end before it: on every route that the call may
+"""Sequences behind a common prefix whose contexts end before it, or that have no tokens: on every route that the call may
 take (each sequence for itself, units of 16, 32 and 128 rows of the prefix, 8, 16 and 128 of what follows it)."""
 import numpy as np
 import pytest
@@ -34,3 +34,19 @@ def test_fewer_positions_than_tokens_behind_a_prefix_are_refused(dev, dim, kv, G
             rows = np.arange(B.start[s], B.start[s + 1])
             assert status == CACHE and (out[rows] == 7).all(), (s, value)
             assert np.array_equal(np.delete(out, rows, 0), np.delete(good, rows, 0)), (s, value)
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dim,kv,G,qs,ctx,prefix", ROUTES)
+def test_sequences_without_tokens_behind_a_prefix_are_passed_over(dev, dim, kv, G, qs, ctx, prefix):  # noqa: F811
+    """Idle slots of a batch, whatever their contexts: the call is served as without them."""
+    idle = 0, 2, len(qs) + 2
+    qs, ctx = [0, qs[0], 0, *qs[1:], 0], [prefix, ctx[0], prefix, *ctx[1:], prefix]
+    B = Batch(dev, qs, ctx, kv, G, dim, 64, prefix=prefix, seed=dim)
+    status, want = B.shared()
+    assert status == OK and (want[:, : B.heads * dim] != 7).all()
+    for values, expect in (((0, 0, 0), OK), ((1, prefix - 1, 0), OK), ((0, -1, prefix), CACHE), ((10 ** 6, 0, 0), CACHE)):
+        c = np.array(ctx)
+        c[list(idle)] = values
+        status, out = B.shared(ctx=c)
+        assert status == expect and np.array_equal(out, want), values
