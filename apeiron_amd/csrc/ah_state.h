@@ -51,9 +51,10 @@ __host__ __device__ inline constexpr DeltaBlock delta_block(uint32_t dk, uint32_
     const uint32_t rows = 4 * (dk / 32) * 2048, w = 0, k = w + rows, q = k + rows, p = q + rows, u = p + 6 * 2048, f = u + (dv / 16) * 4096;
     return {w, k, q, p, u, f, f + 1024};
 }
-// Factors, in floats: of o's rows; then W's largest magnitude and inverse scale, each [tile of tokens][slice of 32 channels]; the
-// inverse scales of the keys by slice, of P and of q by tile; U0's largest magnitude by columns; e^(the chunk's decay).
-constexpr uint32_t kFRow = 0, kFWMax = 64, kFW = 80, kFK = 96, kFP = 100, kFQ = 104, kFU = 108, kFDecay = 124;
+// Factors, in floats: of o's rows from S (the inverse scales of q's rows in them); then W's largest magnitude and inverse scale,
+// each [tile of tokens][slice of 32 channels]; the inverse scales of the keys by slice; U0's largest magnitude by columns; e^(the
+// chunk's decay); of o's rows from P (the inverse scales of q's and P's rows in them).
+constexpr uint32_t kFRow = 0, kFWMax = 64, kFW = 80, kFK = 96, kFU = 108, kFDecay = 124, kFP = 128;
 
 hipError_t ah_launch_conv(const ConvArgs &a, hipStream_t stream);
 hipError_t ah_launch_delta(const DeltaArgs &a, bool steps, bool chunks, hipStream_t stream);

@@ -244,7 +244,7 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
 // products of 64 tokens on the matrix cores and a chain 64 times shorter (301 us).  Shorter chunks have a longer chain, longer
 // ones more of the triangle (T by recursion: 64 is four tiles of 16).
 //   f32 by f16: every factor of a product is carried as hi + lo, two f16 of a value scaled by a power of two so that the largest
-// of its group (a tile, a slice, a chunk) lies in [2^13, 2^14): 22 bits, or 2^-38 of the group's largest.  Three products
+// of its group (a row of q, k or P, a tile, a slice, a chunk) lies in [2^13, 2^14): 22 bits, or 2^-38 of the group's largest.  Three products
 // (hi hi, hi lo, lo hi) are summed in the f32 accumulator, at 5 times the rate of the f32 matrix instructions.
 //   Layouts: a lane (r, h) = (lane & 15, lane >> 4) of a 16x16 product holds column r and rows 4 h + i of the result, and of an
 // operand row (or column) r and a quarter of the 32 values that are summed over.  Which those are is free as long as both
@@ -296,12 +296,15 @@ AH_DEV Scale scale_of(float top) {
 template <int CTRL> AH_DEV float dpp(float v) {
     return __builtin_bit_cast(float, __builtin_amdgcn_update_dpp(0, __builtin_bit_cast(int, v), CTRL, 0xF, 0xF, true));
 }
-AH_DEV float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
-AH_DEV float wave_max(float v) {
-    v = __builtin_fmaxf(v, dpp<0x121>(v));  // rotations by 1, 2, 4 and 8 of each 16 lanes
+AH_DEV float max16(float v) {  // over each 16 lanes
+    v = __builtin_fmaxf(v, dpp<0x121>(v));  // rotations by 1, 2, 4 and 8
     v = __builtin_fmaxf(v, dpp<0x122>(v));
     v = __builtin_fmaxf(v, dpp<0x124>(v));
-    v = __builtin_fmaxf(v, dpp<0x128>(v));
+    return __builtin_fmaxf(v, dpp<0x128>(v));
+}
+AH_DEV float lane_of(float v, int lane) { return __builtin_bit_cast(float, __builtin_amdgcn_readlane(__builtin_bit_cast(int, v), lane)); }
+AH_DEV float wave_max(float v) {
+    v = max16(v);
     return __builtin_fmaxf(__builtin_fmaxf(lane_of(v, 0), lane_of(v, 16)), __builtin_fmaxf(lane_of(v, 32), lane_of(v, 48)));
 }
 AH_DEV float top4(float top, f32x4 v) {
@@ -375,7 +378,7 @@ template <int DK> struct PrepareLds {
         u32x4 t[6][2][64];
     };
     double gamma[64];
-    float beta[64], fk[64], fq[64], fw[64], fd[64], red[4], tinv[4];
+    float beta[64], fk[64], fq[64], fw[64], fd[64], tinv[4];  // (fk, fq: the rows' scales undone)
 };
 // Eight waves a chunk and head.  Waves 0 to 3 have the keys and beta_i k_i . k_j of 16 tokens i each, and make T of them; waves 4 to
 // 7 have q of the same tokens, P and q's fragments.  W and U0 are shared by all.  Barriers wait for LDS alone: loads and stores stay
@@ -416,32 +419,36 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
         L.gamma[lane] = gamma;
         L.beta[lane] = beta;
     }
-    float top = 0.0f;
+    // Every row by a scale of its own: its length is no part of what it is to the rule, where it is divided by it (with one scale
+    // for a chunk's 64 keys a key of 2^-20 of the longest kept 18 bits).
+    float up[R::kLoads];
 #pragma unroll
     for (uint32_t i = 0; i < R::kLoads; ++i) {
         const uint32_t t = 16 * w + R::row(i, lane);
         __asm__("" : "+v"(x.x[i]));  // (the loads themselves stay outside the choice)
         x.x[i] = t < c.live ? x.x[i] : (f32x4)0.0f;
-        top = top4(top, x.x[i]);
-        float sum = 0.0f;
+        float sum = 0.0f, top = max16(top4(0.0f, x.x[i]));
 #pragma unroll
         for (int n = 0; n < 4; ++n) sum = __builtin_fmaf(x.x[i][n], x.x[i][n], sum);
         sum = sum16(sum);
-        if (DK == 128) sum += __shfl_xor(sum, 16, 64);
+        if (DK == 128) {
+            sum += __shfl_xor(sum, 16, 64);
+            top = __builtin_fmaxf(top, __shfl_xor(top, 16, 64));
+        }
+        const Scale z = scale_of(top);
+        up[i] = z.up;
         if (R::col(lane) == 0) {
             const float f = keys ? 1.0f : a.scale, v = a.norm_eps >= 0.0f ? f / __builtin_sqrtf(sum + a.norm_eps) : f;
-            (keys ? L.fk : L.fq)[t] = t < c.live ? v : 0.0f;
+            (keys ? L.fk : L.fq)[t] = t < c.live ? v * z.down : 0.0f;
         }
     }
-    top = wave_max(top);
-    if (keys && lane == 0) L.red[w] = top;
-    auto put_rows = [&](float up) {
+    auto put_rows = [&] {
 #pragma unroll
         for (uint32_t i = 0; i < R::kLoads; ++i) {
             const uint32_t t = 16 * w + R::row(i, lane), col = R::col(lane);
             uint32_t hi[2], lo[2];
-            split2(x.x[i][0] * up, x.x[i][1] * up, hi[0], lo[0]);
-            split2(x.x[i][2] * up, x.x[i][3] * up, hi[1], lo[1]);
+            split2(x.x[i][0] * up[i], x.x[i][1] * up[i], hi[0], lo[0]);
+            split2(x.x[i][2] * up[i], x.x[i][3] * up[i], hi[1], lo[1]);
             __builtin_memcpy(&L.kh[t][col], hi, 8);
             __builtin_memcpy(&L.kl[t][col], lo, 8);
         }
@@ -458,9 +465,8 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
     };
     const uint32_t row = 16 * w + r;
     Frag f[NT];  // of the wave's rows
-    const Scale qs = scale_of(top);
     if (!keys) {  // through the keys' place, before they are there
-        put_rows(qs.up);
+        put_rows();
         __builtin_amdgcn_wave_barrier();
 #pragma unroll
         for (int t = 0; t < NT; ++t) {
@@ -472,12 +478,10 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
             };
             store_frag(B.q + (w * NT + t) * 2048, {halves(f[t].hi), halves(f[t].lo)});
         }
-        if (lane == 0) fac[kFQ + w] = qs.down;
     }
     ah_lds_barrier();
-    const Scale ks = scale_of(__builtin_fmaxf(__builtin_fmaxf(L.red[0], L.red[1]), __builtin_fmaxf(L.red[2], L.red[3])));
     const double gr = L.gamma[row], all = L.gamma[63];
-    if (keys) put_rows(ks.up);
+    if (keys) put_rows();
     else if (h == 0) fac[kFRow + row] = L.fq[row] * expf((float)gr);
     if (wave == 4) {  // e^gamma of each token to W's keys, what is left of the chunk's decay to the state's
         const double gamma = L.gamma[lane];
@@ -493,7 +497,7 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
         for (int t = 0; t < NT; ++t) f[t] = row_frag(row, t);
     }
     const uint32_t end = keys ? row : row + 1;
-    const float fr = keys ? L.beta[row] * L.fk[row] * ks.down * ks.down : L.fq[row] * ks.down * qs.down;
+    const float fr = keys ? L.beta[row] * L.fk[row] : 1.0f;  // (q's own length follows with o's rows)
     f32x4 p[4];
 #pragma unroll
     for (uint32_t jt = 0; jt < 4; ++jt) {
@@ -565,8 +569,9 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
         float most = 0.0f;
 #pragma unroll
         for (int t = 0; t < 4; ++t) most = top4(most, p[t]);
-        const Scale s = scale_of(wave_max(most));
-        if (lane == 0) fac[kFP + w] = s.down;
+        most = __builtin_fmaxf(most, __shfl_xor(most, 16, 64));
+        const Scale s = scale_of(__builtin_fmaxf(most, __shfl_xor(most, 32, 64)));  // of the row
+        if (h == 0) fac[kFP + row] = L.fq[row] * s.down;
 #pragma unroll
         for (uint32_t t = 0; t < 2; ++t) {
             if (t == 1 && w < 2) continue;
@@ -636,7 +641,7 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
                 __builtin_memcpy(&lo, &L.kl[j][32 * w + 2 * r], 4);
 #pragma unroll
                 for (int k = 0; k < 2; ++k) {
-                    const float v = ((float)hi[k] + (float)lo[k]) * ks.down;
+                    const float v = (float)hi[k] + (float)lo[k];
                     y[k][t][n] = v;
                     wt = __builtin_fmaxf(wt, __builtin_fabsf(v * fw[t][n]));
                     dt = __builtin_fmaxf(dt, __builtin_fabsf(v * fd[t][n]));
@@ -917,8 +922,7 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
     } else {
         struct Ahead {
             Frag Q[NT], P[2];
-            f32x4 qf;
-            float f;
+            f32x4 qf, pf;
             uint32_t touched;
         } ahead[2];
         auto load_first = [&](uint32_t n, Ahead &x) {
@@ -929,9 +933,9 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
         auto load_second = [&](uint32_t n, Ahead &x) {
             const uint8_t *b = block_of(n);
             __builtin_memcpy(&x.qf, reinterpret_cast<const float *>(b + B.f) + kFRow + 16 * w + 4 * h, 16);
+            __builtin_memcpy(&x.pf, reinterpret_cast<const float *>(b + B.f) + kFP + 16 * w + 4 * h, 16);
 #pragma unroll
             for (uint32_t t = 0; t < 2; ++t) x.P[t] = frag(b + B.p + tri(w, w < 2 ? 0 : t) * 2048);
-            x.f = reinterpret_cast<const float *>(b + B.f)[64 + lane];
         };
         // A line of 128 bytes for each lane, of what all of a head's workgroups read: each takes a part, each wave of it a fourth.
         const uint32_t parts = dv / (16 * NC), lines = B.u / 128, each = (lines + 4 * parts - 1) / (4 * parts);
@@ -943,7 +947,6 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
         };
         auto chunk = [&](uint32_t n, Ahead &x) {
             f32x4 o[NC];
-            const float qinv = lane_of(x.f, kFQ - 64 + w);
 #pragma unroll
             for (int c = 0; c < NC; ++c) o[c] = (f32x4)0.0f;
 #pragma unroll
@@ -951,19 +954,18 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
 #pragma unroll
                 for (int c = 0; c < NC; ++c) {
                     const Frag f = {sf[c][t][0][lane], sf[c][t][1][lane]};
-                    o[c] += mm3(x.Q[t], f, (f32x4)0.0f) * (qinv * sinv[c][t]);
+                    o[c] += mm3(x.Q[t], f, (f32x4)0.0f) * sinv[c][t];
                 }
             }
 #pragma unroll
             for (int c = 0; c < NC; ++c) o[c] *= x.qf;
             load_first(n + 2, x);
             ah_lds_barrier();
-            const float pinv = lane_of(x.f, kFP - 64 + w);
 #pragma unroll
             for (int c = 0; c < NC; ++c) {
                 f32x4 v = mm3(x.P[0], {uf[c][0][0][lane], uf[c][0][1][lane]}, (f32x4)0.0f);
                 if (w >= 2) v = mm3(x.P[1], {uf[c][1][0][lane], uf[c][1][1][lane]}, v);
-                o[c] += v * (pinv * uinv[c]);
+                o[c] += v * (x.pf * uinv[c]);
             }
             load_second(n + 2, x);
             // (range-checked stores: a branch around them would have every later wait for loads wait for them too)

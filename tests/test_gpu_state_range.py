@@ -1,14 +1,17 @@
-"""The recurrent layer's operators over the whole range of their inputs: activations far from zero.
+"""The recurrent layer's operators over the whole range of their inputs: activations far from zero, rows of very different
+lengths in one chunk.
 
 Tolerances (u = 2^-24, f32's rounding):
   SiLU   v / (1 + e^-v): the exponential takes up to 2 u (v_exp_f32's last place) and two roundings, the sum, the quotient's
          product and its Newton step one each: 6 u of the result, and half of f32's smallest number (2^-150), where it is
          below the normal ones.  With a bias of zero and one weight of one the value before it is the input itself.
+  delta  as in tests/test_gpu_state_ops.py: a key's or query's own length is no part of the rule where they are divided by it,
+         and where they are not, outputs and their tolerance are as long as the query.  So it is held by every token.
 """
 import numpy as np
 import pytest
 
-from test_gpu_state_ops import OK, U, conv, dev  # noqa: F401
+from test_gpu_state_ops import OK, Rule, U, close, conv, delta_bound, dev  # noqa: F401
 
 torch = pytest.importorskip("torch")
 
@@ -33,3 +36,26 @@ def test_silu_of_any_finite_value(dev, qs):  # noqa: F811
         ref = v / (1 + np.exp(-v))
     assert status == OK
     assert (np.abs(y - ref) <= 6 * U * np.abs(ref) + 2.0 ** -150).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("K,H,dk,dv", [(2, 4, 128, 128), (1, 2, 64, 256), (3, 3, 128, 64)])
+@pytest.mark.parametrize("qs", [[1, 1, 1], [9, 8, 10], [7, 300, 64], [129, 128, 127]])
+@pytest.mark.parametrize("norm", [True, False])
+def test_delta_rule_of_rows_of_very_different_lengths(dev, K, H, dk, dv, qs, norm):  # noqa: F811
+    R = Rule(qs, K, H, dk, dv, seed=dk + dv + len(qs), kind="plain" if norm else "given", slots=3)
+    rng = np.random.default_rng(sum(qs))
+    n = sum(qs)
+    if norm:
+        R.eps = 1e-30
+        R.k *= np.exp2(rng.integers(-32, 33, (n, K, 1))).astype(np.float32)
+        R.q *= np.exp2(rng.integers(-32, 33, (n, K, 1))).astype(np.float32)
+    else:  # (keys no longer than one)
+        R.k *= np.exp2(rng.integers(-24, 1, (n, K, 1))).astype(np.float32)
+        R.q *= np.exp2(rng.integers(-32, 33, (n, K, 1))).astype(np.float32)
+    status, out, state = R(dev, [0, 1, -1], [0, 1, 2])
+    ref, want, mag = R.reference([0, 1, -1], [0, 1, 2])
+    assert status == OK
+    tol = delta_bound(dk, max(qs))
+    close(out, ref, tol, per=(0, 1), mag=mag)
+    close(state, want, tol, per=(0, 1))
