@@ -33,16 +33,16 @@ AH_DEV Seq seq_of(const StateSeqs &a, uint32_t s) {
 // channels with a library exponential and division: 41 us for 39.)
 AH_DEV float silu(float v) {
     constexpr float kHi = -1.44269502162933349609f, kLo = -1.92596299112661746887e-8f, kLn2 = 0.69314718f;
-    const float w = v < -130.0f ? -130.0f : v;
+    const float m = v < -130.0f ? -130.0f : v, w = __builtin_fminf(m, 130.0f);  // (past 130 the power is 0, and 1 + it 1)
     float t = w * kHi;
     __asm__("" : "+v"(t));  // (t - 64 of the rounded product, which r belongs to: no fused w kHi - 64)
     const float r = __builtin_fmaf(w, kHi, -t) + w * kLo;
     const bool far = t > 100.0f;
     float e = __builtin_amdgcn_exp2f(far ? t - 64.0f : t);
-    e = __builtin_fmaf(e, t > -126.0f ? r * kLn2 : 0.0f, e);
+    e = __builtin_fmaf(e, r * kLn2, e);
     const float d = 1.0f + e, q = __builtin_amdgcn_rcpf(d);
-    float y = w * q;
-    y = __builtin_fmaf(__builtin_fmaf(-d, y, w), q, y);
+    float y = m * q;
+    y = __builtin_fmaf(__builtin_fmaf(-d, y, m), q, y);
     return far ? y * 0x1p-64f : y;
 }
 AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
