@@ -917,7 +917,10 @@ template <int DK, int NC> AH_DEV void chain(const DeltaArgs &a, ChainLds<DK, NC>
 #pragma unroll
                 for (int k = 0; k < 2; ++k)
 #pragma unroll
-                    for (int i = 0; i < 4; ++i) to[(size_t)(2 * i + k) * dv + 16 * c] = S[c][k][i];
+                    for (int i = 0; i < 4; ++i) {
+                        to[(size_t)(2 * i + k) * dv + 16 * c] = S[c][k][i];
+                        odd = odd || (p.nq && !finite(S[c][k][i]));  // (the last chunk's U may be finite and what it adds not)
+                    }
         }
     } else {
         struct Ahead {

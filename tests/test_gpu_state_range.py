@@ -11,7 +11,7 @@ Tolerances (u = 2^-24, f32's rounding):
 import numpy as np
 import pytest
 
-from test_gpu_state_ops import OK, Rule, U, close, conv, delta_bound, dev  # noqa: F401
+from test_gpu_state_ops import NONFINITE, OK, Rule, U, close, conv, delta_bound, dev  # noqa: F401
 
 torch = pytest.importorskip("torch")
 
@@ -59,3 +59,19 @@ def test_delta_rule_of_rows_of_very_different_lengths(dev, K, H, dk, dv, qs, nor
     tol = delta_bound(dk, max(qs))
     close(out, ref, tol, per=(0, 1), mag=mag)
     close(state, want, tol, per=(0, 1))
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("qs,at", [([3], 2), ([8, 1], 7), ([64], 63), ([100, 20], 99), ([130], 10)])
+def test_a_state_that_leaves_f32_is_refused(dev, qs, at):  # noqa: F811
+    """What a token adds, k (beta (v - S^T k))^T, overflows where both factors are finite and no query reads it."""
+    R = Rule(qs, 2, 2, 64, 64, seed=1, kind="given", slots=2)
+    R.q[:] = 0
+    R.a[:], R.b[:] = 0, 1
+    src = list(range(len(qs)))
+    status, _, good = R(dev, src, src)
+    assert status == OK
+    R.k[at, 1, 3], R.v[at, 1, 5] = 16, 1e38
+    status, out, state = R(dev, src, src)
+    assert status == NONFINITE and not np.isfinite(state[0, 1]).all()
+    assert np.array_equal(state[0, 0], good[0, 0]) and np.array_equal(state[1:], good[1:]) and (out[:, 0] == 0).all()
