@@ -46,6 +46,8 @@ AH_DEV float silu(float v) {
     return far ? y * 0x1p-64f : y;
 }
 AH_DEV bool finite(float v) { return __builtin_fabsf(v) < __builtin_inff(); }
+// 1 / sqrt(sum + eps): NaN, not 0, for a sum of squares that left f32, so that the row is refused rather than taken as zeros.
+AH_DEV float inverse_norm(float sum, float eps) { return 1.0f / __builtin_sqrtf(sum + eps) + (sum - sum); }
 
 // ---- the short causal convolution --------------------------------------------------------------------
 //
@@ -197,8 +199,8 @@ template <int DK> AH_DEV void steps(const DeltaArgs &a, uint32_t unit) {  // a w
                 kk = __builtin_fmaf(k[i], k[i], kk);
                 qq = __builtin_fmaf(q[i], q[i], qq);
             }
-            fk = 1.0f / __builtin_sqrtf(sum_rows(kk) + a.norm_eps);
-            fq *= 1.0f / __builtin_sqrtf(sum_rows(qq) + a.norm_eps);
+            fk = inverse_norm(sum_rows(kk), a.norm_eps);
+            fq *= inverse_norm(sum_rows(qq), a.norm_eps);
         }
         f32x4 m = (f32x4)0.0f, o = (f32x4)0.0f;
 #pragma unroll
@@ -438,7 +440,7 @@ template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32
         const Scale z = scale_of(top);
         up[i] = z.up;
         if (R::col(lane) == 0) {
-            const float f = keys ? 1.0f : a.scale, v = a.norm_eps >= 0.0f ? f / __builtin_sqrtf(sum + a.norm_eps) : f;
+            const float f = keys ? 1.0f : a.scale, v = a.norm_eps >= 0.0f ? f * inverse_norm(sum, a.norm_eps) : f;
             (keys ? L.fk : L.fq)[t] = t < c.live ? v * z.down : 0.0f;
         }
     }

@@ -534,7 +534,8 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *args,
  *   S = e^g S;  S += k (beta (v - S^T k))^T;  out = scale S^T q.
  * Head h takes q and k of head h / (n_heads / n_k_heads).  With d_a_log, g = -e^a_log log(1 + e^(a + dt_bias)) and
  * beta = 1 / (1 + e^-b); without (NULL), a is g and b is beta.  norm_eps >= 0: q and k are divided by
- * sqrt(their sum of squares + norm_eps) first; negative: taken as they are.  k_dim 64 or 128, v_dim 64, 128 or 256.  d_q,
+ * sqrt(their sum of squares + norm_eps) first (a sum that is not finite in f32 is refused as a result that is not);
+ * negative: taken as they are.  k_dim 64 or 128, v_dim 64, 128 or 256.  d_q,
  * d_k: [n_tok] rows of n_k_heads heads, d_v, d_out: of n_heads, d_a, d_b: one value a head.  Uses the context's scratch
  * (as ah_gemm_f32_dev, also for calls captured into a graph): 768 k_dim + 256 v_dim + 13 KB for every 64 tokens and head
  * and for every sequence and head, less where few sequences are long. */

@@ -75,3 +75,27 @@ def test_a_state_that_leaves_f32_is_refused(dev, qs, at):  # noqa: F811
     status, out, state = R(dev, src, src)
     assert status == NONFINITE and not np.isfinite(state[0, 1]).all()
     assert np.array_equal(state[0, 0], good[0, 0]) and np.array_equal(state[1:], good[1:]) and (out[:, 0] == 0).all()
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("name", ["q", "k"])
+@pytest.mark.parametrize("qs,at", [([3, 2], 1), ([64, 3], 40), ([130, 70], 70)])
+def test_rows_whose_squares_leave_f32_are_refused(dev, name, qs, at):  # noqa: F811
+    """A row that is divided by its length, the sum of whose squares is not finite in f32: no row of zeros in its place."""
+    R = Rule(qs, 2, 2, 64, 64, seed=2, slots=2)
+    status, good, kept = R(dev, [0, 1], [0, 1])
+    assert status == OK
+    x = getattr(R, name).copy()
+    for value, expect in ((1e18, OK), (3e19, NONFINITE), (-3e38, NONFINITE)):
+        getattr(R, name)[at, 1] = value
+        status, out, state = R(dev, [0, 1], [0, 1])
+        assert status == expect, value
+        same = np.ones(out.shape, bool)
+        same[at // 64 * 64:qs[0], 1] = False
+        assert np.array_equal(out[same], good[same]) and np.array_equal(state[1], kept[1]) and np.array_equal(state[0, 0], kept[0, 0])
+        if expect == OK:
+            ref, want, mag = R.reference([0, 1], [0, 1])
+            close(out, ref, delta_bound(64, max(qs)), per=(1,), mag=mag)
+            close(state, want, delta_bound(64, max(qs)), per=(0, 1))
+    getattr(R, name)[:] = x
+    assert R(dev, [0, 1], [0, 1])[0] == OK
