@@ -248,6 +248,9 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
 //   f32 by f16: every factor of a product is carried as hi + lo, two f16 of a value scaled by a power of two so that the largest
 // of its group (a row of q, k or P, a tile, a slice, a chunk) lies in [2^13, 2^14): 22 bits, or 2^-38 of the group's largest.  Three products
 // (hi hi, hi lo, lo hi) are summed in the f32 accumulator, at 5 times the rate of the f32 matrix instructions.
+//   Tokens that are summed over share a scale (beta v: 64 of them, 16 columns; U: the same, by a bound of up to 32 dk / 32 times the
+// largest |S| above it), so that U is held to 2^-31 of the largest |S| and 2^-37 of the largest |beta v|, and not to 22 bits of
+// itself where a decay clears a far larger state within the chunk.
 //   Layouts: a lane (r, h) = (lane & 15, lane >> 4) of a 16x16 product holds column r and rows 4 h + i of the result, and of an
 // operand row (or column) r and a quarter of the 32 values that are summed over.  Which those are is free as long as both
 // operands agree: rows 4 h + i of two neighbouring tiles.  So a result is the next product's operand where it lies.  Row m of the

@@ -536,9 +536,13 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *args,
  * beta = 1 / (1 + e^-b); without (NULL), a is g and b is beta.  norm_eps >= 0: q and k are divided by
  * sqrt(their sum of squares + norm_eps) first (a sum that is not finite in f32 is refused as a result that is not);
  * negative: taken as they are.  k_dim 64 or 128, v_dim 64, 128 or 256.  d_q,
- * d_k: [n_tok] rows of n_k_heads heads, d_v, d_out: of n_heads, d_a, d_b: one value a head.  Uses the context's scratch
- * (as ah_gemm_f32_dev, also for calls captured into a graph): 768 k_dim + 256 v_dim + 13 KB for every 64 tokens and head
- * and for every sequence and head, less where few sequences are long. */
+ * d_k: [n_tok] rows of n_k_heads heads, d_v, d_out: of n_heads, d_a, d_b: one value a head.
+ * Up to 8 tokens of a sequence (16 or 24 in large batches) go one by one, in f32; more go by chunks of 64, where what a token
+ * adds, beta (v - S^T k), is held to about 2^-31 of the largest |S| and 2^-37 of the largest |beta v| of its chunk and 16
+ * columns of S: as f32 where it is no less than 2^-7 of that |S|, and not to its own last place where a decay within the chunk
+ * clears a far larger state.
+ * Uses the context's scratch (as ah_gemm_f32_dev, also for calls captured into a graph): 768 k_dim + 256 v_dim + 13 KB for
+ * every 64 tokens and head and for every sequence and head, less where few sequences are long. */
 typedef struct ah_delta_rule {
     size_t n_heads, n_k_heads, k_dim, v_dim;
     const float *d_a_log, *d_dt_bias; /* [n_heads], both or neither */

@@ -7,6 +7,9 @@ Tolerances (u = 2^-24, f32's rounding):
          below the normal ones.  With a bias of zero and one weight of one the value before it is the input itself.
   delta  as in tests/test_gpu_state_ops.py: a key's or query's own length is no part of the rule where they are divided by it,
          and where they are not, outputs and their tolerance are as long as the query.  So it is held by every token.
+         By chunks a token's part of the state, u = beta (v - S^T k), is held to 2^-31 of the largest |S| and 2^-37 of the
+         largest |beta v| of its chunk: an output of keys and queries of length one is off by at most scale times that for
+         each of up to 64 tokens since a decay that cleared the state, a state's element by that for each.
 """
 import numpy as np
 import pytest
@@ -99,3 +102,22 @@ def test_rows_whose_squares_leave_f32_are_refused(dev, name, qs, at):  # noqa: F
             close(state, want, delta_bound(64, max(qs)), per=(0, 1))
     getattr(R, name)[:] = x
     assert R(dev, [0, 1], [0, 1])[0] == OK
+
+
+@pytest.mark.gpu
+@pytest.mark.parametrize("dk,dv", [(128, 128), (64, 64)])
+@pytest.mark.parametrize("at", [5, 16, 40])
+@pytest.mark.parametrize("shrink", [10, 24])
+def test_small_values_behind_a_decay_that_clears_a_large_state(dev, dk, dv, at, shrink):  # noqa: F811
+    R = Rule([64], 2, 2, dk, dv, seed=at + shrink, kind="given", slots=1)
+    R.eps = 1e-6
+    R.a[at] = -np.inf
+    R.v[at:] *= np.float32(2.0 ** -shrink)
+    status, out, state = R(dev, [0], [0])
+    ref, want, mag = R.reference([0], [0])
+    assert status == OK
+    tol, top = delta_bound(dk, 64), 2.0 ** -31 * np.abs(R.state).max() + 2.0 ** -37 * np.abs(R.v).max()
+    close(out[:at], ref[:at], tol, per=(1,), mag=mag[:at])
+    size = lambda x, axis: np.sqrt((x * x).mean(axis, keepdims=True))  # noqa: E731
+    assert (np.abs(out - ref)[at:] <= 64 * tol * size(mag[at:], 2) + 64 * R.scale * top).all()
+    assert (np.abs(state - want) <= 64 * tol * size(want, (2, 3)) + 64 * top).all()
