@@ -537,20 +537,37 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     b.first = (uint32_t)blocks->n_first;
     b.last = (uint32_t)blocks->n_last;
     b.chosen = d_chosen;
-    // Lists, then scores that do not fit a workgroup's LDS, then the attention's partial results.
-    const size_t places = a.table_stride * per_page, all = places < kMaxU32 / 32 ? places : kMaxU32 / 32, read = b.top + (size_t)b.first + b.last + 1, entries = read < all ? read : all;
+    // Lists, then the attention's partial results.  `room`: blocks that a table has pages for; `planned`: of the largest context
+    // expected, which the choice's LDS and the attention's pieces go by (a table is as wide as the longest context allowed).
+    const size_t places = a.table_stride * per_page, room = places < kMaxU32 / 32 ? places : kMaxU32 / 32;
+    const size_t expected = p->max_ctx / blocks->block_len + (p->max_ctx % blocks->block_len != 0), planned = expected < room ? expected : room;
+    const size_t read = b.top + (size_t)b.first + b.last + 1, entries = read < room ? read : room;
     a.list_stride = (uint32_t)entries + 1;
     a.block_shift = b.shift - 5;
-    b.most = (uint32_t)all;
-    b.lds_keys = (uint32_t)(all < kLdsKeys ? all : kLdsKeys);
-    // Where 16 tokens' scores fit LDS, 16 tokens of a sequence are chosen for together once every CU has two (token, KV
-    // head)s (four with heads of 256, whose workgroups are smaller).  2 KV heads, 8192 keys, us a token for itself and together:
-    // heads of 128, 128 tokens of a sequence 35 and 42, 256 51 and 51, 512 88 and 62, 64 x 4 55 and 50; of 256, 256 tokens 71
-    // and 81, 512 124 and 97.  (Tiles of one or two tokens: 512 x 1 104 and 112, 128 x 2 56 and 62.)
-    const bool together = a.max_q >= 4 && units >= (a.c.dim == 256 ? 4 : 2) * (size_t)ctx->cu_count && 16 * (a.c.dim + 2 + all + 1) <= kLdsKeys;
+    // Scores of a query's blocks in LDS (8 bytes), all of a context of the planned length; those of a longer one, or past what LDS
+    // holds, go by passes behind the largest so far with their numbers (4 bytes).  `rows` queries; `more`: 8 bytes beside each.
+    struct Fit {
+        size_t keys, bytes;
+    };
+    auto fit = [&](size_t rows, size_t more) {
+        const size_t least = b.top + (size_t)256 < room ? b.top + (size_t)256 : room;  // (a pass is 256 blocks and more)
+        const size_t held = kChoiceLds / (8 * rows) - more, passes = held > b.top / 2 + 1 ? held - (b.top / 2 + 1) : 0;
+        const size_t want = planned > least ? planned : least, keys = want <= held && want == room ? want : want < passes ? want : passes;
+        return Fit{keys, rows * (keys + more) * 8 + (keys < room ? rows * b.top * 4 : 0)};
+    };
+    // 16 tokens of a sequence are chosen for together once every CU has two (token, KV head)s (four with heads of 256, whose
+    // workgroups are smaller).  2 KV heads, 8192 keys, us a token for itself and together: heads of 128, 128 tokens of a sequence
+    // 35 and 42, 256 51 and 51, 512 88 and 62, 64 x 4 55 and 50; of 256, 256 tokens 71 and 81, 512 124 and 97.  (Tiles of one or two
+    // tokens: 512 x 1 104 and 112, 128 x 2 56 and 62.)  By passes too, where 16 tokens' scores outgrow LDS and one's don't: blocks
+    // of 64, heads of 128, 2048 tokens over 70000, 100000 and 200000 keys 280 and 147, 321 and 158, 477 and 205, 512 over 100000 108 and
+    // 93; of 256, 2048 over 100000 552 and 274; 400 blocks of 100000 2242 and 2107, 550 the same; past that a pass is too short.
+    const Fit one = fit(1, 0), many = fit(16, a.c.dim + 3);
+    const bool together = a.max_q >= 4 && units >= (a.c.dim == 256 ? 4 : 2) * (size_t)ctx->cu_count && (many.keys == room || many.keys >= b.top + (size_t)128);
+    b.lds_keys = (uint32_t)(together ? many : one).keys;
+    b.lds_bytes = (uint32_t)(together ? many : one).bytes;
     b.tiles = together ? a.n_tok / 16 + a.n_seq : 0;
     if ((size_t)b.tiles * a.c.n_kv > max_grid(1024) || (!together && units > max_grid(1024))) return AH_ERR_INVALID_ARG;
-    const size_t keys_at = align256(units * a.list_stride * sizeof(uint32_t)), kept = keys_at + (all > kLdsKeys ? align256(units * all * sizeof(uint64_t)) : 0);
+    const size_t kept = align256(units * a.list_stride * sizeof(uint32_t));
     // Up to eight queries a KV head, and lists enough for four waves a CU and more: a wave each.  (us with a wave each and in
     // pieces, 2 KV heads, lists of 1152 keys: heads of 64, 512 lists 46 and 39, 1024 49 and 52; of 128 61 and 53, 63 and 74; of
     // 256 94 and 83, 98 and 119.)
@@ -563,11 +580,10 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
         st = ensure_scratch(ctx, kept, stream);
     } else {
         rows.n_seq = a.n_tok;  // every token for itself
-        st = attn_rows_plan(ctx, rows, entries << a.block_shift, a.group, kept, stream);
+        st = attn_rows_plan(ctx, rows, (planned < entries ? planned : entries) << a.block_shift, a.group, kept, stream);
     }
     if (st) return st;
     b.list = static_cast<uint32_t *>(ctx->scratch.p);
-    b.keys = reinterpret_cast<uint64_t *>(static_cast<uint8_t *>(ctx->scratch.p) + keys_at);
     rows.list = b.list;
     AH_HIP(ctx, ah_launch_block_choice(b, pick(ctx, stream)));
     if (alone) AH_HIP(ctx, ah_launch_attend_lists(rows, pick(ctx, stream)));

@@ -237,12 +237,28 @@ template <class K, class E, class M> AH_DEV void many_keys(uint32_t n, uint32_t 
 // The choice for a (token, KV head) by a workgroup of W waves, into `list` (as attention's, kNoList where the token is no
 // sequence's).  Scores: D / 8 lanes a block, eight channels each, the means of several blocks a lane on their way (a load touches
 // few lines; with a lane for a whole mean it touches 64).  16 waves: all blocks of 32768 keys are on their way at once.
-template <int W> struct ChoiceLds {
+//   Where a context has more blocks than LDS has room for scores (it is longer than planned, or the longest of all), they go by
+// passes: after one, the `top` largest stand in front, in the order of their blocks, with their numbers, and the next pass's behind
+// them; of equal scores the first is still the first.
+struct Passes {
+    uint64_t *keys;    // [what LDS holds]
+    uint32_t *number;  // [top]: of what is kept
+    uint32_t top;
+    // (blocks are counted from the first that is chosen among)
+    AH_DEV uint32_t block_of(uint32_t i, uint32_t kept, uint32_t done) const { return i < kept ? number[i] : done + (i - kept); }
+    AH_DEV void keep(uint32_t at, uint32_t i, uint32_t block) const {  // (at <= i: nothing is overwritten that is still to be read)
+        const uint64_t key = keys[i];
+        keys[at] = key;
+        number[at] = block;
+    }
+};
+template <int D, int W> struct ChoiceLds {
+    double q[D];
     uint64_t room[128];
     uint32_t cnt[2][W], done;
 };
-template <int D, int W> AH_DEV void choose(const BlockArgs &b, uint32_t unit, uint32_t *list, uint64_t *lds_keys, ChoiceLds<W> &L) {
-    constexpr uint32_t kLanes = D / 8, kPer = 64 / kLanes, kAhead = W >= 16 ? 4 : 8;  // lanes of a block's mean, blocks of a wave
+template <int D, int W> AH_DEV void choose(const BlockArgs &b, uint32_t unit, uint32_t *list, uint64_t *lds_keys, ChoiceLds<D, W> &L) {
+    constexpr uint32_t kLanes = D / 8, kPer = 64 / kLanes, kAhead = W >= 16 ? D == 256 ? 3 : 4 : 8;  // lanes of a block's mean, blocks of a wave
     const AttnArgs &a = b.a;
     const uint32_t tok = unit / a.c.n_kv, kvh = unit - tok * a.c.n_kv, tid = threadIdx.x, lane = tid & 63;
     const uint32_t wave = __builtin_amdgcn_readfirstlane(tid >> 6), g = lane % kLanes;
@@ -265,7 +281,7 @@ template <int D, int W> AH_DEV void choose(const BlockArgs &b, uint32_t unit, ui
         const Span p = span_of(a, i);
         return tok >= p.q0 && tok - p.q0 < p.nq;
     };
-    const uint32_t s = sequence_of(a, tok, start, holds);
+    const uint32_t s = __builtin_amdgcn_readfirstlane(sequence_of(a, tok, start, holds));
     const Span p = span_of(a, s);
     int32_t *chosen = b.chosen ? b.chosen + (size_t)unit * b.top : nullptr;
     if (tok < p.q0 || tok - p.q0 >= p.nq) {
@@ -275,28 +291,17 @@ template <int D, int W> AH_DEV void choose(const BlockArgs &b, uint32_t unit, ui
     }
     const Query x = query_of(b, p, s, tok);
     const uint32_t n = x.n;
-    const bool in_lds = n <= b.lds_keys;
-    uint64_t *far = b.keys + (size_t)unit * b.most;
-    auto key_at = [&](uint32_t i) { return in_lds ? lds_keys[i] : far[i]; };
-    auto emit = [&](uint32_t at, uint32_t i) {
-        list[1 + b.first + at] = entry_of(b, s, kvh, b.first + i);
-        if (chosen) chosen[at] = (int32_t)(b.first + i);
-    };
-    if (n > b.top) {
+    auto score = [&](uint32_t from, uint32_t num, uint64_t *keys) {  // of the blocks from .. from + num - 1
         const uint32_t first = wave * kPer + lane / kLanes, step = W * kPer;
-        for (uint32_t base = 0; base < n; base += step * kAhead) {
+        for (uint32_t base = 0; base < num; base += step * kAhead) {
             f16x8 m[kAhead];
             uint32_t page[kAhead];
+            auto block_at = [&](uint32_t i) { return b.first + from + (i < num ? i : num - 1); };
 #pragma unroll
-            for (uint32_t j = 0; j < kAhead; ++j) {
-                const uint32_t i = base + j * step + first;
-                page[j] = page_of(b, s, b.first + (i < n ? i : n - 1));
-            }
+            for (uint32_t j = 0; j < kAhead; ++j) page[j] = page_of(b, s, block_at(base + j * step + first));
 #pragma unroll
-            for (uint32_t j = 0; j < kAhead; ++j) {
-                const uint32_t i = base + j * step + first;
-                __builtin_memcpy(&m[j], b.means + mean_at(b, page[j] < a.c.n_pages ? page[j] : 0, kvh, b.first + (i < n ? i : n - 1)) * D + 8 * g, 16);
-            }
+            for (uint32_t j = 0; j < kAhead; ++j)
+                __builtin_memcpy(&m[j], b.means + mean_at(b, page[j] < a.c.n_pages ? page[j] : 0, kvh, block_at(base + j * step + first)) * D + 8 * g, 16);
 #pragma unroll
             for (uint32_t j = 0; j < kAhead; ++j) {
                 const uint32_t i = base + j * step + first;
@@ -309,44 +314,80 @@ template <int D, int W> AH_DEV void choose(const BlockArgs &b, uint32_t unit, ui
                 if (kLanes >= 16) v += dpp64<0x140>(v);  // of sixteen
                 if (kLanes == 32) v += __shfl_xor(v, 16, 64);
                 const uint64_t key = page[j] < a.c.n_pages ? rank_of(v) : 0;
-                if (i < n && g == 0) {
-                    if (in_lds) lds_keys[i] = key;
-                    else far[i] = key;
-                }
+                if (i < num && g == 0) keys[i] = key;
             }
         }
-        __syncthreads();
-        if (wave == 0) {
-            const bool all = few_keys(n, b.top, L.room, key_at, emit);
-            if (lane == 0) L.done = all;
-        }
-    }
-    if (wave == 1) {
+    };
+    auto fixed = [&] {
         (void)list_fixed(b, x, kvh, list, chosen, lane, 64);
         if (lane == 0) record_bad(b, unit, gridDim.x);
-    }
-    if (n <= b.top) return;
-    __syncthreads();
-    if (L.done) return;
-    uint32_t turn = 0;
-    auto many = [&](uint64_t at_least) {
-        uint32_t c = 0;
-        for (uint32_t base = 64 * wave; base < n; base += 64 * W) c += count(base + lane < n && key_at(base + lane) >= at_least);
-        if (lane == 0) L.cnt[turn][wave] = c;
-        __syncthreads();
-        c = 0;
-#pragma unroll
-        for (uint32_t w = 0; w < W; ++w) c += L.cnt[turn][w];
-        turn ^= 1;
-        return c;
     };
-    many_keys(n, b.top, key_at, [&](uint32_t at, uint32_t i) {
-        if (wave == 0) emit(at, i);
-    }, many);
+    auto key_at = [&](uint32_t i) { return lds_keys[i]; };
+    auto choice = [&](uint32_t num, auto emit, bool begin) {  // among the keys in LDS
+        __syncthreads();
+        if (wave == 0) {
+            const bool all = few_keys(num, b.top, L.room, key_at, emit);
+            if (lane == 0) L.done = all;
+        }
+        if (begin && wave == 1) fixed();
+        __syncthreads();
+        if (L.done) return;
+        uint32_t turn = 0;
+        auto many = [&](uint64_t at_least) {
+            uint32_t c = 0;
+            for (uint32_t base = 64 * wave; base < num; base += 64 * W) c += count(base + lane < num && key_at(base + lane) >= at_least);
+            if (lane == 0) L.cnt[turn][wave] = c;
+            __syncthreads();
+            c = 0;
+#pragma unroll
+            for (uint32_t w = 0; w < W; ++w) c += L.cnt[turn][w];
+            turn ^= 1;
+            return c;
+        };
+        many_keys(num, b.top, key_at, [&](uint32_t at, uint32_t i) {
+            if (wave == 0) emit(at, i);
+        }, many);
+    };
+    auto put = [&](uint32_t at, uint32_t block) {
+        list[1 + b.first + at] = entry_of(b, s, kvh, b.first + block);
+        if (chosen) chosen[at] = (int32_t)(b.first + block);
+    };
+    if (n <= b.top) {
+        if (wave == 1) fixed();
+        return;
+    }
+    if (__builtin_expect(n <= b.lds_keys, true)) {
+        score(0, n, lds_keys);
+        choice(n, put, true);
+        return;
+    }
+    // Blocks done .. done + now - 1, behind the `kept` largest of those before them.
+    if (wave == 0 && lane < kLanes) {  // (for every pass, rather than in registers through the choice)
+#pragma unroll
+        for (int i = 0; i < 8; ++i) L.q[8 * g + i] = q[i];
+    }
+    const Passes P = {lds_keys, reinterpret_cast<uint32_t *>(lds_keys + b.lds_keys), b.top};
+    uint32_t done = 0, kept = 0;
+    for (;;) {
+        const uint32_t now = n - done < b.lds_keys - kept ? n - done : b.lds_keys - kept;
+        const bool last = done + now == n;
+        __syncthreads();
+#pragma unroll
+        for (int i = 0; i < 8; ++i) q[i] = L.q[8 * g + i];
+        score(done, now, lds_keys + kept);
+        choice(kept + now, [&](uint32_t at, uint32_t i) {
+            const uint32_t block = P.block_of(i, kept, done);
+            if (last) put(at, block);
+            else P.keep(at, i, block);
+        }, done == 0);
+        if (last) return;
+        done += now;
+        kept = b.top;
+    }
 }
-template <int D> __global__ void __launch_bounds__(1024) block_choice_kernel(BlockArgs b) {
+template <int D> __global__ void __launch_bounds__(1024, 8) block_choice_kernel(BlockArgs b) {
     extern __shared__ uint64_t lds_keys[];  // [b.lds_keys]
-    __shared__ ChoiceLds<16> L;
+    __shared__ ChoiceLds<D, 16> L;
     choose<D, 16>(b, blockIdx.x, b.list + (size_t)blockIdx.x * b.a.list_stride, lds_keys, L);
 }
 
@@ -376,7 +417,8 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves<D>) block_cho
     const uint32_t tile = at - start(s);
     if (tile >= (p.nq + 15) / 16) return;
     const uint32_t tok0 = p.q0 + 16 * tile, live = p.nq - 16 * tile < 16 ? p.nq - 16 * tile : 16;
-    const uint32_t most = query_of(b, p, s, tok0 + live - 1).n;  // (the last token's: the most)
+    const uint32_t most = query_of(b, p, s, tok0 + live - 1).n;  // (the last token's: the most; no other has two fewer)
+    uint32_t *numbers = reinterpret_cast<uint32_t *>(keys + 16 * stride);  // [16][top]
     if (most > b.top) {
         for (uint32_t i = threadIdx.x; i < 16 * D; i += 64 * kSomeWaves<D>) {
             const uint32_t t = i / D, c = i % D;
@@ -387,43 +429,62 @@ template <int D> __global__ void __launch_bounds__(64 * kSomeWaves<D>) block_cho
             qs[t * (D + 2) + c] = v * (double)a.scale;
         }
         __syncthreads();
-        double q[Q];
-#pragma unroll
-        for (int i = 0; i < Q; ++i) q[i] = qs[r * (D + 2) + h * Q + i];
-        for (uint32_t base = 16 * wave; base < most; base += 16 * kSomeWaves<D>) {
-            const uint32_t i = base + r, block = b.first + (i < most ? i : most - 1), page = page_of(b, s, block);
-            const bool ok = page < a.c.n_pages;
-            _Float16 m[Q];
-            __builtin_memcpy(m, b.means + mean_at(b, ok ? page : 0, kvh, block) * D + h * Q, 2 * Q);
-            f64x4 v = {0.0, 0.0, 0.0, 0.0};
-#pragma unroll
-            for (int c = 0; c < Q; ++c) v = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)m[c], q[c], v, 0, 0, 0);
-            const uint32_t good = (uint32_t)__builtin_amdgcn_ballot_w64(ok);  // of the blocks: lanes 0 to 15
-#pragma unroll
-            for (int n = 0; n < 4; ++n) {
-                const uint32_t j = h + 4 * n;
-                if (base + j < most) keys[r * stride + base + j] = good >> j & 1 ? rank_of(v[n]) : 0;
-            }
-        }
-        __syncthreads();
     }
-    for (uint32_t t = wave; t < live; t += kSomeWaves<D>) {
-        const uint32_t tok = tok0 + t, unit = tok * a.c.n_kv + kvh;
-        const Query x = query_of(b, p, s, tok);
-        uint32_t *list = b.list + (size_t)unit * a.list_stride;
-        int32_t *chosen = b.chosen ? b.chosen + (size_t)unit * b.top : nullptr;
-        if (list_fixed(b, x, kvh, list, chosen, lane, 64)) continue;
-        auto key_at = [&](uint32_t i) { return keys[t * stride + i]; };
-        auto emit = [&](uint32_t to, uint32_t i) {
-            list[1 + b.first + to] = entry_of(b, s, kvh, b.first + i);
-            if (chosen) chosen[to] = (int32_t)(b.first + i);
-        };
-        if (few_keys(x.n, b.top, room[wave], key_at, emit)) continue;
-        many_keys(x.n, b.top, key_at, emit, [&](uint64_t at_least) {
-            uint32_t c = 0;
-            for (uint32_t i = lane; i < (x.n + 63) / 64 * 64; i += 64) c += count(i < x.n && key_at(i) >= at_least);
-            return c;
-        });
+    // Blocks done .. done + now - 1, behind the `kept` largest of those before them (Passes).
+    uint32_t done = 0, kept = 0;
+    for (;;) {
+        const uint32_t now = most <= b.top ? most : most - done < b.lds_keys - kept ? most - done : b.lds_keys - kept;
+        const bool last = done + now == most;
+        if (most > b.top) {
+            double q[Q];
+#pragma unroll
+            for (int i = 0; i < Q; ++i) q[i] = qs[r * (D + 2) + h * Q + i];
+            for (uint32_t base = 16 * wave; base < now; base += 16 * kSomeWaves<D>) {
+                const uint32_t i = base + r, block = b.first + done + (i < now ? i : now - 1), page = page_of(b, s, block);
+                const bool ok = page < a.c.n_pages;
+                _Float16 m[Q];
+                __builtin_memcpy(m, b.means + mean_at(b, ok ? page : 0, kvh, block) * D + h * Q, 2 * Q);
+                f64x4 v = {0.0, 0.0, 0.0, 0.0};
+#pragma unroll
+                for (int c = 0; c < Q; ++c) v = __builtin_amdgcn_mfma_f64_16x16x4f64((double)(float)m[c], q[c], v, 0, 0, 0);
+                const uint32_t good = (uint32_t)__builtin_amdgcn_ballot_w64(ok);  // of the blocks: lanes 0 to 15
+#pragma unroll
+                for (int n = 0; n < 4; ++n) {
+                    const uint32_t j = h + 4 * n;
+                    if (base + j < now) keys[r * stride + kept + base + j] = good >> j & 1 ? rank_of(v[n]) : 0;
+                }
+            }
+            __syncthreads();
+        }
+        for (uint32_t t = wave; t < live; t += kSomeWaves<D>) {
+            const uint32_t tok = tok0 + t, unit = tok * a.c.n_kv + kvh;
+            const Query x = query_of(b, p, s, tok);
+            uint32_t *list = b.list + (size_t)unit * a.list_stride;
+            int32_t *chosen = b.chosen ? b.chosen + (size_t)unit * b.top : nullptr;
+            if (done ? x.n <= b.top : list_fixed(b, x, kvh, list, chosen, lane, 64)) continue;
+            const Passes P = {keys + t * stride, numbers + t * b.top, b.top};
+            const uint32_t n = kept + (x.n - done < now ? x.n - done : now);
+            auto key_at = [&](uint32_t i) { return P.keys[i]; };
+            auto emit = [&](uint32_t to, uint32_t i) {
+                const uint32_t block = P.block_of(i, kept, done);
+                if (last) {
+                    list[1 + b.first + to] = entry_of(b, s, kvh, b.first + block);
+                    if (chosen) chosen[to] = (int32_t)(b.first + block);
+                } else {
+                    P.keep(to, i, block);
+                }
+            };
+            if (few_keys(n, b.top, room[wave], key_at, emit)) continue;
+            many_keys(n, b.top, key_at, emit, [&](uint64_t at_least) {
+                uint32_t c = 0;
+                for (uint32_t i = lane; i < (n + 63) / 64 * 64; i += 64) c += count(i < n && key_at(i) >= at_least);
+                return c;
+            });
+        }
+        if (last) return;
+        done += now;
+        kept = b.top;
+        __syncthreads();
     }
 }
 
@@ -596,10 +657,10 @@ hipError_t ah_launch_block_means(const MeansArgs &a, hipStream_t stream) {
 
 template <int D> void launch_choice(const BlockArgs &a, hipStream_t stream) {
     if (!a.tiles) {
-        hipLaunchKernelGGL(block_choice_kernel<D>, dim3(a.a.n_tok * a.a.c.n_kv), dim3(1024), a.lds_keys * sizeof(uint64_t), stream, a);
+        hipLaunchKernelGGL(block_choice_kernel<D>, dim3(a.a.n_tok * a.a.c.n_kv), dim3(1024), a.lds_bytes, stream, a);
         return;
     }
-    hipLaunchKernelGGL(block_choices_kernel<D>, dim3(a.tiles * a.a.c.n_kv), dim3(64 * kSomeWaves<D>), 16 * (D + 2 + a.lds_keys + 1) * sizeof(uint64_t), stream, a);
+    hipLaunchKernelGGL(block_choices_kernel<D>, dim3(a.tiles * a.a.c.n_kv), dim3(64 * kSomeWaves<D>), a.lds_bytes, stream, a);
 }
 
 hipError_t ah_launch_block_choice(const BlockArgs &a, hipStream_t stream) {
@@ -618,7 +679,7 @@ hipError_t ah_launch_attend_lists(const AttnArgs &a, hipStream_t stream) {
 }
 
 hipError_t ah_blocks_init_attrs() {
-    const int most = (int)(kLdsKeys * sizeof(uint64_t));
+    const int most = (int)kChoiceLds;
     hipError_t e = hipSuccess;
     for (const void *k : {(const void *)block_choice_kernel<64>, (const void *)block_choice_kernel<128>, (const void *)block_choice_kernel<256>,
                           (const void *)block_choices_kernel<64>, (const void *)block_choices_kernel<128>, (const void *)block_choices_kernel<256>})

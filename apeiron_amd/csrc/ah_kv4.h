@@ -142,7 +142,7 @@ struct AttnArgs {
     uint32_t seqs;  // where tokens of no sequence have no list: the sequences to look a token up among (n_seq: the tokens)
 };
 constexpr uint32_t kNoList = 0xffffffffu;
-constexpr uint32_t kLdsKeys = 16384;  // scores of a query's blocks that the choice keeps in LDS, at most
+constexpr uint32_t kChoiceLds = 144 * 1024;  // bytes of LDS in which the choice keeps scores, at most
 
 // The choice of blocks (ah_blocks.hip): a's sequences, tokens, queries, table and scale.
 struct BlockArgs {
@@ -151,8 +151,7 @@ struct BlockArgs {
     uint32_t shift, top, first, last;  // positions of a block: 1 << shift
     uint32_t *list;
     int32_t *chosen;
-    uint64_t *keys;  // [token, KV head][most]: the scores' ranks, where they do not fit LDS
-    uint32_t most, lds_keys;
+    uint32_t lds_keys, lds_bytes;  // scores of a query that LDS holds (more than `top`, or all that there can be), and its size
     uint32_t tiles;  // numbers of groups of 16 tokens of a sequence, chosen for together; 0: every token by itself
 };
 struct MeansArgs {
