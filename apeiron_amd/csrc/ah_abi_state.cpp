@@ -102,10 +102,13 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
         // A workgroup of the chain takes 16 columns of S; 32 or 64 where there are more of them than CUs and then than fill six
         // rounds: a chunk's block is read by fewer workgroups.  (16 heads of 128 x 128, us with 16, 32, 64: 1 x 64 tokens 25,
         // 25, 30; 2 x 301 35, 39, 52; 5 x 301 66, 62, 63; 4 x 2048 274, 205, 336; 8 x 1024 326, 241, 246; 16 x 512 410, 284,
-        // 269; columns of 64: 64 x 512 1189, 801, 692.  Uneven, one of 512 among 16 single tokens 53, 46, 67, among 64 70, 62, 83, among
-        // 256 166, 146, 146; 16 of up to 301 220, 157, 143.)
+        // 269; columns of 64: 64 x 512 1189, 801, 692.)  In an uneven batch, where `as_long` counts the single tokens in and their
+        // workgroups stand beside the chain's, 32 from 7/8 of the CUs on.  (One of 512 among 16 single tokens, us with 16, 32: 12, 14,
+        // 15, 16, 17 and 24 heads (192 to 384 columns) 43 and 45, 48 and 49, 53 and 49, 45 and 45, 55 and 51, 55 and 49; among 64 54 and
+        // 53, 66 and 57, 64 and 60, 62 and 55, 69 and 63, 83 and 72; heads of 64 x 64, 24, 30 and 32 among 16: 35 and 36, 40 and 41, 37
+        // and 38; among 256, 16 of 128 166 and 146; 16 of up to 301 220 and 157, with 64 143.)
         a.longs = (uint32_t)longs;
-        a.tiles = columns >= 6 * cus ? 4 : columns > cus || (!even && columns == cus) ? 2 : 1;
+        a.tiles = columns >= 6 * cus ? 4 : columns > cus || (!even && 8 * columns >= 7 * cus) ? 2 : 1;
         // All chunks are prepared at once, or, where the chain leaves half of the CUs without work and the blocks would not
         // stay in the 256 MB of the last cache, by groups of as many as give every CU one, the next group's preparation beside a
         // group's chain.  (us at once and by groups: 16 heads, 4096 tokens (148 MB) 151 and 160, 6144 249 and 232, 8192 348 and
