@@ -95,6 +95,7 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
     const size_t cus = (size_t)ctx->cu_count, units = (size_t)a.s.n_seq * H, most_steps = units < cus ? 8 : units < 2 * cus ? 16 : 24;
     const bool chunks = a.s.max_q > most_steps, even = a.s.n_seq == 1 || n == (size_t)a.s.n_seq * a.s.max_q;
     a.chunk_from = !chunks ? 0xffffffffu : even ? 0 : (uint32_t)most_steps + 1;
+    if (!chunks && units * (dv / 32) > 4 * kMaxGrid) return AH_ERR_INVALID_ARG;
     if (chunks) {
         // (uneven: at most `longs` sequences go by chunks, and as many of the longest would have the batch's tokens)
         const size_t longest = n / (most_steps + 1), longs = even || longest > a.s.n_seq ? a.s.n_seq : longest, as_long = (n + a.s.max_q - 1) / a.s.max_q;
@@ -126,7 +127,8 @@ int32_t ah_delta_rule_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_delta
             a.slot_seq = even || by_seq <= by_tokens;
             a.slot_shift = a.slot_seq ? 6 : 3;
             const size_t slots = a.slot_seq ? by_seq : by_tokens;
-            if (slots * H > kMaxGrid / 2 || units * (dv / 16) > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
+            const size_t alone = even ? 0 : (units * (dv / 32) + 7) / 8;  // workgroups of the sequences that go token by token
+            if (slots * H > kMaxGrid / 2 || longs * H * (dv / 16) / a.tiles + alone > kMaxGrid / 2) return AH_ERR_INVALID_ARG;
             a.slots = (uint32_t)slots;
             need = slots * H * bytes;
         }

@@ -490,7 +490,9 @@ int32_t ah_kv4_attn_shared_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
  * 16-byte aligned; ah_kv4_block_means_dev fills in the blocks whose last position is among the tokens (each block's f64
  * mean, rounded to f32 and then to f16), after their append.  Only whole blocks are ever scored.
  * d_chosen (optional): [n_tok][n_kv_heads][n_top], the blocks chosen by score, ascending, then -1.
- * 1 <= n_top <= 4096, n_first and n_last <= 4096.  d_out may not overlap d_q.  Uses the context's scratch. */
+ * 1 <= n_top <= 4096, n_first and n_last <= 4096; n_tok n_kv_heads under 2^22, at most 4096 queries a KV head.  d_out may not
+ * overlap d_q.  Uses the context's scratch (a list of n_top + n_first + n_last + 2 numbers for every token and KV head, and
+ * what ah_kv4_attn_dev takes). */
 typedef struct ah_kv4_blocks {
     size_t block_len, n_top, n_first, n_last;
     const uint16_t *d_means;
@@ -519,7 +521,8 @@ typedef struct ah_state_seqs {
 
 /* The short causal convolution of every channel with its own weights, optionally with SiLU:
  * y_t = act(bias + sum_i weight[i] x_(t - width + 1 + i)), where the inputs before the call's are the state
- * [n_slots][width - 1][n_channels], the last one last.  width 2 to 8, at most 2^20 channels. */
+ * [n_slots][width - 1][n_channels], the last one last.  width 2 to 8, at most 2^20 channels; (n_tok / 8 + n_seq) times
+ * n_channels / 1024, each rounded up, under 2^24. */
 typedef struct ah_conv {
     size_t n_channels, width;
     const float *d_weight; /* [n_channels][width] */
@@ -541,6 +544,8 @@ int32_t ah_conv_dev(ah_ctx *ctx, const ah_state_seqs *seqs, const ah_conv *args,
  * adds, beta (v - S^T k), is held to about 2^-31 of the largest |S| and 2^-37 of the largest |beta v| of its chunk and 16
  * columns of S: as f32 where it is no less than 2^-7 of that |S|, and not to its own last place where a decay within the chunk
  * clears a far larger state.
+ * Up to n_seq n_heads v_dim = 2^26 and n_tok n_heads = 2^28 every call is served; above, one with more workgroups than a launch
+ * holds is refused with AH_ERR_INVALID_ARG.
  * Uses the context's scratch (as ah_gemm_f32_dev, also for calls captured into a graph): 768 k_dim + 256 v_dim + 13 KB for
  * every 64 tokens and head and for every sequence and head, less where few sequences are long. */
 typedef struct ah_delta_rule {
