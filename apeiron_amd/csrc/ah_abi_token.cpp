@@ -562,11 +562,13 @@ int32_t ah_kv4_attn_blocks_dev(ah_ctx *ctx, const ah_kv4 *cache, const ah_kv4_at
     // of 64, heads of 128, 2048 tokens over 70000, 100000 and 200000 keys 280 and 147, 321 and 158, 477 and 205, 512 over 100000 108 and
     // 93; of 256, 2048 over 100000 552 and 274; 400 blocks of 100000 2242 and 2107, 550 the same; past that a pass is too short.
     const Fit one = fit(1, 0), many = fit(16, a.c.dim + 3);
-    const bool together = a.max_q >= 4 && units >= (a.c.dim == 256 ? 4 : 2) * (size_t)ctx->cu_count && (many.keys == room || many.keys >= b.top + (size_t)128);
+    const size_t tiles = (size_t)a.n_tok / 16 + a.n_seq;
+    const bool together = a.max_q >= 4 && units >= (a.c.dim == 256 ? 4 : 2) * (size_t)ctx->cu_count && (many.keys == room || many.keys >= b.top + (size_t)128) &&
+                          tiles * a.c.n_kv <= max_grid(1024);
     b.lds_keys = (uint32_t)(together ? many : one).keys;
     b.lds_bytes = (uint32_t)(together ? many : one).bytes;
-    b.tiles = together ? a.n_tok / 16 + a.n_seq : 0;
-    if ((size_t)b.tiles * a.c.n_kv > max_grid(1024) || (!together && units > max_grid(1024))) return AH_ERR_INVALID_ARG;
+    b.tiles = together ? (uint32_t)tiles : 0;
+    if (!together && units > max_grid(1024)) return AH_ERR_INVALID_ARG;
     const size_t kept = align256(units * a.list_stride * sizeof(uint32_t));
     // Up to eight queries a KV head, and lists enough for four waves a CU and more: a wave each.  (us with a wave each and in
     // pieces, 2 KV heads, lists of 1152 keys: heads of 64, 512 lists 46 and 39, 1024 49 and 52; of 128 61 and 53, 63 and 74; of

@@ -92,3 +92,22 @@ def test_equal_scores_take_the_first_blocks_by_passes_too(dev, blocks, top, n): 
                 score = value[: pos // 32, h].astype(np.float64) @ B.q[t, 128 * h:128 * h + 128].reshape(2, 64).astype(np.float64).sum(0)
                 score[10] = -np.inf
                 assert np.array_equal(chosen[t, h], np.sort(np.argsort(-score, kind="stable")[:top])), (t, h, max_ctx)
+
+
+@pytest.mark.gpu
+def test_tens_of_thousands_of_idle_sequences_and_many_kv_heads(dev):  # noqa: F811
+    """As without them, where they would be too many tiles of 16 tokens for a launch."""
+    B = Batch(dev, [8], [290], 80, 1, 64, 32, seed=3)
+    means = B.means(32)
+    status, want, chosen = B.blocks(means, 32, 3, 1, 0)
+    assert status == OK
+    n_seq = 65535
+    start, c = np.full(n_seq + 1, 8, np.int32), np.zeros(n_seq, np.int32)
+    start[0], c[0] = 0, 290
+    table = torch.zeros(n_seq, B.P.per, dtype=torch.int32, device="cuda")
+    table[0] = B.P.table[0]
+    status, out, picked = B.blocks(means, 32, 3, 1, 0, start=start, ctx=c, table=table, n_seq=n_seq)
+    assert status == OK and np.array_equal(picked, chosen)
+    see = B.choose(0, 32, 3, 1, 0)[1]
+    for x in (out, want):
+        compare(B.rows(0, x), B.rows(0, B.q), B.k[0], B.v[0], see, B.scale)
