@@ -243,7 +243,7 @@ template <int DK> __global__ void __launch_bounds__(256) delta_step_kernel(Delta
 // delta_prepare_kernel makes W, U0, P and the decayed keys of all chunks at once; delta_chain_kernel then walks a sequence's
 // chunks with S in registers, two products deep a chunk.  No exponent above a sum of g's is ever formed, and sums of g are f64.
 //   Token by token a head's S passes registers once a token (8192 tokens of 16 heads: 20.7 ms); by chunks of 64 it takes 6 dk dv
-// products of 64 tokens on the matrix cores and a chain 64 times shorter (301 us).  Shorter chunks have a longer chain, longer
+// products of 64 tokens on the matrix cores and a chain 64 times shorter (306 us).  Shorter chunks have a longer chain, longer
 // ones more of the triangle (T by recursion: 64 is four tiles of 16).
 //   f32 by f16: every factor of a product is carried as hi + lo, two f16 of a value scaled by a power of two so that the largest
 // of its group (a row of q, k or P, a tile, a slice, a chunk) lies in [2^13, 2^14): 22 bits, or 2^-38 of the group's largest.  Three products
@@ -387,7 +387,7 @@ template <int DK> struct PrepareLds {
 };
 // Eight waves a chunk and head.  Waves 0 to 3 have the keys and beta_i k_i . k_j of 16 tokens i each, and make T of them; waves 4 to
 // 7 have q of the same tokens, P and q's fragments.  W and U0 are shared by all.  Barriers wait for LDS alone: loads and stores stay
-// on their way.  What bounds it is vector work beside the waits at barriers (58% of a SIMD's cycles while a CU works, products 9%):
+// on their way.  What bounds it is vector work beside the waits at barriers (62% of a SIMD's cycles while a CU works, products 9%):
 // halves of every factor, T's recursion, the scales.  A chunk and head of 128 x 128 takes 26 us where two share a CU (5 x 301
 // tokens, 16 heads), 2048 of them 110.
 template <int DK> AH_DEV void prepare(const DeltaArgs &a, const Chunk &c, uint32_t hd, uint8_t *block, PrepareLds<DK> &L) {
@@ -729,17 +729,9 @@ template <int DK> __global__ void __launch_bounds__(512, 4) delta_prepare_kernel
     if (c.live) prepare<DK>(a, c, hd, a.blocks + ((size_t)at * a.n_heads + hd) * delta_block(DK, a.v_dim).bytes, *reinterpret_cast<PrepareLds<DK> *>(lds_bytes));
 }
 
-// A sequence's chunks in turn, for NC times 16 columns of a head's S.  Waves 0 to 3 are the chain: wave w makes U of the tokens
-// 16 w .. 16 w + 15 (the first half of a chunk's time) and the rows of slice w of S (the second); what the others need goes
-// through LDS as operands.  Waves 4 to 7 make o of the same tokens: q S beside U, P U beside S.  Two barriers a chunk.
-//   What comes from memory is asked for two chunks ahead, and touched a few chunks before that, each of a head's workgroups a
-// part, so that it waits in the XCD's L2.
-//   What bounds it is that chain of two products, their scales and halves, and two barriers: 1.9 us a chunk of 128 x 128 where the
-// blocks lie in the last cache (8192 tokens of 16 heads: 128 workgroups of 256 CUs, 238 us), whatever the columns; more columns
-// a workgroup take longer a chunk and read a block fewer times.  In 5 x 301 tokens (NC 2, 28 us) products take 16% of a SIMD's
-// cycles while a CU works, vector work 27%, and the waves wait 37% of theirs.
-// The nth sequence that goes by chunks, from the lanes that look for it; n_seq if there is none.  (Workgroups for every sequence of a batch of mostly single tokens
-// ended at once, but took as long to start as the others: one of 512 tokens among 256 158 us for 146, among 16 67 for 46.)
+// The nth sequence that goes by chunks, from the lanes that look for it; n_seq if there is none.  (Workgroups for every sequence
+// of a batch of mostly single tokens ended at once, but took as long to start as the others: one of 512 tokens among 256 158 us
+// for 146, among 16 67 for 46.)
 AH_DEV uint32_t nth_long(const DeltaArgs &a, uint32_t nth, Seq &found) {
     for (uint32_t base = 0; base < a.s.n_seq; base += 64) {
         const uint32_t i = base + (threadIdx.x & 63);
@@ -757,6 +749,15 @@ AH_DEV uint32_t nth_long(const DeltaArgs &a, uint32_t nth, Seq &found) {
     }
     return a.s.n_seq;
 }
+// A sequence's chunks in turn, for NC times 16 columns of a head's S.  Waves 0 to 3 are the chain: wave w makes U of the tokens
+// 16 w .. 16 w + 15 (the first half of a chunk's time) and the rows of slice w of S (the second); what the others need goes
+// through LDS as operands.  Waves 4 to 7 make o of the same tokens: q S beside U, P U beside S.  Two barriers a chunk.
+//   What comes from memory is asked for two chunks ahead, and touched a few chunks before that, each of a head's workgroups a
+// part, so that it waits in the XCD's L2.
+//   What bounds it is that chain of two products, their scales and halves, and two barriers: 1.9 us a chunk of 128 x 128 where the
+// blocks lie in the last cache (8192 tokens of 16 heads: 128 workgroups of 256 CUs, 238 us), whatever the columns; more columns
+// a workgroup take longer a chunk and read a block fewer times.  In 5 x 301 tokens (NC 2, 29 us) products take 16% of a SIMD's
+// cycles while a CU works, vector work 27%, and the waves wait 37% of theirs.
 template <int DK, int NC> struct ChainLds {
     u32x4 sf[NC][DK / 32][2][64], uf[NC][2][2][64];
     float sinv[NC][4], stop[NC][4], uinv[NC];
@@ -1018,7 +1019,7 @@ template <int DK, int NC> __global__ void __launch_bounds__(512) delta_chain_ker
 }
 // The chain of one group of chunks beside the preparation of the next, where the chain leaves CUs to it: every sequence's chunks
 // begin .. begin + ring / 2 - 1 and, by the workgroups after the chain's, the ring / 2 after those.  The blocks of two groups
-// are there at once, [sequence][ring][head].  A launch of 16 chunks of 16 heads takes 38 us: 30 of chain, and 256 preparations
+// are there at once, [sequence][ring][head].  A launch of 16 chunks of 16 heads takes 40 us: 30 of chain, and 256 preparations
 // in the 128 CUs that it leaves, one a CU (the chain's registers leave a CU no room for two).
 template <int DK> __global__ void __launch_bounds__(512) delta_both_kernel(DeltaArgs a) {
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_bytes[];
